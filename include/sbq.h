@@ -422,6 +422,47 @@ int sbq_sample_rows(const float* logits, int64_t M, int64_t V, int64_t ld, float
                     float top_p, const float* u, int64_t* tokens, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/* ---- linears with 4-bit weights and group scales ------------------------ */
+
+/* The int8 weight-only linear's counterpart at half the weight bytes; no
+ * counterpart in the reference.  A row of the weight has one scale per group
+ * of 32, 64 or 128 consecutive columns (the last group of a ragged K is
+ * shorter), held in bf16:
+ *   scale[n,G] = bf16(max(max_{k in G} |w[n,k]|, 1e-8f) / 7.0f)
+ *   q[n,k]     = clamp(rint(w[n,k] / fp32(scale[n,G])), -7, 7)
+ * (IEEE fp32 divisions, half to even; the weights must be finite).
+ * w: device [N, K] (row stride ldw), F32, F16 or BF16.  q: device int8 [N, K]
+ * (row stride ldq).  scale: device bf16 [N, ceil(K/group)]. */
+int sbq_quantize_groups(const void* w, int w_dtype, int64_t N, int64_t K, int64_t ldw, int group,
+                        int8_t* q, int64_t ldq, void* scale, void* stream);
+
+/* The layout that sbq_linear_w4 streams.  packed: ceil(N/16) x ceil(K/128)
+ * tiles of 1 KiB; tile (nt,kt) holds rows nt*16..+15 and columns
+ * kt*128..+127, its 32-bit word lane*4 + s, lane = g*16 + r, the 8 columns
+ * kt*128 + 32s + 8g + j of row nt*16 + r: column j = 2i in bits 4i..4i+3,
+ * column 2i + 1 in bits 16+4i..19+4i, each as q + 8 (padding 8, that is 0).
+ * gscale: bf16 [ceil(N/16)][ceil(K/128) * 128/group][16], the 16 rows of a
+ * tile side by side (padding 0).  q: values outside -8..7 are clamped.
+ * packed and gscale: device, 16-byte aligned. */
+int64_t sbq_w4_packed_bytes(int64_t N, int64_t K);
+int64_t sbq_w4_scale_count(int64_t N, int64_t K, int group);
+int sbq_repack_w4(const int8_t* q, int64_t N, int64_t K, int64_t ldq, const void* scale, int group,
+                  uint8_t* packed, void* gscale, void* stream);
+/* The inverse. */
+int sbq_unpack_w4(const uint8_t* packed, const void* gscale, int64_t N, int64_t K, int group,
+                  int8_t* q, int64_t ldq, void* scale, void* stream);
+
+/* y[m,n] = sum_G fp32(scale[n,G]) * (sum_{k in G} q[n,k] * x[m,k]) (+ bias[n])
+ * x: device [M, K] (row stride ldx), F32, F16 or BF16, any alignment
+ * (16-byte aligned rows are faster).  fp16 and bf16 are used exactly, fp32 to
+ * 22 significant bits (of each value, or 2^-39 of the largest in its 128
+ * columns).  Accumulation is fp32.  bias: device fp32 [N] or NULL.  y: device
+ * [M, N] (row stride ldy), F32, F16 or BF16.  Meant for M up to 64; more rows
+ * run in blocks of 64 that each read the weight again. */
+int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
+                  const uint8_t* packed, const void* gscale, const float* bias, int64_t N, int group,
+                  void* y, int y_dtype, int64_t ldy, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,10 @@ inline bool y_vec_ok(const void* y, int yt, int64_t ldy, int64_t N) {
   return aligned(y, a) && (ldy * esize(yt)) % a == 0 && N % 4 == 0;
 }
 
+inline bool valid_group(int group) { return group == 32 || group == 64 || group == 128; }
+// Sizes whose packing launches fit a grid (one thread per 8 columns).
+inline bool w4_size_ok(int64_t N, int64_t K) { return N <= (1 << 30) && K <= (1 << 30) && (N + 15) * (K + 127) <= (int64_t)1 << 41; }
+
 // W8A8 workspace layout (from the first 256-byte boundary): min/max partials
 // (kMinMaxPartials float2), then (s_x, zp) in 256 bytes, then the quantized
 // activations xq [M][Kc*64] (s8) for the GEMM path.
@@ -613,6 +617,56 @@ int sbq_sample_rows(const float* logits, int64_t M, int64_t V, int64_t ld, float
   if (!workspace || (int64_t)workspace_bytes < sbq_sample_workspace_bytes(M, V)) return SBQ_ERR_WORKSPACE;
   void* ws = (void*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
   return sbq::launch_sample_rows(logits, M, V, ld, temperature, top_k, top_p, u, tokens, ws, st);
+}
+
+// ---- 4-bit weights with group scales ----
+
+int64_t sbq_w4_packed_bytes(int64_t N, int64_t K) {
+  if (N < 1 || K < 1 || N > kIntMax || K > kIntMax) return 0;
+  return (N + 15) / 16 * ((K + 127) / 128) * 1024;
+}
+
+int64_t sbq_w4_scale_count(int64_t N, int64_t K, int group) {
+  if (N < 1 || K < 1 || N > kIntMax || K > kIntMax || !valid_group(group)) return 0;
+  return (N + 15) / 16 * 16 * ((K + 127) / 128) * (128 / group);
+}
+
+int sbq_quantize_groups(const void* w, int w_dtype, int64_t N, int64_t K, int64_t ldw, int group, int8_t* q, int64_t ldq,
+                        void* scale, void* stream) {
+  if (!valid_dtype(w_dtype)) return SBQ_ERR_DTYPE;
+  if (N < 0 || K < 1 || ldw < K || ldq < K || !valid_group(group) || !w4_size_ok(N, K)) return SBQ_ERR_ARG;
+  if (N == 0) return SBQ_OK;
+  if (!w || !q || !scale) return SBQ_ERR_ARG;
+  return sbq::launch_quantize_groups(w, w_dtype, N, K, ldw, group, q, ldq, (uint16_t*)scale, (hipStream_t)stream);
+}
+
+int sbq_repack_w4(const int8_t* q, int64_t N, int64_t K, int64_t ldq, const void* scale, int group, uint8_t* packed,
+                  void* gscale, void* stream) {
+  if (N < 1 || K < 1 || ldq < K || !valid_group(group) || !w4_size_ok(N, K)) return SBQ_ERR_ARG;
+  if (!q || !scale || !packed || !gscale) return SBQ_ERR_ARG;
+  if (!aligned(packed, 16) || !aligned(gscale, 16)) return SBQ_ERR_ALIGN;
+  return sbq::launch_repack_w4(q, N, K, ldq, (const uint16_t*)scale, group, packed, (uint16_t*)gscale,
+                               (hipStream_t)stream);
+}
+
+int sbq_unpack_w4(const uint8_t* packed, const void* gscale, int64_t N, int64_t K, int group, int8_t* q, int64_t ldq,
+                  void* scale, void* stream) {
+  if (N < 1 || K < 1 || ldq < K || !valid_group(group) || !w4_size_ok(N, K)) return SBQ_ERR_ARG;
+  if (!q || !scale || !packed || !gscale) return SBQ_ERR_ARG;
+  if (!aligned(packed, 16) || !aligned(gscale, 16)) return SBQ_ERR_ALIGN;
+  return sbq::launch_unpack_w4(packed, (const uint16_t*)gscale, N, K, group, q, ldq, (uint16_t*)scale,
+                               (hipStream_t)stream);
+}
+
+int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* packed, const void* gscale,
+                  const float* bias, int64_t N, int group, void* y, int y_dtype, int64_t ldy, void* stream) {
+  int rc = check_linear(x, x_dtype, M, K, ldx, packed, (const float*)gscale, N, y, y_dtype, ldy);
+  if (rc) return rc;
+  if (!valid_group(group) || !w4_size_ok(N, K)) return SBQ_ERR_ARG;
+  if (M == 0) return SBQ_OK;
+  if (!aligned(gscale, 16)) return SBQ_ERR_ALIGN;
+  return sbq::launch_linear_w4(x, x_dtype, M, K, ldx, x_vec_ok(x, x_dtype, ldx), packed, (const uint16_t*)gscale, bias, N,
+                               group, y, y_dtype, ldy, y_vec_ok(y, y_dtype, ldy, N), (hipStream_t)stream);
 }
 
 }  // extern "C"

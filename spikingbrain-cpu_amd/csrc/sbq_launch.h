@@ -220,4 +220,16 @@ int launch_gemm_w8a8(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, b
                      bool yvec, uint8_t* split = nullptr, int64_t split_bytes = 0,
                      const u32x2* parts = nullptr);
 
+// Linears with 4-bit weights and group scales (sbq_w4.hip).  group: 32, 64 or
+// 128; scales are bf16 bits.
+int launch_quantize_groups(const void* w, int wt, int64_t N, int64_t K, int64_t ldw, int group, int8_t* q, int64_t ldq,
+                           uint16_t* scale, hipStream_t st);
+int launch_repack_w4(const int8_t* q, int64_t N, int64_t K, int64_t ldq, const uint16_t* scale, int group, uint8_t* packed,
+                     uint16_t* gscale, hipStream_t st);
+int launch_unpack_w4(const uint8_t* packed, const uint16_t* gscale, int64_t N, int64_t K, int group, int8_t* q, int64_t ldq,
+                     uint16_t* scale, hipStream_t st);
+int launch_linear_w4(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, bool xvec, const uint8_t* packed,
+                     const uint16_t* gscale, const float* bias, int64_t N, int group, void* y, int yt, int64_t ldy, bool yvec,
+                     hipStream_t st);
+
 }  // namespace sbq

@@ -1,0 +1,478 @@
+// sbq_w4.hip - linears with 4-bit weights and one scale per group of columns.
+//
+//   y[m,n] = sum_G s[n,G] * (sum_{k in G} q[n,k] x[m,k]) (+ bias[n]),
+//   q in -8..7, G = groups of 32, 64 or 128 columns, s in bf16.
+//
+// What bounds it: the weight stream (N K / 2 bytes) at one to a few rows of
+// x; from about 16 rows on also the conversions.  A packed tile is 16 rows x
+// 128 columns in 1 KiB, one 16-byte load per lane, in the order of the MFMA A
+// operand: lane = g*16 + r holds row r, dword s the columns 32 s + 8 g + 0..7
+// of the tile, so that each group of 32 columns is one 16x16x32 MFMA step and
+// the scale is applied to the fp32 partial sums of its group (a weight
+// rounded with its scale to 16 bits would lose half of the bits of fp32
+// activations).
+//
+// A workgroup of KS waves owns G 16-row tiles of the weight; its waves take
+// the K tiles in turn and are summed through LDS in wave order.
+//
+// Activations: fp16 and bf16 are the MFMA's own operands (weights converted to
+// the same type, exactly).  fp32 is split into two fp16 planes after a
+// power-of-two scaling per row and K tile: 22 significant bits, 2^-39 of the
+// tile's maximum at least, below the rounding of an fp32 sum.
+//   STAGE   up to 8 rows: the wave converts its K tile once (16 lanes per
+//           row) into LDS and reads fragments from there; a fragment read
+//           straight from memory would be converted 16 times over at one row
+//   direct  otherwise: each lane converts the fragment it multiplies
+#include "sbq_common.h"
+#include "sbq_launch.h"
+
+namespace sbq {
+
+namespace {
+
+constexpr int kW4MaxWaves = 8;
+
+// 8 nibbles u = q + 8 -> fp16 q: element 2i in nibble i, 2i + 1 in nibble
+// i + 4; 0x6400 | u is 1024 + u.
+__device__ __forceinline__ f16x8 w4_to_f16(uint32_t w) {
+  const f16x2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
+  f16x8 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 p = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - bias;
+    o[2 * i] = p.x;
+    o[2 * i + 1] = p.y;
+  }
+  return o;
+}
+
+// ... -> bf16 q: 0x4300 | u is 128 + u; the difference to 136 is taken in fp32
+// (there is no packed bf16 subtract) and its upper half is exact.
+__device__ __forceinline__ bf16x8 w4_to_bf16(uint32_t w) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const uint32_t lo = __float_as_uint(__uint_as_float(p << 16) - 136.0f);
+    const uint32_t hi = __float_as_uint(__uint_as_float(p & 0xffff0000u) - 136.0f);
+    o[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+  }
+  return __builtin_bit_cast(bf16x8, o);
+}
+
+template <int XT>
+struct W4Math {
+  typedef f16x8 V;
+  static __device__ __forceinline__ V weight(uint32_t w) { return w4_to_f16(w); }
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct W4Math<XT_BF16> {
+  typedef bf16x8 V;
+  static __device__ __forceinline__ V weight(uint32_t w) { return w4_to_bf16(w); }
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// 8 consecutive activations, as they are in memory.
+template <int XT>
+struct X8 {
+  typedef typename XElem<XT>::T T;
+  typedef T V __attribute__((ext_vector_type(8)));
+  V v;
+  // `vec`: the row is 16-byte aligned.  Columns from K on are zero.
+  __device__ __forceinline__ void load(const T* row, int k0, int K, bool vec) {
+    if (vec && k0 + 8 <= K) {
+      v = *(const V*)(row + k0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = k0 + j < K ? row[k0 + j] : (T)0.0f;
+    }
+  }
+};
+
+// Largest finite magnitude of 8 fp32 values (NaN and infinities left out).
+__device__ __forceinline__ float max_abs8(const X8<XT_F32>::V& v) {
+  float m = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = __builtin_fabsf(v[j]);
+    m = a <= 3.4028235e38f ? __builtin_fmaxf(m, a) : m;
+  }
+  return m;
+}
+
+// Two fp16 planes of v * 2^e: hi rounded to nearest, lo the remainder.  An
+// infinity stays one (its remainder would be NaN).
+__device__ __forceinline__ void split_f16(const X8<XT_F32>::V& v, float s, f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = v[j] * s;
+    hi[j] = (_Float16)t;
+    const float r = t - (float)hi[j];
+    lo[j] = (_Float16)(__builtin_fabsf(t) > 3.4028235e38f ? 0.0f : r);
+  }
+}
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Exponent for a tile's maximum (>= 0, finite): it lands in [2^14, 2^15).
+__device__ __forceinline__ int tile_exp(float mx) {
+  const int e = 141 - (int)(__float_as_uint(mx) >> 23);
+  return mx > 0.0f ? min(max(e, -112), 120) : 0;
+}
+
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+struct W4Args {
+  const void* x;
+  const uint8_t* packed;
+  const uint16_t* gscale;
+  const float* bias;
+  void* y;
+  int64_t ldx, ldy;
+  int M, N, K, Nt, Kc, yt;
+  bool xvec, yvec;
+};
+
+// XT: activations; MT: 16-row tiles of x; G: 16-row tiles of the weight; GS:
+// MFMA steps per group (1, 2, 4); PASSES: 0 direct, else STAGE with 4 rows of
+// x per pass; D: K tiles loaded together.
+template <int XT, int MT, int G, int GS, int PASSES, int D>
+__global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
+  typedef typename XElem<XT>::T T;
+  typedef W4Math<XT> Math;
+  typedef typename Math::V V;
+  constexpr int P = XT == XT_F32 ? 2 : 1;  // planes of x
+  constexpr int GPT = 4 / GS;              // groups per tile
+  constexpr int ROWS = PASSES * 4;
+  constexpr int XR = PASSES ? PASSES : 4;  // 8-element pieces of x per lane
+  static_assert(!PASSES || MT == 1, "staging serves one row tile");
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.y * (MT * 16), M = min(a.M - m0, MT * 16);
+  const int nt0 = blockIdx.x * G;
+  const T* const x = (const T*)a.x + (int64_t)m0 * a.ldx;
+
+  f32x4 acc[G][MT];
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[i][t] = (f32x4)(0.0f);
+
+  // STAGE: the wave's own LDS: P planes of ROWS rows of 16 pieces, then the rows' factors
+  uint8_t* const stage = lds + ks * (P * ROWS * 256 + (P == 2 ? ROWS * 4 : 0));
+  float* const factor = (float*)(stage + P * ROWS * 256);
+
+  for (int kb = ks; kb < a.Kc; kb += D * KS) {
+    u32x4 w[D][G];
+    u32x2 sc[D][G][GPT];
+    X8<XT> raw[D][XR];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int kt = min(kb + d * KS, a.Kc - 1);  // (a surplus tile is loaded again, not used)
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int64_t nt = min(nt0 + i, a.Nt - 1);
+        w[d][i] = *(const u32x4*)(a.packed + ((nt * a.Kc + kt) * 64 + lane) * 16);
+#pragma unroll
+        for (int q = 0; q < GPT; ++q)
+          sc[d][i][q] = *(const u32x2*)(a.gscale + ((nt * a.Kc + kt) * GPT + q) * 16 + 4 * g);
+      }
+      if constexpr (PASSES > 0) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p)
+          raw[d][p].load(x + (int64_t)min(p * 4 + g, M - 1) * a.ldx, kt * 128 + c * 8, a.K, a.xvec);
+      } else if constexpr (MT == 1) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          raw[d][s].load(x + (int64_t)min(c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int kt = kb + d * KS;
+      if (kt >= a.Kc) break;
+      V wv[G][4];
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) wv[i][s] = Math::weight(w[d][i][s]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        V xv[P][4];
+        float f = 1.0f;
+        if constexpr (PASSES > 0) {
+          wave_lds_fence();
+#pragma unroll
+          for (int p = 0; p < PASSES; ++p) {
+            const int row = p * 4 + g;
+            uint8_t* const to = stage + row * 256 + ((c ^ row) & 15) * 16;
+            if constexpr (XT == XT_F32) {
+              float mx = max_abs8(raw[d][p].v);
+#pragma unroll
+              for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
+              const int e = tile_exp(mx);
+              f16x8 hi, lo;
+              split_f16(raw[d][p].v, exp2i(e), hi, lo);
+              *(f16x8*)to = hi;
+              *(f16x8*)(to + ROWS * 256) = lo;
+              if (c == 0) factor[row] = exp2i(-e);
+            } else {
+              *(V*)to = __builtin_bit_cast(V, raw[d][p].v);
+            }
+          }
+          wave_lds_fence();
+          const int row = min(c, M - 1);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const uint8_t* const from = stage + row * 256 + (((s * 4 + g) ^ row) & 15) * 16;
+#pragma unroll
+            for (int p = 0; p < P; ++p) xv[p][s] = *(const V*)(from + p * ROWS * 256);
+          }
+          if constexpr (XT == XT_F32) f = factor[row];
+        } else {
+          if constexpr (MT > 1) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              raw[d][s].load(x + (int64_t)min(t * 16 + c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
+          }
+          if constexpr (XT == XT_F32) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) mx = __builtin_fmaxf(mx, max_abs8(raw[d][s].v));
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const int e = tile_exp(mx);
+            f = exp2i(-e);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) split_f16(raw[d][s].v, exp2i(e), xv[0][s], xv[1][s]);
+          } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) xv[0][s] = __builtin_bit_cast(V, raw[d][s].v);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+          for (int q = 0; q < GPT; ++q) {
+            f32x4 part = (f32x4)(0.0f);
+#pragma unroll
+            for (int s = q * GS; s < q * GS + GS; ++s)
+#pragma unroll
+              for (int p = 0; p < P; ++p) part = Math::mfma(wv[i][s], xv[p][s], part);
+            const u32x2 b = sc[d][i][q];
+            const f32x4 s4 = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u),
+                              __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[i][t][v] = __builtin_fmaf(part[v], s4[v] * f, acc[i][t][v]);
+          }
+      }
+    }
+  }
+
+  // the waves' partial sums, added in wave order
+  if (KS > 1) {
+    f32x4* const red = (f32x4*)lds;
+    __syncthreads();  // (the staging area is done with)
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) red[(ks * G * MT + i * MT + t) * 64 + lane] = acc[i][t];
+    __syncthreads();
+  }
+  for (int u = ks; u < G * MT; u += KS) {
+    const int i = u / MT, t = u % MT;
+    f32x4 v;
+    if (KS > 1) {
+      const f32x4* const red = (const f32x4*)lds;
+      v = red[u * 64 + lane];
+      for (int k = 1; k < KS; ++k) v += red[(k * G * MT + u) * 64 + lane];
+    } else {
+#pragma unroll
+      for (int ii = 0; ii < G; ++ii)
+#pragma unroll
+        for (int tt = 0; tt < MT; ++tt)
+          if (ii == i && tt == t) v = acc[ii][tt];
+    }
+    const int m = t * 16 + c, n = (nt0 + i) * 16 + 4 * g;
+    if (m >= M || n >= a.N) continue;
+    if (a.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += n + j < a.N ? a.bias[n + j] : 0.0f;
+    }
+    store_y4(a.y, a.yt, (int64_t)(m0 + m) * a.ldy + n, v, a.yvec, a.N - n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// quantizing and packing (once per weight)
+// ---------------------------------------------------------------------------
+// One group per 32 lanes: s = bf16(max(max |w|, 1e-8) / 7), q = rint(w / s)
+// clamped to -7..7, so the rounding of the scale to bf16 costs nothing: q is
+// taken against the rounded one.
+template <int XT>
+__global__ __launch_bounds__(256) void quantize_groups_kernel(const void* w, int64_t ldw, int N, int K, int group, int Gn,
+                                                              int8_t* q, int64_t ldq, uint16_t* scale) {
+  typedef typename XElem<XT>::T T;
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (id >= (int64_t)N * Gn) return;
+  const int n = (int)(id / Gn), G = (int)(id % Gn), l = threadIdx.x & 31;
+  const T* const row = (const T*)w + n * ldw;
+  float v[4], mx = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = G * group + i * 32 + l;
+    v[i] = i * 32 < group && k < K ? XElem<XT>::to_f32(row[k]) : 0.0f;
+    mx = __builtin_fmaxf(mx, __builtin_fabsf(v[i]));
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
+  const __bf16 sb = (__bf16)(__builtin_fmaxf(mx, 1e-8f) / 7.0f);
+  const float s = (float)sb;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = G * group + i * 32 + l;
+    if (i * 32 < group && k < K)
+      q[n * ldq + k] = (int8_t)__builtin_fminf(__builtin_fmaxf(__builtin_rintf(v[i] / s), -7.0f), 7.0f);
+  }
+  if (l == 0) scale[id] = __builtin_bit_cast(uint16_t, sb);
+}
+
+// One dword (8 columns of one row) of the packed tiles per thread.
+__global__ __launch_bounds__(256) void pack_w4_kernel(const int8_t* q, int64_t ldq, int N, int K, int Kc, int64_t count,
+                                                      uint32_t* packed) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= count) return;
+  const int s = id & 3, lane = (id >> 2) & 63;
+  const int64_t tile = id >> 8;
+  const int64_t n = tile / Kc * 16 + (lane & 15);
+  const int k0 = (int)(tile % Kc) * 128 + s * 32 + (lane >> 4) * 8;
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int v = n < N && k0 + j < K ? min(max((int)q[n * ldq + k0 + j], -8), 7) : 0;
+    w |= (uint32_t)(v + 8) << (4 * (j / 2) + 16 * (j % 2));
+  }
+  packed[id] = w;
+}
+
+// Scales [N][Gn] -> [Nt][Gp][16], padding 0 (Gp: the groups of whole tiles).
+__global__ __launch_bounds__(256) void pack_scale_kernel(const uint16_t* scale, int N, int Gn, int Gp, int64_t count,
+                                                         uint16_t* gscale) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= count) return;
+  const int64_t n = id / 16 / Gp * 16 + (id & 15);
+  const int G = (int)(id / 16 % Gp);
+  gscale[id] = n < N && G < Gn ? scale[n * Gn + G] : 0;
+}
+
+__global__ __launch_bounds__(256) void unpack_w4_kernel(const uint32_t* packed, int N, int K, int Kc, int64_t count,
+                                                        int8_t* q, int64_t ldq) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= count) return;
+  const int s = id & 3, lane = (id >> 2) & 63;
+  const int64_t tile = id >> 8;
+  const int64_t n = tile / Kc * 16 + (lane & 15);
+  const int k0 = (int)(tile % Kc) * 128 + s * 32 + (lane >> 4) * 8;
+  const uint32_t w = packed[id];
+  if (n >= N) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (k0 + j < K) q[n * ldq + k0 + j] = (int8_t)((int)((w >> (4 * (j / 2) + 16 * (j % 2))) & 15) - 8);
+}
+
+__global__ __launch_bounds__(256) void unpack_scale_kernel(const uint16_t* gscale, int Gn, int Gp, int64_t count,
+                                                           uint16_t* scale) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= count) return;
+  const int64_t n = id / Gn;
+  scale[id] = gscale[(n / 16 * Gp + id % Gn) * 16 + n % 16];
+}
+
+inline unsigned blocks(int64_t count) { return (unsigned)((count + 255) / 256); }
+
+template <int XT, int MT, int G, int PASSES, int D>
+int launch_w4(const W4Args& a, int group, int KS, hipStream_t st) {
+  constexpr int P = XT == XT_F32 ? 2 : 1, ROWS = PASSES * 4;
+  const int stage = KS * (P * ROWS * 256 + (P == 2 ? ROWS * 4 : 0)), red = KS > 1 ? KS * G * MT * 1024 : 0;
+  const size_t lds = (size_t)(stage > red ? stage : red);
+  const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
+  if (group == 32)
+    linear_w4_kernel<XT, MT, G, 1, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+  else if (group == 64)
+    linear_w4_kernel<XT, MT, G, 2, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+  else
+    linear_w4_kernel<XT, MT, G, 4, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+  return check_launch();
+}
+
+template <int XT>
+int pick_w4(const W4Args& a, int group, hipStream_t st) {
+  int KS = 1;
+  while (KS < kW4MaxWaves && KS * 2 < a.Kc) KS *= 2;
+  if (a.M <= 4) return launch_w4<XT, 1, 1, 1, 4>(a, group, KS, st);
+  if (a.M <= 8) return launch_w4<XT, 1, 1, 2, 2>(a, group, KS, st);
+  if (a.M <= 16) return launch_w4<XT, 1, 1, 0, 2>(a, group, KS, st);
+  if (a.M <= 32) return launch_w4<XT, 2, 2, 0, 1>(a, group, KS, st);
+  return launch_w4<XT, 4, 2, 0, 1>(a, group, KS, st);
+}
+
+}  // namespace
+
+int launch_quantize_groups(const void* w, int wt, int64_t N, int64_t K, int64_t ldw, int group, int8_t* q, int64_t ldq,
+                           uint16_t* scale, hipStream_t st) {
+  const int Gn = (int)((K + group - 1) / group);
+  const unsigned grid = (unsigned)((N * Gn + 7) / 8);
+  if (wt == XT_F32)
+    quantize_groups_kernel<XT_F32><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
+  else if (wt == XT_F16)
+    quantize_groups_kernel<XT_F16><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
+  else
+    quantize_groups_kernel<XT_BF16><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
+  return check_launch();
+}
+
+int launch_repack_w4(const int8_t* q, int64_t N, int64_t K, int64_t ldq, const uint16_t* scale, int group, uint8_t* packed,
+                     uint16_t* gscale, hipStream_t st) {
+  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gp = Kc * (128 / group);
+  const int64_t words = Nt * Kc * 256, scales = Nt * Gp * 16;
+  pack_w4_kernel<<<blocks(words), 256, 0, st>>>(q, ldq, (int)N, (int)K, (int)Kc, words, (uint32_t*)packed);
+  pack_scale_kernel<<<blocks(scales), 256, 0, st>>>(scale, (int)N, (int)((K + group - 1) / group), (int)Gp, scales, gscale);
+  return check_launch();
+}
+
+int launch_unpack_w4(const uint8_t* packed, const uint16_t* gscale, int64_t N, int64_t K, int group, int8_t* q, int64_t ldq,
+                     uint16_t* scale, hipStream_t st) {
+  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gn = (K + group - 1) / group;
+  const int64_t words = Nt * Kc * 256, scales = N * Gn;
+  unpack_w4_kernel<<<blocks(words), 256, 0, st>>>((const uint32_t*)packed, (int)N, (int)K, (int)Kc, words, q, ldq);
+  unpack_scale_kernel<<<blocks(scales), 256, 0, st>>>(gscale, (int)Gn, (int)(Kc * (128 / group)), scales, scale);
+  return check_launch();
+}
+
+int launch_linear_w4(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, bool xvec, const uint8_t* packed,
+                     const uint16_t* gscale, const float* bias, int64_t N, int group, void* y, int yt, int64_t ldy, bool yvec,
+                     hipStream_t st) {
+  constexpr int64_t kRows = 1 << 20;  // rows per launch (the grid's second dimension holds 65535 blocks)
+  const int64_t xs = xt == XT_F32 ? 4 : 2, ys = yt == XT_F32 ? 4 : 2;
+  for (int64_t m = 0; m < M; m += kRows) {
+    const W4Args a{(const uint8_t*)x + m * ldx * xs, packed, gscale, bias, (uint8_t*)y + m * ldy * ys, ldx, ldy,
+                   (int)(M - m < kRows ? M - m : kRows), (int)N, (int)K, (int)((N + 15) / 16), (int)((K + 127) / 128), yt,
+                   xvec, yvec};
+    const int rc = xt == XT_F32   ? pick_w4<XT_F32>(a, group, st)
+                   : xt == XT_F16 ? pick_w4<XT_F16>(a, group, st)
+                                  : pick_w4<XT_BF16>(a, group, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+}  // namespace sbq

@@ -50,6 +50,12 @@ SIGNATURES = {
     "sbq_linear_w8_argmax": (_I, [_P, _I, _L, _L, _L, _P, _P, _P, _L, _P, _L, _P, _P, _S, _P, _P]),
     "sbq_linear_w8a8_argmax": (_I, [_P, _I, _L, _L, _L, _P, _P, _P, _P, _L, _P, _L, _P, _P, _S, _P, _P]),
     "sbq_sample_workspace_bytes": (_L, [_L, _L]),
+    "sbq_w4_packed_bytes": (_L, [_L, _L]),
+    "sbq_w4_scale_count": (_L, [_L, _L, _I]),
+    "sbq_quantize_groups": (_I, [_P, _I, _L, _L, _L, _I, _P, _L, _P, _P]),
+    "sbq_repack_w4": (_I, [_P, _L, _L, _L, _P, _I, _P, _P, _P]),
+    "sbq_unpack_w4": (_I, [_P, _P, _L, _L, _I, _P, _L, _P, _P]),
+    "sbq_linear_w4": (_I, [_P, _I, _L, _L, _L, _P, _P, _P, _L, _I, _P, _I, _L, _P]),
     "sbq_sample_rows": (_I, [_P, _L, _L, _L, ctypes.c_float, _L, ctypes.c_float, _P, _P, _P, _S, _P]),
 }
 

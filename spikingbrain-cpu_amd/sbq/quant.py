@@ -14,6 +14,9 @@ formats run on hand-written gfx950 kernels through libsbq.so:
               (quant.py:56-66): the fbgemm dynamic-linear arithmetic,
               reproduced bit for bit (uint8 activations, exact int32
               accumulation on i8 MFMA, fp32 epilogue).
+``int4``      4-bit weights with one bf16 scale per group of columns,
+              weight-only, for decode (up to some 64 rows); not one of the
+              reference's formats, so not in ``FORMATS``.
 ``float32`` / ``bfloat16`` / ``float16``
               plain torch GPU linears kept so that ``make_linear`` accepts every
               format the reference does; they are not part of the quantized
@@ -684,6 +687,105 @@ def linear_w8a8_argmax(x2: torch.Tensor, packed: torch.Tensor, scale: torch.Tens
     return y, idx
 
 
+W4_GROUPS = (32, 64, 128)  # columns per scale
+
+
+def quantize_groups(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """4-bit rows of a GPU weight [N, K]: (q int8 [N, K] in -7..7, scale bf16
+    [N, ceil(K / group)]), scale = bf16(max(max |w|, 1e-8) / 7) per group of
+    `group` columns, q = clamp(rint(w / scale), -7, 7).  The weights must be
+    finite."""
+    if weight.dim() != 2 or not weight.is_cuda or weight.shape[1] < 1:
+        raise ValueError("quantize_groups expects a 2-D GPU weight")
+    if group not in W4_GROUPS:
+        raise ValueError(f"quantize_groups: group must be one of {W4_GROUPS}")
+    w = weight if weight.dtype in _DTYPE_CODE else weight.float()
+    if w.stride(-1) != 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1]):
+        w = w.contiguous()
+    N, K = w.shape
+    q = torch.empty((N, K), dtype=torch.int8, device=w.device)
+    scale = torch.empty((N, -(-K // group)), dtype=torch.bfloat16, device=w.device)
+    with _on_device(w.device):
+        _lib.check(_lib.load().sbq_quantize_groups(_ptr(w), _code(w.dtype), N, K, _ldx(w), group, _ptr(q), K,
+                                                   _ptr(scale), _stream(w.device)), "sbq_quantize_groups")
+    return q, scale
+
+
+def repack_w4(q: torch.Tensor, scale: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q int8 [N, K] in -8..7, scale bf16 [N, ceil(K / group)]) on the GPU ->
+    (packed uint8 tiles, gscale bf16), the layout linear_w4 streams."""
+    if q.dtype != torch.int8 or q.dim() != 2 or not q.is_cuda or q.numel() == 0:
+        raise ValueError("repack_w4 expects a 2-D int8 GPU tensor")
+    if group not in W4_GROUPS:
+        raise ValueError(f"repack_w4: group must be one of {W4_GROUPS}")
+    N, K = q.shape
+    if scale.dtype != torch.bfloat16 or scale.device != q.device or scale.shape != (N, -(-K // group)):
+        raise ValueError(f"repack_w4: scale must be bfloat16 [N, ceil(K / group)] = [{N}, {-(-K // group)}] on {q.device}")
+    q, scale = q.contiguous(), scale.contiguous()
+    L = _lib.load()
+    packed = torch.empty((L.sbq_w4_packed_bytes(N, K),), dtype=torch.uint8, device=q.device)
+    gscale = torch.empty((L.sbq_w4_scale_count(N, K, group),), dtype=torch.bfloat16, device=q.device)
+    with _on_device(q.device):
+        _lib.check(L.sbq_repack_w4(_ptr(q), N, K, K, _ptr(scale), group, _ptr(packed), _ptr(gscale), _stream(q.device)),
+                   "sbq_repack_w4")
+    return packed, gscale
+
+
+def _check_w4(fn: str, packed: torch.Tensor, gscale: torch.Tensor, N: int, K: int, group: int, gpu: int) -> None:
+    if group not in W4_GROUPS:
+        raise ValueError(f"{fn}: group must be one of {W4_GROUPS}")
+    if N < 1 or K < 1:
+        raise ValueError(f"{fn}: N and K must be >= 1")
+    tiles = -(-N // 16) * -(-K // 128)
+    if (packed.dtype != torch.uint8 or packed.get_device() != gpu or not packed.is_contiguous()
+            or packed.numel() < tiles * 1024):
+        raise ValueError(f"{fn}: packed must be contiguous uint8 on GPU {gpu} with >= {tiles * 1024} bytes (N={N}, K={K})")
+    need = tiles * 16 * (128 // group)
+    if (gscale.dtype != torch.bfloat16 or gscale.get_device() != gpu or not gscale.is_contiguous()
+            or gscale.numel() < need):
+        raise ValueError(f"{fn}: gscale must be contiguous bfloat16 on GPU {gpu} with >= {need} elements "
+                         f"(N={N}, K={K}, group={group})")
+
+
+def unpack_w4(packed: torch.Tensor, gscale: torch.Tensor, N: int, K: int, group: int = 128
+              ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The inverse of repack_w4: (q int8 [N, K], scale bf16 [N, ceil(K / group)])."""
+    if not packed.is_cuda:
+        raise ValueError("unpack_w4 expects GPU tiles")
+    _check_w4("unpack_w4", packed, gscale, N, K, group, packed.get_device())
+    q = torch.empty((N, K), dtype=torch.int8, device=packed.device)
+    scale = torch.empty((N, -(-K // group)), dtype=torch.bfloat16, device=packed.device)
+    with _on_device(packed.device):
+        _lib.check(_lib.load().sbq_unpack_w4(_ptr(packed), _ptr(gscale), N, K, group, _ptr(q), K, _ptr(scale),
+                                             _stream(packed.device)), "sbq_unpack_w4")
+    return q, scale
+
+
+def linear_w4(x2: torch.Tensor, packed: torch.Tensor, gscale: torch.Tensor, bias: torch.Tensor | None, N: int,
+              group: int = 128, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[m, n] = sum over groups of scale[n, G] * (q[n, G] . x2[m, G]) (+ bias[n])
+    for x2 [M, K] on the GPU, the weight as repack_w4 lays it out.  One launch,
+    no workspace; meant for up to some 64 rows (decode, a tree of drafted
+    tokens): every further 64 rows read the weight again."""
+    x2 = _as_activation(x2)
+    M, K = x2.shape
+    gpu = x2.get_device()
+    if gpu < 0 or not x2.is_cuda:
+        raise ValueError("linear_w4: x must be a GPU tensor")
+    _check_w4("linear_w4", packed, gscale, N, K, group, gpu)
+    if bias is not None and (bias.dtype != torch.float32 or bias.get_device() != gpu or not bias.is_contiguous()
+                             or bias.numel() < N):
+        raise ValueError(f"linear_w4: bias must be a contiguous float32 tensor of N={N} elements on {x2.device}")
+    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=x2.device)
+    if y.get_device() != gpu or y.shape != (M, N) or y.stride(-1) != 1 or (M > 1 and y.stride(0) < N):
+        raise ValueError(f"linear_w4: out must be a [M={M}, N={N}] tensor with unit column stride on {x2.device}")
+    with _on_device(x2.device):
+        _lib.check(_lib.load().sbq_linear_w4(_ptr(x2), _code(x2.dtype), M, K, _ldx(x2), _ptr(packed), _ptr(gscale),
+                                             _ptr(bias), N, group, _ptr(y), _code(y.dtype), _ldx(y), _stream(x2.device)),
+                   "sbq_linear_w4")
+    return y
+
+
 def _greedy_state(module: nn.Module, device: torch.device) -> torch.Tensor:
     """The module's fused-argmax state for the current stream on `device`:
     calls on one stream run one after another and leave the state zero, so
@@ -938,6 +1040,73 @@ def _dyn_from_quantized(qweight: torch.Tensor, scale: torch.Tensor, bias: torch.
 DynamicInt8Linear.from_quantized = staticmethod(_dyn_from_quantized)
 
 
+class Int4Linear(_Fp32Buffers, nn.Module):
+    """A weight-only linear with 4-bit weights and one bf16 scale per `group`
+    (32, 64 or 128) columns: Int8Linear's decode step at half the weight bytes.
+    No counterpart in the reference.  Buffers ``packed`` and ``gscale`` (the
+    layout of repack_w4, persisted as it is) and ``bias`` (fp32 or None); the
+    scales and bias keep their type under .half() / .to(dtype).  ``qweight``
+    and ``scale`` give the int8 rows and scales back.  fp32 outputs, as the
+    int8 formats', unless ``out_dtype`` is set."""
+
+    _fp32_buffers = ("gscale", "bias")
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, group: int = 128):
+        if weight.dim() != 2 or weight.numel() == 0:
+            raise ValueError("Int4Linear expects a 2-D weight")
+        if group not in W4_GROUPS:
+            raise ValueError(f"Int4Linear: group must be one of {W4_GROUPS}")
+        super().__init__()
+        self._build(*quantize_groups(weight.to(_gpu_for(weight)), group), bias, group)
+
+    def _build(self, q, scale, bias, group):
+        self.out_features, self.in_features = q.shape
+        self.group = group
+        packed, gscale = repack_w4(q, scale, group)
+        self.register_buffer("packed", packed)
+        self.register_buffer("gscale", gscale)
+        self.register_buffer("bias", None if bias is None else bias.to(q.device).float().contiguous())
+        if bias is not None and self.bias.shape != (self.out_features,):
+            raise ValueError(f"Int4Linear: bias must have {self.out_features} elements")
+        self.out_dtype = torch.float32
+
+    @classmethod
+    def from_quantized(cls, qweight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None,
+                       group: int = 128) -> "Int4Linear":
+        """An Int4Linear from int8 rows [N, K] with values in -8..7 and their
+        bf16 scales [N, ceil(K / group)]."""
+        if qweight.dtype != torch.int8 or qweight.dim() != 2 or qweight.numel() == 0:
+            raise ValueError("from_quantized expects int8 qweight [N, K]")
+        device = _gpu_for(qweight)
+        q = qweight.to(device)
+        lo, hi = torch.aminmax(q)
+        if int(lo) < -8 or int(hi) > 7:
+            raise ValueError("from_quantized: 4-bit values lie in -8..7")
+        self = cls.__new__(cls)
+        nn.Module.__init__(self)
+        self._build(q, scale.to(device), bias, group)
+        return self
+
+    @property
+    def qweight(self) -> torch.Tensor:
+        return unpack_w4(self.packed, self.gscale, self.out_features, self.in_features, self.group)[0]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return unpack_w4(self.packed, self.gscale, self.out_features, self.in_features, self.group)[1]
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        packed = self.packed
+        if not packed.is_cuda:
+            raise RuntimeError("sbq Int4Linear: weights are on the CPU; move the module to a ROCm GPU")
+        _check_in_features(x, self.in_features)
+
+        def run(xd):
+            return linear_w4(_rows(xd), packed, self.gscale, self.bias, self.out_features, self.group, self.out_dtype)
+
+        return _like_rows(run(x) if x.device == packed.device else _run_on_device(x, packed.device, run), x.shape)
+
+
 def save_quantized(layers: dict[str, nn.Module], path: str) -> None:
     """Write the int8 rows and fp32 scales (and biases) of Int8Linear /
     DynamicInt8Linear layers to a safetensors file (keys <name>.qweight,
@@ -1153,7 +1322,8 @@ def fuse_linears(parts: list[nn.Module]) -> FusedLinear:
 
 
 def make_linear(fmt: str, weight: torch.Tensor, bias: torch.Tensor | None = None) -> nn.Module:
-    """quant.py:100-111 - same dispatch and the same ValueError for unknown formats."""
+    """quant.py:100-111 - same dispatch and the same ValueError for unknown
+    formats; also "int4" (Int4Linear with groups of 128 columns)."""
     if fmt == "float32":
         return FloatLinear(weight, bias)
     if fmt == "bfloat16":
@@ -1164,4 +1334,6 @@ def make_linear(fmt: str, weight: torch.Tensor, bias: torch.Tensor | None = None
         return Int8Linear(weight, bias)
     if fmt == "int8-dyn":
         return DynamicInt8Linear(weight, bias)
+    if fmt == "int4":
+        return Int4Linear(weight, bias)
     raise ValueError("unknown weight format " + fmt)
