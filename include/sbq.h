@@ -463,6 +463,49 @@ int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
                   const uint8_t* packed, const void* gscale, const float* bias, int64_t N, int group,
                   void* y, int y_dtype, int64_t ldy, void* stream);
 
+/* ---- attention over a cache and a tree of drafted tokens ----------------- */
+
+/* Most query tokens of one sbq_tree_attention call. */
+#define SBQ_ATTN_MAX_T 1024
+
+/* The attention of model.py:208-229 for T query tokens over a cache whose
+ * slots carry their positions, and over the keys of the T tokens themselves
+ * where they are given (drafts that are not in the cache: a tree of drafted
+ * tokens, verified in one pass):
+ *   out[t,h] = sum_s p[t,h,s] v[s, h / (heads / kv_heads)],
+ *   p[t,h,:] = softmax of scale * q[t,h] . k[s, ...] over what t sees:
+ *   cached slot s iff 0 <= slot_pos[s] <= q_pos[t], and with a window
+ *     (window > 0) slot_pos[s] > q_pos[t] - window;
+ *   draft j (k_new[j], v_new[j], at position q_pos[j]) iff tree[t * tree_ld +
+ *     j] != 0 (tree NULL: iff j <= t), and with a window q_pos[j] > q_pos[t] -
+ *     window.
+ * A row that sees nothing (or only scores of -infinity) is 0.  What a row does
+ * not see does not reach it, infinities and NaN included.
+ * q: device [T, heads, D], strides q_st and q_sh in elements, unit stride in
+ * D; F32, or the cache's type.  k, v: device [slots, kv_heads, D], both with
+ * strides k_ss and k_sh; k_new, v_new (NULL: none): device [T, kv_heads, D]
+ * of the cache's type, both with strides n_ss and n_sh.  slot_pos: device
+ * int64 [slots].  q_pos: device int64 [T].  out: device [T, heads, D] of q's
+ * type.  1 <= D <= 256, heads a multiple of kv_heads, T <= SBQ_ATTN_MAX_T,
+ * slots <= 2^30.
+ * Scores, maxima and sums are fp32; with 2-byte queries the weights p are
+ * rounded to their type (half to even) for the product with v, with F32
+ * queries everything is fp32.  Unit strides and 16-byte aligned rows of a
+ * D of 64, 128 or 256 are the fastest.
+ * weight: NULL, or device fp32 [slots]: weight[s] += sum_{t,h} p[t,h,s], the
+ * attention weight the cached slots received (for eviction by it).
+ * workspace: >= sbq_attn_workspace_bytes bytes, any content; one call at a
+ * time.  The result does not depend on timing. */
+int64_t sbq_attn_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots,
+                                 int weight);
+int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t D, int64_t q_st,
+                       int64_t q_sh, const void* k, const void* v, int kv_dtype, int64_t slots,
+                       int64_t kv_heads, int64_t k_ss, int64_t k_sh, const int64_t* slot_pos,
+                       const int64_t* q_pos, const void* k_new, const void* v_new, int64_t n_ss,
+                       int64_t n_sh, const uint8_t* tree, int64_t tree_ld, int64_t window, float scale,
+                       void* out, int64_t o_st, int64_t o_sh, float* weight, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -669,4 +669,47 @@ int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
                                group, y, y_dtype, ldy, y_vec_ok(y, y_dtype, ldy, N), (hipStream_t)stream);
 }
 
+// ---- attention over a cache, with drafts ----
+
+static int check_attn(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots) {
+  if (T < 0 || T > SBQ_ATTN_MAX_T || kv_heads < 1 || heads < 1 || heads > 65536 || heads % kv_heads || D < 1 || D > 256 ||
+      slots < 1 || slots > (1 << 30))
+    return SBQ_ERR_ARG;
+  return SBQ_OK;
+}
+
+int64_t sbq_attn_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots, int weight) {
+  if (T == 0 || check_attn(T, heads, kv_heads, D, slots)) return 0;
+  return sbq::attn_workspace_bytes(T, heads, kv_heads, D, slots, weight != 0) + 256;  // + alignment slack
+}
+
+int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t D, int64_t q_st, int64_t q_sh,
+                       const void* k, const void* v, int kv_dtype, int64_t slots, int64_t kv_heads, int64_t k_ss,
+                       int64_t k_sh, const int64_t* slot_pos, const int64_t* q_pos, const void* k_new, const void* v_new,
+                       int64_t n_ss, int64_t n_sh, const uint8_t* tree, int64_t tree_ld, int64_t window, float scale,
+                       void* out, int64_t o_st, int64_t o_sh, float* weight, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  if (!valid_dtype(q_dtype) || !valid_dtype(kv_dtype)) return SBQ_ERR_DTYPE;
+  if (q_dtype != SBQ_F32 && q_dtype != kv_dtype) return SBQ_ERR_DTYPE;
+  if (check_attn(T, heads, kv_heads, D, slots) || window < 0 || scale != scale) return SBQ_ERR_ARG;
+  if (T == 0) return SBQ_OK;
+  if (!q || !k || !v || !slot_pos || !q_pos || !out || (!k_new != !v_new) || (tree && !k_new)) return SBQ_ERR_ARG;
+  if (q_st < 0 || q_sh < 0 || k_ss < 0 || k_sh < 0 || o_st < 0 || o_sh < 0) return SBQ_ERR_ARG;
+  if (k_new && (n_ss < 0 || n_sh < 0)) return SBQ_ERR_ARG;
+  if (tree && tree_ld < T) return SBQ_ERR_ARG;
+  const int64_t es = esize(kv_dtype), eq = esize(q_dtype);
+  if (!aligned(q, eq) || !aligned(out, eq) || !aligned(k, es) || !aligned(v, es) || !aligned(k_new, es) ||
+      !aligned(v_new, es) || !aligned(slot_pos, 8) || !aligned(q_pos, 8) || !aligned(weight, 4))
+    return SBQ_ERR_ALIGN;
+  const int64_t need = sbq_attn_workspace_bytes(T, heads, kv_heads, D, slots, weight != nullptr);
+  if (!workspace || (int64_t)workspace_bytes < need) return SBQ_ERR_WORKSPACE;
+  sbq::AttnCall c{};
+  c.q = q, c.k = k, c.v = v, c.kn = k_new, c.vn = v_new, c.slot_pos = slot_pos, c.q_pos = q_pos, c.tree = tree;
+  c.out = out, c.weight = weight, c.ws = (void*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  c.T = T, c.heads = heads, c.Hk = kv_heads, c.D = D, c.slots = slots, c.Tn = k_new ? T : 0, c.window = window;
+  c.q_st = q_st, c.q_sh = q_sh, c.k_ss = k_ss, c.k_sh = k_sh, c.n_ss = n_ss, c.n_sh = n_sh, c.o_st = o_st, c.o_sh = o_sh;
+  c.tree_ld = tree_ld, c.qt = q_dtype, c.ct = kv_dtype, c.scale = scale;
+  return sbq::launch_tree_attention(c, (hipStream_t)stream);
+}
+
 }  // extern "C"

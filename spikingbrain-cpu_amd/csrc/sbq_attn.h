@@ -1,0 +1,441 @@
+// sbq_attn.h - attention of a few query tokens over a cache of keys and values
+// and over each other's (a tree of drafted tokens): the kernel and its
+// arguments, included by the files that instantiate it.
+//
+//   o[t,h] = sum_s softmax_s(scale * q[t,h] . k[s,h/rep]) v[s,h/rep]
+//
+// over the cached slots whose position lies in (q_pos[t] - window, q_pos[t]]
+// and the drafts that tree[t] names.  The cache is read once, which is what
+// bounds it at a few tokens; the rep = H / Hk query heads of a key head and
+// the T tokens make R = rep * T rows that share every key and value.
+//
+// A wave owns RT tiles of 16 rows and walks blocks of slots.  Both products
+// put the rows in the matrix instruction's columns: S^T = K Q^T leaves lane
+// (g, c) the scores of row c and four slots 4g + v, which is exactly the
+// operand that O^T = V^T P^T needs (k = the lane group's own slots), so the
+// softmax's weights go from one product to the other in their registers, a
+// row's running maximum and sum belong to its lanes, and its rescaling needs
+// no lane crossing.  V^T's operand holds one column of V for the lane
+// group's slots: a lane loads 16 bytes of a V row per slot and the 2-byte
+// types pair up two slots with one byte permute per register.  K and V go
+// from memory straight to registers; LDS only joins the waves.
+//
+// M16: 2-byte cache and queries of one type on 16x16x32, the weights rounded
+// to that type (half a step each, averaged over the slots of a sum; the sum
+// of weights itself stays in fp32).  Otherwise all products are fp32
+// (16x16x4), whatever the cache holds.
+//
+// The blocks are dealt in turn to the waves of all `splits` workgroups of a
+// row tile, so that a cache that is filled only at its front still keeps
+// every workgroup busy; a block that no row sees is left out after a look at
+// its positions.
+#pragma once
+
+#include "sbq_common.h"
+
+namespace sbq {
+
+constexpr int kAttnWaves = 4;
+
+struct AttnArgs {
+  const void *q, *k, *v, *kn, *vn;
+  const int64_t *slot_pos, *q_pos;
+  const uint8_t* tree;          // [T][tree_ld], null: draft j is seen by t >= j
+  void* out;
+  float *part_o, *scores;       // [Hk*R][splits][DP]; [Hk*R][spad] (null: not wanted)
+  float2* part_ml;              // [Hk*R][splits]
+  float2* row_ml;               // [Hk*R] (maximum, 1 / sum), with scores
+  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld, spad;
+  int64_t window;               // 0: none
+  int T, Hk, rep, D, slots, Tn, splits, rtiles, qt;
+  float scale;                  // times log2(e)
+};
+
+template <int CT>
+struct CElem {
+  typedef typename XElem<CT>::T T;
+  static constexpr int E = CT == XT_F32 ? 4 : 8;  // elements in 16 bytes
+};
+
+// N consecutive elements from d on; MODE 2: all inside D and aligned, 1: all
+// or none inside D, aligned, 0: any.  Elements from D on are zero.
+template <int CT, int N, int MODE>
+struct Piece {
+  typedef typename XElem<CT>::T T;
+  typedef T V __attribute__((ext_vector_type(N)));
+  V v;
+  __device__ __forceinline__ void load(const T* row, int d, int D) {
+    if constexpr (MODE == 2) {
+      v = *(const V*)(row + d);
+    } else if constexpr (MODE == 1) {
+      if (d < D) {
+        v = *(const V*)(row + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = d + j < D ? row[d + j] : (T)0.0f;
+    }
+  }
+};
+
+template <int CT>
+struct AttnMath;
+template <>
+struct AttnMath<XT_F16> {
+  typedef f16x8 V;
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct AttnMath<XT_BF16> {
+  typedef bf16x8 V;
+  static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct AttnMath<XT_F32> {
+  typedef f32x4 V;
+};
+
+__device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
+  return qt == XT_F32 ? ((const float*)q)[i] : qt == XT_F16 ? (float)((const _Float16*)q)[i] : (float)((const __bf16*)q)[i];
+}
+
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
+
+template <int CT, bool M16, int DP, int MODE, int RT>
+__global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
+  typedef typename XElem<CT>::T T;
+  typedef AttnMath<CT> Math;
+  constexpr int E = CElem<CT>::E, NCH = DP / (4 * E);
+  constexpr int SUB = M16 ? 2 : 1, SB = 16 * SUB, VS = M16 ? 8 : 4;
+  constexpr int EV = E < DP / 16 ? E : DP / 16, DB = DP / (16 * EV), NF = DB * EV;
+  constexpr int HP = DP < 128 ? DP : 128, OLD = HP + 4;  // columns of O joined at a time, LDS row of them
+  constexpr float kNone = -__builtin_inff();
+  __shared__ __align__(16) float lds_o[kAttnWaves * 16 * OLD];
+  __shared__ float lds_m[kAttnWaves][16], lds_l[kAttnWaves][16];
+
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.x % a.Hk, rtile = blockIdx.x / a.Hk % a.rtiles, split = blockIdx.x / a.Hk / a.rtiles;
+  const int R = a.rep * a.T, row0 = rtile * (16 * RT);
+
+  // the lane's rows and what they see: positions lo..hi
+  int row[RT], tok[RT];
+  int64_t lo[RT], hi[RT];
+  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    row[i] = row0 + i * 16 + c;
+    tok[i] = min(row[i], R - 1) / a.rep;
+    hi[i] = a.q_pos[tok[i]];
+    lo[i] = a.window > 0 && hi[i] - a.window + 1 > 0 ? hi[i] - a.window + 1 : 0;
+    // (a row past the last one is the last one again)
+    lo_min = min(lo_min, lo[i]), lo_max = max(lo_max, lo[i]), hi_min = min(hi_min, hi[i]), hi_max = max(hi_max, hi[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
+    lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
+    hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
+    hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
+  }
+
+  // Q^T operands
+  typename Math::V qf[RT][M16 ? NCH : 1];
+  float q32[RT][M16 ? 1 : NCH][E];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = min(row[i], R - 1);
+    const int64_t at = (int64_t)tok[i] * a.q_st + (int64_t)(kvh * a.rep + r % a.rep) * a.q_sh;
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int d = ch * 4 * E + g * E + j;
+        if constexpr (M16)
+          qf[i][ch][j] = d < a.D ? ((const T*)a.q)[at + d] : (T)0.0f;
+        else
+          q32[i][ch][j] = d < a.D ? load_q(a.q, a.qt, at + d) : 0.0f;
+      }
+  }
+
+  f32x4 o[RT][NF];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    m[i] = kNone, l[i] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[i][f] = (f32x4)(0.0f);
+  }
+
+  const int nbc = (a.slots + SB - 1) / SB, nb = nbc + (a.Tn + SB - 1) / SB, W = a.splits * kAttnWaves;
+  for (int b = split * kAttnWaves + w; b < nb; b += W) {
+    const bool fresh = b >= nbc;
+    const int base = (fresh ? b - nbc : b) * SB, last = (fresh ? a.Tn : a.slots) - 1;
+    bool full = false;
+    if (!fresh) {
+      const int s = base + (lane & (SB - 1));
+      const int64_t sp = s <= last ? a.slot_pos[s] : -1;
+      if (!__any(sp >= lo_min && sp <= hi_max)) continue;
+      full = __all(sp >= lo_max && sp <= hi_min);
+    }
+    const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
+    const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
+    const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
+
+    Piece<CT, E, MODE> kf[SUB][NCH];
+    Piece<CT, EV, MODE> vf[VS][DB];
+#pragma unroll
+    for (int st = 0; st < SUB; ++st)
+#pragma unroll
+      for (int ch = 0; ch < NCH; ++ch)
+        kf[st][ch].load(kp + min(base + st * 16 + c, last) * ss, ch * 4 * E + g * E, a.D);
+#pragma unroll
+    for (int j = 0; j < VS; ++j)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        vf[j][db].load(vp + min(base + (j >> 2) * 16 + 4 * g + (j & 3), last) * ss, db * 16 * EV + c * EV, a.D);
+
+    float p[RT][SUB][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+#pragma unroll
+      for (int st = 0; st < SUB; ++st) {
+        f32x4 s = (f32x4)(0.0f);
+#pragma unroll
+        for (int ch = 0; ch < NCH; ++ch) {
+          if constexpr (M16) {
+            s = Math::mfma(__builtin_bit_cast(typename Math::V, kf[st][ch].v), qf[i][ch], s);
+          } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              s = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kf[st][ch].v[j], q32[i][ch][j], s, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[i][st][v] = s[v] * a.scale;
+        if (a.scores && !fresh && row[i] < R)
+          *(f32x4*)(a.scores + ((int64_t)kvh * R + row[i]) * a.spad + base + st * 16 + 4 * g) =
+              (f32x4){p[i][st][0], p[i][st][1], p[i][st][2], p[i][st][3]};
+      }
+      uint32_t seen = 0xff;  // bit st * 4 + v
+      if (!full) {
+        seen = 0;
+#pragma unroll
+        for (int st = 0; st < SUB; ++st)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int s = base + st * 16 + 4 * g + v;
+            bool ok = s <= last;
+            if (ok && !fresh) {
+              const int64_t sp = a.slot_pos[s];
+              ok = sp >= lo[i] && sp <= hi[i];
+            } else if (ok) {
+              ok = a.tree ? a.tree[(int64_t)tok[i] * a.tree_ld + s] != 0 : s <= tok[i];
+              ok = ok && (a.window == 0 || a.q_pos[s] > hi[i] - a.window);
+            }
+            seen |= ok ? 1u << (st * 4 + v) : 0u;
+          }
+      }
+      float mx = kNone;
+#pragma unroll
+      for (int st = 0; st < SUB; ++st)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (seen >> (st * 4 + v) & 1) mx = __builtin_fmaxf(mx, p[i][st][v]);
+      if (__any(mx > m[i])) {
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float up = __builtin_fmaxf(m[i], mx);
+        const float alpha = up == kNone ? 1.0f : __builtin_exp2f(m[i] - up);
+        m[i] = up;
+        l[i] *= alpha;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[i][f] *= alpha;
+      }
+      const float from = m[i] == kNone ? 0.0f : m[i];
+#pragma unroll
+      for (int st = 0; st < SUB; ++st)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float e = __builtin_exp2f(p[i][st][v] - from);
+          p[i][st][v] = seen >> (st * 4 + v) & 1 ? e : 0.0f;
+          l[i] += p[i][st][v];
+        }
+      // Where a row does not see every slot, an infinity or NaN in a V that
+      // is hidden from it must not reach it as 0 * inf: such values are
+      // taken out of the product and added to the rows that do see them.
+      if (!full) {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < VS; ++j)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int e = 0; e < EV; ++e) odd |= !finite((float)vf[j][db].v[e]);
+        if (__any(odd)) {
+          float* const own = lds_o + w * 16 * OLD;  // [SB][16]
+#pragma unroll
+          for (int st = 0; st < SUB; ++st)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              own[(st * 16 + 4 * g + v) * 16 + c] = seen >> (st * 4 + v) & 1 ? p[i][st][v] : -1.0f;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+          for (int s = 0; s < SB; ++s) {
+            const float ps = own[s * 16 + c];
+            const T* const vr = vp + min(base + s, last) * ss;
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const int d = f / EV * 16 * EV + (4 * g + v) * EV + f % EV;
+                const float x = d < a.D ? (float)vr[d] : 0.0f;
+                if (!finite(x) && !(ps < 0.0f)) o[i][f][v] += ps * x;
+              }
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+    if (!full) {
+#pragma unroll
+      for (int j = 0; j < VS; ++j)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < EV; ++e)
+            vf[j][db].v[e] = finite((float)vf[j][db].v[e]) ? vf[j][db].v[e] : (T)0.0f;
+    }
+
+    // O^T += V^T P^T
+    if constexpr (M16) {
+      typename Math::V pf[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[i][j] = (T)p[i][j >> 2][j & 3];
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        typedef uint32_t Words __attribute__((ext_vector_type(EV / 2)));
+        Words vw[VS];
+#pragma unroll
+        for (int j = 0; j < VS; ++j) vw[j] = __builtin_bit_cast(Words, vf[j][db].v);
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          u32x4 t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          const typename Math::V vt = __builtin_bit_cast(typename Math::V, t);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) o[i][db * EV + e] = Math::mfma(vt, pf[i], o[i][db * EV + e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < EV; ++e)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+              o[i][db * EV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)vf[j][db].v[e], p[i][0][j],
+                                                                       o[i][db * EV + e], 0, 0, 0);
+    }
+  }
+
+  // the workgroup's waves joined, one row tile at a time
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    l[i] += __shfl_xor(l[i], 16, 64);
+    l[i] += __shfl_xor(l[i], 32, 64);
+#pragma unroll
+    for (int h0 = 0; h0 < DP; h0 += HP) {
+      __syncthreads();  // (lds_o is free)
+      if (g == 0) lds_m[w][c] = m[i], lds_l[w][c] = l[i];
+      float* const to = lds_o + (w * 16 + c) * OLD;
+#pragma unroll
+      for (int db = h0 / (16 * EV); db < (h0 + HP) / (16 * EV); ++db)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int e = 0; e < EV; ++e) to[db * 16 * EV - h0 + (4 * g + v) * EV + e] = o[i][db * EV + e][v];
+      __syncthreads();
+      const int r0 = row0 + i * 16;
+      for (int u = threadIdx.x; u < 16 * (HP / 4); u += kAttnWaves * 64) {
+        const int rr = u / (HP / 4), d = h0 + u % (HP / 4) * 4;
+        if (r0 + rr >= R) continue;
+        float top = kNone;
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k) top = __builtin_fmaxf(top, lds_m[k][rr]);
+        const float from = top == kNone ? 0.0f : top;
+        f32x4 sum = (f32x4)(0.0f);
+        float ls = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k) {
+          const float f = __builtin_exp2f(lds_m[k][rr] - from);
+          const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
+          if (lds_l[k][rr] != 0.0f) {  // (a wave that saw nothing adds nothing)
+            sum += x * f;
+            ls += lds_l[k][rr] * f;
+          }
+        }
+        const int64_t at = (int64_t)kvh * R + r0 + rr;
+        if (a.splits > 1) {
+          *(f32x4*)(a.part_o + (at * a.splits + split) * DP + d) = sum;
+          if (d == 0) a.part_ml[at * a.splits + split] = make_float2(top, ls);
+        } else {
+          const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
+          const int t = (r0 + rr) / a.rep, h = kvh * a.rep + (r0 + rr) % a.rep;
+          const int64_t out = (int64_t)t * a.o_st + (int64_t)h * a.o_sh + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.D) store_y(a.out, a.qt, out + e, sum[e] * inv);
+          if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
+        }
+      }
+    }
+  }
+}
+
+// One attention launch of a configuration; defined per pair (cache type,
+// 2-byte products) in the files that instantiate the kernel.
+template <int CT, bool M16, int DP>
+int launch_attn_dp(const AttnArgs& a, int mode, int RT, hipStream_t st) {
+  const dim3 grid((unsigned)(a.Hk * a.rtiles * a.splits));
+  if (mode == 2) {
+    bool done = false;
+    if constexpr (M16 || DP < 256) {  // (two tiles of 256 fp32 columns do not fit the registers)
+      if ((done = RT == 2)) attn_kernel<CT, M16, DP, 2, 2><<<grid, kAttnWaves * 64, 0, st>>>(a);
+    }
+    if (!done) attn_kernel<CT, M16, DP, 2, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
+  } else if (mode == 1) {
+    attn_kernel<CT, M16, DP, 1, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
+  } else if constexpr (!M16) {
+    attn_kernel<CT, M16, DP, 0, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : -5;
+}
+
+template <int CT, bool M16>
+int launch_attn_ct(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st) {
+  return DP == 64 ? launch_attn_dp<CT, M16, 64>(a, mode, RT, st)
+         : DP == 128 ? launch_attn_dp<CT, M16, 128>(a, mode, RT, st)
+                     : launch_attn_dp<CT, M16, 256>(a, mode, RT, st);
+}
+
+int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st);
+int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st);
+int launch_attn_bf16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st);
+
+}  // namespace sbq

@@ -1,0 +1,161 @@
+// sbq_attn.hip - attention over a cache with a tree of drafted tokens: the
+// instances for an fp32 cache, the plan, the joining of the splits and the
+// attention weight that each slot received (sbq_attn.h holds the kernel).
+#include "sbq_attn.h"
+
+#include "sbq_launch.h"
+
+namespace sbq {
+
+int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st) {
+  return launch_attn_ct<XT_F32, false>(a, DP, mode, RT, st);
+}
+
+namespace {
+
+// One row's splits joined: the maximum over their maxima, then the partial
+// sums scaled to it.
+template <int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int ND = DP / 4, NG = 256 / ND;
+  __shared__ __align__(16) f32x4 lds[NG][ND];
+  __shared__ float lds_l[NG];
+  const int64_t at = blockIdx.x;
+  const int R = a.rep * a.T, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
+  const float2* const ml = a.part_ml + at * a.splits;
+  float top = -__builtin_inff();
+  for (int s = 0; s < a.splits; ++s) top = __builtin_fmaxf(top, ml[s].x);
+  const float from = top == -__builtin_inff() ? 0.0f : top;
+  f32x4 sum = (f32x4)(0.0f);
+  float l = 0.0f;
+  for (int s = grp; s < a.splits; s += NG) {
+    const f32x4 x = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
+    const float f = __builtin_exp2f(ml[s].x - from);
+    if (ml[s].y != 0.0f) {  // (a split that saw nothing adds nothing)
+      sum += x * f;
+      l += ml[s].y * f;
+    }
+  }
+  lds[grp][threadIdx.x % ND] = sum;
+  if (d == 0) lds_l[grp] = l;
+  __syncthreads();
+  if (grp) return;
+  l = lds_l[0];
+  for (int k = 1; k < NG; ++k) {
+    sum += lds[k][threadIdx.x];
+    l += lds_l[k];
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const int kvh = (int)(at / R), r = (int)(at % R);
+  const int64_t out = (int64_t)(r / a.rep) * a.o_st + (int64_t)(kvh * a.rep + r % a.rep) * a.o_sh + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < a.D) store_y(a.out, a.qt, out + e, sum[e] * inv);
+  if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
+}
+
+// weight[s] += sum over the rows that see slot s of exp2(score - max) / sum,
+// 64 slots per workgroup, the rows dealt to its waves and added in wave order.
+__global__ __launch_bounds__(256) void attn_weight_kernel(AttnArgs a, float* weight) {
+  __shared__ float lds[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, s = blockIdx.x * 64 + lane;
+  const int R = a.rep * a.T;
+  const int64_t sp = s < a.slots ? a.slot_pos[s] : -1;
+  float sum = 0.0f;
+  for (int kvh = 0; kvh < a.Hk; ++kvh)
+    for (int r = w; r < R; r += 4) {
+      const int64_t hi = a.q_pos[r / a.rep], lo = a.window > 0 ? hi - a.window + 1 : 0, at = (int64_t)kvh * R + r;
+      if (sp < 0 || sp < lo || sp > hi) continue;
+      const float2 ml = a.row_ml[at];
+      sum += __builtin_exp2f(a.scores[at * a.spad + s] - ml.x) * ml.y;
+    }
+  lds[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && s < a.slots) weight[s] += lds[0][lane] + lds[1][lane] + lds[2][lane] + lds[3][lane];
+}
+
+constexpr int kAttnGroups = 512;  // workgroups aimed at
+
+int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+struct AttnPlan {
+  int RT, rtiles, splits;
+};
+AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t blocks, bool wide) {
+  AttnPlan p;
+  p.RT = wide && R > 16 ? 2 : 1;
+  p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
+  const int64_t room = kAttnGroups / (Hk * p.rtiles), most = (blocks + kAttnWaves - 1) / kAttnWaves;
+  p.splits = (int)(room < 1 ? 1 : room < most ? room : most);
+  return p;
+}
+
+int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t slots, bool weight) {
+  const int64_t R = heads / Hk * T, rows = Hk * R;
+  int64_t splits = 1;
+  for (int wide = 0; wide < 2; ++wide) {
+    const int64_t s = attn_plan(R, Hk, (slots + 15) / 16 + (T + 15) / 16, wide).splits;
+    splits = s > splits ? s : splits;
+  }
+  int64_t n = 0;
+  if (splits > 1) n += round256(rows * splits * attn_dp(D) * 4) + round256(rows * splits * 8);
+  if (weight) n += round256(rows * 8) + round256(rows * ((slots + 31) / 32 * 32) * 4);
+  return n;
+}
+
+int launch_tree_attention(const AttnCall& c, hipStream_t st) {
+  const int64_t es = c.ct == XT_F32 ? 4 : 2;
+  auto vec = [&](const void* p, int64_t a, int64_t b) {
+    return (uintptr_t)p % 16 == 0 && a * es % 16 == 0 && b * es % 16 == 0;
+  };
+  const int DP = attn_dp(c.D);
+  const bool aligned = c.D * es % 16 == 0 && vec(c.k, c.k_ss, c.k_sh) && vec(c.v, c.k_ss, c.k_sh) &&
+                       (c.Tn == 0 || (vec(c.kn, c.n_ss, c.n_sh) && vec(c.vn, c.n_ss, c.n_sh)));
+  const int mode = !aligned ? 0 : c.D == DP ? 2 : 1;
+  const bool m16 = c.ct != XT_F32 && c.qt == c.ct && mode > 0;
+  const int64_t Hk = c.Hk, rep = c.heads / Hk, R = rep * c.T, SB = m16 ? 32 : 16;
+  const AttnPlan p = attn_plan(R, Hk, (c.slots + SB - 1) / SB + (c.Tn + SB - 1) / SB, mode == 2 && (m16 || DP < 256));
+  AttnArgs a{};
+  a.q = c.q, a.k = c.k, a.v = c.v, a.kn = c.kn, a.vn = c.vn, a.slot_pos = c.slot_pos, a.q_pos = c.q_pos, a.tree = c.tree;
+  a.out = c.out;
+  a.q_st = c.q_st, a.q_sh = c.q_sh, a.k_ss = c.k_ss, a.k_sh = c.k_sh, a.n_ss = c.n_ss, a.n_sh = c.n_sh;
+  a.o_st = c.o_st, a.o_sh = c.o_sh, a.tree_ld = c.tree_ld, a.window = c.window;
+  a.T = (int)c.T, a.Hk = (int)Hk, a.rep = (int)rep, a.D = (int)c.D, a.slots = (int)c.slots, a.Tn = (int)c.Tn;
+  a.splits = p.splits, a.rtiles = p.rtiles, a.qt = c.qt;
+  a.scale = c.scale * 1.44269504f;
+  uint8_t* ws = (uint8_t*)c.ws;
+  if (p.splits > 1) {
+    a.part_o = (float*)ws;
+    ws += round256(Hk * R * p.splits * DP * 4);
+    a.part_ml = (float2*)ws;
+    ws += round256(Hk * R * p.splits * 8);
+  }
+  if (c.weight) {
+    a.row_ml = (float2*)ws;
+    ws += round256(Hk * R * 8);
+    a.scores = (float*)ws;
+    a.spad = (c.slots + 31) / 32 * 32;
+  }
+  int rc = c.ct == XT_F32   ? launch_attn_f32(a, DP, mode, p.RT, st)
+           : c.ct == XT_F16 ? launch_attn_f16(a, m16, DP, mode, p.RT, st)
+                            : launch_attn_bf16(a, m16, DP, mode, p.RT, st);
+  if (rc) return rc;
+  if (p.splits > 1) {
+    const unsigned grid = (unsigned)(Hk * R);
+    if (DP == 64)
+      attn_join_kernel<64><<<grid, 256, 0, st>>>(a);
+    else if (DP == 128)
+      attn_join_kernel<128><<<grid, 256, 0, st>>>(a);
+    else
+      attn_join_kernel<256><<<grid, 256, 0, st>>>(a);
+    if ((rc = check_launch())) return rc;
+  }
+  if (c.weight) attn_weight_kernel<<<(unsigned)((c.slots + 63) / 64), 256, 0, st>>>(a, c.weight);
+  return check_launch();
+}
+
+}  // namespace sbq

@@ -1,0 +1,12 @@
+// sbq_attn_f16.hip - attention over a cache of fp16 (sbq_attn.h): 2-byte products where
+// the queries are of the same type, fp32 products for fp32 queries and for
+// rows that 16-byte loads cannot read.
+#include "sbq_attn.h"
+
+namespace sbq {
+
+int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st) {
+  return m16 ? launch_attn_ct<XT_F16, true>(a, DP, mode, RT, st) : launch_attn_ct<XT_F16, false>(a, DP, mode, RT, st);
+}
+
+}  // namespace sbq

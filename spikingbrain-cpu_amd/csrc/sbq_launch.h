@@ -232,4 +232,21 @@ int launch_linear_w4(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, b
                      const uint16_t* gscale, const float* bias, int64_t N, int group, void* y, int yt, int64_t ldy, bool yvec,
                      hipStream_t st);
 
+// Attention over a cache and a tree of drafted tokens (sbq_attn.hip); strides
+// in elements, k and v share theirs, kn and vn theirs.
+struct AttnCall {
+  const void *q, *k, *v, *kn, *vn;
+  const int64_t *slot_pos, *q_pos;
+  const uint8_t* tree;
+  void* out;
+  float* weight;
+  void* ws;
+  int64_t T, heads, Hk, D, slots, Tn, window;
+  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld;
+  int qt, ct;
+  float scale;
+};
+int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t slots, bool weight);
+int launch_tree_attention(const AttnCall& c, hipStream_t st);
+
 }  // namespace sbq

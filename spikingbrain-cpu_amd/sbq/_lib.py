@@ -14,6 +14,7 @@ SBQ_OK = 0
 SBQ_F32, SBQ_F16, SBQ_BF16 = 0, 1, 2
 SBQ_NOALLOC_XQ_BYTES = 8 << 20  # include/sbq.h
 SBQ_ARGMAX_WS_BYTES = 16640  # include/sbq.h
+SBQ_ATTN_MAX_T = 1024  # query tokens of one sbq_tree_attention call (include/sbq.h)
 SBQ_MAX_GROUP = 4  # linears per sbq_linear_w8_grouped / sbq_linear_w8a8_grouped call (include/sbq.h)
 
 # Every entry point declared in include/sbq.h, with its ctypes signature.
@@ -56,6 +57,9 @@ SIGNATURES = {
     "sbq_repack_w4": (_I, [_P, _L, _L, _L, _P, _I, _P, _P, _P]),
     "sbq_unpack_w4": (_I, [_P, _P, _L, _L, _I, _P, _L, _P, _P]),
     "sbq_linear_w4": (_I, [_P, _I, _L, _L, _L, _P, _P, _P, _L, _I, _P, _I, _L, _P]),
+    "sbq_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _I]),
+    "sbq_tree_attention": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L,
+                                _L, ctypes.c_float, _P, _L, _L, _P, _P, _S, _P]),
     "sbq_sample_rows": (_I, [_P, _L, _L, _L, ctypes.c_float, _L, ctypes.c_float, _P, _P, _P, _S, _P]),
 }
 

@@ -31,11 +31,110 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import _lib
+from .quant import _DTYPE_CODE, _on_device, _stream
+
 
 def _as_pos(p, device: torch.device) -> torch.Tensor:
     if isinstance(p, torch.Tensor):
         return p.reshape(1).to(device=device, dtype=torch.long)
     return torch.tensor([int(p)], dtype=torch.long, device=device)
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """t [n, heads, dim] with unit stride in dim (else a contiguous copy)."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def attention_workspace(T: int, heads: int, kv_heads: int, dim: int, slots: int, weight: bool,
+                        device: torch.device) -> torch.Tensor:
+    """Scratch of tree_attention for these sizes (any content; one call at a time)."""
+    n = _lib.load().sbq_attn_workspace_bytes(T, heads, kv_heads, dim, slots, int(weight))
+    return torch.empty((n,), dtype=torch.uint8, device=device)
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: torch.Tensor, q_pos: torch.Tensor,
+                   k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None,
+                   tree: torch.Tensor | None = None, window: int | None = None, scale: float | None = None,
+                   weight: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention of model.py:208-229 on the GPU for q [T, heads, dim] at
+    positions q_pos [T] over a cache k, v [slots, kv_heads, dim] whose slots
+    hold the positions slot_pos [slots] (-1: empty), and over the T tokens'
+    own keys and values k_new, v_new [T, kv_heads, dim] where they are given:
+    drafted tokens that are not in the cache, verified in one pass.  Query
+    head h reads key head h // (heads / kv_heads).
+
+    Token t sees a cached slot iff 0 <= slot_pos <= q_pos[t], and draft j iff
+    tree[t, j] (bool [T, T], normally t's ancestors and itself; None: j <= t);
+    with a window also only positions > q_pos[t] - window.  A row that sees
+    nothing is 0; what a row does not see does not reach it.
+
+    q has the cache's dtype or fp32 (then all products are fp32); the result
+    has q's.  scale defaults to dim ** -0.5.  weight: fp32 [slots], to which
+    the attention weight that each cached slot received, summed over tokens
+    and heads, is added."""
+    if not q.is_cuda:
+        raise ValueError("tree_attention: q must be a GPU tensor")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise ValueError("tree_attention: expected q [T, heads, dim] and k, v [slots, kv_heads, dim]")
+    gpu = q.get_device()
+    T, heads, dim = q.shape
+    slots, kv_heads = k.shape[0], k.shape[1]
+    if k.dtype not in _DTYPE_CODE or v.dtype != k.dtype or (q.dtype != k.dtype and q.dtype != torch.float32):
+        raise ValueError("tree_attention: k and v must share a dtype (float32, float16 or bfloat16), q have it or float32")
+    if not 1 <= dim <= 256 or kv_heads < 1 or heads < 1 or heads % kv_heads or slots < 1:
+        raise ValueError("tree_attention: 1 <= dim <= 256, heads a multiple of kv_heads, and slots >= 1")
+    if T > _lib.SBQ_ATTN_MAX_T:
+        raise ValueError(f"tree_attention: at most {_lib.SBQ_ATTN_MAX_T} tokens per call")
+    if k.get_device() != gpu or v.get_device() != gpu or k.stride() != v.stride() or (dim > 1 and k.stride(2) != 1):
+        raise ValueError(f"tree_attention: k and v must be on {q.device}, with the same strides and unit stride in dim")
+    if (slot_pos.dtype != torch.int64 or slot_pos.get_device() != gpu or slot_pos.shape != (slots,)
+            or not slot_pos.is_contiguous()):
+        raise ValueError(f"tree_attention: slot_pos must be a contiguous int64 [{slots}] tensor on {q.device}")
+    if q_pos.dtype != torch.int64 or q_pos.get_device() != gpu or q_pos.numel() != T or not q_pos.is_contiguous():
+        raise ValueError(f"tree_attention: q_pos must be a contiguous int64 tensor of {T} positions on {q.device}")
+    if window is not None and window < 1:
+        raise ValueError("tree_attention: window must be >= 1")
+    if (k_new is None) != (v_new is None) or (tree is not None and k_new is None):
+        raise ValueError("tree_attention: k_new and v_new go together, and tree with them")
+    if k_new is not None:
+        if k_new.shape != (T, kv_heads, dim) or v_new.shape != k_new.shape or k_new.get_device() != gpu \
+                or v_new.get_device() != gpu or k_new.dtype != k.dtype or v_new.dtype != k.dtype:
+            raise ValueError(f"tree_attention: k_new and v_new must be {k.dtype} [T={T}, {kv_heads}, {dim}] on {q.device}")
+        k_new, v_new = _rows_of(k_new), _rows_of(v_new)
+        if k_new.stride() != v_new.stride():
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    if tree is not None:
+        if tree.dtype not in (torch.bool, torch.uint8) or tree.shape != (T, T) or tree.get_device() != gpu:
+            raise ValueError(f"tree_attention: tree must be a bool [T={T}, T] tensor on {q.device}")
+        if not tree.is_contiguous():
+            tree = tree.contiguous()
+    if weight is not None and (weight.dtype != torch.float32 or weight.get_device() != gpu or weight.shape != (slots,)
+                               or not weight.is_contiguous()):
+        raise ValueError(f"tree_attention: weight must be a contiguous float32 [{slots}] tensor on {q.device}")
+    if out is None:
+        out = torch.empty((T, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(2) != 1):
+        raise ValueError("tree_attention: out must have q's shape, dtype and device, with unit stride in dim")
+    if T == 0:
+        return out
+    q = _rows_of(q)
+    if workspace is None:
+        workspace = attention_workspace(T, heads, kv_heads, dim, slots, weight is not None, q.device)
+    elif workspace.get_device() != gpu or not workspace.is_contiguous():
+        raise ValueError(f"tree_attention: workspace must be a contiguous tensor on {q.device}")
+    qs, ks, os_ = q.stride(), k.stride(), out.stride()
+    ns = (0, 0) if k_new is None else k_new.stride()
+    with _on_device(q.device):
+        _lib.check(_lib.load().sbq_tree_attention(
+            q.data_ptr(), _DTYPE_CODE[q.dtype], T, heads, dim, qs[0], qs[1], k.data_ptr(), v.data_ptr(),
+            _DTYPE_CODE[k.dtype], slots, kv_heads, ks[0], ks[1], slot_pos.data_ptr(), q_pos.data_ptr(),
+            None if k_new is None else k_new.data_ptr(), None if v_new is None else v_new.data_ptr(), ns[0], ns[1],
+            None if tree is None else tree.data_ptr(), T, window or 0, dim ** -0.5 if scale is None else scale,
+            out.data_ptr(), os_[0], os_[1], None if weight is None else weight.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream(q.device)), "sbq_tree_attention")
+    return out
 
 
 class DeviceKVBuffer:
@@ -98,6 +197,18 @@ class DeviceKVBuffer:
         if self.window is not None:
             ok &= kp > qp - self.window
         return ok
+
+    def attend(self, q: torch.Tensor, q_pos: torch.Tensor, k_new: torch.Tensor | None = None,
+               v_new: torch.Tensor | None = None, tree: torch.Tensor | None = None, scale: float | None = None,
+               weight: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """The attention of queries q [T, heads, dim] at positions q_pos [T]
+        over the stored keys that visible(q_pos) names and, for a tree of
+        drafted tokens, over their own k_new, v_new [T, self.heads, dim] by
+        tree [T, T]; see tree_attention.  Drafts are not stored: append the
+        accepted ones.  A whole call can be captured in a HIP graph."""
+        return tree_attention(q, self.k, self.v, self.slot_pos, q_pos, k_new, v_new, tree, self.window, scale, weight,
+                              out, workspace)
 
     def truncate(self, length) -> None:
         """Forget positions >= length (the engine's prefix reuse restores a

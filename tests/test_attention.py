@@ -1,0 +1,340 @@
+"""Attention over a cache and a tree of drafted tokens (sbq.state.
+tree_attention, DeviceKVBuffer.attend) against the formula in 64 bits.
+
+Tolerances, from the arithmetic: with x = sum of |scale q k| over dim, a
+score carries at most (dim + 2) fp32 roundings, 2^-24 (dim + 2) x, and so
+does the exponent of its weight; exp2, the rescalings and the sums of n
+weights add at most 2^-24 (n / 16 + 64) relative (a lane group's sums run
+over a quarter of the rows; 64 covers the joins); every weight error is at
+most e = 2^-24 (dim + 2) max x + 2^-24 (n / 16 + 64) relative, in numerator
+and denominator, so an output is off by 2 e max|v| at most.  2-byte queries
+round each weight and the output by half a step of their type.  A slot's
+summed attention weight is off by 2 e of itself and its additions.
+"""
+import ctypes
+
+import pytest
+import torch
+
+from conftest import announce
+from sbq import _lib
+from sbq.state import DeviceKVBuffer, tree_attention
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+# ---------------------------------------------------------------------------
+# refusals (CPU)
+# ---------------------------------------------------------------------------
+def test_c_abi_refuses_bad_arguments():
+    L = _lib.load()
+    p = 1 << 16  # never read: every call below is refused
+
+    def attn(q=p, qt=0, T=1, H=4, D=64, qst=256, qsh=64, k=p, v=p, ct=0, slots=8, Hk=2, kss=128, ksh=64, sp=p, qp=p, kn=None,
+             vn=None, nss=0, nsh=0, tree=None, tld=0, window=0, scale=0.1, out=p, ost=256, osh=64, weight=None, ws=p,
+             nws=1 << 30):
+        return L.sbq_tree_attention(q, qt, T, H, D, qst, qsh, k, v, ct, slots, Hk, kss, ksh, sp, qp, kn, vn, nss, nsh, tree,
+                                    tld, window, scale, out, ost, osh, weight, ws, nws, None)
+
+    assert attn(qt=5) == -2 and attn(ct=-1) == -2 and attn(qt=1) == -2 and attn(qt=1, ct=2) == -2
+    assert attn(T=-1) == -1 and attn(T=1025) == -1 and attn(H=5) == -1 and attn(D=0) == -1 and attn(D=257) == -1
+    assert attn(slots=0) == -1 and attn(slots=(1 << 30) + 1) == -1 and attn(Hk=0) == -1 and attn(window=-1) == -1
+    assert attn(scale=float("nan")) == -1
+    for name in ("q", "k", "v", "sp", "qp", "out"):
+        assert attn(**{name: None}) == -1
+    assert attn(kn=p) == -1 and attn(vn=p) == -1 and attn(tree=p, tld=1) == -1
+    assert attn(kn=p, vn=p, tree=p, tld=0) == -1 and attn(kss=-1) == -1
+    assert attn(sp=p + 4) == -3 and attn(q=p + 2) == -3 and attn(weight=p + 2) == -3
+    assert attn(ws=None) == -4 and attn(nws=8) == -4
+    assert attn(T=0) == 0
+    need = L.sbq_attn_workspace_bytes(1, 32, 8, 128, 4096, 1)
+    assert need > L.sbq_attn_workspace_bytes(1, 32, 8, 128, 4096, 0) > 0
+    assert attn(H=32, Hk=8, D=128, slots=4096, weight=p, nws=need - 1) == -4
+    assert L.sbq_attn_workspace_bytes(1, 5, 2, 64, 8, 0) == 0 and L.sbq_attn_workspace_bytes(0, 4, 2, 64, 8, 0) == 0
+
+
+def test_python_refuses_cpu_tensors():
+    buf = DeviceKVBuffer(2, 8, 16, device="cpu")
+    with pytest.raises(ValueError, match="GPU"):
+        buf.attend(torch.zeros(1, 4, 8), torch.zeros(1, dtype=torch.long))
+
+
+# ---------------------------------------------------------------------------
+# the formula
+# ---------------------------------------------------------------------------
+def _formula(q, k, v, see, scale):
+    """(out, p) in 64 bits; see [T, slots]; a row that sees nothing is 0."""
+    T, H, D = q.shape
+    rep = H // k.shape[1]
+    out, ps = torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(H, T, k.shape[0], dtype=torch.float64)
+    xmax = 0.0
+    for h in range(H):
+        kh, vh, qh = k[:, h // rep].double(), v[:, h // rep].double(), q[:, h].double()
+        z = (qh @ kh.t()) * scale
+        xmax = max(xmax, float((qh.abs() @ kh.abs().t()).max()) * abs(scale))
+        for t in range(T):
+            at = see[t].nonzero()[:, 0]
+            if len(at):
+                p = torch.softmax(z[t, at], 0)
+                ps[h, t, at] = p
+                out[t, h] = p @ vh[at]
+    return out, ps, xmax
+
+
+def _compare(o, weight, weight0, q, k, v, see, scale, slots):
+    """Outputs (on the CPU) against the formula; k, v hold the drafts last."""
+    want, p, xmax = _formula(q, k, v, see, scale)
+    D, n = q.shape[2], k.shape[0]
+    e = 2.0 ** -24 * ((D + 2) * xmax + n / 16 + 64)
+    half = torch.finfo(o.dtype).eps / 2
+    vmax = float(v.double().abs().max())
+    tol = 2 * e * vmax
+    if q.dtype != F32:
+        tol += half * vmax  # the weights' roundings: at most half a step of each
+        if q.dtype == F16:
+            tol += n * 2.0 ** -25 * vmax  # ... or of fp16's smallest step, against a sum of at least 1
+    off = (o.double() - want).abs()
+    bound = tol + (want.abs() + tol) * half + torch.finfo(o.dtype).tiny
+    assert bool((off <= bound).all()), f"worst {float((off / bound).max()):.3g} of the bound"
+    if weight is not None:
+        w = p[:, :, :slots].sum((0, 1))
+        tol = 2 * e * w + 2.0 ** -24 * (w + weight0.double().abs()) * (p.shape[0] * p.shape[1] / 4 + 6)
+        off = (weight.double() - weight0.double() - w).abs()
+        assert bool((off <= tol + 1e-30).all()), f"weight: {float((off - tol).max()):.3g} over the bound"
+
+
+def _tree(T, g):
+    parent = [-1] + [int(torch.randint(0, i, (1,), generator=g)) for i in range(1, T)]
+    tree, depth = torch.eye(T, dtype=torch.bool), [0] * T
+    for i in range(1, T):
+        tree[i] |= tree[parent[i]]
+        depth[i] = depth[parent[i]] + 1
+    return tree, torch.tensor(depth)
+
+
+def _see(slot_pos, q_pos, tree, window):
+    far = window or 1 << 40
+    age = q_pos[:, None] - slot_pos[None]
+    see = (slot_pos[None] >= 0) & (age >= 0) & (age < far)
+    if tree is not None:
+        see = torch.cat([see, tree & (q_pos[:, None] - q_pos[None] < far)], 1)
+    return see
+
+
+def _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight, seed=0):
+    g = torch.Generator().manual_seed(seed + T * 31 + slots)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    k, v, q = r(slots, kv, D).to(ct), r(slots, kv, D).to(ct), (r(T, heads, D) * 1.5).to(qt)
+    at = torch.arange(slots)
+    if window:
+        pos = filled - 1 - (filled - 1 - at) % slots
+        pos = torch.where(pos < 0, -1, pos)
+    else:
+        pos = torch.where(at < filled, at, -1)
+    kn = vn = tree = None
+    if drafts:
+        kn, vn = r(T, kv, D).to(ct), r(T, kv, D).to(ct)
+        tree, depth = _tree(T, g)
+        q_pos = filled + depth
+    else:
+        q_pos = filled - T + torch.arange(T)
+    w0 = torch.rand(slots, generator=g) if weight else None
+    to = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    buf = DeviceKVBuffer(kv, D, slots, window, dev, ct)
+    buf.k.copy_(k), buf.v.copy_(v), buf.slot_pos.copy_(pos)
+    wd = to(w0)
+    announce(f"attend T={T} heads={heads}/{kv} D={D} slots={slots} filled={filled} window={window} {qt} over {ct} "
+             f"drafts={drafts} weight={weight}")
+    o = buf.attend(to(q), to(q_pos), to(kn), to(vn), to(tree), weight=wd)
+    assert o.dtype == qt and o.shape == q.shape
+    if drafts:
+        k, v = torch.cat([k, kn]), torch.cat([v, vn])
+    _compare(o.cpu(), None if wd is None else wd.cpu(), w0, q, k, v, _see(pos, q_pos, tree, window), D ** -0.5, slots)
+    return buf, q, q_pos, o
+
+
+TYPES = [(F32, F32), (F16, F16), (BF16, BF16), (F32, F16), (F32, BF16)]
+IDS = ["f32", "f16", "bf16", "f32_f16", "f32_bf16"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [64, 128, 256, 80, 1, 33, 200])
+def test_attend_types_and_widths(dev, D, qt, ct):
+    for T, heads, kv, slots, filled, window, drafts, weight in (
+            (1, 4, 1, 1, 1, None, False, False), (1, 8, 2, 100, 77, None, False, True),
+            (5, 14, 2, 257, 300, 200, True, True), (9, 8, 8, 640, 640, None, True, False),
+            (3, 6, 3, 70, 90, 60, False, True)):
+        _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+def test_attend_long_and_many_rows(dev, qt, ct):
+    for T, heads, kv, D, slots, filled, window, drafts, weight in (
+            (1, 32, 8, 128, 5000, 4321, None, False, True), (16, 8, 2, 128, 3000, 2990, None, True, True),
+            (64, 16, 2, 64, 1111, 1000, None, True, False), (130, 2, 1, 128, 500, 200, None, True, True),
+            (64, 4, 4, 256, 1500, 1400, None, False, False), (33, 7, 1, 128, 900, 2000, 850, True, True)):
+        _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+def test_attend_empty_rows_and_hidden_values(dev, qt, ct):
+    """Rows that see nothing are 0; infinities and NaN in what a row does not
+    see do not reach it, in what it sees they do."""
+    for D, slots in ((128, 96), (64, 33), (80, 50)):
+        T, heads, kv = 6, 4, 2
+        g = torch.Generator().manual_seed(D)
+        r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+        q, k, v = r(T, heads, D).to(qt), r(slots, kv, D).to(ct), r(slots, kv, D).to(ct)
+        kn, vn = r(T, kv, D).to(ct), r(T, kv, D).to(ct)
+        pos = torch.arange(slots)
+        pos[::3] = -1                   # empty slots hold anything
+        k[::3], v[::3] = float("nan"), float("inf")
+        q_pos = torch.tensor([-5, 7, slots + 3, slots + 3, 7, slots + 4])
+        tree = torch.eye(T, dtype=torch.bool)
+        tree[0, 0] = False              # row 0 sees nothing at all
+        tree[5, 3] = True
+        v[8:11] = float("inf")          # hidden from rows 1 and 4
+        k[20, 1] = float("nan")
+        kn[4], vn[4] = float("nan"), float("nan")   # draft 4: seen by itself alone
+        to = lambda t: t.to(dev)        # noqa: E731
+        announce(f"hidden values D={D} {qt} over {ct}")
+        weight = torch.zeros(slots, device=dev)
+        o = tree_attention(to(q), to(k), to(v), to(pos), to(q_pos), to(kn), to(vn), to(tree), weight=weight).cpu()
+        assert bool((o[0] == 0).all())
+        see = _see(pos, q_pos, tree, None)
+        rows = [1]
+        clean = lambda t: torch.nan_to_num(t.float(), 0.0, 0.0, 0.0).to(t.dtype)  # noqa: E731
+        kk, vv = torch.cat([k, kn]), torch.cat([v, vn])
+        _compare(o[rows], None, None, q[rows], clean(kk), clean(vv), see[rows], D ** -0.5, slots)
+        assert bool(torch.isnan(o[4]).all())
+        assert bool(torch.isinf(o[2:4, :2]).all()) and bool(torch.isnan(o[2:4, 2:]).all())  # v inf; k NaN in head 1
+    # a cache that nobody sees, without drafts
+    o = tree_attention(torch.ones(2, 2, 64, device=dev).to(qt), torch.full((40, 1, 64), float("nan"), device=dev).to(ct),
+                       torch.full((40, 1, 64), float("nan"), device=dev).to(ct),
+                       torch.full((40,), -1, device=dev), torch.arange(2, device=dev))
+    assert bool((o == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", [(F32, F32), (F16, F16), (F32, BF16)], ids=["f32", "f16", "f32_bf16"])
+def test_attend_strides(dev, qt, ct):
+    """Head-major caches, sliced and misaligned rows, an out of its own strides."""
+    g = torch.Generator().manual_seed(3)
+    T, heads, kv, D, slots = 4, 8, 2, 64, 150
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    k, v, q = r(slots, kv, D).to(ct), r(slots, kv, D).to(ct), r(T, heads, D).to(qt)
+    kn, vn = r(T, kv, D).to(ct), r(T, kv, D).to(ct)
+    pos, q_pos = torch.arange(slots), slots + torch.arange(T)
+    tree = torch.ones(T, T, dtype=torch.bool).tril()
+    see = _see(pos, q_pos, tree, None)
+
+    def layouts(t):
+        yield t.to(dev)
+        yield t.transpose(0, 1).contiguous().to(dev).transpose(0, 1)             # [heads, n, dim]
+        pad = torch.zeros(t.shape[0], t.shape[1], D + 3, dtype=t.dtype)
+        pad[..., 1:1 + D] = t
+        yield pad.to(dev)[..., 1:1 + D]                                          # off 16 bytes
+        yield t.transpose(1, 2).contiguous().to(dev).transpose(1, 2)             # dim not innermost
+
+    for i, (kd, vd) in enumerate(zip(layouts(k), layouts(v))):
+        for qd, knd, vnd in zip(layouts(q), layouts(kn), layouts(vn)):
+            if i == 3:
+                with pytest.raises(ValueError, match="unit stride"):
+                    tree_attention(qd, kd, vd, pos.to(dev), q_pos.to(dev))
+                continue
+            out = torch.full((T, heads + 1, D + 2), 7.0, dtype=qt, device=dev)
+            announce(f"strides cache {i} q {qd.stride()}")
+            o = tree_attention(qd, kd, vd, pos.to(dev), q_pos.to(dev), knd, vnd, tree.to(dev).t().contiguous().t(),
+                               out=out[:, :heads, 1:1 + D])
+            _compare(o.cpu(), None, None, q, torch.cat([k, kn]), torch.cat([v, vn]), see, D ** -0.5, slots)
+            assert bool((out[:, heads] == 7).all()) and bool((out[..., 0] == 7).all()) and bool((out[..., -1] == 7).all())
+    # no tree: a chain
+    a = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), q_pos.to(dev), kn.to(dev), vn.to(dev))
+    b = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), q_pos.to(dev), kn.to(dev), vn.to(dev), tree.to(dev))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_attend_far_positions_and_long_cache(dev):
+    """Positions past 2^31, and a cache whose offsets pass 2^31 elements."""
+    buf, q, q_pos, o = _case(dev, 3, 4, 2, 64, 100, 90, None, F32, F32, True, False)
+    far = 5 << 31
+    pos = torch.where(buf.slot_pos >= 0, buf.slot_pos + far, -1)
+    g = torch.Generator().manual_seed(3 * 31 + 100)
+    # the same keys and drafts at far positions give the same result
+    k2 = tree_attention(q.to(dev), buf.k, buf.v, buf.slot_pos, q_pos.to(dev))
+    k3 = tree_attention(q.to(dev), buf.k, buf.v, pos, q_pos.to(dev) + far)
+    assert torch.equal(k2, k3)
+    slots, stride = 70, 1 << 25   # a view of few slots far apart: offsets up to 2^31 + 2^27 elements
+    big = torch.empty(slots * stride, dtype=F16, device=dev)
+    k, v = (big.as_strided((slots, 1, 128), (stride, 128, 1), at) for at in (0, 4096))
+    for t in (k, v):
+        t.copy_(torch.randn(slots, 1, 128, generator=g).to(F16))
+    q = torch.randn(2, 2, 128, generator=g).to(F16)
+    announce("attend, offsets past 2^31")
+    o = tree_attention(q.to(dev), k, v, torch.arange(slots, device=dev), torch.tensor([slots - 1, 30], device=dev))
+    _compare(o.cpu(), None, None, q, k.cpu(), v.cpu(), _see(torch.arange(slots), torch.tensor([slots - 1, 30]), None, None),
+             128 ** -0.5, slots)
+
+
+@pytest.mark.gpu
+def test_attend_refuses(dev):
+    k = torch.zeros(8, 2, 64, device=dev)
+    ok = dict(q=torch.zeros(2, 4, 64, device=dev), k=k, v=k, slot_pos=torch.arange(8, device=dev),
+              q_pos=torch.arange(2, device=dev))
+    kn = torch.zeros(2, 2, 64, device=dev)
+    for bad in (dict(q=torch.zeros(2, 5, 64, device=dev)), dict(q=torch.zeros(2, 4, 32, device=dev)),
+                dict(q=ok["q"].half()), dict(k=k.half()), dict(v=k.cpu()), dict(v=k.transpose(0, 1).contiguous().transpose(0, 1)),
+                dict(slot_pos=ok["slot_pos"].int()), dict(slot_pos=ok["slot_pos"][:7]), dict(q_pos=ok["q_pos"][:1]),
+                dict(q_pos=ok["q_pos"].cpu()), dict(window=0), dict(k_new=kn), dict(tree=torch.ones(2, 2, device=dev).bool()),
+                dict(k_new=kn, v_new=kn.half()), dict(k_new=kn[:1], v_new=kn[:1]),
+                dict(k_new=kn, v_new=kn, tree=torch.ones(2, 3, device=dev).bool()),
+                dict(k_new=kn, v_new=kn, tree=torch.ones(2, 2, device=dev)), dict(weight=torch.zeros(7, device=dev)),
+                dict(weight=torch.zeros(8, device=dev).double()), dict(out=torch.zeros(2, 4, 64, device=dev).half()),
+                dict(workspace=torch.zeros(8, device=dev)), dict(q=torch.zeros(1025, 4, 64, device=dev),
+                                                                 q_pos=torch.zeros(1025, dtype=torch.long, device=dev)),
+                dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            tree_attention(**{**ok, **bad})
+    empty = tree_attention(ok["q"][:0], k, k, ok["slot_pos"], ok["q_pos"][:0])
+    assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
+def test_attend_streams_and_graph(dev):
+    """Repeatable; on another stream; captured and replayed with new inputs."""
+    g = torch.Generator().manual_seed(4)
+    slots, kv, D, T, heads = 2000, 2, 128, 7, 8
+    buf = DeviceKVBuffer(kv, D, slots, device=dev, dtype=BF16)
+    buf.append(torch.randn(1500, kv, D, generator=g).to(dev), torch.randn(1500, kv, D, generator=g).to(dev))
+    tree, depth = _tree(T, g)
+    tree, q_pos = tree.to(dev), (1500 + depth).to(dev)
+    q = torch.zeros(T, heads, D, dtype=BF16, device=dev)
+    kn, vn = torch.zeros(T, kv, D, dtype=BF16, device=dev), torch.zeros(T, kv, D, dtype=BF16, device=dev)
+    weight = torch.zeros(slots, device=dev)
+
+    def step():
+        return buf.attend(q, q_pos, kn, vn, tree, weight=weight)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step()
+    for seed in range(4):
+        for t in (q, kn, vn):
+            t.copy_(torch.randn(t.shape, generator=g).to(dev))
+        weight.zero_()
+        graph.replay()
+        w = weight.clone()
+        got = o.clone()
+        weight.zero_()
+        assert torch.equal(step(), got) and torch.equal(weight, w)
+        torch.cuda.synchronize()
+        assert float(w.sum()) > 0
