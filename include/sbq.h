@@ -506,6 +506,43 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
                        void* out, int64_t o_st, int64_t o_sh, float* weight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* ---- a bounded cache, evicted by attention weight ------------------------ */
+
+/* A cache of `slots` slots that holds more positions than it has room for: it
+ * gives up the slots that received the least attention weight (weight [slots],
+ * the running sums sbq_tree_attention adds to).  Slots are given up in this
+ * order, equal ones by their index: free slots (slot_pos < 0); then by
+ * weight, the least first (NaN last); last the slots of the `recent` newest
+ * positions.  No counterpart in the reference.
+ *
+ * sbq_kv_append: T new tokens, at positions *start .. *start + T - 1, take the
+ * first T slots of that order, in ascending slot order (the newest positions
+ * are those >= *start + T - recent): their keys and values (k_new, v_new:
+ * device [T, kv_heads, D], strides n_ss and n_sh, F32, F16 or BF16) are
+ * rounded to the cache's type and written to k, v (device [slots, kv_heads,
+ * D], strides k_ss and k_sh), slot_pos is set, weight is 0, and *end = *start
+ * + T.  start, end: device int64[1], the same one or not.  0 <= recent <=
+ * slots, T <= slots.
+ *
+ * sbq_kv_take: the used slots among the last `capacity` of that order (newest:
+ * >= *end - recent) of a cache of any size are copied, in slot order, to the
+ * first slots of another (strides t_ss and t_sh) with their positions and
+ * weights; its other slots become free (slot_pos -1, weight 0; k and v left
+ * as they were), *to_end = *end.  The two must not overlap.
+ *
+ * workspace: >= sbq_kv_workspace_bytes(T or capacity), any content. */
+int64_t sbq_kv_workspace_bytes(int64_t count);
+int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end, const int64_t* start,
+                  int64_t recent, void* k, void* v, int kv_dtype, int64_t kv_heads, int64_t D,
+                  int64_t k_ss, int64_t k_sh, const void* k_new, const void* v_new, int new_dtype,
+                  int64_t T, int64_t n_ss, int64_t n_sh, void* workspace, size_t workspace_bytes,
+                  void* stream);
+int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, const int64_t* end,
+                const void* k, const void* v, int kv_dtype, int64_t kv_heads, int64_t D, int64_t k_ss,
+                int64_t k_sh, int64_t capacity, int64_t recent, int64_t* to_pos, float* to_weight,
+                int64_t* to_end, void* to_k, void* to_v, int64_t t_ss, int64_t t_sh, void* workspace,
+                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

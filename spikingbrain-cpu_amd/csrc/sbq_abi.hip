@@ -712,4 +712,57 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
   return sbq::launch_tree_attention(c, (hipStream_t)stream);
 }
 
+// ---- a bounded cache, evicted by attention weight ----
+
+static bool kv_sizes_ok(int64_t slots, int64_t kv_heads, int64_t D) {
+  return slots >= 1 && slots <= (1 << 30) && kv_heads >= 1 && D >= 1 && kv_heads <= 65536 && D <= 65536 &&
+         kv_heads * D <= (1 << 24);
+}
+
+int64_t sbq_kv_workspace_bytes(int64_t count) { return count < 1 || count > (1 << 30) ? 0 : (count + 1) * 4 + 16; }
+
+int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end, const int64_t* start, int64_t recent,
+                  void* k, void* v, int kv_dtype, int64_t kv_heads, int64_t D, int64_t k_ss, int64_t k_sh,
+                  const void* k_new, const void* v_new, int new_dtype, int64_t T, int64_t n_ss, int64_t n_sh,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(kv_dtype) || !valid_dtype(new_dtype)) return SBQ_ERR_DTYPE;
+  if (!kv_sizes_ok(slots, kv_heads, D) || recent < 0 || recent > slots || T < 0 || T > slots) return SBQ_ERR_ARG;
+  if (k_ss < 0 || k_sh < 0 || n_ss < 0 || n_sh < 0) return SBQ_ERR_ARG;
+  if (T == 0) return SBQ_OK;
+  if (!slot_pos || !weight || !end || !start || !k || !v || !k_new || !v_new) return SBQ_ERR_ARG;
+  const int64_t es = esize(kv_dtype), en = esize(new_dtype);
+  if (!aligned(slot_pos, 8) || !aligned(weight, 4) || !aligned(end, 8) || !aligned(start, 8) || !aligned(k, es) ||
+      !aligned(v, es) || !aligned(k_new, en) || !aligned(v_new, en))
+    return SBQ_ERR_ALIGN;
+  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(T)) return SBQ_ERR_WORKSPACE;
+  sbq::KvAppend c{};
+  c.slot_pos = slot_pos, c.weight = weight, c.end = end, c.start = start, c.k = k, c.v = v, c.kn = k_new, c.vn = v_new;
+  c.ws = (void*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
+  c.slots = slots, c.T = T, c.recent = recent, c.Hk = kv_heads, c.D = D, c.k_ss = k_ss, c.k_sh = k_sh, c.n_ss = n_ss,
+  c.n_sh = n_sh, c.ct = kv_dtype, c.nt = new_dtype;
+  return sbq::launch_kv_append(c, (hipStream_t)stream);
+}
+
+int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, const int64_t* end, const void* k,
+                const void* v, int kv_dtype, int64_t kv_heads, int64_t D, int64_t k_ss, int64_t k_sh, int64_t capacity,
+                int64_t recent, int64_t* to_pos, float* to_weight, int64_t* to_end, void* to_k, void* to_v, int64_t t_ss,
+                int64_t t_sh, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(kv_dtype)) return SBQ_ERR_DTYPE;
+  if (!kv_sizes_ok(slots, kv_heads, D) || capacity < 1 || capacity > (1 << 30) || recent < 0 || recent > capacity)
+    return SBQ_ERR_ARG;
+  if (k_ss < 0 || k_sh < 0 || t_ss < 0 || t_sh < 0) return SBQ_ERR_ARG;
+  if (!slot_pos || !weight || !end || !k || !v || !to_pos || !to_weight || !to_end || !to_k || !to_v) return SBQ_ERR_ARG;
+  const int64_t es = esize(kv_dtype);
+  if (!aligned(slot_pos, 8) || !aligned(weight, 4) || !aligned(end, 8) || !aligned(to_pos, 8) || !aligned(to_weight, 4) ||
+      !aligned(to_end, 8) || !aligned(k, es) || !aligned(v, es) || !aligned(to_k, es) || !aligned(to_v, es))
+    return SBQ_ERR_ALIGN;
+  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(capacity)) return SBQ_ERR_WORKSPACE;
+  sbq::KvTake c{};
+  c.slot_pos = slot_pos, c.end = end, c.weight = weight, c.k = k, c.v = v, c.to_pos = to_pos, c.to_end = to_end;
+  c.to_weight = to_weight, c.to_k = to_k, c.to_v = to_v, c.ws = (void*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
+  c.slots = slots, c.capacity = capacity, c.recent = recent, c.Hk = kv_heads, c.D = D, c.k_ss = k_ss, c.k_sh = k_sh;
+  c.t_ss = t_ss, c.t_sh = t_sh, c.ct = kv_dtype;
+  return sbq::launch_kv_take(c, (hipStream_t)stream);
+}
+
 }  // extern "C"

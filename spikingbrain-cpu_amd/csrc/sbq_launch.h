@@ -249,4 +249,31 @@ struct AttnCall {
 int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t slots, bool weight);
 int launch_tree_attention(const AttnCall& c, hipStream_t st);
 
+// A bounded cache that gives up its least attended slots (sbq_evict.hip); ws:
+// int32 [T] / [capacity + 1].
+struct KvAppend {
+  int64_t* slot_pos;
+  float* weight;
+  int64_t* end;
+  const int64_t* start;
+  void *k, *v;
+  const void *kn, *vn;
+  void* ws;
+  int64_t slots, T, recent, Hk, D, k_ss, k_sh, n_ss, n_sh;
+  int ct, nt;
+};
+int launch_kv_append(const KvAppend& c, hipStream_t st);
+struct KvTake {
+  const int64_t *slot_pos, *end;
+  const float* weight;
+  const void *k, *v;
+  int64_t *to_pos, *to_end;
+  float* to_weight;
+  void *to_k, *to_v;
+  void* ws;
+  int64_t slots, capacity, recent, Hk, D, k_ss, k_sh, t_ss, t_sh;
+  int ct;
+};
+int launch_kv_take(const KvTake& c, hipStream_t st);
+
 }  // namespace sbq

@@ -218,6 +218,108 @@ class DeviceKVBuffer:
         self.end.copy_(torch.minimum(self.end, n))
 
 
+class DeviceBudgetKVBuffer(DeviceKVBuffer):
+    """A full-attention buffer of `capacity` slots for more positions than
+    that: once it is full, an append takes the slots which received the least
+    attention weight so far, the `recent` newest positions (the appended ones
+    among them) last.  `weight` [capacity] holds the running sums, which
+    attend adds to; a new token starts at 0.  No counterpart in the reference,
+    whose softmax layers keep every position.
+
+    GPU only (attend and append are kernels of libsbq.so).  Every tensor keeps
+    its address, so append and attend can be captured in a HIP graph."""
+
+    def __init__(self, heads: int, dim: int, capacity: int, recent: int = 0, device: torch.device | str | None = None,
+                 dtype: torch.dtype = torch.float32):
+        if not 0 <= recent <= capacity:
+            raise ValueError("DeviceBudgetKVBuffer: recent must be between 0 and capacity")
+        super().__init__(heads, dim, capacity, None, device, dtype)
+        self.recent = recent
+        self.weight = torch.zeros(capacity, dtype=torch.float32, device=self.k.device)
+
+    def reset(self) -> None:
+        super().reset()
+        self.weight.zero_()
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, start=None):
+        """Store k, v [T, heads, dim] at positions start .. start + T - 1
+        (default: after the last append), T <= capacity; start may be an int
+        or a device tensor.  Free slots are taken first, then those of least
+        weight (equal ones by slot), in ascending slot order."""
+        kv = self.k
+        gpu = kv.get_device()
+        if k.shape != v.shape or k.dim() != 3 or k.shape[1] != self.heads or k.shape[2] != self.dim:
+            raise ValueError(f"DeviceBudgetKVBuffer.append: expected [T, {self.heads}, {self.dim}] keys and values")
+        T = k.shape[0]
+        if T > self.capacity:
+            raise ValueError("DeviceBudgetKVBuffer.append: more tokens than slots")
+        if not kv.is_cuda or k.get_device() != gpu or v.get_device() != gpu:
+            raise ValueError("DeviceBudgetKVBuffer.append: the buffer, k and v must be on one GPU")
+        if T == 0:
+            if start is not None:
+                self.end.copy_(_as_pos(start, kv.device))
+            return kv, self.v, self.slot_pos
+        if k.dtype not in _DTYPE_CODE or v.dtype != k.dtype:
+            k, v = k.to(kv.dtype), v.to(kv.dtype)
+        k, v = _rows_of(k), _rows_of(v)
+        if k.stride() != v.stride():
+            k, v = k.contiguous(), v.contiguous()
+        s = self.end if start is None else _as_pos(start, kv.device)
+        L = _lib.load()
+        ws = torch.empty((4 * T + 20,), dtype=torch.uint8, device=kv.device)  # sbq_kv_workspace_bytes(T)
+        ks, ns = kv.stride(), k.stride()
+        with _on_device(kv.device):
+            _lib.check(L.sbq_kv_append(
+                self.slot_pos.data_ptr(), self.weight.data_ptr(), self.capacity, self.end.data_ptr(), s.data_ptr(),
+                self.recent, kv.data_ptr(), self.v.data_ptr(), _DTYPE_CODE[kv.dtype], self.heads, self.dim, ks[0], ks[1],
+                k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], T, ns[0], ns[1], ws.data_ptr(), ws.numel(),
+                _stream(kv.device)), "sbq_kv_append")
+        return kv, self.v, self.slot_pos
+
+    def take(self, source: DeviceKVBuffer, weight: torch.Tensor | None = None):
+        """Become what is worth keeping of `source` (after a long prompt): its
+        slots in the order of append's rule, the last `capacity` of them kept
+        in slot order with their positions and weights.  weight: fp32, one per
+        slot of source (default: source.weight); end becomes source.end."""
+        kv = self.k
+        if weight is None:
+            weight = getattr(source, "weight", None)
+        if source is self or not kv.is_cuda or source.k.device != kv.device:
+            raise ValueError("DeviceBudgetKVBuffer.take: source must be another buffer on this buffer's GPU")
+        if source.k.shape[1:] != kv.shape[1:] or source.k.dtype != kv.dtype:
+            raise ValueError("DeviceBudgetKVBuffer.take: source must have this buffer's heads, dim and dtype")
+        if (weight is None or weight.dtype != torch.float32 or weight.device != kv.device
+                or weight.shape != (source.capacity,) or not weight.is_contiguous()):
+            raise ValueError(f"DeviceBudgetKVBuffer.take: weight must be a contiguous float32 [{source.capacity}] tensor on "
+                             f"{kv.device}")
+        L = _lib.load()
+        ws = torch.empty((4 * self.capacity + 20,), dtype=torch.uint8, device=kv.device)
+        ks, ts = source.k.stride(), kv.stride()
+        with _on_device(kv.device):
+            _lib.check(L.sbq_kv_take(
+                source.slot_pos.data_ptr(), weight.data_ptr(), source.capacity, source.end.data_ptr(), source.k.data_ptr(),
+                source.v.data_ptr(), _DTYPE_CODE[kv.dtype], self.heads, self.dim, ks[0], ks[1], self.capacity, self.recent,
+                self.slot_pos.data_ptr(), self.weight.data_ptr(), self.end.data_ptr(), kv.data_ptr(), self.v.data_ptr(),
+                ts[0], ts[1], ws.data_ptr(), ws.numel(), _stream(kv.device)), "sbq_kv_take")
+        return kv, self.v, self.slot_pos
+
+    def attend(self, q: torch.Tensor, q_pos: torch.Tensor, k_new: torch.Tensor | None = None,
+               v_new: torch.Tensor | None = None, tree: torch.Tensor | None = None, scale: float | None = None,
+               weight: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None, count: bool = True) -> torch.Tensor:
+        """DeviceKVBuffer.attend, which also adds the attention weight that
+        every slot received to `weight` (this buffer's own by default; count
+        False: nowhere).  All T query rows count, drafts that are rejected
+        later among them."""
+        if weight is None and count:
+            weight = self.weight
+        return super().attend(q, q_pos, k_new, v_new, tree, scale, weight, out, workspace)
+
+    def truncate(self, length) -> None:
+        super().truncate(length)
+        self.weight.masked_fill_(self.slot_pos < 0, 0.0)
+
+
 @dataclass
 class DeviceLayerState:
     """model.py:94-97 LayerState: the layer's key / value buffer and, for a
@@ -266,13 +368,15 @@ class DeviceInferenceState:
 
 def new_device_state(hybrid: list[bool], heads: int, head_dim: int, kv_heads: int, partitions: int,
                      window: int, capacity: int, device: torch.device | str | None = None,
-                     ring_extra: int = 1) -> DeviceInferenceState:
+                     ring_extra: int = 1, budget: int | None = None, recent: int = 0) -> DeviceInferenceState:
     """model.py:412-424 new_state on the device: per layer a key / value
     buffer (windowed, a ring of window + ring_extra slots, for hybrid layers;
     `capacity` positions for softmax layers) and, for hybrid layers, zeroed
     shared [heads, head_dim, head_dim] and partition [partitions, heads,
     head_dim, head_dim] fp32 states.  ring_extra is the most tokens one call
-    appends (1 for decode; the prefill chunk otherwise)."""
+    appends (1 for decode; the prefill chunk otherwise).  budget: slots of a
+    softmax layer's buffer when it is to be smaller than `capacity` positions
+    (DeviceBudgetKVBuffer, the `recent` newest positions kept)."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     layers = []
     for is_hybrid in hybrid:
@@ -281,6 +385,8 @@ def new_device_state(hybrid: list[bool], heads: int, head_dim: int, kv_heads: in
                 kv=DeviceKVBuffer(kv_heads, head_dim, window + ring_extra, window, dev),
                 shared=torch.zeros(heads, head_dim, head_dim, device=dev),
                 partitions=torch.zeros(partitions, heads, head_dim, head_dim, device=dev)))
+        elif budget is not None and budget < capacity:
+            layers.append(DeviceLayerState(kv=DeviceBudgetKVBuffer(kv_heads, head_dim, budget, recent, dev)))
         else:
             layers.append(DeviceLayerState(kv=DeviceKVBuffer(kv_heads, head_dim, capacity, None, dev)))
     return DeviceInferenceState(layers=layers, position=torch.zeros((1,), dtype=torch.long, device=dev),
