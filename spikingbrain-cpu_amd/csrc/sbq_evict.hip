@@ -4,13 +4,16 @@
 // Slots are ordered by one 32-bit key: free ones 0, then the running sum of
 // attention weight as an ordered integer, the `recent` newest positions
 // highest; equal keys by slot.  One workgroup finds the m-th smallest key
-// digit by digit (11, 11 and 10 bits, a histogram in LDS each; only keys that
-// share the digits so far count) and then lists the slots on one side of it in
-// slot order.  What bounds it is that workgroup's reading of 12 bytes per
-// slot and its steps' latency: a second level over several workgroups would
-// cost another launch, more than the reading up to some 32768 slots, which
-// the 1024 threads hold in registers.  Integer counts only, so the result
-// does not depend on timing.
+// digit by digit (11, 11 and 10 bits, a histogram each; only keys that share
+// the digits so far count) and lists the slots on one side of it in slot
+// order.  The keys stay in LDS (up to 32768 slots; more are read again for
+// every pass), each thread's own ones side by side, so that one scan over the
+// threads gives every place in the list.  A single new token needs no more
+// than the smallest key and its slot.  What bounds it is that workgroup's
+// reading of 12 bytes per slot and the latency of its steps; a first level
+// over several workgroups would cost another launch, which is more than the
+// reading up to some 32768 slots.  Integer counts only, so the result does
+// not depend on timing.
 #include "sbq_common.h"
 #include "sbq_launch.h"
 
@@ -59,32 +62,45 @@ struct Select {
   int64_t keep_from;
 };
 
-// Keys of the threads' slots in segment `seg`: slot = seg * NK * 1024 + i *
-// 1024 + thread; slots past the end get no key (bit i of `in` clear).
-template <int NK>
-__device__ __forceinline__ uint32_t load_keys(const Select& q, int64_t seg, uint32_t (&key)[NK]) {
-  uint32_t in = 0;
+// A thread's keys of a segment of per * 1024 slots lie side by side in LDS,
+// 4 words of padding after every 32 (a thread's 16-byte reads would all meet
+// in the same banks).
+constexpr int kSegKeys = 32;  // per thread at most
+__device__ __forceinline__ int key_at(int s) { return s + (s >> 5) * 4; }
+constexpr int key_words(int per) { return per * kSelThreads / 32 * 36; }
+int keys_per_thread(int64_t n) {
+  const int64_t k = (n + kSelThreads - 1) / kSelThreads;
+  return k > kSegKeys ? kSegKeys : (int)((k + 3) / 4 * 4);
+}
+
+// Keys of segment `seg` into LDS (slots past the end: key 0, never looked at).
+__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per, uint32_t* keys) {
+  const int64_t s0 = seg * per * kSelThreads;
+#pragma unroll 1
+  for (int i = 0; i < per; i += 4) {
+    int64_t pos[4];
+    float w[4];
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const int64_t s = (seg * NK + i) * kSelThreads + threadIdx.x;
-    key[i] = 0;
-    if (s < q.n) {
-      key[i] = evict_key(q.slot_pos[s], q.weight[s], q.keep_from);
-      in |= 1u << i;
+    for (int j = 0; j < 4; ++j) {
+      const int64_t s = s0 + (i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
+      pos[j] = q.slot_pos[at];
+      w[j] = q.weight[at];
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) keys[key_at((i + j) * kSelThreads + threadIdx.x)] = evict_key(pos[j], w[j], q.keep_from);
   }
-  return in;
 }
 
 // The slots with the m smallest keys (side 0) or the used ones among the
 // others (side 1), listed in slot order; returns how many (0 <= m <= n).
-template <int NK>
 __device__ __forceinline__ int select_slots(const Select& q, int m, int side, int32_t* list) {
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ uint32_t hist[kBins], scan[kSelWaves], found[2];
-  __shared__ uint32_t counts[2][NK * kSelWaves];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t segs = ((int64_t)q.n + NK * kSelThreads - 1) / (NK * kSelThreads);
-  uint32_t key[NK], in = load_keys<NK>(q, 0, key);
+  const int lane = threadIdx.x & 63;
+  const int64_t want = ((int64_t)q.n + kSelThreads - 1) / kSelThreads;
+  const int per = want > kSegKeys ? kSegKeys : (int)((want + 3) / 4 * 4);
+  const int64_t segs = (want + per - 1) / per;
+  load_keys(q, 0, per, keys);
 
   // the m-th smallest key `kth`, of which `ties` (lowest slots first) belong to the m
   uint32_t kth = 0, ties = m;
@@ -94,22 +110,30 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       const uint32_t above = pass == 0 ? 0u : ~0u << (shift + bits);
       for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
 #pragma unroll 1
       for (int64_t seg = 0; seg < segs; ++seg) {
-        if (segs > 1) in = load_keys<NK>(q, seg, key);
+        if (segs > 1) {
+          __syncthreads();  // (everyone is done with the keys before)
+          load_keys(q, seg, per, keys);
+        }
+        __syncthreads();
+        const int64_t s0 = (seg * kSelThreads + threadIdx.x) * per;
+#pragma unroll 1
+        for (int i = 0; i < per; i += 4) {
+          const u32x4 k4 = *(const u32x4*)(keys + key_at(threadIdx.x * per + i));
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const bool on = (in >> i & 1) && ((key[i] ^ kth) & above) == 0;
-          const unsigned long long who = __ballot(on);
-          if (!who) continue;
-          const uint32_t digit = key[i] >> shift & ((1u << bits) - 1);
-          // (a wave whose keys share the digit, as equal weights do, counts once)
-          const uint32_t first = __builtin_amdgcn_readlane(digit, __ffsll(who) - 1);
-          if (__ballot(on && digit == first) == who) {
-            if (lane == __ffsll(who) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(who));
-          } else if (on) {
-            atomicAdd(&hist[digit], 1u);
+          for (int j = 0; j < 4; ++j) {
+            const bool on = s0 + i + j < q.n && ((k4[j] ^ kth) & above) == 0;
+            const unsigned long long who = __ballot(on);
+            if (!who) continue;
+            const uint32_t digit = k4[j] >> shift & ((1u << bits) - 1);
+            // (a wave whose keys share the digit, as equal weights do, counts once)
+            const uint32_t first = __builtin_amdgcn_readlane(digit, __ffsll(who) - 1);
+            if (__ballot(on && digit == first) == who) {
+              if (lane == __ffsll(who) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(who));
+            } else if (on) {
+              atomicAdd(&hist[digit], 1u);
+            }
           }
         }
       }
@@ -122,49 +146,86 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
       __syncthreads();
       kth |= found[0] << shift;
       ties -= found[1];
-      __syncthreads();
     }
   }
 
-  uint32_t seen = 0, listed = 0;  // keys equal to kth, slots listed before this segment
+  // Of the keys equal to kth the first `ties` are among the m; free slots
+  // (key 0) are never among the used ones.  Before a thread's own slots lie
+  // `out` listed ones off kth and `eq` equal ones.
+  uint32_t out = 0, eq = 0;
 #pragma unroll 1
   for (int64_t seg = 0; seg < segs; ++seg) {
-    if (segs > 1) in = load_keys<NK>(q, seg, key);
-    unsigned long long eq[NK];
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      eq[i] = __ballot((in >> i & 1) && key[i] == kth);
-      if (lane == 0) counts[0][i * kSelWaves + w] = __popcll(eq[i]);
+    __syncthreads();
+    if (segs > 1) {
+      load_keys(q, seg, per, keys);
+      __syncthreads();
     }
-    __syncthreads();
-    constexpr int NC = NK * kSelWaves;  // <= kSelThreads
-    uint32_t total, mine = threadIdx.x < NC ? counts[0][threadIdx.x] : 0u;
-    uint32_t before = block_scan(mine, scan, &total);
-    if (threadIdx.x < NC) counts[0][threadIdx.x] = seen + before;
-    seen += total;
-    __syncthreads();
-    unsigned long long take[NK];
+    const int64_t s0 = (seg * kSelThreads + threadIdx.x) * per;
+    uint32_t my_out = 0, my_eq = 0;
+#pragma unroll 1
+    for (int i = 0; i < per; i += 4) {
+      const u32x4 k4 = *(const u32x4*)(keys + key_at(threadIdx.x * per + i));
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const uint32_t rank = counts[0][i * kSelWaves + w] + __popcll(eq[i] & ((1ull << lane) - 1));
-      const bool low = m > 0 && (key[i] < kth || (key[i] == kth && rank < ties));
-      take[i] = __ballot((in >> i & 1) && (side == 0 ? low : !low && key[i] != 0));
-      if (lane == 0) counts[1][i * kSelWaves + w] = __popcll(take[i]);
+      for (int j = 0; j < 4; ++j) {
+        const bool in = s0 + i + j < q.n;
+        my_out += in && (side == 0 ? k4[j] < kth : k4[j] > kth);
+        my_eq += in && k4[j] == kth;
+      }
     }
-    __syncthreads();
-    mine = threadIdx.x < NC ? counts[1][threadIdx.x] : 0u;
-    before = block_scan(mine, scan, &total);
-    if (threadIdx.x < NC) counts[1][threadIdx.x] = listed + before;
-    listed += total;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NK; ++i)
-      if (take[i] >> lane & 1)
-        list[counts[1][i * kSelWaves + w] + __popcll(take[i] & ((1ull << lane) - 1))] =
-            (int32_t)((seg * NK + i) * kSelThreads + threadIdx.x);
-    __syncthreads();  // (the list is written, counts are free)
+    uint32_t all_out, all_eq;
+    const uint32_t out0 = out + block_scan(my_out, scan, &all_out), eq0 = eq + block_scan(my_eq, scan, &all_eq);
+    uint32_t o = out0, e = eq0;
+    if (my_out + my_eq > 0) {
+#pragma unroll 1
+      for (int i = 0; i < per; ++i) {
+        const uint32_t k = keys[key_at(threadIdx.x * per + i)];
+        if (s0 + i >= q.n) break;
+        const uint32_t low_eq = min(e, ties), high_eq = kth == 0 ? 0u : e - low_eq;  // equal ones before, on each side
+        const bool low = k < kth || (k == kth && e < ties), high = k > kth || (k == kth && e >= ties && kth != 0);
+        if (side == 0 ? low : high) list[o + (side == 0 ? low_eq : high_eq)] = (int32_t)(s0 + i);
+        o += side == 0 ? k < kth : k > kth;
+        e += k == kth;
+      }
+    }
+    out += all_out;
+    eq += all_eq;
   }
-  return (int)listed;
+  const uint32_t low_eq = min(eq, ties);
+  return (int)(out + (side == 0 ? low_eq : kth == 0 ? 0u : eq - low_eq));
+}
+
+// The slot of the smallest key (the lowest of equal ones).
+__device__ __forceinline__ int first_slot(const Select& q) {
+  __shared__ unsigned long long best[kSelWaves];
+  unsigned long long v = ~0ull;
+#pragma unroll 1
+  for (int64_t s0 = threadIdx.x; s0 < q.n; s0 += 4 * kSelThreads) {
+    int64_t pos[4];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t s = s0 + j * kSelThreads, at = s < q.n ? s : s0;
+      pos[j] = q.slot_pos[at];
+      w[j] = q.weight[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t s = s0 + j * kSelThreads;
+      const unsigned long long k = (unsigned long long)evict_key(pos[j], w[j], q.keep_from) << 32 | (uint32_t)s;
+      if (s < q.n && k < v) v = k;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned long long t = __shfl_xor(v, o, 64);
+    v = t < v ? t : v;
+  }
+  if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = best[0];
+#pragma unroll
+  for (int k = 1; k < kSelWaves; ++k) v = best[k] < v ? best[k] : v;
+  return (int)(uint32_t)v;
 }
 
 // n elements of a row from type ST to type DT; equal types copy bits.
@@ -219,11 +280,26 @@ struct AppendArgs {
   bool rows_too;
 };
 
-template <int NK, int ST, int DT>
+// A single token, then several.
+template <int ST, int DT>
+__global__ __launch_bounds__(kSelThreads) void kv_append_one_kernel(AppendArgs a) {
+  const int64_t start = *a.start;
+  const Select q{a.slot_pos, a.weight, a.n, start + 1 - a.recent};
+  const int s = first_slot(q);  // (every thread has read its slots and *start)
+  if (threadIdx.x == 0) {
+    a.slot_pos[s] = start;
+    a.weight[s] = 0.0f;
+    *a.end = start + 1;
+  }
+  copy_row<ST, DT>(a.fresh, 0, a.cache, s, a.D, threadIdx.x, a.Hk * a.D, kSelThreads);
+}
+
+template <int ST, int DT>
 __global__ __launch_bounds__(kSelThreads) void kv_append_kernel(AppendArgs a) {
   const int64_t start = *a.start;
   const Select q{a.slot_pos, a.weight, a.n, start + a.T - a.recent};
-  select_slots<NK>(q, a.T, 0, a.list);
+  select_slots(q, a.T, 0, a.list);
+  __syncthreads();  // the list is written
   for (int i = threadIdx.x; i < a.T; i += kSelThreads) {
     const int s = a.list[i];
     a.slot_pos[s] = start + i;
@@ -254,11 +330,10 @@ struct TakeArgs {
   bool vec;
 };
 
-template <int NK>
 __global__ __launch_bounds__(kSelThreads) void kv_take_kernel(TakeArgs a) {
   const int64_t end = *a.end;
   const Select q{a.slot_pos, a.weight, a.n, end - a.recent};
-  const int kept = select_slots<NK>(q, a.n > a.capacity ? a.n - a.capacity : 0, 1, a.list);
+  const int kept = select_slots(q, a.n > a.capacity ? a.n - a.capacity : 0, 1, a.list);
   if (threadIdx.x == 0) {
     a.list[a.capacity] = kept;
     *a.to_end = end;
@@ -293,12 +368,11 @@ constexpr int kInlineElems = 1 << 15;  // key elements that the selecting workgr
 
 template <int ST, int DT>
 int append_types(const AppendArgs& a, hipStream_t st) {
-  if (a.n <= 4 * kSelThreads)
-    kv_append_kernel<4, ST, DT><<<1, kSelThreads, 0, st>>>(a);
-  else if (a.n <= 16 * kSelThreads)
-    kv_append_kernel<16, ST, DT><<<1, kSelThreads, 0, st>>>(a);
-  else
-    kv_append_kernel<32, ST, DT><<<1, kSelThreads, 0, st>>>(a);
+  if (a.T == 1) {
+    kv_append_one_kernel<ST, DT><<<1, kSelThreads, 0, st>>>(a);
+    return check_launch();
+  }
+  kv_append_kernel<ST, DT><<<1, kSelThreads, key_words(keys_per_thread(a.n)) * 4, st>>>(a);
   int rc = check_launch();
   if (rc || a.rows_too) return rc;
   kv_rows_kernel<ST, DT><<<a.T, 256, 0, st>>>(a);
@@ -329,12 +403,7 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
   TakeArgs a{c.slot_pos, c.end, c.weight, c.to_pos, c.to_end, c.to_weight,
              Rows{const_cast<void*>(c.k), const_cast<void*>(c.v), c.k_ss, c.k_sh}, Rows{c.to_k, c.to_v, c.t_ss, c.t_sh},
              (int32_t*)c.ws, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
-  if (a.n <= 4 * kSelThreads)
-    kv_take_kernel<4><<<1, kSelThreads, 0, st>>>(a);
-  else if (a.n <= 16 * kSelThreads)
-    kv_take_kernel<16><<<1, kSelThreads, 0, st>>>(a);
-  else
-    kv_take_kernel<32><<<1, kSelThreads, 0, st>>>(a);
+  kv_take_kernel<<<1, kSelThreads, key_words(keys_per_thread(a.n)) * 4, st>>>(a);
   const int rc = check_launch();
   if (rc) return rc;
   kv_take_rows_kernel<<<a.capacity, 256, 0, st>>>(a);
