@@ -48,7 +48,8 @@ struct AttnArgs {
   int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld, spad;
   int64_t window;               // 0: none
   int T, Hk, rep, D, slots, Tn, splits, rtiles, qt;
-  float scale;                  // times log2(e)
+  float scale;                  // times log2(e), >= 0 (`neg`: q is negated instead)
+  bool neg, qvec;               // qvec: q's rows take 16-byte loads
 };
 
 template <int CT>
@@ -109,7 +110,7 @@ __device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
 
 template <int CT, bool M16, int DP, int MODE, int RT>
-__global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT == 2 ? 2 : 3) void attn_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
   typedef AttnMath<CT> Math;
   constexpr int E = CElem<CT>::E, NCH = DP / (4 * E);
@@ -124,25 +125,23 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
   const int kvh = blockIdx.x % a.Hk, rtile = blockIdx.x / a.Hk % a.rtiles, split = blockIdx.x / a.Hk / a.rtiles;
   const int R = a.rep * a.T, row0 = rtile * (16 * RT);
 
+  const int nbc = (a.slots + SB - 1) / SB, nb = nbc + (a.Tn + SB - 1) / SB, W = a.splits * kAttnWaves;
+  // position of the lane's slot (lane % SB) of block b; -1 past the cache
+  auto position = [&](int b) -> int64_t {
+    const int s = b * SB + (lane & (SB - 1));
+    return s < a.slots ? a.slot_pos[s] : -1;
+  };
+  int b = split * kAttnWaves + w;
+  int64_t sp = position(b);
+
   // the lane's rows and what they see: positions lo..hi
   int row[RT], tok[RT];
   int64_t lo[RT], hi[RT];
-  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     row[i] = row0 + i * 16 + c;
     tok[i] = min(row[i], R - 1) / a.rep;
     hi[i] = a.q_pos[tok[i]];
-    lo[i] = a.window > 0 && hi[i] - a.window + 1 > 0 ? hi[i] - a.window + 1 : 0;
-    // (a row past the last one is the last one again)
-    lo_min = min(lo_min, lo[i]), lo_max = max(lo_max, lo[i]), hi_min = min(hi_min, hi[i]), hi_max = max(hi_max, hi[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
-    lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
-    hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
-    hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
   }
 
   // Q^T operands
@@ -153,15 +152,53 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
     const int r = min(row[i], R - 1);
     const int64_t at = (int64_t)tok[i] * a.q_st + (int64_t)(kvh * a.rep + r % a.rep) * a.q_sh;
 #pragma unroll
-    for (int ch = 0; ch < NCH; ++ch)
+    for (int ch = 0; ch < NCH; ++ch) {
+      const int d = ch * 4 * E + g * E;
+      if constexpr (M16) {
+        Piece<CT, E, MODE> x;
+        if (a.qvec) {
+          x.load((const T*)a.q + at, d, a.D);
+        } else {
+          Piece<CT, E, 0> y;
+          y.load((const T*)a.q + at, d, a.D);
+          x.v = y.v;
+        }
+        u32x4 bits = __builtin_bit_cast(u32x4, x.v);
+        if (a.neg) bits ^= 0x80008000u;
+        qf[i][ch] = __builtin_bit_cast(typename Math::V, bits);
+      } else if (a.qvec) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int d = ch * 4 * E + g * E + j;
-        if constexpr (M16)
-          qf[i][ch][j] = d < a.D ? ((const T*)a.q)[at + d] : (T)0.0f;
-        else
-          q32[i][ch][j] = d < a.D ? load_q(a.q, a.qt, at + d) : 0.0f;
+        for (int j = 0; j < E; j += 4) {
+          Piece<XT_F32, 4, MODE == 2 ? 2 : 1> x;
+          x.load((const float*)a.q + at, d + j, a.D);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) q32[i][ch][j + k] = a.neg ? -x.v[k] : x.v[k];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float x = d + j < a.D ? load_q(a.q, a.qt, at + d + j) : 0.0f;
+          q32[i][ch][j] = a.neg ? -x : x;
+        }
       }
+    }
+  }
+
+  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    lo[i] = a.window > 0 && hi[i] - a.window + 1 > 0 ? hi[i] - a.window + 1 : 0;
+    // (a row past the last one is the last one again)
+    lo_min = min(lo_min, lo[i]), lo_max = max(lo_max, lo[i]), hi_min = min(hi_min, hi[i]), hi_max = max(hi_max, hi[i]);
+  }
+  if (a.T > 1) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
+      lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
+      hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
+      hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
+    }
   }
 
   f32x4 o[RT][NF];
@@ -173,17 +210,14 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
     for (int f = 0; f < NF; ++f) o[i][f] = (f32x4)(0.0f);
   }
 
-  const int nbc = (a.slots + SB - 1) / SB, nb = nbc + (a.Tn + SB - 1) / SB, W = a.splits * kAttnWaves;
-  for (int b = split * kAttnWaves + w; b < nb; b += W) {
+  while (b < nb) {
     const bool fresh = b >= nbc;
     const int base = (fresh ? b - nbc : b) * SB, last = (fresh ? a.Tn : a.slots) - 1;
-    bool full = false;
-    if (!fresh) {
-      const int s = base + (lane & (SB - 1));
-      const int64_t sp = s <= last ? a.slot_pos[s] : -1;
-      if (!__any(sp >= lo_min && sp <= hi_max)) continue;
-      full = __all(sp >= lo_max && sp <= hi_min);
-    }
+    const bool any = fresh || __any(sp >= lo_min && sp <= hi_max);
+    const bool full = !fresh && __all(sp >= lo_max && sp <= hi_min);
+    b += W;
+    if (b < nbc) sp = position(b);
+    if (!any) continue;
     const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
     const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
     const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
@@ -191,17 +225,20 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
     Piece<CT, E, MODE> kf[SUB][NCH];
     Piece<CT, EV, MODE> vf[VS][DB];
 #pragma unroll
-    for (int st = 0; st < SUB; ++st)
+    for (int st = 0; st < SUB; ++st) {
+      const T* const kr = kp + min(base + st * 16 + c, last) * ss;
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch)
-        kf[st][ch].load(kp + min(base + st * 16 + c, last) * ss, ch * 4 * E + g * E, a.D);
+      for (int ch = 0; ch < NCH; ++ch) kf[st][ch].load(kr, ch * 4 * E + g * E, a.D);
+    }
 #pragma unroll
-    for (int j = 0; j < VS; ++j)
+    for (int j = 0; j < VS; ++j) {
+      const T* const vr = vp + min(base + (j >> 2) * 16 + 4 * g + (j & 3), last) * ss;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
-        vf[j][db].load(vp + min(base + (j >> 2) * 16 + 4 * g + (j & 3), last) * ss, db * 16 * EV + c * EV, a.D);
+      for (int db = 0; db < DB; ++db) vf[j][db].load(vr, db * 16 * EV + c * EV, a.D);
+    }
 
     float p[RT][SUB][4];
+    uint32_t seen[RT];  // bit st * 4 + v, where not every row sees every slot
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
 #pragma unroll
@@ -218,14 +255,18 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
           }
         }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) p[i][st][v] = s[v] * a.scale;
+        for (int v = 0; v < 4; ++v) p[i][st][v] = s[v];
         if (a.scores && !fresh && row[i] < R)
-          *(f32x4*)(a.scores + ((int64_t)kvh * R + row[i]) * a.spad + base + st * 16 + 4 * g) =
-              (f32x4){p[i][st][0], p[i][st][1], p[i][st][2], p[i][st][3]};
+          *(f32x4*)(a.scores + ((int64_t)kvh * R + row[i]) * a.spad + base + st * 16 + 4 * g) = s * a.scale;
       }
-      uint32_t seen = 0xff;  // bit st * 4 + v
-      if (!full) {
-        seen = 0;
+      float mx = kNone;
+      if (full) {
+#pragma unroll
+        for (int st = 0; st < SUB; ++st)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, p[i][st][v]);
+      } else {
+        seen[i] = 0;
 #pragma unroll
         for (int st = 0; st < SUB; ++st)
 #pragma unroll
@@ -233,26 +274,22 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
             const int s = base + st * 16 + 4 * g + v;
             bool ok = s <= last;
             if (ok && !fresh) {
-              const int64_t sp = a.slot_pos[s];
-              ok = sp >= lo[i] && sp <= hi[i];
+              const int64_t at = a.slot_pos[s];
+              ok = at >= lo[i] && at <= hi[i];
             } else if (ok) {
               ok = a.tree ? a.tree[(int64_t)tok[i] * a.tree_ld + s] != 0 : s <= tok[i];
               ok = ok && (a.window == 0 || a.q_pos[s] > hi[i] - a.window);
             }
-            seen |= ok ? 1u << (st * 4 + v) : 0u;
+            seen[i] |= ok ? 1u << (st * 4 + v) : 0u;
+            mx = ok ? __builtin_fmaxf(mx, p[i][st][v]) : mx;
           }
       }
-      float mx = kNone;
-#pragma unroll
-      for (int st = 0; st < SUB; ++st)
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          if (seen >> (st * 4 + v) & 1) mx = __builtin_fmaxf(mx, p[i][st][v]);
+      mx *= a.scale;
       if (__any(mx > m[i])) {
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float up = __builtin_fmaxf(m[i], mx);
-        const float alpha = up == kNone ? 1.0f : __builtin_exp2f(m[i] - up);
+        const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[i] - up);
         m[i] = up;
         l[i] *= alpha;
 #pragma unroll
@@ -263,56 +300,67 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
       for (int st = 0; st < SUB; ++st)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float e = __builtin_exp2f(p[i][st][v] - from);
-          p[i][st][v] = seen >> (st * 4 + v) & 1 ? e : 0.0f;
-          l[i] += p[i][st][v];
+          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][st][v], a.scale, -from));
+          if (!full) e = seen[i] >> (st * 4 + v) & 1 ? e : 0.0f;
+          p[i][st][v] = e;
+          l[i] += e;
         }
-      // Where a row does not see every slot, an infinity or NaN in a V that
-      // is hidden from it must not reach it as 0 * inf: such values are
-      // taken out of the product and added to the rows that do see them.
-      if (!full) {
-        bool odd = false;
-#pragma unroll
-        for (int j = 0; j < VS; ++j)
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int e = 0; e < EV; ++e) odd |= !finite((float)vf[j][db].v[e]);
-        if (__any(odd)) {
-          float* const own = lds_o + w * 16 * OLD;  // [SB][16]
-#pragma unroll
-          for (int st = 0; st < SUB; ++st)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              own[(st * 16 + 4 * g + v) * 16 + c] = seen >> (st * 4 + v) & 1 ? p[i][st][v] : -1.0f;
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-          for (int s = 0; s < SB; ++s) {
-            const float ps = own[s * 16 + c];
-            const T* const vr = vp + min(base + s, last) * ss;
-#pragma unroll
-            for (int f = 0; f < NF; ++f)
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                const int d = f / EV * 16 * EV + (4 * g + v) * EV + f % EV;
-                const float x = d < a.D ? (float)vr[d] : 0.0f;
-                if (!finite(x) && !(ps < 0.0f)) o[i][f][v] += ps * x;
-              }
-          }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-        }
-      }
     }
+
+    // Where a row does not see every slot, an infinity or NaN in a V that is
+    // hidden from it would reach it as 0 * inf: such a block adds its slots
+    // one by one, each to the rows that see it.
+    bool apart = false;
     if (!full) {
 #pragma unroll
       for (int j = 0; j < VS; ++j)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int e = 0; e < EV; ++e)
-            vf[j][db].v[e] = finite((float)vf[j][db].v[e]) ? vf[j][db].v[e] : (T)0.0f;
+          for (int e = 0; e < EV; ++e) apart |= !finite((float)vf[j][db].v[e]);
+      apart = __any(apart);
+    }
+    if (apart) {
+      float* const own = lds_o + w * 16 * OLD;  // [SB][16]: a row's weight, -1 where it does not see the slot
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+#pragma unroll
+        for (int st = 0; st < SUB; ++st)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            own[(st * 16 + 4 * g + v) * 16 + c] = seen[i] >> (st * 4 + v) & 1 ? p[i][st][v] : -1.0f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int s = 0; s < SB; ++s) {
+          const float ps = own[s * 16 + c];
+          const bool sees = !(ps < 0.0f), first = g == 0;  // the slot is k = 0, which lane group 0 holds
+          const T* const vr = vp + min(base + s, last) * ss;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            Piece<CT, EV, MODE> x;
+            x.load(vr, db * 16 * EV + c * EV, a.D);
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+              f32x4& to = o[i][db * EV + e];
+              f32x4 sum;
+              if constexpr (M16) {
+                typename Math::V va = {}, pa = {};
+                va[0] = first ? x.v[e] : (T)0.0f;
+                pa[0] = first && sees ? (T)ps : (T)0.0f;
+                sum = Math::mfma(va, pa, to);
+              } else {
+                sum = __builtin_amdgcn_mfma_f32_16x16x4f32(first ? (float)x.v[e] : 0.0f, first && sees ? ps : 0.0f, to, 0, 0, 0);
+              }
+#pragma unroll
+              for (int v = 0; v < 4; ++v) to[v] = sees ? sum[v] : to[v];
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      continue;
     }
 
     // O^T += V^T P^T
@@ -382,7 +430,7 @@ __global__ __launch_bounds__(kAttnWaves * 64) void attn_kernel(AttnArgs a) {
         float ls = 0.0f;
 #pragma unroll
         for (int k = 0; k < kAttnWaves; ++k) {
-          const float f = __builtin_exp2f(lds_m[k][rr] - from);
+          const float f = __builtin_amdgcn_exp2f(lds_m[k][rr] - from);
           const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
           if (lds_l[k][rr] != 0.0f) {  // (a wave that saw nothing adds nothing)
             sum += x * f;

@@ -14,26 +14,37 @@ int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st)
 namespace {
 
 // One row's splits joined: the maximum over their maxima, then the partial
-// sums scaled to it.
+// sums scaled to it.  A thread's loads are independent, four at a time.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int ND = DP / 4, NG = 256 / ND;
   __shared__ __align__(16) f32x4 lds[NG][ND];
   __shared__ float lds_l[NG];
   const int64_t at = blockIdx.x;
-  const int R = a.rep * a.T, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
+  const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
   const float2* const ml = a.part_ml + at * a.splits;
   float top = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) top = __builtin_fmaxf(top, ml[s].x);
+  for (int s = lane; s < a.splits; s += 64) top = __builtin_fmaxf(top, ml[s].x);
+  top = wave_max(top);
   const float from = top == -__builtin_inff() ? 0.0f : top;
   f32x4 sum = (f32x4)(0.0f);
   float l = 0.0f;
-  for (int s = grp; s < a.splits; s += NG) {
-    const f32x4 x = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
-    const float f = __builtin_exp2f(ml[s].x - from);
-    if (ml[s].y != 0.0f) {  // (a split that saw nothing adds nothing)
-      sum += x * f;
-      l += ml[s].y * f;
+  for (int s0 = grp; s0 < a.splits; s0 += 4 * NG) {
+    f32x4 x[4];
+    float2 y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = min(s0 + k * NG, a.splits - 1);
+      x[k] = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
+      y[k] = ml[s];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = __builtin_amdgcn_exp2f(y[k].x - from);
+      if (s0 + k * NG < a.splits && y[k].y != 0.0f) {  // (a split that saw nothing adds nothing)
+        sum += x[k] * f;
+        l += y[k].y * f;
+      }
     }
   }
   lds[grp][threadIdx.x % ND] = sum;
@@ -41,6 +52,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __syncthreads();
   if (grp) return;
   l = lds_l[0];
+#pragma unroll
   for (int k = 1; k < NG; ++k) {
     sum += lds[k][threadIdx.x];
     l += lds_l[k];
@@ -67,7 +79,7 @@ __global__ __launch_bounds__(256) void attn_weight_kernel(AttnArgs a, float* wei
       const int64_t hi = a.q_pos[r / a.rep], lo = a.window > 0 ? hi - a.window + 1 : 0, at = (int64_t)kvh * R + r;
       if (sp < 0 || sp < lo || sp > hi) continue;
       const float2 ml = a.row_ml[at];
-      sum += __builtin_exp2f(a.scores[at * a.spad + s] - ml.x) * ml.y;
+      sum += __builtin_amdgcn_exp2f(a.scores[at * a.spad + s] - ml.x) * ml.y;
     }
   lds[w][lane] = sum;
   __syncthreads();
@@ -85,8 +97,9 @@ AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t blocks, bool wide) {
   AttnPlan p;
   p.RT = wide && R > 16 ? 2 : 1;
   p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
-  const int64_t room = kAttnGroups / (Hk * p.rtiles), most = (blocks + kAttnWaves - 1) / kAttnWaves;
-  p.splits = (int)(room < 1 ? 1 : room < most ? room : most);
+  const int64_t room = kAttnGroups / (Hk * p.rtiles) < 1 ? 1 : kAttnGroups / (Hk * p.rtiles);
+  const int64_t each = (blocks + kAttnWaves * room - 1) / (kAttnWaves * room);  // blocks of a wave at most
+  p.splits = (int)((blocks + kAttnWaves * each - 1) / (kAttnWaves * each));
   return p;
 }
 
@@ -126,7 +139,11 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
   a.o_st = c.o_st, a.o_sh = c.o_sh, a.tree_ld = c.tree_ld, a.window = c.window;
   a.T = (int)c.T, a.Hk = (int)Hk, a.rep = (int)rep, a.D = (int)c.D, a.slots = (int)c.slots, a.Tn = (int)c.Tn;
   a.splits = p.splits, a.rtiles = p.rtiles, a.qt = c.qt;
-  a.scale = c.scale * 1.44269504f;
+  a.neg = c.scale < 0.0f;
+  a.scale = (a.neg ? -c.scale : c.scale) * 1.44269504f;
+  const int64_t eq = c.qt == XT_F32 ? 4 : 2;
+  a.qvec = (m16 || c.qt == XT_F32) && c.D * eq % 16 == 0 && (uintptr_t)c.q % 16 == 0 && c.q_st * eq % 16 == 0 &&
+           c.q_sh * eq % 16 == 0;
   uint8_t* ws = (uint8_t*)c.ws;
   if (p.splits > 1) {
     a.part_o = (float*)ws;

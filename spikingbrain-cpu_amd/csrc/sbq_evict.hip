@@ -4,11 +4,11 @@
 // Slots are ordered by one 32-bit key: free ones 0, then the running sum of
 // attention weight as an ordered integer, the `recent` newest positions
 // highest; equal keys by slot.  One workgroup finds the m-th smallest key
-// digit by digit (11, 11 and 10 bits, a histogram each; only keys that share
-// the digits so far count) and lists the slots on one side of it in slot
-// order.  The keys stay in LDS (up to 32768 slots; more are read again for
-// every pass), each thread's own ones side by side, so that one scan over the
-// threads gives every place in the list.  A single new token needs no more
+// digit by digit (11, 11 and 10 bits, a histogram each) and lists the slots on
+// one side of it in slot order.  The keys stay in LDS (up to 32768 slots; more
+// are read again for every pass), each thread's own ones side by side, so that
+// one scan over the threads gives every place in the list; the few keys that
+// share the first digit are set apart for the other two passes.  A single new token needs no more
 // than the smallest key and its slot.  What bounds it is that workgroup's
 // reading of 12 bytes per slot and the latency of its steps; a first level
 // over several workgroups would cost another launch, which is more than the
@@ -62,32 +62,60 @@ struct Select {
   int64_t keep_from;
 };
 
-// A thread's keys of a segment of per * 1024 slots lie side by side in LDS,
-// 4 words of padding after every 32 (a thread's 16-byte reads would all meet
-// in the same banks).
-constexpr int kSegKeys = 32;  // per thread at most
-__device__ __forceinline__ int key_at(int s) { return s + (s >> 5) * 4; }
-constexpr int key_words(int per) { return per * kSelThreads / 32 * 36; }
-int keys_per_thread(int64_t n) {
-  const int64_t k = (n + kSelThreads - 1) / kSelThreads;
-  return k > kSegKeys ? kSegKeys : (int)((k + 3) / 4 * 4);
+// A thread's `per` (4, 8, 16 or 32) keys of a segment of per * 1024 slots lie
+// side by side in LDS, their 16-byte pieces permuted by the thread (else the
+// threads' reads would all meet in the same banks).
+constexpr int kSegKeys = 32, kCand = 2048;
+__host__ __device__ constexpr int keys_per_thread(int64_t n) {
+  int per = 4;
+  while (per < kSegKeys && (int64_t)per * kSelThreads < n) per *= 2;
+  return per;
+}
+__device__ __forceinline__ int key_at(int s, int per) {
+  const int t = s / per, i = s % per;
+  return t * per + ((((i >> 2) ^ t) & (per / 4 - 1)) << 2 | (i & 3));
+}
+__device__ __forceinline__ u32x4 own_keys(const uint32_t* keys, int per, int i) {
+  return *(const u32x4*)(keys + key_at(threadIdx.x * per + i, per));
 }
 
-// Keys of segment `seg` into LDS (slots past the end: key 0, never looked at).
-__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per, uint32_t* keys) {
+__device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit) {
+  // (a wave whose keys share the digit, as equal weights do, counts once)
+  const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
+  const unsigned long long on = __ballot(true);
+  if (__ballot(digit == first) == on) {
+    if ((threadIdx.x & 63) == (unsigned)__ffsll(on) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(on));
+  } else {
+    atomicAdd(&hist[digit], 1u);
+  }
+}
+
+// Keys of segment `seg` into LDS, their first digits counted where hist is
+// given.  Slots past the end get the largest key: with m <= n they come after
+// every slot that is wanted.
+__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per, uint32_t* keys, uint32_t* hist) {
   const int64_t s0 = seg * per * kSelThreads;
+  constexpr int U = 8;
 #pragma unroll 1
-  for (int i = 0; i < per; i += 4) {
-    int64_t pos[4];
-    float w[4];
+  for (int i = 0; i < per; i += U) {
+    int64_t pos[U];
+    float w[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t s = s0 + (i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
-      pos[j] = q.slot_pos[at];
-      w[j] = q.weight[at];
+    for (int j = 0; j < U; ++j) {
+      const int64_t s = s0 + (int64_t)(i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
+      if (j < 4 || per > 4) {
+        pos[j] = q.slot_pos[at];
+        w[j] = q.weight[at];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) keys[key_at((i + j) * kSelThreads + threadIdx.x)] = evict_key(pos[j], w[j], q.keep_from);
+    for (int j = 0; j < U; ++j) {
+      if (j >= 4 && per == 4) break;
+      const int s = (i + j) * kSelThreads + threadIdx.x;
+      const uint32_t k = s0 + s < q.n ? evict_key(pos[j], w[j], q.keep_from) : ~0u;
+      keys[key_at(s, per)] = k;
+      if (hist) count_digit(hist, k >> 21);
+    }
   }
 }
 
@@ -95,103 +123,125 @@ __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per,
 // others (side 1), listed in slot order; returns how many (0 <= m <= n).
 __device__ __forceinline__ int select_slots(const Select& q, int m, int side, int32_t* list) {
   extern __shared__ __align__(16) uint32_t keys[];
-  __shared__ uint32_t hist[kBins], scan[kSelWaves], found[2];
-  const int lane = threadIdx.x & 63;
-  const int64_t want = ((int64_t)q.n + kSelThreads - 1) / kSelThreads;
-  const int per = want > kSegKeys ? kSegKeys : (int)((want + 3) / 4 * 4);
-  const int64_t segs = (want + per - 1) / per;
-  load_keys(q, 0, per, keys);
+  __shared__ uint32_t hist[kBins], cand[kCand], scan[kSelWaves], found[3], ncand;
+  const int per = keys_per_thread(q.n);
+  const int64_t segs = ((int64_t)q.n + per * kSelThreads - 1) / (per * kSelThreads);
+  for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
+  if (threadIdx.x == 0) ncand = 0;
+  __syncthreads();
+  for (int64_t seg = 0; seg < segs; ++seg) {
+    load_keys(q, seg, per, keys, m > 0 ? hist : nullptr);
+    if (segs > 1) __syncthreads();
+  }
+  __syncthreads();
 
   // the m-th smallest key `kth`, of which `ties` (lowest slots first) belong to the m
   uint32_t kth = 0, ties = m;
   if (m > 0) {
+    bool few = false;  // the keys that share the first digit are in `cand`
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       const uint32_t above = pass == 0 ? 0u : ~0u << (shift + bits);
-      for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
-#pragma unroll 1
-      for (int64_t seg = 0; seg < segs; ++seg) {
-        if (segs > 1) {
-          __syncthreads();  // (everyone is done with the keys before)
-          load_keys(q, seg, per, keys);
-        }
+      if (pass > 0) {
+        for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        const int64_t s0 = (seg * kSelThreads + threadIdx.x) * per;
+        if (few) {
+          for (unsigned i = threadIdx.x; i < ncand; i += kSelThreads) {
+            const uint32_t k = cand[i];
+            if (((k ^ kth) & above) == 0) count_digit(hist, k >> shift & ((1u << bits) - 1));
+          }
+        } else {
 #pragma unroll 1
-        for (int i = 0; i < per; i += 4) {
-          const u32x4 k4 = *(const u32x4*)(keys + key_at(threadIdx.x * per + i));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool on = s0 + i + j < q.n && ((k4[j] ^ kth) & above) == 0;
-            const unsigned long long who = __ballot(on);
-            if (!who) continue;
-            const uint32_t digit = k4[j] >> shift & ((1u << bits) - 1);
-            // (a wave whose keys share the digit, as equal weights do, counts once)
-            const uint32_t first = __builtin_amdgcn_readlane(digit, __ffsll(who) - 1);
-            if (__ballot(on && digit == first) == who) {
-              if (lane == __ffsll(who) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(who));
-            } else if (on) {
-              atomicAdd(&hist[digit], 1u);
+          for (int64_t seg = 0; seg < segs; ++seg) {
+            if (segs > 1) {
+              load_keys(q, seg, per, keys, nullptr);
+              __syncthreads();
             }
+#pragma unroll 1
+            for (int i = 0; i < per; i += 4) {
+              const u32x4 k4 = own_keys(keys, per, i);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (((k4[j] ^ kth) & above) == 0) count_digit(hist, k4[j] >> shift & ((1u << bits) - 1));
+            }
+            if (segs > 1) __syncthreads();
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
       const uint32_t a = hist[2 * threadIdx.x], b = hist[2 * threadIdx.x + 1];
       uint32_t total;
       const uint32_t before = block_scan(a + b, scan, &total);
-      if (before < ties && ties <= before + a) found[0] = 2 * threadIdx.x, found[1] = before;
-      if (before + a < ties && ties <= before + a + b) found[0] = 2 * threadIdx.x + 1, found[1] = before + a;
+      if (before < ties && ties <= before + a) found[0] = 2 * threadIdx.x, found[1] = before, found[2] = a;
+      if (before + a < ties && ties <= before + a + b)
+        found[0] = 2 * threadIdx.x + 1, found[1] = before + a, found[2] = b;
       __syncthreads();
       kth |= found[0] << shift;
       ties -= found[1];
+      if (pass == 0 && segs == 1 && found[2] <= kCand) {
+        few = true;
+#pragma unroll 1
+        for (int i = 0; i < per; i += 4) {
+          const u32x4 k4 = own_keys(keys, per, i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (k4[j] >> 21 == found[0]) cand[atomicAdd(&ncand, 1u)] = k4[j];
+        }
+      }
+      __syncthreads();
     }
   }
 
   // Of the keys equal to kth the first `ties` are among the m; free slots
   // (key 0) are never among the used ones.  Before a thread's own slots lie
-  // `out` listed ones off kth and `eq` equal ones.
+  // `out` keys strictly on the wanted side and `eq` equal ones.
   uint32_t out = 0, eq = 0;
 #pragma unroll 1
   for (int64_t seg = 0; seg < segs; ++seg) {
-    __syncthreads();
     if (segs > 1) {
-      load_keys(q, seg, per, keys);
+      load_keys(q, seg, per, keys, nullptr);
       __syncthreads();
     }
     const int64_t s0 = (seg * kSelThreads + threadIdx.x) * per;
-    uint32_t my_out = 0, my_eq = 0;
+    uint32_t strict = 0, same = 0;  // one bit per own key
 #pragma unroll 1
     for (int i = 0; i < per; i += 4) {
-      const u32x4 k4 = *(const u32x4*)(keys + key_at(threadIdx.x * per + i));
+      const u32x4 k4 = own_keys(keys, per, i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool in = s0 + i + j < q.n;
-        my_out += in && (side == 0 ? k4[j] < kth : k4[j] > kth);
-        my_eq += in && k4[j] == kth;
+        strict |= (uint32_t)(side == 0 ? k4[j] < kth : k4[j] > kth) << (i + j);
+        same |= (uint32_t)(k4[j] == kth) << (i + j);
       }
     }
+    if (s0 + per > q.n) {
+      const uint32_t in = s0 >= q.n ? 0u : (1u << (q.n - s0)) - 1;
+      strict &= in;
+      same &= in;
+    }
     uint32_t all_out, all_eq;
-    const uint32_t out0 = out + block_scan(my_out, scan, &all_out), eq0 = eq + block_scan(my_eq, scan, &all_eq);
-    uint32_t o = out0, e = eq0;
-    if (my_out + my_eq > 0) {
-#pragma unroll 1
-      for (int i = 0; i < per; ++i) {
-        const uint32_t k = keys[key_at(threadIdx.x * per + i)];
-        if (s0 + i >= q.n) break;
-        const uint32_t low_eq = min(e, ties), high_eq = kth == 0 ? 0u : e - low_eq;  // equal ones before, on each side
-        const bool low = k < kth || (k == kth && e < ties), high = k > kth || (k == kth && e >= ties && kth != 0);
-        if (side == 0 ? low : high) list[o + (side == 0 ? low_eq : high_eq)] = (int32_t)(s0 + i);
-        o += side == 0 ? k < kth : k > kth;
-        e += k == kth;
+    const uint32_t out0 = out + block_scan(__popc(strict), scan, &all_out);
+    const uint32_t eq0 = eq + block_scan(__popc(same), scan, &all_eq);
+    const uint32_t low0 = min(eq0, ties);
+    const uint32_t mine = min(eq0 + (uint32_t)__popc(same), ties) - low0;  // own equal ones among the m
+    uint32_t place = out0 + (side == 0 ? low0 : kth == 0 ? 0u : eq0 - low0);
+    uint32_t skip = mine, todo = strict | same;
+    while (todo) {
+      const uint32_t bit = todo & (0u - todo);
+      todo ^= bit;
+      bool take = strict & bit;
+      if (!take) {
+        take = side == 0 ? skip > 0 : skip == 0 && kth != 0;
+        skip -= skip > 0;
       }
+      if (take) list[place++] = (int32_t)(s0 + __ffs(bit) - 1);
     }
     out += all_out;
     eq += all_eq;
+    if (segs > 1) __syncthreads();
   }
-  const uint32_t low_eq = min(eq, ties);
-  return (int)(out + (side == 0 ? low_eq : kth == 0 ? 0u : eq - low_eq));
+  const uint32_t low = min(eq, ties);
+  return (int)(out + (side == 0 ? low : kth == 0 ? 0u : eq - low));
 }
 
 // The slot of the smallest key (the lowest of equal ones).
@@ -257,14 +307,17 @@ __device__ __forceinline__ void copy_row(const Rows& src, int64_t from, const Ro
   }
 }
 
-// 16 bytes at a time (equal types, aligned rows): e counts 16-byte pieces.
+// 16 bytes at a time (equal types, aligned rows): `per` pieces a head, the
+// keys' before the values' over the threads.
 __device__ __forceinline__ void copy_row16(const Rows& src, int64_t from, const Rows& dst, int64_t to, int per, int es,
-                                           int e0, int e1, int step) {
-  for (int e = e0; e < e1; e += step) {
-    const int64_t h = e / per, d = e % per * (16 / es);
+                                           int heads) {
+  const int half = heads * per;
+  for (int e = threadIdx.x; e < 2 * half; e += blockDim.x) {
+    const bool val = e >= half;
+    const int u = val ? e - half : e;
+    const int64_t h = u / per, d = u % per * (16 / es);
     const int64_t fi = (from * src.ss + h * src.sh + d) * es, ti = (to * dst.ss + h * dst.sh + d) * es;
-    *(u32x4*)((uint8_t*)dst.k + ti) = *(const u32x4*)((const uint8_t*)src.k + fi);
-    *(u32x4*)((uint8_t*)dst.v + ti) = *(const u32x4*)((const uint8_t*)src.v + fi);
+    *(u32x4*)((uint8_t*)(val ? dst.v : dst.k) + ti) = *(const u32x4*)((const uint8_t*)(val ? src.v : src.k) + fi);
   }
 }
 
@@ -355,8 +408,7 @@ __global__ __launch_bounds__(256) void kv_take_rows_kernel(TakeArgs a) {
     a.to_weight[i] = a.weight[s];
   }
   if (a.vec) {
-    const int per = a.D * a.es / 16;
-    copy_row16(a.src, s, a.dst, i, per, a.es, threadIdx.x, a.Hk * per, 256);
+    copy_row16(a.src, s, a.dst, i, a.D * a.es / 16, a.es, a.Hk);
   } else if (a.es == 4) {
     copy_row<XT_F32, XT_F32>(a.src, s, a.dst, i, a.D, threadIdx.x, a.Hk * a.D, 256);
   } else {
@@ -372,7 +424,7 @@ int append_types(const AppendArgs& a, hipStream_t st) {
     kv_append_one_kernel<ST, DT><<<1, kSelThreads, 0, st>>>(a);
     return check_launch();
   }
-  kv_append_kernel<ST, DT><<<1, kSelThreads, key_words(keys_per_thread(a.n)) * 4, st>>>(a);
+  kv_append_kernel<ST, DT><<<1, kSelThreads, keys_per_thread(a.n) * kSelThreads * 4, st>>>(a);
   int rc = check_launch();
   if (rc || a.rows_too) return rc;
   kv_rows_kernel<ST, DT><<<a.T, 256, 0, st>>>(a);
@@ -403,7 +455,7 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
   TakeArgs a{c.slot_pos, c.end, c.weight, c.to_pos, c.to_end, c.to_weight,
              Rows{const_cast<void*>(c.k), const_cast<void*>(c.v), c.k_ss, c.k_sh}, Rows{c.to_k, c.to_v, c.t_ss, c.t_sh},
              (int32_t*)c.ws, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
-  kv_take_kernel<<<1, kSelThreads, key_words(keys_per_thread(a.n)) * 4, st>>>(a);
+  kv_take_kernel<<<1, kSelThreads, keys_per_thread(a.n) * kSelThreads * 4, st>>>(a);
   const int rc = check_launch();
   if (rc) return rc;
   kv_take_rows_kernel<<<a.capacity, 256, 0, st>>>(a);
