@@ -42,10 +42,10 @@ struct AttnArgs {
   const int64_t *slot_pos, *q_pos;
   const uint8_t* tree;          // [T][tree_ld], null: draft j is seen by t >= j
   void* out;
-  float *part_o, *scores;       // [Hk*R][splits][DP]; [Hk*R][spad] (null: not wanted)
+  float* part_o;                // [Hk*R][splits][DP]
   float2* part_ml;              // [Hk*R][splits]
-  float2* row_ml;               // [Hk*R] (maximum, 1 / sum), with scores
-  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld, spad;
+  float2* row_ml;               // [Hk*R] (maximum, 1 / sum), where the slots' weights are wanted
+  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld;
   int64_t window;               // 0: none
   int T, Hk, rep, D, slots, Tn, splits, rtiles, qt;
   float scale;                  // times log2(e), >= 0 (`neg`: q is negated instead)
@@ -109,6 +109,50 @@ __device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
 
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
 
+// One row of Q as the S^T product's operand: lane group g holds the columns
+// ch * 4E + g * E + 0..E-1 of every piece ch.
+template <int CT, bool M16, int DP, int MODE>
+struct QRow {
+  static constexpr int E = CElem<CT>::E, NCH = DP / (4 * E);
+  typename AttnMath<CT>::V v[M16 ? NCH : 1];
+  float f[M16 ? 1 : NCH][E];
+  __device__ __forceinline__ void load(const AttnArgs& a, int kvh, int r, int g) {
+    typedef typename XElem<CT>::T T;
+    const int64_t at = (int64_t)(r / a.rep) * a.q_st + (int64_t)(kvh * a.rep + r % a.rep) * a.q_sh;
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) {
+      const int d = ch * 4 * E + g * E;
+      if constexpr (M16) {
+        Piece<CT, E, MODE> x;
+        if (a.qvec) {
+          x.load((const T*)a.q + at, d, a.D);
+        } else {
+          Piece<CT, E, 0> y;
+          y.load((const T*)a.q + at, d, a.D);
+          x.v = y.v;
+        }
+        u32x4 bits = __builtin_bit_cast(u32x4, x.v);
+        if (a.neg) bits ^= 0x80008000u;
+        v[ch] = __builtin_bit_cast(typename AttnMath<CT>::V, bits);
+      } else if (a.qvec) {
+#pragma unroll
+        for (int j = 0; j < E; j += 4) {
+          Piece<XT_F32, 4, MODE == 2 ? 2 : 1> x;
+          x.load((const float*)a.q + at, d + j, a.D);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[ch][j + k] = a.neg ? -x.v[k] : x.v[k];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float x = d + j < a.D ? load_q(a.q, a.qt, at + d + j) : 0.0f;
+          f[ch][j] = a.neg ? -x : x;
+        }
+      }
+    }
+  }
+};
+
 template <int CT, bool M16, int DP, int MODE, int RT>
 __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT == 2 ? 2 : 3) void attn_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
@@ -144,45 +188,9 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
     hi[i] = a.q_pos[tok[i]];
   }
 
-  // Q^T operands
-  typename Math::V qf[RT][M16 ? NCH : 1];
-  float q32[RT][M16 ? 1 : NCH][E];
+  QRow<CT, M16, DP, MODE> qr[RT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int r = min(row[i], R - 1);
-    const int64_t at = (int64_t)tok[i] * a.q_st + (int64_t)(kvh * a.rep + r % a.rep) * a.q_sh;
-#pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) {
-      const int d = ch * 4 * E + g * E;
-      if constexpr (M16) {
-        Piece<CT, E, MODE> x;
-        if (a.qvec) {
-          x.load((const T*)a.q + at, d, a.D);
-        } else {
-          Piece<CT, E, 0> y;
-          y.load((const T*)a.q + at, d, a.D);
-          x.v = y.v;
-        }
-        u32x4 bits = __builtin_bit_cast(u32x4, x.v);
-        if (a.neg) bits ^= 0x80008000u;
-        qf[i][ch] = __builtin_bit_cast(typename Math::V, bits);
-      } else if (a.qvec) {
-#pragma unroll
-        for (int j = 0; j < E; j += 4) {
-          Piece<XT_F32, 4, MODE == 2 ? 2 : 1> x;
-          x.load((const float*)a.q + at, d + j, a.D);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) q32[i][ch][j + k] = a.neg ? -x.v[k] : x.v[k];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float x = d + j < a.D ? load_q(a.q, a.qt, at + d + j) : 0.0f;
-          q32[i][ch][j] = a.neg ? -x : x;
-        }
-      }
-    }
-  }
+  for (int i = 0; i < RT; ++i) qr[i].load(a, kvh, min(row[i], R - 1), g);
 
   int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
 #pragma unroll
@@ -247,17 +255,15 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
         for (int ch = 0; ch < NCH; ++ch) {
           if constexpr (M16) {
-            s = Math::mfma(__builtin_bit_cast(typename Math::V, kf[st][ch].v), qf[i][ch], s);
+            s = Math::mfma(__builtin_bit_cast(typename Math::V, kf[st][ch].v), qr[i].v[ch], s);
           } else {
 #pragma unroll
             for (int j = 0; j < E; ++j)
-              s = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kf[st][ch].v[j], q32[i][ch][j], s, 0, 0, 0);
+              s = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kf[st][ch].v[j], qr[i].f[ch][j], s, 0, 0, 0);
           }
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[i][st][v] = s[v];
-        if (a.scores && !fresh && row[i] < R)
-          *(f32x4*)(a.scores + ((int64_t)kvh * R + row[i]) * a.spad + base + st * 16 + 4 * g) = s * a.scale;
       }
       float mx = kNone;
       if (full) {
@@ -455,6 +461,104 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
   }
 }
 
+// weight[s] += sum over the rows that see slot s of exp2(score - maximum) /
+// sum, the scores computed once more: storing them would move 8 bytes per row
+// and slot, more than a key's own bytes from some 16 rows on, and hold them in
+// memory.  A workgroup takes SB slots and every row; its waves share the
+// (key head, 16-row tile) pairs, keep the slots' keys in registers while the
+// head stays, and add up in wave order.
+constexpr int kWeightWaves = 8;
+template <int CT, bool M16, int DP, int MODE>
+__global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs a, float* weight) {
+  typedef typename XElem<CT>::T T;
+  typedef AttnMath<CT> Math;
+  constexpr int E = CElem<CT>::E, NCH = DP / (4 * E), SUB = M16 ? 2 : 1, SB = 16 * SUB;
+  __shared__ float sums[kWeightWaves][SB];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int R = a.rep * a.T, tiles = (R + 15) / 16, base = blockIdx.x * SB, last = a.slots - 1;
+
+  // is there a row that sees any of the slots, do all rows see all of them?
+  const int own = base + (lane & (SB - 1));
+  const int64_t sp = own <= last ? a.slot_pos[own] : -1;
+  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
+  for (int t = lane; t < a.T; t += 64) {
+    const int64_t hi = a.q_pos[t], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+    lo_min = min(lo_min, lo), lo_max = max(lo_max, lo), hi_min = min(hi_min, hi), hi_max = max(hi_max, hi);
+  }
+  for (int o = 1; o < 64 && o < a.T; o <<= 1) {
+    lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
+    lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
+    hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
+    hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
+  }
+  lo_min = __shfl((long long)lo_min, 0, 64), lo_max = __shfl((long long)lo_max, 0, 64);
+  hi_min = __shfl((long long)hi_min, 0, 64), hi_max = __shfl((long long)hi_max, 0, 64);
+  if (!__any(sp >= lo_min && sp <= hi_max)) return;  // (the same for every wave)
+  const bool full = __all(sp >= lo_max && sp <= hi_min);
+
+  Piece<CT, E, MODE> kf[SUB][NCH];
+  float acc[SUB][4] = {};
+  const int units = a.Hk * tiles, u1 = (int)((int64_t)(w + 1) * units / kWeightWaves);
+  int held = -1;
+  for (int u = (int)((int64_t)w * units / kWeightWaves); u < u1; ++u) {
+    const int kvh = u / tiles, r = u % tiles * 16 + c, rc = min(r, R - 1);
+    QRow<CT, M16, DP, MODE> qr;
+    qr.load(a, kvh, rc, g);
+    const float2 ml = a.row_ml[(int64_t)kvh * R + rc];
+    const int64_t hi = a.q_pos[rc / a.rep], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+    if (kvh != held) {
+      held = kvh;
+#pragma unroll
+      for (int st = 0; st < SUB; ++st) {
+        const T* const kr = (const T*)a.k + (int64_t)kvh * a.k_sh + min(base + st * 16 + c, last) * a.k_ss;
+#pragma unroll
+        for (int ch = 0; ch < NCH; ++ch) kf[st][ch].load(kr, ch * 4 * E + g * E, a.D);
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < SUB; ++st) {
+      f32x4 s = (f32x4)(0.0f);
+#pragma unroll
+      for (int ch = 0; ch < NCH; ++ch) {
+        if constexpr (M16) {
+          s = Math::mfma(__builtin_bit_cast(typename Math::V, kf[st][ch].v), qr.v[ch], s);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kf[st][ch].v[j], qr.f[ch][j], s, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.scale, -ml.x)) * ml.y;
+        bool ok = r < R;
+        if (!full) {
+          const int at = base + st * 16 + 4 * g + v;
+          const int64_t pos = at <= last ? a.slot_pos[at] : -1;
+          ok = ok && pos >= lo && pos <= hi;
+        }
+        acc[st][v] += ok ? p : 0.0f;
+      }
+    }
+  }
+#pragma unroll
+  for (int st = 0; st < SUB; ++st)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      float x = acc[st][v];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
+      if (c == 0) sums[w][st * 16 + 4 * g + v] = x;
+    }
+  __syncthreads();
+  if (threadIdx.x < SB && base + (int)threadIdx.x <= last) {
+    float x = sums[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kWeightWaves; ++k) x += sums[k][threadIdx.x];
+    weight[base + threadIdx.x] += x;
+  }
+}
+
 // One attention launch of a configuration; defined per pair (cache type,
 // 2-byte products) in the files that instantiate the kernel.
 template <int CT, bool M16, int DP>
@@ -475,15 +579,34 @@ int launch_attn_dp(const AttnArgs& a, int mode, int RT, hipStream_t st) {
   return e == hipSuccess ? 0 : -5;
 }
 
+template <int CT, bool M16, int DP>
+int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st) {
+  constexpr int SB = M16 ? 32 : 16, threads = kWeightWaves * 64;
+  const dim3 grid((unsigned)((a.slots + SB - 1) / SB));
+  if (mode == 2)
+    attn_weight_kernel<CT, M16, DP, 2><<<grid, threads, 0, st>>>(a, weight);
+  else if (mode == 1)
+    attn_weight_kernel<CT, M16, DP, 1><<<grid, threads, 0, st>>>(a, weight);
+  else if constexpr (!M16)
+    attn_weight_kernel<CT, M16, DP, 0><<<grid, threads, 0, st>>>(a, weight);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : -5;
+}
+
+// `weight` null: the attention; else the slots' weights after it.
 template <int CT, bool M16>
-int launch_attn_ct(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st) {
+int launch_attn_ct(const AttnArgs& a, int DP, int mode, int RT, float* weight, hipStream_t st) {
+  if (weight)
+    return DP == 64 ? launch_weight_dp<CT, M16, 64>(a, mode, weight, st)
+           : DP == 128 ? launch_weight_dp<CT, M16, 128>(a, mode, weight, st)
+                       : launch_weight_dp<CT, M16, 256>(a, mode, weight, st);
   return DP == 64 ? launch_attn_dp<CT, M16, 64>(a, mode, RT, st)
          : DP == 128 ? launch_attn_dp<CT, M16, 128>(a, mode, RT, st)
                      : launch_attn_dp<CT, M16, 256>(a, mode, RT, st);
 }
 
-int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st);
-int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st);
-int launch_attn_bf16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st);
+int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, float* weight, hipStream_t st);
+int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, float* weight, hipStream_t st);
+int launch_attn_bf16(const AttnArgs& a, bool m16, int DP, int mode, int RT, float* weight, hipStream_t st);
 
 }  // namespace sbq

@@ -7,8 +7,8 @@
 
 namespace sbq {
 
-int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, hipStream_t st) {
-  return launch_attn_ct<XT_F32, false>(a, DP, mode, RT, st);
+int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, float* weight, hipStream_t st) {
+  return launch_attn_ct<XT_F32, false>(a, DP, mode, RT, weight, st);
 }
 
 namespace {
@@ -66,26 +66,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
 }
 
-// weight[s] += sum over the rows that see slot s of exp2(score - max) / sum,
-// 64 slots per workgroup, the rows dealt to its waves and added in wave order.
-__global__ __launch_bounds__(256) void attn_weight_kernel(AttnArgs a, float* weight) {
-  __shared__ float lds[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, s = blockIdx.x * 64 + lane;
-  const int R = a.rep * a.T;
-  const int64_t sp = s < a.slots ? a.slot_pos[s] : -1;
-  float sum = 0.0f;
-  for (int kvh = 0; kvh < a.Hk; ++kvh)
-    for (int r = w; r < R; r += 4) {
-      const int64_t hi = a.q_pos[r / a.rep], lo = a.window > 0 ? hi - a.window + 1 : 0, at = (int64_t)kvh * R + r;
-      if (sp < 0 || sp < lo || sp > hi) continue;
-      const float2 ml = a.row_ml[at];
-      sum += __builtin_amdgcn_exp2f(a.scores[at * a.spad + s] - ml.x) * ml.y;
-    }
-  lds[w][lane] = sum;
-  __syncthreads();
-  if (w == 0 && s < a.slots) weight[s] += lds[0][lane] + lds[1][lane] + lds[2][lane] + lds[3][lane];
-}
-
 constexpr int kAttnGroups = 512;  // workgroups aimed at
 
 int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
@@ -116,7 +96,7 @@ int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, in
   }
   int64_t n = 0;
   if (splits > 1) n += round256(rows * splits * attn_dp(D) * 4) + round256(rows * splits * 8);
-  if (weight) n += round256(rows * 8) + round256(rows * ((slots + 31) / 32 * 32) * 4);
+  if (weight) n += round256(rows * 8);
   return n;
 }
 
@@ -151,15 +131,13 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
     a.part_ml = (float2*)ws;
     ws += round256(Hk * R * p.splits * 8);
   }
-  if (c.weight) {
-    a.row_ml = (float2*)ws;
-    ws += round256(Hk * R * 8);
-    a.scores = (float*)ws;
-    a.spad = (c.slots + 31) / 32 * 32;
-  }
-  int rc = c.ct == XT_F32   ? launch_attn_f32(a, DP, mode, p.RT, st)
-           : c.ct == XT_F16 ? launch_attn_f16(a, m16, DP, mode, p.RT, st)
-                            : launch_attn_bf16(a, m16, DP, mode, p.RT, st);
+  if (c.weight) a.row_ml = (float2*)ws;
+  auto launch = [&](float* weight) {
+    return c.ct == XT_F32   ? launch_attn_f32(a, DP, mode, p.RT, weight, st)
+           : c.ct == XT_F16 ? launch_attn_f16(a, m16, DP, mode, p.RT, weight, st)
+                            : launch_attn_bf16(a, m16, DP, mode, p.RT, weight, st);
+  };
+  int rc = launch(nullptr);
   if (rc) return rc;
   if (p.splits > 1) {
     const unsigned grid = (unsigned)(Hk * R);
@@ -171,8 +149,7 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
       attn_join_kernel<256><<<grid, 256, 0, st>>>(a);
     if ((rc = check_launch())) return rc;
   }
-  if (c.weight) attn_weight_kernel<<<(unsigned)((c.slots + 63) / 64), 256, 0, st>>>(a, c.weight);
-  return check_launch();
+  return c.weight ? launch(c.weight) : 0;
 }
 
 }  // namespace sbq

@@ -5,8 +5,9 @@
 
 namespace sbq {
 
-int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, hipStream_t st) {
-  return m16 ? launch_attn_ct<XT_F16, true>(a, DP, mode, RT, st) : launch_attn_ct<XT_F16, false>(a, DP, mode, RT, st);
+int launch_attn_f16(const AttnArgs& a, bool m16, int DP, int mode, int RT, float* weight, hipStream_t st) {
+  return m16 ? launch_attn_ct<XT_F16, true>(a, DP, mode, RT, weight, st)
+             : launch_attn_ct<XT_F16, false>(a, DP, mode, RT, weight, st);
 }
 
 }  // namespace sbq

@@ -66,17 +66,17 @@ struct Select {
 // side by side in LDS, their 16-byte pieces permuted by the thread (else the
 // threads' reads would all meet in the same banks).
 constexpr int kSegKeys = 32, kCand = 2048;
-__host__ __device__ constexpr int keys_per_thread(int64_t n) {
-  int per = 4;
-  while (per < kSegKeys && (int64_t)per * kSelThreads < n) per *= 2;
-  return per;
+__host__ __device__ constexpr int keys_log(int64_t n) {
+  int log = 2;
+  while (1 << log < kSegKeys && ((int64_t)kSelThreads << log) < n) ++log;
+  return log;
 }
-__device__ __forceinline__ int key_at(int s, int per) {
-  const int t = s / per, i = s % per;
-  return t * per + ((((i >> 2) ^ t) & (per / 4 - 1)) << 2 | (i & 3));
+// Place of key i of thread t, `per` = 1 << log.
+__device__ __forceinline__ int key_at(int t, int i, int log) {
+  return (t << log) + ((((i >> 2) ^ t) & ((1 << log) / 4 - 1)) << 2 | (i & 3));
 }
-__device__ __forceinline__ u32x4 own_keys(const uint32_t* keys, int per, int i) {
-  return *(const u32x4*)(keys + key_at(threadIdx.x * per + i, per));
+__device__ __forceinline__ u32x4 own_keys(const uint32_t* keys, int log, int i) {
+  return *(const u32x4*)(keys + key_at(threadIdx.x, i, log));
 }
 
 __device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit) {
@@ -93,7 +93,8 @@ __device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit) {
 // Keys of segment `seg` into LDS, their first digits counted where hist is
 // given.  Slots past the end get the largest key: with m <= n they come after
 // every slot that is wanted.
-__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per, uint32_t* keys, uint32_t* hist) {
+__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int log, uint32_t* keys, uint32_t* hist) {
+  const int per = 1 << log;
   const int64_t s0 = seg * per * kSelThreads;
   constexpr int U = 8;
 #pragma unroll 1
@@ -113,7 +114,7 @@ __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per,
       if (j >= 4 && per == 4) break;
       const int s = (i + j) * kSelThreads + threadIdx.x;
       const uint32_t k = s0 + s < q.n ? evict_key(pos[j], w[j], q.keep_from) : ~0u;
-      keys[key_at(s, per)] = k;
+      keys[key_at(s >> log, s & (per - 1), log)] = k;
       if (hist) count_digit(hist, k >> 21);
     }
   }
@@ -124,13 +125,13 @@ __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int per,
 __device__ __forceinline__ int select_slots(const Select& q, int m, int side, int32_t* list) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ uint32_t hist[kBins], cand[kCand], scan[kSelWaves], found[3], ncand;
-  const int per = keys_per_thread(q.n);
-  const int64_t segs = ((int64_t)q.n + per * kSelThreads - 1) / (per * kSelThreads);
+  const int log = keys_log(q.n), per = 1 << log;
+  const int segs = (int)(((int64_t)q.n + per * kSelThreads - 1) >> (log + 10));
   for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
   if (threadIdx.x == 0) ncand = 0;
   __syncthreads();
-  for (int64_t seg = 0; seg < segs; ++seg) {
-    load_keys(q, seg, per, keys, m > 0 ? hist : nullptr);
+  for (int seg = 0; seg < segs; ++seg) {
+    load_keys(q, seg, log, keys, m > 0 ? hist : nullptr);
     if (segs > 1) __syncthreads();
   }
   __syncthreads();
@@ -153,14 +154,14 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
           }
         } else {
 #pragma unroll 1
-          for (int64_t seg = 0; seg < segs; ++seg) {
+          for (int seg = 0; seg < segs; ++seg) {
             if (segs > 1) {
-              load_keys(q, seg, per, keys, nullptr);
+              load_keys(q, seg, log, keys, nullptr);
               __syncthreads();
             }
 #pragma unroll 1
             for (int i = 0; i < per; i += 4) {
-              const u32x4 k4 = own_keys(keys, per, i);
+              const u32x4 k4 = own_keys(keys, log, i);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 if (((k4[j] ^ kth) & above) == 0) count_digit(hist, k4[j] >> shift & ((1u << bits) - 1));
@@ -183,7 +184,7 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
         few = true;
 #pragma unroll 1
         for (int i = 0; i < per; i += 4) {
-          const u32x4 k4 = own_keys(keys, per, i);
+          const u32x4 k4 = own_keys(keys, log, i);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (k4[j] >> 21 == found[0]) cand[atomicAdd(&ncand, 1u)] = k4[j];
@@ -198,16 +199,16 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
   // `out` keys strictly on the wanted side and `eq` equal ones.
   uint32_t out = 0, eq = 0;
 #pragma unroll 1
-  for (int64_t seg = 0; seg < segs; ++seg) {
+  for (int seg = 0; seg < segs; ++seg) {
     if (segs > 1) {
-      load_keys(q, seg, per, keys, nullptr);
+      load_keys(q, seg, log, keys, nullptr);
       __syncthreads();
     }
-    const int64_t s0 = (seg * kSelThreads + threadIdx.x) * per;
+    const int64_t s0 = ((int64_t)seg * kSelThreads + threadIdx.x) * per;
     uint32_t strict = 0, same = 0;  // one bit per own key
 #pragma unroll 1
     for (int i = 0; i < per; i += 4) {
-      const u32x4 k4 = own_keys(keys, per, i);
+      const u32x4 k4 = own_keys(keys, log, i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         strict |= (uint32_t)(side == 0 ? k4[j] < kth : k4[j] > kth) << (i + j);
@@ -424,7 +425,7 @@ int append_types(const AppendArgs& a, hipStream_t st) {
     kv_append_one_kernel<ST, DT><<<1, kSelThreads, 0, st>>>(a);
     return check_launch();
   }
-  kv_append_kernel<ST, DT><<<1, kSelThreads, keys_per_thread(a.n) * kSelThreads * 4, st>>>(a);
+  kv_append_kernel<ST, DT><<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(a.n), st>>>(a);
   int rc = check_launch();
   if (rc || a.rows_too) return rc;
   kv_rows_kernel<ST, DT><<<a.T, 256, 0, st>>>(a);
@@ -455,7 +456,7 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
   TakeArgs a{c.slot_pos, c.end, c.weight, c.to_pos, c.to_end, c.to_weight,
              Rows{const_cast<void*>(c.k), const_cast<void*>(c.v), c.k_ss, c.k_sh}, Rows{c.to_k, c.to_v, c.t_ss, c.t_sh},
              (int32_t*)c.ws, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
-  kv_take_kernel<<<1, kSelThreads, keys_per_thread(a.n) * kSelThreads * 4, st>>>(a);
+  kv_take_kernel<<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(a.n), st>>>(a);
   const int rc = check_launch();
   if (rc) return rc;
   kv_take_rows_kernel<<<a.capacity, 256, 0, st>>>(a);
