@@ -530,8 +530,9 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
  * weights; its other slots become free (slot_pos -1, weight 0; k and v left
  * as they were), *to_end = *end.  The two must not overlap.
  *
- * workspace: >= sbq_kv_workspace_bytes(T or capacity), any content. */
-int64_t sbq_kv_workspace_bytes(int64_t count);
+ * workspace: >= sbq_kv_workspace_bytes(slots, T or capacity), any content; one
+ * call at a time. */
+int64_t sbq_kv_workspace_bytes(int64_t slots, int64_t count);
 int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end, const int64_t* start,
                   int64_t recent, void* k, void* v, int kv_dtype, int64_t kv_heads, int64_t D,
                   int64_t k_ss, int64_t k_sh, const void* k_new, const void* v_new, int new_dtype,

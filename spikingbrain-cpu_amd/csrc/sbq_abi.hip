@@ -719,7 +719,10 @@ static bool kv_sizes_ok(int64_t slots, int64_t kv_heads, int64_t D) {
          kv_heads * D <= (1 << 24);
 }
 
-int64_t sbq_kv_workspace_bytes(int64_t count) { return count < 1 || count > (1 << 30) ? 0 : (count + 1) * 4 + 16; }
+int64_t sbq_kv_workspace_bytes(int64_t slots, int64_t count) {
+  if (slots < 1 || count < 1 || slots > (1 << 30) || count > (1 << 30)) return 0;
+  return sbq::kv_workspace_bytes(slots, count) + 16;  // + alignment slack
+}
 
 int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end, const int64_t* start, int64_t recent,
                   void* k, void* v, int kv_dtype, int64_t kv_heads, int64_t D, int64_t k_ss, int64_t k_sh,
@@ -734,7 +737,7 @@ int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end,
   if (!aligned(slot_pos, 8) || !aligned(weight, 4) || !aligned(end, 8) || !aligned(start, 8) || !aligned(k, es) ||
       !aligned(v, es) || !aligned(k_new, en) || !aligned(v_new, en))
     return SBQ_ERR_ALIGN;
-  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(T)) return SBQ_ERR_WORKSPACE;
+  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(slots, T)) return SBQ_ERR_WORKSPACE;
   sbq::KvAppend c{};
   c.slot_pos = slot_pos, c.weight = weight, c.end = end, c.start = start, c.k = k, c.v = v, c.kn = k_new, c.vn = v_new;
   c.ws = (void*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);
@@ -756,7 +759,7 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
   if (!aligned(slot_pos, 8) || !aligned(weight, 4) || !aligned(end, 8) || !aligned(to_pos, 8) || !aligned(to_weight, 4) ||
       !aligned(to_end, 8) || !aligned(k, es) || !aligned(v, es) || !aligned(to_k, es) || !aligned(to_v, es))
     return SBQ_ERR_ALIGN;
-  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(capacity)) return SBQ_ERR_WORKSPACE;
+  if (!workspace || (int64_t)workspace_bytes < sbq_kv_workspace_bytes(slots, capacity)) return SBQ_ERR_WORKSPACE;
   sbq::KvTake c{};
   c.slot_pos = slot_pos, c.end = end, c.weight = weight, c.k = k, c.v = v, c.to_pos = to_pos, c.to_end = to_end;
   c.to_weight = to_weight, c.to_k = to_k, c.to_v = to_v, c.ws = (void*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15);

@@ -36,6 +36,7 @@
 namespace sbq {
 
 constexpr int kAttnWaves = 4;
+constexpr int kTileSlots = 64, kTileWaves = 8;  // attn_tile_kernel: slots per step, waves per workgroup at most
 
 struct AttnArgs {
   const void *q, *k, *v, *kn, *vn;
@@ -108,6 +109,36 @@ __device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
 }
 
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
+
+// Infinities and NaN of V.  Where a row does not see every slot of a block,
+// such a value must not reach it as 0 * inf: the block's product takes the
+// finite values only, and the others are counted by a product of zeros and
+// ones (V's element is of the kind, the row sees the slot): a row that sees
+// one has it added.  kind: 0 +inf, 1 -inf, 2 NaN.
+__device__ __forceinline__ float odd_value(int kind) {
+  return kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+}
+__device__ __forceinline__ float odd_one(float x, int kind) {
+  const bool is = kind == 0 ? x == __builtin_inff() : kind == 1 ? x == -__builtin_inff() : x != x;
+  return is ? 1.0f : 0.0f;
+}
+// ... on two 2-byte values side by side
+template <int CT>
+struct Odd2 {
+  static constexpr uint32_t kExp = CT == XT_F16 ? 0x7c00u : 0x7f80u, kOne = CT == XT_F16 ? 0x3c00u : 0x3f80u;
+  static __device__ __forceinline__ bool any(uint32_t w) {
+    return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+  }
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+    return ((w & kExp) == kExp ? 0u : w & 0xffffu) | ((w >> 16 & kExp) == kExp ? 0u : w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ bool is(uint32_t x, int kind) {
+    return kind == 2 ? (x & 0x7fffu) > kExp : x == (kind ? kExp | 0x8000u : kExp);
+  }
+  static __device__ __forceinline__ uint32_t ones(uint32_t w, int kind) {
+    return (is(w & 0xffffu, kind) ? kOne : 0u) | (is(w >> 16, kind) ? kOne << 16 : 0u);
+  }
+};
 
 // One row of Q as the S^T product's operand: lane group g holds the columns
 // ch * 4E + g * E + 0..E-1 of every piece ch.
@@ -246,7 +277,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
     }
 
     float p[RT][SUB][4];
-    uint32_t seen[RT];  // bit st * 4 + v, where not every row sees every slot
+    uint32_t seen[RT];  // bit st * 4 + v, where not every row sees every slot (= V's slot j of the lane)
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
 #pragma unroll
@@ -313,60 +344,15 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
         }
     }
 
-    // Where a row does not see every slot, an infinity or NaN in a V that is
-    // hidden from it would reach it as 0 * inf: such a block adds its slots
-    // one by one, each to the rows that see it.
-    bool apart = false;
+    bool odd = false;  // infinities or NaN in V, and rows that do not see every slot
     if (!full) {
 #pragma unroll
       for (int j = 0; j < VS; ++j)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int e = 0; e < EV; ++e) apart |= !finite((float)vf[j][db].v[e]);
-      apart = __any(apart);
-    }
-    if (apart) {
-      float* const own = lds_o + w * 16 * OLD;  // [SB][16]: a row's weight, -1 where it does not see the slot
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-#pragma unroll
-        for (int st = 0; st < SUB; ++st)
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            own[(st * 16 + 4 * g + v) * 16 + c] = seen[i] >> (st * 4 + v) & 1 ? p[i][st][v] : -1.0f;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int s = 0; s < SB; ++s) {
-          const float ps = own[s * 16 + c];
-          const bool sees = !(ps < 0.0f), first = g == 0;  // the slot is k = 0, which lane group 0 holds
-          const T* const vr = vp + min(base + s, last) * ss;
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            Piece<CT, EV, MODE> x;
-            x.load(vr, db * 16 * EV + c * EV, a.D);
-#pragma unroll
-            for (int e = 0; e < EV; ++e) {
-              f32x4& to = o[i][db * EV + e];
-              f32x4 sum;
-              if constexpr (M16) {
-                typename Math::V va = {}, pa = {};
-                va[0] = first ? x.v[e] : (T)0.0f;
-                pa[0] = first && sees ? (T)ps : (T)0.0f;
-                sum = Math::mfma(va, pa, to);
-              } else {
-                sum = __builtin_amdgcn_mfma_f32_16x16x4f32(first ? (float)x.v[e] : 0.0f, first && sees ? ps : 0.0f, to, 0, 0, 0);
-              }
-#pragma unroll
-              for (int v = 0; v < 4; ++v) to[v] = sees ? sum[v] : to[v];
-            }
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
-      continue;
+          for (int e = 0; e < EV; ++e) odd |= !finite((float)vf[j][db].v[e]);
+      odd = __any(odd);
     }
 
     // O^T += V^T P^T
@@ -388,6 +374,26 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          if (odd) {
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {
+              u32x4 ones;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) ones[j] = Odd2<CT>::ones(t[j], kind);
+#pragma unroll
+              for (int i = 0; i < RT; ++i) {
+                typename Math::V sees;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sees[j] = (T)(seen[i] >> j & 1 ? 1.0f : 0.0f);
+                const f32x4 n = Math::mfma(__builtin_bit_cast(typename Math::V, ones), sees, (f32x4)(0.0f));
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                  if (n[v] > 0.0f) o[i][db * EV + e][v] += odd_value(kind);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = Odd2<CT>::finite(t[j]);
+          }
           const typename Math::V vt = __builtin_bit_cast(typename Math::V, t);
 #pragma unroll
           for (int i = 0; i < RT; ++i) o[i][db * EV + e] = Math::mfma(vt, pf[i], o[i][db * EV + e]);
@@ -399,11 +405,25 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int e = 0; e < EV; ++e)
+          for (int e = 0; e < EV; ++e) {
+            float x = (float)vf[j][db].v[e];
+            if (odd) {
+#pragma unroll 1
+              for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                  const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x4f32(odd_one(x, kind), seen[i] >> j & 1 ? 1.0f : 0.0f,
+                                                                       (f32x4)(0.0f), 0, 0, 0);
+#pragma unroll
+                  for (int v = 0; v < 4; ++v)
+                    if (n[v] > 0.0f) o[i][db * EV + e][v] += odd_value(kind);
+                }
+              x = finite(x) ? x : 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < RT; ++i)
-              o[i][db * EV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)vf[j][db].v[e], p[i][0][j],
-                                                                       o[i][db * EV + e], 0, 0, 0);
+              o[i][db * EV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i][0][j], o[i][db * EV + e], 0, 0, 0);
+          }
     }
   }
 
@@ -458,6 +478,253 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
         }
       }
     }
+  }
+}
+
+// The same for many rows (128 and more of a key head) over 2-byte caches of
+// 64 or 128 columns: a wave owns 32 rows, the workgroup's waves share every
+// tile of 64 slots through LDS, double-buffered (global -> LDS copies of the
+// next tile run under the products of this one), and 32x32x16 products halve
+// the operand reads per product.  K and V rows lie in LDS as in memory, their
+// 16-byte pieces permuted by the row (source side: the copy writes lane after
+// lane), so that the operand reads of 32 rows meet all banks.  S^T and O^T as
+// above: lane (h, r) holds the scores of row r and the slots 8 (v / 4) + 4 h +
+// v % 4, which 16 at a time are the operand of V^T's product in that slot
+// order.  What bounds it: per 64 scores 32 cycles of products and some 30 of
+// exponentials and sums per SIMD, two waves of which overlap.
+template <int CT, int DP>
+__global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs a) {
+  typedef typename XElem<CT>::T T;
+  typedef AttnMath<CT> Math;
+  typedef typename Math::V V;
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  constexpr int TS = kTileSlots, KK = DP / 16, EV = DP / 32, CPR = DP / 8, ROWB = DP * 2;
+  constexpr int TILEB = TS * ROWB, BUFB = 2 * TILEB;  // K then V
+  constexpr float kNone = -__builtin_inff();
+  extern __shared__ __align__(16) uint8_t lds[];  // two tiles
+  auto product = [](V x, V y, f32x16 z) {
+    if constexpr (CT == XT_F16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
+  };
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, NW = blockDim.x >> 6, r = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x % a.Hk, rtile = blockIdx.x / a.Hk % a.rtiles, split = blockIdx.x / a.Hk / a.rtiles;
+  const int R = a.rep * a.T, row = (rtile * NW + w) * 32 + r, rowc = min(row, R - 1), tok = rowc / a.rep;
+
+  const int nbc = (a.slots + TS - 1) / TS, nb = nbc + (a.Tn + TS - 1) / TS;
+  auto position = [&](int b) -> int64_t {
+    const int s = b * TS + lane;
+    return s < a.slots ? a.slot_pos[s] : -1;
+  };
+  // what the tokens of the whole call see (the workgroup's skipping is uniform)
+  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
+  for (int t = lane; t < a.T; t += 64) {
+    const int64_t hi = a.q_pos[t], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+    lo_min = min(lo_min, lo), lo_max = max(lo_max, lo), hi_min = min(hi_min, hi), hi_max = max(hi_max, hi);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
+    lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
+    hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
+    hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
+  }
+  const int64_t hi = a.q_pos[tok], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+
+  // Q^T operand: lane (h, r) holds columns 16 kk + 8 h + 0..7 of row r
+  V qf[KK];
+  {
+    const int64_t at = (int64_t)tok * a.q_st + (int64_t)(kvh * a.rep + rowc % a.rep) * a.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      u32x4 bits;
+      if (a.qvec) {
+        bits = *(const u32x4*)((const T*)a.q + at + kk * 16 + h * 8);
+      } else {
+        Piece<CT, 8, 0> y;
+        y.load((const T*)a.q + at, kk * 16 + h * 8, DP);
+        bits = __builtin_bit_cast(u32x4, y.v);
+      }
+      if (a.neg) bits ^= 0x80008000u;
+      qf[kk] = __builtin_bit_cast(V, bits);
+    }
+  }
+
+  // the next tile at or after b that some token sees (nb: none), and whether all see all of it
+  auto visible = [&](int b, bool& full) {
+    for (; b < nbc; b += a.splits) {
+      const int64_t sp = position(b);
+      if (__any(sp >= lo_min && sp <= hi_max)) {
+        full = __all(sp >= lo_max && sp <= hi_min);
+        return b;
+      }
+    }
+    full = false;
+    return b;
+  };
+  auto copy_tile = [&](int b, int buf) {
+    const bool fresh = b >= nbc;
+    const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
+    const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
+    const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
+    const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
+    for (int q = w; q < BUFB / 1024; q += NW) {  // 64 pieces of 16 bytes a wave
+      const int piece = q * 64 + lane, val = piece >= TS * CPR, u = piece & (TS * CPR - 1), s = u / CPR;
+      const T* const src = (val ? vp : kp) + min(base + s, last) * ss + ((u ^ s) & (CPR - 1)) * 8;
+      __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(lds + buf * BUFB + q * 1024),
+                                       16, 0, 0);
+    }
+  };
+
+  f32x16 o[EV];
+  float m = kNone, l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < EV; ++e) o[e] = (f32x16)(0.0f);
+
+  bool full, next_full = false;
+  int b = visible(split, full), buf = 0;
+  if (b < nb) copy_tile(b, 0);
+  while (b < nb) {
+    __syncthreads();  // this tile has arrived; everyone is done with the other buffer
+    const int next = visible(b + a.splits, next_full);
+    if (next < nb) copy_tile(next, buf ^ 1);
+    const bool fresh = b >= nbc;
+    const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
+    const uint8_t* const kt = lds + buf * BUFB;
+    const uint8_t* const vt = kt + TILEB;
+#pragma unroll 1
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 s = (f32x16)(0.0f);
+      {
+        const uint8_t* const kr = kt + (sub * 32 + r) * ROWB;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const V kf = *(const V*)(kr + (((kk * 2 + h) ^ (sub * 32 + r)) & (CPR - 1)) * 16);
+          s = product(kf, qf[kk], s);
+        }
+      }
+      uint32_t seen = 0;
+      float mx = kNone;
+      if (full) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = __builtin_fmaxf(mx, s[v]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int at = base + sub * 32 + (v / 4) * 8 + 4 * h + v % 4;
+          bool ok = at <= last;
+          if (ok && !fresh) {
+            const int64_t sp = a.slot_pos[at];
+            ok = sp >= lo && sp <= hi;
+          } else if (ok) {
+            ok = a.tree ? a.tree[(int64_t)tok * a.tree_ld + at] != 0 : at <= tok;
+            ok = ok && (a.window == 0 || a.q_pos[at] > hi - a.window);
+          }
+          seen |= ok ? 1u << v : 0u;
+          mx = ok ? __builtin_fmaxf(mx, s[v]) : mx;
+        }
+      }
+      mx *= a.scale;
+      if (__any(mx > m)) {
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float up = __builtin_fmaxf(m, mx);
+        const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < EV; ++e) o[e] *= alpha;
+      }
+      const float from = m == kNone ? 0.0f : m;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.scale, -from));
+        if (!full) p = seen >> v & 1 ? p : 0.0f;
+        s[v] = p;
+        l += p;
+      }
+      // V^T's operand for 16 slots: 8 of the lane's slots, EV columns each
+      auto v_words = [&](int kc, uint32_t (&vw)[8][EV / 2]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int sl = sub * 32 + kc * 16 + (j >> 2) * 8 + 4 * h + (j & 3);
+          const int byte = r * EV * 2;
+          const uint8_t* const at = vt + sl * ROWB + (((byte >> 4) ^ sl) & (CPR - 1)) * 16 + (byte & 15);
+          if constexpr (EV == 4) {
+            const u32x2 x = *(const u32x2*)at;
+            vw[j][0] = x.x, vw[j][1] = x.y;
+          } else {
+            vw[j][0] = *(const uint32_t*)at;
+          }
+        }
+      };
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        uint32_t vw[8][EV / 2];
+        v_words(kc, vw);
+        bool odd = false;
+        if (!full) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < EV / 2; ++e) odd |= Odd2<CT>::any(vw[j][e]);
+          odd = __any(odd);
+        }
+        V pf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[j] = (T)s[kc * 8 + j];
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          u32x4 t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          if (odd) {
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {
+              u32x4 ones;
+              V sees;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) ones[j] = Odd2<CT>::ones(t[j], kind);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) sees[j] = (T)(seen >> (kc * 8 + j) & 1 ? 1.0f : 0.0f);
+              const f32x16 n = product(__builtin_bit_cast(V, ones), sees, (f32x16)(0.0f));
+#pragma unroll
+              for (int v = 0; v < 16; ++v)
+                if (n[v] > 0.0f) o[e][v] += odd_value(kind);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = Odd2<CT>::finite(t[j]);
+          }
+          o[e] = product(__builtin_bit_cast(V, t), pf, o[e]);
+        }
+      }
+    }
+    b = next, full = next_full, buf ^= 1;
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (row >= R) return;
+  const int64_t at = (int64_t)kvh * R + row;
+  const bool joined = a.splits > 1;
+  const float from = m == kNone ? 0.0f : m, inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const int64_t out = (int64_t)tok * a.o_st + (int64_t)(kvh * a.rep + row % a.rep) * a.o_sh;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int d = ((v / 4) * 8 + 4 * h + v % 4) * EV;
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      if (joined)
+        a.part_o[(at * a.splits + split) * DP + d + e] = o[e][v];
+      else
+        store_y(a.out, a.qt, out + d + e, o[e][v] * inv);
+    }
+  }
+  if (h == 0) {
+    if (joined)
+      a.part_ml[at * a.splits + split] = make_float2(m, l);
+    else if (a.row_ml)
+      a.row_ml[at] = make_float2(from, inv);
   }
 }
 
@@ -579,6 +846,14 @@ int launch_attn_dp(const AttnArgs& a, int mode, int RT, hipStream_t st) {
   return e == hipSuccess ? 0 : -5;
 }
 
+template <int CT, int DP>
+int launch_tile_dp(const AttnArgs& a, int waves, hipStream_t st) {
+  constexpr int lds = 2 * 2 * kTileSlots * DP * 2;
+  attn_tile_kernel<CT, DP><<<dim3((unsigned)(a.Hk * a.rtiles * a.splits)), waves * 64, lds, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : -5;
+}
+
 template <int CT, bool M16, int DP>
 int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st) {
   constexpr int SB = M16 ? 32 : 16, threads = kWeightWaves * 64;
@@ -593,13 +868,17 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
   return e == hipSuccess ? 0 : -5;
 }
 
-// `weight` null: the attention; else the slots' weights after it.
+// `weight` null: the attention (RT < 0: attn_tile_kernel with -RT waves a
+// workgroup); else the slots' weights after it.
 template <int CT, bool M16>
 int launch_attn_ct(const AttnArgs& a, int DP, int mode, int RT, float* weight, hipStream_t st) {
   if (weight)
     return DP == 64 ? launch_weight_dp<CT, M16, 64>(a, mode, weight, st)
            : DP == 128 ? launch_weight_dp<CT, M16, 128>(a, mode, weight, st)
                        : launch_weight_dp<CT, M16, 256>(a, mode, weight, st);
+  if constexpr (M16) {
+    if (RT < 0) return DP == 64 ? launch_tile_dp<CT, 64>(a, -RT, st) : launch_tile_dp<CT, 128>(a, -RT, st);
+  }
   return DP == 64 ? launch_attn_dp<CT, M16, 64>(a, mode, RT, st)
          : DP == 128 ? launch_attn_dp<CT, M16, 128>(a, mode, RT, st)
                      : launch_attn_dp<CT, M16, 256>(a, mode, RT, st);

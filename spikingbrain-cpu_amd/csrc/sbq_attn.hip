@@ -66,20 +66,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
 }
 
-constexpr int kAttnGroups = 512;  // workgroups aimed at
+constexpr int kAttnGroups = 512;    // workgroups aimed at
+constexpr int kTileGroups = 2048;   // waves aimed at by attn_tile_kernel: 8 per CU
+constexpr int64_t kTileRows = 128;  // rows of a key head from which it is taken
 
 int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct AttnPlan {
-  int RT, rtiles, splits;
+  int RT, rtiles, splits;  // RT: row tiles per wave, or -(waves) of attn_tile_kernel
 };
-AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t blocks, bool wide) {
+// vec: rows of exactly DP columns by 16-byte loads; m16: 2-byte products.
+AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, bool vec, bool m16) {
   AttnPlan p;
-  p.RT = wide && R > 16 ? 2 : 1;
-  p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
-  const int64_t room = kAttnGroups / (Hk * p.rtiles) < 1 ? 1 : kAttnGroups / (Hk * p.rtiles);
-  const int64_t each = (blocks + kAttnWaves * room - 1) / (kAttnWaves * room);  // blocks of a wave at most
-  p.splits = (int)((blocks + kAttnWaves * each - 1) / (kAttnWaves * each));
+  int64_t groups = kAttnGroups, each = kAttnWaves, SB = m16 ? 32 : 16;
+  if (vec && m16 && DP <= 128 && R >= kTileRows) {
+    const int64_t waves = (R + 31) / 32;
+    p.RT = -(int)(waves < kTileWaves ? waves : kTileWaves);
+    p.rtiles = (int)((waves - p.RT - 1) / -p.RT);
+    groups = kTileGroups / -p.RT;
+    each = 1, SB = kTileSlots;
+  } else {
+    p.RT = vec && R > 16 && (m16 || DP < 256) ? 2 : 1;  // (two tiles of 256 fp32 columns do not fit the registers)
+    p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
+  }
+  const int64_t room = groups / (Hk * p.rtiles) < 1 ? 1 : groups / (Hk * p.rtiles);
+  const int64_t blocks = (slots + SB - 1) / SB + (Tn + SB - 1) / SB;
+  const int64_t most = (blocks + each * room - 1) / (each * room);  // blocks of a wave (of a workgroup) at most
+  p.splits = (int)((blocks + each * most - 1) / (each * most));
   return p;
 }
 
@@ -90,8 +103,8 @@ int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t slots, bool weight) {
   const int64_t R = heads / Hk * T, rows = Hk * R;
   int64_t splits = 1;
-  for (int wide = 0; wide < 2; ++wide) {
-    const int64_t s = attn_plan(R, Hk, (slots + 15) / 16 + (T + 15) / 16, wide).splits;
+  for (int way = 0; way < 8; ++way) {  // types, alignment and drafts are not known here
+    const int64_t s = attn_plan(R, Hk, slots, way & 4 ? T : 0, attn_dp(D), way & 1, way & 2).splits;
     splits = s > splits ? s : splits;
   }
   int64_t n = 0;
@@ -110,8 +123,8 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
                        (c.Tn == 0 || (vec(c.kn, c.n_ss, c.n_sh) && vec(c.vn, c.n_ss, c.n_sh)));
   const int mode = !aligned ? 0 : c.D == DP ? 2 : 1;
   const bool m16 = c.ct != XT_F32 && c.qt == c.ct && mode > 0;
-  const int64_t Hk = c.Hk, rep = c.heads / Hk, R = rep * c.T, SB = m16 ? 32 : 16;
-  const AttnPlan p = attn_plan(R, Hk, (c.slots + SB - 1) / SB + (c.Tn + SB - 1) / SB, mode == 2 && (m16 || DP < 256));
+  const int64_t Hk = c.Hk, rep = c.heads / Hk, R = rep * c.T;
+  const AttnPlan p = attn_plan(R, Hk, c.slots, c.Tn, DP, mode == 2, m16);
   AttnArgs a{};
   a.q = c.q, a.k = c.k, a.v = c.v, a.kn = c.kn, a.vn = c.vn, a.slot_pos = c.slot_pos, a.q_pos = c.q_pos, a.tree = c.tree;
   a.out = c.out;

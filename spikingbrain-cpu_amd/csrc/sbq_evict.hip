@@ -8,12 +8,14 @@
 // one side of it in slot order.  The keys stay in LDS (up to 32768 slots; more
 // are read again for every pass), each thread's own ones side by side, so that
 // one scan over the threads gives every place in the list; the few keys that
-// share the first digit are set apart for the other two passes.  A single new token needs no more
-// than the smallest key and its slot.  What bounds it is that workgroup's
-// reading of 12 bytes per slot and the latency of its steps; a first level
-// over several workgroups would cost another launch, which is more than the
-// reading up to some 32768 slots.  Integer counts only, so the result does
-// not depend on timing.
+// share the first digit are set apart for the other two passes.  A single new
+// token needs no more than the smallest key and its slot.
+//
+// What bounds it is one CU's reading from HBM (12 bytes per slot at some 23
+// GB/s) and the latency of the steps, so from 8192 slots on a launch before it
+// spreads the reading: for an append every workgroup leaves the T first of its
+// 4096 slots (which hold the T first of all), for a take the 4-byte keys.
+// Integer counts only, so the result does not depend on timing.
 #include "sbq_common.h"
 #include "sbq_launch.h"
 
@@ -60,6 +62,7 @@ struct Select {
   const float* weight;
   int n;
   int64_t keep_from;
+  const uint32_t* ready;  // not null: the keys themselves
 };
 
 // A thread's `per` (4, 8, 16 or 32) keys of a segment of per * 1024 slots lie
@@ -101,19 +104,24 @@ __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int log,
   for (int i = 0; i < per; i += U) {
     int64_t pos[U];
     float w[U];
+    uint32_t key[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int64_t s = s0 + (int64_t)(i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
       if (j < 4 || per > 4) {
-        pos[j] = q.slot_pos[at];
-        w[j] = q.weight[at];
+        if (q.ready) {
+          key[j] = q.ready[at];
+        } else {
+          pos[j] = q.slot_pos[at];
+          w[j] = q.weight[at];
+        }
       }
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (j >= 4 && per == 4) break;
       const int s = (i + j) * kSelThreads + threadIdx.x;
-      const uint32_t k = s0 + s < q.n ? evict_key(pos[j], w[j], q.keep_from) : ~0u;
+      const uint32_t k = s0 + s >= q.n ? ~0u : q.ready ? key[j] : evict_key(pos[j], w[j], q.keep_from);
       keys[key_at(s >> log, s & (per - 1), log)] = k;
       if (hist) count_digit(hist, k >> 21);
     }
@@ -329,6 +337,8 @@ struct AppendArgs {
   const int64_t* start;
   Rows cache, fresh;
   int32_t* list;
+  uint32_t* cand_key;  // with several workgroups: the T first of each one's slots
+  int32_t* cand_slot;
   int n, T, Hk, D;
   int64_t recent;
   bool rows_too;
@@ -338,7 +348,7 @@ struct AppendArgs {
 template <int ST, int DT>
 __global__ __launch_bounds__(kSelThreads) void kv_append_one_kernel(AppendArgs a) {
   const int64_t start = *a.start;
-  const Select q{a.slot_pos, a.weight, a.n, start + 1 - a.recent};
+  const Select q{a.slot_pos, a.weight, a.n, start + 1 - a.recent, nullptr};
   const int s = first_slot(q);  // (every thread has read its slots and *start)
   if (threadIdx.x == 0) {
     a.slot_pos[s] = start;
@@ -348,19 +358,39 @@ __global__ __launch_bounds__(kSelThreads) void kv_append_one_kernel(AppendArgs a
   copy_row<ST, DT>(a.fresh, 0, a.cache, s, a.D, threadIdx.x, a.Hk * a.D, kSelThreads);
 }
 
+// The T first of every kChunk slots, in slot order, with their keys.
+constexpr int kChunk = 4 * kSelThreads, kSpreadFrom = 2 * kChunk, kSpreadTokens = kChunk / 8;
+__global__ __launch_bounds__(kSelThreads) void kv_first_kernel(AppendArgs a) {
+  const int s0 = blockIdx.x * kChunk, n = min(kChunk, a.n - s0), m = min(a.T, n);
+  const Select q{a.slot_pos + s0, a.weight + s0, n, *a.start + a.T - a.recent, nullptr};
+  int32_t* const list = a.cand_slot + (int64_t)blockIdx.x * a.T;
+  select_slots(q, m, 0, list);
+  __syncthreads();  // the list is written
+  for (int i = threadIdx.x; i < m; i += kSelThreads) {
+    const int s = list[i];
+    a.cand_key[(int64_t)blockIdx.x * a.T + i] = evict_key(q.slot_pos[s], q.weight[s], q.keep_from);
+    list[i] = s0 + s;
+  }
+}
+
 template <int ST, int DT>
 __global__ __launch_bounds__(kSelThreads) void kv_append_kernel(AppendArgs a) {
   const int64_t start = *a.start;
-  const Select q{a.slot_pos, a.weight, a.n, start + a.T - a.recent};
+  const int chunks = (a.n + kChunk - 1) / kChunk;
+  Select q{a.slot_pos, a.weight, a.n, start + a.T - a.recent, a.cand_key};
+  // (only the last workgroup may have had fewer than T slots, so the candidates are dense and in slot order)
+  if (a.cand_key) q.n = (chunks - 1) * a.T + min(a.T, a.n - (chunks - 1) * kChunk);
   select_slots(q, a.T, 0, a.list);
   __syncthreads();  // the list is written
   for (int i = threadIdx.x; i < a.T; i += kSelThreads) {
-    const int s = a.list[i];
+    int s = a.list[i];
+    if (a.cand_key) a.list[i] = s = a.cand_slot[s];
     a.slot_pos[s] = start + i;
     a.weight[s] = 0.0f;
   }
   if (threadIdx.x == 0) *a.end = start + a.T;
   if (a.rows_too) {
+    __syncthreads();  // the list is in slots
     const int row = a.Hk * a.D;
     for (int i = 0; i < a.T; ++i)
       copy_row<ST, DT>(a.fresh, i, a.cache, a.list[i], a.D, threadIdx.x, row, kSelThreads);
@@ -378,15 +408,21 @@ struct TakeArgs {
   int64_t *to_pos, *to_end;
   float* to_weight;
   Rows src, dst;
-  int32_t* list;  // [capacity], then the count
+  int32_t* list;   // [capacity], then the count
+  uint32_t* keys;  // [n] where a launch before the selection computes them
   int n, capacity, Hk, D, es;
   int64_t recent;
   bool vec;
 };
 
+__global__ __launch_bounds__(256) void kv_keys_kernel(TakeArgs a) {
+  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (s < a.n) a.keys[s] = evict_key(a.slot_pos[s], a.weight[s], *a.end - a.recent);
+}
+
 __global__ __launch_bounds__(kSelThreads) void kv_take_kernel(TakeArgs a) {
   const int64_t end = *a.end;
-  const Select q{a.slot_pos, a.weight, a.n, end - a.recent};
+  const Select q{a.slot_pos, a.weight, a.n, end - a.recent, a.keys};
   const int kept = select_slots(q, a.n > a.capacity ? a.n - a.capacity : 0, 1, a.list);
   if (threadIdx.x == 0) {
     a.list[a.capacity] = kept;
@@ -425,8 +461,16 @@ int append_types(const AppendArgs& a, hipStream_t st) {
     kv_append_one_kernel<ST, DT><<<1, kSelThreads, 0, st>>>(a);
     return check_launch();
   }
-  kv_append_kernel<ST, DT><<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(a.n), st>>>(a);
-  int rc = check_launch();
+  int rc = 0;
+  int64_t n = a.n;
+  if (a.cand_key) {
+    const int chunks = (a.n + kChunk - 1) / kChunk;
+    kv_first_kernel<<<chunks, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(kChunk), st>>>(a);
+    if ((rc = check_launch())) return rc;
+    n = (int64_t)chunks * a.T;
+  }
+  kv_append_kernel<ST, DT><<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(n), st>>>(a);
+  rc = check_launch();
   if (rc || a.rows_too) return rc;
   kv_rows_kernel<ST, DT><<<a.T, 256, 0, st>>>(a);
   return check_launch();
@@ -440,10 +484,18 @@ int append_from(const AppendArgs& a, int ct, hipStream_t st) {
 
 }  // namespace
 
+// The list (one count more), then the candidates of an append or the keys of a take.
+int64_t kv_workspace_bytes(int64_t slots, int64_t count) { return 4 * (count + 1) + (slots >= kSpreadFrom ? 4 * slots : 0); }
+static_assert(kSpreadTokens * 8 <= kChunk && 2 * kSpreadTokens * 8 <= 3 * kSpreadFrom, "candidates fit 4 bytes a slot");
+
 int launch_kv_append(const KvAppend& c, hipStream_t st) {
   AppendArgs a{c.slot_pos, c.weight, c.end, c.start, Rows{c.k, c.v, c.k_ss, c.k_sh},
-               Rows{const_cast<void*>(c.kn), const_cast<void*>(c.vn), c.n_ss, c.n_sh}, (int32_t*)c.ws, (int)c.slots, (int)c.T,
-               (int)c.Hk, (int)c.D, c.recent, c.T * c.Hk * c.D <= kInlineElems};
+               Rows{const_cast<void*>(c.kn), const_cast<void*>(c.vn), c.n_ss, c.n_sh}, (int32_t*)c.ws, nullptr, nullptr,
+               (int)c.slots, (int)c.T, (int)c.Hk, (int)c.D, c.recent, c.T * c.Hk * c.D <= kInlineElems};
+  if (c.slots >= kSpreadFrom && c.T > 1 && c.T <= kSpreadTokens) {  // candidates: at most n bytes, and one chunk's
+    a.cand_slot = a.list + c.T;
+    a.cand_key = (uint32_t*)(a.cand_slot + (c.slots + kChunk - 1) / kChunk * c.T);
+  }
   return c.nt == XT_F32 ? append_from<XT_F32>(a, c.ct, st) : c.nt == XT_F16 ? append_from<XT_F16>(a, c.ct, st)
                                                                              : append_from<XT_BF16>(a, c.ct, st);
 }
@@ -455,7 +507,12 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
                    ok(c.to_v, c.t_ss, c.t_sh);
   TakeArgs a{c.slot_pos, c.end, c.weight, c.to_pos, c.to_end, c.to_weight,
              Rows{const_cast<void*>(c.k), const_cast<void*>(c.v), c.k_ss, c.k_sh}, Rows{c.to_k, c.to_v, c.t_ss, c.t_sh},
-             (int32_t*)c.ws, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
+             (int32_t*)c.ws, c.slots >= kSpreadFrom ? (uint32_t*)c.ws + c.capacity + 1 : nullptr, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
+  if (a.keys) {
+    kv_keys_kernel<<<(a.n + 255) / 256, 256, 0, st>>>(a);
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
   kv_take_kernel<<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(a.n), st>>>(a);
   const int rc = check_launch();
   if (rc) return rc;

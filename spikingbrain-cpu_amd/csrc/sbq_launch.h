@@ -250,7 +250,8 @@ int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, in
 int launch_tree_attention(const AttnCall& c, hipStream_t st);
 
 // A bounded cache that gives up its least attended slots (sbq_evict.hip); ws:
-// int32 [T] / [capacity + 1].
+// kv_workspace_bytes(slots, T or capacity), 16-byte aligned.
+int64_t kv_workspace_bytes(int64_t slots, int64_t count);
 struct KvAppend {
   int64_t* slot_pos;
   float* weight;

@@ -60,7 +60,7 @@ SIGNATURES = {
     "sbq_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _I]),
     "sbq_tree_attention": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L,
                                 _L, ctypes.c_float, _P, _L, _L, _P, _P, _S, _P]),
-    "sbq_kv_workspace_bytes": (_L, [_L]),
+    "sbq_kv_workspace_bytes": (_L, [_L, _L]),
     "sbq_kv_append": (_I, [_P, _P, _L, _P, _P, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _P, _S, _P]),
     "sbq_kv_take": (_I, [_P, _P, _L, _P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _L, _P, _S, _P]),
     "sbq_sample_rows": (_I, [_P, _L, _L, _L, ctypes.c_float, _L, ctypes.c_float, _P, _P, _P, _S, _P]),

@@ -266,7 +266,7 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
             k, v = k.contiguous(), v.contiguous()
         s = self.end if start is None else _as_pos(start, kv.device)
         L = _lib.load()
-        ws = torch.empty((4 * T + 20,), dtype=torch.uint8, device=kv.device)  # sbq_kv_workspace_bytes(T)
+        ws = torch.empty((L.sbq_kv_workspace_bytes(self.capacity, T),), dtype=torch.uint8, device=kv.device)
         ks, ns = kv.stride(), k.stride()
         with _on_device(kv.device):
             _lib.check(L.sbq_kv_append(
@@ -293,7 +293,7 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
             raise ValueError(f"DeviceBudgetKVBuffer.take: weight must be a contiguous float32 [{source.capacity}] tensor on "
                              f"{kv.device}")
         L = _lib.load()
-        ws = torch.empty((4 * self.capacity + 20,), dtype=torch.uint8, device=kv.device)
+        ws = torch.empty((L.sbq_kv_workspace_bytes(source.capacity, self.capacity),), dtype=torch.uint8, device=kv.device)
         ks, ts = source.k.stride(), kv.stride()
         with _on_device(kv.device):
             _lib.check(L.sbq_kv_take(

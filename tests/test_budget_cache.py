@@ -42,7 +42,8 @@ def test_c_abi_refuses_bad_arguments():
     for name in ("sp", "w", "end", "k", "v", "tp", "tw", "te", "tk", "tv"):
         assert take(**{name: None}) == -1
     assert take(te=p + 4) == -3 and take(ws=None) == -4 and take(nws=16) == -4
-    assert L.sbq_kv_workspace_bytes(0) == 0 and L.sbq_kv_workspace_bytes(12) == 4 * 12 + 20
+    assert L.sbq_kv_workspace_bytes(8, 0) == 0 and L.sbq_kv_workspace_bytes(0, 8) == 0
+    assert L.sbq_kv_workspace_bytes(8, 12) == 4 * 12 + 20 and app(nws=L.sbq_kv_workspace_bytes(8, 1) - 1) == -4
 
 
 def test_buffer_refuses_and_new_state():
@@ -123,7 +124,7 @@ def _same(a, b):
 
 APPENDS = [(1, 1, 0, 1), (5, 3, 5, 5), (64, 1, 0, 64), (64, 64, 64, 30), (1000, 7, 100, 1000), (1000, 400, 3, 700),
            (4096, 1, 512, 4096), (4097, 12, 4000, 4097), (20000, 33, 64, 19990), (32768, 1, 1, 32768), (32769, 64, 7, 32769),
-           (100003, 5, 1024, 99000)]
+           (100003, 5, 1024, 99000), (8192, 512, 100, 8192), (8195, 513, 0, 8000), (12290, 300, 4000, 12290)]
 
 
 @pytest.mark.gpu
