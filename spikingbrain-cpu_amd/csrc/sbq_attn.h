@@ -32,11 +32,12 @@
 #pragma once
 
 #include "sbq_common.h"
+#include "sbq_dma.h"
 
 namespace sbq {
 
 constexpr int kAttnWaves = 4;
-constexpr int kTileSlots = 64, kTileWaves = 8;  // attn_tile_kernel: slots per step, waves per workgroup at most
+constexpr int kTileSlots = 64;  // attn_tile_kernel: slots per step
 
 struct AttnArgs {
   const void *q, *k, *v, *kn, *vn;
@@ -52,6 +53,8 @@ struct AttnArgs {
   float scale;                  // times log2(e), >= 0 (`neg`: q is negated instead)
   bool neg, qvec;               // qvec: q's rows take 16-byte loads
 };
+
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0) alone
 
 template <int CT>
 struct CElem {
@@ -483,17 +486,17 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 
 // The same for many rows (128 and more of a key head) over 2-byte caches of
 // 64 or 128 columns: a wave owns 32 rows, the workgroup's waves share every
-// tile of 64 slots through LDS, double-buffered (global -> LDS copies of the
-// next tile run under the products of this one), and 32x32x16 products halve
-// the operand reads per product.  K and V rows lie in LDS as in memory, their
+// tile of 64 slots through LDS (global -> LDS copies of the next NBUF - 1 tiles
+// run under the products of this one), and 32x32x16 products halve the operand
+// reads per product.  K and V rows lie in LDS as in memory, their
 // 16-byte pieces permuted by the row (source side: the copy writes lane after
 // lane), so that the operand reads of 32 rows meet all banks.  S^T and O^T as
 // above: lane (h, r) holds the scores of row r and the slots 8 (v / 4) + 4 h +
 // v % 4, which 16 at a time are the operand of V^T's product in that slot
 // order.  What bounds it: per 64 scores 32 cycles of products and some 30 of
 // exponentials and sums per SIMD, two waves of which overlap.
-template <int CT, int DP>
-__global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs a) {
+template <int CT, int DP, int NW, int NBUF>
+__global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
   typedef AttnMath<CT> Math;
   typedef typename Math::V V;
@@ -501,14 +504,14 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
   constexpr int TS = kTileSlots, KK = DP / 16, EV = DP / 32, CPR = DP / 8, ROWB = DP * 2;
   constexpr int TILEB = TS * ROWB, BUFB = 2 * TILEB;  // K then V
   constexpr float kNone = -__builtin_inff();
-  extern __shared__ __align__(16) uint8_t lds[];  // two tiles
+  extern __shared__ __align__(16) uint8_t lds[];  // NBUF tiles
   auto product = [](V x, V y, f32x16 z) {
     if constexpr (CT == XT_F16)
       return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
     else
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
   };
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, NW = blockDim.x >> 6, r = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.x % a.Hk, rtile = blockIdx.x / a.Hk % a.rtiles, split = blockIdx.x / a.Hk / a.rtiles;
   const int R = a.rep * a.T, row = (rtile * NW + w) * 32 + r, rowc = min(row, R - 1), tok = rowc / a.rep;
 
@@ -551,26 +554,40 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
     }
   }
 
-  // the next tile at or after b that some token sees (nb: none), and whether all see all of it
-  auto visible = [&](int b, bool& full) {
-    for (; b < nbc; b += a.splits) {
-      const int64_t sp = position(b);
-      if (__any(sp >= lo_min && sp <= hi_max)) {
-        full = __all(sp >= lo_max && sp <= hi_min);
-        return b;
-      }
-    }
-    full = false;
-    return b;
+  // The tiles of this workgroup that some token sees, in turn: `ahead` is the
+  // one looked at next, its positions on their way.
+  int ahead = split;
+  int64_t ahead_sp = position(ahead);
+  struct Tile {
+    int b;
+    bool full;  // every token sees every slot
   };
+  auto next_tile = [&]() -> Tile {
+    while (ahead < nbc) {
+      const int b = ahead;
+      const int64_t sp = ahead_sp;
+      ahead += a.splits;
+      if (ahead < nbc) ahead_sp = position(ahead);
+      if (__any(sp >= lo_min && sp <= hi_max)) return Tile{b, (bool)__all(sp >= lo_max && sp <= hi_min)};
+    }
+    const int b = ahead;  // the drafts, then none
+    ahead += a.splits;
+    return Tile{b < nb ? b : nb, false};
+  };
+  // Every call issues the same number of copies, so that counting them is
+  // enough to wait for a tile (past the last one it copies the last again).
+  constexpr int COPIES = BUFB / 1024 / NW;
+  static_assert(BUFB % (1024 * NW) == 0, "whole copies per wave");
   auto copy_tile = [&](int b, int buf) {
+    b = min(b, nb - 1);
     const bool fresh = b >= nbc;
     const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
     const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
     const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
     const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
-    for (int q = w; q < BUFB / 1024; q += NW) {  // 64 pieces of 16 bytes a wave
-      const int piece = q * 64 + lane, val = piece >= TS * CPR, u = piece & (TS * CPR - 1), s = u / CPR;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {  // 64 pieces of 16 bytes a wave
+      const int q = i * NW + w, piece = q * 64 + lane, val = q >= TILEB / 1024, u = piece & (TS * CPR - 1), s = u / CPR;
       const T* const src = (val ? vp : kp) + min(base + s, last) * ss + ((u ^ s) & (CPR - 1)) * 8;
       __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(lds + buf * BUFB + q * 1024),
                                        16, 0, 0);
@@ -582,13 +599,25 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
 #pragma unroll
   for (int e = 0; e < EV; ++e) o[e] = (f32x16)(0.0f);
 
-  bool full, next_full = false;
-  int b = visible(split, full), buf = 0;
-  if (b < nb) copy_tile(b, 0);
-  while (b < nb) {
-    __syncthreads();  // this tile has arrived; everyone is done with the other buffer
-    const int next = visible(b + a.splits, next_full);
-    if (next < nb) copy_tile(next, buf ^ 1);
+  Tile tile[NBUF];  // tile[0]: the current one
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i) {
+    tile[i] = next_tile();
+    copy_tile(tile[i].b, i);
+  }
+  int buf = 0;
+  while (tile[0].b < nb) {
+    // This wave's copies of the current tile have arrived (loads return in
+    // order; at most those of the NBUF - 2 tiles after it are under way), and
+    // behind the barrier everyone's; everyone is also done with the tile
+    // before, whose place the next copy takes.
+    wait_vmcnt<(NBUF - 2) * COPIES>();
+    wait_lds();
+    barrier_nofence();
+    tile[NBUF - 1] = next_tile();
+    copy_tile(tile[NBUF - 1].b, (buf + NBUF - 1) % NBUF);
+    const int b = tile[0].b;
+    const bool full = tile[0].full;
     const bool fresh = b >= nbc;
     const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
     const uint8_t* const kt = lds + buf * BUFB;
@@ -700,8 +729,11 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
         }
       }
     }
-    b = next, full = next_full, buf ^= 1;
+    buf = (buf + 1) % NBUF;
+#pragma unroll
+    for (int i = 0; i < NBUF - 1; ++i) tile[i] = tile[i + 1];
   }
+  wait_vmcnt<0>();  // (no copy outlives the workgroup's LDS)
 
   l += __shfl_xor(l, 32, 64);
   if (row >= R) return;
@@ -734,7 +766,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
 // memory.  A workgroup takes SB slots and every row; its waves share the
 // (key head, 16-row tile) pairs, keep the slots' keys in registers while the
 // head stays, and add up in wave order.
-constexpr int kWeightWaves = 8;
+constexpr int kWeightWaves = 8, kWeightTileRows = 64;  // rows of a key head from which Q goes through LDS
 template <int CT, bool M16, int DP, int MODE>
 __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs a, float* weight) {
   typedef typename XElem<CT>::T T;
@@ -826,6 +858,112 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
   }
 }
 
+// The same for many rows over 2-byte caches of 64 or 128 columns: a wave
+// takes 32 slots (their keys of one head in registers, the next head's on
+// their way), the workgroup's 8 waves share every 32 rows of Q through LDS, so
+// that Q is read once per 256 slots.
+template <int CT, int DP>
+__global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(AttnArgs a, float* weight) {
+  typedef typename XElem<CT>::T T;
+  typedef typename AttnMath<CT>::V V;
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  constexpr int KK = DP / 16, CPR = DP / 8, ROWB = DP * 2, TILEB = 32 * ROWB, NBUF = 4;
+  constexpr int PARTS = TILEB / 1024;  // of one tile of Q: a wave each (with 64 columns two waves copy the same)
+  __shared__ __align__(16) uint8_t lds[NBUF * TILEB];
+  __shared__ __align__(16) float2 lds_ml[NBUF][32];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+  const int R = a.rep * a.T, tiles = (R + 31) / 32, units = a.Hk * tiles;
+  const int base = blockIdx.x * (32 * kWeightWaves) + w * 32, last = a.slots - 1;
+
+  const int64_t sp = base + r <= last ? a.slot_pos[base + r] : -1;
+  int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
+  for (int t = lane; t < a.T; t += 64) {
+    const int64_t hi = a.q_pos[t], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+    lo_min = min(lo_min, lo), lo_max = max(lo_max, lo), hi_min = min(hi_min, hi), hi_max = max(hi_max, hi);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lo_min = min(lo_min, (int64_t)__shfl_xor((long long)lo_min, o, 64));
+    lo_max = max(lo_max, (int64_t)__shfl_xor((long long)lo_max, o, 64));
+    hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
+    hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
+  }
+  const bool any = __any(sp >= lo_min && sp <= hi_max), full = __all(sp >= lo_max && sp <= hi_min);
+  if (!__syncthreads_or(any)) return;
+
+  // Rows of unit u (key head, 32 rows), and their maxima and sums: two copies by every wave.
+  auto copy_rows = [&](int u) {
+    const int to = u % NBUF;
+    u = min(u, units - 1);
+    const int part = w % PARTS, piece = part * 64 + lane, s = piece / CPR, row = min(u % tiles * 32 + s, R - 1);
+    const T* const src = (const T*)a.q + (int64_t)(row / a.rep) * a.q_st +
+                         (int64_t)(u / tiles * a.rep + row % a.rep) * a.q_sh + ((piece ^ s) & (CPR - 1)) * 8;
+    __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(lds + to * TILEB + part * 1024),
+                                     16, 0, 0);
+    const float* const ml = (const float*)(a.row_ml + (int64_t)(u / tiles) * R + min(u % tiles * 32 + (lane >> 1), R - 1));
+    __builtin_amdgcn_global_load_lds((const void*)(ml + (lane & 1)), (__attribute__((address_space(3))) void*)lds_ml[to], 4, 0, 0);
+  };
+  auto load_k = [&](int kvh, V (&kf)[KK]) {
+    const T* const kr = (const T*)a.k + (int64_t)min(kvh, a.Hk - 1) * a.k_sh + min(base + r, last) * a.k_ss;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const V*)(kr + kk * 16 + h * 8);
+  };
+
+  V kf[KK], kn[KK];
+  load_k(0, kn);
+  float acc[16] = {};
+  for (int u = 0; u < NBUF - 1; ++u) copy_rows(u);
+  for (int u = 0; u < units; ++u) {
+    const int row = u % tiles * 32 + r, rc = min(row, R - 1);
+    // as in attn_tile_kernel: this unit's rows are there, the place of the unit before is free
+    wait_vmcnt<(NBUF - 2) * 2>();
+    wait_lds();
+    barrier_nofence();
+    if (u % tiles == 0) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) kf[kk] = kn[kk];
+      load_k(u / tiles + 1, kn);
+    }
+    copy_rows(u + NBUF - 1);
+    const float2 ml = lds_ml[u % NBUF][r];
+    if (!any) continue;
+    const uint8_t* const qr = lds + u % NBUF * TILEB + r * ROWB;
+    f32x16 s = (f32x16)(0.0f);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      V qf = *(const V*)(qr + (((kk * 2 + h) ^ r) & (CPR - 1)) * 16);
+      if constexpr (CT == XT_F16)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], qf, s, 0, 0, 0);
+      else
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf, s, 0, 0, 0);
+    }
+    const float scale = a.neg ? -a.scale : a.scale, inv = row < R ? ml.y : 0.0f;
+    if (full) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)), inv, acc[v]);
+    } else {
+      const int64_t hi = a.q_pos[rc / a.rep], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int at = base + (v / 4) * 8 + 4 * h + v % 4;
+        const int64_t pos = at <= last ? a.slot_pos[at] : -1;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)) * inv;
+        acc[v] += row < R && pos >= lo && pos <= hi ? p : 0.0f;
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // (no copy outlives the workgroup's LDS)
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    float x = acc[v];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) x += __shfl_xor(x, o, 64);
+    const int at = base + (v / 4) * 8 + 4 * h + v % 4;
+    if (r == 0 && at <= last) weight[at] += x;
+  }
+}
+
 // One attention launch of a configuration; defined per pair (cache type,
 // 2-byte products) in the files that instantiate the kernel.
 template <int CT, bool M16, int DP>
@@ -846,17 +984,28 @@ int launch_attn_dp(const AttnArgs& a, int mode, int RT, hipStream_t st) {
   return e == hipSuccess ? 0 : -5;
 }
 
-template <int CT, int DP>
-int launch_tile_dp(const AttnArgs& a, int waves, hipStream_t st) {
-  constexpr int lds = 2 * 2 * kTileSlots * DP * 2;
-  attn_tile_kernel<CT, DP><<<dim3((unsigned)(a.Hk * a.rtiles * a.splits)), waves * 64, lds, st>>>(a);
+template <int CT, int DP, int NW>
+int launch_tile_nw(const AttnArgs& a, hipStream_t st) {
+  // one workgroup of 8 waves or two of 4 on a CU
+  constexpr int NBUF = NW == 8 ? 4 : DP == 64 ? 4 : 2, lds = NBUF * 2 * kTileSlots * DP * 2;
+  attn_tile_kernel<CT, DP, NW, NBUF><<<dim3((unsigned)(a.Hk * a.rtiles * a.splits)), NW * 64, lds, st>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : -5;
+}
+template <int CT, int DP>
+int launch_tile_dp(const AttnArgs& a, int waves, hipStream_t st) {
+  return waves == 4 ? launch_tile_nw<CT, DP, 4>(a, st) : launch_tile_nw<CT, DP, 8>(a, st);
 }
 
 template <int CT, bool M16, int DP>
 int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st) {
   constexpr int SB = M16 ? 32 : 16, threads = kWeightWaves * 64;
+  if constexpr (M16 && DP <= 128) {
+    if (mode == 2 && a.qvec && a.rep * a.T >= kWeightTileRows) {
+      attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, 0, st>>>(a, weight);
+      return hipGetLastError() == hipSuccess ? 0 : -5;
+    }
+  }
   const dim3 grid((unsigned)((a.slots + SB - 1) / SB));
   if (mode == 2)
     attn_weight_kernel<CT, M16, DP, 2><<<grid, threads, 0, st>>>(a, weight);

@@ -81,7 +81,7 @@ AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, boo
   int64_t groups = kAttnGroups, each = kAttnWaves, SB = m16 ? 32 : 16;
   if (vec && m16 && DP <= 128 && R >= kTileRows) {
     const int64_t waves = (R + 31) / 32;
-    p.RT = -(int)(waves < kTileWaves ? waves : kTileWaves);
+    p.RT = waves <= 4 ? -4 : -8;
     p.rtiles = (int)((waves - p.RT - 1) / -p.RT);
     groups = kTileGroups / -p.RT;
     each = 1, SB = kTileSlots;
