@@ -495,6 +495,10 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 // v % 4, which 16 at a time are the operand of V^T's product in that slot
 // order.  What bounds it: per 64 scores 32 cycles of products and some 30 of
 // exponentials and sums per SIMD, two waves of which overlap.
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 template <int CT, int DP, int NW, int NBUF>
 __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
@@ -516,10 +520,6 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
   const int R = a.rep * a.T, row = (rtile * NW + w) * 32 + r, rowc = min(row, R - 1), tok = rowc / a.rep;
 
   const int nbc = (a.slots + TS - 1) / TS, nb = nbc + (a.Tn + TS - 1) / TS;
-  auto position = [&](int b) -> int64_t {
-    const int s = b * TS + lane;
-    return s < a.slots ? a.slot_pos[s] : -1;
-  };
   // what the tokens of the whole call see (the workgroup's skipping is uniform)
   int64_t lo_min = INT64_MAX, lo_max = 0, hi_min = INT64_MAX, hi_max = -1;
   for (int t = lane; t < a.T; t += 64) {
@@ -533,7 +533,6 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
     hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
   }
-  const int64_t hi = a.q_pos[tok], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
 
   // Q^T operand: lane (h, r) holds columns 16 kk + 8 h + 0..7 of row r
   V qf[KK];
@@ -554,43 +553,39 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     }
   }
 
-  // The tiles of this workgroup that some token sees, in turn: `ahead` is the
-  // one looked at next, its positions on their way.
-  int ahead = split;
-  int64_t ahead_sp = position(ahead);
-  struct Tile {
-    int b;
-    bool full;  // every token sees every slot
-  };
-  auto next_tile = [&]() -> Tile {
-    while (ahead < nbc) {
-      const int b = ahead;
-      const int64_t sp = ahead_sp;
-      ahead += a.splits;
-      if (ahead < nbc) ahead_sp = position(ahead);
-      if (__any(sp >= lo_min && sp <= hi_max)) return Tile{b, (bool)__all(sp >= lo_max && sp <= hi_min)};
-    }
-    const int b = ahead;  // the drafts, then none
-    ahead += a.splits;
-    return Tile{b < nb ? b : nb, false};
-  };
-  // Every call issues the same number of copies, so that counting them is
-  // enough to wait for a tile (past the last one it copies the last again).
+  // Copies of a tile: COPIES pieces of 16 bytes a lane, the same number by
+  // every call, so that counting them is enough to wait for a tile.
   constexpr int COPIES = BUFB / 1024 / NW;
   static_assert(BUFB % (1024 * NW) == 0, "whole copies per wave");
-  auto copy_tile = [&](int b, int buf) {
-    b = min(b, nb - 1);
-    const bool fresh = b >= nbc;
-    const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
-    const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
-    const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
-    const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
+  static_assert(COPIES % 2 == 0, "as many of K as of V");
+  uint32_t piece_at[COPIES / 2];  // bytes from a tile's start to the lane's pieces, the same in K and V
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) {  // 64 pieces of 16 bytes a wave
-      const int q = i * NW + w, piece = q * 64 + lane, val = q >= TILEB / 1024, u = piece & (TS * CPR - 1), s = u / CPR;
-      const T* const src = (val ? vp : kp) + min(base + s, last) * ss + ((u ^ s) & (CPR - 1)) * 8;
-      __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(lds + buf * BUFB + q * 1024),
-                                       16, 0, 0);
+  for (int i = 0; i < COPIES / 2; ++i) {
+    const int u = (i * NW + w) * 64 + lane, s = u / CPR;
+    piece_at[i] = (uint32_t)(s * a.k_ss + ((u ^ s) & (CPR - 1)) * 8) * 2;
+  }
+  const bool near = a.k_ss < (1 << 23);  // (the offsets fit 32 bits)
+  auto copy_tile = [&](int b, int buf) {
+    uint8_t* const to = lds + buf * BUFB + w * 1024;
+    if (near && (b + 1) * TS <= a.slots) {
+      const int64_t first = (int64_t)kvh * a.k_sh + (int64_t)b * TS * a.k_ss;
+      const uint8_t* const kp = (const uint8_t*)((const T*)a.k + first);
+      const uint8_t* const vp = (const uint8_t*)((const T*)a.v + first);
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)((i < COPIES / 2 ? kp : vp) + piece_at[i % (COPIES / 2)]),
+                                         (__attribute__((address_space(3))) void*)(to + i * NW * 1024), 16, 0, 0);
+    } else {  // the cache's end, or drafts: slots past the last one are the last one again
+      const bool fresh = b >= nbc;
+      const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
+      const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int q = i * NW + w, u = (q * 64 + lane) & (TS * CPR - 1), s = u / CPR;
+        const void* const p = q >= TILEB / 1024 ? (fresh ? a.vn : a.v) : (fresh ? a.kn : a.k);
+        const T* const src = (const T*)p + head + min(base + s, last) * ss + ((u ^ s) & (CPR - 1)) * 8;
+        __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(to + i * NW * 1024), 16, 0, 0);
+      }
     }
   };
 
@@ -599,115 +594,92 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
   for (int e = 0; e < EV; ++e) o[e] = (f32x16)(0.0f);
 
-  Tile tile[NBUF];  // tile[0]: the current one
+  // The lane's K piece 0 of a tile's first 32 slots and its V piece of slot 4 h
+  // of the first 16.  Its other pieces lie at offsets that differ from these
+  // in the permuted bits alone: one exclusive or each.
+  const uint32_t k0 = r * ROWB + ((h ^ r) & (CPR - 1)) * 16;
+  const uint32_t v0 = TILEB + 4 * h * ROWB + ((((r * EV * 2) >> 4) ^ 4 * h) & (CPR - 1)) * 16 + (r * EV * 2 & 15);
+  // 32 slots of tile b, which lie from `at` on in LDS; FULL: every row sees all of them.
+  auto half = [&](int b, uint32_t at, auto FULL) {
+    constexpr bool kFull = decltype(FULL)::value;
+    f32x16 s = (f32x16)(0.0f);
 #pragma unroll
-  for (int i = 0; i < NBUF - 1; ++i) {
-    tile[i] = next_tile();
-    copy_tile(tile[i].b, i);
-  }
-  int buf = 0;
-  while (tile[0].b < nb) {
-    // This wave's copies of the current tile have arrived (loads return in
-    // order; at most those of the NBUF - 2 tiles after it are under way), and
-    // behind the barrier everyone's; everyone is also done with the tile
-    // before, whose place the next copy takes.
-    wait_vmcnt<(NBUF - 2) * COPIES>();
-    wait_lds();
-    barrier_nofence();
-    tile[NBUF - 1] = next_tile();
-    copy_tile(tile[NBUF - 1].b, (buf + NBUF - 1) % NBUF);
-    const int b = tile[0].b;
-    const bool full = tile[0].full;
-    const bool fresh = b >= nbc;
-    const int base = (fresh ? b - nbc : b) * TS, last = (fresh ? a.Tn : a.slots) - 1;
-    const uint8_t* const kt = lds + buf * BUFB;
-    const uint8_t* const vt = kt + TILEB;
-#pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
-      f32x16 s = (f32x16)(0.0f);
-      {
-        const uint8_t* const kr = kt + (sub * 32 + r) * ROWB;
+    for (int kk = 0; kk < KK; ++kk) s = product(*(const V*)(lds + ((at + k0) ^ kk * 32)), qf[kk], s);
+    uint32_t seen = 0;
+    float mx = kNone;
+    if constexpr (kFull) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const V kf = *(const V*)(kr + (((kk * 2 + h) ^ (sub * 32 + r)) & (CPR - 1)) * 16);
-          s = product(kf, qf[kk], s);
-        }
-      }
-      uint32_t seen = 0;
-      float mx = kNone;
-      if (full) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) mx = __builtin_fmaxf(mx, s[v]);
-      } else {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int at = base + sub * 32 + (v / 4) * 8 + 4 * h + v % 4;
-          bool ok = at <= last;
-          if (ok && !fresh) {
-            const int64_t sp = a.slot_pos[at];
-            ok = sp >= lo && sp <= hi;
-          } else if (ok) {
-            ok = a.tree ? a.tree[(int64_t)tok * a.tree_ld + at] != 0 : at <= tok;
-            ok = ok && (a.window == 0 || a.q_pos[at] > hi - a.window);
-          }
-          seen |= ok ? 1u << v : 0u;
-          mx = ok ? __builtin_fmaxf(mx, s[v]) : mx;
-        }
-      }
-      mx *= a.scale;
-      if (__any(mx > m)) {
-        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float up = __builtin_fmaxf(m, mx);
-        const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - up);
-        m = up;
-        l *= alpha;
-#pragma unroll
-        for (int e = 0; e < EV; ++e) o[e] *= alpha;
-      }
-      const float from = m == kNone ? 0.0f : m;
+      for (int v = 0; v < 16; ++v) mx = __builtin_fmaxf(mx, s[v]);
+    } else {
+      const bool fresh = b >= nbc;
+      const int base = (fresh ? b - nbc : b) * TS + (at & (TILEB - 1) ? 32 : 0), last = (fresh ? a.Tn : a.slots) - 1;
+      const int64_t hi = a.q_pos[tok], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.scale, -from));
-        if (!full) p = seen >> v & 1 ? p : 0.0f;
-        s[v] = p;
-        l += p;
+        const int sl = base + (v / 4) * 8 + 4 * h + v % 4;
+        bool ok = sl <= last;
+        if (ok && !fresh) {
+          const int64_t sp = a.slot_pos[sl];
+          ok = sp >= lo && sp <= hi;
+        } else if (ok) {
+          ok = a.tree ? a.tree[(int64_t)tok * a.tree_ld + sl] != 0 : sl <= tok;
+          ok = ok && (a.window == 0 || a.q_pos[sl] > hi - a.window);
+        }
+        seen |= ok ? 1u << v : 0u;
+        mx = ok ? __builtin_fmaxf(mx, s[v]) : mx;
       }
-      // V^T's operand for 16 slots: 8 of the lane's slots, EV columns each
-      auto v_words = [&](int kc, uint32_t (&vw)[8][EV / 2]) {
+    }
+    mx *= a.scale;
+    if (__any(mx > m)) {
+      mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float up = __builtin_fmaxf(m, mx);
+      const float alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+      m = up;
+      l *= alpha;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int sl = sub * 32 + kc * 16 + (j >> 2) * 8 + 4 * h + (j & 3);
-          const int byte = r * EV * 2;
-          const uint8_t* const at = vt + sl * ROWB + (((byte >> 4) ^ sl) & (CPR - 1)) * 16 + (byte & 15);
-          if constexpr (EV == 4) {
-            const u32x2 x = *(const u32x2*)at;
-            vw[j][0] = x.x, vw[j][1] = x.y;
-          } else {
-            vw[j][0] = *(const uint32_t*)at;
-          }
+      for (int e = 0; e < EV; ++e) o[e] *= alpha;
+    }
+    const float from = m == kNone ? 0.0f : m;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.scale, -from));
+      if constexpr (!kFull) p = seen >> v & 1 ? p : 0.0f;
+      s[v] = p;
+      l += p;
+    }
+    // V^T's operand for 16 slots: 8 of the lane's slots, EV columns each
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      uint32_t vw[8][EV / 2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int sl = (j >> 2) * 8 + (j & 3);  // beyond 4 h
+        const uint8_t* const x = lds + ((at + v0) ^ (sl & (CPR - 1)) * 16) + (kc * 16 + sl) * ROWB;
+        if constexpr (EV == 4) {
+          const u32x2 y = *(const u32x2*)x;
+          vw[j][0] = y.x, vw[j][1] = y.y;
+        } else {
+          vw[j][0] = *(const uint32_t*)x;
         }
-      };
+      }
+      bool odd = false;
+      if constexpr (!kFull) {
 #pragma unroll
-      for (int kc = 0; kc < 2; ++kc) {
-        uint32_t vw[8][EV / 2];
-        v_words(kc, vw);
-        bool odd = false;
-        if (!full) {
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int e = 0; e < EV / 2; ++e) odd |= Odd2<CT>::any(vw[j][e]);
+        odd = __any(odd);
+      }
+      V pf;
 #pragma unroll
-            for (int e = 0; e < EV / 2; ++e) odd |= Odd2<CT>::any(vw[j][e]);
-          odd = __any(odd);
-        }
-        V pf;
+      for (int j = 0; j < 8; ++j) pf[j] = (T)s[kc * 8 + j];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pf[j] = (T)s[kc * 8 + j];
+      for (int e = 0; e < EV; ++e) {
+        u32x4 t;
 #pragma unroll
-        for (int e = 0; e < EV; ++e) {
-          u32x4 t;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        for (int j = 0; j < 4; ++j)
+          t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        if constexpr (!kFull) {
           if (odd) {
 #pragma unroll 1
             for (int kind = 0; kind < 3; ++kind) {
@@ -725,15 +697,74 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) t[j] = Odd2<CT>::finite(t[j]);
           }
-          o[e] = product(__builtin_bit_cast(V, t), pf, o[e]);
         }
+        o[e] = product(__builtin_bit_cast(V, t), pf, o[e]);
       }
     }
-    buf = (buf + 1) % NBUF;
+  };
+
+  // The workgroup's tiles, 64 at a time: one bit each for "some token sees a
+  // slot" and "every token sees every slot" (the waves look at 64 / NW each;
+  // positions loaded between the copies would drain them).
+#pragma unroll 1
+  for (int64_t b0 = split; b0 < nb; b0 += (int64_t)64 * a.splits) {
+    uint64_t some = 0, every = 0;
 #pragma unroll
-    for (int i = 0; i < NBUF - 1; ++i) tile[i] = tile[i + 1];
+    for (int i = 0; i < 64 / NW; ++i) {
+      const int64_t b = b0 + (int64_t)(w * (64 / NW) + i) * a.splits, at = b * TS + lane;
+      const int64_t sp = at < a.slots ? a.slot_pos[at] : -1;
+      const bool any = (b >= nbc && b < nb) || (b < nbc && __any(sp >= lo_min && sp <= hi_max));
+      some |= (uint64_t)any << i;
+      every |= (uint64_t)(b < nbc && __all(sp >= lo_max && sp <= hi_min)) << i;
+    }
+    uint64_t* const flags = (uint64_t*)lds;  // [2][NW]
+    __syncthreads();                         // (the tiles before are done with)
+    if (lane == 0) flags[w] = some, flags[NW + w] = every;
+    __syncthreads();
+    some = every = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      some |= flags[k] << (k * (64 / NW));
+      every |= flags[NW + k] << (k * (64 / NW));
+    }
+    some = (uint64_t)__builtin_amdgcn_readfirstlane((int)(some >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)some);
+    every = (uint64_t)__builtin_amdgcn_readfirstlane((int)(every >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)every);
+    if (!some) continue;
+    __syncthreads();  // (the flags are read)
+
+    uint64_t coming = some;  // tiles not copied yet
+    int last_copied = 0;
+    auto copy_next = [&](int buf) {  // (past the last one it copies that again)
+      if (coming) last_copied = __builtin_ctzll(coming);
+      coming &= coming - 1;
+      copy_tile((int)(b0 + (int64_t)last_copied * a.splits), buf);
+    };
+#pragma unroll
+    for (int i = 0; i < NBUF - 1; ++i) copy_next(i);
+    int buf = 0;
+#pragma unroll 1
+    for (; some; some &= some - 1, buf = (buf + 1) % NBUF) {
+      // This wave's copies of the current tile have arrived (loads return in
+      // order; those of the NBUF - 2 tiles after it may be under way), and
+      // behind the barrier everyone's; everyone is also done with the tile
+      // before, whose place the next copy takes.
+      wait_vmcnt<(NBUF - 2) * COPIES>();
+      wait_lds();
+      barrier_nofence();
+      copy_next((buf + NBUF - 1) % NBUF);
+      const int j = __builtin_ctzll(some), b = (int)(b0 + (int64_t)j * a.splits);
+      const uint32_t at = buf * BUFB;
+      if (every >> j & 1) {
+        half(b, at, Bool<true>{});
+        __builtin_amdgcn_sched_barrier(0);  // (both halves at once do not fit the registers)
+        half(b, at + 32 * ROWB, Bool<true>{});
+      } else {
+#pragma unroll 1
+        for (int sub = 0; sub < 2; ++sub) half(b, at + sub * 32 * ROWB, Bool<false>{});
+      }
+    }
+    wait_vmcnt<0>();  // (no copy outlives its buffer)
   }
-  wait_vmcnt<0>();  // (no copy outlives the workgroup's LDS)
 
   l += __shfl_xor(l, 32, 64);
   if (row >= R) return;
@@ -867,12 +898,13 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
   typedef typename XElem<CT>::T T;
   typedef typename AttnMath<CT>::V V;
   typedef float f32x16 __attribute__((ext_vector_type(16)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
   constexpr int KK = DP / 16, CPR = DP / 8, ROWB = DP * 2, TILEB = 32 * ROWB, NBUF = 4;
   constexpr int PARTS = TILEB / 1024;  // of one tile of Q: a wave each (with 64 columns two waves copy the same)
-  __shared__ __align__(16) uint8_t lds[NBUF * TILEB];
-  __shared__ __align__(16) float2 lds_ml[NBUF][32];
+  // (one dynamic object: before a read of a static one the compiler waits for every copy under way)
+  extern __shared__ __align__(16) uint8_t lds[];  // NBUF tiles of rows, then their maxima and sums
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-  const int R = a.rep * a.T, tiles = (R + 31) / 32, units = a.Hk * tiles;
+  const int R = a.rep * a.T;
   const int base = blockIdx.x * (32 * kWeightWaves) + w * 32, last = a.slots - 1;
 
   const int64_t sp = base + r <= last ? a.slot_pos[base + r] : -1;
@@ -891,43 +923,58 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
   const bool any = __any(sp >= lo_min && sp <= hi_max), full = __all(sp >= lo_max && sp <= hi_min);
   if (!__syncthreads_or(any)) return;
 
-  // Rows of unit u (key head, 32 rows), and their maxima and sums: two copies by every wave.
-  auto copy_rows = [&](int u) {
-    const int to = u % NBUF;
-    u = min(u, units - 1);
-    const int part = w % PARTS, piece = part * 64 + lane, s = piece / CPR, row = min(u % tiles * 32 + s, R - 1);
-    const T* const src = (const T*)a.q + (int64_t)(row / a.rep) * a.q_st +
-                         (int64_t)(u / tiles * a.rep + row % a.rep) * a.q_sh + ((piece ^ s) & (CPR - 1)) * 8;
-    __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)(lds + to * TILEB + part * 1024),
-                                     16, 0, 0);
-    const float* const ml = (const float*)(a.row_ml + (int64_t)(u / tiles) * R + min(u % tiles * 32 + (lane >> 1), R - 1));
-    __builtin_amdgcn_global_load_lds((const void*)(ml + (lane & 1)), (__attribute__((address_space(3))) void*)lds_ml[to], 4, 0, 0);
+  // The rows that are copied next, 32 of a key head: two copies by every wave,
+  // of its part of the rows and of all rows' maxima and sums.
+  const int part = w % PARTS, piece = part * 64 + lane, rs = piece / CPR, chunk = (piece ^ rs) & (CPR - 1);
+  const int r0 = min(rs, R - 1), t0 = r0 / a.rep, j0 = r0 % a.rep, tl = (R - 1) / a.rep, jl = (R - 1) % a.rep;
+  int c_head = 0, c_row = rs, c_tok = t0, c_sub = j0, c_buf = 0;  // (sub: the row's head among the key head's)
+  auto copy_rows = [&]() {
+    const bool in = c_row < R;
+    const T* const src = (const T*)a.q + (int64_t)(in ? c_tok : tl) * a.q_st +
+                         (int64_t)(c_head * a.rep + (in ? c_sub : jl)) * a.q_sh + chunk * 8;
+    __builtin_amdgcn_global_load_lds((const void*)src,
+                                     (__attribute__((address_space(3))) void*)(lds + c_buf * TILEB + part * 1024), 16, 0, 0);
+    const float* const ml = (const float*)(a.row_ml + (int64_t)c_head * R + min(c_row - rs + (lane >> 1), R - 1));
+    __builtin_amdgcn_global_load_lds((const void*)(ml + (lane & 1)),
+                                     (__attribute__((address_space(3))) void*)(lds + NBUF * TILEB + c_buf * 256), 4, 0, 0);
+    c_buf = (c_buf + 1) % NBUF;
+    c_row += 32, c_tok += 32 / a.rep, c_sub += 32 % a.rep;
+    if (c_sub >= a.rep) c_sub -= a.rep, ++c_tok;
+    if (c_row - rs >= R) {  // the next key head; past the last one its rows once more
+      c_head = min(c_head + 1, a.Hk - 1);
+      c_row = rs, c_tok = t0, c_sub = j0;
+    }
   };
-  auto load_k = [&](int kvh, V (&kf)[KK]) {
-    const T* const kr = (const T*)a.k + (int64_t)min(kvh, a.Hk - 1) * a.k_sh + min(base + r, last) * a.k_ss;
+  const T* kr = (const T*)a.k + min(base + r, last) * a.k_ss + h * 8;  // the lane's slot, of the head loaded next
+  auto load_k = [&](V (&to)[KK]) {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const V*)(kr + kk * 16 + h * 8);
+    for (int kk = 0; kk < KK; ++kk) to[kk] = *(const V*)(kr + kk * 16);
   };
 
   V kf[KK], kn[KK];
-  load_k(0, kn);
+  load_k(kn);
   float acc[16] = {};
-  for (int u = 0; u < NBUF - 1; ++u) copy_rows(u);
-  for (int u = 0; u < units; ++u) {
-    const int row = u % tiles * 32 + r, rc = min(row, R - 1);
-    // as in attn_tile_kernel: this unit's rows are there, the place of the unit before is free
+  const float scale = a.neg ? -a.scale : a.scale;
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i) copy_rows();
+  int buf = 0;
+#pragma unroll 1
+  for (int kvh = 0; kvh < a.Hk; ++kvh) {
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) kf[kk] = kn[kk];
+    kr += kvh + 1 < a.Hk ? a.k_sh : 0;
+    load_k(kn);
+#pragma unroll 1
+  for (int row = r; row - r < R; row += 32, buf = (buf + 1) % NBUF) {
+    const int rc = min(row, R - 1);
+    // as in attn_tile_kernel: these rows are there, the place of the rows before is free
     wait_vmcnt<(NBUF - 2) * 2>();
     wait_lds();
     barrier_nofence();
-    if (u % tiles == 0) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) kf[kk] = kn[kk];
-      load_k(u / tiles + 1, kn);
-    }
-    copy_rows(u + NBUF - 1);
-    const float2 ml = lds_ml[u % NBUF][r];
+    copy_rows();
+    const f32x2 ml = *(const f32x2*)(lds + NBUF * TILEB + buf * 256 + r * 8);
     if (!any) continue;
-    const uint8_t* const qr = lds + u % NBUF * TILEB + r * ROWB;
+    const uint8_t* const qr = lds + buf * TILEB + r * ROWB;
     f32x16 s = (f32x16)(0.0f);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -937,7 +984,7 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
       else
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf, s, 0, 0, 0);
     }
-    const float scale = a.neg ? -a.scale : a.scale, inv = row < R ? ml.y : 0.0f;
+    const float inv = row < R ? ml.y : 0.0f;
     if (full) {
 #pragma unroll
       for (int v = 0; v < 16; ++v)
@@ -952,6 +999,7 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
         acc[v] += row < R && pos >= lo && pos <= hi ? p : 0.0f;
       }
     }
+  }
   }
   __builtin_amdgcn_s_waitcnt(0);  // (no copy outlives the workgroup's LDS)
 #pragma unroll
@@ -1002,7 +1050,7 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
   constexpr int SB = M16 ? 32 : 16, threads = kWeightWaves * 64;
   if constexpr (M16 && DP <= 128) {
     if (mode == 2 && a.qvec && a.rep * a.T >= kWeightTileRows) {
-      attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, 0, st>>>(a, weight);
+      attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, 4 * (32 * DP * 2 + 256), st>>>(a, weight);
       return hipGetLastError() == hipSuccess ? 0 : -5;
     }
   }
