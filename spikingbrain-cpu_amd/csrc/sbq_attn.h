@@ -39,6 +39,11 @@ namespace sbq {
 constexpr int kAttnWaves = 4;
 constexpr int kTileSlots = 64;  // attn_tile_kernel: slots per step
 
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
 struct AttnArgs {
   const void *q, *k, *v, *kn, *vn;
   const int64_t *slot_pos, *q_pos;
@@ -112,6 +117,43 @@ __device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
 }
 
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
+
+// Which of N slots token `tok` sees, one bit each; slot(v) is the v-th one's
+// index in the cache (or among the drafts), valid up to `last`.  All loads
+// before the first comparison: one after the other they would cost a memory
+// latency each.
+template <int N, class F>
+__device__ __forceinline__ uint32_t sees(const AttnArgs& a, bool fresh, int tok, int last, F slot) {
+  const int64_t hi = a.q_pos[tok], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+  uint32_t bits = 0;
+  if (!fresh) {
+    int64_t sp[N];
+#pragma unroll
+    for (int v = 0; v < N; ++v) sp[v] = a.slot_pos[min(slot(v), last)];
+#pragma unroll
+    for (int v = 0; v < N; ++v) bits |= slot(v) <= last && sp[v] >= lo && sp[v] <= hi ? 1u << v : 0u;
+    return bits;
+  }
+  if (a.tree) {
+    uint8_t t[N];
+#pragma unroll
+    for (int v = 0; v < N; ++v) t[v] = a.tree[(int64_t)tok * a.tree_ld + min(slot(v), last)];
+#pragma unroll
+    for (int v = 0; v < N; ++v) bits |= slot(v) <= last && t[v] ? 1u << v : 0u;
+  } else {
+#pragma unroll
+    for (int v = 0; v < N; ++v) bits |= slot(v) <= tok ? 1u << v : 0u;  // (tok <= last)
+  }
+  if (a.window > 0) {
+    int64_t qp[N];
+#pragma unroll
+    for (int v = 0; v < N; ++v) qp[v] = a.q_pos[min(slot(v), last)];
+#pragma unroll
+    for (int v = 0; v < N; ++v)
+      if (qp[v] <= hi - a.window) bits &= ~(1u << v);
+  }
+  return bits;
+}
 
 // Infinities and NaN of V.  Where a row does not see every slot of a block,
 // such a value must not reach it as 0 * inf: the block's product takes the
@@ -252,14 +294,12 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
     for (int f = 0; f < NF; ++f) o[i][f] = (f32x4)(0.0f);
   }
 
-  while (b < nb) {
-    const bool fresh = b >= nbc;
+  // Block b of the cache (b < nbc) or of the drafts; FULL: of the cache, and
+  // every row sees all of it.
+  auto block = [&](int b, auto FULL) {
+    constexpr bool full = decltype(FULL)::value != 0;
+    const bool fresh = !full && b >= nbc;
     const int base = (fresh ? b - nbc : b) * SB, last = (fresh ? a.Tn : a.slots) - 1;
-    const bool any = fresh || __any(sp >= lo_min && sp <= hi_max);
-    const bool full = !fresh && __all(sp >= lo_max && sp <= hi_min);
-    b += W;
-    if (b < nbc) sp = position(b);
-    if (!any) continue;
     const int64_t ss = fresh ? a.n_ss : a.k_ss, head = (int64_t)kvh * (fresh ? a.n_sh : a.k_sh);
     const T* const kp = (const T*)(fresh ? a.kn : a.k) + head;
     const T* const vp = (const T*)(fresh ? a.vn : a.v) + head;
@@ -280,7 +320,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
     }
 
     float p[RT][SUB][4];
-    uint32_t seen[RT];  // bit st * 4 + v, where not every row sees every slot (= V's slot j of the lane)
+    uint32_t seen[RT] = {};  // bit st * 4 + v (= V's slot j of the lane), where not every row sees every slot
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
 #pragma unroll
@@ -300,29 +340,17 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
         for (int v = 0; v < 4; ++v) p[i][st][v] = s[v];
       }
       float mx = kNone;
-      if (full) {
+      if constexpr (full) {
 #pragma unroll
         for (int st = 0; st < SUB; ++st)
 #pragma unroll
           for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, p[i][st][v]);
       } else {
-        seen[i] = 0;
+        seen[i] = sees<SUB * 4>(a, fresh, tok[i], last, [&](int v) { return base + (v >> 2) * 16 + 4 * g + (v & 3); });
 #pragma unroll
         for (int st = 0; st < SUB; ++st)
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int s = base + st * 16 + 4 * g + v;
-            bool ok = s <= last;
-            if (ok && !fresh) {
-              const int64_t at = a.slot_pos[s];
-              ok = at >= lo[i] && at <= hi[i];
-            } else if (ok) {
-              ok = a.tree ? a.tree[(int64_t)tok[i] * a.tree_ld + s] != 0 : s <= tok[i];
-              ok = ok && (a.window == 0 || a.q_pos[s] > hi[i] - a.window);
-            }
-            seen[i] |= ok ? 1u << (st * 4 + v) : 0u;
-            mx = ok ? __builtin_fmaxf(mx, p[i][st][v]) : mx;
-          }
+          for (int v = 0; v < 4; ++v) mx = seen[i] >> (st * 4 + v) & 1 ? __builtin_fmaxf(mx, p[i][st][v]) : mx;
       }
       mx *= a.scale;
       if (__any(mx > m[i])) {
@@ -341,14 +369,14 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][st][v], a.scale, -from));
-          if (!full) e = seen[i] >> (st * 4 + v) & 1 ? e : 0.0f;
+          if constexpr (!full) e = seen[i] >> (st * 4 + v) & 1 ? e : 0.0f;
           p[i][st][v] = e;
           l[i] += e;
         }
     }
 
     bool odd = false;  // infinities or NaN in V, and rows that do not see every slot
-    if (!full) {
+    if constexpr (!full) {
 #pragma unroll
       for (int j = 0; j < VS; ++j)
 #pragma unroll
@@ -377,7 +405,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             t[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e / 2], vw[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-          if (odd) {
+          if (!full && odd) {
 #pragma unroll 1
             for (int kind = 0; kind < 3; ++kind) {
               u32x4 ones;
@@ -410,7 +438,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
           for (int e = 0; e < EV; ++e) {
             float x = (float)vf[j][db].v[e];
-            if (odd) {
+            if (!full && odd) {
 #pragma unroll 1
               for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
@@ -428,6 +456,29 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
               o[i][db * EV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i][0][j], o[i][db * EV + e], 0, 0, 0);
           }
     }
+  };
+
+  // The wave's blocks, 64 at a time: those that every row sees whole, then the
+  // others; a loop each, so that the masks of the second cost the first no
+  // registers.
+#pragma unroll 1
+  while (b < nb) {
+    const int b0 = b;
+    uint64_t later = 0;
+#pragma unroll 1
+    for (int i = 0; i < 64 && b < nb; ++i) {
+      const int at = b;
+      const bool fresh = at >= nbc, any = fresh || __any(sp >= lo_min && sp <= hi_max);
+      const bool full = !fresh && __all(sp >= lo_max && sp <= hi_min);
+      b += W;
+      if (b < nbc) sp = position(b);
+      if (full)
+        block(at, Const<1>{});
+      else
+        later |= (uint64_t)any << i;
+    }
+#pragma unroll 1
+    for (; later; later &= later - 1) block(b0 + __builtin_ctzll(later) * W, Const<0>{});
   }
 
   // the workgroup's waves joined, one row tile at a time
@@ -495,10 +546,6 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 // v % 4, which 16 at a time are the operand of V^T's product in that slot
 // order.  What bounds it: per 64 scores 32 cycles of products and some 30 of
 // exponentials and sums per SIMD, two waves of which overlap.
-template <bool B>
-struct Bool {
-  static constexpr bool value = B;
-};
 template <int CT, int DP, int NW, int NBUF>
 __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
@@ -594,17 +641,22 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
   for (int e = 0; e < EV; ++e) o[e] = (f32x16)(0.0f);
 
-  // The lane's K piece 0 of a tile's first 32 slots and its V piece of slot 4 h
-  // of the first 16.  Its other pieces lie at offsets that differ from these
-  // in the permuted bits alone: one exclusive or each.
-  const uint32_t k0 = r * ROWB + ((h ^ r) & (CPR - 1)) * 16;
-  const uint32_t v0 = TILEB + 4 * h * ROWB + ((((r * EV * 2) >> 4) ^ 4 * h) & (CPR - 1)) * 16 + (r * EV * 2 & 15);
+  // Offsets in a tile of the lane's K pieces of its first 32 slots and V pieces
+  // of its first 16 (the permutation depends on the slot modulo CPR alone).
+  uint32_t koff[KK], voff[8];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) koff[kk] = r * ROWB + (((kk * 2 + h) ^ r) & (CPR - 1)) * 16;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int sl = (j >> 2) * 8 + 4 * h + (j & 3), byte = r * EV * 2;
+    voff[j] = TILEB + sl * ROWB + (((byte >> 4) ^ sl) & (CPR - 1)) * 16 + (byte & 15);
+  }
   // 32 slots of tile b, which lie from `at` on in LDS; FULL: every row sees all of them.
   auto half = [&](int b, uint32_t at, auto FULL) {
-    constexpr bool kFull = decltype(FULL)::value;
+    constexpr bool kFull = decltype(FULL)::value != 0;
     f32x16 s = (f32x16)(0.0f);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s = product(*(const V*)(lds + ((at + k0) ^ kk * 32)), qf[kk], s);
+    for (int kk = 0; kk < KK; ++kk) s = product(*(const V*)(lds + at + koff[kk]), qf[kk], s);
     uint32_t seen = 0;
     float mx = kNone;
     if constexpr (kFull) {
@@ -613,21 +665,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     } else {
       const bool fresh = b >= nbc;
       const int base = (fresh ? b - nbc : b) * TS + (at & (TILEB - 1) ? 32 : 0), last = (fresh ? a.Tn : a.slots) - 1;
-      const int64_t hi = a.q_pos[tok], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+      seen = sees<16>(a, fresh, tok, last, [&](int v) { return base + (v / 4) * 8 + 4 * h + v % 4; });
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int sl = base + (v / 4) * 8 + 4 * h + v % 4;
-        bool ok = sl <= last;
-        if (ok && !fresh) {
-          const int64_t sp = a.slot_pos[sl];
-          ok = sp >= lo && sp <= hi;
-        } else if (ok) {
-          ok = a.tree ? a.tree[(int64_t)tok * a.tree_ld + sl] != 0 : sl <= tok;
-          ok = ok && (a.window == 0 || a.q_pos[sl] > hi - a.window);
-        }
-        seen |= ok ? 1u << v : 0u;
-        mx = ok ? __builtin_fmaxf(mx, s[v]) : mx;
-      }
+      for (int v = 0; v < 16; ++v) mx = seen >> v & 1 ? __builtin_fmaxf(mx, s[v]) : mx;
     }
     mx *= a.scale;
     if (__any(mx > m)) {
@@ -637,7 +677,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       m = up;
       l *= alpha;
 #pragma unroll
-      for (int e = 0; e < EV; ++e) o[e] *= alpha;
+      for (int e = 0; e < EV; ++e)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          float x = o[e][v];
+          asm("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(alpha));  // (in place: the compiler would copy all of o for the branch)
+          o[e][v] = x;
+        }
     }
     const float from = m == kNone ? 0.0f : m;
 #pragma unroll
@@ -653,8 +699,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       uint32_t vw[8][EV / 2];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int sl = (j >> 2) * 8 + (j & 3);  // beyond 4 h
-        const uint8_t* const x = lds + ((at + v0) ^ (sl & (CPR - 1)) * 16) + (kc * 16 + sl) * ROWB;
+        const uint8_t* const x = lds + at + kc * 16 * ROWB + voff[j];
         if constexpr (EV == 4) {
           const u32x2 y = *(const u32x2*)x;
           vw[j][0] = y.x, vw[j][1] = y.y;
@@ -703,19 +748,24 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     }
   };
 
-  // The workgroup's tiles, 64 at a time: one bit each for "some token sees a
-  // slot" and "every token sees every slot" (the waves look at 64 / NW each;
-  // positions loaded between the copies would drain them).
-#pragma unroll 1
-  for (int64_t b0 = split; b0 < nb; b0 += (int64_t)64 * a.splits) {
+  // 64 of the workgroup's tiles from b0 on, one bit each: `part` of them are
+  // seen by some token, `whole` by every token in every slot (the waves look at
+  // 64 / NW each; positions loaded between the copies would drain them).
+  auto look = [&](int64_t b0, uint64_t& part, uint64_t& whole) {
     uint64_t some = 0, every = 0;
+    int64_t sp[64 / NW];  // (all loads before the first comparison)
 #pragma unroll
     for (int i = 0; i < 64 / NW; ++i) {
-      const int64_t b = b0 + (int64_t)(w * (64 / NW) + i) * a.splits, at = b * TS + lane;
-      const int64_t sp = at < a.slots ? a.slot_pos[at] : -1;
-      const bool any = (b >= nbc && b < nb) || (b < nbc && __any(sp >= lo_min && sp <= hi_max));
-      some |= (uint64_t)any << i;
-      every |= (uint64_t)(b < nbc && __all(sp >= lo_max && sp <= hi_min)) << i;
+      const int64_t at = (b0 + (int64_t)(w * (64 / NW) + i) * a.splits) * TS + lane;
+      sp[i] = a.slot_pos[at < a.slots ? at : a.slots - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < 64 / NW; ++i) {
+      const int64_t b = b0 + (int64_t)(w * (64 / NW) + i) * a.splits;
+      const int64_t pos = b * TS + lane < a.slots ? sp[i] : -1;
+      const bool any = __any(pos >= lo_min && pos <= hi_max), all = __all(pos >= lo_max && pos <= hi_min);
+      some |= (uint64_t)(b < nbc ? any : b < nb) << i;
+      every |= (uint64_t)(b < nbc && all) << i;
     }
     uint64_t* const flags = (uint64_t*)lds;  // [2][NW]
     __syncthreads();                         // (the tiles before are done with)
@@ -727,12 +777,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       some |= flags[k] << (k * (64 / NW));
       every |= flags[NW + k] << (k * (64 / NW));
     }
-    some = (uint64_t)__builtin_amdgcn_readfirstlane((int)(some >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)some);
-    every = (uint64_t)__builtin_amdgcn_readfirstlane((int)(every >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)every);
-    if (!some) continue;
     __syncthreads();  // (the flags are read)
+    part = (uint64_t)__builtin_amdgcn_readfirstlane((int)(some >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)some);
+    whole = (uint64_t)__builtin_amdgcn_readfirstlane((int)(every >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)every);
+  };
 
-    uint64_t coming = some;  // tiles not copied yet
+  // Tiles that every row sees whole, then the others: one loop each, so that
+  // the masks of the second cost the first no registers.
+#pragma unroll 1
+  for (int64_t b0 = split; b0 < nbc; b0 += (int64_t)64 * a.splits) {
+    uint64_t part, todo;
+    look(b0, part, todo);
+    if (!todo) continue;
+    uint64_t coming = todo;  // tiles not copied yet
     int last_copied = 0;
     auto copy_next = [&](int buf) {  // (past the last one it copies that again)
       if (coming) last_copied = __builtin_ctzll(coming);
@@ -741,9 +798,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     };
 #pragma unroll
     for (int i = 0; i < NBUF - 1; ++i) copy_next(i);
-    int buf = 0;
-#pragma unroll 1
-    for (; some; some &= some - 1, buf = (buf + 1) % NBUF) {
+    auto step = [&](auto BUF) {  // (a constant buffer, whose offsets are then the reads' own)
+      constexpr int buf = decltype(BUF)::value;
       // This wave's copies of the current tile have arrived (loads return in
       // order; those of the NBUF - 2 tiles after it may be under way), and
       // behind the barrier everyone's; everyone is also done with the tile
@@ -752,18 +808,37 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       wait_lds();
       barrier_nofence();
       copy_next((buf + NBUF - 1) % NBUF);
-      const int j = __builtin_ctzll(some), b = (int)(b0 + (int64_t)j * a.splits);
-      const uint32_t at = buf * BUFB;
-      if (every >> j & 1) {
-        half(b, at, Bool<true>{});
-        __builtin_amdgcn_sched_barrier(0);  // (both halves at once do not fit the registers)
-        half(b, at + 32 * ROWB, Bool<true>{});
-      } else {
+      half(0, buf * BUFB, Const<1>{});
+      __builtin_amdgcn_sched_barrier(0);  // (both halves at once do not fit the registers)
+      half(0, buf * BUFB + 32 * ROWB, Const<1>{});
+      todo &= todo - 1;
+      return todo != 0;
+    };
+    if constexpr (NBUF == 2) {
 #pragma unroll 1
-        for (int sub = 0; sub < 2; ++sub) half(b, at + sub * 32 * ROWB, Bool<false>{});
+      while (step(Const<0>{}) && step(Const<1>{})) {
+      }
+    } else {
+#pragma unroll 1
+      while (step(Const<0>{}) && step(Const<1>{}) && step(Const<2>{}) && step(Const<3>{})) {
       }
     }
     wait_vmcnt<0>();  // (no copy outlives its buffer)
+  }
+#pragma unroll 1
+  for (int64_t b0 = split; b0 < nb; b0 += (int64_t)64 * a.splits) {
+    uint64_t part, whole;
+    look(b0, part, whole);
+#pragma unroll 1
+    for (part &= ~whole; part; part &= part - 1) {
+      const int b = (int)(b0 + (int64_t)__builtin_ctzll(part) * a.splits);
+      __syncthreads();  // (the tile before is done with)
+      copy_tile(b, 0);
+      wait_vmcnt<0>();
+      __syncthreads();
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) half(b, sub * 32 * ROWB, Const<0>{});
+    }
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -835,7 +910,8 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
     QRow<CT, M16, DP, MODE> qr;
     qr.load(a, kvh, rc, g);
     const float2 ml = a.row_ml[(int64_t)kvh * R + rc];
-    const int64_t hi = a.q_pos[rc / a.rep], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+    uint32_t seen = r < R ? ~0u : 0u;
+    if (!full) seen &= sees<SUB * 4>(a, false, rc / a.rep, last, [&](int v) { return base + (v >> 2) * 16 + 4 * g + (v & 3); });
     if (kvh != held) {
       held = kvh;
 #pragma unroll
@@ -861,13 +937,7 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.scale, -ml.x)) * ml.y;
-        bool ok = r < R;
-        if (!full) {
-          const int at = base + st * 16 + 4 * g + v;
-          const int64_t pos = at <= last ? a.slot_pos[at] : -1;
-          ok = ok && pos >= lo && pos <= hi;
-        }
-        acc[st][v] += ok ? p : 0.0f;
+        acc[st][v] += seen >> (st * 4 + v) & 1 ? p : 0.0f;
       }
     }
   }
@@ -990,13 +1060,11 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
       for (int v = 0; v < 16; ++v)
         acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)), inv, acc[v]);
     } else {
-      const int64_t hi = a.q_pos[rc / a.rep], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+      const uint32_t seen = sees<16>(a, false, rc / a.rep, last, [&](int v) { return base + (v / 4) * 8 + 4 * h + v % 4; });
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const int at = base + (v / 4) * 8 + 4 * h + v % 4;
-        const int64_t pos = at <= last ? a.slot_pos[at] : -1;
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)) * inv;
-        acc[v] += row < R && pos >= lo && pos <= hi ? p : 0.0f;
+        acc[v] += row < R && (seen >> v & 1) ? p : 0.0f;
       }
     }
   }
