@@ -56,7 +56,7 @@ struct AttnArgs {
   int64_t window;               // 0: none
   int T, Hk, rep, D, slots, Tn, splits, rtiles, qt;
   float scale;                  // times log2(e), >= 0 (`neg`: q is negated instead)
-  bool neg, qvec;               // qvec: q's rows take 16-byte loads
+  bool neg, qvec, ovec;         // q's rows take 16-byte loads, out's rows stores of 4 elements
 };
 
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }  // lgkmcnt(0) alone
@@ -525,9 +525,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
           const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
           const int t = (r0 + rr) / a.rep, h = kvh * a.rep + (r0 + rr) % a.rep;
           const int64_t out = (int64_t)t * a.o_st + (int64_t)h * a.o_sh + d;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < a.D) store_y(a.out, a.qt, out + e, sum[e] * inv);
+          if (d < a.D) store_y4(a.out, a.qt, out, sum * inv, a.ovec && d + 4 <= a.D, a.D - d);
           if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
         }
       }
@@ -842,28 +840,89 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
   }
 
   l += __shfl_xor(l, 32, 64);
+  const int tile = rtile * NW + w;  // of 32 rows
+  if (tile * 32 >= R) return;
+  if (a.splits > 1) {  // as they lie in the registers: [head][tile][split][v][lane][EV], maxima and sums [32]
+    const int64_t at = ((int64_t)kvh * (a.rtiles * NW) + tile) * a.splits + split;
+    typedef float Row __attribute__((ext_vector_type(EV)));
+    Row* const to = (Row*)a.part_o + at * 1024 + lane;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      Row x;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) x[e] = o[e][v];
+      to[v * 64] = x;
+    }
+    if (h == 0) a.part_ml[at * 32 + r] = make_float2(m, l);
+    return;
+  }
   if (row >= R) return;
-  const int64_t at = (int64_t)kvh * R + row;
-  const bool joined = a.splits > 1;
-  const float from = m == kNone ? 0.0f : m, inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const int64_t out = (int64_t)tok * a.o_st + (int64_t)(kvh * a.rep + row % a.rep) * a.o_sh;
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     const int d = ((v / 4) * 8 + 4 * h + v % 4) * EV;
-#pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      if (joined)
-        a.part_o[(at * a.splits + split) * DP + d + e] = o[e][v];
-      else
-        store_y(a.out, a.qt, out + d + e, o[e][v] * inv);
+    if constexpr (EV == 4) {
+      store_y4(a.out, a.qt, out + d, (f32x4){o[0][v], o[1][v], o[2][v], o[3][v]} * inv, a.ovec, 4);
+    } else {
+      store_y(a.out, a.qt, out + d, o[0][v] * inv);
+      store_y(a.out, a.qt, out + d + 1, o[1][v] * inv);
     }
   }
-  if (h == 0) {
-    if (joined)
-      a.part_ml[at * a.splits + split] = make_float2(m, l);
-    else if (a.row_ml)
-      a.row_ml[at] = make_float2(from, inv);
+  if (h == 0 && a.row_ml) a.row_ml[(int64_t)kvh * R + row] = make_float2(m == kNone ? 0.0f : m, inv);
+}
+
+// The splits of attn_tile_kernel's rows joined: a wave per (key head, tile of
+// 32 rows, v), which reads the partial sums as they were written.
+template <int DP, int NW>
+__global__ __launch_bounds__(64) void attn_tile_join_kernel(AttnArgs a) {
+  constexpr int EV = DP / 32;
+  typedef float Row __attribute__((ext_vector_type(EV)));
+  const int R = a.rep * a.T, tiles = (R + 31) / 32, lane = threadIdx.x, r = lane & 31, h = lane >> 5;
+  const int v = blockIdx.x & 15, tile = (blockIdx.x >> 4) % tiles, kvh = (blockIdx.x >> 4) / tiles;
+  const int64_t at = ((int64_t)kvh * (a.rtiles * NW) + tile) * a.splits;
+  const Row* const from = (const Row*)a.part_o + at * 1024 + v * 64 + lane;
+  const float2* const ml = a.part_ml + at * 32 + r;
+  float top = -__builtin_inff(), l = 0.0f;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = ml[min(s0 + k, a.splits - 1) * 32].x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, x[k]);
   }
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  Row sum = (Row)(0.0f);
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {
+    Row x[4];
+    float2 y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = min(s0 + k, a.splits - 1);
+      x[k] = from[(int64_t)s * 1024];
+      y[k] = ml[s * 32];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = __builtin_amdgcn_exp2f(y[k].x - base);
+      if (s0 + k < a.splits && y[k].y != 0.0f) {  // (a split that saw nothing adds nothing)
+        sum += x[k] * f;
+        l += y[k].y * f;
+      }
+    }
+  }
+  const int row = tile * 32 + r;
+  if (row >= R) return;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const int64_t out = (int64_t)(row / a.rep) * a.o_st + (int64_t)(kvh * a.rep + row % a.rep) * a.o_sh +
+                      ((v / 4) * 8 + 4 * h + v % 4) * EV;
+  if constexpr (EV == 4) {
+    store_y4(a.out, a.qt, out, sum * inv, a.ovec, 4);
+  } else {
+    store_y(a.out, a.qt, out, sum[0] * inv);
+    store_y(a.out, a.qt, out + 1, sum[1] * inv);
+  }
+  if (v == 0 && h == 0 && a.row_ml) a.row_ml[(int64_t)kvh * R + row] = make_float2(base, inv);
 }
 
 // weight[s] += sum over the rows that see slot s of exp2(score - maximum) /
@@ -1105,8 +1164,10 @@ int launch_tile_nw(const AttnArgs& a, hipStream_t st) {
   // one workgroup of 8 waves or two of 4 on a CU
   constexpr int NBUF = NW == 8 ? 4 : DP == 64 ? 4 : 2, lds = NBUF * 2 * kTileSlots * DP * 2;
   attn_tile_kernel<CT, DP, NW, NBUF><<<dim3((unsigned)(a.Hk * a.rtiles * a.splits)), NW * 64, lds, st>>>(a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : -5;
+  if (hipGetLastError() != hipSuccess) return -5;
+  if (a.splits > 1)
+    attn_tile_join_kernel<DP, NW><<<dim3((unsigned)(a.Hk * ((a.rep * a.T + 31) / 32) * 16)), 64, 0, st>>>(a);
+  return hipGetLastError() == hipSuccess ? 0 : -5;
 }
 template <int CT, int DP>
 int launch_tile_dp(const AttnArgs& a, int waves, hipStream_t st) {

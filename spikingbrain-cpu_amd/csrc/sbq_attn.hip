@@ -60,9 +60,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const int kvh = (int)(at / R), r = (int)(at % R);
   const int64_t out = (int64_t)(r / a.rep) * a.o_st + (int64_t)(kvh * a.rep + r % a.rep) * a.o_sh + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (d + e < a.D) store_y(a.out, a.qt, out + e, sum[e] * inv);
+  if (d < a.D) store_y4(a.out, a.qt, out, sum * inv, a.ovec && d + 4 <= a.D, a.D - d);
   if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
 }
 
@@ -74,6 +72,7 @@ int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct AttnPlan {
   int RT, rtiles, splits;  // RT: row tiles per wave, or -(waves) of attn_tile_kernel
+  int64_t rows;            // rows of a key head that partial sums are kept for
 };
 // vec: rows of exactly DP columns by 16-byte loads; m16: 2-byte products.
 AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, bool vec, bool m16) {
@@ -89,6 +88,7 @@ AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, boo
     p.RT = vec && R > 16 && (m16 || DP < 256) ? 2 : 1;  // (two tiles of 256 fp32 columns do not fit the registers)
     p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
   }
+  p.rows = p.RT < 0 ? (int64_t)p.rtiles * -p.RT * 32 : R;
   const int64_t room = groups / (Hk * p.rtiles) < 1 ? 1 : groups / (Hk * p.rtiles);
   const int64_t blocks = (slots + SB - 1) / SB + (Tn + SB - 1) / SB;
   const int64_t most = (blocks + each * room - 1) / (each * room);  // blocks of a wave (of a workgroup) at most
@@ -101,15 +101,15 @@ int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 }  // namespace
 
 int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t slots, bool weight) {
-  const int64_t R = heads / Hk * T, rows = Hk * R;
-  int64_t splits = 1;
-  for (int way = 0; way < 8; ++way) {  // types, alignment and drafts are not known here
-    const int64_t s = attn_plan(R, Hk, slots, way & 4 ? T : 0, attn_dp(D), way & 1, way & 2).splits;
-    splits = s > splits ? s : splits;
-  }
+  const int64_t R = heads / Hk * T;
   int64_t n = 0;
-  if (splits > 1) n += round256(rows * splits * attn_dp(D) * 4) + round256(rows * splits * 8);
-  if (weight) n += round256(rows * 8);
+  for (int way = 0; way < 8; ++way) {  // types, alignment and drafts are not known here
+    const AttnPlan p = attn_plan(R, Hk, slots, way & 4 ? T : 0, attn_dp(D), way & 1, way & 2);
+    const int64_t parts = Hk * p.rows * p.splits;
+    const int64_t need = p.splits > 1 ? round256(parts * attn_dp(D) * 4) + round256(parts * 8) : 0;
+    n = need > n ? need : n;
+  }
+  if (weight) n += round256(Hk * R * 8);
   return n;
 }
 
@@ -137,12 +137,13 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
   const int64_t eq = c.qt == XT_F32 ? 4 : 2;
   a.qvec = (m16 || c.qt == XT_F32) && c.D * eq % 16 == 0 && (uintptr_t)c.q % 16 == 0 && c.q_st * eq % 16 == 0 &&
            c.q_sh * eq % 16 == 0;
+  a.ovec = (uintptr_t)c.out % (4 * eq) == 0 && c.o_st % 4 == 0 && c.o_sh % 4 == 0;
   uint8_t* ws = (uint8_t*)c.ws;
   if (p.splits > 1) {
     a.part_o = (float*)ws;
-    ws += round256(Hk * R * p.splits * DP * 4);
+    ws += round256(Hk * p.rows * p.splits * DP * 4);
     a.part_ml = (float2*)ws;
-    ws += round256(Hk * R * p.splits * 8);
+    ws += round256(Hk * p.rows * p.splits * 8);
   }
   if (c.weight) a.row_ml = (float2*)ws;
   auto launch = [&](float* weight) {
@@ -152,7 +153,7 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
   };
   int rc = launch(nullptr);
   if (rc) return rc;
-  if (p.splits > 1) {
+  if (p.splits > 1 && p.RT > 0) {  // (attn_tile_kernel's launch joins its own)
     const unsigned grid = (unsigned)(Hk * R);
     if (DP == 64)
       attn_join_kernel<64><<<grid, 256, 0, st>>>(a);
