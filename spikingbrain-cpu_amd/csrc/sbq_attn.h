@@ -649,12 +649,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
     const int sl = (j >> 2) * 8 + 4 * h + (j & 3), byte = r * EV * 2;
     voff[j] = TILEB + sl * ROWB + (((byte >> 4) ^ sl) & (CPR - 1)) * 16 + (byte & 15);
   }
-  // 32 slots of tile b, which lie from `at` on in LDS; FULL: every row sees all of them.
-  auto half = [&](int b, uint32_t at, auto FULL) {
-    constexpr bool kFull = decltype(FULL)::value != 0;
+  // Scores of the 32 slots that lie from `at` on in LDS.
+  auto scores = [&](uint32_t at) {
     f32x16 s = (f32x16)(0.0f);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) s = product(*(const V*)(lds + at + koff[kk]), qf[kk], s);
+    return s;
+  };
+  // ... of tile b, taken in; FULL: every row sees all of them.
+  auto half = [&](f32x16 s, int b, uint32_t at, auto FULL) {
+    constexpr bool kFull = decltype(FULL)::value != 0;
     uint32_t seen = 0;
     float mx = kNone;
     if constexpr (kFull) {
@@ -806,9 +810,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       wait_lds();
       barrier_nofence();
       copy_next((buf + NBUF - 1) % NBUF);
-      half(0, buf * BUFB, Const<1>{});
-      __builtin_amdgcn_sched_barrier(0);  // (both halves at once do not fit the registers)
-      half(0, buf * BUFB + 32 * ROWB, Const<1>{});
+      // the second half's scores are on their way while the first is taken in
+      const f32x16 s0 = scores(buf * BUFB), s1 = scores(buf * BUFB + 32 * ROWB);
+      half(s0, 0, buf * BUFB, Const<1>{});
+      __builtin_amdgcn_sched_barrier(0);  // (both at once do not fit the registers)
+      half(s1, 0, buf * BUFB + 32 * ROWB, Const<1>{});
       todo &= todo - 1;
       return todo != 0;
     };
@@ -835,7 +841,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_tile_kernel(AttnArgs a) {
       wait_vmcnt<0>();
       __syncthreads();
 #pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) half(b, sub * 32 * ROWB, Const<0>{});
+      for (int sub = 0; sub < 2; ++sub) half(scores(sub * 32 * ROWB), b, sub * 32 * ROWB, Const<0>{});
     }
   }
 
@@ -931,7 +937,8 @@ __global__ __launch_bounds__(64) void attn_tile_join_kernel(AttnArgs a) {
 // memory.  A workgroup takes SB slots and every row; its waves share the
 // (key head, 16-row tile) pairs, keep the slots' keys in registers while the
 // head stays, and add up in wave order.
-constexpr int kWeightWaves = 8, kWeightTileRows = 64;  // rows of a key head from which Q goes through LDS
+constexpr int kWeightWaves = 8, kWeightBufs = 4;
+constexpr int kWeightTileRows = 64;  // rows of a key head from which Q goes through LDS
 template <int CT, bool M16, int DP, int MODE>
 __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs a, float* weight) {
   typedef typename XElem<CT>::T T;
@@ -1020,16 +1027,17 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
 
 // The same for many rows over 2-byte caches of 64 or 128 columns: a wave
 // takes 32 slots (their keys of one head in registers, the next head's on
-// their way), the workgroup's 8 waves share every 32 rows of Q through LDS, so
-// that Q is read once per 256 slots.
+// their way), the workgroup's 8 waves share every 64 rows of Q through LDS, so
+// that Q is read once per 256 slots, and work on the two halves of the rows
+// side by side.
 template <int CT, int DP>
 __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(AttnArgs a, float* weight) {
   typedef typename XElem<CT>::T T;
   typedef typename AttnMath<CT>::V V;
   typedef float f32x16 __attribute__((ext_vector_type(16)));
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  constexpr int KK = DP / 16, CPR = DP / 8, ROWB = DP * 2, TILEB = 32 * ROWB, NBUF = 4;
-  constexpr int PARTS = TILEB / 1024;  // of one tile of Q: a wave each (with 64 columns two waves copy the same)
+  constexpr int KK = DP / 16, CPR = DP / 8, ROWB = DP * 2, TILEB = 64 * ROWB, NBUF = kWeightBufs;
+  constexpr int PARTS = TILEB / 1024 / kWeightWaves;  // copies of a wave, of 64 pieces of 16 bytes
   // (one dynamic object: before a read of a static one the compiler waits for every copy under way)
   extern __shared__ __align__(16) uint8_t lds[];  // NBUF tiles of rows, then their maxima and sums
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
@@ -1052,26 +1060,41 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
   const bool any = __any(sp >= lo_min && sp <= hi_max), full = __all(sp >= lo_max && sp <= hi_min);
   if (!__syncthreads_or(any)) return;
 
-  // The rows that are copied next, 32 of a key head: two copies by every wave,
-  // of its part of the rows and of all rows' maxima and sums.
-  const int part = w % PARTS, piece = part * 64 + lane, rs = piece / CPR, chunk = (piece ^ rs) & (CPR - 1);
-  const int r0 = min(rs, R - 1), t0 = r0 / a.rep, j0 = r0 % a.rep, tl = (R - 1) / a.rep, jl = (R - 1) % a.rep;
-  int c_head = 0, c_row = rs, c_tok = t0, c_sub = j0, c_buf = 0;  // (sub: the row's head among the key head's)
+  // The rows that are copied next, 64 of a key head, and their maxima and sums
+  // (by every wave, so that all have as many copies under way).
+  int rs[PARTS], chunk[PARTS], t0[PARTS], j0[PARTS], c_tok[PARTS], c_sub[PARTS];  // (sub: the row's head among the key head's)
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int piece = (i * kWeightWaves + w) * 64 + lane;
+    rs[i] = piece / CPR, chunk[i] = ((piece ^ rs[i]) & (CPR - 1)) * 8;
+    c_tok[i] = t0[i] = min(rs[i], R - 1) / a.rep, c_sub[i] = j0[i] = min(rs[i], R - 1) % a.rep;
+  }
+  const int tl = (R - 1) / a.rep, jl = (R - 1) % a.rep, dt = 64 / a.rep, dj = 64 % a.rep;
+  int c_head = 0, c_row = 0, c_buf = 0;
   auto copy_rows = [&]() {
-    const bool in = c_row < R;
-    const T* const src = (const T*)a.q + (int64_t)(in ? c_tok : tl) * a.q_st +
-                         (int64_t)(c_head * a.rep + (in ? c_sub : jl)) * a.q_sh + chunk * 8;
-    __builtin_amdgcn_global_load_lds((const void*)src,
-                                     (__attribute__((address_space(3))) void*)(lds + c_buf * TILEB + part * 1024), 16, 0, 0);
-    const float* const ml = (const float*)(a.row_ml + (int64_t)c_head * R + min(c_row - rs + (lane >> 1), R - 1));
-    __builtin_amdgcn_global_load_lds((const void*)(ml + (lane & 1)),
-                                     (__attribute__((address_space(3))) void*)(lds + NBUF * TILEB + c_buf * 256), 4, 0, 0);
-    c_buf = (c_buf + 1) % NBUF;
-    c_row += 32, c_tok += 32 / a.rep, c_sub += 32 % a.rep;
-    if (c_sub >= a.rep) c_sub -= a.rep, ++c_tok;
-    if (c_row - rs >= R) {  // the next key head; past the last one its rows once more
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const bool in = c_row + rs[i] < R;
+      const T* const src = (const T*)a.q + (int64_t)(in ? c_tok[i] : tl) * a.q_st +
+                           (int64_t)(c_head * a.rep + (in ? c_sub[i] : jl)) * a.q_sh + chunk[i];
+      __builtin_amdgcn_global_load_lds(
+          (const void*)src, (__attribute__((address_space(3))) void*)(lds + c_buf * TILEB + (i * kWeightWaves + w) * 1024), 16, 0, 0);
+      c_tok[i] += dt, c_sub[i] += dj;
+      if (c_sub[i] >= a.rep) c_sub[i] -= a.rep, ++c_tok[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float* const ml = (const float*)(a.row_ml + (int64_t)c_head * R + min(c_row + i * 32 + (lane >> 1), R - 1));
+      __builtin_amdgcn_global_load_lds((const void*)(ml + (lane & 1)),
+                                       (__attribute__((address_space(3))) void*)(lds + NBUF * TILEB + c_buf * 512 + i * 256), 4, 0, 0);
+    }
+    c_buf = c_buf + 1 == NBUF ? 0 : c_buf + 1;
+    c_row += 64;
+    if (c_row >= R) {  // the next key head; past the last one its rows once more
       c_head = min(c_head + 1, a.Hk - 1);
-      c_row = rs, c_tok = t0, c_sub = j0;
+      c_row = 0;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) c_tok[i] = t0[i], c_sub[i] = j0[i];
     }
   };
   const T* kr = (const T*)a.k + min(base + r, last) * a.k_ss + h * 8;  // the lane's slot, of the head loaded next
@@ -1094,39 +1117,47 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
     kr += kvh + 1 < a.Hk ? a.k_sh : 0;
     load_k(kn);
 #pragma unroll 1
-  for (int row = r; row - r < R; row += 32, buf = (buf + 1) % NBUF) {
-    const int rc = min(row, R - 1);
-    // as in attn_tile_kernel: these rows are there, the place of the rows before is free
-    wait_vmcnt<(NBUF - 2) * 2>();
-    wait_lds();
-    barrier_nofence();
-    copy_rows();
-    const f32x2 ml = *(const f32x2*)(lds + NBUF * TILEB + buf * 256 + r * 8);
-    if (!any) continue;
-    const uint8_t* const qr = lds + buf * TILEB + r * ROWB;
-    f32x16 s = (f32x16)(0.0f);
+    for (int row0 = 0; row0 < R; row0 += 64) {
+      // as in attn_tile_kernel: these rows are there, the place of the rows before is free
+      wait_vmcnt<(NBUF - 2) * (PARTS + 2)>();
+      wait_lds();
+      barrier_nofence();
+      copy_rows();
+      const uint8_t* const qt = lds + buf * TILEB + r * ROWB;
+      const uint8_t* const mt = lds + NBUF * TILEB + buf * 512 + r * 8;
+      buf = buf + 1 == NBUF ? 0 : buf + 1;
+      if (!any) continue;
+      f32x16 s[2] = {(f32x16)(0.0f), (f32x16)(0.0f)};
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      V qf = *(const V*)(qr + (((kk * 2 + h) ^ r) & (CPR - 1)) * 16);
-      if constexpr (CT == XT_F16)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], qf, s, 0, 0, 0);
-      else
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf, s, 0, 0, 0);
-    }
-    const float inv = row < R ? ml.y : 0.0f;
-    if (full) {
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)), inv, acc[v]);
-    } else {
-      const uint32_t seen = sees<16>(a, false, rc / a.rep, last, [&](int v) { return base + (v / 4) * 8 + 4 * h + v % 4; });
+        for (int i = 0; i < 2; ++i) {
+          const V qf = *(const V*)(qt + i * 32 * ROWB + (((kk * 2 + h) ^ r) & (CPR - 1)) * 16);
+          if constexpr (CT == XT_F16)
+            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], qf, s[i], 0, 0, 0);
+          else
+            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qf, s[i], 0, 0, 0);
+        }
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale, -ml.x)) * inv;
-        acc[v] += row < R && (seen >> v & 1) ? p : 0.0f;
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + i * 32 + r;
+        const f32x2 ml = *(const f32x2*)(mt + i * 256);
+        const float inv = row < R ? ml.y : 0.0f;
+        if (full) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], scale, -ml.x)), inv, acc[v]);
+        } else {
+          const uint32_t seen = sees<16>(a, false, min(row, R - 1) / a.rep, last,
+                                         [&](int v) { return base + (v / 4) * 8 + 4 * h + v % 4; });
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], scale, -ml.x)) * inv;
+            acc[v] += row < R && (seen >> v & 1) ? p : 0.0f;
+          }
+        }
       }
     }
-  }
   }
   __builtin_amdgcn_s_waitcnt(0);  // (no copy outlives the workgroup's LDS)
 #pragma unroll
@@ -1179,7 +1210,7 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
   constexpr int SB = M16 ? 32 : 16, threads = kWeightWaves * 64;
   if constexpr (M16 && DP <= 128) {
     if (mode == 2 && a.qvec && a.rep * a.T >= kWeightTileRows) {
-      attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, 4 * (32 * DP * 2 + 256), st>>>(a, weight);
+      attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, kWeightBufs * (64 * DP * 2 + 512), st>>>(a, weight);
       return hipGetLastError() == hipSuccess ? 0 : -5;
     }
   }
