@@ -65,30 +65,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 }
 
 constexpr int kAttnGroups = 512;    // workgroups aimed at
-constexpr int kTileGroups = 2048;   // waves aimed at by attn_tile_kernel: 8 per CU
-constexpr int64_t kTileRows = 128;  // rows of a key head from which it is taken
+// attn_tile_kernel: workgroups aimed at (one a CU), and the rows of a key head
+// and rows times slots from which it is taken.  8 key heads of 128 bf16
+// columns, 256 rows each: 65536 slots 122 us against attn_kernel's 185, 32768
+// 74 / 93, 8192 44 / 37; 512 rows: 8192 slots 49 / 58; 128 rows: 65536 slots
+// (with 4 waves) 120 / 106.
+constexpr int kTileGroups = 256;
+constexpr int64_t kTileRows = 256, kTileScores = 1 << 22;
 
 int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct AttnPlan {
-  int RT, rtiles, splits;  // RT: row tiles per wave, or -(waves) of attn_tile_kernel
+  int RT, rtiles, splits;  // RT: row tiles per wave, 0 for attn_tile_kernel
   int64_t rows;            // rows of a key head that partial sums are kept for
 };
 // vec: rows of exactly DP columns by 16-byte loads; m16: 2-byte products.
 AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, bool vec, bool m16) {
   AttnPlan p;
   int64_t groups = kAttnGroups, each = kAttnWaves, SB = m16 ? 32 : 16;
-  if (vec && m16 && DP <= 128 && R >= kTileRows) {
-    const int64_t waves = (R + 31) / 32;
-    p.RT = waves <= 4 ? -4 : -8;
-    p.rtiles = (int)((waves - p.RT - 1) / -p.RT);
-    groups = kTileGroups / -p.RT;
+  if (vec && m16 && DP <= 128 && R >= kTileRows && R * slots >= kTileScores) {
+    p.RT = 0;
+    p.rtiles = (int)((R + 32 * kTileWaves - 1) / (32 * kTileWaves));
+    groups = kTileGroups;
     each = 1, SB = kTileSlots;
   } else {
     p.RT = vec && R > 16 && (m16 || DP < 256) ? 2 : 1;  // (two tiles of 256 fp32 columns do not fit the registers)
     p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
   }
-  p.rows = p.RT < 0 ? (int64_t)p.rtiles * -p.RT * 32 : R;
+  p.rows = p.RT == 0 ? (int64_t)p.rtiles * kTileWaves * 32 : R;
   const int64_t room = groups / (Hk * p.rtiles) < 1 ? 1 : groups / (Hk * p.rtiles);
   const int64_t blocks = (slots + SB - 1) / SB + (Tn + SB - 1) / SB;
   const int64_t most = (blocks + each * room - 1) / (each * room);  // blocks of a wave (of a workgroup) at most
@@ -153,7 +157,7 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
   };
   int rc = launch(nullptr);
   if (rc) return rc;
-  if (p.splits > 1 && p.RT > 0) {  // (attn_tile_kernel's launch joins its own)
+  if (p.splits > 1 && p.RT != 0) {  // (attn_tile_kernel's launch joins its own)
     const unsigned grid = (unsigned)(Hk * R);
     if (DP == 64)
       attn_join_kernel<64><<<grid, 256, 0, st>>>(a);

@@ -63,21 +63,20 @@ def test_python_refuses_cpu_tensors():
 # the formula
 # ---------------------------------------------------------------------------
 def _formula(q, k, v, see, scale):
-    """(out, p) in 64 bits; see [T, slots]; a row that sees nothing is 0."""
+    """(out, p summed over heads, largest score) in 64 bits; see [T, slots]; a
+    row that sees nothing is 0."""
     T, H, D = q.shape
     rep = H // k.shape[1]
-    out, ps = torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(H, T, k.shape[0], dtype=torch.float64)
+    out, ps = torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(T, k.shape[0], dtype=torch.float64)
     xmax = 0.0
     for h in range(H):
         kh, vh, qh = k[:, h // rep].double(), v[:, h // rep].double(), q[:, h].double()
         z = (qh @ kh.t()) * scale
         xmax = max(xmax, float((qh.abs() @ kh.abs().t()).max()) * abs(scale))
-        for t in range(T):
-            at = see[t].nonzero()[:, 0]
-            if len(at):
-                p = torch.softmax(z[t, at], 0)
-                ps[h, t, at] = p
-                out[t, h] = p @ vh[at]
+        p = torch.softmax(torch.where(see, z, float("-inf")), -1)
+        p = torch.where(see.any(-1, keepdim=True), p, 0.0)
+        ps += p
+        out[:, h] = p @ vh
     return out, ps, xmax
 
 
@@ -97,8 +96,8 @@ def _compare(o, weight, weight0, q, k, v, see, scale, slots):
     bound = tol + (want.abs() + tol) * half + torch.finfo(o.dtype).tiny
     assert bool((off <= bound).all()), f"worst {float((off / bound).max()):.3g} of the bound"
     if weight is not None:
-        w = p[:, :, :slots].sum((0, 1))
-        tol = 2 * e * w + 2.0 ** -24 * (w + weight0.double().abs()) * (p.shape[0] * p.shape[1] / 4 + 6)
+        w = p[:, :slots].sum(0)
+        tol = 2 * e * w + 2.0 ** -24 * (w + weight0.double().abs()) * (q.shape[0] * q.shape[1] / 4 + 6)
         off = (weight.double() - weight0.double() - w).abs()
         assert bool((off <= tol + 1e-30).all()), f"weight: {float((off - tol).max()):.3g} over the bound"
 
@@ -176,6 +175,59 @@ def test_attend_long_and_many_rows(dev, qt, ct):
             (64, 16, 2, 64, 1111, 1000, None, True, False), (130, 2, 1, 128, 500, 200, None, True, True),
             (64, 4, 4, 256, 1500, 1400, None, False, False), (33, 7, 1, 128, 900, 2000, 850, True, True)):
         _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight)
+
+
+TILES = [(64, 8, 1, 128, 8300, 8200, None, True, True), (64, 8, 1, 64, 49300, 49000, None, True, True),
+         (33, 16, 2, 128, 17000, 30000, 16900, True, True), (130, 4, 2, 64, 16500, 16400, None, True, False),
+         (256, 1, 1, 128, 16384, 16384, None, False, True), (64, 4, 1, 128, 65536, 20, None, True, True),
+         (16, 16, 1, 128, 49152, 60000, 40000, False, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ct", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("case", TILES, ids=[f"T{c[0]}_D{c[3]}_{c[4]}" for c in TILES])
+def test_attend_tiles(dev, case, ct):
+    """Sizes of the kernels for many rows (256 and more of a key head)."""
+    _case(dev, *case[:7], ct, ct, *case[7:])
+
+
+@pytest.mark.gpu
+def test_attend_tiles_many(dev):
+    """More than 64 tiles of a workgroup: 32 row tiles leave 8 splits of 33000 slots."""
+    _case(dev, 1024, 8, 1, 64, 33000, 32900, None, BF16, BF16, False, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ct", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_tiles_hidden_values(dev, D, ct):
+    """As test_attend_empty_rows_and_hidden_values, in the kernel for many rows."""
+    T, heads, slots = 64, 8, 8400
+    g = torch.Generator().manual_seed(D)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = r(T, heads, D).to(ct), r(slots, 1, D).to(ct), r(slots, 1, D).to(ct)
+    kn, vn = r(T, 1, D).to(ct), r(T, 1, D).to(ct)
+    pos = torch.arange(slots)
+    pos[::5] = -1                      # empty slots hold anything
+    k[::5], v[::5] = float("nan"), float("-inf")
+    q_pos = torch.full((T,), slots + 1)
+    q_pos[3], q_pos[7] = -2, 4000      # row 3 sees no slot, row 7 not all
+    tree = torch.eye(T, dtype=torch.bool)
+    tree[3, 3] = False
+    kn[9], vn[9] = float("nan"), float("inf")   # draft 9: seen by itself and row 11 alone
+    tree[11, 9] = True
+    v[4004] = float("inf")             # hidden from rows 3 and 7 alone
+    announce(f"tiles, hidden values D={D} {ct}")
+    to = lambda t: t.to(dev)           # noqa: E731
+    weight = torch.zeros(slots, device=dev)
+    o = tree_attention(to(q), to(k), to(v), to(pos), to(q_pos), to(kn), to(vn), to(tree), weight=weight).cpu()
+    assert bool((o[3] == 0).all())
+    assert bool(torch.isnan(o[9]).all()) and bool(torch.isnan(o[11]).all())
+    rest = [t for t in range(T) if t not in (3, 7, 9, 11)]
+    assert bool((o[rest] == float("inf")).all())
+    clean = lambda t: torch.nan_to_num(t.float(), 0.0, 0.0, 0.0).to(t.dtype)  # noqa: E731
+    see = _see(pos, q_pos, tree, None)
+    _compare(o[[7]], None, None, q[[7]], clean(torch.cat([k, kn])), clean(torch.cat([v, vn])), see[[7]], D ** -0.5, slots)
 
 
 @pytest.mark.gpu
