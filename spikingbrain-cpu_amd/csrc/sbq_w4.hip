@@ -19,10 +19,12 @@
 // the same type, exactly).  fp32 is split into two fp16 planes after a
 // power-of-two scaling per row and K tile: 22 significant bits, 2^-39 of the
 // tile's maximum at least, below the rounding of an fp32 sum.
-//   STAGE   up to 8 rows: the wave converts its K tile once (16 lanes per
-//           row) into LDS and reads fragments from there; a fragment read
-//           straight from memory would be converted 16 times over at one row
-//   direct  otherwise: each lane converts the fragment it multiplies
+//   STAGE   up to 8 rows: the wave converts its K tiles once into LDS, 16 lanes
+//           per row and tile (a single row: four tiles at a time), and reads
+//           fragments from there; a fragment read straight from memory would be
+//           converted 16 times over at one row
+//   direct  otherwise: each lane converts the fragment it multiplies; the
+//           fragments of all row tiles of a K tile are loaded together
 #include "sbq_common.h"
 #include "sbq_launch.h"
 
@@ -31,6 +33,7 @@ namespace sbq {
 namespace {
 
 constexpr int kW4MaxWaves = 8;
+constexpr int kW4WideTiles = 2048;  // 16-row tiles from which a decode workgroup takes two
 
 // 8 nibbles u = q + 8 -> fp16 q: element 2i in nibble i, 2i + 1 in nibble
 // i + 4; 0x6400 | u is 1024 + u.
@@ -142,18 +145,19 @@ struct W4Args {
 };
 
 // XT: activations; MT: 16-row tiles of x; G: 16-row tiles of the weight; GS:
-// MFMA steps per group (1, 2, 4); PASSES: 0 direct, else STAGE with 4 rows of
-// x per pass; D: K tiles loaded together.
-template <int XT, int MT, int G, int GS, int PASSES, int D>
+// MFMA steps per group (1, 2, 4); ROWS: 0 direct, else STAGE of 1, 2, 4 or 8
+// rows; D: K tiles loaded together.
+template <int XT, int MT, int G, int GS, int ROWS, int D>
 __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
   typedef typename XElem<XT>::T T;
   typedef W4Math<XT> Math;
   typedef typename Math::V V;
   constexpr int P = XT == XT_F32 ? 2 : 1;  // planes of x
   constexpr int GPT = 4 / GS;              // groups per tile
-  constexpr int ROWS = PASSES * 4;
-  constexpr int XR = PASSES ? PASSES : 4;  // 8-element pieces of x per lane
-  static_assert(!PASSES || MT == 1, "staging serves one row tile");
+  // STAGE: the D tiles' ROWS rows are staged 4 (row, tile) pairs at a time
+  constexpr int PASSES = D * ROWS / 4;
+  constexpr int STAGE = P * D * ROWS * 256;  // bytes of a wave, then the pairs' factors
+  static_assert(ROWS == 0 || (MT == 1 && D * ROWS % 4 == 0), "staging serves one row tile, four pairs at a time");
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
@@ -167,14 +171,13 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[i][t] = (f32x4)(0.0f);
 
-  // STAGE: the wave's own LDS: P planes of ROWS rows of 16 pieces, then the rows' factors
-  uint8_t* const stage = lds + ks * (P * ROWS * 256 + (P == 2 ? ROWS * 4 : 0));
-  float* const factor = (float*)(stage + P * ROWS * 256);
+  uint8_t* const stage = lds + ks * (STAGE + (P == 2 ? D * ROWS * 4 : 0));
+  float* const factor = (float*)(stage + STAGE);
 
   for (int kb = ks; kb < a.Kc; kb += D * KS) {
     u32x4 w[D][G];
     u32x2 sc[D][G][GPT];
-    X8<XT> raw[D][XR];
+    X8<XT> raw[ROWS ? PASSES : D][ROWS ? 1 : MT][ROWS ? 1 : 4];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int kt = min(kb + d * KS, a.Kc - 1);  // (a surplus tile is loaded again, not used)
@@ -186,15 +189,40 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
         for (int q = 0; q < GPT; ++q)
           sc[d][i][q] = *(const u32x2*)(a.gscale + ((nt * a.Kc + kt) * GPT + q) * 16 + 4 * g);
       }
-      if constexpr (PASSES > 0) {
+      if constexpr (ROWS == 0) {
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p)
-          raw[d][p].load(x + (int64_t)min(p * 4 + g, M - 1) * a.ldx, kt * 128 + c * 8, a.K, a.xvec);
-      } else if constexpr (MT == 1) {
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          raw[d][s].load(x + (int64_t)min(c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
+          for (int s = 0; s < 4; ++s)
+            raw[d][t][s].load(x + (int64_t)min(t * 16 + c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
       }
+    }
+    if constexpr (ROWS > 0) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {  // lane group g: pair p * 4 + g = (tile, row)
+        const int pair = p * 4 + g, kt = min(kb + pair / ROWS * KS, a.Kc - 1);
+        raw[p][0][0].load(x + (int64_t)min(pair % ROWS, M - 1) * a.ldx, kt * 128 + c * 8, a.K, a.xvec);
+      }
+      wave_lds_fence();
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int pair = p * 4 + g;
+        uint8_t* const to = stage + pair * 256 + ((c ^ pair) & 15) * 16;
+        if constexpr (XT == XT_F32) {
+          float mx = max_abs8(raw[p][0][0].v);
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
+          const int e = tile_exp(mx);
+          f16x8 hi, lo;
+          split_f16(raw[p][0][0].v, exp2i(e), hi, lo);
+          *(f16x8*)to = hi;
+          *(f16x8*)(to + D * ROWS * 256) = lo;
+          if (c == 0) factor[pair] = exp2i(-e);
+        } else {
+          *(V*)to = __builtin_bit_cast(V, raw[p][0][0].v);
+        }
+      }
+      wave_lds_fence();
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -209,55 +237,28 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
       for (int t = 0; t < MT; ++t) {
         V xv[P][4];
         float f = 1.0f;
-        if constexpr (PASSES > 0) {
-          wave_lds_fence();
-#pragma unroll
-          for (int p = 0; p < PASSES; ++p) {
-            const int row = p * 4 + g;
-            uint8_t* const to = stage + row * 256 + ((c ^ row) & 15) * 16;
-            if constexpr (XT == XT_F32) {
-              float mx = max_abs8(raw[d][p].v);
-#pragma unroll
-              for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
-              const int e = tile_exp(mx);
-              f16x8 hi, lo;
-              split_f16(raw[d][p].v, exp2i(e), hi, lo);
-              *(f16x8*)to = hi;
-              *(f16x8*)(to + ROWS * 256) = lo;
-              if (c == 0) factor[row] = exp2i(-e);
-            } else {
-              *(V*)to = __builtin_bit_cast(V, raw[d][p].v);
-            }
-          }
-          wave_lds_fence();
-          const int row = min(c, M - 1);
+        if constexpr (ROWS > 0) {
+          const int pair = d * ROWS + min(c, M - 1);
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const uint8_t* const from = stage + row * 256 + (((s * 4 + g) ^ row) & 15) * 16;
+            const uint8_t* const from = stage + pair * 256 + (((s * 4 + g) ^ pair) & 15) * 16;
 #pragma unroll
-            for (int p = 0; p < P; ++p) xv[p][s] = *(const V*)(from + p * ROWS * 256);
+            for (int p = 0; p < P; ++p) xv[p][s] = *(const V*)(from + p * D * ROWS * 256);
           }
-          if constexpr (XT == XT_F32) f = factor[row];
+          if constexpr (XT == XT_F32) f = factor[pair];
+        } else if constexpr (XT == XT_F32) {
+          float mx = 0.0f;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mx = __builtin_fmaxf(mx, max_abs8(raw[d][t][s].v));
+          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
+          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const int e = tile_exp(mx);
+          f = exp2i(-e);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) split_f16(raw[d][t][s].v, exp2i(e), xv[0][s], xv[1][s]);
         } else {
-          if constexpr (MT > 1) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-              raw[d][s].load(x + (int64_t)min(t * 16 + c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
-          }
-          if constexpr (XT == XT_F32) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) mx = __builtin_fmaxf(mx, max_abs8(raw[d][s].v));
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const int e = tile_exp(mx);
-            f = exp2i(-e);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) split_f16(raw[d][s].v, exp2i(e), xv[0][s], xv[1][s]);
-          } else {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) xv[0][s] = __builtin_bit_cast(V, raw[d][s].v);
-          }
+          for (int s = 0; s < 4; ++s) xv[0][s] = __builtin_bit_cast(V, raw[d][t][s].v);
         }
 #pragma unroll
         for (int i = 0; i < G; ++i)
@@ -399,18 +400,18 @@ __global__ __launch_bounds__(256) void unpack_scale_kernel(const uint16_t* gscal
 
 inline unsigned blocks(int64_t count) { return (unsigned)((count + 255) / 256); }
 
-template <int XT, int MT, int G, int PASSES, int D>
+template <int XT, int MT, int G, int ROWS, int D>
 int launch_w4(const W4Args& a, int group, int KS, hipStream_t st) {
-  constexpr int P = XT == XT_F32 ? 2 : 1, ROWS = PASSES * 4;
-  const int stage = KS * (P * ROWS * 256 + (P == 2 ? ROWS * 4 : 0)), red = KS > 1 ? KS * G * MT * 1024 : 0;
+  constexpr int P = XT == XT_F32 ? 2 : 1;
+  const int stage = KS * D * ROWS * (P * 256 + (P == 2 ? 4 : 0)), red = KS > 1 ? KS * G * MT * 1024 : 0;
   const size_t lds = (size_t)(stage > red ? stage : red);
   const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
   if (group == 32)
-    linear_w4_kernel<XT, MT, G, 1, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 1, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
   else if (group == 64)
-    linear_w4_kernel<XT, MT, G, 2, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 2, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
   else
-    linear_w4_kernel<XT, MT, G, 4, PASSES, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 4, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
   return check_launch();
 }
 
@@ -418,8 +419,11 @@ template <int XT>
 int pick_w4(const W4Args& a, int group, hipStream_t st) {
   int KS = 1;
   while (KS < kW4MaxWaves && KS * 2 < a.Kc) KS *= 2;
-  if (a.M <= 4) return launch_w4<XT, 1, 1, 1, 4>(a, group, KS, st);
-  if (a.M <= 8) return launch_w4<XT, 1, 1, 2, 2>(a, group, KS, st);
+  const bool wide = a.Nt >= kW4WideTiles;
+  if (a.M == 1) return wide ? launch_w4<XT, 1, 2, 1, 4>(a, group, KS, st) : launch_w4<XT, 1, 1, 1, 4>(a, group, KS, st);
+  if (a.M == 2) return wide ? launch_w4<XT, 1, 2, 2, 4>(a, group, KS, st) : launch_w4<XT, 1, 1, 2, 4>(a, group, KS, st);
+  if (a.M <= 4) return wide ? launch_w4<XT, 1, 2, 4, 2>(a, group, KS, st) : launch_w4<XT, 1, 1, 4, 2>(a, group, KS, st);
+  if (a.M <= 8) return launch_w4<XT, 1, 1, 8, 2>(a, group, KS, st);
   if (a.M <= 16) return launch_w4<XT, 1, 1, 0, 2>(a, group, KS, st);
   if (a.M <= 32) return launch_w4<XT, 2, 2, 0, 1>(a, group, KS, st);
   return launch_w4<XT, 4, 2, 0, 1>(a, group, KS, st);
