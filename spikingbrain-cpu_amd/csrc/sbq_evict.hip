@@ -24,6 +24,7 @@ namespace sbq {
 namespace {
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 2048;
+constexpr int kChunk = 4 * kSelThreads;  // slots that one workgroup of a launch before the selection looks at
 
 // The order in which slots are given up.
 __device__ __forceinline__ uint32_t evict_key(int64_t pos, float weight, int64_t keep_from) {
@@ -63,6 +64,7 @@ struct Select {
   int n;
   int64_t keep_from;
   const uint32_t* ready;  // not null: the keys themselves
+  const uint32_t* first;  // not null: their first digits' counts, kBins for each kChunk slots
 };
 
 // A thread's `per` (4, 8, 16 or 32) keys of a segment of per * 1024 slots lie
@@ -96,10 +98,12 @@ __device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit) {
 // Keys of segment `seg` into LDS, their first digits counted where hist is
 // given.  Slots past the end get the largest key: with m <= n they come after
 // every slot that is wanted.
+// All loads of a step are issued before the first is looked at, with no branch
+// between them.
+template <bool READY, int U>
 __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int log, uint32_t* keys, uint32_t* hist) {
   const int per = 1 << log;
   const int64_t s0 = seg * per * kSelThreads;
-  constexpr int U = 8;
 #pragma unroll 1
   for (int i = 0; i < per; i += U) {
     int64_t pos[U];
@@ -107,25 +111,30 @@ __device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int log,
     uint32_t key[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int64_t s = s0 + (int64_t)(i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
-      if (j < 4 || per > 4) {
-        if (q.ready) {
-          key[j] = q.ready[at];
-        } else {
-          pos[j] = q.slot_pos[at];
-          w[j] = q.weight[at];
-        }
+      const int64_t s = s0 + (i + j) * kSelThreads + threadIdx.x, at = s < q.n ? s : q.n - 1;
+      if constexpr (READY) {
+        key[j] = q.ready[at];
+      } else {
+        pos[j] = q.slot_pos[at];
+        w[j] = q.weight[at];
       }
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      if (j >= 4 && per == 4) break;
       const int s = (i + j) * kSelThreads + threadIdx.x;
-      const uint32_t k = s0 + s >= q.n ? ~0u : q.ready ? key[j] : evict_key(pos[j], w[j], q.keep_from);
+      if constexpr (!READY) key[j] = evict_key(pos[j], w[j], q.keep_from);
+      const uint32_t k = s0 + s >= q.n ? ~0u : key[j];
       keys[key_at(s >> log, s & (per - 1), log)] = k;
       if (hist) count_digit(hist, k >> 21);
     }
   }
+}
+
+__device__ __forceinline__ void load_keys(const Select& q, int64_t seg, int log, uint32_t* keys, uint32_t* hist) {
+  if (q.ready)
+    log >= 3 ? load_keys<true, 8>(q, seg, log, keys, hist) : load_keys<true, 4>(q, seg, log, keys, hist);
+  else
+    log >= 3 ? load_keys<false, 8>(q, seg, log, keys, hist) : load_keys<false, 4>(q, seg, log, keys, hist);
 }
 
 // The slots with the m smallest keys (side 0) or the used ones among the
@@ -135,12 +144,29 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
   __shared__ uint32_t hist[kBins], cand[kCand], scan[kSelWaves], found[3], ncand;
   const int log = keys_log(q.n), per = 1 << log;
   const int segs = (int)(((int64_t)q.n + per * kSelThreads - 1) >> (log + 10));
+  // (the counts are under way while the keys are read)
+  const int chunks = (int)(((int64_t)q.n + kChunk - 1) / kChunk);
+  u32x2 first[8];
+  if (m > 0 && q.first) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      first[c] = *(const u32x2*)(q.first + (int64_t)min(c, chunks - 1) * kBins + 2 * threadIdx.x);
+  }
   for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
   if (threadIdx.x == 0) ncand = 0;
   __syncthreads();
   for (int seg = 0; seg < segs; ++seg) {
-    load_keys(q, seg, log, keys, m > 0 ? hist : nullptr);
+    load_keys(q, seg, log, keys, m > 0 && !q.first ? hist : nullptr);
     if (segs > 1) __syncthreads();
+  }
+  if (m > 0 && q.first) {
+    u32x2 sum = (u32x2)(0u);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) sum += c < chunks ? first[c] : (u32x2)(0u);
+#pragma unroll 4
+    for (int c = 8; c < chunks; ++c) sum += *(const u32x2*)(q.first + (int64_t)c * kBins + 2 * threadIdx.x);
+    hist[2 * threadIdx.x] = sum.x;
+    hist[2 * threadIdx.x + 1] = sum.y;
   }
   __syncthreads();
 
@@ -190,13 +216,15 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
       ties -= found[1];
       if (pass == 0 && segs == 1 && found[2] <= kCand) {
         few = true;
+        uint32_t mine = 0;  // one bit per own key
 #pragma unroll 1
         for (int i = 0; i < per; i += 4) {
           const u32x4 k4 = own_keys(keys, log, i);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (k4[j] >> 21 == found[0]) cand[atomicAdd(&ncand, 1u)] = k4[j];
+          for (int j = 0; j < 4; ++j) mine |= (uint32_t)(k4[j] >> 21 == found[0]) << (i + j);
         }
+        uint32_t at = mine ? atomicAdd(&ncand, (uint32_t)__popc(mine)) : 0u;
+        for (; mine; mine &= mine - 1) cand[at++] = keys[key_at(threadIdx.x, __ffs(mine) - 1, log)];
       }
       __syncthreads();
     }
@@ -206,6 +234,10 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
   // (key 0) are never among the used ones.  Before a thread's own slots lie
   // `out` keys strictly on the wanted side and `eq` equal ones.
   uint32_t out = 0, eq = 0;
+  auto listed = [&](uint32_t strictly, uint32_t equal) {  // entries that so many keys make
+    const uint32_t low = min(equal, ties);
+    return strictly + (side == 0 ? low : kth == 0 ? 0u : equal - low);
+  };
 #pragma unroll 1
   for (int seg = 0; seg < segs; ++seg) {
     if (segs > 1) {
@@ -233,7 +265,10 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
     const uint32_t eq0 = eq + block_scan(__popc(same), scan, &all_eq);
     const uint32_t low0 = min(eq0, ties);
     const uint32_t mine = min(eq0 + (uint32_t)__popc(same), ties) - low0;  // own equal ones among the m
-    uint32_t place = out0 + (side == 0 ? low0 : kth == 0 ? 0u : eq0 - low0);
+    // The segment's entries gather in LDS (its keys are done with) and leave from there in whole lines:
+    // a thread's own run stored from here took 64 lines a wave.
+    const uint32_t base = listed(out, eq);
+    uint32_t place = out0 + (side == 0 ? low0 : kth == 0 ? 0u : eq0 - low0) - base;
     uint32_t skip = mine, todo = strict | same;
     while (todo) {
       const uint32_t bit = todo & (0u - todo);
@@ -243,14 +278,45 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
         take = side == 0 ? skip > 0 : skip == 0 && kth != 0;
         skip -= skip > 0;
       }
-      if (take) list[place++] = (int32_t)(s0 + __ffs(bit) - 1);
+      if (take) keys[place++] = (uint32_t)(s0 + __ffs(bit) - 1);
     }
     out += all_out;
     eq += all_eq;
+    __syncthreads();
+    const uint32_t n = listed(out, eq) - base;
+    for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) list[base + i] = (int32_t)keys[i];
     if (segs > 1) __syncthreads();
   }
-  const uint32_t low = min(eq, ties);
-  return (int)(out + (side == 0 ? low : kth == 0 ? 0u : eq - low));
+  return (int)listed(out, eq);
+}
+
+// The m first of up to kRank ready keys, listed in order: each thread counts
+// the keys before its own, then the chosen ones before it (64 candidates: some
+// 1 us where the digits' passes over as few take 12).
+constexpr int kRank = 256;
+__device__ __forceinline__ void rank_slots(const uint32_t* ready, int n, int m, int32_t* list) {
+  __shared__ __align__(16) uint32_t key[kRank];
+  __shared__ unsigned long long chosen[kRank / 64];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  uint32_t k = ~0u;
+  if (t < kRank) key[t] = k = t < n ? ready[t] : ~0u;
+  __syncthreads();
+  int before = 0;
+  if (t < kRank) {
+    for (int i = 0; i < n; i += 4) {
+      const u32x4 k4 = *(const u32x4*)(key + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) before += k4[j] < k || (k4[j] == k && i + j < t);
+    }
+    const unsigned long long on = __ballot(t < n && before < m);
+    if (lane == 0) chosen[w] = on;
+  }
+  __syncthreads();
+  if (t < n && before < m) {
+    int place = __popcll(chosen[w] & ((1ull << lane) - 1));
+    for (int i = 0; i < w; ++i) place += __popcll(chosen[i]);
+    list[place] = t;
+  }
 }
 
 // The slot of the smallest key (the lowest of equal ones).
@@ -348,7 +414,7 @@ struct AppendArgs {
 template <int ST, int DT>
 __global__ __launch_bounds__(kSelThreads) void kv_append_one_kernel(AppendArgs a) {
   const int64_t start = *a.start;
-  const Select q{a.slot_pos, a.weight, a.n, start + 1 - a.recent, nullptr};
+  const Select q{a.slot_pos, a.weight, a.n, start + 1 - a.recent, nullptr, nullptr};
   const int s = first_slot(q);  // (every thread has read its slots and *start)
   if (threadIdx.x == 0) {
     a.slot_pos[s] = start;
@@ -359,10 +425,10 @@ __global__ __launch_bounds__(kSelThreads) void kv_append_one_kernel(AppendArgs a
 }
 
 // The T first of every kChunk slots, in slot order, with their keys.
-constexpr int kChunk = 4 * kSelThreads, kSpreadFrom = 2 * kChunk, kSpreadTokens = kChunk / 8;
+constexpr int kSpreadFrom = 2 * kChunk, kSpreadTokens = kChunk / 8;
 __global__ __launch_bounds__(kSelThreads) void kv_first_kernel(AppendArgs a) {
   const int s0 = blockIdx.x * kChunk, n = min(kChunk, a.n - s0), m = min(a.T, n);
-  const Select q{a.slot_pos + s0, a.weight + s0, n, *a.start + a.T - a.recent, nullptr};
+  const Select q{a.slot_pos + s0, a.weight + s0, n, *a.start + a.T - a.recent, nullptr, nullptr};
   int32_t* const list = a.cand_slot + (int64_t)blockIdx.x * a.T;
   select_slots(q, m, 0, list);
   __syncthreads();  // the list is written
@@ -377,10 +443,13 @@ template <int ST, int DT>
 __global__ __launch_bounds__(kSelThreads) void kv_append_kernel(AppendArgs a) {
   const int64_t start = *a.start;
   const int chunks = (a.n + kChunk - 1) / kChunk;
-  Select q{a.slot_pos, a.weight, a.n, start + a.T - a.recent, a.cand_key};
+  Select q{a.slot_pos, a.weight, a.n, start + a.T - a.recent, a.cand_key, nullptr};
   // (only the last workgroup may have had fewer than T slots, so the candidates are dense and in slot order)
   if (a.cand_key) q.n = (chunks - 1) * a.T + min(a.T, a.n - (chunks - 1) * kChunk);
-  select_slots(q, a.T, 0, a.list);
+  if (a.cand_key && q.n <= kRank)
+    rank_slots(a.cand_key, q.n, a.T, a.list);
+  else
+    select_slots(q, a.T, 0, a.list);
   __syncthreads();  // the list is written
   for (int i = threadIdx.x; i < a.T; i += kSelThreads) {
     int s = a.list[i];
@@ -392,8 +461,11 @@ __global__ __launch_bounds__(kSelThreads) void kv_append_kernel(AppendArgs a) {
   if (a.rows_too) {
     __syncthreads();  // the list is in slots
     const int row = a.Hk * a.D;
-    for (int i = 0; i < a.T; ++i)
-      copy_row<ST, DT>(a.fresh, i, a.cache, a.list[i], a.D, threadIdx.x, row, kSelThreads);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < a.T * row; e += kSelThreads) {
+      const int i = e / row;
+      copy_row<ST, DT>(a.fresh, i, a.cache, a.list[i], a.D, e - i * row, e - i * row + 1, 1);
+    }
   }
 }
 
@@ -409,20 +481,45 @@ struct TakeArgs {
   float* to_weight;
   Rows src, dst;
   int32_t* list;   // [capacity], then the count
-  uint32_t* keys;  // [n] where a launch before the selection computes them
+  uint32_t *keys, *first;  // [n] and [chunks][kBins] where a launch before the selection computes them
   int n, capacity, Hk, D, es;
   int64_t recent;
   bool vec;
 };
 
-__global__ __launch_bounds__(256) void kv_keys_kernel(TakeArgs a) {
-  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (s < a.n) a.keys[s] = evict_key(a.slot_pos[s], a.weight[s], *a.end - a.recent);
+// The keys, and how often each first digit occurs in every kChunk slots: few
+// bins (the exponents of like weights) take most of the counts, whose atomics
+// wait for each other, so they are spread over workgroups and four copies.
+__global__ __launch_bounds__(kSelThreads) void kv_keys_kernel(TakeArgs a) {
+  __shared__ uint32_t hist[kBins * 4];
+  for (int i = threadIdx.x; i < kBins * 4; i += kSelThreads) hist[i] = 0;
+  const int64_t s0 = (int64_t)blockIdx.x * kChunk + threadIdx.x, keep_from = *a.end - a.recent;
+  int64_t pos[4];
+  float w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t s = s0 + j * kSelThreads, at = s < a.n ? s : a.n - 1;
+    pos[j] = a.slot_pos[at];
+    w[j] = a.weight[at];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t s = s0 + j * kSelThreads;
+    const uint32_t k = s < a.n ? evict_key(pos[j], w[j], keep_from) : ~0u;  // (as the selection counts the missing ones)
+    if (s < a.n) a.keys[s] = k;
+    atomicAdd(&hist[(k >> 21) * 4 + (threadIdx.x & 3)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSelThreads) {
+    const u32x4 h = *(const u32x4*)(hist + 4 * i);
+    a.first[(int64_t)blockIdx.x * kBins + i] = h.x + h.y + h.z + h.w;
+  }
 }
 
 __global__ __launch_bounds__(kSelThreads) void kv_take_kernel(TakeArgs a) {
   const int64_t end = *a.end;
-  const Select q{a.slot_pos, a.weight, a.n, end - a.recent, a.keys};
+  const Select q{a.slot_pos, a.weight, a.n, end - a.recent, a.keys, a.first};
   const int kept = select_slots(q, a.n > a.capacity ? a.n - a.capacity : 0, 1, a.list);
   if (threadIdx.x == 0) {
     a.list[a.capacity] = kept;
@@ -453,7 +550,7 @@ __global__ __launch_bounds__(256) void kv_take_rows_kernel(TakeArgs a) {
   }
 }
 
-constexpr int kInlineElems = 1 << 15;  // key elements that the selecting workgroup still writes itself
+constexpr int kInlineElems = 1 << 12;  // key elements that the selecting workgroup still writes itself
 
 template <int ST, int DT>
 int append_types(const AppendArgs& a, hipStream_t st) {
@@ -484,8 +581,11 @@ int append_from(const AppendArgs& a, int ct, hipStream_t st) {
 
 }  // namespace
 
-// The list (one count more), then the candidates of an append or the keys of a take.
-int64_t kv_workspace_bytes(int64_t slots, int64_t count) { return 4 * (count + 1) + (slots >= kSpreadFrom ? 4 * slots : 0); }
+// The list (one count more), then the candidates of an append or the counts and keys of a take.
+int64_t list_words(int64_t count) { return (count + 1 + 3) / 4 * 4; }
+int64_t kv_workspace_bytes(int64_t slots, int64_t count) {
+  return 4 * list_words(count) + (slots >= kSpreadFrom ? 4 * (slots + (slots + kChunk - 1) / kChunk * kBins) : 0);
+}
 static_assert(kSpreadTokens * 8 <= kChunk && 2 * kSpreadTokens * 8 <= 3 * kSpreadFrom, "candidates fit 4 bytes a slot");
 
 int launch_kv_append(const KvAppend& c, hipStream_t st) {
@@ -505,11 +605,14 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
   auto ok = [&](const void* p, int64_t ss, int64_t sh) { return (uintptr_t)p % 16 == 0 && ss * es % 16 == 0 && sh * es % 16 == 0; };
   const bool vec = c.D * es % 16 == 0 && ok(c.k, c.k_ss, c.k_sh) && ok(c.v, c.k_ss, c.k_sh) && ok(c.to_k, c.t_ss, c.t_sh) &&
                    ok(c.to_v, c.t_ss, c.t_sh);
+  uint32_t* const more = (uint32_t*)c.ws + list_words(c.capacity);
+  const bool spread = c.slots >= kSpreadFrom;
   TakeArgs a{c.slot_pos, c.end, c.weight, c.to_pos, c.to_end, c.to_weight,
              Rows{const_cast<void*>(c.k), const_cast<void*>(c.v), c.k_ss, c.k_sh}, Rows{c.to_k, c.to_v, c.t_ss, c.t_sh},
-             (int32_t*)c.ws, c.slots >= kSpreadFrom ? (uint32_t*)c.ws + c.capacity + 1 : nullptr, (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
+             (int32_t*)c.ws, spread ? more + (c.slots + kChunk - 1) / kChunk * kBins : nullptr, spread ? more : nullptr,
+             (int)c.slots, (int)c.capacity, (int)c.Hk, (int)c.D, es, c.recent, vec};
   if (a.keys) {
-    kv_keys_kernel<<<(a.n + 255) / 256, 256, 0, st>>>(a);
+    kv_keys_kernel<<<(a.n + kChunk - 1) / kChunk, kSelThreads, 0, st>>>(a);
     const int rc = check_launch();
     if (rc) return rc;
   }
