@@ -49,10 +49,11 @@ struct AttnArgs {
   const int64_t *slot_pos, *q_pos;
   const uint8_t* tree;          // [T][tree_ld], null: draft j is seen by t >= j
   void* out;
-  float* part_o;                // [Hk*R][splits][DP]
+  float* part_o;                // [Hk*R][splits][DP]; null: a workgroup has the whole row
   float2* part_ml;              // [Hk*R][splits]
+  float* scores;                // [Hk*R][score_ld] of the cached slots, where they are kept for the slots' weights
   float2* row_ml;               // [Hk*R] (maximum, 1 / sum), where the slots' weights are wanted
-  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld;
+  int64_t q_st, q_sh, k_ss, k_sh, n_ss, n_sh, o_st, o_sh, tree_ld, score_ld;
   int64_t window;               // 0: none
   int T, Hk, rep, D, slots, Tn, splits, rtiles, qt;
   float scale;                  // times log2(e), >= 0 (`neg`: q is negated instead)
@@ -338,6 +339,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[i][st][v] = s[v];
+        if (RT == 1 && a.scores && !fresh && row[i] < R)  // (as many as fit whole blocks have room)
+          *(f32x4*)(a.scores + ((int64_t)kvh * R + row[i]) * a.score_ld + base + st * 16 + 4 * g) = s;
       }
       float mx = kNone;
       if constexpr (full) {
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
           }
         }
         const int64_t at = (int64_t)kvh * R + r0 + rr;
-        if (a.splits > 1) {
+        if (a.part_o) {
           *(f32x4*)(a.part_o + (at * a.splits + split) * DP + d) = sum;
           if (d == 0) a.part_ml[at * a.splits + split] = make_float2(top, ls);
         } else {
@@ -928,9 +931,9 @@ __global__ __launch_bounds__(64) void attn_tile_join_kernel(AttnArgs a) {
 }
 
 // weight[s] += sum over the rows that see slot s of exp2(score - maximum) /
-// sum, the scores computed once more: storing them would move 8 bytes per row
-// and slot, more than a key's own bytes from some 16 rows on, and hold them in
-// memory.  A workgroup takes SB slots and every row; its waves share the
+// sum, for more rows than attn_join_weight_kernel takes: the scores are computed
+// once more, as storing them would move 8 bytes per row and slot, more than a
+// key's own bytes, and hold them in memory.  A workgroup takes SB slots and every row; its waves share the
 // (key head, 16-row tile) pairs, keep the slots' keys in registers while the
 // head stays, and add up in wave order.
 constexpr int kWeightWaves = 8, kWeightBufs = 4;

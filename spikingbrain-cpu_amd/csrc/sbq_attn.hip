@@ -16,11 +16,10 @@ namespace {
 // One row's splits joined: the maximum over their maxima, then the partial
 // sums scaled to it.  A thread's loads are independent, four at a time.
 template <int DP>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+__device__ __forceinline__ void join_row(const AttnArgs& a, int64_t at) {
   constexpr int ND = DP / 4, NG = 256 / ND;
   __shared__ __align__(16) f32x4 lds[NG][ND];
   __shared__ float lds_l[NG];
-  const int64_t at = blockIdx.x;
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
   const float2* const ml = a.part_ml + at * a.splits;
   float top = -__builtin_inff();
@@ -64,6 +63,82 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (d == 0 && a.row_ml) a.row_ml[at] = make_float2(from, inv);
 }
 
+template <int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  join_row<DP>(a, blockIdx.x);
+}
+
+// The joining and, in further workgroups of the same launch, what every slot
+// received: weight[s] += sum over the rows that see slot s of exp2(score -
+// maximum) / sum, from the scores that the attention kept.  Each of these
+// workgroups takes the rows' maxima and sums from the partial ones itself, so
+// that none waits for a joined row.  A wave adds up every fourth row, the waves
+// are added in order.  What bounds it is the latency of two loads after another
+// (few rows: 32 rows over 2304 slots take 0.3 MB).
+constexpr int kScoreR = 8, kScoreRows = 256, kScoreStats = 4096;  // rows of a key head, of all; all rows x splits
+constexpr int kScoreSlots = 64;  // slots of a step
+template <int DP>
+__global__ __launch_bounds__(256) void attn_join_weight_kernel(AttnArgs a, float* weight, int strips) {
+  __shared__ float2 ml[kScoreRows];
+  __shared__ int64_t top_pos[kScoreRows];
+  __shared__ float sums[4][kScoreSlots];
+  const int R = a.rep * a.T, rows = a.Hk * R, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if ((int)blockIdx.x < rows) {
+    join_row<DP>(a, blockIdx.x);
+    return;
+  }
+  constexpr int U = 8;
+  float s[U];
+  auto load = [&](int slot, int row0) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      s[k] = a.scores[(int64_t)min(row0 + 4 * k, rows - 1) * a.score_ld + slot];  // (slot < score_ld)
+  };
+  const int strip0 = ((int)blockIdx.x - rows) * strips;
+  load(min(strip0 * kScoreSlots + lane, (int)a.score_ld - 1), w);  // (the first strip's, under the maxima)
+
+  for (int row = threadIdx.x >> 3; row < rows; row += 32) {  // 8 lanes a row
+    const float2* const part = a.part_ml + (int64_t)row * a.splits;
+    const int first = threadIdx.x & 7;
+    float top = -__builtin_inff(), l = 0.0f;
+    for (int i = first; i < a.splits; i += 8) top = __builtin_fmaxf(top, part[i].x);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 64));
+    const float from = top == -__builtin_inff() ? 0.0f : top;
+    for (int i = first; i < a.splits; i += 8)
+      if (part[i].y != 0.0f) l += part[i].y * __builtin_amdgcn_exp2f(part[i].x - from);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) l += __shfl_xor(l, o, 64);
+    if (first == 0) {
+      ml[row] = make_float2(from, l != 0.0f ? 1.0f / l : 0.0f);
+      top_pos[row] = a.q_pos[row % R / a.rep];
+    }
+  }
+  for (int strip = strip0; strip < strip0 + strips && strip * kScoreSlots < a.slots; ++strip) {
+    const int slot = strip * kScoreSlots + lane;
+    const int64_t pos = slot < a.slots ? a.slot_pos[slot] : -1;
+    if (strip > strip0) load(min(slot, (int)a.score_ld - 1), w);
+    __syncthreads();  // the maxima are there, the last strip's sums are read
+    float sum = 0.0f;
+    for (int row0 = w;;) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int row = row0 + 4 * k;
+        if (row >= rows) break;
+        const int64_t hi = top_pos[row], lo = a.window > 0 && hi - a.window + 1 > 0 ? hi - a.window + 1 : 0;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], a.scale, -ml[row].x)) * ml[row].y;
+        sum += pos >= lo && pos <= hi ? p : 0.0f;
+      }
+      row0 += 4 * U;
+      if (row0 >= rows) break;
+      load(min(slot, (int)a.score_ld - 1), row0);
+    }
+    sums[w][lane] = sum;
+    __syncthreads();
+    if (w == 0 && slot < a.slots) weight[slot] += sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+  }
+}
+
 constexpr int kAttnGroups = 512;    // workgroups aimed at
 // attn_tile_kernel: workgroups aimed at (one a CU), and the rows of a key head
 // and rows times slots from which it is taken.  8 key heads of 128 bf16
@@ -100,6 +175,16 @@ AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, boo
   return p;
 }
 
+// Are the scores kept for the slots' weights, [Hk * R][score_ld], and the partial
+// results always?  For so few rows that every workgroup can join their maxima.
+// 8 key heads of 128 bf16 columns, the weights' share of a call, kept against
+// computed again (and a launch less): 4 rows each, 65536 slots 11 us / 32 us,
+// 32768 6 / 18; 8 rows 24 / 34 and 13 / 18; 16 rows 49 / 36 and 26 / 19.
+bool keeps_scores(const AttnPlan& p, int64_t R, int64_t Hk, bool weight) {
+  return weight && p.RT == 1 && R <= kScoreR && Hk * R <= kScoreRows && Hk * R * p.splits <= kScoreStats;
+}
+int64_t score_ld(int64_t slots) { return (slots + 31) & ~(int64_t)31; }
+
 int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 }  // namespace
@@ -110,7 +195,9 @@ int64_t attn_workspace_bytes(int64_t T, int64_t heads, int64_t Hk, int64_t D, in
   for (int way = 0; way < 8; ++way) {  // types, alignment and drafts are not known here
     const AttnPlan p = attn_plan(R, Hk, slots, way & 4 ? T : 0, attn_dp(D), way & 1, way & 2);
     const int64_t parts = Hk * p.rows * p.splits;
-    const int64_t need = p.splits > 1 ? round256(parts * attn_dp(D) * 4) + round256(parts * 8) : 0;
+    const bool kept = keeps_scores(p, R, Hk, weight);
+    int64_t need = p.splits > 1 || kept ? round256(parts * attn_dp(D) * 4) + round256(parts * 8) : 0;
+    if (kept) need += round256(Hk * R * score_ld(slots) * 4);
     n = need > n ? need : n;
   }
   if (weight) n += round256(Hk * R * 8);
@@ -143,13 +230,19 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
            c.q_sh * eq % 16 == 0;
   a.ovec = (uintptr_t)c.out % (4 * eq) == 0 && c.o_st % 4 == 0 && c.o_sh % 4 == 0;
   uint8_t* ws = (uint8_t*)c.ws;
-  if (p.splits > 1) {
+  const bool kept = keeps_scores(p, R, Hk, c.weight);
+  if (p.splits > 1 || kept) {
     a.part_o = (float*)ws;
     ws += round256(Hk * p.rows * p.splits * DP * 4);
     a.part_ml = (float2*)ws;
     ws += round256(Hk * p.rows * p.splits * 8);
   }
-  if (c.weight) a.row_ml = (float2*)ws;
+  if (kept) {
+    a.scores = (float*)ws;
+    a.score_ld = score_ld(c.slots);
+  } else if (c.weight) {
+    a.row_ml = (float2*)ws;
+  }
   auto launch = [&](float* weight) {
     return c.ct == XT_F32   ? launch_attn_f32(a, DP, mode, p.RT, weight, st)
            : c.ct == XT_F16 ? launch_attn_f16(a, m16, DP, mode, p.RT, weight, st)
@@ -157,6 +250,18 @@ int launch_tree_attention(const AttnCall& c, hipStream_t st) {
   };
   int rc = launch(nullptr);
   if (rc) return rc;
+  if (kept) {
+    const int64_t all = (c.slots + kScoreSlots - 1) / kScoreSlots;
+    const int strips = (int)((all + 255) / 256);
+    const unsigned grid = (unsigned)(Hk * R + (all + strips - 1) / strips);
+    if (DP == 64)
+      attn_join_weight_kernel<64><<<grid, 256, 0, st>>>(a, c.weight, strips);
+    else if (DP == 128)
+      attn_join_weight_kernel<128><<<grid, 256, 0, st>>>(a, c.weight, strips);
+    else
+      attn_join_weight_kernel<256><<<grid, 256, 0, st>>>(a, c.weight, strips);
+    return check_launch();
+  }
   if (p.splits > 1 && p.RT != 0) {  // (attn_tile_kernel's launch joins its own)
     const unsigned grid = (unsigned)(Hk * R);
     if (DP == 64)

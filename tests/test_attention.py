@@ -18,7 +18,7 @@ import torch
 
 from conftest import announce
 from sbq import _lib
-from sbq.state import DeviceKVBuffer, tree_attention
+from sbq.state import DeviceKVBuffer, attention_workspace, tree_attention
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -175,6 +175,47 @@ def test_attend_long_and_many_rows(dev, qt, ct):
             (64, 16, 2, 64, 1111, 1000, None, True, False), (130, 2, 1, 128, 500, 200, None, True, True),
             (64, 4, 4, 256, 1500, 1400, None, False, False), (33, 7, 1, 128, 900, 2000, 850, True, True)):
         _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight)
+
+
+FEW = [(1, 8, 1, 128, 1, 1, None, False, True), (2, 8, 2, 64, 20001, 19000, None, True, True),
+       (4, 4, 2, 128, 17000, 40000, 16990, True, True), (8, 3, 3, 80, 300, 290, None, False, True),
+       (1, 256, 256, 64, 130, 130, None, False, True), (1, 264, 264, 64, 130, 120, None, False, True),
+       (1, 4, 1, 256, 33000, 32990, None, False, True), (2, 4, 1, 128, 70000, 100, None, True, True),
+       (1, 64, 8, 128, 40000, 39999, None, True, True), (9, 1, 1, 64, 700, 650, None, False, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", [(F32, F32), (BF16, BF16), (F32, F16)], ids=["f32", "bf16", "f32_f16"])
+@pytest.mark.parametrize("case", FEW, ids=[f"T{c[0]}_H{c[1]}_D{c[3]}_{c[4]}" for c in FEW])
+def test_attend_few_rows_weight(dev, case, qt, ct):
+    """The slots' weights of few rows come from scores that the attention kept; on both sides of its limits."""
+    _case(dev, *case[:7], qt, ct, *case[7:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+def test_attend_few_rows_hidden_values(dev, qt, ct):
+    """Slots that a row does not see (some in blocks that no row sees) get nothing from it, whatever they hold."""
+    T, heads, slots, D = 3, 2, 700, 128
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(n, heads, D, generator=g) for n in (T, slots, slots))
+    q, k, v = q.to(qt), k.to(ct), v.to(ct)
+    pos = torch.arange(slots)
+    pos[::7] = -1
+    pos[256:400] = -1
+    k[pos < 0] = float("nan")
+    k[650:] = float("inf")
+    q_pos = torch.tensor([600, -1, 640])
+    for workspace in (0, 255):  # (what it held before does not count)
+        ws = torch.full((attention_workspace(T, heads, heads, D, slots, True, dev).numel(),), workspace, dtype=torch.uint8,
+                        device=dev)
+        weight = torch.zeros(slots, device=dev)
+        o = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), q_pos.to(dev), weight=weight, workspace=ws)
+        see = _see(pos, q_pos, None, None)[:, :slots]
+        clean = k.clone()
+        clean[(pos < 0) | (pos > 640)] = 0.0
+        assert bool((o[1] == 0).all())
+        _compare(o.cpu(), weight.cpu(), torch.zeros(slots), q, clean, v, see, D ** -0.5, slots)
 
 
 TILES = [(64, 8, 1, 128, 8300, 8200, None, True, True), (64, 8, 1, 64, 49300, 49000, None, True, True),
