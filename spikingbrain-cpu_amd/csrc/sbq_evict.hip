@@ -584,7 +584,8 @@ int append_from(const AppendArgs& a, int ct, hipStream_t st) {
 // The list (one count more), then the candidates of an append or the counts and keys of a take.
 int64_t list_words(int64_t count) { return (count + 1 + 3) / 4 * 4; }
 int64_t kv_workspace_bytes(int64_t slots, int64_t count) {
-  return 4 * list_words(count) + (slots >= kSpreadFrom ? 4 * (slots + (slots + kChunk - 1) / kChunk * kBins) : 0);
+  if (slots < kSpreadFrom) return 4 * (count + 1);
+  return 4 * (list_words(count) + slots + (slots + kChunk - 1) / kChunk * kBins);
 }
 static_assert(kSpreadTokens * 8 <= kChunk && 2 * kSpreadTokens * 8 <= 3 * kSpreadFrom, "candidates fit 4 bytes a slot");
 

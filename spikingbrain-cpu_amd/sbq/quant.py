@@ -769,20 +769,24 @@ def linear_w4(x2: torch.Tensor, packed: torch.Tensor, gscale: torch.Tensor, bias
     tokens): every further 64 rows read the weight again."""
     x2 = _as_activation(x2)
     M, K = x2.shape
-    gpu = x2.get_device()
-    if gpu < 0 or not x2.is_cuda:
+    gpu, device = x2.get_device(), x2.device
+    if gpu < 0:
         raise ValueError("linear_w4: x must be a GPU tensor")
     _check_w4("linear_w4", packed, gscale, N, K, group, gpu)
     if bias is not None and (bias.dtype != torch.float32 or bias.get_device() != gpu or not bias.is_contiguous()
                              or bias.numel() < N):
-        raise ValueError(f"linear_w4: bias must be a contiguous float32 tensor of N={N} elements on {x2.device}")
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=x2.device)
-    if y.get_device() != gpu or y.shape != (M, N) or y.stride(-1) != 1 or (M > 1 and y.stride(0) < N):
-        raise ValueError(f"linear_w4: out must be a [M={M}, N={N}] tensor with unit column stride on {x2.device}")
-    with _on_device(x2.device):
-        _lib.check(_lib.load().sbq_linear_w4(_ptr(x2), _code(x2.dtype), M, K, _ldx(x2), _ptr(packed), _ptr(gscale),
-                                             _ptr(bias), N, group, _ptr(y), _code(y.dtype), _ldx(y), _stream(x2.device)),
-                   "sbq_linear_w4")
+        raise ValueError(f"linear_w4: bias must be a contiguous float32 tensor of N={N} elements on {device}")
+    if out is None:
+        y, ldy = torch.empty((M, N), dtype=out_dtype, device=device), N
+    elif out.get_device() != gpu or out.shape != (M, N) or out.stride(-1) != 1 or (M > 1 and out.stride(0) < N):
+        raise ValueError(f"linear_w4: out must be a [M={M}, N={N}] tensor with unit column stride on {device}")
+    else:
+        y, ldy = out, _ldx(out)
+    with _on_device(device):
+        _lib.check(_lib.load().sbq_linear_w4(
+            x2.data_ptr(), _DTYPE_CODE[x2.dtype], M, K, K if M <= 1 else x2.stride(0), packed.data_ptr(),
+            gscale.data_ptr(), None if bias is None else bias.data_ptr(), N, group, y.data_ptr(), _code(y.dtype), ldy,
+            _stream(device)), "sbq_linear_w4")
     return y
 
 
@@ -1096,15 +1100,18 @@ class Int4Linear(_Fp32Buffers, nn.Module):
         return unpack_w4(self.packed, self.gscale, self.out_features, self.in_features, self.group)[1]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        packed = self.packed
+        buffers = self._buffers  # (nn.Module's attribute lookup of each costs a good part of a small call)
+        packed = buffers["packed"]
         if not packed.is_cuda:
             raise RuntimeError("sbq Int4Linear: weights are on the CPU; move the module to a ROCm GPU")
         _check_in_features(x, self.in_features)
 
         def run(xd):
-            return linear_w4(_rows(xd), packed, self.gscale, self.bias, self.out_features, self.group, self.out_dtype)
+            return linear_w4(_rows(xd), packed, buffers["gscale"], buffers["bias"], self.out_features, self.group,
+                             self.out_dtype)
 
-        return _like_rows(run(x) if x.device == packed.device else _run_on_device(x, packed.device, run), x.shape)
+        y = run(x) if x.get_device() == packed.get_device() else _run_on_device(x, packed.device, run)
+        return y if x.dim() == 2 else _like_rows(y, x.shape)
 
 
 def save_quantized(layers: dict[str, nn.Module], path: str) -> None:

@@ -74,20 +74,22 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
     has q's.  scale defaults to dim ** -0.5.  weight: fp32 [slots], to which
     the attention weight that each cached slot received, summed over tokens
     and heads, is added."""
-    if not q.is_cuda:
+    gpu, device = q.get_device(), q.device
+    if gpu < 0:
         raise ValueError("tree_attention: q must be a GPU tensor")
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
         raise ValueError("tree_attention: expected q [T, heads, dim] and k, v [slots, kv_heads, dim]")
-    gpu = q.get_device()
     T, heads, dim = q.shape
-    slots, kv_heads = k.shape[0], k.shape[1]
-    if k.dtype not in _DTYPE_CODE or v.dtype != k.dtype or (q.dtype != k.dtype and q.dtype != torch.float32):
+    slots, kv_heads, _ = k.shape
+    qt, ct = q.dtype, k.dtype
+    if ct not in _DTYPE_CODE or v.dtype != ct or (qt != ct and qt != torch.float32):
         raise ValueError("tree_attention: k and v must share a dtype (float32, float16 or bfloat16), q have it or float32")
     if not 1 <= dim <= 256 or kv_heads < 1 or heads < 1 or heads % kv_heads or slots < 1:
         raise ValueError("tree_attention: 1 <= dim <= 256, heads a multiple of kv_heads, and slots >= 1")
     if T > _lib.SBQ_ATTN_MAX_T:
         raise ValueError(f"tree_attention: at most {_lib.SBQ_ATTN_MAX_T} tokens per call")
-    if k.get_device() != gpu or v.get_device() != gpu or k.stride() != v.stride() or (dim > 1 and k.stride(2) != 1):
+    ks = k.stride()
+    if k.get_device() != gpu or v.get_device() != gpu or ks != v.stride() or (dim > 1 and ks[2] != 1):
         raise ValueError(f"tree_attention: k and v must be on {q.device}, with the same strides and unit stride in dim")
     if (slot_pos.dtype != torch.int64 or slot_pos.get_device() != gpu or slot_pos.shape != (slots,)
             or not slot_pos.is_contiguous()):
@@ -114,26 +116,26 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
                                or not weight.is_contiguous()):
         raise ValueError(f"tree_attention: weight must be a contiguous float32 [{slots}] tensor on {q.device}")
     if out is None:
-        out = torch.empty((T, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(2) != 1):
+        out = torch.empty((T, heads, dim), dtype=qt, device=device)
+    elif out.shape != q.shape or out.dtype != qt or out.get_device() != gpu or (dim > 1 and out.stride(2) != 1):
         raise ValueError("tree_attention: out must have q's shape, dtype and device, with unit stride in dim")
     if T == 0:
         return out
     q = _rows_of(q)
     if workspace is None:
-        workspace = attention_workspace(T, heads, kv_heads, dim, slots, weight is not None, q.device)
+        workspace = attention_workspace(T, heads, kv_heads, dim, slots, weight is not None, device)
     elif workspace.get_device() != gpu or not workspace.is_contiguous():
         raise ValueError(f"tree_attention: workspace must be a contiguous tensor on {q.device}")
-    qs, ks, os_ = q.stride(), k.stride(), out.stride()
+    qs, os_ = q.stride(), out.stride()
     ns = (0, 0) if k_new is None else k_new.stride()
-    with _on_device(q.device):
+    with _on_device(device):
         _lib.check(_lib.load().sbq_tree_attention(
-            q.data_ptr(), _DTYPE_CODE[q.dtype], T, heads, dim, qs[0], qs[1], k.data_ptr(), v.data_ptr(),
-            _DTYPE_CODE[k.dtype], slots, kv_heads, ks[0], ks[1], slot_pos.data_ptr(), q_pos.data_ptr(),
+            q.data_ptr(), _DTYPE_CODE[qt], T, heads, dim, qs[0], qs[1], k.data_ptr(), v.data_ptr(), _DTYPE_CODE[ct], slots,
+            kv_heads, ks[0], ks[1], slot_pos.data_ptr(), q_pos.data_ptr(),
             None if k_new is None else k_new.data_ptr(), None if v_new is None else v_new.data_ptr(), ns[0], ns[1],
             None if tree is None else tree.data_ptr(), T, window or 0, dim ** -0.5 if scale is None else scale,
             out.data_ptr(), os_[0], os_[1], None if weight is None else weight.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream(q.device)), "sbq_tree_attention")
+            workspace.numel() * workspace.element_size(), _stream(device)), "sbq_tree_attention")
     return out
 
 
