@@ -86,14 +86,18 @@ struct X8 {
   typedef typename XElem<XT>::T T;
   typedef T V __attribute__((ext_vector_type(8)));
   V v;
-  // `vec`: the row is 16-byte aligned.  Columns from K on are zero.
-  __device__ __forceinline__ void load(const T* row, int k0, int K, bool vec) {
-    if (vec && k0 + 8 <= K) {
-      v = *(const V*)(row + k0);
-    } else {
+  // VEC: the row is 16-byte aligned and K a multiple of 16 bytes.  Columns from
+  // K on are zero.  No branches: those of a piece that may end inside cost more
+  // than the products (64 rows 39 us, without 2x us).
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* row, int k0, int K) {
+    constexpr int N = VEC ? 16 / sizeof(T) : 1;
+    typedef T Part __attribute__((ext_vector_type(N)));
+    Part p[8 / N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = k0 + j < K ? row[k0 + j] : (T)0.0f;
-    }
+    for (int j = 0; j < 8; j += N) p[j / N] = *(const Part*)(row + (k0 + j < K ? k0 + j : 0));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k0 + j / N * N < K ? p[j / N][j % N] : (T)0.0f;
   }
 };
 
@@ -141,13 +145,13 @@ struct W4Args {
   void* y;
   int64_t ldx, ldy;
   int M, N, K, Nt, Kc, yt;
-  bool xvec, yvec;
+  bool yvec;
 };
 
 // XT: activations; MT: 16-row tiles of x; G: 16-row tiles of the weight; GS:
 // MFMA steps per group (1, 2, 4); ROWS: 0 direct, else STAGE of 1, 2, 4 or 8
-// rows; D: K tiles loaded together.
-template <int XT, int MT, int G, int GS, int ROWS, int D>
+// rows; D: K tiles loaded together; VEC: as X8::load.
+template <int XT, int MT, int G, int GS, int ROWS, int D, bool VEC>
 __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
   typedef typename XElem<XT>::T T;
   typedef W4Math<XT> Math;
@@ -194,14 +198,14 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            raw[d][t][s].load(x + (int64_t)min(t * 16 + c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K, a.xvec);
+            raw[d][t][s].template load<VEC>(x + (int64_t)min(t * 16 + c, M - 1) * a.ldx, kt * 128 + s * 32 + g * 8, a.K);
       }
     }
     if constexpr (ROWS > 0) {
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {  // lane group g: pair p * 4 + g = (tile, row)
         const int pair = p * 4 + g, kt = min(kb + pair / ROWS * KS, a.Kc - 1);
-        raw[p][0][0].load(x + (int64_t)min(pair % ROWS, M - 1) * a.ldx, kt * 128 + c * 8, a.K, a.xvec);
+        raw[p][0][0].template load<VEC>(x + (int64_t)min(pair % ROWS, M - 1) * a.ldx, kt * 128 + c * 8, a.K);
       }
       wave_lds_fence();
 #pragma unroll
@@ -400,25 +404,31 @@ __global__ __launch_bounds__(256) void unpack_scale_kernel(const uint16_t* gscal
 
 inline unsigned blocks(int64_t count) { return (unsigned)((count + 255) / 256); }
 
-template <int XT, int MT, int G, int ROWS, int D>
+template <int XT, int MT, int G, int ROWS, int D, bool VEC = true>
 int launch_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   constexpr int P = XT == XT_F32 ? 2 : 1;
   const int stage = KS * D * ROWS * (P * 256 + (P == 2 ? 4 : 0)), red = KS > 1 ? KS * G * MT * 1024 : 0;
   const size_t lds = (size_t)(stage > red ? stage : red);
   const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
   if (group == 32)
-    linear_w4_kernel<XT, MT, G, 1, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 1, ROWS, D, VEC><<<grid, KS * 64, lds, st>>>(a);
   else if (group == 64)
-    linear_w4_kernel<XT, MT, G, 2, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 2, ROWS, D, VEC><<<grid, KS * 64, lds, st>>>(a);
   else
-    linear_w4_kernel<XT, MT, G, 4, ROWS, D><<<grid, KS * 64, lds, st>>>(a);
+    linear_w4_kernel<XT, MT, G, 4, ROWS, D, VEC><<<grid, KS * 64, lds, st>>>(a);
   return check_launch();
 }
 
 template <int XT>
-int pick_w4(const W4Args& a, int group, hipStream_t st) {
+int pick_w4(const W4Args& a, bool xvec, int group, hipStream_t st) {
   int KS = 1;
   while (KS < kW4MaxWaves && KS * 2 < a.Kc) KS *= 2;
+  if (!xvec) {  // rows that are not aligned: element by element, in the widest form of each kind
+    if (a.M == 1) return launch_w4<XT, 1, 1, 1, 4, false>(a, group, KS, st);
+    if (a.M <= 8) return launch_w4<XT, 1, 1, 8, 2, false>(a, group, KS, st);
+    if (a.M <= 16) return launch_w4<XT, 1, 1, 0, 1, false>(a, group, KS, st);
+    return launch_w4<XT, 4, 2, 0, 1, false>(a, group, KS, st);
+  }
   const bool wide = a.Nt >= kW4WideTiles;
   if (a.M == 1) return wide ? launch_w4<XT, 1, 2, 1, 4>(a, group, KS, st) : launch_w4<XT, 1, 1, 1, 4>(a, group, KS, st);
   if (a.M == 2) return wide ? launch_w4<XT, 1, 2, 2, 4>(a, group, KS, st) : launch_w4<XT, 1, 1, 2, 4>(a, group, KS, st);
@@ -467,13 +477,14 @@ int launch_linear_w4(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, b
                      hipStream_t st) {
   constexpr int64_t kRows = 1 << 20;  // rows per launch (the grid's second dimension holds 65535 blocks)
   const int64_t xs = xt == XT_F32 ? 4 : 2, ys = yt == XT_F32 ? 4 : 2;
+  xvec = xvec && K * xs % 16 == 0;
   for (int64_t m = 0; m < M; m += kRows) {
     const W4Args a{(const uint8_t*)x + m * ldx * xs, packed, gscale, bias, (uint8_t*)y + m * ldy * ys, ldx, ldy,
                    (int)(M - m < kRows ? M - m : kRows), (int)N, (int)K, (int)((N + 15) / 16), (int)((K + 127) / 128), yt,
-                   xvec, yvec};
-    const int rc = xt == XT_F32   ? pick_w4<XT_F32>(a, group, st)
-                   : xt == XT_F16 ? pick_w4<XT_F16>(a, group, st)
-                                  : pick_w4<XT_BF16>(a, group, st);
+                   yvec};
+    const int rc = xt == XT_F32   ? pick_w4<XT_F32>(a, xvec, group, st)
+                   : xt == XT_F16 ? pick_w4<XT_F16>(a, xvec, group, st)
+                                  : pick_w4<XT_BF16>(a, xvec, group, st);
     if (rc) return rc;
   }
   return 0;
