@@ -26,6 +26,7 @@
 //   direct  otherwise: each lane converts the fragment it multiplies; the
 //           fragments of all row tiles of a K tile are loaded together
 #include "sbq_common.h"
+#include "sbq_dma.h"
 #include "sbq_launch.h"
 
 namespace sbq {
@@ -33,6 +34,7 @@ namespace sbq {
 namespace {
 
 constexpr int kW4MaxWaves = 8;
+constexpr int kW4RowGroups = 256;
 constexpr int kW4WideTiles = 2048;  // 16-row tiles from which a decode workgroup takes two
 
 // 8 nibbles u = q + 8 -> fp16 q: element 2i in nibble i, 2i + 1 in nibble
@@ -101,26 +103,32 @@ struct X8 {
   }
 };
 
-// Largest finite magnitude of 8 fp32 values (NaN and infinities left out).
+// Largest magnitude of 8 fp32 values (NaN left out; FINITE: infinities too).
+template <bool FINITE>
 __device__ __forceinline__ float max_abs8(const X8<XT_F32>::V& v) {
   float m = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float a = __builtin_fabsf(v[j]);
-    m = a <= 3.4028235e38f ? __builtin_fmaxf(m, a) : m;
+    m = !FINITE || a <= 3.4028235e38f ? __builtin_fmaxf(m, a) : m;
   }
   return m;
 }
 
-// Two fp16 planes of v * 2^e: hi rounded to nearest, lo the remainder.  An
-// infinity stays one (its remainder would be NaN).
+// Two fp16 planes of v * 2^e (s = 2^e): hi rounded to nearest, lo the
+// remainder.  An infinity stays one (ODD; its remainder would be NaN).  Two
+// values at a time: this conversion is most of a wave's work at fp32.
+template <bool ODD>
 __device__ __forceinline__ void split_f16(const X8<XT_F32>::V& v, float s, f16x8& hi, f16x8& lo) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = v[j] * s;
-    hi[j] = (_Float16)t;
-    const float r = t - (float)hi[j];
-    lo[j] = (_Float16)(__builtin_fabsf(t) > 3.4028235e38f ? 0.0f : r);
+  for (int j = 0; j < 8; j += 2) {
+    const f32x2 t = {v[j] * s, v[j + 1] * s};
+    const f16x2 h = __builtin_convertvector(t, f16x2);
+    f32x2 r = {__builtin_fmaf(v[j], s, -(float)h.x), __builtin_fmaf(v[j + 1], s, -(float)h.y)};
+    if (ODD) r = f32x2{__builtin_fabsf(t.x) > 3.4028235e38f ? 0.0f : r.x, __builtin_fabsf(t.y) > 3.4028235e38f ? 0.0f : r.y};
+    const f16x2 l = __builtin_convertvector(r, f16x2);
+    hi[j] = h.x, hi[j + 1] = h.y, lo[j] = l.x, lo[j + 1] = l.y;
   }
 }
 
@@ -137,6 +145,57 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// The two planes of the lane's N pieces of a row's K tile, whose maximum
+// `across` takes over the lanes that share the row; the factor to multiply the
+// products by.
+template <int N, class F>
+__device__ __forceinline__ float split_tile(const X8<XT_F32> (&raw)[N], f16x8 (&hi)[N], f16x8 (&lo)[N], F across) {
+  float mx = 0.0f;
+#pragma unroll
+  for (int s = 0; s < N; ++s) mx = __builtin_fmaxf(mx, max_abs8<false>(raw[s].v));
+  mx = across(mx);
+  const bool odd = __any(mx == __builtin_inff());
+  if (__builtin_expect(odd, false)) {
+    mx = 0.0f;
+#pragma unroll
+    for (int s = 0; s < N; ++s) mx = __builtin_fmaxf(mx, max_abs8<true>(raw[s].v));
+    mx = across(mx);
+  }
+  const int e = tile_exp(mx);
+  if (__builtin_expect(odd, false)) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) split_f16<true>(raw[s].v, exp2i(e), hi[s], lo[s]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < N; ++s) split_f16<false>(raw[s].v, exp2i(e), hi[s], lo[s]);
+  }
+  return exp2i(-e);
+}
+// ... over the lane groups of a fragment's row
+__device__ __forceinline__ float max_groups(float mx) {
+  mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
+  return __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+}
+
+// acc += one 16x16 tile over a K tile: each group's partial sums times its
+// scales (b: bf16, four rows of the weight) and the row's factor f.
+template <int XT, int GS, int P>
+__device__ __forceinline__ void add_tile(const typename W4Math<XT>::V (&wv)[4], const typename W4Math<XT>::V (&xv)[P][4],
+                                         const u32x2 (&b)[4 / GS], float f, f32x4& acc) {
+#pragma unroll
+  for (int q = 0; q < 4 / GS; ++q) {
+    f32x4 part = (f32x4)(0.0f);
+#pragma unroll
+    for (int s = q * GS; s < q * GS + GS; ++s)
+#pragma unroll
+      for (int p = 0; p < P; ++p) part = W4Math<XT>::mfma(wv[s], xv[p][s], part);
+    const f32x4 s4 = {__uint_as_float(b[q].x << 16), __uint_as_float(b[q].x & 0xffff0000u),
+                      __uint_as_float(b[q].y << 16), __uint_as_float(b[q].y & 0xffff0000u)};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(part[v], s4[v] * f, acc[v]);
+  }
+}
+
 struct W4Args {
   const void* x;
   const uint8_t* packed;
@@ -147,6 +206,45 @@ struct W4Args {
   int M, N, K, Nt, Kc, yt;
   bool yvec;
 };
+
+// The waves' partial sums, added in wave order, and the rows out.  lds is free
+// once every wave is here.
+template <int G, int MT>
+__device__ __forceinline__ void join_w4(const W4Args& a, const f32x4 (&acc)[G][MT], uint8_t* lds, int nt0, int m0) {
+  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int c = lane & 15, g = lane >> 4, M = min(a.M - m0, MT * 16);
+  if (KS > 1) {
+    f32x4* const red = (f32x4*)lds;
+    __syncthreads();  // (the staging area is done with)
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) red[(ks * G * MT + i * MT + t) * 64 + lane] = acc[i][t];
+    __syncthreads();
+  }
+  for (int u = ks; u < G * MT; u += KS) {
+    const int i = u / MT, t = u % MT;
+    f32x4 v;
+    if (KS > 1) {
+      const f32x4* const red = (const f32x4*)lds;
+      v = red[u * 64 + lane];
+      for (int k = 1; k < KS; ++k) v += red[(k * G * MT + u) * 64 + lane];
+    } else {
+#pragma unroll
+      for (int ii = 0; ii < G; ++ii)
+#pragma unroll
+        for (int tt = 0; tt < MT; ++tt)
+          if (ii == i && tt == t) v = acc[ii][tt];
+    }
+    const int m = t * 16 + c, n = (nt0 + i) * 16 + 4 * g;
+    if (m >= M || n >= a.N) continue;
+    if (a.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += n + j < a.N ? a.bias[n + j] : 0.0f;
+    }
+    store_y4(a.y, a.yt, (int64_t)(m0 + m) * a.ldy + n, v, a.yvec, a.N - n);
+  }
+}
 
 // XT: activations; MT: 16-row tiles of x; G: 16-row tiles of the weight; GS:
 // MFMA steps per group (1, 2, 4); ROWS: 0 direct, else STAGE of 1, 2, 4 or 8
@@ -213,15 +311,15 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
         const int pair = p * 4 + g;
         uint8_t* const to = stage + pair * 256 + ((c ^ pair) & 15) * 16;
         if constexpr (XT == XT_F32) {
-          float mx = max_abs8(raw[p][0][0].v);
+          f16x8 hi[1], lo[1];
+          const float f = split_tile(raw[p][0], hi, lo, [](float mx) {
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
-          const int e = tile_exp(mx);
-          f16x8 hi, lo;
-          split_f16(raw[p][0][0].v, exp2i(e), hi, lo);
-          *(f16x8*)to = hi;
-          *(f16x8*)(to + D * ROWS * 256) = lo;
-          if (c == 0) factor[pair] = exp2i(-e);
+            for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
+            return mx;
+          });
+          *(f16x8*)to = hi[0];
+          *(f16x8*)(to + D * ROWS * 256) = lo[0];
+          if (c == 0) factor[pair] = f;
         } else {
           *(V*)to = __builtin_bit_cast(V, raw[p][0][0].v);
         }
@@ -251,70 +349,133 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
           }
           if constexpr (XT == XT_F32) f = factor[pair];
         } else if constexpr (XT == XT_F32) {
-          float mx = 0.0f;
-#pragma unroll
-          for (int s = 0; s < 4; ++s) mx = __builtin_fmaxf(mx, max_abs8(raw[d][t][s].v));
-          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const int e = tile_exp(mx);
-          f = exp2i(-e);
-#pragma unroll
-          for (int s = 0; s < 4; ++s) split_f16(raw[d][t][s].v, exp2i(e), xv[0][s], xv[1][s]);
+          f = split_tile(raw[d][t], xv[0], xv[1], max_groups);
         } else {
 #pragma unroll
           for (int s = 0; s < 4; ++s) xv[0][s] = __builtin_bit_cast(V, raw[d][t][s].v);
         }
 #pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-          for (int q = 0; q < GPT; ++q) {
-            f32x4 part = (f32x4)(0.0f);
-#pragma unroll
-            for (int s = q * GS; s < q * GS + GS; ++s)
-#pragma unroll
-              for (int p = 0; p < P; ++p) part = Math::mfma(wv[i][s], xv[p][s], part);
-            const u32x2 b = sc[d][i][q];
-            const f32x4 s4 = {__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u),
-                              __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
-#pragma unroll
-            for (int v = 0; v < 4; ++v) acc[i][t][v] = __builtin_fmaf(part[v], s4[v] * f, acc[i][t][v]);
-          }
+        for (int i = 0; i < G; ++i) add_tile<XT, GS>(wv[i], xv, sc[d][i], f, acc[i][t]);
       }
     }
   }
 
-  // the waves' partial sums, added in wave order
-  if (KS > 1) {
-    f32x4* const red = (f32x4*)lds;
-    __syncthreads();  // (the staging area is done with)
+  join_w4<G, MT>(a, acc, lds, nt0, m0);
+}
+
+// More than 8 rows, aligned.  A fragment read straight from memory takes one
+// line per lane (its lanes are 16 rows), four times the time of the bytes, so
+// the wave copies its K tiles' rows into LDS 8 KiB at a time (whole rows' 256
+// or 512 bytes, two chunks under way, their 16-byte pieces permuted by the row)
+// and reads fragments there.  Two chunks and one K tile's weights are always
+// under way; the last ones of a wave once more.
+template <int XT, int MT, int G, int GS>
+__global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
+  typedef typename XElem<XT>::T T;
+  typedef W4Math<XT> Math;
+  typedef typename Math::V V;
+  constexpr int P = XT == XT_F32 ? 2 : 1, ES = sizeof(T), GPT = 4 / GS;
+  constexpr int CT = MT < 4 / ES ? MT : 4 / ES, NCH = MT / CT;  // row tiles of a chunk, chunks of a K tile
+  constexpr int PPR = 8 * ES, NDMA = CT * 2 * ES, CHUNK = CT * 16 * 128 * ES, NW = G * (1 + GPT);
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int c = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.y * (MT * 16), M = min(a.M - m0, MT * 16);
+  const int nt0 = blockIdx.x * G;
+  const T* const x = (const T*)a.x + (int64_t)m0 * a.ldx;
+  uint8_t* const own = lds + ks * (2 * CHUNK);
+
+  f32x4 acc[G][MT];
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[i][t] = (f32x4)(0.0f);
+
+  u32x4 w[G];
+  u32x2 sc[2][G][GPT];
+  auto load = [&](int kt, u32x2 (&sc)[G][GPT]) {
+    asm volatile("" ::: "memory");  // (their order among the copies is counted on)
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int64_t at = (int64_t)min(nt0 + i, a.Nt - 1) * a.Kc + kt;
+      w[i] = *(const u32x4*)(a.packed + (at * 64 + lane) * 16);
+#pragma unroll
+      for (int q = 0; q < GPT; ++q) sc[i][q] = *(const u32x2*)(a.gscale + (at * GPT + q) * 16 + 4 * g);
+    }
+    asm volatile("" ::: "memory");
+  };
+  auto copy = [&](int kt, int ch, int buf) {
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (else the addresses of all copies are kept in registers)
+#pragma unroll
+    for (int i = 0; i < NDMA; ++i) {
+      const int row = i * (64 / PPR) + l / PPR, k = kt * 128 + ((l % PPR) ^ (row & 15)) * (16 / ES);
+      const T* const src = x + (int64_t)min(ch * CT * 16 + row, M - 1) * a.ldx + (k < a.K ? k : 0);
+      __builtin_amdgcn_global_load_lds((const void*)src,
+                                       (__attribute__((address_space(3))) void*)(own + buf * CHUNK + i * 1024), 16, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  };
+
+  int buf = 0;
+  auto tile = [&](int kt, const u32x2 (&b)[G][GPT], u32x2 (&next)[G][GPT]) {
+    V wv[G][4];
 #pragma unroll
     for (int i = 0; i < G; ++i)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) red[(ks * G * MT + i * MT + t) * 64 + lane] = acc[i][t];
-    __syncthreads();
-  }
-  for (int u = ks; u < G * MT; u += KS) {
-    const int i = u / MT, t = u % MT;
-    f32x4 v;
-    if (KS > 1) {
-      const f32x4* const red = (const f32x4*)lds;
-      v = red[u * 64 + lane];
-      for (int k = 1; k < KS; ++k) v += red[(k * G * MT + u) * 64 + lane];
-    } else {
+      for (int s = 0; s < 4; ++s) wv[i][s] = Math::weight(w[i][s]);
+    load(min(kt + KS, a.Kc - 1), next);
+    const bool tail = kt * 128 + 128 > a.K;
 #pragma unroll
-      for (int ii = 0; ii < G; ++ii)
+    for (int ch = 0; ch < NCH; ++ch) {
+      if (ch < 2)  // all but the next chunk, and the next weights where they came after this one
+        wait_vmcnt<NDMA + NW>();
+      else
+        wait_vmcnt<NDMA>();
+      asm volatile("" ::: "memory");
 #pragma unroll
-        for (int tt = 0; tt < MT; ++tt)
-          if (ii == i && tt == t) v = acc[ii][tt];
+      for (int tc = 0; tc < CT; ++tc) {
+        const int t = ch * CT + tc;
+        X8<XT> raw[4];
+        const uint8_t* const from = own + buf * CHUNK + (tc * 16 + c) * (128 * ES);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          u32x4 piece[ES / 2];
+#pragma unroll
+          for (int h = 0; h < ES / 2; ++h) {
+            const int p = (s * 4 + g) * (ES / 2) + h;
+            piece[h] = *(const u32x4*)(from + (p ^ c) * 16);
+            if (tail && kt * 128 + p * (16 / ES) >= a.K) piece[h] = (u32x4)(0u);
+          }
+          __builtin_memcpy(&raw[s].v, piece, sizeof(piece));
+        }
+        V xv[P][4];
+        float f = 1.0f;
+        if constexpr (XT == XT_F32) {
+          f = split_tile(raw, xv[0], xv[1], max_groups);
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) xv[0][s] = __builtin_bit_cast(V, raw[s].v);
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) add_tile<XT, GS>(wv[i], xv, b[i], f, acc[i][t]);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the chunk is read
+      asm volatile("" ::: "memory");
+      copy(min(kt + (ch + 2) / NCH * KS, a.Kc - 1), (ch + 2) % NCH, buf);
+      buf ^= 1;
     }
-    const int m = t * 16 + c, n = (nt0 + i) * 16 + 4 * g;
-    if (m >= M || n >= a.N) continue;
-    if (a.bias) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += n + j < a.N ? a.bias[n + j] : 0.0f;
-    }
-    store_y4(a.y, a.yt, (int64_t)(m0 + m) * a.ldy + n, v, a.yvec, a.N - n);
+  };
+  load(ks, sc[0]);
+  copy(ks, 0, 0);
+  copy(NCH == 1 ? min(ks + KS, a.Kc - 1) : ks, NCH == 1 ? 0 : 1, 1);
+#pragma unroll 1
+  for (int kt = ks; kt < a.Kc; kt += 2 * KS) {
+    tile(kt, sc[0], sc[1]);
+    if (kt + KS < a.Kc) tile(kt + KS, sc[1], sc[0]);
   }
+  wait_vmcnt<0>();  // (no copy outlives the area)
+  join_w4<G, MT>(a, acc, lds, nt0, m0);
 }
 
 // ---------------------------------------------------------------------------
@@ -419,6 +580,27 @@ int launch_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   return check_launch();
 }
 
+template <int XT, int MT, int G>
+int launch_rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
+  constexpr int ES = XT == XT_F32 ? 4 : 2, CT = MT < 4 / ES ? MT : 4 / ES;
+  const int stage = KS * 2 * CT * 16 * 128 * ES, red = KS > 1 ? KS * G * MT * 1024 : 0;
+  const size_t lds = (size_t)(stage > red ? stage : red);
+  const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
+  if (group == 32)
+    rows_w4_kernel<XT, MT, G, 1><<<grid, KS * 64, lds, st>>>(a);
+  else if (group == 64)
+    rows_w4_kernel<XT, MT, G, 2><<<grid, KS * 64, lds, st>>>(a);
+  else
+    rows_w4_kernel<XT, MT, G, 4><<<grid, KS * 64, lds, st>>>(a);
+  return check_launch();
+}
+template <int XT, int MT>
+int rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
+  if (a.Nt <= kW4RowGroups) return launch_rows_w4<XT, MT, 1>(a, group, KS, st);
+  if (XT == XT_F32 || a.Nt <= 2 * kW4RowGroups) return launch_rows_w4<XT, MT, 2>(a, group, KS, st);
+  if constexpr (XT != XT_F32) return launch_rows_w4<XT, MT, 3>(a, group, KS, st);
+}
+
 template <int XT>
 int pick_w4(const W4Args& a, bool xvec, int group, hipStream_t st) {
   int KS = 1;
@@ -434,9 +616,9 @@ int pick_w4(const W4Args& a, bool xvec, int group, hipStream_t st) {
   if (a.M == 2) return wide ? launch_w4<XT, 1, 2, 2, 4>(a, group, KS, st) : launch_w4<XT, 1, 1, 2, 4>(a, group, KS, st);
   if (a.M <= 4) return wide ? launch_w4<XT, 1, 2, 4, 2>(a, group, KS, st) : launch_w4<XT, 1, 1, 4, 2>(a, group, KS, st);
   if (a.M <= 8) return launch_w4<XT, 1, 1, 8, 2>(a, group, KS, st);
-  if (a.M <= 16) return launch_w4<XT, 1, 1, 0, 2>(a, group, KS, st);
-  if (a.M <= 32) return launch_w4<XT, 2, 2, 0, 1>(a, group, KS, st);
-  return launch_w4<XT, 4, 2, 0, 1>(a, group, KS, st);
+  if (a.M <= 16) return rows_w4<XT, 1>(a, group, KS, st);
+  if (a.M <= 32) return rows_w4<XT, 2>(a, group, KS, st);
+  return rows_w4<XT, 4>(a, group, KS, st);
 }
 
 }  // namespace
