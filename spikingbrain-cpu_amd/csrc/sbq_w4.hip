@@ -211,7 +211,7 @@ struct W4Args {
 // once every wave is here.
 template <int G, int MT>
 __device__ __forceinline__ void join_w4(const W4Args& a, const f32x4 (&acc)[G][MT], uint8_t* lds, int nt0, int m0) {
-  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KS = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4, M = min(a.M - m0, MT * 16);
   if (KS > 1) {
     f32x4* const red = (f32x4*)lds;
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
   constexpr int STAGE = P * D * ROWS * 256;  // bytes of a wave, then the pairs' factors
   static_assert(ROWS == 0 || (MT == 1 && D * ROWS % 4 == 0), "staging serves one row tile, four pairs at a time");
   extern __shared__ __align__(16) uint8_t lds[];
-  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KS = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * (MT * 16), M = min(a.M - m0, MT * 16);
   const int nt0 = blockIdx.x * G;
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
   constexpr int CT = MT < 4 / ES ? MT : 4 / ES, NCH = MT / CT;  // row tiles of a chunk, chunks of a K tile
   constexpr int PPR = 8 * ES, NDMA = CT * 2 * ES, CHUNK = CT * 16 * 128 * ES, NW = G * (1 + GPT);
   extern __shared__ __align__(16) uint8_t lds[];
-  const int lane = threadIdx.x & 63, ks = threadIdx.x >> 6, KS = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KS = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * (MT * 16), M = min(a.M - m0, MT * 16);
   const int nt0 = blockIdx.x * G;
@@ -419,6 +419,8 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
 
   int buf = 0;
   auto tile = [&](int kt, const u32x2 (&b)[G][GPT], u32x2 (&next)[G][GPT]) {
+    wait_vmcnt<2 * NDMA>();  // the weights; the two chunks after them stay under way
+    asm volatile("" ::: "memory");
     V wv[G][4];
 #pragma unroll
     for (int i = 0; i < G; ++i)
@@ -597,7 +599,8 @@ int launch_rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
 template <int XT, int MT>
 int rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   if (a.Nt <= kW4RowGroups) return launch_rows_w4<XT, MT, 1>(a, group, KS, st);
-  if (XT == XT_F32 || a.Nt <= 2 * kW4RowGroups) return launch_rows_w4<XT, MT, 2>(a, group, KS, st);
+  // (three of 32 columns' groups beside 64 rows do not fit the registers)
+  if (XT == XT_F32 || a.Nt <= 2 * kW4RowGroups || (MT == 4 && group == 32)) return launch_rows_w4<XT, MT, 2>(a, group, KS, st);
   if constexpr (XT != XT_F32) return launch_rows_w4<XT, MT, 3>(a, group, KS, st);
 }
 
