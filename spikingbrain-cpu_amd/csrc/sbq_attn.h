@@ -965,7 +965,7 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
   lo_min = __shfl((long long)lo_min, 0, 64), lo_max = __shfl((long long)lo_max, 0, 64);
   hi_min = __shfl((long long)hi_min, 0, 64), hi_max = __shfl((long long)hi_max, 0, 64);
   if (!__any(sp >= lo_min && sp <= hi_max)) return;  // (the same for every wave)
-  const bool full = __all(sp >= lo_max && sp <= hi_min);
+  const bool full = __all(sp < 0 || (sp >= lo_max && sp <= hi_min));  // (an empty slot's sum is not written)
 
   Piece<CT, E, MODE> kf[SUB][NCH];
   float acc[SUB][4] = {};
@@ -1021,7 +1021,7 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
     float x = sums[0][threadIdx.x];
 #pragma unroll
     for (int k = 1; k < kWeightWaves; ++k) x += sums[k][threadIdx.x];
-    weight[base + threadIdx.x] += x;
+    if (a.slot_pos[base + threadIdx.x] >= 0) weight[base + threadIdx.x] += x;
   }
 }
 
@@ -1060,8 +1060,8 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
     hi_min = min(hi_min, (int64_t)__shfl_xor((long long)hi_min, o, 64));
     hi_max = max(hi_max, (int64_t)__shfl_xor((long long)hi_max, o, 64));
   }
-  const bool any = __any(sp >= lo_min && sp <= hi_max), full = __all(sp >= lo_max && sp <= hi_min);
-  if (!__syncthreads_or(any)) return;
+  const bool any = __any(sp >= lo_min && sp <= hi_max), full = __all(sp < 0 || (sp >= lo_max && sp <= hi_min));
+  if (!__syncthreads_or(any)) return;  // (full: an empty slot's sum is not written)
 
   // The rows that are copied next, 64 of a key head, and their maxima and sums
   // (by every wave, so that all have as many copies under way).
@@ -1169,7 +1169,7 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) x += __shfl_xor(x, o, 64);
     const int at = base + (v / 4) * 8 + 4 * h + v % 4;
-    if (r == 0 && at <= last) weight[at] += x;
+    if (r == 0 && at <= last && a.slot_pos[at] >= 0) weight[at] += x;
   }
 }
 
