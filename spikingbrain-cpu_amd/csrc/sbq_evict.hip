@@ -11,10 +11,12 @@
 // share the first digit are set apart for the other two passes.  A single new
 // token needs no more than the smallest key and its slot.
 //
-// What bounds it is one CU's reading from HBM (12 bytes per slot at some 23
-// GB/s) and the latency of the steps, so from 8192 slots on a launch before it
-// spreads the reading: for an append every workgroup leaves the T first of its
-// 4096 slots (which hold the T first of all), for a take the 4-byte keys.
+// What bounds it is the latency of the steps of one workgroup, so from 8192
+// slots on a launch before it spreads the reading: for an append every
+// workgroup leaves the T first of its 4096 slots (which hold the T first of
+// all), for a take the 4-byte keys and their first digits' counts.  One token
+// into 4096 slots of 8 x 128: 3.9 us; 12 into 32768: 11 us, 4.8 for the choice
+// among theirs and 3 for the rows; 4096 of 32768 slots taken: 4, 23 and 7 us.
 // Integer counts only, so the result does not depend on timing.
 #include "sbq_common.h"
 #include "sbq_launch.h"

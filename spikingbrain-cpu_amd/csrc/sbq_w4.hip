@@ -3,8 +3,11 @@
 //   y[m,n] = sum_G s[n,G] * (sum_{k in G} q[n,k] x[m,k]) (+ bias[n]),
 //   q in -8..7, G = groups of 32, 64 or 128 columns, s in bf16.
 //
-// What bounds it: the weight stream (N K / 2 bytes) at one to a few rows of
-// x; from about 16 rows on also the conversions.  A packed tile is 16 rows x
+// What bounds it: at one row the conversions of the weights (some 140 vector
+// instructions a tile and wave; 151936 x 2560: fp16 53 us, fp32 74 us, 39 us
+// for the bytes at a large copy's rate); at many rows reading x, once per
+// workgroup (64 rows over 12288 x 4096: fp16 17 us, bf16 19, fp32 33), and at
+// fp32 splitting it.  A packed tile is 16 rows x
 // 128 columns in 1 KiB, one 16-byte load per lane, in the order of the MFMA A
 // operand: lane = g*16 + r holds row r, dword s the columns 32 s + 8 g + 0..7
 // of the tile, so that each group of 32 columns is one 16x16x32 MFMA step and
@@ -23,8 +26,9 @@
 //           per row and tile (a single row: four tiles at a time), and reads
 //           fragments from there; a fragment read straight from memory would be
 //           converted 16 times over at one row
-//   direct  otherwise: each lane converts the fragment it multiplies; the
-//           fragments of all row tiles of a K tile are loaded together
+//   rows    more: rows are copied into LDS as they are (rows_w4_kernel)
+//   direct  more, and not aligned for those copies: each lane reads the
+//           fragment it multiplies
 #include "sbq_common.h"
 #include "sbq_dma.h"
 #include "sbq_launch.h"
@@ -34,6 +38,10 @@ namespace sbq {
 namespace {
 
 constexpr int kW4MaxWaves = 8;
+// rows_w4_kernel: weight tiles (of 16 rows) up to which a workgroup takes one;
+// two up to twice as many, then three.  A CU holds one workgroup, each of which
+// reads all of x.  64 bf16 rows, K 4096: 256 tiles 13 us by one each, 18 by
+// three; 512 tiles 24 by one, 16 by two, 18 by three; 768 tiles 33, 28 and 19.
 constexpr int kW4RowGroups = 256;
 constexpr int kW4WideTiles = 2048;  // 16-row tiles from which a decode workgroup takes two
 
@@ -89,8 +97,8 @@ struct X8 {
   typedef T V __attribute__((ext_vector_type(8)));
   V v;
   // VEC: the row is 16-byte aligned and K a multiple of 16 bytes.  Columns from
-  // K on are zero.  No branches: those of a piece that may end inside cost more
-  // than the products (64 rows 39 us, without 2x us).
+  // K on are zero, by selection: with a branch per piece one row over 151936 x
+  // 2560 took 87 us, without 79.
   template <bool VEC>
   __device__ __forceinline__ void load(const T* row, int k0, int K) {
     constexpr int N = VEC ? 16 / sizeof(T) : 1;
@@ -367,8 +375,9 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
 // line per lane (its lanes are 16 rows), four times the time of the bytes, so
 // the wave copies its K tiles' rows into LDS 8 KiB at a time (whole rows' 256
 // or 512 bytes, two chunks under way, their 16-byte pieces permuted by the row)
-// and reads fragments there.  Two chunks and one K tile's weights are always
-// under way; the last ones of a wave once more.
+// and reads fragments there: 64 rows over 12288 x 4096, bf16, 39.5 us without,
+// 19 with.  Two chunks and one K tile's weights are always under way; the last
+// ones of a wave once more.
 template <int XT, int MT, int G, int GS>
 __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
   typedef typename XElem<XT>::T T;
@@ -588,9 +597,9 @@ int launch_rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   const int stage = KS * 2 * CT * 16 * 128 * ES, red = KS > 1 ? KS * G * MT * 1024 : 0;
   const size_t lds = (size_t)(stage > red ? stage : red);
   const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
-  if (group == 32)
-    rows_w4_kernel<XT, MT, G, 1><<<grid, KS * 64, lds, st>>>(a);
-  else if (group == 64)
+  if (group == 32) {
+    if constexpr (G < 3 || (MT < 4 && XT != XT_F32)) rows_w4_kernel<XT, MT, G, 1><<<grid, KS * 64, lds, st>>>(a);
+  } else if (group == 64)
     rows_w4_kernel<XT, MT, G, 2><<<grid, KS * 64, lds, st>>>(a);
   else
     rows_w4_kernel<XT, MT, G, 4><<<grid, KS * 64, lds, st>>>(a);
@@ -599,9 +608,9 @@ int launch_rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
 template <int XT, int MT>
 int rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   if (a.Nt <= kW4RowGroups) return launch_rows_w4<XT, MT, 1>(a, group, KS, st);
-  // (three of 32 columns' groups beside 64 rows do not fit the registers)
-  if (XT == XT_F32 || a.Nt <= 2 * kW4RowGroups || (MT == 4 && group == 32)) return launch_rows_w4<XT, MT, 2>(a, group, KS, st);
-  if constexpr (XT != XT_F32) return launch_rows_w4<XT, MT, 3>(a, group, KS, st);
+  // (three tiles of 32-column groups beside 64 rows, or beside fp32's planes, do not fit the registers)
+  if (a.Nt <= 2 * kW4RowGroups || (group == 32 && (MT == 4 || XT == XT_F32))) return launch_rows_w4<XT, MT, 2>(a, group, KS, st);
+  return launch_rows_w4<XT, MT, 3>(a, group, KS, st);
 }
 
 template <int XT>

@@ -126,6 +126,24 @@ def test_linear_w4(dev, N, K, dtype, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("N,K", [(4100, 264), (8208, 2184), (32770, 136)])
+def test_linear_w4_wide(dev, N, K, dtype, group):
+    """Layers wide enough for workgroups of two and three weight tiles, all K
+    ends inside a tile; what lies beyond K in x's rows does not count."""
+    q, s = _weight(N, K, group, N)
+    packed, gscale = quant.repack_w4(q.to(dev), s.to(dev), group)
+    for M in (1, 2, 3, 8, 9, 20, 40, 64, 70) if N < 32770 else (1, 2, 4, 24):
+        x = _x(M, K, dtype, M)
+        wide = torch.full((M, K + 24), float("nan"), dtype=dtype)
+        wide[:, :K] = x
+        announce(f"linear_w4 wide M={M} N={N} K={K} group={group} {dtype}")
+        y = quant.linear_w4(wide.to(dev)[:, :K], packed, gscale, None, N, group)
+        _check(y.cpu(), x, q, s, None, group, F32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_linear_w4_strides_and_alignment(dev, dtype):
     N, K, group = 70, 300, 64
