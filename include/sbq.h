@@ -36,6 +36,10 @@
  *   sbq_linear_w8a8_argmax       engine.py:30-31 (its greedy token) in one launch
  *   sbq_sample_rows           <- spikingbrain_cpu/engine.py:29-42 sample (temperature,
  *                                top-k, top-p and the draw) over the lm_head logits
+ *   sbq_tree_attention        <- spikingbrain_cpu/model.py:208-229 attention over the cached
+ *                                keys (and over a tree of drafted tokens)
+ * Additions without a counterpart: the 4-bit linears (sbq_linear_w4), the bounded
+ * cache (sbq_kv_append, sbq_kv_take).
  */
 #ifndef SBQ_H_
 #define SBQ_H_
@@ -486,14 +490,15 @@ int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
  * strides k_ss and k_sh; k_new, v_new (NULL: none): device [T, kv_heads, D]
  * of the cache's type, both with strides n_ss and n_sh.  slot_pos: device
  * int64 [slots].  q_pos: device int64 [T].  out: device [T, heads, D] of q's
- * type.  1 <= D <= 256, heads a multiple of kv_heads, T <= SBQ_ATTN_MAX_T,
+ * type, no two elements in one place, apart from every input.  1 <= D <= 256, heads a multiple of kv_heads, T <= SBQ_ATTN_MAX_T,
  * slots <= 2^30.
  * Scores, maxima and sums are fp32; with 2-byte queries the weights p are
  * rounded to their type (half to even) for the product with v, with F32
  * queries everything is fp32.  Unit strides and 16-byte aligned rows of a
  * D of 64, 128 or 256 are the fastest.
  * weight: NULL, or device fp32 [slots]: weight[s] += sum_{t,h} p[t,h,s], the
- * attention weight the cached slots received (for eviction by it).
+ * attention weight the cached slots received (for eviction by it); calls
+ * that add to one array must not overlap in time.
  * workspace: >= sbq_attn_workspace_bytes bytes, any content; one call at a
  * time.  The result does not depend on timing. */
 int64_t sbq_attn_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots,
@@ -522,7 +527,7 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
  * rounded to the cache's type and written to k, v (device [slots, kv_heads,
  * D], strides k_ss and k_sh), slot_pos is set, weight is 0, and *end = *start
  * + T.  start, end: device int64[1], the same one or not.  0 <= recent <=
- * slots, T <= slots.
+ * slots, T <= slots.  k_new and v_new must not overlap the cache.
  *
  * sbq_kv_take: the used slots among the last `capacity` of that order (newest:
  * >= *end - recent) of a cache of any size are copied, in slot order, to the

@@ -678,6 +678,13 @@ static int check_attn(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int
   return SBQ_OK;
 }
 
+// Do the elements of a written [n, heads, D] array lie apart?
+static bool apart(int64_t n, int64_t heads, int64_t D, int64_t st, int64_t sh) {
+  const __int128 D1 = D, n1 = n - 1, h1 = heads - 1;
+  return (heads == 1 || sh >= D) && (n == 1 || st >= D) &&
+         (n == 1 || heads == 1 || st >= h1 * sh + D1 || sh >= n1 * st + D1);
+}
+
 int64_t sbq_attn_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots, int weight) {
   if (T == 0 || check_attn(T, heads, kv_heads, D, slots)) return 0;
   return sbq::attn_workspace_bytes(T, heads, kv_heads, D, slots, weight != 0) + 256;  // + alignment slack
@@ -703,10 +710,12 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
     return SBQ_ERR_ALIGN;
   const int64_t need = sbq_attn_workspace_bytes(T, heads, kv_heads, D, slots, weight != nullptr);
   if (!workspace || (int64_t)workspace_bytes < need) return SBQ_ERR_WORKSPACE;
+  if (!apart(T, heads, D, o_st, o_sh)) return SBQ_ERR_ARG;
   sbq::AttnCall c{};
   c.q = q, c.k = k, c.v = v, c.kn = k_new, c.vn = v_new, c.slot_pos = slot_pos, c.q_pos = q_pos, c.tree = tree;
   c.out = out, c.weight = weight, c.ws = (void*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
-  c.T = T, c.heads = heads, c.Hk = kv_heads, c.D = D, c.slots = slots, c.Tn = k_new ? T : 0, c.window = window;
+  c.T = T, c.heads = heads, c.Hk = kv_heads, c.D = D, c.slots = slots, c.Tn = k_new ? T : 0;
+  c.window = window < (int64_t)1 << 62 ? window : (int64_t)1 << 62;  // (no overflow below a position)
   c.q_st = q_st, c.q_sh = q_sh, c.k_ss = k_ss, c.k_sh = k_sh, c.n_ss = n_ss, c.n_sh = n_sh, c.o_st = o_st, c.o_sh = o_sh;
   c.tree_ld = tree_ld, c.qt = q_dtype, c.ct = kv_dtype, c.scale = scale;
   return sbq::launch_tree_attention(c, (hipStream_t)stream);
@@ -730,7 +739,7 @@ int sbq_kv_append(int64_t* slot_pos, float* weight, int64_t slots, int64_t* end,
                   void* workspace, size_t workspace_bytes, void* stream) {
   if (!valid_dtype(kv_dtype) || !valid_dtype(new_dtype)) return SBQ_ERR_DTYPE;
   if (!kv_sizes_ok(slots, kv_heads, D) || recent < 0 || recent > slots || T < 0 || T > slots) return SBQ_ERR_ARG;
-  if (k_ss < 0 || k_sh < 0 || n_ss < 0 || n_sh < 0) return SBQ_ERR_ARG;
+  if (n_ss < 0 || n_sh < 0 || !apart(slots, kv_heads, D, k_ss, k_sh)) return SBQ_ERR_ARG;
   if (T == 0) return SBQ_OK;
   if (!slot_pos || !weight || !end || !start || !k || !v || !k_new || !v_new) return SBQ_ERR_ARG;
   const int64_t es = esize(kv_dtype), en = esize(new_dtype);
@@ -753,7 +762,7 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
   if (!valid_dtype(kv_dtype)) return SBQ_ERR_DTYPE;
   if (!kv_sizes_ok(slots, kv_heads, D) || capacity < 1 || capacity > (1 << 30) || recent < 0 || recent > capacity)
     return SBQ_ERR_ARG;
-  if (k_ss < 0 || k_sh < 0 || t_ss < 0 || t_sh < 0) return SBQ_ERR_ARG;
+  if (k_ss < 0 || k_sh < 0 || !apart(capacity, kv_heads, D, t_ss, t_sh)) return SBQ_ERR_ARG;
   if (!slot_pos || !weight || !end || !k || !v || !to_pos || !to_weight || !to_end || !to_k || !to_v) return SBQ_ERR_ARG;
   const int64_t es = esize(kv_dtype);
   if (!aligned(slot_pos, 8) || !aligned(weight, 4) || !aligned(end, 8) || !aligned(to_pos, 8) || !aligned(to_weight, 4) ||

@@ -158,6 +158,7 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
   if (threadIdx.x == 0) ncand = 0;
   __syncthreads();
   for (int seg = 0; seg < segs; ++seg) {
+    if (segs > 1 && (m == 0 || q.first)) break;  // (read where they are wanted, counted already)
     load_keys(q, seg, log, keys, m > 0 && !q.first ? hist : nullptr);
     if (segs > 1) __syncthreads();
   }

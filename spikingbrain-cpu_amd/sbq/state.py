@@ -46,6 +46,12 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _within(t: torch.Tensor, storage: torch.Tensor) -> bool:
+    """Does t begin inside the contiguous `storage`?"""
+    at = t.data_ptr() - storage.data_ptr()
+    return 0 <= at < storage.numel() * storage.element_size()
+
+
 def attention_workspace(T: int, heads: int, kv_heads: int, dim: int, slots: int, weight: bool,
                         device: torch.device) -> torch.Tensor:
     """Scratch of tree_attention for these sizes (any content; one call at a time)."""
@@ -121,6 +127,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
         raise ValueError("tree_attention: out must have q's shape, dtype and device, with unit stride in dim")
     if T == 0:
         return out
+    if out.data_ptr() == q.data_ptr():
+        raise ValueError("tree_attention: out must not be q itself")
     q = _rows_of(q)
     if workspace is None:
         workspace = attention_workspace(T, heads, kv_heads, dim, slots, weight is not None, device)
@@ -266,6 +274,8 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
         k, v = _rows_of(k), _rows_of(v)
         if k.stride() != v.stride():
             k, v = k.contiguous(), v.contiguous()
+        if T > 1 and (_within(k, kv) or _within(k, self.v) or _within(v, kv) or _within(v, self.v)):
+            k, v = k.clone(), v.clone()  # rows of the cache itself would be overwritten as they are read
         s = self.end if start is None else _as_pos(start, kv.device)
         L = _lib.load()
         ws = torch.empty((L.sbq_kv_workspace_bytes(self.capacity, T),), dtype=torch.uint8, device=kv.device)
@@ -294,6 +304,8 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
                 or weight.shape != (source.capacity,) or not weight.is_contiguous()):
             raise ValueError(f"DeviceBudgetKVBuffer.take: weight must be a contiguous float32 [{source.capacity}] tensor on "
                              f"{kv.device}")
+        if _within(weight, self.weight) or _within(self.weight, weight):
+            raise ValueError("DeviceBudgetKVBuffer.take: weight must not be this buffer's own")
         L = _lib.load()
         ws = torch.empty((L.sbq_kv_workspace_bytes(source.capacity, self.capacity),), dtype=torch.uint8, device=kv.device)
         ks, ts = source.k.stride(), kv.stride()

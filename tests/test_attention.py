@@ -53,6 +53,18 @@ def test_c_abi_refuses_bad_arguments():
     assert L.sbq_attn_workspace_bytes(1, 5, 2, 64, 8, 0) == 0 and L.sbq_attn_workspace_bytes(0, 4, 2, 64, 8, 0) == 0
 
 
+def test_c_abi_refuses_outputs_that_meet():
+    L = _lib.load()
+    p = 1 << 16
+
+    def attn(T, H, D, ost, osh):
+        return L.sbq_tree_attention(p, 0, T, H, D, H * D, D, p, p, 0, 8, 1, D, D, p, p, None, None, 0, 0, None, 0, 0, 0.1, p,
+                                    ost, osh, None, p, 1 << 30, None)
+
+    for bad in ((2, 1, 64, 0, 64), (1, 2, 64, 128, 63), (2, 2, 64, 64, 64), (2, 2, 64, 127, 64), (3, 2, 8, 8, 23)):
+        assert attn(*bad) == -1, bad
+
+
 def test_python_refuses_cpu_tensors():
     buf = DeviceKVBuffer(2, 8, 16, device="cpu")
     with pytest.raises(ValueError, match="GPU"):
@@ -431,3 +443,27 @@ def test_attend_streams_and_graph(dev):
         assert torch.equal(step(), got) and torch.equal(weight, w)
         torch.cuda.synchronize()
         assert float(w.sum()) > 0
+
+
+@pytest.mark.gpu
+def test_attend_out_layouts_and_alias(dev):
+    """out as a part of a larger array, tokens outside or inside; never q itself, nor with elements that meet."""
+    T, heads, kv, D, slots = 3, 4, 2, 64, 200
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(n, h, D, generator=g).to(dev) for n, h in ((T, heads), (slots, kv), (slots, kv)))
+    pos, q_pos = torch.arange(slots, device=dev), torch.arange(T, device=dev) + 150
+    want = tree_attention(q, k, v, pos, q_pos)
+    wide = torch.full((T, heads + 2, D + 8), 7.0, device=dev)
+    tree_attention(q, k, v, pos, q_pos, out=wide[:, 1:1 + heads, :D])
+    assert torch.equal(wide[:, 1:1 + heads, :D], want)
+    wide[:, 1:1 + heads, :D] = 7.0
+    assert bool((wide == 7).all())
+    inside = torch.empty(heads, T, D, device=dev).transpose(0, 1)
+    tree_attention(q, k, v, pos, q_pos, out=inside)
+    assert torch.equal(inside, want)
+    for bad in (q, torch.zeros(1, heads, D, device=dev).expand(T, heads, D)):
+        with pytest.raises(ValueError):
+            tree_attention(q, k, v, pos, q_pos, out=bad)
+    far = tree_attention(q, k, v, pos, q_pos - 1000, q[:, :kv].contiguous(), q[:, :kv].contiguous(), window=2 ** 63 - 1)
+    near = tree_attention(q, k, v, torch.full_like(pos, -1), q_pos, q[:, :kv].contiguous(), q[:, :kv].contiguous())
+    assert torch.equal(far, near)  # only the drafts are seen, however wide the window

@@ -331,3 +331,52 @@ def test_drafted_steps_through_a_bounded_layer(dev, fmt):
         slots[torch.from_numpy(at).to(dev)] = k[path]
         assert b.slot_pos.tolist() == pos.tolist() and torch.equal(b.k, slots) and int(b.end) == end + len(path)
     assert int((b.slot_pos >= int(b.end) - recent).sum()) == recent
+
+
+def test_c_abi_refuses_rows_that_meet():
+    L = _lib.load()
+    p = 1 << 16
+    for kss, ksh in ((0, 4), (8, 3), (7, 4), (4, 4)):
+        assert L.sbq_kv_append(p, p, 8, p, p, 2, p, p, 0, 2, 4, kss, ksh, p, p, 0, 1, 8, 4, p, 1 << 20, None) == -1
+        assert L.sbq_kv_take(p, p, 8, p, p, p, 0, 2, 4, 8, 4, 4, 2, p, p, p, p, p, kss, ksh, p, 1 << 20, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_append_rows_of_the_cache_itself(dev, dtype):
+    """Tokens whose keys and values are the cache's own rows, which the append takes over."""
+    n = 40
+    g = torch.Generator().manual_seed(5)
+    buf = DeviceBudgetKVBuffer(2, 64, n, 0, dev, dtype)
+    k, v = (torch.randn(n, 2, 64, generator=g).to(dev, dtype) for _ in range(2))
+    buf.append(k, v)
+    buf.weight.copy_(torch.rand(n, generator=g).to(dev))
+    slots = torch.sort(torch.argsort(buf.weight)[:6]).values
+    at = int(slots[0])
+    rows = min(at, n - 6)
+    announce(f"append own rows {rows}..{rows + 5} {dtype}")
+    buf.append(buf.k[rows:rows + 6], buf.v[rows:rows + 6])
+    assert torch.equal(buf.k[slots], k[rows:rows + 6]) and torch.equal(buf.v[slots], v[rows:rows + 6])
+
+
+@pytest.mark.gpu
+def test_take_refuses_its_own_weight(dev):
+    src, dst = DeviceBudgetKVBuffer(2, 64, 32, 0, dev), DeviceBudgetKVBuffer(2, 64, 32, 0, dev)
+    with pytest.raises(ValueError, match="own"):
+        dst.take(src, dst.weight)
+
+
+@pytest.mark.gpu
+def test_take_from_a_very_long_cache(dev):
+    """More slots than stay in LDS: every pass reads the keys again."""
+    n, cap, recent = 70001, 5000, 100
+    g = torch.Generator().manual_seed(6)
+    src, dst = DeviceBudgetKVBuffer(1, 8, n, 0, dev), DeviceBudgetKVBuffer(1, 8, cap, recent, dev)
+    src.append(torch.randn(60000, 1, 8, generator=g).to(dev), torch.randn(60000, 1, 8, generator=g).to(dev))
+    weight = (torch.rand(n, generator=g) * 50).round() / 50   # (many equal ones)
+    announce("take 5000 of 70001 slots")
+    dst.take(src, weight.to(dev))
+    order = torch.where(src.slot_pos.cpu() < 0, -1.0, torch.where(src.slot_pos.cpu() >= 60000 - recent, 1e9, weight.double()))
+    kept = torch.sort(torch.argsort(order, stable=True)[n - cap:]).values
+    assert torch.equal(dst.slot_pos.cpu(), src.slot_pos.cpu()[kept]) and torch.equal(dst.weight.cpu(), weight[kept])
+    assert torch.equal(dst.k.cpu(), src.k.cpu()[kept]) and torch.equal(dst.v.cpu(), src.v.cpu()[kept])
