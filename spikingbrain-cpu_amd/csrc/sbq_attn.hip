@@ -148,6 +148,13 @@ constexpr int kAttnGroups = 512;    // workgroups aimed at
 constexpr int kTileGroups = 256;
 constexpr int64_t kTileRows = 256, kTileScores = 1 << 22;
 
+// Scores from which a wave takes two row tiles: they share its loads of keys and
+// values, but fewer waves fit a CU, which costs more while a wave has only a few
+// blocks.  8 key heads of 128 columns, two tiles against one: 64 rows over 4096
+// slots 19.5 us / 15.9 (bf16), 34 / 29 (fp32), over 8192 21.6 / 21.3 and 45 / 44,
+// over 16384 26.7 / 31.1 and 65 / 73; 32 rows over 16384 25.5 / 22.3 and 49 / 45.
+constexpr int64_t kPairScores = 1 << 22;
+
 int attn_dp(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct AttnPlan {
@@ -164,7 +171,8 @@ AttnPlan attn_plan(int64_t R, int64_t Hk, int64_t slots, int64_t Tn, int DP, boo
     groups = kTileGroups;
     each = 1, SB = kTileSlots;
   } else {
-    p.RT = vec && R > 16 && (m16 || DP < 256) ? 2 : 1;  // (two tiles of 256 fp32 columns do not fit the registers)
+    // (two tiles of 256 fp32 columns do not fit the registers)
+    p.RT = vec && R > 16 && Hk * R * slots > kPairScores && (m16 || DP < 256) ? 2 : 1;
     p.rtiles = (int)((R + 16 * p.RT - 1) / (16 * p.RT));
   }
   p.rows = p.RT == 0 ? (int64_t)p.rtiles * kTileWaves * 32 : R;

@@ -467,3 +467,45 @@ def test_attend_out_layouts_and_alias(dev):
     far = tree_attention(q, k, v, pos, q_pos - 1000, q[:, :kv].contiguous(), q[:, :kv].contiguous(), window=2 ** 63 - 1)
     near = tree_attention(q, k, v, torch.full_like(pos, -1), q_pos, q[:, :kv].contiguous(), q[:, :kv].contiguous())
     assert torch.equal(far, near)  # only the drafts are seen, however wide the window
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attend_pairs_of_row_tiles(dev, D, qt, ct):
+    """Sizes from which a wave takes two row tiles, the last one not full."""
+    for T, heads, kv, slots, filled, window, drafts, weight in (
+            (15, 8, 2, 36001, 35000, None, True, True), (5, 14, 2, 61000, 100000, 60990, False, False)):
+        _case(dev, T, heads, kv, D, slots, filled, window, qt, ct, drafts, weight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_pairs_hidden_values(dev, D, qt, ct):
+    """As test_attend_tiles_hidden_values, with two row tiles a wave."""
+    T, heads, slots = 24, 2, 88000
+    g = torch.Generator().manual_seed(D + 1)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = r(T, heads, D).to(qt), r(slots, 1, D).to(ct), r(slots, 1, D).to(ct)
+    kn, vn = r(T, 1, D).to(ct), r(T, 1, D).to(ct)
+    pos = torch.arange(slots)
+    pos[::5] = -1                      # empty slots hold anything
+    k[::5], v[::5] = float("nan"), float("-inf")
+    q_pos = torch.full((T,), slots + 1)
+    q_pos[3], q_pos[7] = -2, 4000      # row 3 sees no slot, row 7 not all
+    tree = torch.eye(T, dtype=torch.bool)
+    tree[3, 3] = False
+    kn[9], vn[9] = float("nan"), float("inf")   # draft 9: seen by itself and row 11 alone
+    tree[11, 9] = True
+    v[4004] = float("inf")             # hidden from rows 3 and 7 alone
+    announce(f"pairs, hidden values D={D} {qt} over {ct}")
+    to = lambda t: t.to(dev)           # noqa: E731
+    o = tree_attention(to(q), to(k), to(v), to(pos), to(q_pos), to(kn), to(vn), to(tree)).cpu()
+    assert bool((o[3] == 0).all())
+    assert bool(torch.isnan(o[9]).all()) and bool(torch.isnan(o[11]).all())
+    rest = [t for t in range(T) if t not in (3, 7, 9, 11)]
+    assert bool((o[rest] == float("inf")).all())
+    clean = lambda t: torch.nan_to_num(t.float(), 0.0, 0.0, 0.0).to(t.dtype)  # noqa: E731
+    see = _see(pos, q_pos, tree, None)
+    _compare(o[[7]], None, None, q[[7]], clean(torch.cat([k, kn])), clean(torch.cat([v, vn])), see[[7]], D ** -0.5, slots)
