@@ -380,3 +380,49 @@ def test_take_from_a_very_long_cache(dev):
     kept = torch.sort(torch.argsort(order, stable=True)[n - cap:]).values
     assert torch.equal(dst.slot_pos.cpu(), src.slot_pos.cpu()[kept]) and torch.equal(dst.weight.cpu(), weight[kept])
     assert torch.equal(dst.k.cpu(), src.k.cpu()[kept]) and torch.equal(dst.v.cpu(), src.v.cpu()[kept])
+
+
+@pytest.mark.gpu
+def test_long_steps_in_a_graph(dev):
+    """The kernels for many rows and long caches captured together and replayed
+    with new inputs: a 4-bit linear, the attention with its weights, a take, an append."""
+    g = torch.Generator().manual_seed(8)
+    slots, cap, T, heads, D = 49152, 9000, 40, 8, 64
+    long = DeviceKVBuffer(1, D, slots, device=dev, dtype=torch.bfloat16)
+    rows = torch.randn(2, 45000, 1, D, generator=g).to(dev)
+    long.append(rows[0], rows[1])
+    lin = quant.Int4Linear(torch.randn(300, 1000, generator=g).to(dev) * 0.1, group=64)
+    x = torch.zeros(T, 1000, device=dev)
+    q, kn, vn = (torch.zeros(T, h, D, dtype=torch.bfloat16, device=dev) for h in (heads, 1, 1))
+    q_pos = torch.full((T,), 45000, device=dev)
+    weight = torch.zeros(slots, device=dev)
+    small = [DeviceBudgetKVBuffer(1, D, cap, 100, dev, torch.bfloat16) for _ in range(2)]
+
+    def step(buf):
+        weight.zero_()
+        y = lin(x)
+        o = long.attend(q, q_pos, kn, vn, weight=weight)
+        buf.take(long, weight)
+        buf.append(kn[:12], vn[:12])
+        return y, o
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(small[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, o = step(small[0])
+    for i in range(4):
+        announce(f"long steps, replay {i}")
+        for t in (x, q, kn, vn):
+            t.copy_(torch.randn(t.shape, generator=g).to(dev))
+        graph.replay()
+        got = y.clone(), o.clone(), weight.clone()
+        want = step(small[1])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], weight)
+        for name in ("slot_pos", "weight", "end", "k", "v"):
+            assert torch.equal(getattr(small[0], name), getattr(small[1], name)), (i, name)
+        assert int(small[0].end) == 45012 and int((small[0].slot_pos >= 45000).sum()) == 12
