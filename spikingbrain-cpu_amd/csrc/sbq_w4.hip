@@ -59,15 +59,17 @@ __device__ __forceinline__ f16x8 w4_to_f16(uint32_t w) {
   return o;
 }
 
-// ... -> bf16 q: 0x4300 | u is 128 + u; the difference to 136 is taken in fp32
-// (there is no packed bf16 subtract) and its upper half is exact.
+// ... -> bf16 q / 16, exactly: v_cvt_off_f32_i4 gives the fp32 value of a
+// two's complement nibble over 16 (u ^ 8), the upper halves of two pair up.
+// The 16 comes back at the end (W4Math::kBack).
 __device__ __forceinline__ bf16x8 w4_to_bf16(uint32_t w) {
   u32x4 o;
+  w ^= 0x88888888u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t p = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    const uint32_t lo = __float_as_uint(__uint_as_float(p << 16) - 136.0f);
-    const uint32_t hi = __float_as_uint(__uint_as_float(p & 0xffff0000u) - 136.0f);
+    const uint32_t p = w >> (4 * i);
+    const uint32_t lo = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)p));
+    const uint32_t hi = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)(p >> 16)));
     o[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
   }
   return __builtin_bit_cast(bf16x8, o);
@@ -76,6 +78,7 @@ __device__ __forceinline__ bf16x8 w4_to_bf16(uint32_t w) {
 template <int XT>
 struct W4Math {
   typedef f16x8 V;
+  static constexpr float kBack = 1.0f;
   static __device__ __forceinline__ V weight(uint32_t w) { return w4_to_f16(w); }
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -84,6 +87,7 @@ struct W4Math {
 template <>
 struct W4Math<XT_BF16> {
   typedef bf16x8 V;
+  static constexpr float kBack = 16.0f;
   static __device__ __forceinline__ V weight(uint32_t w) { return w4_to_bf16(w); }
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -217,7 +221,7 @@ struct W4Args {
 
 // The waves' partial sums, added in wave order, and the rows out.  lds is free
 // once every wave is here.
-template <int G, int MT>
+template <int XT, int G, int MT>
 __device__ __forceinline__ void join_w4(const W4Args& a, const f32x4 (&acc)[G][MT], uint8_t* lds, int nt0, int m0) {
   const int lane = threadIdx.x & 63, ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KS = blockDim.x >> 6;
   const int c = lane & 15, g = lane >> 4, M = min(a.M - m0, MT * 16);
@@ -246,6 +250,7 @@ __device__ __forceinline__ void join_w4(const W4Args& a, const f32x4 (&acc)[G][M
     }
     const int m = t * 16 + c, n = (nt0 + i) * 16 + 4 * g;
     if (m >= M || n >= a.N) continue;
+    v *= W4Math<XT>::kBack;
     if (a.bias) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += n + j < a.N ? a.bias[n + j] : 0.0f;
@@ -368,7 +373,7 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
     }
   }
 
-  join_w4<G, MT>(a, acc, lds, nt0, m0);
+  join_w4<XT, G, MT>(a, acc, lds, nt0, m0);
 }
 
 // More than 8 rows, aligned.  A fragment read straight from memory takes one
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
     if (kt + KS < a.Kc) tile(kt + KS, sc[1], sc[0]);
   }
   wait_vmcnt<0>();  // (no copy outlives the area)
-  join_w4<G, MT>(a, acc, lds, nt0, m0);
+  join_w4<XT, G, MT>(a, acc, lds, nt0, m0);
 }
 
 // ---------------------------------------------------------------------------
