@@ -29,7 +29,7 @@
 // row tile, so that a cache that is filled only at its front still keeps
 // every workgroup busy; a block that no row sees is left out after a look at
 // its positions.  A decode step of 32 heads over 2048 slots of 8 x 128 fp32
-// takes 10 us and 5.5 for the joining (the latency of a few loads after each
+// takes 9 us and 4.4 for the joining (the latency of a few loads after each
 // other; 3.3 us for the bytes), over 65536 bf16 48 us, 5.6 TB/s.
 #pragma once
 

@@ -14,10 +14,10 @@ int launch_attn_f32(const AttnArgs& a, int DP, int mode, int RT, float* weight, 
 namespace {
 
 // One row's splits joined: the maximum over their maxima, then the partial
-// sums scaled to it.  A thread's loads are independent, four at a time.
+// sums scaled to it.  A thread's loads are independent, eight at a time.
 template <int DP>
 __device__ __forceinline__ void join_row(const AttnArgs& a, int64_t at) {
-  constexpr int ND = DP / 4, NG = 256 / ND;
+  constexpr int ND = DP / 4, NG = 256 / ND, U = 8;
   __shared__ __align__(16) f32x4 lds[NG][ND];
   __shared__ float lds_l[NG];
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
@@ -28,17 +28,17 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int64_t at) {
   const float from = top == -__builtin_inff() ? 0.0f : top;
   f32x4 sum = (f32x4)(0.0f);
   float l = 0.0f;
-  for (int s0 = grp; s0 < a.splits; s0 += 4 * NG) {
-    f32x4 x[4];
-    float2 y[4];
+  for (int s0 = grp; s0 < a.splits; s0 += U * NG) {
+    f32x4 x[U];
+    float2 y[U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < U; ++k) {
       const int s = min(s0 + k * NG, a.splits - 1);
       x[k] = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
       y[k] = ml[s];
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < U; ++k) {
       const float f = __builtin_amdgcn_exp2f(y[k].x - from);
       if (s0 + k * NG < a.splits && y[k].y != 0.0f) {  // (a split that saw nothing adds nothing)
         sum += x[k] * f;
@@ -101,12 +101,26 @@ __global__ __launch_bounds__(256) void attn_join_weight_kernel(AttnArgs a, float
     const float2* const part = a.part_ml + (int64_t)row * a.splits;
     const int first = threadIdx.x & 7;
     float top = -__builtin_inff(), l = 0.0f;
-    for (int i = first; i < a.splits; i += 8) top = __builtin_fmaxf(top, part[i].x);
+#pragma unroll 1
+    for (int s0 = 0; s0 < a.splits; s0 += 8 * U) {  // (the loads of a step together)
+      float2 y[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) y[k] = part[min(s0 + first + 8 * k, a.splits - 1)];
+      float up = top;
+#pragma unroll
+      for (int k = 0; k < U; ++k) up = __builtin_fmaxf(up, y[k].x);
+      const float from = up == -__builtin_inff() ? 0.0f : up;
+      l *= __builtin_amdgcn_exp2f(top - from);
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (s0 + first + 8 * k < a.splits && y[k].y != 0.0f) l += y[k].y * __builtin_amdgcn_exp2f(y[k].x - from);
+      top = up;
+    }
+    const float own = top;
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 64));
     const float from = top == -__builtin_inff() ? 0.0f : top;
-    for (int i = first; i < a.splits; i += 8)
-      if (part[i].y != 0.0f) l += part[i].y * __builtin_amdgcn_exp2f(part[i].x - from);
+    l *= __builtin_amdgcn_exp2f(own - from);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) l += __shfl_xor(l, o, 64);
     if (first == 0) {
