@@ -777,7 +777,7 @@ def linear_w4(x2: torch.Tensor, packed: torch.Tensor, gscale: torch.Tensor, bias
                              or bias.numel() < N):
         raise ValueError(f"linear_w4: bias must be a contiguous float32 tensor of N={N} elements on {device}")
     if out is None:
-        y, ldy = torch.empty((M, N), dtype=out_dtype, device=device), N
+        y, ldy = torch.empty(M, N, dtype=out_dtype, device=device), N
     elif out.get_device() != gpu or out.shape != (M, N) or out.stride(-1) != 1 or (M > 1 and out.stride(0) < N):
         raise ValueError(f"linear_w4: out must be a [M={M}, N={N}] tensor with unit column stride on {device}")
     else:

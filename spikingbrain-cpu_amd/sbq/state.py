@@ -56,7 +56,7 @@ def attention_workspace(T: int, heads: int, kv_heads: int, dim: int, slots: int,
                         device: torch.device) -> torch.Tensor:
     """Scratch of tree_attention for these sizes (any content; one call at a time)."""
     n = _lib.load().sbq_attn_workspace_bytes(T, heads, kv_heads, dim, slots, int(weight))
-    return torch.empty((n,), dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: torch.Tensor, q_pos: torch.Tensor,
@@ -122,7 +122,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
                                or not weight.is_contiguous()):
         raise ValueError(f"tree_attention: weight must be a contiguous float32 [{slots}] tensor on {q.device}")
     if out is None:
-        out = torch.empty((T, heads, dim), dtype=qt, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(T, heads, dim, dtype=qt, device=device)
     elif out.shape != q.shape or out.dtype != qt or out.get_device() != gpu or (dim > 1 and out.stride(2) != 1):
         raise ValueError("tree_attention: out must have q's shape, dtype and device, with unit stride in dim")
     if T == 0:
@@ -278,7 +278,7 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
             k, v = k.clone(), v.clone()  # rows of the cache itself would be overwritten as they are read
         s = self.end if start is None else _as_pos(start, kv.device)
         L = _lib.load()
-        ws = torch.empty((L.sbq_kv_workspace_bytes(self.capacity, T),), dtype=torch.uint8, device=kv.device)
+        ws = torch.empty(L.sbq_kv_workspace_bytes(self.capacity, T), dtype=torch.uint8, device=kv.device)
         ks, ns = kv.stride(), k.stride()
         with _on_device(kv.device):
             _lib.check(L.sbq_kv_append(
@@ -307,7 +307,7 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
         if _within(weight, self.weight) or _within(self.weight, weight):
             raise ValueError("DeviceBudgetKVBuffer.take: weight must not be this buffer's own")
         L = _lib.load()
-        ws = torch.empty((L.sbq_kv_workspace_bytes(source.capacity, self.capacity),), dtype=torch.uint8, device=kv.device)
+        ws = torch.empty(L.sbq_kv_workspace_bytes(source.capacity, self.capacity), dtype=torch.uint8, device=kv.device)
         ks, ts = source.k.stride(), kv.stride()
         with _on_device(kv.device):
             _lib.check(L.sbq_kv_take(
