@@ -144,6 +144,18 @@ def test_append_takes_the_least_attended(dev, n, T, recent, used, kind):
     assert int(b.end) == 3 * n + T
 
 
+FEW_CANDIDATES = [(8195, 12, 100, 8195), (8192, 128, 0, 8192), (8193, 127, 8000, 8193), (8192, 129, 50, 8192),
+                  (32768, 2, 1024, 32768), (12289, 64, 12289, 12289), (20000, 51, 10, 19990)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal", "odd"])
+@pytest.mark.parametrize("n,T,recent,used", FEW_CANDIDATES)
+def test_append_few_candidates(dev, n, T, recent, used, kind):
+    """Workgroups' first slots, on both sides of the number that is ranked; a last workgroup with fewer slots than tokens."""
+    test_append_takes_the_least_attended(dev, n, T, recent, used, kind)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("ct", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 @pytest.mark.parametrize("nt", [F32, F16, BF16, torch.float64], ids=["f32", "f16", "bf16", "f64"])
