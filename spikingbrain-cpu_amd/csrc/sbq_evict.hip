@@ -19,14 +19,14 @@
 // among theirs and 3 for the rows; 4096 of 32768 slots taken: 4, 23 and 7 us.
 // Integer counts only, so the result does not depend on timing.
 #include "sbq_common.h"
+#include "sbq_index.h"
 #include "sbq_launch.h"
 
 namespace sbq {
 
 namespace {
 
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 2048;
-constexpr int kChunk = 4 * kSelThreads;  // slots that one workgroup of a launch before the selection looks at
+constexpr int kSelWaves = kSelThreads / 64, kBins = 2048;
 
 // The order in which slots are given up.
 __device__ __forceinline__ uint32_t evict_key(int64_t pos, float weight, int64_t keep_from) {
@@ -72,12 +72,6 @@ struct Select {
 // A thread's `per` (4, 8, 16 or 32) keys of a segment of per * 1024 slots lie
 // side by side in LDS, their 16-byte pieces permuted by the thread (else the
 // threads' reads would all meet in the same banks).
-constexpr int kSegKeys = 32, kCand = 2048;
-__host__ __device__ constexpr int keys_log(int64_t n) {
-  int log = 2;
-  while (1 << log < kSegKeys && ((int64_t)kSelThreads << log) < n) ++log;
-  return log;
-}
 // Place of key i of thread t, `per` = 1 << log.
 __device__ __forceinline__ int key_at(int t, int i, int log) {
   return (t << log) + ((((i >> 2) ^ t) & ((1 << log) / 4 - 1)) << 2 | (i & 3));
@@ -226,6 +220,7 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
 #pragma unroll
           for (int j = 0; j < 4; ++j) mine |= (uint32_t)(k4[j] >> 21 == found[0]) << (i + j);
         }
+        mine &= slot_mask(q.n, (int64_t)threadIdx.x * per);  // (those past the end are not all in found[2])
         uint32_t at = mine ? atomicAdd(&ncand, (uint32_t)__popc(mine)) : 0u;
         for (; mine; mine &= mine - 1) cand[at++] = keys[key_at(threadIdx.x, __ffs(mine) - 1, log)];
       }
@@ -258,11 +253,9 @@ __device__ __forceinline__ int select_slots(const Select& q, int m, int side, in
         same |= (uint32_t)(k4[j] == kth) << (i + j);
       }
     }
-    if (s0 + per > q.n) {
-      const uint32_t in = s0 >= q.n ? 0u : (1u << (q.n - s0)) - 1;
-      strict &= in;
-      same &= in;
-    }
+    const uint32_t in = slot_mask(q.n, s0);
+    strict &= in;
+    same &= in;
     uint32_t all_out, all_eq;
     const uint32_t out0 = out + block_scan(__popc(strict), scan, &all_out);
     const uint32_t eq0 = eq + block_scan(__popc(same), scan, &all_eq);

@@ -62,6 +62,25 @@ SBQ_HD int64_t part_base(uint32_t word, int64_t M) {
   return M * pstart - start;
 }
 
+// The bounded cache's selection (sbq_evict.hip) by one workgroup: a thread holds
+// 1 << keys_log(n) slots side by side, of segments of as many per thread; slots
+// past the last one are keys too, larger than any other.  Keys that share the
+// wanted first digit are set apart in kCand words where no more are counted, in
+// numbers that a launch before the selection may have taken kChunk slots at a
+// time, so that the two see different numbers of slots past the last one: only
+// those of slot_mask are set apart.
+constexpr int kSelThreads = 1024, kSegKeys = 32, kCand = 2048;
+constexpr int kChunk = 4 * kSelThreads;  // slots that one workgroup of a launch before the selection looks at
+SBQ_HD constexpr int keys_log(int64_t n) {
+  int log = 2;
+  while (1 << log < kSegKeys && ((int64_t)kSelThreads << log) < n) ++log;
+  return log;
+}
+// Which of a thread's slots, s0 and up to 31 after it, there are (n in all); one bit each.
+SBQ_HD uint32_t slot_mask(int64_t n, int64_t s0) {
+  return n - s0 >= 32 ? ~0u : n <= s0 ? 0u : (1u << (n - s0)) - 1u;
+}
+
 // Column index of a key from argmax_key.
 SBQ_HD int argmax_key_index(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
 

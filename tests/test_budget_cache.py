@@ -438,3 +438,22 @@ def test_long_steps_in_a_graph(dev):
         for name in ("slot_pos", "weight", "end", "k", "v"):
             assert torch.equal(getattr(small[0], name), getattr(small[1], name)), (i, name)
         assert int(small[0].end) == 45012 and int((small[0].slot_pos >= 45000).sum()) == 12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,capacity,newest", [(8192, 256, 600), (12288, 256, 600), (12289, 300, 2040), (20480, 256, 600),
+                                               (20480, 2000, 2048), (24576, 256, 2049), (32768, 100, 600),
+                                               (40000, 256, 600), (28000, 4000, 28000)])
+def test_take_with_more_newest_slots_than_capacity(dev, n, capacity, newest):
+    """`end` moved back (an append at an earlier start): more slots than are
+    kept hold one of the newest positions, and the last of them stay."""
+    recent = min(capacity, 100)
+    src, pos, w, g = _filled(dev, n, 1, 4, F32, 0, "spread", n, n)
+    end = int(np.sort(pos)[n - newest]) + recent
+    src.end.fill_(end)
+    b = DeviceBudgetKVBuffer(1, 4, capacity, recent, dev, F32)
+    announce(f"take n={n} capacity={capacity}, {newest} slots of the newest positions")
+    b.take(src)
+    at = np.sort(_order(pos, w, end, recent)[n - capacity:])
+    assert torch.equal(b.slot_pos.cpu(), torch.from_numpy(pos[at])) and _same(b.weight, torch.from_numpy(w[at]))
+    assert _same(b.k, src.k.cpu()[at]) and _same(b.v, src.v.cpu()[at]) and int(b.end) == end
