@@ -146,10 +146,12 @@ __device__ __forceinline__ void split_f16(const X8<XT_F32>::V& v, float s, f16x8
 
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Exponent for a tile's maximum (>= 0, finite): it lands in [2^14, 2^15).
+// Exponent for a tile's maximum (>= 0, finite): it lands in [2^14, 2^15), or
+// below where the maximum is under 2^-106.  (-113 at least, for the largest
+// values; exp2i holds it and its inverse.)
 __device__ __forceinline__ int tile_exp(float mx) {
   const int e = 141 - (int)(__float_as_uint(mx) >> 23);
-  return mx > 0.0f ? min(max(e, -112), 120) : 0;
+  return mx > 0.0f ? min(e, 120) : 0;
 }
 
 __device__ __forceinline__ void wave_lds_fence() {

@@ -284,3 +284,27 @@ def test_linear_w4_streams_and_graph(dev):
         graph.replay()
         assert torch.equal(y, lin(x))
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 2, 4, 8, 12, 24, 40, 70])
+def test_linear_w4_largest_values(dev, M, group):
+    """fp32 rows that hold the largest finite values, alone and beside ordinary
+    ones (each other group of 128 columns), aligned and not."""
+    N, K = 48, 640
+    q, s = _weight(N, K, group, M)
+    s = (s.float() * 2.0 ** -20).to(BF16)  # (640 columns of 8 * 2.8 * 2^-20 times the largest value stay finite)
+    packed, gscale = quant.repack_w4(q.to(dev), s.to(dev), group)
+    top = torch.finfo(F32).max
+    for big in (top, -top, 65520 * 2.0 ** 112, 65519 * 2.0 ** 112):
+        x = _x(M, K, F32, M)
+        x[:, ::97] = big
+        x[:, 128:256] = x[:, 128:256].clamp(-1e3, 1e3)
+        if M > 1:
+            x[M - 1] = big
+        wide = torch.zeros(M, K + 1)
+        wide[:, 1:] = x
+        for xd in (x.to(dev), wide.to(dev)[:, 1:]):
+            announce(f"linear_w4 largest values M={M} group={group} {big:.7g} stride {xd.stride(0)}")
+            _check(quant.linear_w4(xd, packed, gscale, None, N, group).cpu(), x, q, s, None, group, F32)
