@@ -517,7 +517,7 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
  * gives up the slots that received the least attention weight (weight [slots],
  * the running sums sbq_tree_attention adds to).  Slots are given up in this
  * order, equal ones by their index: free slots (slot_pos < 0); then by
- * weight, the least first (NaN last); last the slots of the `recent` newest
+ * weight, the least first (-0 equals 0, NaN last); last the slots of the `recent` newest
  * positions.  No counterpart in the reference.
  *
  * sbq_kv_append: T new tokens, at positions *start .. *start + T - 1, take the

@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t evict_key(int64_t pos, float weight, int64_t
   if (pos < 0) return 0u;                // free
   if (pos >= keep_from) return ~0u;      // one of the newest
   if (weight != weight) return 0xff900000u;
-  const uint32_t b = __float_as_uint(weight);
+  const uint32_t b = __float_as_uint(weight + 0.0f);  // (-0 is 0)
   return b >> 31 ? ~b : b | 0x80000000u;  // 0x007fffff (-inf) .. 0xff800000 (+inf)
 }
 

@@ -457,3 +457,31 @@ def test_take_with_more_newest_slots_than_capacity(dev, n, capacity, newest):
     at = np.sort(_order(pos, w, end, recent)[n - capacity:])
     assert torch.equal(b.slot_pos.cpu(), torch.from_numpy(pos[at])) and _same(b.weight, torch.from_numpy(w[at]))
     assert _same(b.k, src.k.cpu()[at]) and _same(b.v, src.v.cpu()[at]) and int(b.end) == end
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,T", [(5, 1), (300, 1), (300, 100), (9000, 40), (9000, 700), (40000, 12)])
+def test_zeros_of_either_sign_are_equal(dev, n, T):
+    """Slots of weight 0 and -0 are given up by index; a kept one keeps its bits."""
+    r = np.random.default_rng(n + T)
+    w = np.where(r.random(n) < 0.5, -0.0, 0.0).astype(np.float32)
+    w[0] = 0.0
+    w[r.permutation(n)[:T // 2]] = -1e-45
+    at = np.sort(_order(np.arange(n), np.abs(w) * -1 + 0.0, n + T, 0)[:T])
+    g = torch.Generator().manual_seed(n)
+    for op in ("append", "take"):
+        b = DeviceBudgetKVBuffer(1, 4, n, 0, dev)
+        k = torch.randn(n, 1, 4, generator=g).to(dev)
+        b.append(k, k)
+        b.weight.copy_(torch.from_numpy(w))
+        announce(f"{op}, zeros of either sign, n={n} T={T}")
+        if op == "append":
+            b.append(torch.ones(T, 1, 4, device=dev), torch.ones(T, 1, 4, device=dev))
+            pos, want = np.arange(n), w.copy()
+            pos[at], want[at] = n + np.arange(T), 0.0
+        else:
+            small = DeviceBudgetKVBuffer(1, 4, n - T, 0, dev)
+            small.take(b)
+            b, pos = small, np.delete(np.arange(n), at)
+            want = w[pos]
+        assert torch.equal(b.slot_pos.cpu(), torch.from_numpy(pos)) and _same(b.weight, torch.from_numpy(want))
