@@ -509,3 +509,35 @@ def test_attend_pairs_hidden_values(dev, D, qt, ct):
     clean = lambda t: torch.nan_to_num(t.float(), 0.0, 0.0, 0.0).to(t.dtype)  # noqa: E731
     see = _see(pos, q_pos, tree, None)
     _compare(o[[7]], None, None, q[[7]], clean(torch.cat([k, kn])), clean(torch.cat([v, vn])), see[[7]], D ** -0.5, slots)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+@pytest.mark.parametrize("T,heads,kv,D,slots", [(1, 8, 1, 64, 40000), (1, 256, 256, 8, 16000), (64, 64, 64, 64, 4096),
+                                                (512, 32, 32, 64, 8192), (512, 16, 16, 128, 8200), (2, 128, 64, 256, 3000)])
+def test_attend_many_slots_beside_a_large_one(dev, T, heads, kv, D, slots, qt, ct):
+    """One slot of value 0 takes almost all of the weight, the others some
+    2^-25 of it each; so many heads or rows that a wave takes many of them.  All values and weights are >= 0, so that each weight's
+    relative error, e and half a step of the type, is the output's at most;
+    2^-39 of the largest weight is half of fp16's smallest step below 2^14."""
+    g = torch.Generator().manual_seed(D + T)
+    q, k, v = torch.zeros(T, heads, D), torch.zeros(slots, kv, D), torch.rand(slots, kv, D, generator=g) + 0.5
+    q[..., :2] = 1.0
+    k[..., 0] = -17.5
+    k[..., 1] = torch.randint(-2, 3, (slots, kv), generator=g) / 4
+    k[0], v[0] = 0.0, 0.0
+    q, k, v = q.to(qt), k.to(ct), v.to(ct)
+    pos, q_pos = torch.arange(slots), slots + torch.arange(T)
+    weight = torch.zeros(slots, device=dev)
+    announce(f"attend, many slots beside a large one T={T} heads={heads}/{kv} D={D} slots={slots} {qt} over {ct}")
+    o = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), q_pos.to(dev), scale=1.0, weight=weight).cpu()
+    want, p, xmax = _formula(q[:1], k, v, torch.ones(1, slots, dtype=torch.bool), 1.0)
+    e = 2.0 ** -24 * ((D + 2) * xmax + slots / 16 + 64)
+    half = torch.finfo(qt).eps / 2 if qt != F32 else 0.0
+    bound = want * (2 * e + half) + slots * 2.0 ** -39
+    bound = bound + (want + bound) * torch.finfo(qt).eps / 2
+    off = (o.double() - want).abs()
+    assert bool((off <= bound).all()), f"worst {float((off / bound).max()):.3g} of the bound"
+    w = p[0] * T
+    off = (weight.cpu().double() - w).abs()
+    assert bool((off <= (2 * e + 2.0 ** -24 * (T * heads / 4 + 6)) * w + 1e-30).all())
