@@ -887,6 +887,10 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
   }
   if (row >= R) return;
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  if (l == 0.0f) {  // (scores of -infinity alone; infinities of V have made its sums NaN)
+#pragma unroll
+    for (int e = 0; e < EV; ++e) o[e] = (f32x16)(0.0f);
+  }
   const int64_t out = (int64_t)tok * a.o_st + (int64_t)(kvh * a.rep + row % a.rep) * a.o_sh;
 #pragma unroll
   for (int v = 0; v < 16; ++v) {

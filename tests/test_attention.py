@@ -541,3 +541,24 @@ def test_attend_many_slots_beside_a_large_one(dev, T, heads, kv, D, slots, qt, c
     w = p[0] * T
     off = (weight.cpu().double() - w).abs()
     assert bool((off <= (2 * e + 2.0 ** -24 * (T * heads / 4 + 6)) * w + 1e-30).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,heads,kv,slots", [(768, 64, 64, 5504), (64, 8, 1, 8300), (6, 8, 2, 700), (15, 8, 2, 36001)])
+@pytest.mark.parametrize("ct", [F16, BF16], ids=["f16", "bf16"])
+def test_attend_only_scores_of_minus_infinity(dev, T, heads, kv, slots, ct):
+    """A row whose scores are all -infinity is 0, whatever the values; in
+    kernels with and without a joining launch."""
+    g = torch.Generator().manual_seed(T)
+    D = 64
+    q, k, v = (torch.randn(n, h, D, generator=g) for n, h in ((T, heads), (slots, kv), (slots, kv)))
+    k[..., 0] = 1.0
+    q[5, :, 0] = float("-inf")
+    v[3, :, 1], v[slots - 2, :, 2] = float("inf"), float("nan")
+    announce(f"attend, scores of -infinity T={T} heads={heads}/{kv} slots={slots} {ct}")
+    o = tree_attention(q.to(dev, ct), k.to(dev, ct), v.to(dev, ct), torch.arange(slots, device=dev),
+                       torch.full((T,), slots, device=dev)).cpu()
+    assert bool((o[5] == 0).all())
+    rest = [t for t in range(T) if t != 5]
+    assert bool((o[rest][..., 1] == float("inf")).all()) and bool(torch.isnan(o[rest][..., 2]).all())
+    assert bool(torch.isfinite(o[rest][..., [0] + list(range(3, D))]).all())
