@@ -42,7 +42,7 @@ inline bool y_vec_ok(const void* y, int yt, int64_t ldy, int64_t N) {
 }
 
 inline bool valid_group(int group) { return group == 32 || group == 64 || group == 128; }
-// Sizes whose packing launches fit a grid (one thread per 8 columns).
+// Rows and columns that an int holds with their padding, weights of up to 1 TiB packed.
 inline bool w4_size_ok(int64_t N, int64_t K) { return N <= (1 << 30) && K <= (1 << 30) && (N + 15) * (K + 127) <= (int64_t)1 << 41; }
 
 // W8A8 workspace layout (from the first 256-byte boundary): min/max partials

@@ -35,6 +35,7 @@
 
 #include "sbq_common.h"
 #include "sbq_dma.h"
+#include "sbq_launch.h"
 
 namespace sbq {
 
@@ -1237,15 +1238,22 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
       return hipGetLastError() == hipSuccess ? 0 : -5;
     }
   }
-  const dim3 grid((unsigned)((a.slots + SB - 1) / SB));
-  if (mode == 2)
-    attn_weight_kernel<CT, M16, DP, 2><<<grid, threads, 0, st>>>(a, weight);
-  else if (mode == 1)
-    attn_weight_kernel<CT, M16, DP, 1><<<grid, threads, 0, st>>>(a, weight);
-  else if constexpr (!M16)
-    attn_weight_kernel<CT, M16, DP, 0><<<grid, threads, 0, st>>>(a, weight);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : -5;
+  constexpr int64_t kStep = kLaunchThreads / threads * SB;  // slots per launch
+  for (int64_t s = 0; s < a.slots; s += kStep) {
+    AttnArgs part = a;
+    part.k = (const typename XElem<CT>::T*)a.k + s * a.k_ss;
+    part.slot_pos = a.slot_pos + s;
+    part.slots = (int)(a.slots - s < kStep ? a.slots - s : kStep);
+    const dim3 grid((unsigned)((part.slots + SB - 1) / SB));
+    if (mode == 2)
+      attn_weight_kernel<CT, M16, DP, 2><<<grid, threads, 0, st>>>(part, weight + s);
+    else if (mode == 1)
+      attn_weight_kernel<CT, M16, DP, 1><<<grid, threads, 0, st>>>(part, weight + s);
+    else if constexpr (!M16)
+      attn_weight_kernel<CT, M16, DP, 0><<<grid, threads, 0, st>>>(part, weight + s);
+    if (hipGetLastError() != hipSuccess) return -5;
+  }
+  return 0;
 }
 
 // `weight` null: the attention (RT 0: attn_tile_kernel); else the slots'

@@ -466,8 +466,9 @@ __global__ __launch_bounds__(kSelThreads) void kv_append_kernel(AppendArgs a) {
 }
 
 template <int ST, int DT>
-__global__ __launch_bounds__(256) void kv_rows_kernel(AppendArgs a) {
-  copy_row<ST, DT>(a.fresh, blockIdx.x, a.cache, a.list[blockIdx.x], a.D, threadIdx.x, a.Hk * a.D, 256);
+__global__ __launch_bounds__(256) void kv_rows_kernel(AppendArgs a, int first) {
+  const int i = first + (int)blockIdx.x;
+  copy_row<ST, DT>(a.fresh, i, a.cache, a.list[i], a.D, threadIdx.x, a.Hk * a.D, 256);
 }
 
 struct TakeArgs {
@@ -523,8 +524,8 @@ __global__ __launch_bounds__(kSelThreads) void kv_take_kernel(TakeArgs a) {
   }
 }
 
-__global__ __launch_bounds__(256) void kv_take_rows_kernel(TakeArgs a) {
-  const int i = blockIdx.x;
+__global__ __launch_bounds__(256) void kv_take_rows_kernel(TakeArgs a, int first) {
+  const int i = first + (int)blockIdx.x;
   if (i >= a.list[a.capacity]) {
     if (threadIdx.x == 0) {
       a.to_pos[i] = -1;
@@ -546,6 +547,7 @@ __global__ __launch_bounds__(256) void kv_take_rows_kernel(TakeArgs a) {
   }
 }
 
+constexpr int64_t kRowsStep = kLaunchThreads / 256;  // rows per launch
 constexpr int kInlineElems = 1 << 12;  // key elements that the selecting workgroup still writes itself
 
 template <int ST, int DT>
@@ -564,9 +566,12 @@ int append_types(const AppendArgs& a, hipStream_t st) {
   }
   kv_append_kernel<ST, DT><<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(n), st>>>(a);
   rc = check_launch();
-  if (rc || a.rows_too) return rc;
-  kv_rows_kernel<ST, DT><<<a.T, 256, 0, st>>>(a);
-  return check_launch();
+  if (a.rows_too) return rc;
+  for (int64_t i = 0; i < a.T && !rc; i += kRowsStep) {
+    kv_rows_kernel<ST, DT><<<(unsigned)(a.T - i < kRowsStep ? a.T - i : kRowsStep), 256, 0, st>>>(a, (int)i);
+    rc = check_launch();
+  }
+  return rc;
 }
 
 template <int ST>
@@ -614,10 +619,12 @@ int launch_kv_take(const KvTake& c, hipStream_t st) {
     if (rc) return rc;
   }
   kv_take_kernel<<<1, kSelThreads, (size_t)(kSelThreads * 4) << keys_log(a.n), st>>>(a);
-  const int rc = check_launch();
-  if (rc) return rc;
-  kv_take_rows_kernel<<<a.capacity, 256, 0, st>>>(a);
-  return check_launch();
+  int rc = check_launch();
+  for (int64_t i = 0; i < a.capacity && !rc; i += kRowsStep) {
+    kv_take_rows_kernel<<<(unsigned)(a.capacity - i < kRowsStep ? a.capacity - i : kRowsStep), 256, 0, st>>>(a, (int)i);
+    rc = check_launch();
+  }
+  return rc;
 }
 
 }  // namespace sbq

@@ -14,6 +14,10 @@ inline int check_launch() {
   return e == hipSuccess ? 0 : -5;
 }
 
+// A grid holds fewer than 2^32 threads along an axis; what grows with the size
+// of a whole weight or cache is launched in parts of so many threads.
+constexpr int64_t kLaunchThreads = (int64_t)1 << 28;
+
 // One pass over weight rows (sbq_quant.hip pack_weight_kernel): wt a dtype
 // (quantize_per_channel) or XT_S8 (rows as they are); scale is for a dtype
 // only; q, packed, colsum: each may be null.

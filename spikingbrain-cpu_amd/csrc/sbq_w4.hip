@@ -645,49 +645,79 @@ int pick_w4(const W4Args& a, bool xvec, int group, hipStream_t st) {
 int launch_quantize_groups(const void* w, int wt, int64_t N, int64_t K, int64_t ldw, int group, int8_t* q, int64_t ldq,
                            uint16_t* scale, hipStream_t st) {
   const int Gn = (int)((K + group - 1) / group);
-  const unsigned grid = (unsigned)((N * Gn + 7) / 8);
-  if (wt == XT_F32)
-    quantize_groups_kernel<XT_F32><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
-  else if (wt == XT_F16)
-    quantize_groups_kernel<XT_F16><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
-  else
-    quantize_groups_kernel<XT_BF16><<<grid, 256, 0, st>>>(w, ldw, (int)N, (int)K, group, Gn, q, ldq, scale);
-  return check_launch();
+  const int64_t es = wt == XT_F32 ? 4 : 2, step = kLaunchThreads / 32 / Gn > 0 ? kLaunchThreads / 32 / Gn : 1;
+  for (int64_t n = 0; n < N; n += step) {
+    const int rows = (int)(N - n < step ? N - n : step);
+    const unsigned grid = (unsigned)(((int64_t)rows * Gn + 7) / 8);
+    const void* const wn = (const uint8_t*)w + n * ldw * es;
+    int8_t* const qn = q + n * ldq;
+    uint16_t* const sn = scale + n * Gn;
+    if (wt == XT_F32)
+      quantize_groups_kernel<XT_F32><<<grid, 256, 0, st>>>(wn, ldw, rows, (int)K, group, Gn, qn, ldq, sn);
+    else if (wt == XT_F16)
+      quantize_groups_kernel<XT_F16><<<grid, 256, 0, st>>>(wn, ldw, rows, (int)K, group, Gn, qn, ldq, sn);
+    else
+      quantize_groups_kernel<XT_BF16><<<grid, 256, 0, st>>>(wn, ldw, rows, (int)K, group, Gn, qn, ldq, sn);
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
+  return 0;
 }
+
+// 16-row tiles that a packing launch takes.
+static int64_t tiles_step(int64_t Kc) { return kLaunchThreads / 256 / Kc > 0 ? kLaunchThreads / 256 / Kc : 1; }
 
 int launch_repack_w4(const int8_t* q, int64_t N, int64_t K, int64_t ldq, const uint16_t* scale, int group, uint8_t* packed,
                      uint16_t* gscale, hipStream_t st) {
-  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gp = Kc * (128 / group);
-  const int64_t words = Nt * Kc * 256, scales = Nt * Gp * 16;
-  pack_w4_kernel<<<blocks(words), 256, 0, st>>>(q, ldq, (int)N, (int)K, (int)Kc, words, (uint32_t*)packed);
-  pack_scale_kernel<<<blocks(scales), 256, 0, st>>>(scale, (int)N, (int)((K + group - 1) / group), (int)Gp, scales, gscale);
-  return check_launch();
+  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gp = Kc * (128 / group), Gn = (K + group - 1) / group;
+  const int64_t step = tiles_step(Kc);
+  for (int64_t t = 0; t < Nt; t += step) {
+    const int64_t tiles = Nt - t < step ? Nt - t : step, words = tiles * Kc * 256, scales = tiles * Gp * 16;
+    const int rows = (int)(N - t * 16 < tiles * 16 ? N - t * 16 : tiles * 16);
+    pack_w4_kernel<<<blocks(words), 256, 0, st>>>(q + t * 16 * ldq, ldq, rows, (int)K, (int)Kc, words,
+                                                  (uint32_t*)packed + t * Kc * 256);
+    pack_scale_kernel<<<blocks(scales), 256, 0, st>>>(scale + t * 16 * Gn, rows, (int)Gn, (int)Gp, scales,
+                                                      gscale + t * Gp * 16);
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 int launch_unpack_w4(const uint8_t* packed, const uint16_t* gscale, int64_t N, int64_t K, int group, int8_t* q, int64_t ldq,
                      uint16_t* scale, hipStream_t st) {
-  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gn = (K + group - 1) / group;
-  const int64_t words = Nt * Kc * 256, scales = N * Gn;
-  unpack_w4_kernel<<<blocks(words), 256, 0, st>>>((const uint32_t*)packed, (int)N, (int)K, (int)Kc, words, q, ldq);
-  unpack_scale_kernel<<<blocks(scales), 256, 0, st>>>(gscale, (int)Gn, (int)(Kc * (128 / group)), scales, scale);
-  return check_launch();
+  const int64_t Nt = (N + 15) / 16, Kc = (K + 127) / 128, Gp = Kc * (128 / group), Gn = (K + group - 1) / group;
+  const int64_t step = tiles_step(Kc);
+  for (int64_t t = 0; t < Nt; t += step) {
+    const int64_t tiles = Nt - t < step ? Nt - t : step, words = tiles * Kc * 256;
+    const int64_t rows = N - t * 16 < tiles * 16 ? N - t * 16 : tiles * 16, scales = rows * Gn;
+    unpack_w4_kernel<<<blocks(words), 256, 0, st>>>((const uint32_t*)packed + t * Kc * 256, (int)rows, (int)K, (int)Kc, words,
+                                                    q + t * 16 * ldq, ldq);
+    unpack_scale_kernel<<<blocks(scales), 256, 0, st>>>(gscale + t * Gp * 16, (int)Gn, (int)Gp, scales, scale + t * 16 * Gn);
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 int launch_linear_w4(const void* x, int xt, int64_t M, int64_t K, int64_t ldx, bool xvec, const uint8_t* packed,
                      const uint16_t* gscale, const float* bias, int64_t N, int group, void* y, int yt, int64_t ldy, bool yvec,
                      hipStream_t st) {
   constexpr int64_t kRows = 1 << 20;  // rows per launch (the grid's second dimension holds 65535 blocks)
-  const int64_t xs = xt == XT_F32 ? 4 : 2, ys = yt == XT_F32 ? 4 : 2;
+  constexpr int64_t kTiles = kLaunchThreads / (kW4MaxWaves * 64);  // weight tiles per launch
+  const int64_t xs = xt == XT_F32 ? 4 : 2, ys = yt == XT_F32 ? 4 : 2, Nt = (N + 15) / 16, Kc = (K + 127) / 128;
   xvec = xvec && K * xs % 16 == 0;
-  for (int64_t m = 0; m < M; m += kRows) {
-    const W4Args a{(const uint8_t*)x + m * ldx * xs, packed, gscale, bias, (uint8_t*)y + m * ldy * ys, ldx, ldy,
-                   (int)(M - m < kRows ? M - m : kRows), (int)N, (int)K, (int)((N + 15) / 16), (int)((K + 127) / 128), yt,
-                   yvec};
-    const int rc = xt == XT_F32   ? pick_w4<XT_F32>(a, xvec, group, st)
-                   : xt == XT_F16 ? pick_w4<XT_F16>(a, xvec, group, st)
-                                  : pick_w4<XT_BF16>(a, xvec, group, st);
-    if (rc) return rc;
-  }
+  for (int64_t m = 0; m < M; m += kRows)
+    for (int64_t t = 0; t < Nt; t += kTiles) {
+      const int64_t tiles = Nt - t < kTiles ? Nt - t : kTiles, n = t * 16, rest = N - n < tiles * 16 ? N - n : tiles * 16;
+      const W4Args a{(const uint8_t*)x + m * ldx * xs, packed + t * Kc * 1024, gscale + t * Kc * (128 / group) * 16,
+                     bias ? bias + n : nullptr, (uint8_t*)y + (m * ldy + n) * ys, ldx, ldy,
+                     (int)(M - m < kRows ? M - m : kRows), (int)rest, (int)K, (int)tiles, (int)Kc, yt, yvec};
+      const int rc = xt == XT_F32   ? pick_w4<XT_F32>(a, xvec, group, st)
+                     : xt == XT_F16 ? pick_w4<XT_F16>(a, xvec, group, st)
+                                    : pick_w4<XT_BF16>(a, xvec, group, st);
+      if (rc) return rc;
+    }
   return 0;
 }
 
