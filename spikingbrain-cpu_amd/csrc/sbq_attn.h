@@ -1204,29 +1204,36 @@ __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(
 template <int CT, bool M16, int DP>
 int launch_attn_dp(const AttnArgs& a, int mode, int RT, hipStream_t st) {
   const dim3 grid((unsigned)(a.Hk * a.rtiles * a.splits));
-  if (mode == 2) {
-    bool done = false;
+  if (RT == 2) {
     if constexpr (M16 || DP < 256) {  // (two tiles of 256 fp32 columns do not fit the registers)
-      if ((done = RT == 2)) attn_kernel<CT, M16, DP, 2, 2><<<grid, kAttnWaves * 64, 0, st>>>(a);
+      if (mode != 2) return -1;
+      attn_kernel<CT, M16, DP, 2, 2><<<grid, kAttnWaves * 64, 0, st>>>(a);
+    } else {
+      return -1;  // no such kernel (the plan never asks for it)
     }
-    if (!done) attn_kernel<CT, M16, DP, 2, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
+  } else if (RT != 1) {
+    return -1;
+  } else if (mode == 2) {
+    attn_kernel<CT, M16, DP, 2, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
   } else if (mode == 1) {
     attn_kernel<CT, M16, DP, 1, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
   } else if constexpr (!M16) {
     attn_kernel<CT, M16, DP, 0, 1><<<grid, kAttnWaves * 64, 0, st>>>(a);
+  } else {
+    return -1;
   }
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : -5;
+  return check_launch();
 }
 
 template <int CT, int DP>
 int launch_tile_dp(const AttnArgs& a, hipStream_t st) {
   constexpr int lds = kTileBufs * 2 * kTileSlots * DP * 2;
   attn_tile_kernel<CT, DP><<<dim3((unsigned)(a.Hk * a.rtiles * a.splits)), kTileWaves * 64, lds, st>>>(a);
-  if (hipGetLastError() != hipSuccess) return -5;
+  const int rc = check_launch();
+  if (rc) return rc;
   if (a.splits > 1)
     attn_tile_join_kernel<DP><<<dim3((unsigned)(a.Hk * ((a.rep * a.T + 31) / 32) * 16)), 64, 0, st>>>(a);
-  return hipGetLastError() == hipSuccess ? 0 : -5;
+  return check_launch();
 }
 
 template <int CT, bool M16, int DP>
@@ -1235,7 +1242,7 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
   if constexpr (M16 && DP <= 128) {
     if (mode == 2 && a.qvec && a.rep * a.T >= kWeightTileRows && a.slots >= kWeightTileSlots) {
       attn_weight_tile_kernel<CT, DP><<<(unsigned)((a.slots + 255) / 256), threads, kWeightBufs * (64 * DP * 2 + 512), st>>>(a, weight);
-      return hipGetLastError() == hipSuccess ? 0 : -5;
+      return check_launch();
     }
   }
   constexpr int64_t kStep = kLaunchThreads / threads * SB;  // slots per launch
@@ -1251,7 +1258,10 @@ int launch_weight_dp(const AttnArgs& a, int mode, float* weight, hipStream_t st)
       attn_weight_kernel<CT, M16, DP, 1><<<grid, threads, 0, st>>>(part, weight + s);
     else if constexpr (!M16)
       attn_weight_kernel<CT, M16, DP, 0><<<grid, threads, 0, st>>>(part, weight + s);
-    if (hipGetLastError() != hipSuccess) return -5;
+    else
+      return -1;
+    const int rc = check_launch();
+    if (rc) return rc;
   }
   return 0;
 }

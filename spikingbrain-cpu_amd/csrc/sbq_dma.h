@@ -1,5 +1,5 @@
 // sbq_dma.h - global -> LDS copy helpers and waits shared by the tiled GEMM
-// GEMM kernels (sbq_gemm.hip).
+// (sbq_gemm.hip), the 4-bit linears (sbq_w4.hip) and the attention (sbq_attn.h).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -385,6 +385,10 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void linear_w4_kernel(W4Args a) {
 // and reads fragments there: 64 rows over 12288 x 4096, bf16, 39.5 us without,
 // 19 with.  Two chunks and one K tile's weights are always under way; the last
 // ones of a wave once more.
+// Order of issue, a K tile's weights w(i) and chunks c(i): w0 c0 c1, w1 after
+// w0 is read, then a chunk after each one read.  With two or more chunks a K
+// tile, w(i) is older than the two chunks under way; with one it is between
+// them, and only the compiler's own wait for its registers retires it.
 template <int XT, int MT, int G, int GS>
 __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
   typedef typename XElem<XT>::T T;
@@ -435,7 +439,7 @@ __global__ __launch_bounds__(kW4MaxWaves * 64) void rows_w4_kernel(W4Args a) {
 
   int buf = 0;
   auto tile = [&](int kt, const u32x2 (&b)[G][GPT], u32x2 (&next)[G][GPT]) {
-    wait_vmcnt<2 * NDMA>();  // the weights; the two chunks after them stay under way
+    wait_vmcnt<2 * NDMA>();  // the weights where NCH > 1; the two chunks after them stay under way
     asm volatile("" ::: "memory");
     V wv[G][4];
 #pragma unroll
@@ -605,11 +609,15 @@ int launch_rows_w4(const W4Args& a, int group, int KS, hipStream_t st) {
   const size_t lds = (size_t)(stage > red ? stage : red);
   const dim3 grid((unsigned)((a.Nt + G - 1) / G), (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
   if (group == 32) {
-    if constexpr (G < 3 || (MT < 4 && XT != XT_F32)) rows_w4_kernel<XT, MT, G, 1><<<grid, KS * 64, lds, st>>>(a);
-  } else if (group == 64)
+    if constexpr (G < 3 || (MT < 4 && XT != XT_F32))
+      rows_w4_kernel<XT, MT, G, 1><<<grid, KS * 64, lds, st>>>(a);
+    else
+      return -1;  // no such kernel (rows_w4 never asks for it)
+  } else if (group == 64) {
     rows_w4_kernel<XT, MT, G, 2><<<grid, KS * 64, lds, st>>>(a);
-  else
+  } else {
     rows_w4_kernel<XT, MT, G, 4><<<grid, KS * 64, lds, st>>>(a);
+  }
   return check_launch();
 }
 template <int XT, int MT>
