@@ -485,3 +485,44 @@ def test_zeros_of_either_sign_are_equal(dev, n, T):
             b, pos = small, np.delete(np.arange(n), at)
             want = w[pos]
         assert torch.equal(b.slot_pos.cpu(), torch.from_numpy(pos)) and _same(b.weight, torch.from_numpy(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ct", [F32, BF16], ids=["f32", "bf16"])
+def test_prompt_weights_slot_by_slot(dev, ct):
+    """A prompt in chunks with its weights counted, then drafts: every slot's
+    sum against the formula in 64 bits, to its own bound, which a single query
+    row of one head left out (of the formula) would pass.  A weight is off by
+    2 e of itself, e = 2^-24 ((D + 2) times the largest sum of |scale q k|, n / 16
+    + 64 roundings in sums of weights), a sum by 2^-24 for each of the T * heads / 4
+    + 6 terms that a lane adds."""
+    heads, kv, D, prompt, chunk, T = 8, 2, 64, 300, 100, 9
+    g = torch.Generator().manual_seed(12)
+    buf = DeviceKVBuffer(kv, D, prompt, None, dev, ct)
+    weight = torch.zeros(prompt, device=dev)
+    for at in list(range(0, prompt, chunk)) + [prompt]:
+        n = chunk if at < prompt else T
+        q, k, v = ((torch.randn(n, h, D, generator=g) * 1.5).to(dev, ct) for h in (heads, kv, kv))
+        q_pos = at + torch.arange(n)
+        before = weight.cpu().double()
+        announce(f"prompt weights at {at} {ct}")
+        if at < prompt:
+            buf.append(k, v)
+            buf.attend(q, q_pos.to(dev), weight=weight)
+            keys, see = buf.k.cpu().double(), torch.arange(prompt)[None] <= q_pos[:, None]
+        else:
+            buf.attend(q, q_pos.to(dev), k, v, weight=weight)
+            keys = torch.cat([buf.k, k]).cpu().double()
+            see = torch.cat([torch.ones(n, prompt, dtype=torch.bool), torch.ones(n, n, dtype=torch.bool).tril()], 1)
+        p, xmax = torch.zeros(n, heads, keys.shape[0], dtype=torch.float64), 0.0
+        for h in range(heads):
+            qh, kh = q[:, h].cpu().double(), keys[:, h // (heads // kv)]
+            xmax = max(xmax, float((qh.abs() @ kh.abs().t()).max()) * D ** -0.5)
+            p[:, h] = torch.softmax((qh @ kh.t() * D ** -0.5).masked_fill(~see, float("-inf")), -1)
+        w = p.sum((0, 1))[:prompt]
+        e = 2.0 ** -24 * ((D + 2) * xmax + keys.shape[0] / 16 + 64)
+        bound = 2 * e * w + 2.0 ** -24 * (w + before) * (n * heads / 4 + 6) + 1e-30
+        off = weight.cpu().double() - before - w
+        assert bool((off.abs() <= bound).all()), f"worst {float((off.abs() / bound).max()):.3g} of the bound"
+        without = off + p[..., :prompt]  # the distance where this row's and head's weights were not counted
+        assert bool((without.abs() > bound).any(-1).all())
