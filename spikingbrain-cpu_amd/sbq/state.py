@@ -95,7 +95,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
     if T > _lib.SBQ_ATTN_MAX_T:
         raise ValueError(f"tree_attention: at most {_lib.SBQ_ATTN_MAX_T} tokens per call")
     ks = k.stride()
-    if k.get_device() != gpu or v.get_device() != gpu or ks != v.stride() or (dim > 1 and ks[2] != 1):
+    if (k.get_device() != gpu or v.get_device() != gpu or (dim > 1 and ks[2] != 1)
+            or (ks != v.stride() and any(n > 1 and a != b for n, a, b in zip(k.shape, ks, v.stride())))):
         raise ValueError(f"tree_attention: k and v must be on {q.device}, with the same strides and unit stride in dim")
     if (slot_pos.dtype != torch.int64 or slot_pos.get_device() != gpu or slot_pos.shape != (slots,)
             or not slot_pos.is_contiguous()):

@@ -562,3 +562,19 @@ def test_attend_only_scores_of_minus_infinity(dev, T, heads, kv, slots, ct):
     rest = [t for t in range(T) if t != 5]
     assert bool((o[rest][..., 1] == float("inf")).all()) and bool(torch.isnan(o[rest][..., 2]).all())
     assert bool(torch.isfinite(o[rest][..., [0] + list(range(3, D))]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+def test_attend_strides_of_single_entries(dev, qt, ct):
+    """The stride of an axis of one entry does not count: one key head, one slot, one column."""
+    g = torch.Generator().manual_seed(13)
+    for slots, kv, D in ((90, 1, 64), (1, 2, 64), (1, 1, 16), (40, 2, 1)):
+        q, k, v = (torch.randn(n, h, D, generator=g) for n, h in ((2, 4), (slots, kv), (slots, kv)))
+        q, k, v = q.to(qt), k.to(ct), v.to(ct)
+        pos, q_pos = torch.arange(slots), torch.tensor([slots, slots + 1])
+        vd, (s0, s1, s2) = v.to(dev), v.stride()
+        vd = vd.as_strided(v.shape, (s0 if slots > 1 else 7, s1 if kv > 1 else 5, s2 if D > 1 else 3))
+        announce(f"strides of single entries slots={slots} kv={kv} D={D} {qt} over {ct}")
+        o = tree_attention(q.to(dev), k.to(dev), vd, pos.to(dev), q_pos.to(dev))
+        _compare(o.cpu(), None, None, q, k, v, _see(pos, q_pos, None, None), D ** -0.5, slots)
