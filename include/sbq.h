@@ -528,7 +528,9 @@ int sbq_tree_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int
  * rounded to the cache's type and written to k, v (device [slots, kv_heads,
  * D], strides k_ss and k_sh), slot_pos is set, weight is 0, and *end = *start
  * + T.  start, end: device int64[1], the same one or not.  0 <= recent <=
- * slots, T <= slots.  k_new and v_new must not overlap the cache.
+ * slots, T <= slots.  k_new and v_new must not overlap the cache.  Slots that
+ * hold positions from *start on already are not replaced: where tokens are taken
+ * back, free their slots (slot_pos -1) first.
  *
  * sbq_kv_take: the used slots among the last `capacity` of that order (newest:
  * >= *end - recent) of a cache of any size are copied, in slot order, to the

@@ -256,7 +256,9 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
         """Store k, v [T, heads, dim] at positions start .. start + T - 1
         (default: after the last append), T <= capacity; start may be an int
         or a device tensor.  Free slots are taken first, then those of least
-        weight (equal ones by slot), in ascending slot order."""
+        weight (equal ones by slot), in ascending slot order.  Going back to an
+        earlier start, truncate(start) first: positions from start on that the
+        buffer holds would stay beside the new ones (and count as newest)."""
         kv = self.k
         gpu = kv.get_device()
         if k.shape != v.shape or k.dim() != 3 or k.shape[1] != self.heads or k.shape[2] != self.dim:

@@ -8,7 +8,7 @@ import torch
 
 from conftest import announce
 from sbq import _lib, quant
-from sbq.state import DeviceBudgetKVBuffer, DeviceKVBuffer, new_device_state
+from sbq.state import DeviceBudgetKVBuffer, DeviceKVBuffer, new_device_state, tree_attention
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -526,3 +526,35 @@ def test_prompt_weights_slot_by_slot(dev, ct):
         assert bool((off.abs() <= bound).all()), f"worst {float((off.abs() / bound).max()):.3g} of the bound"
         without = off + p[..., :prompt]  # the distance where this row's and head's weights were not counted
         assert bool((without.abs() > bound).any(-1).all())
+
+
+@pytest.mark.gpu
+def test_tokens_taken_back(dev):
+    """truncate, then appends from there on: every position is held once, freed
+    slots go first, and the attention is that of the tokens that are left."""
+    kv, D, n, heads = 2, 64, 24, 4
+    g = torch.Generator().manual_seed(14)
+    buf, line = DeviceBudgetKVBuffer(kv, D, n, 4, dev), DeviceKVBuffer(kv, D, 200, None, dev)
+    end = 0
+    for i in range(12):
+        k, v = (torch.randn(5, kv, D, generator=g).to(dev) for _ in range(2))
+        if i % 3 == 2:
+            end -= 4
+            buf.truncate(end), line.truncate(end)
+        buf.append(k, v, end), line.append(k, v, end)
+        end += 5
+        held = sorted(p for p in buf.slot_pos.tolist() if p >= 0)
+        assert len(set(held)) == len(held) and int(buf.end) == end and set(range(end - 4, end)) <= set(held)
+        assert len(held) == min(n, end) or i % 3 == 2
+        at = buf.slot_pos.cpu()
+        for slot in (at >= 0).nonzero().flatten().tolist():
+            assert torch.equal(buf.k[slot], line.k[int(at[slot])]) and torch.equal(buf.v[slot], line.v[int(at[slot])])
+        q, q_pos = torch.randn(2, heads, D, generator=g).to(dev), torch.tensor([end - 2, end - 1], device=dev)
+        announce(f"tokens taken back, step {i}")
+        o = buf.attend(q, q_pos)
+        keep = torch.full_like(line.slot_pos, -1)
+        keep[held] = torch.tensor(held, device=dev)
+        # each side: weights to e = 2^-24 ((D + 2) sum |scale q k| + 66), outputs to 2 e max |v|
+        e = 2.0 ** -24 * ((D + 2) * float(q.abs().sum(-1).max() * line.k.abs().max()) * D ** -0.5 + 66)
+        other = tree_attention(q, line.k, line.v, keep, q_pos)
+        assert torch.allclose(o, other, rtol=0, atol=4 * e * float(line.v.abs().max()))
