@@ -495,7 +495,7 @@ int sbq_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
  * Scores, maxima and sums are fp32; with 2-byte queries the weights p are
  * rounded to their type (half to even; in fp16 at half a step of each down to
  * 2^-28 of the largest) for the product with v, with F32 queries everything is
- * fp32.  Unit strides and 16-byte aligned rows of a
+ * fp32.  scale * q . k is to stay below 2^27 in magnitude, or be infinite.  Unit strides and 16-byte aligned rows of a
  * D of 64, 128 or 256 are the fastest.
  * weight: NULL, or device fp32 [slots]: weight[s] += sum_{t,h} p[t,h,s], the
  * attention weight the cached slots received (for eviction by it); calls

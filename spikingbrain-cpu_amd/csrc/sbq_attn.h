@@ -21,8 +21,8 @@
 // from memory straight to registers; LDS only joins the waves.
 //
 // M16: 2-byte cache and queries of one type on 16x16x32, the weights rounded
-// to that type (half a step each, averaged over the slots of a sum, see kUp;
-// the sum of weights itself stays in fp32).  Otherwise all products are fp32
+// to that type (half a step each, averaged over the slots of a sum, see
+// reference(); the sum of weights itself stays in fp32).  Otherwise all products are fp32
 // (16x16x4), whatever the cache holds.
 //
 // The blocks are dealt in turn to the waves of all `splits` workgroups of a
@@ -116,14 +116,19 @@ struct AttnMath<XT_F32> {
   typedef f32x4 V;
 };
 
-// The softmax's weights are taken against 2^-kUp of the running maximum, up to
-// 2^kUp: rounded to fp16 for the product with V, one far below the largest
-// (many slots beside one that takes most of the weight) keeps all bits down to
-// 2^-28 of it, where against the maximum itself they end at 2^-14 and the
-// weight at 2^-25.  Sums and partial results carry the factor until the sum of
-// weights divides it out.  bf16 has fp32's exponents.
+// What a block's weights are taken against, from its largest score: fp16 weights
+// against 2^-14 of it, up to 2^14.  Rounded for the product with V, one far
+// below the largest (many slots beside one that takes most of the weight) keeps
+// all bits down to 2^-28 of it, where against the maximum itself they end at
+// 2^-14 and the weight at 2^-25.  Sums and partial results carry the factor
+// until the sum of weights divides it out.  From 2^23 on the maximum's own
+// rounding is half a power and more, which the room above 2^14 is left to.
+// bf16 has fp32's exponents.
 template <int CT, bool M16>
-constexpr float kUp = M16 && CT == XT_F16 ? 14.0f : 0.0f;
+__device__ __forceinline__ float reference(float mx) {
+  if constexpr (M16 && CT == XT_F16) return __builtin_fabsf(mx) < 8388608.0f ? mx - 14.0f : mx;
+  return mx;
+}
 
 __device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
   return qt == XT_F32 ? ((const float*)q)[i] : qt == XT_F16 ? (float)((const _Float16*)q)[i] : (float)((const __bf16*)q)[i];
@@ -377,8 +382,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 #pragma unroll
           for (int v = 0; v < 4; ++v) mx = seen[i] >> (st * 4 + v) & 1 ? __builtin_fmaxf(mx, p[i][st][v]) : mx;
       }
-      mx *= a.scale;
-      if constexpr (kUp<CT, M16> != 0.0f) mx -= kUp<CT, M16>;
+      mx = reference<CT, M16>(mx * a.scale);
       if (__any(mx > m[i])) {
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -698,8 +702,7 @@ __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs 
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = seen >> v & 1 ? __builtin_fmaxf(mx, s[v]) : mx;
     }
-    mx *= a.scale;
-    if constexpr (kUp<CT, true> != 0.0f) mx -= kUp<CT, true>;
+    mx = reference<CT, true>(mx * a.scale);
     if (__any(mx > m)) {
       mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float up = __builtin_fmaxf(m, mx);

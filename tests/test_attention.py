@@ -578,3 +578,32 @@ def test_attend_strides_of_single_entries(dev, qt, ct):
         announce(f"strides of single entries slots={slots} kv={kv} D={D} {qt} over {ct}")
         o = tree_attention(q.to(dev), k.to(dev), vd, pos.to(dev), q_pos.to(dev))
         _compare(o.cpu(), None, None, q, k, v, _see(pos, q_pos, None, None), D ** -0.5, slots)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt,ct", TYPES, ids=IDS)
+@pytest.mark.parametrize("T,heads,kv,D,slots", [(1, 4, 2, 64, 300), (40, 2, 1, 80, 200), (8, 8, 1, 128, 70000), (64, 8, 1, 64, 8300)])
+def test_attend_very_large_scores(dev, T, heads, kv, D, slots, qt, ct):
+    """Scores (times log2 e) up to 2^27, of either sign, products and sums exact
+    in fp32 and more than 2^12 apart or equal: a row is the mean of the values
+    of its largest score, to the rounding of the mean and of the output."""
+    g = torch.Generator().manual_seed(slots)
+    for top in (2 ** 10, 2 ** 22, 2 ** 23, 2 ** 24, 2 ** 25, 2 ** 26):
+        for sign in (1, -1):
+            q, k, v = torch.zeros(T, heads, D), torch.zeros(slots, kv, D), torch.randn(slots, kv, D, generator=g)
+            b = min(4096, top // 64)                 # query times key: b * (top / b) (1 - i / 16), i = 0..7
+            q[..., 0] = b * sign
+            k[..., 0] = (top // b) * (1 - torch.randint(0, 8, (slots, kv), generator=g) / 16)
+            q, k, v = q.to(qt), k.to(ct), v.to(ct)
+            pos, q_pos = torch.arange(slots), torch.full((T,), slots)
+            announce(f"attend, scores {sign * top} T={T} heads={heads}/{kv} D={D} slots={slots} {qt} over {ct}")
+            o = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), q_pos.to(dev), scale=1.0).cpu().double()
+            z = q[0, 0, 0].double() * k[..., 0].double()
+            for h in range(heads):
+                zh, vh = z[:, h // (heads // kv)], v[:, h // (heads // kv)].double()
+                want = vh[zh == zh.max()].mean(0)
+                tol = (slots / 16 + 64) * 2.0 ** -24 * float(vh.abs().max())
+                tol = tol + (want.abs() + tol) * torch.finfo(qt).eps / 2
+                if qt != F32:  # the weights' roundings
+                    tol = tol + torch.finfo(qt).eps / 2 * float(vh.abs().max())
+                assert bool(((o[:, h] - want).abs() <= tol).all()), (top, sign, h)
