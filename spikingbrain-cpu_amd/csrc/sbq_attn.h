@@ -29,8 +29,9 @@
 // row tile, so that a cache that is filled only at its front still keeps
 // every workgroup busy; a block that no row sees is left out after a look at
 // its positions.  A decode step of 32 heads over 2048 slots of 8 x 128 fp32
-// takes 9 us and 4.4 for the joining (the latency of a few loads after each
-// other; 3.3 us for the bytes), over 65536 bf16 48 us, 5.6 TB/s.
+// takes 10 us and 4.3 for the joining (kernel trace; the latency of a few loads
+// after each other; 3.3 us for the bytes), over 65536 bf16 47 us with the
+// joining (replayed graph), 5.7 TB/s.
 #pragma once
 
 #include "sbq_common.h"
@@ -574,7 +575,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, DP == 256 ? (RT == 2 ? 1 : 2) : RT
 // v % 4, which 16 at a time are the operand of V^T's product in that slot
 // order.  What bounds it: per 64 scores 32 cycles of products and some 30 of
 // exponentials and sums per SIMD, two waves of which overlap.  64 tokens of 32
-// heads over 65000 slots of 8 x 128 bf16: 116 us, 590 TFLOP/s.
+// heads over 65000 slots of 8 x 128 bf16: 115 us with the joining (replayed
+// graph), 590 TFLOP/s.
 template <int CT, int DP>
 __global__ __launch_bounds__(kTileWaves * 64, 2) void attn_tile_kernel(AttnArgs a) {
   typedef typename XElem<CT>::T T;
@@ -1059,9 +1061,13 @@ __global__ __launch_bounds__(kWeightWaves * 64) void attn_weight_kernel(AttnArgs
 // their way), the workgroup's 8 waves share every 64 rows of Q through LDS, so
 // that Q is read once per 256 slots, and work on the two halves of the rows
 // side by side.  It pays from 256 rows of a key head and enough slots to fill
-// many CUs 256 at a time: 64 tokens of 32 heads over 40000 slots of 8 x 128
-// bf16 62 us against 89 us for attn_weight_kernel, over 32768 62 / 73, over
-// 24576 62 / 56, over 8192 60 / 23; 128 tokens over 24576 102 / 100.
+// many CUs 256 at a time: 64 tokens of 32 heads over 65000 slots of 8 x 128
+// bf16 71 us against 143 us for attn_weight_kernel, over 40000 63 / 89, over
+// 32768 63 / 73, over 24576 62 / 56, over 8192 61 / 23; 128 tokens over 24576
+// 105 / 100 (replayed graphs, a call with weights less one without; other
+// numbers of key heads are not measured).  The workgroups whose slots not every
+// row sees look at positions per row and take longest: a chunk of 64 tokens
+// whose own slots are the last of 32768 takes 108 us / 81, of 65000 119 / 151.
 template <int CT, int DP>
 __global__ __launch_bounds__(kWeightWaves * 64, 2) void attn_weight_tile_kernel(AttnArgs a, float* weight) {
   typedef typename XElem<CT>::T T;

@@ -158,7 +158,7 @@ constexpr int kAttnGroups = 512;    // workgroups aimed at
 // and rows times slots from which it is taken.  8 key heads of 128 bf16
 // columns, 256 rows each: 65536 slots 122 us against attn_kernel's 185, 32768
 // 74 / 93, 8192 44 / 37; 512 rows: 8192 slots 49 / 58; 128 rows: 65536 slots
-// (with 4 waves) 120 / 106.
+// (with 4 waves) 120 / 106.  Other numbers of key heads are not measured.
 constexpr int kTileGroups = 256;
 constexpr int64_t kTileRows = 256, kTileScores = 1 << 22;
 

@@ -4,10 +4,11 @@
 //   q in -8..7, G = groups of 32, 64 or 128 columns, s in bf16.
 //
 // What bounds it: at one row the conversions of the weights (some 140 vector
-// instructions a tile and wave; 151936 x 2560: fp16 53 us, fp32 74 us, 39 us
+// instructions a tile and wave; 151936 x 2560: fp16 54 us, fp32 73 us, 39 us
 // for the bytes at a large copy's rate); at many rows reading x, once per
-// workgroup (64 rows over 12288 x 4096: fp16 17 us, bf16 19, fp32 33), and at
-// fp32 splitting it.  A packed tile is 16 rows x
+// workgroup (64 rows over 12288 x 4096, groups of 128: bf16 17 us, fp32 32;
+// of 64: 18 and 43), and at fp32 splitting it.  (Times of replayed graphs, four
+// weights in turn.)  A packed tile is 16 rows x
 // 128 columns in 1 KiB, one 16-byte load per lane, in the order of the MFMA A
 // operand: lane = g*16 + r holds row r, dword s the columns 32 s + 8 g + 0..7
 // of the tile, so that each group of 32 columns is one 16x16x32 MFMA step and
