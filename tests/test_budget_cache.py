@@ -8,7 +8,7 @@ import torch
 
 from conftest import announce
 from sbq import _lib, quant
-from sbq.state import DeviceBudgetKVBuffer, DeviceKVBuffer, new_device_state, tree_attention
+from sbq.state import DeviceBudgetKVBuffer, DeviceKVBuffer, new_device_state
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -556,5 +556,7 @@ def test_tokens_taken_back(dev):
         keep[held] = torch.tensor(held, device=dev)
         # each side: weights to e = 2^-24 ((D + 2) sum |scale q k| + 66), outputs to 2 e max |v|
         e = 2.0 ** -24 * ((D + 2) * float(q.abs().sum(-1).max() * line.k.abs().max()) * D ** -0.5 + 66)
-        other = tree_attention(q, line.k, line.v, keep, q_pos)
+        line.slot_pos, was = keep, line.slot_pos
+        other = line.attend(q, q_pos)
+        line.slot_pos = was
         assert torch.allclose(o, other, rtol=0, atol=4 * e * float(line.v.abs().max()))
