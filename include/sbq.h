@@ -38,8 +38,12 @@
  *                                top-k, top-p and the draw) over the lm_head logits
  *   sbq_tree_attention        <- spikingbrain_cpu/model.py:208-229 attention over the cached
  *                                keys (and over a tree of drafted tokens)
+ *   sbq_qk_norm_rope          <- spikingbrain_cpu/model.py:260-270 (the head norms) and
+ *                                model.py:46-51 (the rotation), before the attention
  * Additions without a counterpart: the 4-bit linears (sbq_linear_w4), the bounded
- * cache (sbq_kv_append, sbq_kv_take).
+ * cache (sbq_kv_append, sbq_kv_take), the paged cache of several sequences
+ * (sbq_paged_append, sbq_paged_read, sbq_paged_attention), the choice among
+ * drafted tokens (sbq_verify_drafts).
  */
 #ifndef SBQ_H_
 #define SBQ_H_
@@ -551,6 +555,125 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
                 int64_t k_sh, int64_t capacity, int64_t recent, int64_t* to_pos, float* to_weight,
                 int64_t* to_end, void* to_k, void* to_v, int64_t t_ss, int64_t t_sh, void* workspace,
                 size_t workspace_bytes, void* stream);
+
+/* ---- head norms and rotation to the positions --------------------------- */
+
+/* model.py:260-270: the RMS norm of each head's queries and keys and their
+ * rotation, in one pass.  For every vector x of D columns:
+ *   y = x / sqrt(mean(x^2) + eps) * w          (w NULL: y = x)
+ *   (y[a], y[b]) <- (y[a] cos - y[b] sin, y[b] cos + y[a] sin) for each pair
+ *     i < pairs, at the angle position * inv_freq[i]: a = i, b = i + pairs, or
+ *     with `interleaved` a = 2i, b = 2i + 1; columns from 2 * pairs on stay.
+ * The angle is exact (a 64-bit product, reduced in 64 bits), everything else
+ * fp32, rounded once to the output's type.
+ * q: device [tokens, heads, D], k: device [tokens, kv_heads, D] (kv_heads 0:
+ * none) of one type, strides in elements, unit stride in D <= 256.
+ * positions: device int64; token t stands at positions[t / per] + t % per.
+ * inv_freq: device fp32 [pairs].  q_weight, k_weight: device [D] of
+ * weight_dtype, or NULL.  q_out, k_out: device, of q's type, the input itself
+ * (with its strides) or apart from both inputs. */
+int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, int64_t heads,
+                     int64_t kv_heads, int64_t D, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                     const int64_t* positions, int64_t per, const float* inv_freq, int64_t pairs,
+                     int interleaved, const void* q_weight, const void* k_weight, int weight_dtype,
+                     float eps, void* q_out, void* k_out, int64_t qo_st, int64_t qo_sh, int64_t ko_st,
+                     int64_t ko_sh, void* stream);
+
+/* ---- a paged cache of several sequences ---------------------------------- */
+
+/* Cache types beside SBQ_F32, SBQ_F16 and SBQ_BF16: 8-bit codes with a scale. */
+#define SBQ_I8 3
+#define SBQ_E4M3 4
+/* Most query tokens of a sequence in one sbq_paged_attention call. */
+#define SBQ_PAGED_MAX_T 1024
+
+/* A pool of pages that the sequences' positions are spread over.  No
+ * counterpart in the reference, whose engine holds one sequence.
+ * k, v: device [pages][kv_heads][page][row], row = D rounded up to a multiple
+ * of 16, columns from D on zero; page a power of two from 16 to 1024.
+ * k_scale, v_scale: device fp32 [pages][kv_heads][page] for SBQ_I8 and
+ * SBQ_E4M3 (else not looked at): a vector is its codes times its scale.
+ * table: device int32 [sequences][max_pages]: position p of sequence b stands
+ * in page table[b][p / page], row p % page; an entry outside 0 .. pages - 1
+ * is no page: what stands there is neither written nor seen.  Pages that two
+ * sequences write to must differ.  length: device int64 [sequences]: positions
+ * held.  max_pages * page <= 2^30, sequences <= 65536.  k, v and the scales
+ * are 16-byte aligned.
+ *
+ * sbq_paged_append: T new tokens of each sequence (k_new, v_new: device
+ * [sequences, T, kv_heads, D], both with strides n_sb, n_st, n_sh, F32, F16 or
+ * BF16), of which the first counts[b] (NULL: all; device int64, limited to 0 ..
+ * T) are there, go to the positions start[b] on (device int64; may be `length`
+ * itself, not a part of it elsewhere); length[b] = start[b] + counts[b], at
+ * most max_pages * page (a token past that is dropped).  8-bit caches:
+ *   scale = max |x| / 127 (I8) or / 448 (E4M3), code = the nearest to x / scale
+ * (fp32 IEEE divisions, half to even; a scale of 0: codes 0).  A vector with
+ * an infinity or NaN reads back as NaN (scale NaN, codes 0).
+ *
+ * sbq_paged_read: positions start[b] .. start[b] + count - 1 of each sequence,
+ * to k_out, v_out (device [sequences, count, kv_heads, D], strides o_sb, o_st,
+ * o_sh, rounded to out_dtype); positions that it does not hold are 0. */
+int sbq_paged_append(void* k, void* v, float* k_scale, float* v_scale, int cache_dtype, int64_t pages,
+                     int64_t page, int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences,
+                     int64_t max_pages, int64_t* length, const int64_t* start, const int64_t* counts,
+                     const void* k_new, const void* v_new, int new_dtype, int64_t T, int64_t n_sb,
+                     int64_t n_st, int64_t n_sh, void* stream);
+int sbq_paged_read(const void* k, const void* v, const float* k_scale, const float* v_scale,
+                   int cache_dtype, int64_t pages, int64_t page, int64_t kv_heads, int64_t D,
+                   const int32_t* table, int64_t sequences, int64_t max_pages, const int64_t* length,
+                   const int64_t* start, int64_t count, void* k_out, void* v_out, int out_dtype,
+                   int64_t o_sb, int64_t o_st, int64_t o_sh, void* stream);
+
+/* The attention of T tokens of each sequence over its pages:
+ *   out[b,t,h] = sum_p softmax_p(scale * q[b,t,h] . k[b,p]) v[b,p], key head
+ *   h / (heads / kv_heads),
+ * over the positions p < length[b] that token t sees: p <= start[b] + t, and
+ * with a window (> 0) p > start[b] + t - window.  start NULL: length[b] -
+ * counts[b], the tokens appended last.  Tokens from counts[b] (NULL: T) on
+ * see nothing.  A row that sees nothing (or only scores of -infinity) is 0.
+ * What a row does not see does not reach it, infinities and NaN included.
+ * q: device [sequences, T, heads, D], T <= SBQ_PAGED_MAX_T, F32, or the
+ * cache's type (8-bit caches: any); out: the same shape and type, apart from
+ * every input.  Scores, maxima and sums are fp32; fp32 queries are multiplied
+ * to 22 significant bits or more, and so are their weights; with 2-byte
+ * queries the weights keep 11 bits (bf16 caches: 16).  scale * q . k is to
+ * stay below 2^27 in magnitude.
+ * workspace: >= sbq_paged_attn_workspace_bytes bytes, any content; one call at
+ * a time.  The result does not depend on timing, nor on other sequences'
+ * lengths. */
+int64_t sbq_paged_attn_workspace_bytes(int64_t sequences, int64_t T, int64_t heads, int64_t kv_heads,
+                                       int64_t D, int64_t page, int64_t max_pages, int cache_dtype);
+int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t q_sb, int64_t q_st,
+                        int64_t q_sh, const void* k, const void* v, const float* k_scale,
+                        const float* v_scale, int cache_dtype, int64_t pages, int64_t page,
+                        int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences,
+                        int64_t max_pages, const int64_t* length, const int64_t* start,
+                        const int64_t* counts, int64_t window, float scale, void* out, int64_t o_sb,
+                        int64_t o_st, int64_t o_sh, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* ---- drafted tokens against the target's probabilities ------------------- */
+
+/* B sequences with T drafted tokens each (counts[b] of them where counts,
+ * device int64 [B], is given; limited to 0 .. T).  p: the target's
+ * probabilities, device [B, T + 1, V] (row t: after the drafts before t), q:
+ * those that the drafts were drawn from, device [B, T, V], or NULL (each draft
+ * was certain); strides p_sb, p_st, q_sb, q_st in elements, unit stride in V
+ * <= 2^23, both F32, F16 or BF16, none negative; a row need not sum to 1.
+ * tokens: device int64 [B, T].  u: device fp32 [B, T + 1] uniforms in [0, 1).
+ *   kept[b]: the drafts before the first t with not u[b,t] q[x] < p[x];
+ *   token[b]: the first index (vocabulary order) whose prefix of mass exceeds
+ *     u[b,T] * (whole mass), the mass being max(p - q, 0) of the refused
+ *     draft's rows (p's own where nothing is left), or p's row counts[b].
+ * Products and sums are 64-bit.  A draft outside 0 .. V - 1 is refused.  token
+ * is -1 where the whole mass is 0, infinite or NaN.  B, T <= 65535.
+ * kept, token: device int64 [B].  workspace: >= sbq_verify_workspace_bytes
+ * bytes, any content; one call at a time. */
+int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V);
+int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st,
+                      int dtype, int64_t B, int64_t T, int64_t V, const int64_t* tokens, const float* u,
+                      const int64_t* counts, int64_t* kept, int64_t* token, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

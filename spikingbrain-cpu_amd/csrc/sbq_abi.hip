@@ -777,4 +777,173 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
   return sbq::launch_kv_take(c, (hipStream_t)stream);
 }
 
+// ---- head norms and rotation ----
+
+int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t D,
+                     int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, const int64_t* positions, int64_t per,
+                     const float* inv_freq, int64_t pairs, int interleaved, const void* q_weight, const void* k_weight,
+                     int weight_dtype, float eps, void* q_out, void* k_out, int64_t qo_st, int64_t qo_sh, int64_t ko_st,
+                     int64_t ko_sh, void* stream) {
+  if (!valid_dtype(dtype) || !valid_dtype(weight_dtype)) return SBQ_ERR_DTYPE;
+  if (tokens < 0 || tokens > kIntMax || heads < 1 || heads > 65536 || kv_heads < 0 || kv_heads > 65536 || D < 1 || D > 256 ||
+      per < 1 || pairs < 0 || 2 * pairs > D || !(eps >= 0.0f))
+    return SBQ_ERR_ARG;
+  if (q_st < 0 || q_sh < 0 || k_st < 0 || k_sh < 0) return SBQ_ERR_ARG;
+  if (tokens == 0) return SBQ_OK;
+  if (!q || !q_out || !positions || (pairs > 0 && !inv_freq) || (kv_heads > 0 && (!k || !k_out))) return SBQ_ERR_ARG;
+  if (!apart(tokens, heads, D, qo_st, qo_sh) || (kv_heads > 0 && !apart(tokens, kv_heads, D, ko_st, ko_sh))) return SBQ_ERR_ARG;
+  const int64_t es = esize(dtype), ew = esize(weight_dtype);
+  if (!aligned(q, es) || !aligned(k, es) || !aligned(q_out, es) || !aligned(k_out, es) || !aligned(positions, 8) ||
+      !aligned(inv_freq, 4) || !aligned(q_weight, ew) || !aligned(k_weight, ew))
+    return SBQ_ERR_ALIGN;
+  sbq::RopeArgs a{};
+  a.q = q, a.k = k, a.positions = positions, a.inv_freq = inv_freq, a.q_weight = q_weight, a.k_weight = k_weight;
+  a.q_out = q_out, a.k_out = k_out, a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.qo_st = qo_st;
+  a.qo_sh = qo_sh, a.ko_st = ko_st, a.ko_sh = ko_sh, a.T = tokens, a.per = per, a.heads = (int)heads;
+  a.kv_heads = (int)kv_heads, a.D = (int)D, a.pairs = (int)pairs, a.wt = weight_dtype, a.eps = eps;
+  return sbq::launch_rope(a, interleaved != 0, dtype, (hipStream_t)stream);
+}
+
+// ---- a paged cache of several sequences ----
+
+static bool valid_cache_dtype(int t) { return valid_dtype(t) || t == SBQ_I8 || t == SBQ_E4M3; }
+
+static int check_paged(const void* k, const void* v, const float* k_scale, const float* v_scale, int cache_dtype,
+                       int64_t pages, int64_t page, int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences,
+                       int64_t max_pages, const int64_t* length, sbq::PagedCache* c) {
+  if (!valid_cache_dtype(cache_dtype)) return SBQ_ERR_DTYPE;
+  if (D < 1 || D > 256 || kv_heads < 1 || kv_heads > 65536 || pages < 1 || pages > (1 << 30) || page < 16 || page > 1024 ||
+      (page & (page - 1)) || sequences < 0 || sequences > 65536 || max_pages < 1 || max_pages > (1 << 30) / page)
+    return SBQ_ERR_ARG;
+  if (sequences == 0) return SBQ_OK;
+  const bool b8 = cache_dtype == SBQ_I8 || cache_dtype == SBQ_E4M3;
+  if (!k || !v || !table || !length || (b8 && (!k_scale || !v_scale))) return SBQ_ERR_ARG;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_scale, 16) || !aligned(v_scale, 16) || !aligned(table, 4) ||
+      !aligned(length, 8))
+    return SBQ_ERR_ALIGN;
+  c->k = const_cast<void*>(k), c->v = const_cast<void*>(v), c->k_scale = const_cast<float*>(k_scale);
+  c->v_scale = const_cast<float*>(v_scale), c->table = table, c->length = const_cast<int64_t*>(length), c->pages = pages;
+  c->B = sequences, c->page_log = __builtin_ctzll(page), c->Hk = (int)kv_heads, c->D = (int)D;
+  c->row = (int)((D + 15) / 16 * 16), c->max_pages = (int)max_pages;
+  return SBQ_OK;
+}
+
+// Does [p, p + n) of int64 meet [q, q + n) elsewhere than on the same elements?
+static bool shifted(const int64_t* p, const int64_t* q, int64_t n) { return p != q && p < q + n && q < p + n; }
+
+int sbq_paged_append(void* k, void* v, float* k_scale, float* v_scale, int cache_dtype, int64_t pages, int64_t page,
+                     int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences, int64_t max_pages, int64_t* length,
+                     const int64_t* start, const int64_t* counts, const void* k_new, const void* v_new, int new_dtype, int64_t T,
+                     int64_t n_sb, int64_t n_st, int64_t n_sh, void* stream) {
+  if (!valid_dtype(new_dtype)) return SBQ_ERR_DTYPE;
+  sbq::PagedStore s{};
+  const int rc = check_paged(k, v, k_scale, v_scale, cache_dtype, pages, page, kv_heads, D, table, sequences, max_pages,
+                             length, &s.c);
+  if (rc) return rc;
+  if (T < 0 || T > (1 << 30) || n_sb < 0 || n_st < 0 || n_sh < 0) return SBQ_ERR_ARG;
+  if (sequences == 0) return SBQ_OK;
+  if (!start || (T > 0 && (!k_new || !v_new)) || shifted(start, length, sequences)) return SBQ_ERR_ARG;
+  if (counts && (counts == length || shifted(counts, length, sequences))) return SBQ_ERR_ARG;
+  const int64_t es = esize(new_dtype);
+  if (!aligned(start, 8) || !aligned(counts, 8) || !aligned(k_new, es) || !aligned(v_new, es)) return SBQ_ERR_ALIGN;
+  s.start = start, s.counts = counts, s.kn = k_new, s.vn = v_new, s.T = T, s.n_sb = n_sb, s.n_st = n_st, s.n_sh = n_sh;
+  s.ct = cache_dtype, s.xt = new_dtype;
+  return sbq::launch_paged_append(s, (hipStream_t)stream);
+}
+
+int sbq_paged_read(const void* k, const void* v, const float* k_scale, const float* v_scale, int cache_dtype, int64_t pages,
+                   int64_t page, int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences, int64_t max_pages,
+                   const int64_t* length, const int64_t* start, int64_t count, void* k_out, void* v_out, int out_dtype,
+                   int64_t o_sb, int64_t o_st, int64_t o_sh, void* stream) {
+  if (!valid_dtype(out_dtype)) return SBQ_ERR_DTYPE;
+  sbq::PagedStore s{};
+  const int rc = check_paged(k, v, k_scale, v_scale, cache_dtype, pages, page, kv_heads, D, table, sequences, max_pages,
+                             length, &s.c);
+  if (rc) return rc;
+  if (count < 0 || count > (1 << 30)) return SBQ_ERR_ARG;
+  if (sequences == 0 || count == 0) return SBQ_OK;
+  if (!start || !k_out || !v_out) return SBQ_ERR_ARG;
+  // (a sequence's [count, kv_heads, D] lies apart from the next one's)
+  if (!apart(count, kv_heads, D, o_st, o_sh) ||
+      (sequences > 1 && (__int128)o_sb < (__int128)(count - 1) * o_st + (__int128)(kv_heads - 1) * o_sh + D))
+    return SBQ_ERR_ARG;
+  const int64_t es = esize(out_dtype);
+  if (!aligned(start, 8) || !aligned(k_out, es) || !aligned(v_out, es)) return SBQ_ERR_ALIGN;
+  s.start = start, s.k_out = k_out, s.v_out = v_out, s.T = count, s.n_sb = o_sb, s.n_st = o_st, s.n_sh = o_sh;
+  s.ct = cache_dtype, s.xt = out_dtype;
+  return sbq::launch_paged_read(s, (hipStream_t)stream);
+}
+
+static bool paged_rows_ok(int64_t T, int64_t heads, int64_t kv_heads) {
+  return T >= 0 && T <= SBQ_PAGED_MAX_T && heads >= 1 && heads <= 65536 && kv_heads >= 1 && heads % kv_heads == 0;
+}
+
+int64_t sbq_paged_attn_workspace_bytes(int64_t sequences, int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
+                                       int64_t max_pages, int cache_dtype) {
+  if (!valid_cache_dtype(cache_dtype) || !paged_rows_ok(T, heads, kv_heads) || T == 0 || sequences < 1 || sequences > 65536 ||
+      D < 1 || D > 256 || page < 16 || page > 1024 || (page & (page - 1)) || max_pages < 1 || max_pages > (1 << 30) / page)
+    return 0;
+  return sbq::paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page * max_pages, cache_dtype) + 256;
+}
+
+int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                        const void* k, const void* v, const float* k_scale, const float* v_scale, int cache_dtype,
+                        int64_t pages, int64_t page, int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences,
+                        int64_t max_pages, const int64_t* length, const int64_t* start, const int64_t* counts, int64_t window,
+                        float scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(q_dtype) || !valid_cache_dtype(cache_dtype)) return SBQ_ERR_DTYPE;
+  if (valid_dtype(cache_dtype) && q_dtype != SBQ_F32 && q_dtype != cache_dtype) return SBQ_ERR_DTYPE;
+  sbq::PagedCall c{};
+  const int rc = check_paged(k, v, k_scale, v_scale, cache_dtype, pages, page, kv_heads, D, table, sequences, max_pages,
+                             length, &c.c);
+  if (rc) return rc;
+  if (!paged_rows_ok(T, heads, kv_heads) || window < 0 || scale != scale) return SBQ_ERR_ARG;
+  if (sequences == 0 || T == 0) return SBQ_OK;
+  if (!q || !out || q_sb < 0 || q_st < 0 || q_sh < 0) return SBQ_ERR_ARG;
+  if (!apart(T, heads, D, o_st, o_sh) ||
+      (sequences > 1 && (__int128)o_sb < (__int128)(T - 1) * o_st + (__int128)(heads - 1) * o_sh + D))
+    return SBQ_ERR_ARG;
+  const int64_t es = esize(q_dtype);
+  if (!aligned(q, es) || !aligned(out, es) || !aligned(start, 8) || !aligned(counts, 8)) return SBQ_ERR_ALIGN;
+  if (!workspace ||
+      (int64_t)workspace_bytes < sbq_paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page, max_pages, cache_dtype))
+    return SBQ_ERR_WORKSPACE;
+  c.q = q, c.start = start, c.counts = counts, c.out = out, c.ws = (void*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  c.T = T, c.heads = heads, c.window = window < (int64_t)1 << 62 ? window : (int64_t)1 << 62;
+  c.q_sb = q_sb, c.q_st = q_st, c.q_sh = q_sh, c.o_sb = o_sb, c.o_st = o_st, c.o_sh = o_sh;
+  c.qt = q_dtype, c.ct = cache_dtype, c.scale = scale;
+  return sbq::launch_paged_attention(c, (hipStream_t)stream);
+}
+
+// ---- drafted tokens against the target's probabilities ----
+
+static bool verify_sizes_ok(int64_t B, int64_t T, int64_t V) {
+  return B >= 0 && B <= 65535 && T >= 0 && T <= 65535 && V >= 1 && V <= ((int64_t)1 << 23);
+}
+
+int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V) {
+  if (!verify_sizes_ok(B, 0, V) || B == 0) return 0;
+  return sbq::verify_workspace_bytes(B, V) + 16;  // + alignment slack
+}
+
+int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st, int dtype,
+                      int64_t B, int64_t T, int64_t V, const int64_t* tokens, const float* u, const int64_t* counts,
+                      int64_t* kept, int64_t* token, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype)) return SBQ_ERR_DTYPE;
+  if (!verify_sizes_ok(B, T, V) || p_sb < 0 || p_st < 0 || q_sb < 0 || q_st < 0) return SBQ_ERR_ARG;
+  if (B == 0) return SBQ_OK;
+  if (!p || !u || !kept || !token || (T > 0 && !tokens)) return SBQ_ERR_ARG;
+  const int64_t es = esize(dtype);
+  if (!aligned(p, es) || !aligned(q, es) || !aligned(tokens, 8) || !aligned(u, 4) || !aligned(counts, 8) || !aligned(kept, 8) ||
+      !aligned(token, 8))
+    return SBQ_ERR_ALIGN;
+  if (!workspace || (int64_t)workspace_bytes < sbq_verify_workspace_bytes(B, V)) return SBQ_ERR_WORKSPACE;
+  sbq::VerifyArgs a{};
+  a.p = p, a.q = q, a.tokens = tokens, a.counts = counts, a.u = u, a.kept = kept, a.token = token;
+  a.part = (double2*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15), a.B = B, a.T = T, a.V = V, a.p_sb = p_sb, a.p_st = p_st;
+  a.q_sb = q_sb, a.q_st = q_st;
+  return sbq::launch_verify(a, dtype, (hipStream_t)stream);
+}
+
 }  // extern "C"

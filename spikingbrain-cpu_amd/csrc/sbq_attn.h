@@ -131,10 +131,6 @@ __device__ __forceinline__ float reference(float mx) {
   return mx;
 }
 
-__device__ __forceinline__ float load_q(const void* q, int qt, int64_t i) {
-  return qt == XT_F32 ? ((const float*)q)[i] : qt == XT_F16 ? (float)((const _Float16*)q)[i] : (float)((const __bf16*)q)[i];
-}
-
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.4028235e38f; }
 
 // Which of N slots token `tok` sees, one bit each; slot(v) is the v-th one's
@@ -240,7 +236,7 @@ struct QRow {
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const float x = d + j < a.D ? load_q(a.q, a.qt, at + d + j) : 0.0f;
+          const float x = d + j < a.D ? load_elem(a.q, a.qt, at + d + j) : 0.0f;
           f[ch][j] = a.neg ? -x : x;
         }
       }

@@ -120,6 +120,11 @@ struct XElem<XT_BF16> {
   static __device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
 };
 
+// Element i of an array whose type is known at run time.
+__device__ __forceinline__ float load_elem(const void* x, int xt, int64_t i) {
+  return xt == XT_F32 ? ((const float*)x)[i] : xt == XT_F16 ? (float)((const _Float16*)x)[i] : (float)((const __bf16*)x)[i];
+}
+
 // 8 consecutive activations x[m][k0..k0+7] widened to fp32.  `vec` = the row
 // is 16-byte aligned at k0 and all 8 columns are < K; otherwise each element is
 // loaded alone and columns >= K read as zero.  Rows >= M read as zero.

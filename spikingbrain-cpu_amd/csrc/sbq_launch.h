@@ -281,4 +281,72 @@ struct KvTake {
 };
 int launch_kv_take(const KvTake& c, hipStream_t st);
 
+// Head norms and rotation (sbq_rope.hip); strides in elements.  wt: the
+// weights' type.  rows .. first are the launcher's.
+struct RopeArgs {
+  const void *q, *k;
+  const int64_t* positions;  // token t stands at positions[t / per] + t % per
+  const float* inv_freq;
+  const void *q_weight, *k_weight;
+  void *q_out, *k_out;
+  int64_t q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, T, per;
+  int heads, kv_heads, D, pairs, wt;
+  float eps;
+  int rows, lanes, tokens, parts;  // vectors of a token, lanes of a vector, tokens and shares of their vectors a workgroup
+  int64_t first;                   // the launch's first token
+};
+int launch_rope(const RopeArgs& c, bool inter, int xt, hipStream_t st);
+
+// Drafted tokens against the target's probabilities (sbq_verify.hip); part:
+// verify_workspace_bytes(B, V), 16-byte aligned.
+struct VerifyArgs {
+  const void *p, *q;  // [B][T + 1][V], [B][T][V] or null (one-hot at the token)
+  const int64_t *tokens, *counts;
+  const float* u;
+  int64_t *kept, *token;
+  double2* part;  // [B][segs]: mass left after the refused draft, the target's own
+  int64_t B, T, V, p_sb, p_st, q_sb, q_st;
+  int64_t first;  // the launch's first sequence, and segments of a row: the launcher's
+  int segs;
+};
+// The paged cache (sbq_paged.h).
+struct PagedCache {
+  void *k, *v;               // [pages][Hk][1 << page_log][row]
+  float *k_scale, *v_scale;  // [pages][Hk][1 << page_log], 8-bit pools
+  const int32_t* table;      // [B][max_pages]
+  int64_t* length;           // [B]
+  int64_t pages, B;
+  int page_log, Hk, D, row, max_pages;
+};
+// New keys and values into it, or out of it (sbq_paged.hip); strides in
+// elements, kn and vn (k_out and v_out) share theirs.
+struct PagedStore {
+  PagedCache c;
+  const int64_t *start, *counts;
+  const void *kn, *vn;
+  void *k_out, *v_out;
+  int64_t T, n_sb, n_st, n_sh;
+  int ct, xt;
+  int lanes, parts;  // lanes of a vector, workgroups of a sequence, and what follows: the launcher's
+  bool vec, set_length;
+};
+int launch_paged_append(const PagedStore& c, hipStream_t st);
+int launch_paged_read(const PagedStore& c, hipStream_t st);
+// The new tokens' attention over it; ws: paged_attn_workspace_bytes, 256-byte
+// aligned.  room: positions that a sequence's row of the table names.
+struct PagedCall {
+  PagedCache c;
+  const void* q;
+  const int64_t *start, *counts;
+  void *out, *ws;
+  int64_t T, heads, window, q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  int qt, ct;
+  float scale;
+};
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct);
+int launch_paged_attention(const PagedCall& c, hipStream_t st);
+
+int64_t verify_workspace_bytes(int64_t B, int64_t V);
+int launch_verify(const VerifyArgs& c, int xt, hipStream_t st);
+
 }  // namespace sbq

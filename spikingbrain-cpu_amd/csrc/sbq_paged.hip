@@ -1,0 +1,401 @@
+// sbq_paged.hip - the paged cache's writing and reading back (sbq_paged.h
+// describes the pool).
+//
+// An 8-bit pool keeps of each token's keys (values) of a head the scale
+// max |x| / 127 (int8) or / 448 (e4m3), in fp32, and the nearest codes of x /
+// scale (IEEE division, half to even): half a step of 1/127 of the largest
+// value, or 2^-4 of each.  Each vector is read once and written once; a lane
+// takes 8 columns, so that a vector of 128 lies in 16 lanes and its maximum
+// crosses those alone.  A prompt is bound by its bytes, a step's few rows by
+// the loads one after another: start, table, row.
+#include "sbq_paged.h"
+
+#include <algorithm>
+
+namespace sbq {
+
+namespace {
+
+constexpr int kStoreThreads = 256;
+constexpr int kStoreAlone = 256;  // vectors of a sequence that one workgroup stores by itself
+
+// Largest code of an 8-bit type.
+template <int CT>
+__device__ __forceinline__ float largest() {
+  return CT == CT_I8 ? 127.0f : 448.0f;
+}
+
+template <int XT, bool VEC>
+__device__ __forceinline__ void load_cols(const typename XElem<XT>::T* p, int n, float (&x)[8]) {
+  if constexpr (VEC) {
+    if (n > 0) {
+      load8_f32_vec<XT>(p, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+  }
+}
+
+// Eight codes of x / scale (scale 0 or NaN: zeros), the first in the low byte.
+template <int CT>
+__device__ __forceinline__ u32x2 codes(const float (&x)[8], float scale) {
+  const bool any = scale > 0.0f;
+  u32x2 w = {0u, 0u};
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float q = any ? x[j] / scale : 0.0f;
+    y[j] = __builtin_fminf(__builtin_fmaxf(q, -largest<CT>()), largest<CT>());  // (a subnormal scale's own rounding)
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (CT == CT_I8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[h] |= (uint32_t)((int)__builtin_rintf(y[4 * h + j]) & 255) << (8 * j);
+    } else {
+      int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], v, true);
+    }
+  }
+  return w;
+}
+
+// One vector's columns to the pool; the lanes of a vector are neighbours, a
+// power of two of them.
+template <int CT>
+__device__ __forceinline__ void store_cols(const PagedCache& c, bool value, int64_t at, int d, int n, const float (&x)[8],
+                                           int lanes) {
+  void* const pool = value ? c.v : c.k;
+  if constexpr (is_8bit(CT)) {
+    float most = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      most = __builtin_fmaxf(most, __builtin_fabsf(x[j]));
+      odd |= !finite(x[j]);
+    }
+    if (odd) most = __builtin_inff();
+    for (int o = 1; o < lanes; o <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o, 64));
+    // (a vector with an infinity or NaN has no codes: it reads back as NaN)
+    const float scale = finite(most) ? most / largest<CT>() : __builtin_nanf("");
+    if (n <= 0) return;
+    *(u32x2*)((uint8_t*)pool + at * c.row + d) = codes<CT>(x, scale);  // (columns past D: zeros again)
+    if (d == 0) (value ? c.v_scale : c.k_scale)[at] = scale;
+  } else {
+    if (n <= 0) return;
+    store_y4(pool, CT, at * c.row + d, (f32x4){x[0], x[1], x[2], x[3]}, true, 4);
+    store_y4(pool, CT, at * c.row + d + 4, (f32x4){x[4], x[5], x[6], x[7]}, true, 4);
+  }
+}
+
+// The length after `count` tokens from `start` on.
+__device__ __forceinline__ int64_t paged_end(int64_t start, int64_t count, int64_t room) {
+  if (start < 0) return 0;
+  return start >= room ? room : start + count < room ? start + count : room;
+}
+
+// Rows [b][t][head][k or v], a group of `lanes` lanes each.  ALONE: one
+// workgroup a sequence, which moves the length itself after reading it.
+template <int CT, int XT, bool VEC>
+__global__ __launch_bounds__(kStoreThreads) void paged_append_kernel(PagedStore a) {
+  typedef typename XElem<XT>::T T;
+  const PagedCache& c = a.c;
+  const int lane = threadIdx.x & (a.lanes - 1), groups = kStoreThreads / a.lanes, d = lane * 8;
+  const int64_t b = blockIdx.x / a.parts, each = a.T * c.Hk * 2;
+  const int part = blockIdx.x % a.parts, n = c.D - d;
+  const int64_t start = a.start[b], count = paged_count(a.counts, b, a.T);
+  const int64_t room = (int64_t)c.max_pages << c.page_log;
+  for (int64_t r = (int64_t)part * groups + threadIdx.x / a.lanes; r < each; r += (int64_t)groups * a.parts) {
+    const bool value = r & 1;
+    const int64_t th = r >> 1, t = th / c.Hk, h = th - t * c.Hk, pos = start + t;
+    // (the lanes of a vector go together; those past it keep up for the maximum)
+    if (t >= count || start < 0 || start >= room || pos >= room) continue;
+    const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
+    if (!valid_page(c, id)) continue;
+    float x[8];
+    load_cols<XT, VEC>((const T*)(value ? a.vn : a.kn) + b * a.n_sb + t * a.n_st + h * a.n_sh + d, n, x);
+    store_cols<CT>(c, value, (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1)), d, n, x, a.lanes);
+  }
+  if (a.set_length && part == 0) {
+    __syncthreads();  // (start may be the length itself, then with one workgroup a sequence)
+    if (threadIdx.x == 0) {
+      c.length[b] = paged_end(start, count, room);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kStoreThreads) void paged_length_kernel(PagedStore a) {
+  const int64_t b = (int64_t)blockIdx.x * kStoreThreads + threadIdx.x;
+  if (b >= a.c.B) return;
+  const int64_t room = (int64_t)a.c.max_pages << a.c.page_log, start = a.start[b];
+  a.c.length[b] = paged_end(start, paged_count(a.counts, b, a.T), room);
+}
+
+template <int CT>
+__device__ __forceinline__ void read_cols(const PagedCache& c, bool value, int64_t at, int d, float (&x)[8]) {
+  const void* const pool = value ? c.v : c.k;
+  if constexpr (is_8bit(CT)) {
+    const u32x2 w = *(const u32x2*)((const uint8_t*)pool + at * c.row + d);
+    const float scale = (value ? c.v_scale : c.k_scale)[at];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (CT == CT_I8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * h + j] = (float)(int8_t)(w[h] >> (8 * j)) * scale;
+      } else {
+        x[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 0) * scale;
+        x[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 1) * scale;
+        x[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 2) * scale;
+        x[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 3) * scale;
+      }
+    }
+  } else {
+    load8_f32_vec<CT>((const typename XElem<CT>::T*)pool + at * c.row + d, x);
+  }
+}
+
+// Positions start .. start + T - 1 of each sequence, zeros for those it does not hold.
+template <int CT>
+__global__ __launch_bounds__(kStoreThreads) void paged_read_kernel(PagedStore a) {
+  const PagedCache& c = a.c;
+  const int lane = threadIdx.x & (a.lanes - 1), groups = kStoreThreads / a.lanes, d = lane * 8, n = c.D - d;
+  const int64_t b = blockIdx.x / a.parts, each = a.T * c.Hk * 2, part = blockIdx.x % a.parts;
+  const int64_t start = a.start[b], room = (int64_t)c.max_pages << c.page_log, held = c.length[b] < room ? c.length[b] : room;
+  if (n <= 0) return;
+  for (int64_t r = part * groups + threadIdx.x / a.lanes; r < each; r += (int64_t)groups * a.parts) {
+    const bool value = r & 1;
+    const int64_t th = r >> 1, t = th / c.Hk, h = th - t * c.Hk, pos = start + t;
+    float x[8] = {};
+    if (pos >= 0 && pos < held) {
+      const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
+      if (valid_page(c, id))
+        read_cols<CT>(c, value, (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1)), d, x);
+    }
+    void* const out = value ? a.v_out : a.k_out;
+    const int64_t to = b * a.n_sb + t * a.n_st + h * a.n_sh + d;
+    store_y4(out, a.xt, to, (f32x4){x[0], x[1], x[2], x[3]}, a.vec && n >= 4, n);
+    store_y4(out, a.xt, to + 4, (f32x4){x[4], x[5], x[6], x[7]}, a.vec && n >= 8, n - 4);
+  }
+}
+
+template <int CT, int XT>
+int launch_append_xt(const PagedStore& a, unsigned grid, hipStream_t st) {
+  if (a.vec)
+    paged_append_kernel<CT, XT, true><<<grid, kStoreThreads, 0, st>>>(a);
+  else
+    paged_append_kernel<CT, XT, false><<<grid, kStoreThreads, 0, st>>>(a);
+  return check_launch();
+}
+template <int CT>
+int launch_append_ct(const PagedStore& a, unsigned grid, hipStream_t st) {
+  return a.xt == XT_F32   ? launch_append_xt<CT, XT_F32>(a, grid, st)
+         : a.xt == XT_F16 ? launch_append_xt<CT, XT_F16>(a, grid, st)
+                          : launch_append_xt<CT, XT_BF16>(a, grid, st);
+}
+template <int CT>
+int launch_read_ct(const PagedStore& a, unsigned grid, hipStream_t st) {
+  paged_read_kernel<CT><<<grid, kStoreThreads, 0, st>>>(a);
+  return check_launch();
+}
+
+// Lanes of a vector, and how many workgroups share a sequence's vectors: each
+// wave a few, up to about 8 workgroups a CU.
+void plan(PagedStore& a) {
+  a.lanes = 1;
+  while (a.lanes * 8 < a.c.D) a.lanes <<= 1;
+  const int64_t groups = kStoreThreads / a.lanes, each = a.T * a.c.Hk * 2;
+  const int64_t want = (each + groups - 1) / groups, room = std::max<int64_t>(1, 4096 / a.c.B);
+  a.parts = (int)std::max<int64_t>(1, std::min(want, room));
+}
+
+// One row's splits joined: the maximum over their maxima, then the partial sums
+// scaled to it, independent loads eight at a time.  How many splits have
+// written theirs follows from the length, as in paged_attn_kernel.
+template <int DP>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
+  constexpr int ND = DP / 4, NG = 256 / ND, U = 8;
+  __shared__ __align__(16) f32x4 lds[NG][ND];
+  __shared__ float lds_l[NG];
+  const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
+  const int64_t at = a.first * a.c.Hk * R + blockIdx.x, b = at / ((int64_t)a.c.Hk * R);
+  const int r = (int)(at % R), kvh = (int)(at / R % a.c.Hk), t = r / a.rep, row0 = r & ~15;
+  const PagedSpan span(a, b);
+  int lo, hi;
+  span.all(a, row0 / a.rep, min(row0 + 15, R - 1) / a.rep, lo, hi);
+  const int blocks = hi >= lo ? hi / SB + 1 - lo / SB : 0;
+  const int used = max(1, min(a.splits, (blocks + kAttnWaves - 1) / kAttnWaves));
+  if (used == 1) return;  // (written by the one workgroup)
+  const float2* const ml = a.part_ml + at * a.splits;
+  float top = -__builtin_inff();
+  for (int s = lane; s < used; s += 64) top = __builtin_fmaxf(top, ml[s].x);
+  top = wave_max(top);
+  const float from = top == -__builtin_inff() ? 0.0f : top;
+  f32x4 sum = (f32x4)(0.0f);
+  float l = 0.0f;
+  for (int s0 = grp; s0 < used; s0 += U * NG) {
+    f32x4 x[U];
+    float2 y[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int s = min(s0 + k * NG, used - 1);
+      x[k] = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
+      y[k] = ml[s];
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float f = __builtin_amdgcn_exp2f(y[k].x - from);
+      if (s0 + k * NG < used && y[k].y != 0.0f) {  // (a split that saw nothing adds nothing)
+        sum += x[k] * f;
+        l += y[k].y * f;
+      }
+    }
+  }
+  lds[grp][threadIdx.x % ND] = sum;
+  if (d == 0) lds_l[grp] = l;
+  __syncthreads();
+  if (grp) return;
+  l = lds_l[0];
+#pragma unroll
+  for (int k = 1; k < NG; ++k) {
+    sum += lds[k][threadIdx.x];
+    l += lds_l[k];
+  }
+  span.of(a, t, lo, hi);
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  sum = hi >= lo ? sum * inv : (f32x4)(0.0f);
+  const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r % a.rep) * a.o_sh + d;
+  if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
+}
+
+constexpr int64_t kPagedGroups = 1024;  // workgroups aimed at
+
+struct PagedPlan {
+  int DP, SB, rtiles, splits;
+};
+// The split goes by the table's room: how much of it is filled is known on the
+// device alone, where workgroups that a shorter sequence has no blocks for
+// leave at once.
+PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, int ct) {
+  PagedPlan p;
+  p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  p.SB = ct == XT_F32 ? 16 : is_8bit(ct) ? 64 : 32;
+  p.rtiles = (int)((R + 15) / 16);
+  const int64_t base = B * Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB;
+  const int64_t most = (blocks + kAttnWaves - 1) / kAttnWaves;
+  p.splits = (int)std::max<int64_t>(1, std::min(most, (kPagedGroups + base - 1) / base));
+  return p;
+}
+
+int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct) {
+  const int64_t R = heads / Hk * T;
+  const PagedPlan p = paged_plan(B, R, Hk, D, room, ct);
+  if (p.splits == 1) return 0;
+  const int64_t parts = B * Hk * R * p.splits;
+  return round256(parts * p.DP * 4) + round256(parts * 8);
+}
+
+int launch_paged_attention(const PagedCall& c, hipStream_t st) {
+  const int64_t Hk = c.c.Hk, rep = c.heads / Hk, R = rep * c.T, B = c.c.B;
+  const PagedPlan p = paged_plan(B, R, Hk, c.c.D, (int64_t)c.c.max_pages << c.c.page_log, c.ct);
+  PagedArgs a{};
+  a.c = c.c, a.q = c.q, a.start = c.start, a.counts = c.counts, a.out = c.out;
+  a.q_sb = c.q_sb, a.q_st = c.q_st, a.q_sh = c.q_sh, a.o_sb = c.o_sb, a.o_st = c.o_st, a.o_sh = c.o_sh;
+  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.splits = p.splits, a.rtiles = p.rtiles, a.qt = c.qt;
+  a.scale = c.scale * 1.44269504f;
+  const int64_t eq = c.qt == XT_F32 ? 4 : 2;
+  auto vec = [&](const void* x, int64_t n, int64_t sb, int64_t ss, int64_t sh) {  // n elements at once, 16 bytes at most
+    const int64_t by = n * eq < 16 ? n * eq : 16;
+    return (uintptr_t)x % by == 0 && sb * eq % by == 0 && ss * eq % by == 0 && sh * eq % by == 0;
+  };
+  a.qvec = vec(c.q, 8, c.q_sb, c.q_st, c.q_sh);
+  a.ovec = vec(c.out, 4, c.o_sb, c.o_st, c.o_sh);
+  if (p.splits > 1) {
+    a.part_o = (float*)c.ws;
+    a.part_ml = (float2*)((uint8_t*)c.ws + round256(B * Hk * R * p.splits * p.DP * 4));
+  }
+  const int64_t each = Hk * p.rtiles * p.splits, rows = Hk * R;
+  const int64_t most = std::max<int64_t>(1, kLaunchThreads / 256 / std::max(each, rows));  // sequences of a launch
+  for (a.first = 0; a.first < B; a.first += most) {
+    const int64_t n = std::min(most, B - a.first);
+    const unsigned grid = (unsigned)(n * each);
+    int rc = c.ct == XT_F32    ? launch_paged_attn_f32(a, p.DP, grid, st)
+             : c.ct == XT_F16  ? launch_paged_attn_f16(a, p.DP, grid, st)
+             : c.ct == XT_BF16 ? launch_paged_attn_bf16(a, p.DP, grid, st)
+             : c.ct == CT_I8   ? launch_paged_attn_i8(a, p.DP, grid, st)
+                               : launch_paged_attn_e4m3(a, p.DP, grid, st);
+    if (rc || p.splits == 1) {
+      if (rc) return rc;
+      continue;
+    }
+    const unsigned joins = (unsigned)(n * rows);
+    if (p.DP == 64)
+      paged_join_kernel<64><<<joins, 256, 0, st>>>(a, p.SB);
+    else if (p.DP == 128)
+      paged_join_kernel<128><<<joins, 256, 0, st>>>(a, p.SB);
+    else
+      paged_join_kernel<256><<<joins, 256, 0, st>>>(a, p.SB);
+    if ((rc = check_launch())) return rc;
+  }
+  return 0;
+}
+
+int launch_paged_append(const PagedStore& c, hipStream_t st) {
+  PagedStore a = c;
+  plan(a);
+  const int64_t es = a.xt == XT_F32 ? 4 : 2;
+  auto vec = [&](const void* p) { return (uintptr_t)p % 16 == 0; };
+  a.vec = a.c.D % 8 == 0 && vec(a.kn) && vec(a.vn) && a.n_sb * es % 16 == 0 && a.n_st * es % 16 == 0 && a.n_sh * es % 16 == 0;
+  const bool own = a.start == a.c.length;  // the length is read by every workgroup: moved by one that no other reads after
+  if (own && a.T * a.c.Hk * 2 <= kStoreAlone) a.parts = 1;
+  a.set_length = !own || a.parts == 1;
+  const int64_t B = a.c.B, most = std::max<int64_t>(1, kLaunchThreads / kStoreThreads / a.parts);
+  for (int64_t b0 = 0; b0 < B; b0 += most) {
+    PagedStore s = a;
+    s.c.B = std::min(most, B - b0);
+    s.c.table += b0 * a.c.max_pages, s.c.length += b0, s.start += b0;
+    if (s.counts) s.counts += b0;
+    s.kn = (const char*)a.kn + b0 * a.n_sb * es, s.vn = (const char*)a.vn + b0 * a.n_sb * es;
+    const unsigned grid = (unsigned)(s.c.B * s.parts);
+    const int rc = a.ct == XT_F32    ? launch_append_ct<XT_F32>(s, grid, st)
+                   : a.ct == XT_F16  ? launch_append_ct<XT_F16>(s, grid, st)
+                   : a.ct == XT_BF16 ? launch_append_ct<XT_BF16>(s, grid, st)
+                   : a.ct == CT_I8   ? launch_append_ct<CT_I8>(s, grid, st)
+                                     : launch_append_ct<CT_E4M3>(s, grid, st);
+    if (rc) return rc;
+  }
+  if (a.set_length) return 0;
+  paged_length_kernel<<<(unsigned)((B + kStoreThreads - 1) / kStoreThreads), kStoreThreads, 0, st>>>(a);
+  return check_launch();
+}
+
+int launch_paged_read(const PagedStore& c, hipStream_t st) {
+  PagedStore a = c;
+  plan(a);
+  const int64_t n = a.xt == XT_F32 ? 16 : 8;
+  a.vec = (uintptr_t)a.k_out % n == 0 && (uintptr_t)a.v_out % n == 0 && a.n_sb % 4 == 0 && a.n_st % 4 == 0 && a.n_sh % 4 == 0;
+  const int64_t es = a.xt == XT_F32 ? 4 : 2, B = a.c.B, most = std::max<int64_t>(1, kLaunchThreads / kStoreThreads / a.parts);
+  for (int64_t b0 = 0; b0 < B; b0 += most) {
+    PagedStore s = a;
+    s.c.B = std::min(most, B - b0);
+    s.c.table += b0 * a.c.max_pages, s.c.length += b0, s.start += b0;
+    s.k_out = (char*)a.k_out + b0 * a.n_sb * es, s.v_out = (char*)a.v_out + b0 * a.n_sb * es;
+    const unsigned grid = (unsigned)(s.c.B * s.parts);
+    const int rc = a.ct == XT_F32    ? launch_read_ct<XT_F32>(s, grid, st)
+                   : a.ct == XT_F16  ? launch_read_ct<XT_F16>(s, grid, st)
+                   : a.ct == XT_BF16 ? launch_read_ct<XT_BF16>(s, grid, st)
+                   : a.ct == CT_I8   ? launch_read_ct<CT_I8>(s, grid, st)
+                                     : launch_read_ct<CT_E4M3>(s, grid, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+}  // namespace sbq

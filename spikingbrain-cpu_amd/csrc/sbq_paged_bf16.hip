@@ -1,0 +1,10 @@
+// sbq_paged_bf16.hip - the attention over a bf16 cache in pages (sbq_paged.h).
+#include "sbq_paged.h"
+
+namespace sbq {
+
+int launch_paged_attn_bf16(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
+  return a.qt == XT_F32 ? launch_paged_types<XT_BF16, 3, 3>(a, DP, grid, st) : launch_paged_types<XT_BF16, 1, 2>(a, DP, grid, st);
+}
+
+}  // namespace sbq

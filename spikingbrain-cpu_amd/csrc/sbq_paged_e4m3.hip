@@ -1,0 +1,10 @@
+// sbq_paged_e4m3.hip - the attention over an e4m3 cache in pages (sbq_paged.h).
+#include "sbq_paged.h"
+
+namespace sbq {
+
+int launch_paged_attn_e4m3(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
+  return a.qt == XT_F32 ? launch_paged_types<CT_E4M3, 2, 2>(a, DP, grid, st) : launch_paged_types<CT_E4M3, 1, 1>(a, DP, grid, st);
+}
+
+}  // namespace sbq

@@ -15,6 +15,8 @@ SBQ_F32, SBQ_F16, SBQ_BF16 = 0, 1, 2
 SBQ_NOALLOC_XQ_BYTES = 8 << 20  # include/sbq.h
 SBQ_ARGMAX_WS_BYTES = 16640  # include/sbq.h
 SBQ_ATTN_MAX_T = 1024  # query tokens of one sbq_tree_attention call (include/sbq.h)
+SBQ_I8, SBQ_E4M3 = 3, 4  # cache types (include/sbq.h)
+SBQ_PAGED_MAX_T = 1024  # query tokens of a sequence in one sbq_paged_attention call (include/sbq.h)
 SBQ_MAX_GROUP = 4  # linears per sbq_linear_w8_grouped / sbq_linear_w8a8_grouped call (include/sbq.h)
 
 # Every entry point declared in include/sbq.h, with its ctypes signature.
@@ -63,6 +65,15 @@ SIGNATURES = {
     "sbq_kv_workspace_bytes": (_L, [_L, _L]),
     "sbq_kv_append": (_I, [_P, _P, _L, _P, _P, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _I, _L, _L, _L, _P, _S, _P]),
     "sbq_kv_take": (_I, [_P, _P, _L, _P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _L, _P, _S, _P]),
+    "sbq_qk_norm_rope": (_I, [_P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _L, _P, _L, _P, _L, _I, _P, _P, _I, ctypes.c_float, _P,
+                              _P, _L, _L, _L, _L, _P]),
+    "sbq_paged_append": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P]),
+    "sbq_paged_read": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _L, _P, _P, _I, _L, _L, _L, _P]),
+    "sbq_paged_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _I]),
+    "sbq_paged_attention": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _P, _L,
+                                 ctypes.c_float, _P, _L, _L, _L, _P, _S, _P]),
+    "sbq_verify_workspace_bytes": (_L, [_L, _L]),
+    "sbq_verify_drafts": (_I, [_P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _S, _P]),
     "sbq_sample_rows": (_I, [_P, _L, _L, _L, ctypes.c_float, _L, ctypes.c_float, _P, _P, _P, _S, _P]),
 }
 

@@ -617,6 +617,64 @@ def sample(logits: torch.Tensor, params, generator: torch.Generator | None = Non
     return int(tok[0])
 
 
+def verify_workspace(B: int, V: int, device: torch.device) -> torch.Tensor:
+    """Scratch of verify_drafts for B sequences and V tokens (any content; one call at a time)."""
+    return torch.empty((_lib.load().sbq_verify_workspace_bytes(B, V),), dtype=torch.uint8, device=device)
+
+
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, u: torch.Tensor,
+                  counts: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens a step keeps, and the token after them: (kept,
+    token), int64 [B] each, such that the tokens are distributed as the target
+    alone would sample them.
+
+    target [B, T + 1, V]: the target's probabilities after each prefix of the
+    drafts; draft [B, T, V]: those that the drafts `tokens` (int64 [B, T]) were
+    drawn from, of target's dtype (None: each draft was certain, for instance
+    greedy or looked up).  u: fp32 [B, T + 1] uniforms in [0, 1).  counts (int64
+    [B]): the sequences' own numbers of drafts, where fewer than T.
+
+    Draft t is kept while u[t] * draft[t, x] < target[t, x].  The token is drawn
+    with u[T] from max(target - draft, 0) of the first refused draft's row, or
+    after the last draft from target's next row, as sample_tokens draws: the
+    first index whose prefix of mass exceeds u[T] times the whole.  Products
+    and sums are 64-bit.  token is -1 where that mass is 0, infinite or NaN.  A
+    draft that is no token (outside 0 .. V - 1) is refused."""
+    if not target.is_cuda or target.dim() != 3 or target.dtype not in _DTYPE_CODE:
+        raise ValueError("verify_drafts: target must be a float32, float16 or bfloat16 GPU tensor [B, T + 1, V]")
+    B, T, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    dev = target.device
+    if T < 0 or V < 1:
+        raise ValueError("verify_drafts: target must hold a row at least, and a token")
+    if draft is not None and (draft.shape != (B, T, V) or draft.dtype != target.dtype or draft.device != dev):
+        raise ValueError(f"verify_drafts: draft must be a {target.dtype} [{B}, {T}, {V}] tensor on {dev}")
+    if tokens.dtype != torch.int64 or tokens.shape != (B, T) or tokens.device != dev:
+        raise ValueError(f"verify_drafts: tokens must be an int64 [{B}, {T}] tensor on {dev}")
+    if u.dtype != torch.float32 or u.shape != (B, T + 1) or u.device != dev:
+        raise ValueError(f"verify_drafts: u must be a float32 [{B}, {T + 1}] tensor on {dev}")
+    if counts is not None and (counts.dtype != torch.int64 or counts.shape != (B,) or counts.device != dev):
+        raise ValueError(f"verify_drafts: counts must be an int64 [{B}] tensor on {dev}")
+    if V > 1 and target.stride(2) != 1:
+        target = target.contiguous()
+    if draft is not None and V > 1 and draft.stride(2) != 1:
+        draft = draft.contiguous()
+    tokens, u = tokens.contiguous(), u.contiguous()
+    counts = None if counts is None else counts.contiguous()
+    both = torch.empty((2, B), dtype=torch.int64, device=dev)
+    if workspace is None:
+        workspace = verify_workspace(B, V, dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device")
+    ps, qs = target.stride(), (0, 0) if draft is None else draft.stride()
+    with _on_device(dev):
+        _lib.check(_lib.load().sbq_verify_drafts(
+            _ptr(target), ps[0], ps[1], _ptr(draft), qs[0], qs[1], _DTYPE_CODE[target.dtype], B, T, V, _ptr(tokens), _ptr(u),
+            _ptr(counts), both.data_ptr(), both.data_ptr() + 8 * B, _ptr(workspace), _nbytes(workspace), _stream(dev)),
+            "sbq_verify_drafts")
+    return both[0], both[1]
+
+
 def argmax_state(device: torch.device) -> torch.Tensor:
     """The zeroed state (keys and count) of linear_w8_argmax /
     linear_w8a8_argmax: every call leaves it zero again, so one state serves

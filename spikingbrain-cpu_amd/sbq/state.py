@@ -20,6 +20,9 @@ for the attention) rather than by slicing.  A whole decode step, the token
 feeding the next step included, can therefore be captured in a HIP graph and
 replayed once per token with no host work in between.
 
+For several sequences at once DevicePagedKVBuffer holds the keys and values in
+pages of one pool, optionally in 8 bits.
+
 Capacity: a full-attention buffer holds ``capacity`` positions (slot =
 position).  A sliding-window buffer is a ring of ``capacity`` slots (slot =
 position mod capacity); it must hold the window plus the tokens appended by
@@ -146,6 +149,74 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_pos: 
             out.data_ptr(), os_[0], os_[1], None if weight is None else weight.data_ptr(), workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), _stream(device)), "sbq_tree_attention")
     return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 interleaved: bool = False, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The head norms and the rotation between the projections and the
+    attention (model.py:260-270, rotary 46-51) in one pass: q [tokens, heads,
+    dim] and k [tokens, kv_heads, dim] (or None) of one dtype, for instance
+    views of a fused projection's output.  Every vector is divided by its root
+    mean square (+ eps) and multiplied by q_weight / k_weight [dim] (None: no
+    norm), then its first 2 * len(inv_freq) columns are rotated by position *
+    inv_freq[i]: column i with i + len(inv_freq), or with `interleaved` 2i with
+    2i + 1.  The angle is exact (the reference's fp32 product is not, far into
+    a context), the rest fp32, rounded once.
+
+    positions: int64 [n], tokens a multiple of n: token t stands at positions[t
+    // (tokens / n)] + t % (tokens / n), so [tokens] gives each its own and the
+    starts of n sequences are enough for their next tokens.  q_out, k_out: q and
+    k themselves, or tensors apart from both (default: new ones)."""
+    gpu, dtype = q.get_device(), q.dtype
+    if gpu < 0:
+        raise ValueError("qk_norm_rope: q must be a GPU tensor")
+    if dtype not in _DTYPE_CODE:
+        raise ValueError(f"qk_norm_rope: unsupported dtype {dtype}; expected float32, float16 or bfloat16")
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]
+                                           or k.dtype != dtype or k.get_device() != gpu)):
+        raise ValueError("qk_norm_rope: expected q [tokens, heads, dim] and k [tokens, kv_heads, dim] of one dtype on one GPU")
+    tokens, heads, dim = q.shape
+    n = positions.numel()
+    if positions.dtype != torch.int64 or positions.get_device() != gpu or not positions.is_contiguous() \
+            or (tokens % n if n else tokens):
+        raise ValueError(f"qk_norm_rope: positions must be a contiguous int64 tensor on {q.device} whose size divides {tokens} "
+                         "tokens")
+    if (inv_freq.dtype != torch.float32 or inv_freq.get_device() != gpu or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
+            or 2 * inv_freq.numel() > dim or dim > 256):
+        raise ValueError(f"qk_norm_rope: inv_freq must be a contiguous float32 tensor on {q.device} of at most dim / 2 entries, "
+                         "dim at most 256")
+    wt = None
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.shape != (dim,) or w.get_device() != gpu or not w.is_contiguous() or w.dtype not in _DTYPE_CODE:
+                raise ValueError(f"qk_norm_rope: weights must be contiguous float [{dim}] tensors on {q.device}")
+            if wt is not None and w.dtype != wt:
+                raise ValueError("qk_norm_rope: q_weight and k_weight must share a dtype")
+            wt = w.dtype
+    outs = []
+    for name, x, out in (("q_out", q, q_out), ("k_out", k, k_out)):
+        if out is None:
+            out = None if x is None else torch.empty(x.shape, dtype=dtype, device=q.device)
+        elif (x is None or out.shape != x.shape or out.dtype != dtype or out.get_device() != gpu
+              or (dim > 1 and out.stride(2) != 1) or (out.data_ptr() == x.data_ptr() and out.stride() != x.stride())):
+            raise ValueError(f"qk_norm_rope: {name} must have its input's shape, dtype and device, with unit stride in dim")
+        outs.append(out)
+    if tokens == 0:
+        return outs[0], outs[1]
+    q = _rows_of(q)
+    k = None if k is None else _rows_of(k)
+    qs, qo = q.stride(), outs[0].stride()
+    ks, ko = ((0, 0), (0, 0)) if k is None else (k.stride(), outs[1].stride())
+    with _on_device(q.device):
+        _lib.check(_lib.load().sbq_qk_norm_rope(
+            q.data_ptr(), None if k is None else k.data_ptr(), _DTYPE_CODE[dtype], tokens, heads, 0 if k is None else k.shape[1],
+            dim, qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), tokens // n, inv_freq.data_ptr(), inv_freq.numel(),
+            int(interleaved), None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), 0 if wt is None else _DTYPE_CODE[wt], eps, outs[0].data_ptr(),
+            None if k is None else outs[1].data_ptr(), qo[0], qo[1], ko[0], ko[1], _stream(q.device)), "sbq_qk_norm_rope")
+    return outs[0], outs[1]
 
 
 class DeviceKVBuffer:
@@ -335,6 +406,283 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
     def truncate(self, length) -> None:
         super().truncate(length)
         self.weight.masked_fill_(self.slot_pos < 0, 0.0)
+
+
+_CACHE_CODE = {**_DTYPE_CODE, torch.int8: _lib.SBQ_I8, torch.float8_e4m3fn: _lib.SBQ_E4M3}
+
+
+class DevicePagedKVBuffer:
+    """Keys and values of several sequences in pages of one pool, for a step
+    that runs all of them at once.  No counterpart in the reference, whose
+    engine holds one sequence.
+
+    dtype: float32, float16 or bfloat16, or int8 or float8_e4m3fn: then a
+    token's keys (values) of a head are kept as 8-bit codes and one fp32 scale,
+    max |x| / 127 or / 448, as they are written, and multiplied out as they are
+    read.  The pool is k, v [pages, heads, page, dim] (rows padded to 16
+    columns in memory; k_scale, v_scale [pages, heads, page]).  Sequence b's
+    position p stands in page table[b, p // page] (int32 [sequences,
+    max_pages], -1: none), row p % page, and length [sequences] (int64) is how
+    many positions it holds.
+
+    The host gives pages out: reserve(sequence, length) before an append that
+    reaches so far, release(sequence) when it is done.  append, attend, read
+    and truncate find everything else on the device and keep every address, so
+    a step can be captured in a HIP graph, and replayed for as long as its
+    tokens fit what is reserved.  What an append finds no page for is dropped.
+    GPU only."""
+
+    def __init__(self, sequences: int, heads: int, dim: int, pages: int, page: int = 64, max_pages: int | None = None,
+                 window: int | None = None, device: torch.device | str | None = None, dtype: torch.dtype = torch.float32):
+        max_pages = pages if max_pages is None else max_pages
+        if dtype not in _CACHE_CODE:
+            raise ValueError(f"DevicePagedKVBuffer: unsupported dtype {dtype}; expected float32, float16, bfloat16, int8 or "
+                             "float8_e4m3fn")
+        if not 1 <= sequences <= 65536 or not 1 <= heads <= 65536 or not 1 <= dim <= 256 or not 1 <= pages <= 1 << 30:
+            raise ValueError("DevicePagedKVBuffer: 1 to 65536 sequences and heads, a dim of at most 256, and pages >= 1")
+        if page not in (16, 32, 64, 128, 256, 512, 1024) or max_pages < 1 or max_pages * page > 1 << 30:
+            raise ValueError("DevicePagedKVBuffer: page must be a power of two from 16 to 1024, and max_pages * page at most 2^30")
+        if window is not None and window < 1:
+            raise ValueError("DevicePagedKVBuffer: window must be >= 1")
+        self.sequences, self.heads, self.dim, self.page, self.window = sequences, heads, dim, page, window
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        row, b8 = -(-dim // 16) * 16, dtype in (torch.int8, torch.float8_e4m3fn)
+        self.k = torch.zeros(pages, heads, page, row, dtype=dtype, device=dev)[..., :dim]
+        self.v = torch.zeros(pages, heads, page, row, dtype=dtype, device=dev)[..., :dim]
+        self.k_scale = torch.zeros(pages, heads, page, device=dev) if b8 else None
+        self.v_scale = torch.zeros(pages, heads, page, device=dev) if b8 else None
+        self.table = torch.full((sequences, max_pages), -1, dtype=torch.int32, device=dev)
+        self.length = torch.zeros(sequences, dtype=torch.long, device=dev)
+        self._free = list(range(pages - 1, -1, -1))
+        self._held: list[dict[int, int]] = [{} for _ in range(sequences)]  # page of the sequence -> page of the pool
+        self._first = [0] * sequences  # pages of the sequence before this one were given back
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    def _row(self, fn: str, sequence: int) -> int:
+        if not 0 <= sequence < self.sequences:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: sequence must be 0 .. {self.sequences - 1}")
+        return sequence
+
+    def reserve(self, sequence: int, length: int) -> None:
+        """Give `sequence` the pages that positions below `length` need and it
+        does not have.  All or none of them: ValueError if the table's row is
+        too short, RuntimeError if the pool has too few free pages."""
+        held = self._held[self._row("reserve", sequence)]
+        last = -(-length // self.page)
+        if last > self.table.shape[1]:
+            raise ValueError(f"DevicePagedKVBuffer.reserve: {length} positions are more than the table's row holds")
+        want = [i for i in range(self._first[sequence], last) if i not in held]
+        if len(want) > len(self._free):
+            raise RuntimeError(f"DevicePagedKVBuffer.reserve: {len(want)} pages wanted, {len(self._free)} free")
+        if not want:
+            return
+        for i in want:
+            held[i] = self._free.pop()
+        # (what is held lies side by side from the first page not given back)
+        self.table[sequence, want[0]:want[-1] + 1] = torch.tensor([held[i] for i in range(want[0], want[-1] + 1)],
+                                                                  dtype=torch.int32, device=self.device)
+
+    def release(self, sequence: int, before: int | None = None) -> None:
+        """Take the sequence's pages back and forget its positions; with
+        `before` only the pages that end at or below that position (which a
+        window has left behind)."""
+        held = self._held[self._row("release", sequence)]
+        first = self.table.shape[1] if before is None else max(0, before // self.page)
+        for i in [i for i in held if i < first]:
+            self._free.append(held.pop(i))
+        if before is None:
+            self._first[sequence] = 0
+            self.table[sequence] = -1
+            self.length[sequence] = 0
+        else:
+            self._first[sequence] = max(self._first[sequence], first)
+            self.table[sequence, :first] = -1
+
+    def reset(self) -> None:
+        for i in range(self.sequences):
+            self._held[i].clear()
+            self._first[i] = 0
+        self._free = list(range(self.k.shape[0] - 1, -1, -1))
+        self.table.fill_(-1)
+        self.length.zero_()
+
+    def _cache(self, fn: str, sequence: int | None) -> tuple:
+        """The C ABI's description of the cache (of one sequence's row), from k to length."""
+        k, v, ks, vs, table, length = self.k, self.v, self.k_scale, self.v_scale, self.table, self.length
+        gpu, code, d, page = k.get_device(), _CACHE_CODE.get(k.dtype), self.dim, self.page
+        row = -(-d // 16) * 16
+        strides = (self.heads * page * row, page * row, row, 1)
+        if gpu < 0 or code is None or k.dim() != 4 or k.shape[1:] != (self.heads, page, d) or v.shape != k.shape \
+                or v.dtype != k.dtype or v.get_device() != gpu or k.stride()[:3] != strides[:3] or v.stride()[:3] != strides[:3]:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: k and v must be the buffer's pool on one GPU")
+        if code >= _lib.SBQ_I8:
+            for s in (ks, vs):
+                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.get_device() != gpu \
+                        or not s.is_contiguous():
+                    raise ValueError(f"DevicePagedKVBuffer.{fn}: k_scale and v_scale must be the buffer's scales")
+            ks, vs = ks.data_ptr(), vs.data_ptr()
+        else:
+            ks = vs = None
+        n = self.sequences
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n or not table.is_contiguous() \
+                or table.get_device() != gpu or length.dtype != torch.int64 or length.shape != (n,) \
+                or not length.is_contiguous() or length.get_device() != gpu:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: table must be int32 [{n}, max_pages] and length int64 [{n}]")
+        width = table.shape[1]
+        at = 0 if sequence is None else self._row(fn, sequence)
+        return (k.data_ptr(), v.data_ptr(), ks, vs, code, k.shape[0], page, self.heads, d, table.data_ptr() + 4 * width * at,
+                n if sequence is None else 1, width, length.data_ptr() + 8 * at)
+
+    def _places(self, fn: str, name: str, t, n: int) -> torch.Tensor:
+        """int64 [n] on the device; an int for every sequence."""
+        if not isinstance(t, torch.Tensor):
+            return torch.full((n,), int(t), dtype=torch.long, device=self.device)
+        if t.dtype != torch.int64 or t.numel() != n or t.get_device() != self.k.get_device() or not t.is_contiguous():
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: {name} must be a contiguous int64 tensor of {n} on {self.device}")
+        return t
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, start=None, counts: torch.Tensor | None = None,
+               sequence: int | None = None) -> None:
+        """Store k, v [sequences, T, heads, dim] at each sequence's positions
+        start .. start + T - 1 (default: after those it holds; an int or int64
+        [sequences]), the first counts[b] of them where counts (int64
+        [sequences]) is given; length becomes start + counts.  With `sequence`
+        k, v [T, heads, dim] go to that one alone, and start and counts are of
+        one entry."""
+        cache = self._cache("append", sequence)
+        n, lead = cache[10], 1 if sequence is None else 0
+        if k.shape != v.shape or k.dim() != 3 + lead or tuple(k.shape[1 + lead:]) != (self.heads, self.dim) \
+                or (lead and k.shape[0] != n):
+            raise ValueError(f"DevicePagedKVBuffer.append: expected {'[' + str(n) + ', T' if lead else '[T'}, {self.heads}, "
+                             f"{self.dim}] keys and values")
+        gpu = self.k.get_device()
+        if k.get_device() != gpu or v.get_device() != gpu:
+            raise ValueError(f"DevicePagedKVBuffer.append: keys and values must be on {self.device}")
+        if k.dtype not in _DTYPE_CODE or v.dtype != k.dtype:
+            k, v = k.float(), v.float()
+        if not lead:
+            k, v = k[None], v[None]
+        if (self.dim > 1 and (k.stride(3) != 1 or v.stride(3) != 1)) or k.stride()[:3] != v.stride()[:3]:
+            k, v = k.contiguous(), v.contiguous()
+        if any(_within(x, p) for x in (k, v) for p in (self.k, self.v)):
+            k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+        length = cache[12]
+        if start is None:
+            at = length
+        else:
+            start = self._places("append", "start", start, n)
+            at = start.data_ptr()
+            if at != length and abs(at - length) < 8 * n:  # (other sequences' lengths, which this call moves)
+                start = start.clone()
+                at = start.data_ptr()
+        if counts is not None:
+            counts = self._places("append", "counts", counts, n)
+            if abs(counts.data_ptr() - length) < 8 * n:
+                counts = counts.clone()
+        st = k.stride()
+        with _on_device(self.device):
+            _lib.check(_lib.load().sbq_paged_append(
+                *cache, at, None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype],
+                k.shape[1], st[0], st[1], st[2], _stream(self.device)), "sbq_paged_append")
+
+    def read(self, start, count: int, dtype: torch.dtype | None = None,
+             sequence: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [sequences, count, heads, dim] of the positions from
+        start (an int or int64 [sequences]) on, multiplied out and rounded to
+        dtype (default: the pool's, float32 for 8 bits); positions that a
+        sequence does not hold are 0.  With `sequence` [count, heads, dim] of
+        that one."""
+        cache = self._cache("read", sequence)
+        n = cache[10]
+        if dtype is None:
+            dtype = self.k.dtype if self.k.dtype in _DTYPE_CODE else torch.float32
+        if dtype not in _DTYPE_CODE or count < 0:
+            raise ValueError("DevicePagedKVBuffer.read: dtype must be float32, float16 or bfloat16, and count >= 0")
+        start = self._places("read", "start", start, n)
+        k = torch.empty(n, count, self.heads, self.dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        with _on_device(self.device):
+            _lib.check(_lib.load().sbq_paged_read(
+                *cache, start.data_ptr(), count, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[dtype], count * self.heads * self.dim,
+                self.heads * self.dim, self.dim, _stream(self.device)), "sbq_paged_read")
+        return (k, v) if sequence is None else (k[0], v[0])
+
+    def attend(self, q: torch.Tensor, start=None, counts: torch.Tensor | None = None, scale: float | None = None,
+               out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """The attention of q [sequences, T, q heads, dim] (or [sequences, q
+        heads, dim], one token each) over each sequence's positions: token t,
+        at start + t, sees those held up to its own, with a window only the
+        last `window` of them.  start (an int or int64 [sequences]) defaults to
+        the tokens appended last: length - counts, counts (int64 [sequences],
+        default T) being how many of the T are there; the others' rows are 0,
+        as is a row that sees nothing.  Query head h reads key head h // (q
+        heads / heads).  q has the pool's dtype or float32 (8-bit pools: any);
+        the result has q's."""
+        cache = self._cache("attend", None)
+        n, gpu = cache[10], self.k.get_device()
+        if q.dim() not in (3, 4) or q.shape[0] != n or q.shape[-1] != self.dim or q.shape[-2] % self.heads \
+                or q.shape[-2] == 0:
+            raise ValueError(f"DevicePagedKVBuffer.attend: expected q [{n}, T, heads, {self.dim}], heads a multiple of "
+                             f"{self.heads}")
+        if q.get_device() != gpu or q.dtype not in _DTYPE_CODE or (self.k_scale is None and q.dtype != self.k.dtype
+                                                                   and q.dtype != torch.float32):
+            raise ValueError(f"DevicePagedKVBuffer.attend: q must be on {self.device}, of the pool's dtype or float32 (8-bit "
+                             "pools: float32, float16 or bfloat16)")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != gpu or (self.dim > 1 and out.stride(-1) != 1):
+            raise ValueError("DevicePagedKVBuffer.attend: out must have q's shape, dtype and device, with unit stride in dim")
+        if out.data_ptr() == q.data_ptr() and q.numel():
+            raise ValueError("DevicePagedKVBuffer.attend: out must not be q itself")
+        q4, o4 = (q[:, None], out[:, None]) if q.dim() == 3 else (q, out)
+        T, heads = q4.shape[1], q4.shape[2]
+        if T > _lib.SBQ_PAGED_MAX_T:
+            raise ValueError(f"DevicePagedKVBuffer.attend: at most {_lib.SBQ_PAGED_MAX_T} tokens per call")
+        if T == 0:
+            return out
+        if self.dim > 1 and q4.stride(3) != 1:
+            q4 = q4.contiguous()
+        L = _lib.load()
+        if workspace is None:
+            workspace = torch.empty(L.sbq_paged_attn_workspace_bytes(n, T, heads, self.heads, self.dim, self.page, cache[11],
+                                                                     cache[4]), dtype=torch.uint8, device=q.device)
+        elif workspace.get_device() != gpu or not workspace.is_contiguous():
+            raise ValueError(f"DevicePagedKVBuffer.attend: workspace must be a contiguous tensor on {self.device}")
+        start = None if start is None else self._places("attend", "start", start, n)
+        counts = None if counts is None else self._places("attend", "counts", counts, n)
+        qs, os_ = q4.stride(), o4.stride()
+        with _on_device(q.device):
+            _lib.check(L.sbq_paged_attention(
+                q4.data_ptr(), _DTYPE_CODE[q.dtype], T, heads, qs[0], qs[1], qs[2], *cache,
+                None if start is None else start.data_ptr(), None if counts is None else counts.data_ptr(), self.window or 0,
+                self.dim ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1], os_[2], workspace.data_ptr(),
+                workspace.numel() * workspace.element_size(), _stream(q.device)), "sbq_paged_attention")
+        return out
+
+    def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
+             q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+             interleaved: bool = False, counts: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+        """What stands between a softmax layer's projections (model.py:260-270)
+        for the next T tokens of every sequence: q [sequences, T, q heads, dim]
+        and k, v [sequences, T, heads, dim] as projected; norms and rotation at
+        the sequences' next positions (qk_norm_rope), append, attend."""
+        if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[0] != self.sequences:
+            raise ValueError(f"DevicePagedKVBuffer.step: expected q [{self.sequences}, T, q heads, dim] and k, v "
+                             f"[{self.sequences}, T, heads, dim]")
+        qr, kr = qk_norm_rope(q.flatten(0, 1), k.flatten(0, 1), self.length, inv_freq, q_weight, k_weight, eps, interleaved)
+        self.append(kr.view(k.shape), v, None, counts)
+        return self.attend(qr.view(q.shape), None, counts, scale)
+
+    def truncate(self, length) -> None:
+        """Forget positions >= length (an int or int64 [sequences]), for
+        instance the drafts that were refused."""
+        if isinstance(length, torch.Tensor):
+            self.length.copy_(torch.minimum(self.length, self._places("truncate", "length", length, self.sequences)))
+        else:
+            self.length.clamp_(max=int(length))
 
 
 @dataclass
