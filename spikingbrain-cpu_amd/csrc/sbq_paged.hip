@@ -11,6 +11,7 @@
 #include "sbq_paged.h"
 
 #include <algorithm>
+#include <stdlib.h>
 
 namespace sbq {
 
@@ -221,17 +222,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   __shared__ __align__(16) f32x4 lds[NG][ND];
   __shared__ float lds_l[NG];
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
-  const int64_t at = a.first * a.c.Hk * R + blockIdx.x, b = at / ((int64_t)a.c.Hk * R);
-  const int r = (int)(at % R), kvh = (int)(at / R % a.c.Hk), t = r / a.rep, row0 = r & ~15;
-  const PagedSpan span(a, b);
-  int lo, hi;
-  span.all(a, row0 / a.rep, min(row0 + 15, R - 1) / a.rep, lo, hi);
-  const int blocks = hi >= lo ? hi / SB + 1 - lo / SB : 0;
-  const int used = max(1, min(a.splits, (blocks + kAttnWaves - 1) / kAttnWaves));
+  const int r = blockIdx.x, kvh = blockIdx.y;
+  int t = 0, t0 = 0, t1 = 0;
+  if (a.T > 1) t = r / a.rep, t0 = (r & ~15) / a.rep, t1 = min(r | 15, R - 1) / a.rep;
+  const PagedPlace p = paged_place<false>(a, blockIdx.z, t0, t1, SB);
+  int place;
+  const int used = paged_places(p, place);
   if (used == 1) return;  // (written by the one workgroup)
-  const float2* const ml = a.part_ml + at * a.splits;
+  const int64_t b = a.first + p.b, at = ((int64_t)kvh * a.places + place) * R + r;
+  const PagedSpan span(a, b);
+  const float2* const ml = a.part_ml + at;
   float top = -__builtin_inff();
-  for (int s = lane; s < used; s += 64) top = __builtin_fmaxf(top, ml[s].x);
+  for (int s = lane; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
   top = wave_max(top);
   const float from = top == -__builtin_inff() ? 0.0f : top;
   f32x4 sum = (f32x4)(0.0f);
@@ -242,8 +244,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int s = min(s0 + k * NG, used - 1);
-      x[k] = *(const f32x4*)(a.part_o + (at * a.splits + s) * DP + d);
-      y[k] = ml[s];
+      x[k] = *(const f32x4*)(a.part_o + (at + (int64_t)s * R) * DP + d);
+      y[k] = ml[(int64_t)s * R];
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -264,29 +266,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
     sum += lds[k][threadIdx.x];
     l += lds_l[k];
   }
-  span.of(a, t, lo, hi);
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  sum = hi >= lo ? sum * inv : (f32x4)(0.0f);
-  const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r % a.rep) * a.o_sh + d;
+  sum = span.last(t) >= span.first(t, a.window) ? sum * inv : (f32x4)(0.0f);
+  const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r - t * a.rep) * a.o_sh + d;
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
 
-constexpr int64_t kPagedGroups = 1024;  // workgroups aimed at
+static int64_t paged_groups() { const char* e = getenv("PG"); return e ? atoi(e) : 1024; }
+constexpr int64_t kPagedGroup = 512;  // sequences of a launch at most (each workgroup scans their lengths)
 
 struct PagedPlan {
-  int DP, SB, rtiles, splits;
+  int DP, SB, slots_log;
+  int64_t rtiles, n, places;
+  bool joins;  // can a sequence need more than one slot?
 };
-// The split goes by the table's room: how much of it is filled is known on the
-// device alone, where workgroups that a shorter sequence has no blocks for
-// leave at once.
+// How many workgroups there are goes by the table's room: how much of it is
+// filled is known on the device alone, where workgroups without a part leave
+// at once.
 PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, int ct) {
   PagedPlan p;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  p.SB = ct == XT_F32 ? 16 : is_8bit(ct) ? 64 : 32;
-  p.rtiles = (int)((R + 15) / 16);
-  const int64_t base = B * Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB;
-  const int64_t most = (blocks + kAttnWaves - 1) / kAttnWaves;
-  p.splits = (int)std::max<int64_t>(1, std::min(most, (kPagedGroups + base - 1) / base));
+  p.SB = ct == XT_F32 ? 16 : 32;
+  p.rtiles = (R + 15) / 16;
+  const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB, fours = (blocks + kAttnWaves - 1) / kAttnWaves;
+  p.n = std::min(B, kPagedGroup);
+  p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 30) / (fours * kAttnWaves)));  // (all blocks fit an int)
+  p.slots_log = 0;
+  while ((one << (p.slots_log + 1)) <= paged_groups() && ((int64_t)1 << p.slots_log) < p.n * fours) ++p.slots_log;
+  p.places = ((int64_t)1 << p.slots_log) + p.n;
+  p.joins = fours > 1;
   return p;
 }
 
@@ -297,8 +305,8 @@ int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct) {
   const int64_t R = heads / Hk * T;
   const PagedPlan p = paged_plan(B, R, Hk, D, room, ct);
-  if (p.splits == 1) return 0;
-  const int64_t parts = B * Hk * R * p.splits;
+  if (!p.joins) return 0;
+  const int64_t parts = Hk * R * p.places;
   return round256(parts * p.DP * 4) + round256(parts * 8);
 }
 
@@ -308,34 +316,26 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   PagedArgs a{};
   a.c = c.c, a.q = c.q, a.start = c.start, a.counts = c.counts, a.out = c.out;
   a.q_sb = c.q_sb, a.q_st = c.q_st, a.q_sh = c.q_sh, a.o_sb = c.o_sb, a.o_st = c.o_st, a.o_sh = c.o_sh;
-  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.splits = p.splits, a.rtiles = p.rtiles, a.qt = c.qt;
+  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots_log = p.slots_log;
+  a.places = (int)p.places;
   a.scale = c.scale * 1.44269504f;
   const int64_t eq = c.qt == XT_F32 ? 4 : 2;
-  auto vec = [&](const void* x, int64_t n, int64_t sb, int64_t ss, int64_t sh) {  // n elements at once, 16 bytes at most
-    const int64_t by = n * eq < 16 ? n * eq : 16;
-    return (uintptr_t)x % by == 0 && sb * eq % by == 0 && ss * eq % by == 0 && sh * eq % by == 0;
-  };
-  a.qvec = vec(c.q, 8, c.q_sb, c.q_st, c.q_sh);
-  a.ovec = vec(c.out, 4, c.o_sb, c.o_st, c.o_sh);
-  if (p.splits > 1) {
+  a.ovec = (uintptr_t)c.out % (4 * eq) == 0 && c.o_sb % 4 == 0 && c.o_st % 4 == 0 && c.o_sh % 4 == 0;
+  if (p.joins) {
     a.part_o = (float*)c.ws;
-    a.part_ml = (float2*)((uint8_t*)c.ws + round256(B * Hk * R * p.splits * p.DP * 4));
+    a.part_ml = (float2*)((uint8_t*)c.ws + round256(Hk * R * p.places * p.DP * 4));
   }
-  const int64_t each = Hk * p.rtiles * p.splits, rows = Hk * R;
-  const int64_t most = std::max<int64_t>(1, kLaunchThreads / 256 / std::max(each, rows));  // sequences of a launch
-  for (a.first = 0; a.first < B; a.first += most) {
-    const int64_t n = std::min(most, B - a.first);
-    const unsigned grid = (unsigned)(n * each);
+  for (a.first = 0; a.first < B; a.first += p.n) {
+    a.n = (int)std::min(p.n, B - a.first);
+    const dim3 grid((unsigned)Hk, 1u << p.slots_log, (unsigned)p.rtiles);
     int rc = c.ct == XT_F32    ? launch_paged_attn_f32(a, p.DP, grid, st)
              : c.ct == XT_F16  ? launch_paged_attn_f16(a, p.DP, grid, st)
              : c.ct == XT_BF16 ? launch_paged_attn_bf16(a, p.DP, grid, st)
              : c.ct == CT_I8   ? launch_paged_attn_i8(a, p.DP, grid, st)
                                : launch_paged_attn_e4m3(a, p.DP, grid, st);
-    if (rc || p.splits == 1) {
-      if (rc) return rc;
-      continue;
-    }
-    const unsigned joins = (unsigned)(n * rows);
+    if (rc) return rc;
+    if (!p.joins) continue;
+    const dim3 joins((unsigned)R, (unsigned)Hk, (unsigned)a.n);
     if (p.DP == 64)
       paged_join_kernel<64><<<joins, 256, 0, st>>>(a, p.SB);
     else if (p.DP == 128)

@@ -3,8 +3,8 @@
 
 namespace sbq {
 
-int launch_paged_attn_bf16(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
-  return a.qt == XT_F32 ? launch_paged_types<XT_BF16, 3, 3>(a, DP, grid, st) : launch_paged_types<XT_BF16, 1, 2>(a, DP, grid, st);
+int launch_paged_attn_bf16(const PagedArgs& a, int DP, dim3 grid, hipStream_t st) {
+  return a.qt == XT_F32 ? launch_paged_types<XT_BF16, XT_F32>(a, DP, grid, st) : launch_paged_types<XT_BF16, XT_BF16>(a, DP, grid, st);
 }
 
 }  // namespace sbq

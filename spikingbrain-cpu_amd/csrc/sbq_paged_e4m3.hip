@@ -3,8 +3,10 @@
 
 namespace sbq {
 
-int launch_paged_attn_e4m3(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
-  return a.qt == XT_F32 ? launch_paged_types<CT_E4M3, 2, 2>(a, DP, grid, st) : launch_paged_types<CT_E4M3, 1, 1>(a, DP, grid, st);
+int launch_paged_attn_e4m3(const PagedArgs& a, int DP, dim3 grid, hipStream_t st) {
+  return a.qt == XT_F32   ? launch_paged_types<CT_E4M3, XT_F32>(a, DP, grid, st)
+         : a.qt == XT_F16 ? launch_paged_types<CT_E4M3, XT_F16>(a, DP, grid, st)
+                          : launch_paged_types<CT_E4M3, XT_BF16>(a, DP, grid, st);
 }
 
 }  // namespace sbq

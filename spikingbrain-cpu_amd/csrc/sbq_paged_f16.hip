@@ -3,8 +3,8 @@
 
 namespace sbq {
 
-int launch_paged_attn_f16(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
-  return a.qt == XT_F32 ? launch_paged_types<XT_F16, 2, 2>(a, DP, grid, st) : launch_paged_types<XT_F16, 1, 1>(a, DP, grid, st);
+int launch_paged_attn_f16(const PagedArgs& a, int DP, dim3 grid, hipStream_t st) {
+  return a.qt == XT_F32 ? launch_paged_types<XT_F16, XT_F32>(a, DP, grid, st) : launch_paged_types<XT_F16, XT_F16>(a, DP, grid, st);
 }
 
 }  // namespace sbq

@@ -3,8 +3,8 @@
 
 namespace sbq {
 
-int launch_paged_attn_f32(const PagedArgs& a, int DP, unsigned grid, hipStream_t st) {
-  return launch_paged_types<XT_F32, 1, 1>(a, DP, grid, st);
+int launch_paged_attn_f32(const PagedArgs& a, int DP, dim3 grid, hipStream_t st) {
+  return launch_paged_types<XT_F32, XT_F32>(a, DP, grid, st);
 }
 
 }  // namespace sbq

@@ -51,118 +51,164 @@ __device__ __forceinline__ void rotate(float a, float b, float2 t, float& ya, fl
   yb = __builtin_fmaf(b, t.x, a * t.y);
 }
 
-// Four consecutive elements, n of them there (VEC: 0 or 4, aligned).
-template <int XT, bool VEC>
-__device__ __forceinline__ void load4(const typename XElem<XT>::T* p, int n, float (&x)[4]) {
+// N consecutive elements, n of them there (VEC: all or none, aligned).
+template <int XT, int N, bool VEC>
+__device__ __forceinline__ void load_piece(const typename XElem<XT>::T* p, int n, float (&x)[N]) {
   typedef typename XElem<XT>::T T;
-  typedef T V __attribute__((ext_vector_type(4)));
+  typedef T V __attribute__((ext_vector_type(N)));
   if constexpr (VEC) {
-    if (n > 0) {
-      const V v = *(const V*)p;
+    V v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
-    } else {
+    for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
+    if (n > 0) v = *(const V*)p;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = 0.0f;
-    }
+    for (int j = 0; j < N; ++j) x[j] = (float)v[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+    for (int j = 0; j < N; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+  }
+}
+template <int XT, int N, bool VEC>
+__device__ __forceinline__ void store_piece(typename XElem<XT>::T* p, int n, const float (&x)[N]) {
+  typedef typename XElem<XT>::T T;
+  typedef T V __attribute__((ext_vector_type(N)));
+  if constexpr (VEC) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (T)fp32_rounded(x[j]);
+    if (n > 0) *(V*)p = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) p[j] = (T)fp32_rounded(x[j]);
   }
 }
 
-template <int XT, bool VEC, bool INTER>
+// N columns in each of a lane's two pieces.
+template <int XT, int N, bool VEC, bool INTER>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   typedef typename XElem<XT>::T T;
-  extern __shared__ __align__(16) float2 cs[];  // [tokens][items * 4]
+  constexpr int U = 2;  // vectors of a lane at a time
+  extern __shared__ __align__(16) float2 cs[];  // [tokens][items * N]
   const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kRopeThreads / a.lanes;
   const int64_t token0 = (int64_t)(blockIdx.x / a.parts) * a.tokens;
   const int part = blockIdx.x % a.parts, n_tok = (int)min((int64_t)a.tokens, a.T - token0);
-  const int rows = n_tok * a.rows;  // a.rows: vectors of a token
-  const int pair_items = (a.pairs + 3) / 4;
+  const int pair_items = (a.pairs + N - 1) / N;
 
-  // the lane's two pieces of four columns: from column pa and pb on, na and nb of them there
+  // the lane's two pieces: from column pa and pb on, na and nb columns of them there
   int pa, pb, na, nb;
   const bool rotated = lane < pair_items;
   if (!rotated) {
-    pa = 2 * a.pairs + 8 * (lane - pair_items), pb = pa + 4;
+    pa = 2 * a.pairs + 2 * N * (lane - pair_items), pb = pa + N;
     na = a.D - pa, nb = a.D - pb;
   } else if (INTER) {
-    pa = 8 * lane, pb = pa + 4;
+    pa = 2 * N * lane, pb = pa + N;
     na = 2 * a.pairs - pa, nb = 2 * a.pairs - pb;
   } else {
-    pa = 4 * lane, pb = a.pairs + pa;
+    pa = N * lane, pb = a.pairs + pa;
     na = nb = a.pairs - pa;
   }
-  na = na < 0 ? 0 : na > 4 ? 4 : na, nb = nb < 0 ? 0 : nb > 4 ? 4 : nb;
+  na = na < 0 ? 0 : na > N ? N : na, nb = nb < 0 ? 0 : nb > N ? N : nb;
 
+  // its vectors: head h of token tok, a step's heads further each time
   const int step = groups * a.parts;
-  int row = part * groups + group;
-  float xa[4], xb[4];
-  auto fetch = [&](int row) {
-    const int tok = row / a.rows, h = row % a.rows;
-    const bool key = h >= a.heads;
-    const T* p = (const T*)(key ? a.k : a.q) + (token0 + tok) * (key ? a.k_st : a.q_st) + (key ? (h - a.heads) * a.k_sh : h * a.q_sh);
-    load4<XT, VEC>(p + pa, na, xa);
-    load4<XT, VEC>(p + pb, nb, xb);
+  int tok[U], h[U];
+  float xa[U][N], xb[U][N];
+  auto next = [&](int u, int from_tok, int from_h, int by) {
+    tok[u] = from_tok, h[u] = from_h + by;
+    while (h[u] >= a.rows) h[u] -= a.rows, ++tok[u];  // a.rows: vectors of a token
   };
-  if (row < rows) fetch(row);  // (the first vector's load goes ahead of the angles)
+  auto fetch = [&](int u) {
+    if (tok[u] >= n_tok) return;
+    const bool key = h[u] >= a.heads;
+    const T* const p = (const T*)(key ? a.k : a.q) + (token0 + tok[u]) * (key ? a.k_st : a.q_st) +
+                       (int64_t)(key ? h[u] - a.heads : h[u]) * (key ? a.k_sh : a.q_sh);
+    load_piece<XT, N, VEC>(p + pa, na, xa[u]);
+    load_piece<XT, N, VEC>(p + pb, nb, xb[u]);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    next(u, 0, part * groups + group, u * step);
+    fetch(u);  // (the first vectors' loads go ahead of the angles)
+  }
 
   for (int i = threadIdx.x; i < n_tok * a.pairs; i += kRopeThreads) {
-    const int tok = i / a.pairs, f = i - tok * a.pairs;
-    const int64_t t = a.first + token0 + tok;
-    cs[tok * pair_items * 4 + f] = turn(a.positions[t / a.per] + t % a.per, a.inv_freq[f]);
+    const int t_in = i / a.pairs, f = i - t_in * a.pairs;
+    const int64_t t = a.first + token0 + t_in;
+    cs[t_in * pair_items * N + f] = turn(a.per == 1 ? a.positions[t] : a.positions[t / a.per] + t % a.per, a.inv_freq[f]);
   }
+  // the weights of its columns
+  float wq[2][N], wk[2][N];
+  auto weights = [&](const void* w, float (&to)[2][N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      to[0][j] = w && j < na ? load_elem(w, a.wt, pa + j) : 0.0f;
+      to[1][j] = w && j < nb ? load_elem(w, a.wt, pb + j) : 0.0f;
+    }
+  };
+  weights(a.q_weight, wq);
+  if (a.kv_heads > 0) weights(a.k_weight, wk);
   __syncthreads();
 
-  for (; row < rows; row += step) {
-    const int tok = row / a.rows, h = row % a.rows;
-    const bool key = h >= a.heads;
-    const void* const w = key ? a.k_weight : a.q_weight;
-    if (w) {
-      float sum = 0.0f;
+  const float mean = 1.0f / (float)a.D;
+  while (tok[0] < n_tok) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = __builtin_fmaf(xa[j], xa[j], __builtin_fmaf(xb[j], xb[j], sum));
-      for (int o = 1; o < a.lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
-      const float r = 1.0f / __builtin_sqrtf(sum / (float)a.D + a.eps);
+    for (int u = 0; u < U; ++u) {
+      if (tok[u] >= n_tok) break;
+      const bool key = h[u] >= a.heads;
+      if (key ? a.k_weight != nullptr : a.q_weight != nullptr) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j < na) xa[j] = xa[j] * r * load_elem(w, a.wt, pa + j);
-        if (j < nb) xb[j] = xb[j] * r * load_elem(w, a.wt, pb + j);
-      }
-    }
-    float ya[4], yb[4];
+        for (int j = 0; j < N; ++j) sum = __builtin_fmaf(xa[u][j], xa[u][j], __builtin_fmaf(xb[u][j], xb[u][j], sum));
+        for (int o = 1; o < a.lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        const float r = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, mean, a.eps));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ya[j] = xa[j], yb[j] = xb[j];
-    if (rotated) {
-      const float2* const t = cs + (tok * pair_items + lane) * 4;
-      if constexpr (INTER) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {  // (entries past the last pair meet columns past it)
-          const float2 u = t[j], v = t[j + 2];
-          rotate(xa[2 * j], xa[2 * j + 1], u, ya[2 * j], ya[2 * j + 1]);
-          rotate(xb[2 * j], xb[2 * j + 1], v, yb[2 * j], yb[2 * j + 1]);
+        for (int j = 0; j < N; ++j) {
+          xa[u][j] = xa[u][j] * r * (key ? wk[0][j] : wq[0][j]);
+          xb[u][j] = xb[u][j] * r * (key ? wk[1][j] : wq[1][j]);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) rotate(xa[j], xb[j], t[j], ya[j], yb[j]);
       }
+      float ya[N], yb[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) ya[j] = xa[u][j], yb[j] = xb[u][j];
+      if (rotated) {
+        const float2* const t = cs + (tok[u] * pair_items + lane) * N;
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < N / 2; ++j) {  // (entries past the last pair meet columns past it)
+            rotate(xa[u][2 * j], xa[u][2 * j + 1], t[j], ya[2 * j], ya[2 * j + 1]);
+            rotate(xb[u][2 * j], xb[u][2 * j + 1], t[j + N / 2], yb[2 * j], yb[2 * j + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) rotate(xa[u][j], xb[u][j], t[j], ya[j], yb[j]);
+        }
+      }
+      T* const to = (T*)(key ? a.k_out : a.q_out) + (token0 + tok[u]) * (key ? a.ko_st : a.qo_st) +
+                    (int64_t)(key ? h[u] - a.heads : h[u]) * (key ? a.ko_sh : a.qo_sh);
+      store_piece<XT, N, VEC>(to + pa, na, ya);
+      store_piece<XT, N, VEC>(to + pb, nb, yb);
+      next(u, tok[u], h[u], U * step);
+      fetch(u);
     }
-    const int64_t to = (token0 + tok) * (key ? a.ko_st : a.qo_st) + (key ? (h - a.heads) * a.ko_sh : h * a.qo_sh);
-    void* const out = key ? a.k_out : a.q_out;
-    store_y4(out, XT, to + pa, (f32x4){ya[0], ya[1], ya[2], ya[3]}, VEC && na == 4, na);
-    store_y4(out, XT, to + pb, (f32x4){yb[0], yb[1], yb[2], yb[3]}, VEC && nb == 4, nb);
-    if (row + step < rows) fetch(row + step);
   }
 }
 
-template <int XT, bool VEC>
+template <int XT, int N, bool VEC>
 int launch_xt(const RopeArgs& a, bool inter, unsigned grid, size_t lds, hipStream_t st) {
   if (inter)
-    rope_kernel<XT, VEC, true><<<grid, kRopeThreads, lds, st>>>(a);
+    rope_kernel<XT, N, VEC, true><<<grid, kRopeThreads, lds, st>>>(a);
   else
-    rope_kernel<XT, VEC, false><<<grid, kRopeThreads, lds, st>>>(a);
+    rope_kernel<XT, N, VEC, false><<<grid, kRopeThreads, lds, st>>>(a);
   return check_launch();
+}
+// vec: elements that every piece may be loaded by at once, 1, 4 or (of 2 bytes) 8.
+template <int XT>
+int launch_vec(const RopeArgs& a, int vec, bool inter, unsigned grid, size_t lds, hipStream_t st) {
+  if constexpr (XT != XT_F32) {
+    if (vec == 8) return launch_xt<XT, 8, true>(a, inter, grid, lds, st);
+  }
+  return vec == 4 ? launch_xt<XT, 4, true>(a, inter, grid, lds, st) : launch_xt<XT, 4, false>(a, inter, grid, lds, st);
 }
 
 }  // namespace
@@ -170,18 +216,23 @@ int launch_xt(const RopeArgs& a, bool inter, unsigned grid, size_t lds, hipStrea
 int launch_rope(const RopeArgs& c, bool inter, int xt, hipStream_t st) {
   RopeArgs a = c;
   a.rows = a.heads + a.kv_heads;
-  const int items = (a.pairs + 3) / 4 + (a.D - 2 * a.pairs + 7) / 8;
+  const int64_t es = xt == XT_F32 ? 4 : 2;
+  auto fits = [&](const void* p, int64_t s, int64_t h, int n) {
+    return (uintptr_t)p % (n * es) == 0 && s % n == 0 && h % n == 0;
+  };
+  auto vec = [&](int n) {
+    return a.pairs % n == 0 && a.D % n == 0 && fits(a.q, a.q_st, a.q_sh, n) && fits(a.q_out, a.qo_st, a.qo_sh, n) &&
+           (a.kv_heads == 0 || (fits(a.k, a.k_st, a.k_sh, n) && fits(a.k_out, a.ko_st, a.ko_sh, n)));
+  };
+  const int v = xt != XT_F32 && vec(8) ? 8 : vec(4) ? 4 : 1, N = v == 8 ? 8 : 4;
+  const int items = (a.pairs + N - 1) / N + (a.D - 2 * a.pairs + 2 * N - 1) / (2 * N);
   a.lanes = 1;
   while (a.lanes < items) a.lanes <<= 1;
   const int groups = kRopeThreads / a.lanes;
   a.tokens = a.T >= 1024 ? kRopeTokens : 1;
   // few tokens: a vector a lane group, on as many workgroups as that takes
   a.parts = a.T < 512 ? (a.rows + groups - 1) / groups : 1;
-  const int64_t es = xt == XT_F32 ? 4 : 2, n = 4 * es;
-  auto vec = [&](const void* p, int64_t s, int64_t h) { return (uintptr_t)p % n == 0 && s % 4 == 0 && h % 4 == 0; };
-  const bool v = a.pairs % 4 == 0 && a.D % 4 == 0 && vec(a.q, a.q_st, a.q_sh) && vec(a.q_out, a.qo_st, a.qo_sh) &&
-                 (a.kv_heads == 0 || (vec(a.k, a.k_st, a.k_sh) && vec(a.k_out, a.ko_st, a.ko_sh)));
-  const size_t lds = (size_t)a.tokens * ((a.pairs + 3) / 4) * 4 * sizeof(float2);
+  const size_t lds = (size_t)a.tokens * ((a.pairs + N - 1) / N) * N * sizeof(float2);
   const int64_t most = kLaunchThreads / kRopeThreads / a.parts * a.tokens;  // tokens of a launch
   for (int64_t t0 = 0; t0 < c.T; t0 += most) {
     a.T = c.T - t0 < most ? c.T - t0 : most;
@@ -189,9 +240,9 @@ int launch_rope(const RopeArgs& c, bool inter, int xt, hipStream_t st) {
     a.q_out = (char*)c.q_out + t0 * c.qo_st * es, a.k_out = (char*)c.k_out + t0 * c.ko_st * es;
     a.first = t0;
     const unsigned grid = (unsigned)((a.T + a.tokens - 1) / a.tokens * a.parts);
-    const int rc = xt == XT_F32   ? v ? launch_xt<XT_F32, true>(a, inter, grid, lds, st) : launch_xt<XT_F32, false>(a, inter, grid, lds, st)
-                   : xt == XT_F16 ? v ? launch_xt<XT_F16, true>(a, inter, grid, lds, st) : launch_xt<XT_F16, false>(a, inter, grid, lds, st)
-                   : v ? launch_xt<XT_BF16, true>(a, inter, grid, lds, st) : launch_xt<XT_BF16, false>(a, inter, grid, lds, st);
+    const int rc = xt == XT_F32   ? launch_vec<XT_F32>(a, v, inter, grid, lds, st)
+                   : xt == XT_F16 ? launch_vec<XT_F16>(a, v, inter, grid, lds, st)
+                                  : launch_vec<XT_BF16>(a, v, inter, grid, lds, st);
     if (rc) return rc;
   }
   return 0;

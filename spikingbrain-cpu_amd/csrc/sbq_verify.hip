@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
   // (without a refusal the two are equal; nothing left after one: p itself)
   const bool use = total_left > 0.0 || total_left != total_left;
   const double total = use ? total_left : total_all, want = (double)a.u[b * (a.T + 1) + a.T] * total;
-  if (threadIdx.x == 0) hit = -1;
+  if (threadIdx.x == 0) hit = -1, found = INT32_MAX, last = -1;
   __syncthreads();
   if (!(total > 0.0 && total < __builtin_inf())) {  // (NaN too)
     if (threadIdx.x == 0) a.token[b] = -1;
@@ -208,30 +208,44 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
     at += use ? part[s].x : part[s].y;
   }
   __syncthreads();
+  // a thread's share of it: neighbours, so that one scan over the threads gives every prefix
   const VerRow r = row_of<XT>(a, b, n, kept);
-  double base = seg_before;
-  if (threadIdx.x == 0) found = INT32_MAX, last = -1;
-  for (int k = 0; k < kVerSeg / kVerPart; ++k) {
-    const int64_t i = (int64_t)seg * kVerSeg + k * kVerPart + threadIdx.x * 4;
-    double l[4], w[4], m[4], sum;
-    masses<XT, VEC>(r, i, a.V, l, w);
+  constexpr int kEach = kVerSeg / kVerThreads;
+  const int64_t i0 = (int64_t)seg * kVerSeg + threadIdx.x * kEach;
+  double m[kEach], sum = 0.0, total_seg;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = use ? l[j] : w[j];
-    double at = base + block_before((m[0] + m[1]) + (m[2] + m[3]), lds, &sum);
+  for (int k = 0; k < kEach; k += 4) {
+    double l[4], w[4];
+    masses<XT, VEC>(r, i0 + k, a.V, l, w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      at += m[j];
-      const int i_in = k * kVerPart + (int)threadIdx.x * 4 + j;
-      if (m[j] > 0.0) {
-        if (at > want) atomicMin(&found, i_in);
-        atomicMax(&last, i_in);
-      }
+      m[k + j] = use ? l[j] : w[j];
+      sum += m[k + j];
     }
-    base += sum;
+  }
+  at = seg_before + block_before(sum, lds, &total_seg);
+  // the first thread whose prefix passes `want`; sums in another order can end a
+  // rounding below it: then the last one with mass
+  const int lane = threadIdx.x & 63;
+  const uint64_t past = __ballot(at + sum > want && sum > 0.0), some = __ballot(sum > 0.0);
+  if (lane == 0) {
+    if (past) atomicMin(&found, (int)threadIdx.x + __builtin_ctzll(past));
+    if (some) atomicMax(&last, (int)threadIdx.x + 63 - __builtin_clzll(some));
   }
   __syncthreads();
-  // (sums in another order can end a rounding below `want`: then the segment's last token with mass)
-  if (threadIdx.x == 0) a.token[b] = (int64_t)seg * kVerSeg + (found != INT32_MAX ? found : last);
+  if ((int)threadIdx.x == (found != INT32_MAX ? found : last)) {
+    int64_t token = -1;
+    bool done = false;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      at += m[j];
+      if (m[j] > 0.0 && !done) {
+        token = i0 + j;
+        done = at > want;
+      }
+    }
+    a.token[b] = token;
+  }
 }
 
 template <int XT, bool VEC>
