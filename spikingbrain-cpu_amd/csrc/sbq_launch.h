@@ -327,7 +327,7 @@ struct PagedStore {
   void *k_out, *v_out;
   int64_t T, n_sb, n_st, n_sh;
   int ct, xt;
-  int lanes, parts;  // lanes of a vector, workgroups of a sequence, and what follows: the launcher's
+  int lanes, tile, parts;  // lanes of a vector, tokens of a tile, workgroups of a sequence, and what follows: the launcher's
   bool vec, set_length;
 };
 int launch_paged_append(const PagedStore& c, hipStream_t st);

@@ -74,7 +74,8 @@ struct PagedArgs {
   float2* part_ml;  // [Hk][places][R]
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
   int T, rep, qt;
-  int n, slots_log, places;  // sequences of the launch, workgroups of a key head and row tile, and both
+  int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile, and both
+  float per_slot;        // 1 / slots
   float scale;               // times log2(e)
   bool ovec;
 };
@@ -84,12 +85,18 @@ struct PagedArgs {
 struct PagedSpan {
   int64_t start;
   int count, held;
-  __device__ __forceinline__ PagedSpan(const PagedArgs& a, int64_t b) {
-    const int64_t room = (int64_t)a.c.max_pages << a.c.page_log, len = a.c.length[b];
+  // UNIFORM: the same sequence in every lane
+  template <bool UNIFORM>
+  __device__ __forceinline__ void of(const PagedArgs& a, int64_t b) {
+    auto load = [&](const int64_t* p) { return UNIFORM ? uniform_load(p + b) : p[b]; };
+    const int64_t room = (int64_t)a.c.max_pages << a.c.page_log, len = load(a.c.length);
     count = a.T;
-    if (a.counts) count = (int)paged_count(a.counts, b, a.T);
+    if (a.counts) {
+      const int64_t n = load(a.counts);
+      count = (int)(n < 0 ? 0 : n < a.T ? n : a.T);
+    }
     start = len - count;
-    if (a.start) start = min(max(a.start[b], -((int64_t)1 << 40)), (int64_t)1 << 40);  // (past every position)
+    if (a.start) start = min(max(load(a.start), -((int64_t)1 << 40)), (int64_t)1 << 40);  // (past every position)
     held = (int)(len < 0 ? 0 : len < room ? len : room);
   }
   __device__ __forceinline__ int last(int t) const {
@@ -114,8 +121,8 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// How the slots, 1 << slots_log workgroups of a key head and row tile, share a
-// launch's sequences.  All sequences' blocks, one sequence after another and
+// How the slots, the workgroups of a key head and row tile, share a launch's
+// sequences.  All sequences' blocks, one sequence after another and
 // each in whole fours (one block for each wave), are cut into equal parts of
 // four blocks or more, one for each slot: a long sequence among short ones has
 // as much of the chip as its length asks for, whatever the host knows of
@@ -128,15 +135,19 @@ struct PagedPlace {
   int before, own;      // the parts' blocks before it, and its own
   int each, total;      // a part's, and all
 };
+template <bool UNIFORM>
 __device__ __forceinline__ void paged_look(const PagedArgs& a, int b, int t0, int t1, int SB, PagedPlace& p) {
-  const PagedSpan span(a, a.first + b);
+  PagedSpan span;
+  span.of<UNIFORM>(a, a.first + b);
   const int lo = span.first(t0, a.window), hi = span.count > t0 ? span.last(min(t1, span.count - 1)) : -1;
   p.from = lo / SB;
   p.blocks = hi >= lo ? hi / SB + 1 - p.from : 0;
   p.own = max(kAttnWaves, (p.blocks + kAttnWaves - 1) & ~(kAttnWaves - 1));
 }
 __device__ __forceinline__ void paged_cut(const PagedArgs& a, PagedPlace& p) {
-  p.each = max(kAttnWaves, (p.total + (1 << a.slots_log) - 1) >> a.slots_log);
+  int n = (int)((float)p.total * a.per_slot);  // (within a few blocks: rounded to 24 bits)
+  while ((int64_t)n * a.slots < p.total) ++n;
+  p.each = max(kAttnWaves, n);
 }
 // BY_SLOT: the sequence that slot `key`'s part begins in, else sequence `key`.
 // t0, t1: the row tile's first and last token.
@@ -145,7 +156,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
   PagedPlace p;
   p.before = 0;
   if (a.n == 1) {
-    paged_look(a, 0, t0, t1, SB, p);
+    paged_look<true>(a, 0, t0, t1, SB, p);
     p.total = p.own;
     paged_cut(a, p);
     p.b = BY_SLOT && key * p.each >= p.total ? 1 : 0;
@@ -155,7 +166,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
   PagedPlace l;
   int sum;
   auto look = [&](int b0) {
-    paged_look(a, min(b0 + lane, a.n - 1), t0, t1, SB, l);
+    paged_look<false>(a, min(b0 + lane, a.n - 1), t0, t1, SB, l);
     if (b0 + lane >= a.n) l.own = 0;
     sum = wave_scan(l.own);
   };
@@ -249,10 +260,15 @@ struct Pair {
   }
 };
 
+// Workgroups of a CU that the registers are bounded for.
+constexpr int paged_occupancy(int ct, int qt, int DP) {
+  return DP == 256 ? is_8bit(ct) && qt != XT_F32 ? 2 : 1 : DP == 128 ? 2 : 3;
+}
+
 // CT: the cache's type, QT: the queries', DP: columns the registers hold (64,
 // 128, 256), EXACT: row == DP.  Grid: key heads x slots x row tiles.
 template <int CT, int QT, int DP, bool EXACT>
-__global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void paged_attn_kernel(PagedArgs a) {
   constexpr bool B8 = is_8bit(CT), F32 = CT == XT_F32, WIDE = QT == XT_F32 && !F32;
   // pieces of a query and of a weight
   constexpr int NQ = !WIDE ? 1 : CT == XT_BF16 ? 3 : 2, NP = WIDE ? NQ : CT == XT_BF16 || QT == XT_F16 ? 2 : 1;
@@ -291,7 +307,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
       const uint32_t row_bytes = pc.row * ES, k_lane = c * row_bytes + g * 16, v_lane = 4 * g * row_bytes + c * EV * ES;
       const int64_t head_bytes = (int64_t)row_bytes << pc.page_log;
       const int64_t b = a.first + p.b;
-      const PagedSpan span(a, b);
+      PagedSpan span;
+      span.of<true>(a, b);
       const int lo = span.first(tok, a.window), hi = span.last(tok);
       // what every row that sees anything sees
       int lo_max = hi < lo ? 0 : lo, hi_min = hi < lo ? INT32_MAX : hi;
@@ -304,6 +321,64 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
       }
       lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
 
+      // A block's keys and values, straight to registers.  The next block's follow as
+      // soon as this one's are used, so that they are on their way meanwhile; the
+      // first one's go ahead of the queries.
+      KV kf[SUB][NCH];
+      VW vf[4 * SUB][DB];
+      f32x4 ks[B8 ? SUB : 1], vs[B8 ? SUB : 1];
+      uint32_t held_k = 0;  // sixteens whose page is there
+      const int32_t* const table = pc.table + b * pc.max_pages;
+      int32_t ids[SUB], ids_v[SUB];
+      auto look_up = [&](int n) {  // (past the table's last page: past the length too, whichever page is read)
+#pragma unroll
+        for (int st = 0; st < SUB; ++st)
+          ids[st] = uniform_load(table + min(((p.from + n) * SB + st * 16) >> pc.page_log, pc.max_pages - 1));
+      };
+      auto load_k = [&](int n) {
+        held_k = 0;
+#pragma unroll
+        for (int st = 0; st < SUB; ++st) {
+          if (valid_page(pc, ids[st])) held_k |= 1u << st;
+          ids_v[st] = valid_page(pc, ids[st]) ? ids[st] : 0;
+          const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
+          const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
+          const char* const kp = (const char*)pc.k + block * head_bytes + in_page * row_bytes;
+#pragma unroll
+          for (int ch = 0; ch < NCH; ++ch) {
+            if (EXACT || ch * 4 * E + g * E < pc.row)
+              kf[st][ch] = *(const KV*)(kp + (k_lane + ch * 64));
+            else
+              kf[st][ch] = (KV)(0u);
+          }
+          if constexpr (B8) ks[st] = *(const f32x4*)(pc.k_scale + (block << pc.page_log) + in_page + 4 * g);
+        }
+      };
+      auto load_v = [&](int n) {
+#pragma unroll
+        for (int st = 0; st < SUB; ++st) {
+          const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
+          const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
+          const char* const vp = (const char*)pc.v + block * head_bytes + in_page * row_bytes;
+          if constexpr (B8) vs[st] = *(const f32x4*)(pc.v_scale + (block << pc.page_log) + in_page + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              if (EXACT || db * 16 * EV + c * EV < pc.row)
+                vf[st * 4 + j][db] = *(const VW*)(vp + (v_lane + j * row_bytes + db * 16 * EV * ES));
+              else
+                vf[st * 4 + j][db] = (VW)(0u);
+            }
+        }
+      };
+      if (n0 + w < n1) {
+        look_up(n0 + w);
+        load_k(n0 + w);
+        load_v(n0 + w);
+        look_up(min(n0 + w + kAttnWaves, n1 - 1));
+      }
+
       // the rows of Q by all threads to LDS, and the lane's share of its own
       MV qm[F32 ? 1 : NFR][NQ];
       f32x4 qf[F32 ? NCH : 1];
@@ -312,21 +387,23 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
         typedef typename XElem<QT>::T T;
         constexpr int LD = DP + 4, STEP = kAttnWaves * 64 / DP;
         const int d = tid & (DP - 1), rows = min(R - row0, 16);
-        int r = tid / DP, t = t0, h = row0 - t0 * a.rep + r;
-        const T* const q = (const T*)a.q + b * a.q_sb + (int64_t)kvh * a.rep * a.q_sh + d;
+        const T* const q = (const T*)a.q + b * a.q_sb + (int64_t)kvh * a.rep * a.q_sh + min(d, pc.D - 1);
         __syncthreads();  // (LDS is free of the last sequence)
 #pragma unroll 1
-        for (; r < rows; r += 4 * STEP) {  // four loads at a time
+        for (int r = tid / DP; r < rows; r += 4 * STEP) {  // four loads at a time
+          int tt[4] = {}, hh[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) hh[i] = min(row0 + r + i * STEP, R - 1);
+          if (a.T > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tt[i] = hh[i] / a.rep, hh[i] -= tt[i] * a.rep;
+          }
           T x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            while (h >= a.rep) h -= a.rep, ++t;
-            x[i] = d < pc.D && r + i * STEP < rows ? q[(int64_t)t * a.q_st + (int64_t)h * a.q_sh] : (T)0.0f;
-            h += STEP;
-          }
+          for (int i = 0; i < 4; ++i) x[i] = q[(int64_t)tt[i] * a.q_st + (int64_t)hh[i] * a.q_sh];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (r + i * STEP < rows) lds_o[(r + i * STEP) * LD + d] = (float)x[i];
+            if (r + i * STEP < rows) lds_o[(r + i * STEP) * LD + d] = d < pc.D ? (float)x[i] : 0.0f;
         }
         __syncthreads();
         const float* const mine = lds_o + (row - row0) * LD;
@@ -378,49 +455,10 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
       for (int f = 0; f < NF; ++f) o[f] = (f32x4)(0.0f);
       float m = kNone, l = 0.0f;
       float vref = 1.17549435e-38f;  // 8-bit: O's unit, the largest value scale that the row saw so far
-      const int32_t* const table = pc.table + b * pc.max_pages;
-
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {
         const int s0 = (p.from + n) * SB;
-        KV kf[SUB][NCH];
-        VW vf[4 * SUB][DB];
-        f32x4 ks[B8 ? SUB : 1], vs[B8 ? SUB : 1];
-        uint32_t held = 0;  // sixteens whose page is there
-#pragma unroll
-        for (int st = 0; st < SUB; ++st) {
-          const int s = s0 + st * 16, page = s >> pc.page_log;
-          int32_t id = page < pc.max_pages ? uniform_load(table + page) : -1;
-          if (valid_page(pc, id))
-            held |= 1u << st;
-          else
-            id = 0;
-          const int64_t block = (int64_t)id * pc.Hk + kvh;
-          const uint32_t in_page = s & page_mask;
-          const char* const kp = (const char*)pc.k + block * head_bytes + in_page * row_bytes;
-          const char* const vp = (const char*)pc.v + block * head_bytes + in_page * row_bytes;
-#pragma unroll
-          for (int ch = 0; ch < NCH; ++ch) {
-            if (EXACT || ch * 4 * E + g * E < pc.row)
-              kf[st][ch] = *(const KV*)(kp + (k_lane + ch * 64));
-            else
-              kf[st][ch] = (KV)(0u);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-              if (EXACT || db * 16 * EV + c * EV < pc.row)
-                vf[st * 4 + j][db] = *(const VW*)(vp + (v_lane + j * row_bytes + db * 16 * EV * ES));
-              else
-                vf[st * 4 + j][db] = (VW)(0u);
-            }
-          if constexpr (B8) {
-            const int64_t sc = (block << pc.page_log) + in_page;
-            ks[st] = *(const f32x4*)(pc.k_scale + sc + 4 * g);
-            vs[st] = *(const f32x4*)(pc.v_scale + sc + 4 * g);
-          }
-        }
+        const uint32_t held = held_k;
         const bool full = held == (1u << SUB) - 1 && s0 >= lo_max && s0 + SB - 1 <= hi_min;
 
         // scores, in powers of two
@@ -458,6 +496,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
 #pragma unroll
           for (int v = 0; v < 4; ++v) e[st][v] = s[v] * (B8 ? factor * ks[st][v] : factor);
         }
+        const bool more = n + kAttnWaves < n1;
+        if (more) load_k(n + kAttnWaves);
 
         uint32_t seen = ~0u;  // bit st * 4 + v: the lane's row sees that position
         if (!full) {
@@ -626,6 +666,10 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
             }
           }
         }
+        if (more) {
+          load_v(n + kAttnWaves);
+          look_up(min(n + 2 * kAttnWaves, n1 - 1));
+        }
       }
 
       // the workgroup's waves joined
@@ -687,7 +731,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, 2) void paged_attn_kernel(PagedArg
     p.before += p.own;
     if (p.before >= x1) break;
     ++p.b;
-    paged_look(a, p.b, t0, t1, SB, p);
+    paged_look<true>(a, p.b, t0, t1, SB, p);
   }
 }
 

@@ -11,14 +11,14 @@
 #include "sbq_paged.h"
 
 #include <algorithm>
-#include <stdlib.h>
 
 namespace sbq {
 
 namespace {
 
 constexpr int kStoreThreads = 256;
-constexpr int kStoreAlone = 256;  // vectors of a sequence that one workgroup stores by itself
+constexpr int kStoreAlone = 128;  // vectors of a sequence that one workgroup stores by itself
+constexpr int64_t kStoreGroups = 2048;  // workgroups of a launch at most
 
 // Largest code of an 8-bit type.
 template <int CT>
@@ -41,22 +41,41 @@ __device__ __forceinline__ void load_cols(const typename XElem<XT>::T* p, int n,
   }
 }
 
-// Eight codes of x / scale (scale 0 or NaN: zeros), the first in the low byte.
+// x / scale for eight values, as IEEE division rounds it: the steps of the
+// division itself (a refined reciprocal, then the quotient twice by its
+// remainder), the reciprocal once for all; where scale is too small or large
+// for them to stay in range, the division.
+__device__ __forceinline__ void quotients(const float (&x)[8], float scale, float (&q)[8]) {
+  if (scale > 0x1p-100f && scale < 0x1p100f) {
+    float r = __builtin_amdgcn_rcpf(scale);
+    r = __builtin_fmaf(__builtin_fmaf(-scale, r, 1.0f), r, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float q0 = x[j] * r, q1 = __builtin_fmaf(__builtin_fmaf(-q0, scale, x[j]), r, q0);
+      q[j] = __builtin_fmaf(__builtin_fmaf(-q1, scale, x[j]), r, q1);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = scale > 0.0f ? x[j] / scale : 0.0f;
+  }
+}
+
+// The nearest codes to eight quotients (scale 0 or NaN: zeros), the first in the low byte.
 template <int CT>
 __device__ __forceinline__ u32x2 codes(const float (&x)[8], float scale) {
-  const bool any = scale > 0.0f;
-  u32x2 w = {0u, 0u};
+  u32x2 w;
   float y[8];
+  quotients(x, scale, y);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float q = any ? x[j] / scale : 0.0f;
-    y[j] = __builtin_fminf(__builtin_fmaxf(q, -largest<CT>()), largest<CT>());  // (a subnormal scale's own rounding)
-  }
+  for (int j = 0; j < 8; ++j) y[j] = __builtin_amdgcn_fmed3f(y[j], -largest<CT>(), largest<CT>());  // (a subnormal scale's own rounding)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if constexpr (CT == CT_I8) {
+      uint32_t n[4];  // (an integer in the low bits, rounded to even by the addition)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[h] |= (uint32_t)((int)__builtin_rintf(y[4 * h + j]) & 255) << (8 * j);
+      for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(y[4 * h + j] + 12582912.0f);
+      w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(n[3], n[2], 0x0c0c0400u), __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0400u),
+                                   0x05040100u);
     } else {
       int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
       w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], v, true);
@@ -72,17 +91,12 @@ __device__ __forceinline__ void store_cols(const PagedCache& c, bool value, int6
                                            int lanes) {
   void* const pool = value ? c.v : c.k;
   if constexpr (is_8bit(CT)) {
-    float most = 0.0f;
-    bool odd = false;
+    uint32_t most = 0;  // the largest magnitude as an integer: infinities and NaN above every number
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      most = __builtin_fmaxf(most, __builtin_fabsf(x[j]));
-      odd |= !finite(x[j]);
-    }
-    if (odd) most = __builtin_inff();
-    for (int o = 1; o < lanes; o <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o, 64));
+    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+    for (int o = 1; o < lanes; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
     // (a vector with an infinity or NaN has no codes: it reads back as NaN)
-    const float scale = finite(most) ? most / largest<CT>() : __builtin_nanf("");
+    const float scale = most < 0x7f800000u ? __uint_as_float(most) / largest<CT>() : __builtin_nanf("");
     if (n <= 0) return;
     *(u32x2*)((uint8_t*)pool + at * c.row + d) = codes<CT>(x, scale);  // (columns past D: zeros again)
     if (d == 0) (value ? c.v_scale : c.k_scale)[at] = scale;
@@ -99,33 +113,68 @@ __device__ __forceinline__ int64_t paged_end(int64_t start, int64_t count, int64
   return start >= room ? room : start + count < room ? start + count : room;
 }
 
-// Rows [b][t][head][k or v], a group of `lanes` lanes each.  ALONE: one
-// workgroup a sequence, which moves the length itself after reading it.
+// Walks a sequence's vectors, `lanes` lanes each, in tiles of a workgroup's lane
+// groups: `tile` neighbouring tokens of a head, which stand side by side in a
+// page (as do their scales, that lines of either are written whole), and as
+// many heads as there are groups left.  U tiles at a time: `load` for all of
+// them, then `use`.
+template <int U, class L, class F>
+__device__ __forceinline__ void paged_walk(const PagedStore& a, int part, L load, F use) {
+  const int group = threadIdx.x / a.lanes, t_in = group & (a.tile - 1), h_in = group / a.tile;
+  const int heads = kStoreThreads / a.lanes / a.tile, across = (a.c.Hk + heads - 1) / heads;  // heads of a tile, tiles across them
+  const int tiles = (int)((a.T + a.tile - 1) / a.tile) * across;
+  for (int q0 = part; q0 < tiles; q0 += U * a.parts) {
+    int ts[U], hs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = q0 + u * a.parts, row = q / across;
+      ts[u] = row * a.tile + t_in, hs[u] = (q - row * across) * heads + h_in;
+      if (q >= tiles || hs[u] >= a.c.Hk) ts[u] = INT32_MAX;
+      load(u, ts[u], hs[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ts[u] < a.T) use(u, ts[u], hs[u]);
+  }
+}
+
+// The row of position pos and head h in the pool; -1: it has none.
+__device__ __forceinline__ int64_t paged_row(const PagedCache& c, int64_t b, int64_t pos, int h) {
+  const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
+  if (!valid_page(c, id)) return -1;
+  return (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1));
+}
+
 template <int CT, int XT, bool VEC>
 __global__ __launch_bounds__(kStoreThreads) void paged_append_kernel(PagedStore a) {
   typedef typename XElem<XT>::T T;
   const PagedCache& c = a.c;
-  const int lane = threadIdx.x & (a.lanes - 1), groups = kStoreThreads / a.lanes, d = lane * 8;
-  const int64_t b = blockIdx.x / a.parts, each = a.T * c.Hk * 2;
-  const int part = blockIdx.x % a.parts, n = c.D - d;
+  const int64_t b = blockIdx.x / a.parts, room = (int64_t)c.max_pages << c.page_log;
+  const int part = blockIdx.x % a.parts, d = (threadIdx.x & (a.lanes - 1)) * 8, n = c.D - d;
   const int64_t start = a.start[b], count = paged_count(a.counts, b, a.T);
-  const int64_t room = (int64_t)c.max_pages << c.page_log;
-  for (int64_t r = (int64_t)part * groups + threadIdx.x / a.lanes; r < each; r += (int64_t)groups * a.parts) {
-    const bool value = r & 1;
-    const int64_t th = r >> 1, t = th / c.Hk, h = th - t * c.Hk, pos = start + t;
-    // (the lanes of a vector go together; those past it keep up for the maximum)
-    if (t >= count || start < 0 || start >= room || pos >= room) continue;
-    const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
-    if (!valid_page(c, id)) continue;
-    float x[8];
-    load_cols<XT, VEC>((const T*)(value ? a.vn : a.kn) + b * a.n_sb + t * a.n_st + h * a.n_sh + d, n, x);
-    store_cols<CT>(c, value, (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1)), d, n, x, a.lanes);
-  }
+  constexpr int U = 2;
+  float k[U][8], v[U][8];
+  int64_t at[U];
+  paged_walk<U>(
+      a, part,
+      [&](int u, int t, int h) {
+        const int64_t pos = start + t;
+        at[u] = -1;
+        // (the lanes of a vector go together)
+        if (t >= count || start < 0 || start >= room || pos >= room) return;
+        const int64_t from = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
+        at[u] = paged_row(c, b, pos, h);
+        load_cols<XT, VEC>((const T*)a.kn + from, n, k[u]);
+        load_cols<XT, VEC>((const T*)a.vn + from, n, v[u]);
+      },
+      [&](int u, int, int) {
+        if (at[u] < 0) return;
+        store_cols<CT>(c, false, at[u], d, n, k[u], a.lanes);
+        store_cols<CT>(c, true, at[u], d, n, v[u], a.lanes);
+      });
   if (a.set_length && part == 0) {
     __syncthreads();  // (start may be the length itself, then with one workgroup a sequence)
-    if (threadIdx.x == 0) {
-      c.length[b] = paged_end(start, count, room);
-    }
+    if (threadIdx.x == 0) c.length[b] = paged_end(start, count, room);
   }
 }
 
@@ -163,24 +212,31 @@ __device__ __forceinline__ void read_cols(const PagedCache& c, bool value, int64
 template <int CT>
 __global__ __launch_bounds__(kStoreThreads) void paged_read_kernel(PagedStore a) {
   const PagedCache& c = a.c;
-  const int lane = threadIdx.x & (a.lanes - 1), groups = kStoreThreads / a.lanes, d = lane * 8, n = c.D - d;
-  const int64_t b = blockIdx.x / a.parts, each = a.T * c.Hk * 2, part = blockIdx.x % a.parts;
-  const int64_t start = a.start[b], room = (int64_t)c.max_pages << c.page_log, held = c.length[b] < room ? c.length[b] : room;
+  const int64_t b = blockIdx.x / a.parts, room = (int64_t)c.max_pages << c.page_log;
+  const int part = blockIdx.x % a.parts, d = (threadIdx.x & (a.lanes - 1)) * 8, n = c.D - d;
+  const int64_t start = a.start[b], held = c.length[b] < room ? c.length[b] : room;
   if (n <= 0) return;
-  for (int64_t r = part * groups + threadIdx.x / a.lanes; r < each; r += (int64_t)groups * a.parts) {
-    const bool value = r & 1;
-    const int64_t th = r >> 1, t = th / c.Hk, h = th - t * c.Hk, pos = start + t;
-    float x[8] = {};
-    if (pos >= 0 && pos < held) {
-      const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
-      if (valid_page(c, id))
-        read_cols<CT>(c, value, (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1)), d, x);
-    }
-    void* const out = value ? a.v_out : a.k_out;
-    const int64_t to = b * a.n_sb + t * a.n_st + h * a.n_sh + d;
-    store_y4(out, a.xt, to, (f32x4){x[0], x[1], x[2], x[3]}, a.vec && n >= 4, n);
-    store_y4(out, a.xt, to + 4, (f32x4){x[4], x[5], x[6], x[7]}, a.vec && n >= 8, n - 4);
-  }
+  constexpr int U = 2;
+  float k[U][8], v[U][8];
+  paged_walk<U>(
+      a, part,
+      [&](int u, int t, int h) {
+        const int64_t pos = start + t;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[u][j] = v[u][j] = 0.0f;
+        if (t >= a.T || pos < 0 || pos >= held) return;
+        const int64_t at = paged_row(c, b, pos, h);
+        if (at < 0) return;
+        read_cols<CT>(c, false, at, d, k[u]);
+        read_cols<CT>(c, true, at, d, v[u]);
+      },
+      [&](int u, int t, int h) {
+        const int64_t to = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
+        store_y4(a.k_out, a.xt, to, (f32x4){k[u][0], k[u][1], k[u][2], k[u][3]}, a.vec && n >= 4, n);
+        store_y4(a.k_out, a.xt, to + 4, (f32x4){k[u][4], k[u][5], k[u][6], k[u][7]}, a.vec && n >= 8, n - 4);
+        store_y4(a.v_out, a.xt, to, (f32x4){v[u][0], v[u][1], v[u][2], v[u][3]}, a.vec && n >= 4, n);
+        store_y4(a.v_out, a.xt, to + 4, (f32x4){v[u][4], v[u][5], v[u][6], v[u][7]}, a.vec && n >= 8, n - 4);
+      });
 }
 
 template <int CT, int XT>
@@ -208,8 +264,11 @@ int launch_read_ct(const PagedStore& a, unsigned grid, hipStream_t st) {
 void plan(PagedStore& a) {
   a.lanes = 1;
   while (a.lanes * 8 < a.c.D) a.lanes <<= 1;
-  const int64_t groups = kStoreThreads / a.lanes, each = a.T * a.c.Hk * 2;
-  const int64_t want = (each + groups - 1) / groups, room = std::max<int64_t>(1, 4096 / a.c.B);
+  const int64_t groups = kStoreThreads / a.lanes;
+  a.tile = 1;
+  while (a.tile < groups && a.tile < a.T) a.tile <<= 1;
+  const int64_t heads = groups / a.tile, want = (a.T + a.tile - 1) / a.tile * ((a.c.Hk + heads - 1) / heads);
+  const int64_t room = std::max<int64_t>(1, kStoreGroups / a.c.B);
   a.parts = (int)std::max<int64_t>(1, std::min(want, room));
 }
 
@@ -230,7 +289,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   const int used = paged_places(p, place);
   if (used == 1) return;  // (written by the one workgroup)
   const int64_t b = a.first + p.b, at = ((int64_t)kvh * a.places + place) * R + r;
-  const PagedSpan span(a, b);
+  PagedSpan span;
+  span.of<true>(a, b);
   const float2* const ml = a.part_ml + at;
   float top = -__builtin_inff();
   for (int s = lane; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
@@ -272,18 +332,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
 
-static int64_t paged_groups() { const char* e = getenv("PG"); return e ? atoi(e) : 1024; }
 constexpr int64_t kPagedGroup = 512;  // sequences of a launch at most (each workgroup scans their lengths)
 
 struct PagedPlan {
-  int DP, SB, slots_log;
-  int64_t rtiles, n, places;
+  int DP, SB;
+  int64_t rtiles, n, slots, places;
   bool joins;  // can a sequence need more than one slot?
 };
 // How many workgroups there are goes by the table's room: how much of it is
 // filled is known on the device alone, where workgroups without a part leave
 // at once.
-PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, int ct) {
+PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, int ct, bool wide) {
   PagedPlan p;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   p.SB = ct == XT_F32 ? 16 : 32;
@@ -291,9 +350,9 @@ PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, 
   const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB, fours = (blocks + kAttnWaves - 1) / kAttnWaves;
   p.n = std::min(B, kPagedGroup);
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 30) / (fours * kAttnWaves)));  // (all blocks fit an int)
-  p.slots_log = 0;
-  while ((one << (p.slots_log + 1)) <= paged_groups() && ((int64_t)1 << p.slots_log) < p.n * fours) ++p.slots_log;
-  p.places = ((int64_t)1 << p.slots_log) + p.n;
+  const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
+  p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
+  p.places = p.slots + p.n;
   p.joins = fours > 1;
   return p;
 }
@@ -304,19 +363,22 @@ int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct) {
   const int64_t R = heads / Hk * T;
-  const PagedPlan p = paged_plan(B, R, Hk, D, room, ct);
-  if (!p.joins) return 0;
-  const int64_t parts = Hk * R * p.places;
-  return round256(parts * p.DP * 4) + round256(parts * 8);
+  int64_t n = 0;
+  for (bool wide : {false, true}) {  // (the queries' type is not known here)
+    const PagedPlan p = paged_plan(B, R, Hk, D, room, ct, wide);
+    const int64_t parts = Hk * R * p.places;
+    if (p.joins) n = std::max(n, round256(parts * p.DP * 4) + round256(parts * 8));
+  }
+  return n;
 }
 
 int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   const int64_t Hk = c.c.Hk, rep = c.heads / Hk, R = rep * c.T, B = c.c.B;
-  const PagedPlan p = paged_plan(B, R, Hk, c.c.D, (int64_t)c.c.max_pages << c.c.page_log, c.ct);
+  const PagedPlan p = paged_plan(B, R, Hk, c.c.D, (int64_t)c.c.max_pages << c.c.page_log, c.ct, c.qt == XT_F32);
   PagedArgs a{};
   a.c = c.c, a.q = c.q, a.start = c.start, a.counts = c.counts, a.out = c.out;
   a.q_sb = c.q_sb, a.q_st = c.q_st, a.q_sh = c.q_sh, a.o_sb = c.o_sb, a.o_st = c.o_st, a.o_sh = c.o_sh;
-  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots_log = p.slots_log;
+  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots = (int)p.slots, a.per_slot = 1.0f / (float)p.slots;
   a.places = (int)p.places;
   a.scale = c.scale * 1.44269504f;
   const int64_t eq = c.qt == XT_F32 ? 4 : 2;
@@ -327,7 +389,7 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   }
   for (a.first = 0; a.first < B; a.first += p.n) {
     a.n = (int)std::min(p.n, B - a.first);
-    const dim3 grid((unsigned)Hk, 1u << p.slots_log, (unsigned)p.rtiles);
+    const dim3 grid((unsigned)Hk, (unsigned)p.slots, (unsigned)p.rtiles);
     int rc = c.ct == XT_F32    ? launch_paged_attn_f32(a, p.DP, grid, st)
              : c.ct == XT_F16  ? launch_paged_attn_f16(a, p.DP, grid, st)
              : c.ct == XT_BF16 ? launch_paged_attn_bf16(a, p.DP, grid, st)
@@ -354,7 +416,7 @@ int launch_paged_append(const PagedStore& c, hipStream_t st) {
   auto vec = [&](const void* p) { return (uintptr_t)p % 16 == 0; };
   a.vec = a.c.D % 8 == 0 && vec(a.kn) && vec(a.vn) && a.n_sb * es % 16 == 0 && a.n_st * es % 16 == 0 && a.n_sh * es % 16 == 0;
   const bool own = a.start == a.c.length;  // the length is read by every workgroup: moved by one that no other reads after
-  if (own && a.T * a.c.Hk * 2 <= kStoreAlone) a.parts = 1;
+  if (own && a.T * a.c.Hk <= kStoreAlone) a.parts = 1;
   a.set_length = !own || a.parts == 1;
   const int64_t B = a.c.B, most = std::max<int64_t>(1, kLaunchThreads / kStoreThreads / a.parts);
   for (int64_t b0 = 0; b0 < B; b0 += most) {

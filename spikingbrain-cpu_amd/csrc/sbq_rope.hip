@@ -13,6 +13,8 @@
 // The angle's product is exact and reduced in 64 bits: at position 131072 an
 // fp32 product is off by up to 2^-8 of a radian.  The cosines of a workgroup's
 // tokens are computed once, a pair a thread, and kept in LDS for all heads.
+#include <algorithm>
+
 #include "sbq_common.h"
 #include "sbq_launch.h"
 
@@ -20,7 +22,9 @@ namespace sbq {
 
 namespace {
 
-constexpr int kRopeThreads = 256, kRopeTokens = 4;  // threads, and at most so many tokens a workgroup
+// Threads, and at most so many tokens a workgroup (from 1024 workgroups on: 8192
+// tokens of 40 x 128 bf16 columns at 2, 4, 8, 16 tokens each take 55, 44, 41, 47 us).
+constexpr int kRopeThreads = 256, kRopeTokens = 8;
 
 // cos and sin of pos * f.  The product as a sum of two doubles, its distance
 // from the nearest quarter turn (pi / 2 in two doubles), then the Taylor series
@@ -229,7 +233,7 @@ int launch_rope(const RopeArgs& c, bool inter, int xt, hipStream_t st) {
   a.lanes = 1;
   while (a.lanes < items) a.lanes <<= 1;
   const int groups = kRopeThreads / a.lanes;
-  a.tokens = a.T >= 1024 ? kRopeTokens : 1;
+  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kRopeTokens, a.T / 1024));
   // few tokens: a vector a lane group, on as many workgroups as that takes
   a.parts = a.T < 512 ? (a.rows + groups - 1) / groups : 1;
   const size_t lds = (size_t)a.tokens * ((a.pairs + N - 1) / N) * N * sizeof(float2);

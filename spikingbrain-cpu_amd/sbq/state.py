@@ -30,6 +30,7 @@ one call, so that no key a query of that call sees is overwritten.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass, field
 
 import torch
@@ -169,54 +170,58 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     // (tokens / n)] + t % (tokens / n), so [tokens] gives each its own and the
     starts of n sequences are enough for their next tokens.  q_out, k_out: q and
     k themselves, or tensors apart from both (default: new ones)."""
-    gpu, dtype = q.get_device(), q.dtype
+    gpu, dtype, shape, device = q.get_device(), q.dtype, q.shape, q.device
     if gpu < 0:
         raise ValueError("qk_norm_rope: q must be a GPU tensor")
-    if dtype not in _DTYPE_CODE:
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
         raise ValueError(f"qk_norm_rope: unsupported dtype {dtype}; expected float32, float16 or bfloat16")
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]
-                                           or k.dtype != dtype or k.get_device() != gpu)):
+    if len(shape) != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2]
+                                              or k.dtype != dtype or k.get_device() != gpu)):
         raise ValueError("qk_norm_rope: expected q [tokens, heads, dim] and k [tokens, kv_heads, dim] of one dtype on one GPU")
-    tokens, heads, dim = q.shape
-    n = positions.numel()
+    tokens, heads, dim = shape
+    n, pairs = positions.numel(), inv_freq.numel()
     if positions.dtype != torch.int64 or positions.get_device() != gpu or not positions.is_contiguous() \
             or (tokens % n if n else tokens):
-        raise ValueError(f"qk_norm_rope: positions must be a contiguous int64 tensor on {q.device} whose size divides {tokens} "
+        raise ValueError(f"qk_norm_rope: positions must be a contiguous int64 tensor on {device} whose size divides {tokens} "
                          "tokens")
-    if (inv_freq.dtype != torch.float32 or inv_freq.get_device() != gpu or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
-            or 2 * inv_freq.numel() > dim or dim > 256):
-        raise ValueError(f"qk_norm_rope: inv_freq must be a contiguous float32 tensor on {q.device} of at most dim / 2 entries, "
+    if (inv_freq.dtype != torch.float32 or inv_freq.get_device() != gpu or not inv_freq.is_contiguous()
+            or 2 * pairs > dim or dim > 256):
+        raise ValueError(f"qk_norm_rope: inv_freq must be a contiguous float32 tensor on {device} of at most dim / 2 entries, "
                          "dim at most 256")
-    wt = None
-    for w in (q_weight, k_weight):
+    wt, w_at = None, [None, None]
+    for i, w in enumerate((q_weight, k_weight)):
         if w is not None:
-            if w.shape != (dim,) or w.get_device() != gpu or not w.is_contiguous() or w.dtype not in _DTYPE_CODE:
-                raise ValueError(f"qk_norm_rope: weights must be contiguous float [{dim}] tensors on {q.device}")
-            if wt is not None and w.dtype != wt:
-                raise ValueError("qk_norm_rope: q_weight and k_weight must share a dtype")
-            wt = w.dtype
-    outs = []
-    for name, x, out in (("q_out", q, q_out), ("k_out", k, k_out)):
-        if out is None:
-            out = None if x is None else torch.empty(x.shape, dtype=dtype, device=q.device)
-        elif (x is None or out.shape != x.shape or out.dtype != dtype or out.get_device() != gpu
-              or (dim > 1 and out.stride(2) != 1) or (out.data_ptr() == x.data_ptr() and out.stride() != x.stride())):
-            raise ValueError(f"qk_norm_rope: {name} must have its input's shape, dtype and device, with unit stride in dim")
-        outs.append(out)
+            if w.numel() != dim or w.get_device() != gpu or not w.is_contiguous() or wt not in (None, w.dtype) \
+                    or w.dtype not in _DTYPE_CODE:
+                raise ValueError(f"qk_norm_rope: weights must be contiguous [{dim}] tensors of one float dtype on {device}")
+            wt, w_at[i] = w.dtype, w.data_ptr()
+    if tokens and dim > 1:
+        q, k = _rows_of(q), None if k is None else _rows_of(k)
+    qs, ks = q.stride(), (0, 0) if k is None else k.stride()
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dtype, device=device)
+    elif q_out.shape != shape or q_out.dtype != dtype or q_out.get_device() != gpu or (dim > 1 and q_out.stride(2) != 1) \
+            or (q_out.data_ptr() == q.data_ptr() and q_out.stride() != qs):
+        raise ValueError("qk_norm_rope: q_out must have q's shape, dtype and device, with unit stride in dim")
+    if k is None:
+        if k_out is not None:
+            raise ValueError("qk_norm_rope: k_out needs k")
+    elif k_out is None:
+        k_out = torch.empty(k.shape, dtype=dtype, device=device)
+    elif k_out.shape != k.shape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1) \
+            or (k_out.data_ptr() == k.data_ptr() and k_out.stride() != ks):
+        raise ValueError("qk_norm_rope: k_out must have k's shape, dtype and device, with unit stride in dim")
     if tokens == 0:
-        return outs[0], outs[1]
-    q = _rows_of(q)
-    k = None if k is None else _rows_of(k)
-    qs, qo = q.stride(), outs[0].stride()
-    ks, ko = ((0, 0), (0, 0)) if k is None else (k.stride(), outs[1].stride())
-    with _on_device(q.device):
+        return q_out, k_out
+    qo, ko = q_out.stride(), (0, 0) if k is None else k_out.stride()
+    with _on_device(device):
         _lib.check(_lib.load().sbq_qk_norm_rope(
-            q.data_ptr(), None if k is None else k.data_ptr(), _DTYPE_CODE[dtype], tokens, heads, 0 if k is None else k.shape[1],
-            dim, qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), tokens // n, inv_freq.data_ptr(), inv_freq.numel(),
-            int(interleaved), None if q_weight is None else q_weight.data_ptr(),
-            None if k_weight is None else k_weight.data_ptr(), 0 if wt is None else _DTYPE_CODE[wt], eps, outs[0].data_ptr(),
-            None if k is None else outs[1].data_ptr(), qo[0], qo[1], ko[0], ko[1], _stream(q.device)), "sbq_qk_norm_rope")
-    return outs[0], outs[1]
+            q.data_ptr(), None if k is None else k.data_ptr(), code, tokens, heads, 0 if k is None else k.shape[1], dim, qs[0],
+            qs[1], ks[0], ks[1], positions.data_ptr(), tokens // n, inv_freq.data_ptr(), pairs, int(interleaved), w_at[0], w_at[1],
+            0 if wt is None else _DTYPE_CODE[wt], eps, q_out.data_ptr(), None if k is None else k_out.data_ptr(), qo[0], qo[1],
+            ko[0], ko[1], _stream(device)), "sbq_qk_norm_rope")
+    return q_out, k_out
 
 
 class DeviceKVBuffer:
@@ -411,6 +416,11 @@ class DeviceBudgetKVBuffer(DeviceKVBuffer):
 _CACHE_CODE = {**_DTYPE_CODE, torch.int8: _lib.SBQ_I8, torch.float8_e4m3fn: _lib.SBQ_E4M3}
 
 
+@functools.lru_cache(maxsize=256)
+def _paged_workspace_bytes(*sizes: int) -> int:
+    return _lib.load().sbq_paged_attn_workspace_bytes(*sizes)
+
+
 class DevicePagedKVBuffer:
     """Keys and values of several sequences in pages of one pool, for a step
     that runs all of them at once.  No counterpart in the reference, whose
@@ -445,6 +455,7 @@ class DevicePagedKVBuffer:
         if window is not None and window < 1:
             raise ValueError("DevicePagedKVBuffer: window must be >= 1")
         self.sequences, self.heads, self.dim, self.page, self.window = sequences, heads, dim, page, window
+        self._tensors: dict[str, torch.Tensor | None] = {}
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         row, b8 = -(-dim // 16) * 16, dtype in (torch.int8, torch.float8_e4m3fn)
         self.k = torch.zeros(pages, heads, page, row, dtype=dtype, device=dev)[..., :dim]
@@ -456,6 +467,18 @@ class DevicePagedKVBuffer:
         self._free = list(range(pages - 1, -1, -1))
         self._held: list[dict[int, int]] = [{} for _ in range(sequences)]  # page of the sequence -> page of the pool
         self._first = [0] * sequences  # pages of the sequence before this one were given back
+
+    # The pool's tensors may be replaced (a caller's own memory); they are checked when that happens.
+    k = property(lambda self: self._tensors["k"], lambda self, t: self._replace("k", t))
+    v = property(lambda self: self._tensors["v"], lambda self, t: self._replace("v", t))
+    k_scale = property(lambda self: self._tensors["k_scale"], lambda self, t: self._replace("k_scale", t))
+    v_scale = property(lambda self: self._tensors["v_scale"], lambda self, t: self._replace("v_scale", t))
+    table = property(lambda self: self._tensors["table"], lambda self, t: self._replace("table", t))
+    length = property(lambda self: self._tensors["length"], lambda self, t: self._replace("length", t))
+
+    def _replace(self, name: str, t: torch.Tensor | None) -> None:
+        self._tensors[name] = t
+        self._sizes = None  # to be checked again
 
     @property
     def device(self) -> torch.device:
@@ -509,38 +532,46 @@ class DevicePagedKVBuffer:
         self.table.fill_(-1)
         self.length.zero_()
 
+    def _check(self) -> tuple:
+        """(cache type, pages, page, heads, dim, max_pages) of the pool, once its tensors fit each other."""
+        k, v, table, length = self.k, self.v, self.table, self.length
+        dev, code, n = k.device, _CACHE_CODE.get(k.dtype), self.sequences
+        row = -(-self.dim // 16) * 16
+        strides = (self.heads * self.page * row, self.page * row, row)
+        if not k.is_cuda:
+            raise ValueError("DevicePagedKVBuffer: the buffer must be on a GPU")
+        if code is None or k.dim() != 4 or any(
+                t.shape != k.shape or t.shape[1:] != (self.heads, self.page, self.dim) or t.dtype != k.dtype or t.device != dev
+                or t.stride()[:3] != strides or (self.dim > 1 and t.stride(3) != 1) for t in (k, v)):
+            raise ValueError(f"DevicePagedKVBuffer: k and v must be [pages, {self.heads}, {self.page}, {self.dim}] of one cache "
+                             f"dtype, in rows of {row}, on one GPU")
+        if code >= _lib.SBQ_I8:
+            for s in (self.k_scale, self.v_scale):
+                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.device != dev or not s.is_contiguous():
+                    raise ValueError("DevicePagedKVBuffer: k_scale and v_scale must be contiguous float32 [pages, heads, page]")
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n or not table.is_contiguous() \
+                or table.device != dev or length.dtype != torch.int64 or length.shape != (n,) \
+                or not length.is_contiguous() or length.device != dev:
+            raise ValueError(f"DevicePagedKVBuffer: table must be int32 [{n}, max_pages] and length int64 [{n}], contiguous")
+        self._sizes = (code, k.shape[0], self.page, self.heads, self.dim, table.shape[1])
+        self._dev, self._gpu, self._b8 = dev, k.get_device(), code >= _lib.SBQ_I8
+        self._bytes = k.shape[0] * strides[0] * k.element_size()
+        return self._sizes
+
     def _cache(self, fn: str, sequence: int | None) -> tuple:
         """The C ABI's description of the cache (of one sequence's row), from k to length."""
-        k, v, ks, vs, table, length = self.k, self.v, self.k_scale, self.v_scale, self.table, self.length
-        gpu, code, d, page = k.get_device(), _CACHE_CODE.get(k.dtype), self.dim, self.page
-        row = -(-d // 16) * 16
-        strides = (self.heads * page * row, page * row, row, 1)
-        if gpu < 0 or code is None or k.dim() != 4 or k.shape[1:] != (self.heads, page, d) or v.shape != k.shape \
-                or v.dtype != k.dtype or v.get_device() != gpu or k.stride()[:3] != strides[:3] or v.stride()[:3] != strides[:3]:
-            raise ValueError(f"DevicePagedKVBuffer.{fn}: k and v must be the buffer's pool on one GPU")
-        if code >= _lib.SBQ_I8:
-            for s in (ks, vs):
-                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.get_device() != gpu \
-                        or not s.is_contiguous():
-                    raise ValueError(f"DevicePagedKVBuffer.{fn}: k_scale and v_scale must be the buffer's scales")
-            ks, vs = ks.data_ptr(), vs.data_ptr()
-        else:
-            ks = vs = None
-        n = self.sequences
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n or not table.is_contiguous() \
-                or table.get_device() != gpu or length.dtype != torch.int64 or length.shape != (n,) \
-                or not length.is_contiguous() or length.get_device() != gpu:
-            raise ValueError(f"DevicePagedKVBuffer.{fn}: table must be int32 [{n}, max_pages] and length int64 [{n}]")
-        width = table.shape[1]
-        at = 0 if sequence is None else self._row(fn, sequence)
-        return (k.data_ptr(), v.data_ptr(), ks, vs, code, k.shape[0], page, self.heads, d, table.data_ptr() + 4 * width * at,
-                n if sequence is None else 1, width, length.data_ptr() + 8 * at)
+        code, pages, page, heads, dim, width = self._sizes or self._check()
+        t, at = self._tensors, 0 if sequence is None else self._row(fn, sequence)
+        ks, vs = (t["k_scale"].data_ptr(), t["v_scale"].data_ptr()) if self._b8 else (None, None)
+        return (t["k"].data_ptr(), t["v"].data_ptr(), ks, vs, code, pages, page, heads, dim,
+                t["table"].data_ptr() + 4 * width * at, self.sequences if sequence is None else 1, width,
+                t["length"].data_ptr() + 8 * at)
 
     def _places(self, fn: str, name: str, t, n: int) -> torch.Tensor:
         """int64 [n] on the device; an int for every sequence."""
         if not isinstance(t, torch.Tensor):
             return torch.full((n,), int(t), dtype=torch.long, device=self.device)
-        if t.dtype != torch.int64 or t.numel() != n or t.get_device() != self.k.get_device() or not t.is_contiguous():
+        if t.dtype != torch.int64 or t.numel() != n or t.device != self.device or not t.is_contiguous():
             raise ValueError(f"DevicePagedKVBuffer.{fn}: {name} must be a contiguous int64 tensor of {n} on {self.device}")
         return t
 
@@ -553,40 +584,46 @@ class DevicePagedKVBuffer:
         k, v [T, heads, dim] go to that one alone, and start and counts are of
         one entry."""
         cache = self._cache("append", sequence)
-        n, lead = cache[10], 1 if sequence is None else 0
-        if k.shape != v.shape or k.dim() != 3 + lead or tuple(k.shape[1 + lead:]) != (self.heads, self.dim) \
-                or (lead and k.shape[0] != n):
-            raise ValueError(f"DevicePagedKVBuffer.append: expected {'[' + str(n) + ', T' if lead else '[T'}, {self.heads}, "
-                             f"{self.dim}] keys and values")
-        gpu = self.k.get_device()
+        n, heads, dim, shape = cache[10], self.heads, self.dim, k.shape
+        if sequence is None:
+            if len(shape) != 4 or shape[0] != n or shape[2] != heads or shape[3] != dim or v.shape != shape:
+                raise ValueError(f"DevicePagedKVBuffer.append: expected [{n}, T, {heads}, {dim}] keys and values")
+        else:
+            if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
+                raise ValueError(f"DevicePagedKVBuffer.append: expected [T, {heads}, {dim}] keys and values")
+            k, v = k[None], v[None]
+        gpu = self._gpu
         if k.get_device() != gpu or v.get_device() != gpu:
             raise ValueError(f"DevicePagedKVBuffer.append: keys and values must be on {self.device}")
-        if k.dtype not in _DTYPE_CODE or v.dtype != k.dtype:
-            k, v = k.float(), v.float()
-        if not lead:
-            k, v = k[None], v[None]
-        if (self.dim > 1 and (k.stride(3) != 1 or v.stride(3) != 1)) or k.stride()[:3] != v.stride()[:3]:
+        code = _DTYPE_CODE.get(k.dtype)
+        if code is None or v.dtype != k.dtype:
+            k, v, code = k.float(), v.float(), _lib.SBQ_F32
+        st = k.stride()
+        if (st[3] != 1 and dim > 1) or st != v.stride():
             k, v = k.contiguous(), v.contiguous()
-        if any(_within(x, p) for x in (k, v) for p in (self.k, self.v)):
+            st = k.stride()
+        at_k, at_v = k.data_ptr(), v.data_ptr()
+        if any(0 <= x - pool < self._bytes for x in (at_k, at_v) for pool in cache[:2]):  # (would be overwritten as they are read)
             k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+            at_k, at_v, st = k.data_ptr(), v.data_ptr(), k.stride()
         length = cache[12]
-        if start is None:
-            at = length
-        else:
+        at = length
+        if start is not None:
             start = self._places("append", "start", start, n)
             at = start.data_ptr()
             if at != length and abs(at - length) < 8 * n:  # (other sequences' lengths, which this call moves)
                 start = start.clone()
                 at = start.data_ptr()
+        at_counts = None
         if counts is not None:
             counts = self._places("append", "counts", counts, n)
             if abs(counts.data_ptr() - length) < 8 * n:
                 counts = counts.clone()
-        st = k.stride()
-        with _on_device(self.device):
-            _lib.check(_lib.load().sbq_paged_append(
-                *cache, at, None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype],
-                k.shape[1], st[0], st[1], st[2], _stream(self.device)), "sbq_paged_append")
+            at_counts = counts.data_ptr()
+        dev = self._dev
+        with _on_device(dev):
+            _lib.check(_lib.load().sbq_paged_append(*cache, at, at_counts, at_k, at_v, code, k.shape[1], st[0], st[1], st[2],
+                                                    _stream(dev)), "sbq_paged_append")
 
     def read(self, start, count: int, dtype: torch.dtype | None = None,
              sequence: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -602,13 +639,13 @@ class DevicePagedKVBuffer:
         if dtype not in _DTYPE_CODE or count < 0:
             raise ValueError("DevicePagedKVBuffer.read: dtype must be float32, float16 or bfloat16, and count >= 0")
         start = self._places("read", "start", start, n)
-        k = torch.empty(n, count, self.heads, self.dim, dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        with _on_device(self.device):
-            _lib.check(_lib.load().sbq_paged_read(
-                *cache, start.data_ptr(), count, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[dtype], count * self.heads * self.dim,
-                self.heads * self.dim, self.dim, _stream(self.device)), "sbq_paged_read")
-        return (k, v) if sequence is None else (k[0], v[0])
+        heads, dim, dev = self.heads, self.dim, self._dev
+        shape = (n, count, heads, dim) if sequence is None else (count, heads, dim)
+        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        with _on_device(dev):
+            _lib.check(_lib.load().sbq_paged_read(*cache, start.data_ptr(), count, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[dtype],
+                                                  count * heads * dim, heads * dim, dim, _stream(dev)), "sbq_paged_read")
+        return k, v
 
     def attend(self, q: torch.Tensor, start=None, counts: torch.Tensor | None = None, scale: float | None = None,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -622,44 +659,42 @@ class DevicePagedKVBuffer:
         heads / heads).  q has the pool's dtype or float32 (8-bit pools: any);
         the result has q's."""
         cache = self._cache("attend", None)
-        n, gpu = cache[10], self.k.get_device()
-        if q.dim() not in (3, 4) or q.shape[0] != n or q.shape[-1] != self.dim or q.shape[-2] % self.heads \
-                or q.shape[-2] == 0:
-            raise ValueError(f"DevicePagedKVBuffer.attend: expected q [{n}, T, heads, {self.dim}], heads a multiple of "
-                             f"{self.heads}")
-        if q.get_device() != gpu or q.dtype not in _DTYPE_CODE or (self.k_scale is None and q.dtype != self.k.dtype
-                                                                   and q.dtype != torch.float32):
-            raise ValueError(f"DevicePagedKVBuffer.attend: q must be on {self.device}, of the pool's dtype or float32 (8-bit "
-                             "pools: float32, float16 or bfloat16)")
+        n, gpu, dim, kv_heads, dev, shape = cache[10], self._gpu, self.dim, self.heads, self._dev, q.shape
+        if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != dim or shape[-2] % kv_heads or shape[-2] == 0:
+            raise ValueError(f"DevicePagedKVBuffer.attend: expected q [{n}, T, heads, {dim}], heads a multiple of {kv_heads}")
+        code = _DTYPE_CODE.get(q.dtype)
+        if q.get_device() != gpu or code is None or not (self._b8 or code in (cache[4], _lib.SBQ_F32)):
+            raise ValueError(f"DevicePagedKVBuffer.attend: q must be on {dev}, of the pool's dtype or float32 (8-bit pools: "
+                             "float32, float16 or bfloat16)")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != gpu or (self.dim > 1 and out.stride(-1) != 1):
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
+        elif out.shape != shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(-1) != 1):
             raise ValueError("DevicePagedKVBuffer.attend: out must have q's shape, dtype and device, with unit stride in dim")
-        if out.data_ptr() == q.data_ptr() and q.numel():
+        elif out.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("DevicePagedKVBuffer.attend: out must not be q itself")
-        q4, o4 = (q[:, None], out[:, None]) if q.dim() == 3 else (q, out)
-        T, heads = q4.shape[1], q4.shape[2]
+        T, heads = shape[1] if len(shape) == 4 else 1, shape[-2]
         if T > _lib.SBQ_PAGED_MAX_T:
             raise ValueError(f"DevicePagedKVBuffer.attend: at most {_lib.SBQ_PAGED_MAX_T} tokens per call")
         if T == 0:
             return out
-        if self.dim > 1 and q4.stride(3) != 1:
-            q4 = q4.contiguous()
-        L = _lib.load()
+        if dim > 1 and q.stride(-1) != 1:
+            q = q.contiguous()
         if workspace is None:
-            workspace = torch.empty(L.sbq_paged_attn_workspace_bytes(n, T, heads, self.heads, self.dim, self.page, cache[11],
-                                                                     cache[4]), dtype=torch.uint8, device=q.device)
+            workspace = torch.empty(_paged_workspace_bytes(n, T, heads, kv_heads, dim, self.page, cache[11], cache[4]),
+                                    dtype=torch.uint8, device=dev)
         elif workspace.get_device() != gpu or not workspace.is_contiguous():
-            raise ValueError(f"DevicePagedKVBuffer.attend: workspace must be a contiguous tensor on {self.device}")
-        start = None if start is None else self._places("attend", "start", start, n)
-        counts = None if counts is None else self._places("attend", "counts", counts, n)
-        qs, os_ = q4.stride(), o4.stride()
-        with _on_device(q.device):
-            _lib.check(L.sbq_paged_attention(
-                q4.data_ptr(), _DTYPE_CODE[q.dtype], T, heads, qs[0], qs[1], qs[2], *cache,
-                None if start is None else start.data_ptr(), None if counts is None else counts.data_ptr(), self.window or 0,
-                self.dim ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1], os_[2], workspace.data_ptr(),
-                workspace.numel() * workspace.element_size(), _stream(q.device)), "sbq_paged_attention")
+            raise ValueError(f"DevicePagedKVBuffer.attend: workspace must be a contiguous tensor on {dev}")
+        if start is not None:
+            start = self._places("attend", "start", start, n)
+        if counts is not None:
+            counts = self._places("attend", "counts", counts, n)
+        qs, os_ = q.stride(), out.stride()
+        with _on_device(dev):
+            _lib.check(_lib.load().sbq_paged_attention(
+                q.data_ptr(), code, T, heads, qs[0], qs[-3], qs[-2], *cache, None if start is None else start.data_ptr(),
+                None if counts is None else counts.data_ptr(), self.window or 0, dim ** -0.5 if scale is None else scale,
+                out.data_ptr(), os_[0], os_[-3], os_[-2], workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                _stream(dev)), "sbq_paged_attention")
         return out
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
