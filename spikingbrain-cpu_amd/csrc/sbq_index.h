@@ -81,6 +81,42 @@ SBQ_HD uint32_t slot_mask(int64_t n, int64_t s0) {
   return n - s0 >= 32 ? ~0u : n <= s0 ? 0u : (1u << (n - s0)) - 1u;
 }
 
+// The paged cache (sbq_paged.h): the row of position pos and head h in the pool,
+// pages of 1 << page_log positions of every one of Hk heads; -1 for an id that
+// is no page of the pool.
+SBQ_HD int64_t paged_row_of(int32_t id, int64_t pages, int64_t pos, int h, int Hk, int page_log) {
+  if (id < 0 || id >= pages) return -1;
+  return (((int64_t)id * Hk + h) << page_log) + (pos & ((1 << page_log) - 1));
+}
+
+// How its attention cuts a launch's sequences into parts, one for each of `slots`
+// workgroups of kPagedWaves waves: a sequence counts its blocks in whole rounds of the
+// waves, one round at least (a sequence that sees nothing writes its zeros); a
+// part is `each` of all those; slot s's piece of sequence b, blocks n0..n1-1 of
+// it, leaves its partial results at place s + b.
+constexpr int kPagedWaves = 4;
+SBQ_HD int paged_own(int blocks) {
+  const int n = (blocks + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
+  return n < kPagedWaves ? kPagedWaves : n;
+}
+SBQ_HD int paged_each(int total, int slots, float per_slot) {  // per_slot: 1 / slots
+  int n = (int)((float)total * per_slot);
+  while (n > 0 && (int64_t)(n - 1) * slots >= total) --n;
+  while ((int64_t)n * slots < total) ++n;
+  return n < kPagedWaves ? kPagedWaves : n;
+}
+SBQ_HD void paged_piece(int slot, int each, int before, int blocks, int& n0, int& n1) {  // (none: n0 >= n1)
+  const int64_t x0 = (int64_t)slot * each;
+  const int own = blocks > 1 ? blocks : 1;
+  n0 = x0 > before ? (int)(x0 - before) : 0;
+  n1 = x0 + each - before < own ? (int)(x0 + each - before) : own;
+}
+SBQ_HD int paged_places(int b, int each, int before, int blocks, int& first) {  // how many, from `first` on
+  const unsigned s0 = (unsigned)before / (unsigned)each, s1 = (unsigned)(before + (blocks > 1 ? blocks : 1) - 1) / (unsigned)each;
+  first = (int)s0 + b;
+  return (int)(s1 - s0) + 1;
+}
+
 // Column index of a key from argmax_key.
 SBQ_HD int argmax_key_index(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
 

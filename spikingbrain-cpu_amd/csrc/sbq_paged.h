@@ -28,6 +28,8 @@ __device__ __forceinline__ T uniform_load(const T* p) {
   return *(Const)(uintptr_t)p;
 }
 
+static_assert(kPagedWaves == kAttnWaves, "the cut deals blocks to a workgroup's waves");
+
 __device__ __forceinline__ bool valid_page(const PagedCache& c, int32_t id) { return id >= 0 && id < c.pages; }
 
 // Tokens of a sequence's T that are there.
@@ -122,7 +124,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // How the slots, the workgroups of a key head and row tile, share a launch's
-// sequences.  All sequences' blocks, one sequence after another and
+// sequences (the arithmetic is in sbq_index.h).  All sequences' blocks, one sequence after another and
 // each in whole fours (one block for each wave), are cut into equal parts of
 // four blocks or more, one for each slot: a long sequence among short ones has
 // as much of the chip as its length asks for, whatever the host knows of
@@ -142,12 +144,7 @@ __device__ __forceinline__ void paged_look(const PagedArgs& a, int b, int t0, in
   const int lo = span.first(t0, a.window), hi = span.count > t0 ? span.last(min(t1, span.count - 1)) : -1;
   p.from = lo / SB;
   p.blocks = hi >= lo ? hi / SB + 1 - p.from : 0;
-  p.own = max(kAttnWaves, (p.blocks + kAttnWaves - 1) & ~(kAttnWaves - 1));
-}
-__device__ __forceinline__ void paged_cut(const PagedArgs& a, PagedPlace& p) {
-  int n = (int)((float)p.total * a.per_slot);  // (within a few blocks: rounded to 24 bits)
-  while ((int64_t)n * a.slots < p.total) ++n;
-  p.each = max(kAttnWaves, n);
+  p.own = paged_own(p.blocks);
 }
 // BY_SLOT: the sequence that slot `key`'s part begins in, else sequence `key`.
 // t0, t1: the row tile's first and last token.
@@ -158,8 +155,8 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
   if (a.n == 1) {
     paged_look<true>(a, 0, t0, t1, SB, p);
     p.total = p.own;
-    paged_cut(a, p);
-    p.b = BY_SLOT && key * p.each >= p.total ? 1 : 0;
+    p.each = paged_each(p.total, a.slots, a.per_slot);
+    p.b = BY_SLOT && (int64_t)key * p.each >= p.total ? 1 : 0;
     return p;
   }
   const int lane = threadIdx.x & 63;
@@ -175,10 +172,10 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
     look(b0);
     p.total += __builtin_amdgcn_readlane(sum, 63);
   }
-  paged_cut(a, p);
-  const int at = key * p.each;  // (at most `slots` parts of a total that an int holds: the launcher's)
+  p.each = paged_each(p.total, a.slots, a.per_slot);
   p.b = a.n;
-  if (BY_SLOT && at >= p.total) return p;
+  if (BY_SLOT && (int64_t)key * p.each >= p.total) return p;
+  const int at = key * p.each;
   for (int b0 = 0; b0 < a.n; b0 += 64) {
     if (a.n > 64) look(b0);
     const int i = BY_SLOT ? __builtin_popcountll(__ballot(p.before + sum <= at)) : key - b0;
@@ -193,13 +190,6 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
   }
   return p;
 }
-// The places that hold partial results of a sequence: from the first on, so many.
-__device__ __forceinline__ int paged_places(const PagedPlace& p, int& first) {
-  const unsigned s0 = (unsigned)p.before / (unsigned)p.each, s1 = (unsigned)(p.before + max(p.blocks, 1) - 1) / (unsigned)p.each;
-  first = (int)s0 + p.b;
-  return (int)(s1 - s0) + 1;
-}
-
 template <int CT>
 struct PagedMath : AttnMath<CT == XT_BF16 ? XT_BF16 : XT_F16> {
   typedef typename XElem<CT == XT_BF16 ? XT_BF16 : XT_F16>::T T;
@@ -266,7 +256,7 @@ constexpr int paged_occupancy(int ct, int qt, int DP) {
 }
 
 // CT: the cache's type, QT: the queries', DP: columns the registers hold (64,
-// 128, 256), EXACT: row == DP.  Grid: key heads x slots x row tiles.
+// 128, 256), EXACT: row == DP.  Grid: key heads of every row tile x slots.
 template <int CT, int QT, int DP, bool EXACT>
 __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void paged_attn_kernel(PagedArgs a) {
   constexpr bool B8 = is_8bit(CT), F32 = CT == XT_F32, WIDE = QT == XT_F32 && !F32;
@@ -276,7 +266,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   constexpr int SUB = F32 ? 1 : 2, SB = 16 * SUB;
   constexpr int EV = E < DP / 16 ? E : DP / 16, DB = DP / (16 * EV), NF = DP / 16;  // columns of a value load, loads
   constexpr int NFR = DP / 32;                                                       // 16x16x32 steps of a score
-  constexpr int HP = DP < 128 ? DP : 128, OLD = HP + 4;
+  constexpr int HP = 16 * EV > 128 || DP < 128 ? DP : 128, OLD = HP + 4;  // columns joined at a time: whole value loads
+  static_assert(HP % (16 * EV) == 0 && DP % HP == 0, "the joining takes whole value loads");
   constexpr float kNone = -__builtin_inff();
   typedef typename PagedMath<CT>::T M;
   typedef typename PagedMath<CT>::V MV;
@@ -286,15 +277,17 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   __shared__ float lds_m[kAttnWaves][16], lds_l[kAttnWaves][16];
 
   const PagedCache& pc = a.c;
-  const int kvh = blockIdx.x, slot = blockIdx.y, row0 = blockIdx.z * 16, R = a.rep * a.T;
+  const int slot = blockIdx.y, R = a.rep * a.T;
+  int kvh = blockIdx.x, row0 = 0;
+  if (R > 16) row0 = kvh / pc.Hk * 16, kvh %= pc.Hk;
   int t0 = 0, t1 = 0;
   if (a.T > 1) t0 = row0 / a.rep, t1 = min(row0 + 15, R - 1) / a.rep;
   PagedPlace p = paged_place<true>(a, slot, t0, t1, SB);
   if (p.b >= a.n) return;
-  const int x0 = slot * p.each, x1 = min(x0 + p.each, p.total);
 
   for (;;) {
-    const int n0 = max(x0 - p.before, 0), n1 = min(x1 - p.before, max(p.blocks, 1));
+    int n0, n1;
+    paged_piece(slot, p.each, p.before, p.blocks, n0, n1);
     if (n0 < n1) {
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));  // (or what depends on it is kept in registers across the sequences)
@@ -674,7 +667,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 
       // the workgroup's waves joined
       int place;
-      const bool alone = paged_places(p, place) == 1;
+      const bool alone = paged_places(p.b, p.each, p.before, p.blocks, place) == 1;
       place = slot + p.b;
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
@@ -729,7 +722,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       }
     }
     p.before += p.own;
-    if (p.before >= x1) break;
+    if (p.before >= p.total || p.before >= (int64_t)(slot + 1) * p.each) break;
     ++p.b;
     paged_look<true>(a, p.b, t0, t1, SB, p);
   }

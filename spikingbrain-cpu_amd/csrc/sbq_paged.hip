@@ -140,9 +140,7 @@ __device__ __forceinline__ void paged_walk(const PagedStore& a, int part, L load
 
 // The row of position pos and head h in the pool; -1: it has none.
 __device__ __forceinline__ int64_t paged_row(const PagedCache& c, int64_t b, int64_t pos, int h) {
-  const int32_t id = c.table[b * c.max_pages + (pos >> c.page_log)];
-  if (!valid_page(c, id)) return -1;
-  return (((int64_t)id * c.Hk + h) << c.page_log) + (pos & ((1 << c.page_log) - 1));
+  return paged_row_of(c.table[b * c.max_pages + (pos >> c.page_log)], c.pages, pos, h, c.Hk, c.page_log);
 }
 
 template <int CT, int XT, bool VEC>
@@ -286,7 +284,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   if (a.T > 1) t = r / a.rep, t0 = (r & ~15) / a.rep, t1 = min(r | 15, R - 1) / a.rep;
   const PagedPlace p = paged_place<false>(a, blockIdx.z, t0, t1, SB);
   int place;
-  const int used = paged_places(p, place);
+  const int used = paged_places(p.b, p.each, p.before, p.blocks, place);
   if (used == 1) return;  // (written by the one workgroup)
   const int64_t b = a.first + p.b, at = ((int64_t)kvh * a.places + place) * R + r;
   PagedSpan span;
@@ -337,7 +335,7 @@ constexpr int64_t kPagedGroup = 512;  // sequences of a launch at most (each wor
 struct PagedPlan {
   int DP, SB;
   int64_t rtiles, n, slots, places;
-  bool joins;  // can a sequence need more than one slot?
+  bool joins;  // can a sequence have several parts?
 };
 // How many workgroups there are goes by the table's room: how much of it is
 // filled is known on the device alone, where workgroups without a part leave
@@ -353,7 +351,7 @@ PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, 
   const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
   p.places = p.slots + p.n;
-  p.joins = fours > 1;
+  p.joins = fours > 1 && p.slots > 1;
   return p;
 }
 
@@ -389,7 +387,7 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   }
   for (a.first = 0; a.first < B; a.first += p.n) {
     a.n = (int)std::min(p.n, B - a.first);
-    const dim3 grid((unsigned)Hk, (unsigned)p.slots, (unsigned)p.rtiles);
+    const dim3 grid((unsigned)(Hk * p.rtiles), (unsigned)p.slots);
     int rc = c.ct == XT_F32    ? launch_paged_attn_f32(a, p.DP, grid, st)
              : c.ct == XT_F16  ? launch_paged_attn_f16(a, p.DP, grid, st)
              : c.ct == XT_BF16 ? launch_paged_attn_bf16(a, p.DP, grid, st)
