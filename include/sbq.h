@@ -638,11 +638,12 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * to 22 significant bits or more, and so are their weights; with 2-byte
  * queries the weights keep 11 bits (bf16 caches: 16).  scale * q . k is to
  * stay below 2^27 in magnitude.
- * workspace: >= sbq_paged_attn_workspace_bytes bytes, any content; one call at
- * a time.  The result does not depend on timing, nor on other sequences'
+ * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
+ * content; one call at a time.  The result does not depend on timing, nor on other sequences'
  * lengths. */
 int64_t sbq_paged_attn_workspace_bytes(int64_t sequences, int64_t T, int64_t heads, int64_t kv_heads,
-                                       int64_t D, int64_t page, int64_t max_pages, int cache_dtype);
+                                       int64_t D, int64_t page, int64_t max_pages, int64_t window,
+                                       int cache_dtype);
 int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t q_sb, int64_t q_st,
                         int64_t q_sh, const void* k, const void* v, const float* k_scale,
                         const float* v_scale, int cache_dtype, int64_t pages, int64_t page,
@@ -668,7 +669,7 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
  * Products and sums are 64-bit.  A draft outside 0 .. V - 1 is refused.  token
  * is -1 where the whole mass is 0, infinite or NaN.  B, T <= 65535.
  * kept, token: device int64 [B].  workspace: >= sbq_verify_workspace_bytes
- * bytes, any content; one call at a time. */
+ * bytes (0: NULL will do), any content; one call at a time. */
 int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V);
 int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st,
                       int dtype, int64_t B, int64_t T, int64_t V, const int64_t* tokens, const float* u,

@@ -879,11 +879,12 @@ static bool paged_rows_ok(int64_t T, int64_t heads, int64_t kv_heads) {
 }
 
 int64_t sbq_paged_attn_workspace_bytes(int64_t sequences, int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t page,
-                                       int64_t max_pages, int cache_dtype) {
+                                       int64_t max_pages, int64_t window, int cache_dtype) {
   if (!valid_cache_dtype(cache_dtype) || !paged_rows_ok(T, heads, kv_heads) || T == 0 || sequences < 1 || sequences > 65536 ||
-      D < 1 || D > 256 || page < 16 || page > 1024 || (page & (page - 1)) || max_pages < 1 || max_pages > (1 << 30) / page)
+      D < 1 || D > 256 || page < 16 || page > 1024 || (page & (page - 1)) || max_pages < 1 || max_pages > (1 << 30) / page || window < 0)
     return 0;
-  return sbq::paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page * max_pages, cache_dtype) + 256;
+  const int64_t n = sbq::paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page * max_pages, window, cache_dtype);
+  return n ? n + 256 : 0;  // + alignment slack
 }
 
 int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, int64_t q_sb, int64_t q_st, int64_t q_sh,
@@ -906,9 +907,8 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
     return SBQ_ERR_ARG;
   const int64_t es = esize(q_dtype);
   if (!aligned(q, es) || !aligned(out, es) || !aligned(start, 8) || !aligned(counts, 8)) return SBQ_ERR_ALIGN;
-  if (!workspace ||
-      (int64_t)workspace_bytes < sbq_paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page, max_pages, cache_dtype))
-    return SBQ_ERR_WORKSPACE;
+  const int64_t need = sbq_paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page, max_pages, window, cache_dtype);
+  if (need && (!workspace || (int64_t)workspace_bytes < need)) return SBQ_ERR_WORKSPACE;
   c.q = q, c.start = start, c.counts = counts, c.out = out, c.ws = (void*)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
   c.T = T, c.heads = heads, c.window = window < (int64_t)1 << 62 ? window : (int64_t)1 << 62;
   c.q_sb = q_sb, c.q_st = q_st, c.q_sh = q_sh, c.o_sb = o_sb, c.o_st = o_st, c.o_sh = o_sh;
@@ -924,7 +924,8 @@ static bool verify_sizes_ok(int64_t B, int64_t T, int64_t V) {
 
 int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V) {
   if (!verify_sizes_ok(B, 0, V) || B == 0) return 0;
-  return sbq::verify_workspace_bytes(B, V) + 16;  // + alignment slack
+  const int64_t n = sbq::verify_workspace_bytes(B, V);
+  return n ? n + 16 : 0;  // + alignment slack
 }
 
 int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st, int dtype,
@@ -938,7 +939,8 @@ int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, 
   if (!aligned(p, es) || !aligned(q, es) || !aligned(tokens, 8) || !aligned(u, 4) || !aligned(counts, 8) || !aligned(kept, 8) ||
       !aligned(token, 8))
     return SBQ_ERR_ALIGN;
-  if (!workspace || (int64_t)workspace_bytes < sbq_verify_workspace_bytes(B, V)) return SBQ_ERR_WORKSPACE;
+  const int64_t need = sbq_verify_workspace_bytes(B, V);
+  if (need && (!workspace || (int64_t)workspace_bytes < need)) return SBQ_ERR_WORKSPACE;
   sbq::VerifyArgs a{};
   a.p = p, a.q = q, a.tokens = tokens, a.counts = counts, a.u = u, a.kept = kept, a.token = token;
   a.part = (double2*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15), a.B = B, a.T = T, a.V = V, a.p_sb = p_sb, a.p_st = p_st;

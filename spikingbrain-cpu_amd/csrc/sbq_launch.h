@@ -343,7 +343,7 @@ struct PagedCall {
   int qt, ct;
   float scale;
 };
-int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct);
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int64_t window, int ct);
 int launch_paged_attention(const PagedCall& c, hipStream_t st);
 
 int64_t verify_workspace_bytes(int64_t B, int64_t V);

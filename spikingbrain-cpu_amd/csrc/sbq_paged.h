@@ -76,7 +76,7 @@ struct PagedArgs {
   float2* part_ml;  // [Hk][places][R]
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
   int T, rep, qt;
-  int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile, and both
+  int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile (0: one each), and both
   float per_slot;        // 1 / slots
   float scale;               // times log2(e)
   bool ovec;
@@ -131,7 +131,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 // lengths, and while there are slots enough none holds two sequences.  A part
 // that meets several does them in turn.  Slot s's piece of sequence b leaves
 // its partial results at place s + b, of which a sequence's are neighbours.
-// Every workgroup finds its part by a scan over the lengths.
+// Every workgroup finds its part by a scan over the lengths.  Where no sequence
+// is long (kPagedWhole), each has a workgroup of its own, and nothing is joined.
 struct PagedPlace {
   int b, from, blocks;  // the sequence (n: none), its first block and how many (0: sees nothing)
   int before, own;      // the parts' blocks before it, and its own
@@ -152,6 +153,12 @@ template <bool BY_SLOT>
 __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, int t0, int t1, int SB) {
   PagedPlace p;
   p.before = 0;
+  if (a.slots == 0) {  // a slot for every sequence
+    p.b = key;
+    paged_look<true>(a, key, t0, t1, SB, p);
+    p.total = p.each = p.own;
+    return p;
+  }
   if (a.n == 1) {
     paged_look<true>(a, 0, t0, t1, SB, p);
     p.total = p.own;
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 
   for (;;) {
     int n0, n1;
-    paged_piece(slot, p.each, p.before, p.blocks, n0, n1);
+    paged_piece(a.slots ? slot : 0, p.each, p.before, p.blocks, n0, n1);
     if (n0 < n1) {
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));  // (or what depends on it is kept in registers across the sequences)
@@ -722,7 +729,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       }
     }
     p.before += p.own;
-    if (p.before >= p.total || p.before >= (int64_t)(slot + 1) * p.each) break;
+    if (p.before >= p.total || p.before >= (int64_t)(slot + 1) * p.each) break;  // (at once where a slot has one sequence)
     ++p.b;
     paged_look<true>(a, p.b, t0, t1, SB, p);
   }

@@ -330,6 +330,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
 
+constexpr int64_t kPagedWhole = 4;    // blocks of a wave up to which a workgroup takes a whole sequence
 constexpr int64_t kPagedGroup = 512;  // sequences of a launch at most (each workgroup scans their lengths)
 
 struct PagedPlan {
@@ -340,18 +341,20 @@ struct PagedPlan {
 // How many workgroups there are goes by the table's room: how much of it is
 // filled is known on the device alone, where workgroups without a part leave
 // at once.
-PagedPlan paged_plan(int64_t B, int64_t R, int64_t Hk, int64_t D, int64_t room, int ct, bool wide) {
+PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int64_t room, int64_t window, int ct, bool wide) {
   PagedPlan p;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   p.SB = ct == XT_F32 ? 16 : 32;
   p.rtiles = (R + 15) / 16;
-  const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB, fours = (blocks + kAttnWaves - 1) / kAttnWaves;
+  if (window > 0 && window + T < room) room = window + T;  // (what the tokens of a call can look at)
+  const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB + (window > 0), fours = (blocks + kAttnWaves - 1) / kAttnWaves;
   p.n = std::min(B, kPagedGroup);
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 30) / (fours * kAttnWaves)));  // (all blocks fit an int)
   const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
+  if (fours <= kPagedWhole) p.slots = 0;
   p.places = p.slots + p.n;
-  p.joins = fours > 1 && p.slots > 1;
+  p.joins = p.slots > 1;
   return p;
 }
 
@@ -359,11 +362,11 @@ int64_t round256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 }  // namespace
 
-int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int ct) {
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t Hk, int64_t D, int64_t room, int64_t window, int ct) {
   const int64_t R = heads / Hk * T;
   int64_t n = 0;
   for (bool wide : {false, true}) {  // (the queries' type is not known here)
-    const PagedPlan p = paged_plan(B, R, Hk, D, room, ct, wide);
+    const PagedPlan p = paged_plan(B, T, R, Hk, D, room, window, ct, wide);
     const int64_t parts = Hk * R * p.places;
     if (p.joins) n = std::max(n, round256(parts * p.DP * 4) + round256(parts * 8));
   }
@@ -372,11 +375,11 @@ int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t 
 
 int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   const int64_t Hk = c.c.Hk, rep = c.heads / Hk, R = rep * c.T, B = c.c.B;
-  const PagedPlan p = paged_plan(B, R, Hk, c.c.D, (int64_t)c.c.max_pages << c.c.page_log, c.ct, c.qt == XT_F32);
+  const PagedPlan p = paged_plan(B, c.T, R, Hk, c.c.D, (int64_t)c.c.max_pages << c.c.page_log, c.window, c.ct, c.qt == XT_F32);
   PagedArgs a{};
   a.c = c.c, a.q = c.q, a.start = c.start, a.counts = c.counts, a.out = c.out;
   a.q_sb = c.q_sb, a.q_st = c.q_st, a.q_sh = c.q_sh, a.o_sb = c.o_sb, a.o_st = c.o_st, a.o_sh = c.o_sh;
-  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots = (int)p.slots, a.per_slot = 1.0f / (float)p.slots;
+  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots = (int)p.slots, a.per_slot = p.slots ? 1.0f / (float)p.slots : 0.0f;
   a.places = (int)p.places;
   a.scale = c.scale * 1.44269504f;
   const int64_t eq = c.qt == XT_F32 ? 4 : 2;
@@ -387,7 +390,7 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   }
   for (a.first = 0; a.first < B; a.first += p.n) {
     a.n = (int)std::min(p.n, B - a.first);
-    const dim3 grid((unsigned)(Hk * p.rtiles), (unsigned)p.slots);
+    const dim3 grid((unsigned)(Hk * p.rtiles), (unsigned)(p.slots ? p.slots : a.n));
     int rc = c.ct == XT_F32    ? launch_paged_attn_f32(a, p.DP, grid, st)
              : c.ct == XT_F16  ? launch_paged_attn_f16(a, p.DP, grid, st)
              : c.ct == XT_BF16 ? launch_paged_attn_bf16(a, p.DP, grid, st)

@@ -11,7 +11,8 @@
 // that a sequence needs, so a first launch finds the row and sums it in
 // segments of kVerSeg tokens, each workgroup deciding by itself which drafts
 // are kept; a second launch looks the segment up and goes through it once
-// more.  Few sequences are bound by the two launches and three dependent loads
+// more.  A row of up to kVerWhole tokens is one workgroup's, in one launch.
+// Few sequences are bound by the two launches and three dependent loads
 // (token, probability, row), many by the rows' bytes.
 #include <algorithm>
 
@@ -23,6 +24,7 @@ namespace sbq {
 namespace {
 
 constexpr int kVerThreads = 256, kVerPart = 4 * kVerThreads, kVerSeg = 4 * kVerPart;
+constexpr int kVerWholeThreads = 1024, kVerWhole = 16 * kVerWholeThreads;  // a row's tokens that one workgroup takes whole
 
 __device__ __forceinline__ double shfl_xor_f64(double v, int o) { return __shfl_xor(v, o, 64); }
 
@@ -32,7 +34,9 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   __syncthreads();  // (lds is free)
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  double sum = 0.0;
+  for (int k = 0; k < (int)blockDim.x >> 6; ++k) sum += lds[k];
+  return sum;
 }
 
 // Sums of the threads before this one, in thread order; `total` of all.
@@ -50,8 +54,7 @@ __device__ __forceinline__ double block_before(double v, double* lds, double* to
   if (lane == 63) lds[w] = sum;
   __syncthreads();
   double base = 0.0, all = 0.0;
-#pragma unroll
-  for (int k = 0; k < kVerThreads / 64; ++k) {
+  for (int k = 0; k < (int)blockDim.x >> 6; ++k) {
     base = k == w ? all : base;
     all += lds[k];
   }
@@ -146,6 +149,36 @@ __device__ __forceinline__ int count_of(const VerifyArgs& a, int64_t b) {
   return (int)(n < 0 ? 0 : n > a.T ? a.T : n);
 }
 
+// The token: threads hold neighbouring masses m, their sums and the sums `at` of
+// those before them.  The first thread whose prefix passes `want` scans its own;
+// sums in another order can end a rounding below it: then the last one with mass.
+template <int N>
+__device__ __forceinline__ void choose(const double (&m)[N], double sum, double at, double want, int64_t i0, int64_t* token) {
+  __shared__ int found, last;
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x == 0) found = INT32_MAX, last = -1;
+  __syncthreads();
+  const uint64_t past = __ballot(at + sum > want && sum > 0.0), some = __ballot(sum > 0.0);
+  if (lane == 0) {
+    if (past) atomicMin(&found, (int)threadIdx.x + __builtin_ctzll(past));
+    if (some) atomicMax(&last, (int)threadIdx.x + 63 - __builtin_clzll(some));
+  }
+  __syncthreads();
+  if ((int)threadIdx.x == (found != INT32_MAX ? found : last)) {
+    int64_t t = -1;
+    bool done = want != want;  // (a uniform that is not a number: no token)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      at += m[j];
+      if (m[j] > 0.0 && !done) {
+        t = i0 + j;
+        done = at > want;
+      }
+    }
+    *token = t;
+  }
+}
+
 template <int XT, bool VEC>
 __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerifyArgs a) {
   __shared__ double lds[4];
@@ -171,7 +204,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerifyArgs a) {
 template <int XT, bool VEC>
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) {
   __shared__ double lds[4], seg_before;
-  __shared__ int hit, found, last;
+  __shared__ int hit;
   const int64_t b = a.first + blockIdx.x;
   const int n = count_of(a, b), kept = (int)a.kept[b], each = (a.segs + kVerThreads - 1) / kVerThreads;
   const double2* const part = a.part + b * a.segs;
@@ -182,7 +215,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
   // (without a refusal the two are equal; nothing left after one: p itself)
   const bool use = total_left > 0.0 || total_left != total_left;
   const double total = use ? total_left : total_all, want = (double)a.u[b * (a.T + 1) + a.T] * total;
-  if (threadIdx.x == 0) hit = -1, found = INT32_MAX, last = -1;
+  if (threadIdx.x == 0) hit = -1;
   __syncthreads();
   if (!(total > 0.0 && total < __builtin_inf())) {  // (NaN too)
     if (threadIdx.x == 0) a.token[b] = -1;
@@ -224,34 +257,58 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
     }
   }
   at = seg_before + block_before(sum, lds, &total_seg);
-  // the first thread whose prefix passes `want`; sums in another order can end a
-  // rounding below it: then the last one with mass
-  const int lane = threadIdx.x & 63;
-  const uint64_t past = __ballot(at + sum > want && sum > 0.0), some = __ballot(sum > 0.0);
-  if (lane == 0) {
-    if (past) atomicMin(&found, (int)threadIdx.x + __builtin_ctzll(past));
-    if (some) atomicMax(&last, (int)threadIdx.x + 63 - __builtin_clzll(some));
-  }
-  __syncthreads();
-  if ((int)threadIdx.x == (found != INT32_MAX ? found : last)) {
-    int64_t token = -1;
-    bool done = false;
+  choose<kEach>(m, sum, at, want, i0, a.token + b);
+}
+
+// Whole rows of up to kVerWhole tokens: a workgroup a sequence, every thread's
+// share in registers from the sums to the choice.
+template <int XT, bool VEC>
+__global__ __launch_bounds__(kVerWholeThreads) void verify_whole_kernel(VerifyArgs a) {
+  __shared__ double lds[kVerWholeThreads / 64];
+  constexpr int kEach = kVerWhole / kVerWholeThreads;
+  const int64_t b = a.first + blockIdx.x;
+  const int n = count_of(a, b), kept = kept_of<XT>(a, b, n);
+  const VerRow r = row_of<XT>(a, b, n, kept);
+  const int each = ((int)(a.V + blockDim.x - 1) / (int)blockDim.x + 3) & ~3;
+  const int64_t i0 = (int64_t)threadIdx.x * each;
+  double left[kEach], all[kEach], sum_left = 0.0, sum_all = 0.0, total;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      at += m[j];
-      if (m[j] > 0.0 && !done) {
-        token = i0 + j;
-        done = at > want;
-      }
+  for (int k = 0; k < kEach; k += 4) {
+    double l[4] = {}, w[4] = {};
+    if (k < each) masses<XT, VEC>(r, i0 + k, a.V, l, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      left[k + j] = l[j], all[k + j] = w[j];
+      sum_left += l[j], sum_all += w[j];
     }
-    a.token[b] = token;
   }
+  if (threadIdx.x == 0) a.kept[b] = kept;
+  double at = block_before(sum_left, lds, &total);
+  // (without a refusal the two are equal; nothing left after one: p itself)
+  const bool use = total > 0.0 || total != total;
+  if (!use) {
+    at = block_before(sum_all, lds, &total);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) left[k] = all[k];
+    sum_left = sum_all;
+  }
+  if (!(total > 0.0 && total < __builtin_inf())) {  // (NaN too)
+    if (threadIdx.x == 0) a.token[b] = -1;
+    return;
+  }
+  choose<kEach>(left, sum_left, at, (double)a.u[b * (a.T + 1) + a.T] * total, i0, a.token + b);
 }
 
 template <int XT, bool VEC>
 int launch_verify_xt(VerifyArgs a, hipStream_t st) {
   const int64_t most = std::max<int64_t>(1, kLaunchThreads / kVerThreads / a.segs);  // sequences of a launch
   const int64_t B = a.B;
+  if (a.V <= kVerWhole) {
+    a.first = 0;
+    const unsigned threads = a.V <= 4096 ? 256 : kVerWholeThreads;
+    verify_whole_kernel<XT, VEC><<<(unsigned)B, threads, 0, st>>>(a);
+    return check_launch();
+  }
   for (a.first = 0; a.first < B; a.first += most) {
     a.B = std::min(most, B - a.first);
     verify_sum_kernel<XT, VEC><<<(unsigned)(a.B * a.segs), kVerThreads, 0, st>>>(a);
@@ -264,7 +321,7 @@ int launch_verify_xt(VerifyArgs a, hipStream_t st) {
 
 }  // namespace
 
-int64_t verify_workspace_bytes(int64_t B, int64_t V) { return B * ((V + kVerSeg - 1) / kVerSeg) * 16; }
+int64_t verify_workspace_bytes(int64_t B, int64_t V) { return V <= kVerWhole ? 0 : B * ((V + kVerSeg - 1) / kVerSeg) * 16; }
 
 int launch_verify(const VerifyArgs& c, int xt, hipStream_t st) {
   VerifyArgs a = c;

@@ -69,7 +69,7 @@ SIGNATURES = {
                               _P, _L, _L, _L, _L, _P]),
     "sbq_paged_append": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P]),
     "sbq_paged_read": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _L, _P, _P, _I, _L, _L, _L, _P]),
-    "sbq_paged_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _I]),
+    "sbq_paged_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
     "sbq_paged_attention": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _L, _L, _P, _P, _P, _L,
                                  ctypes.c_float, _P, _L, _L, _L, _P, _S, _P]),
     "sbq_verify_workspace_bytes": (_L, [_L, _L]),

@@ -663,7 +663,8 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     counts = None if counts is None else counts.contiguous()
     both = torch.empty((2, B), dtype=torch.int64, device=dev)
     if workspace is None:
-        workspace = verify_workspace(B, V, dev)
+        room = _lib.load().sbq_verify_workspace_bytes(B, V)
+        workspace = torch.empty((room,), dtype=torch.uint8, device=dev) if room else None
     elif workspace.device != dev or not workspace.is_contiguous():
         raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device")
     ps, qs = target.stride(), (0, 0) if draft is None else draft.stride()

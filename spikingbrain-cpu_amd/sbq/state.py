@@ -679,11 +679,15 @@ class DevicePagedKVBuffer:
             return out
         if dim > 1 and q.stride(-1) != 1:
             q = q.contiguous()
+        room, window = 0, self.window or 0
         if workspace is None:
-            workspace = torch.empty(_paged_workspace_bytes(n, T, heads, kv_heads, dim, self.page, cache[11], cache[4]),
-                                    dtype=torch.uint8, device=dev)
+            room = _paged_workspace_bytes(n, T, heads, kv_heads, dim, self.page, cache[11], window, cache[4])
+            if room:
+                workspace = torch.empty(room, dtype=torch.uint8, device=dev)
         elif workspace.get_device() != gpu or not workspace.is_contiguous():
             raise ValueError(f"DevicePagedKVBuffer.attend: workspace must be a contiguous tensor on {dev}")
+        else:
+            room = workspace.numel() * workspace.element_size()
         if start is not None:
             start = self._places("attend", "start", start, n)
         if counts is not None:
@@ -692,9 +696,9 @@ class DevicePagedKVBuffer:
         with _on_device(dev):
             _lib.check(_lib.load().sbq_paged_attention(
                 q.data_ptr(), code, T, heads, qs[0], qs[-3], qs[-2], *cache, None if start is None else start.data_ptr(),
-                None if counts is None else counts.data_ptr(), self.window or 0, dim ** -0.5 if scale is None else scale,
-                out.data_ptr(), os_[0], os_[-3], os_[-2], workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                _stream(dev)), "sbq_paged_attention")
+                None if counts is None else counts.data_ptr(), window, dim ** -0.5 if scale is None else scale,
+                out.data_ptr(), os_[0], os_[-3], os_[-2], workspace.data_ptr() if room else None, room, _stream(dev)),
+                "sbq_paged_attention")
         return out
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,

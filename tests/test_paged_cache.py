@@ -72,10 +72,11 @@ def test_c_abi_refuses_bad_arguments():
         assert attend(**bad) == -1, bad
     for bad in (dict(q=p + 2), dict(out=p + 1), dict(start=p + 4), dict(counts=p + 2)):
         assert attend(**bad) == -3, bad
-    need = L.sbq_paged_attn_workspace_bytes(3, 1, 4, 2, 24, 16, 4, 3)
-    assert need >= 256 and attend(ws=None) == -4 and attend(nws=need - 1) == -4 and attend(T=0) == 0
-    for bad in ((0, 1, 4, 2, 24, 16, 4, 3), (3, 0, 4, 2, 24, 16, 4, 3), (3, 1, 5, 2, 24, 16, 4, 3), (3, 1, 4, 2, 257, 16, 4, 3),
-                (3, 1, 4, 2, 24, 17, 4, 3), (3, 1, 4, 2, 24, 16, 0, 3), (3, 1, 4, 2, 24, 16, 4, 9)):
+    need = L.sbq_paged_attn_workspace_bytes(3, 1, 4, 2, 24, 16, 100, 0, 3)
+    assert need > 256 and attend(width=100, ws=None) == -4 and attend(width=100, nws=need - 1) == -4 and attend(T=0) == 0
+    for bad in ((0, 1, 4, 2, 24, 16, 100, 0, 3), (3, 0, 4, 2, 24, 16, 100, 0, 3), (3, 1, 5, 2, 24, 16, 100, 0, 3),
+                (3, 1, 4, 2, 257, 16, 100, 0, 3), (3, 1, 4, 2, 24, 17, 100, 0, 3), (3, 1, 4, 2, 24, 16, 0, 0, 3),
+                (3, 1, 4, 2, 24, 16, 100, -1, 3), (3, 1, 4, 2, 24, 16, 100, 0, 9), (3, 1, 4, 2, 24, 16, 4, 0, 3)):
         assert L.sbq_paged_attn_workspace_bytes(*bad) == 0
 
 
@@ -505,6 +506,8 @@ SHAPES = [  # lengths, T, heads, kv, dim, page, window
     ([400, 33, 17], 9, 8, 2, 250, 16, 100),
     ([130] * 70, 1, 2, 1, 16, 16, None),
     ([1000, 1, 1, 1, 700], 2, 8, 8, 64, 16, None),
+    ([1000, 60, 700], 3, 4, 2, 128, 16, 200),
+    ([513, 512, 511, 600], 1, 2, 1, 256, 64, None),
 ]
 
 
@@ -628,7 +631,7 @@ def test_attention_far_scales(dev, dtype, qt):
 
 @pytest.mark.gpu
 def test_attention_strides_out_and_workspace(dev):
-    b = _buffer(dev, [90, 40, 7], 2, 40, 16, I8, seed=6)
+    b = _buffer(dev, [90, 40, 7], 2, 40, 16, I8, seed=6, room=2000)
     g = torch.Generator().manual_seed(0)
     qkv = torch.randn(3, 2, (6 + 4) * 40, generator=g).to(dev)
     q = qkv[..., :240].unflatten(-1, (6, 40))

@@ -76,10 +76,11 @@ def test_c_abi_refuses_bad_arguments():
     for bad in (dict(t=p + 2), dict(q=p + 1), dict(tok=p + 4), dict(u=p + 2), dict(counts=p + 4), dict(kept=p + 1),
                 dict(token=p + 2)):
         assert call(**bad) == -3, bad
-    assert call(ws=None) == -4 and call(nws=L.sbq_verify_workspace_bytes(2, 10) - 1) == -4
+    wide = dict(V=20000, psb=100000, pst=20000, qsb=80000, qst=20000)
+    assert call(ws=None, **wide) == -4 and call(nws=L.sbq_verify_workspace_bytes(2, 20000) - 1, **wide) == -4
     assert call(B=0) == 0
     assert L.sbq_verify_workspace_bytes(0, 10) == 0 and L.sbq_verify_workspace_bytes(1, 0) == 0
-    assert L.sbq_verify_workspace_bytes(3, 151936) == 3 * 38 * 16 + 16
+    assert L.sbq_verify_workspace_bytes(3, 151936) == 3 * 38 * 16 + 16 and L.sbq_verify_workspace_bytes(3, 16384) == 0
 
 
 def test_python_refuses():
@@ -99,10 +100,12 @@ def test_python_refuses_on_the_gpu(dev):
                       ("tokens", dict(tokens=a["tokens"][:, :2])), ("u must", dict(u=a["u"][:, :3])),
                       ("u must", dict(u=a["u"].double())), ("counts", dict(counts=torch.zeros(2, device=dev))),
                       ("counts", dict(counts=torch.zeros(3, dtype=torch.long, device=dev))),
-                      ("workspace", dict(workspace=torch.zeros(64, dtype=torch.uint8))),
-                      ("workspace", dict(workspace=torch.zeros(8, dtype=torch.uint8, device=dev)))):
+                      ("workspace", dict(workspace=torch.zeros(64, dtype=torch.uint8)))):
         with pytest.raises(ValueError, match=match):
             quant.verify_drafts(**{**a, **kw})
+    with pytest.raises(ValueError, match="workspace"):
+        quant.verify_drafts(torch.rand(1, 1, 20000, device=dev), None, torch.zeros(1, 0, dtype=torch.long, device=dev),
+                            torch.zeros(1, 1, device=dev), workspace=torch.zeros(8, dtype=torch.uint8, device=dev))
 
 
 # ---------------------------------------------------------------------------
@@ -110,7 +113,7 @@ def test_python_refuses_on_the_gpu(dev):
 # ---------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("V", [1, 2, 5, 63, 1000, 4095, 4096, 4097, 20001])
+@pytest.mark.parametrize("V", [1, 2, 5, 63, 1000, 4095, 4096, 4097, 16384, 20001])
 @pytest.mark.parametrize("T", [0, 1, 3, 70])
 def test_rule(dev, T, V, dtype):
     B = 6
@@ -177,7 +180,7 @@ def test_nothing_left_bad_drafts_and_bad_rows(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides_and_workspace(dev, dtype):
-    B, T, V = 5, 3, 4103
+    B, T, V = 5, 3, 17003
     g = torch.Generator().manual_seed(9)
     big = _probs(g, B, T + 1, V + 3, 1.5, dtype).to(dev)
     target = big[:, :, 1:V + 1]             # rows that no vector load takes
