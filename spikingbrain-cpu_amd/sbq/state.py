@@ -171,57 +171,77 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     starts of n sequences are enough for their next tokens.  q_out, k_out: q and
     k themselves, or tensors apart from both (default: new ones)."""
     gpu, dtype, shape, device = q.get_device(), q.dtype, q.shape, q.device
-    if gpu < 0:
-        raise ValueError("qk_norm_rope: q must be a GPU tensor")
-    code = _DTYPE_CODE.get(dtype)
-    if code is None:
-        raise ValueError(f"qk_norm_rope: unsupported dtype {dtype}; expected float32, float16 or bfloat16")
-    if len(shape) != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2]
-                                              or k.dtype != dtype or k.get_device() != gpu)):
-        raise ValueError("qk_norm_rope: expected q [tokens, heads, dim] and k [tokens, kv_heads, dim] of one dtype on one GPU")
+    code, n, pairs = _DTYPE_CODE.get(dtype), positions.numel(), inv_freq.numel()
+    wt = None if q_weight is None else q_weight.dtype
+    if k_weight is not None:
+        wt = k_weight.dtype if wt is None or wt is k_weight.dtype else False
+    if gpu < 0 or code is None or len(shape) != 3 or not (
+            positions.dtype is torch.int64 and positions.get_device() == gpu and positions.is_contiguous()
+            and inv_freq.dtype is torch.float32 and inv_freq.get_device() == gpu and inv_freq.is_contiguous()
+            and 2 * pairs <= shape[2] <= 256 and (shape[0] % n == 0 if n else shape[0] == 0)
+            and (wt is None or wt in _DTYPE_CODE)
+            and (q_weight is None or (q_weight.numel() == shape[2] and q_weight.get_device() == gpu and q_weight.is_contiguous()))
+            and (k_weight is None or (k_weight.numel() == shape[2] and k_weight.get_device() == gpu and k_weight.is_contiguous()))):
+        _refuse_rope(q, positions, inv_freq, q_weight, k_weight)
     tokens, heads, dim = shape
-    n, pairs = positions.numel(), inv_freq.numel()
-    if positions.dtype != torch.int64 or positions.get_device() != gpu or not positions.is_contiguous() \
-            or (tokens % n if n else tokens):
-        raise ValueError(f"qk_norm_rope: positions must be a contiguous int64 tensor on {device} whose size divides {tokens} "
-                         "tokens")
-    if (inv_freq.dtype != torch.float32 or inv_freq.get_device() != gpu or not inv_freq.is_contiguous()
-            or 2 * pairs > dim or dim > 256):
-        raise ValueError(f"qk_norm_rope: inv_freq must be a contiguous float32 tensor on {device} of at most dim / 2 entries, "
-                         "dim at most 256")
-    wt, w_at = None, [None, None]
-    for i, w in enumerate((q_weight, k_weight)):
-        if w is not None:
-            if w.numel() != dim or w.get_device() != gpu or not w.is_contiguous() or wt not in (None, w.dtype) \
-                    or w.dtype not in _DTYPE_CODE:
-                raise ValueError(f"qk_norm_rope: weights must be contiguous [{dim}] tensors of one float dtype on {device}")
-            wt, w_at[i] = w.dtype, w.data_ptr()
-    if tokens and dim > 1:
-        q, k = _rows_of(q), None if k is None else _rows_of(k)
-    qs, ks = q.stride(), (0, 0) if k is None else k.stride()
+    qs = q.stride()
+    if qs[2] != 1 and dim > 1:
+        q = q.contiguous()
+        qs = q.stride()
     if q_out is None:
         q_out = torch.empty(shape, dtype=dtype, device=device)
     elif q_out.shape != shape or q_out.dtype != dtype or q_out.get_device() != gpu or (dim > 1 and q_out.stride(2) != 1) \
             or (q_out.data_ptr() == q.data_ptr() and q_out.stride() != qs):
         raise ValueError("qk_norm_rope: q_out must have q's shape, dtype and device, with unit stride in dim")
+    kv_heads = at_k = at_ko = 0
+    ks = ko = (0, 0)
     if k is None:
         if k_out is not None:
             raise ValueError("qk_norm_rope: k_out needs k")
-    elif k_out is None:
-        k_out = torch.empty(k.shape, dtype=dtype, device=device)
-    elif k_out.shape != k.shape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1) \
-            or (k_out.data_ptr() == k.data_ptr() and k_out.stride() != ks):
-        raise ValueError("qk_norm_rope: k_out must have k's shape, dtype and device, with unit stride in dim")
+    else:
+        kshape, ks = k.shape, k.stride()
+        if len(kshape) != 3 or kshape[0] != tokens or kshape[2] != dim or k.dtype is not dtype or k.get_device() != gpu:
+            raise ValueError("qk_norm_rope: expected q [tokens, heads, dim] and k [tokens, kv_heads, dim] of one dtype on one GPU")
+        if ks[2] != 1 and dim > 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if k_out is None:
+            k_out = torch.empty(kshape, dtype=dtype, device=device)
+        elif k_out.shape != kshape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1) \
+                or (k_out.data_ptr() == k.data_ptr() and k_out.stride() != ks):
+            raise ValueError("qk_norm_rope: k_out must have k's shape, dtype and device, with unit stride in dim")
+        kv_heads, ko, at_k, at_ko = kshape[1], k_out.stride(), k.data_ptr(), k_out.data_ptr()
     if tokens == 0:
         return q_out, k_out
-    qo, ko = q_out.stride(), (0, 0) if k is None else k_out.stride()
+    qo = q_out.stride()
     with _on_device(device):
         _lib.check(_lib.load().sbq_qk_norm_rope(
-            q.data_ptr(), None if k is None else k.data_ptr(), code, tokens, heads, 0 if k is None else k.shape[1], dim, qs[0],
-            qs[1], ks[0], ks[1], positions.data_ptr(), tokens // n, inv_freq.data_ptr(), pairs, int(interleaved), w_at[0], w_at[1],
-            0 if wt is None else _DTYPE_CODE[wt], eps, q_out.data_ptr(), None if k is None else k_out.data_ptr(), qo[0], qo[1],
-            ko[0], ko[1], _stream(device)), "sbq_qk_norm_rope")
+            q.data_ptr(), at_k, code, tokens, heads, kv_heads, dim, qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), tokens // n,
+            inv_freq.data_ptr(), pairs, interleaved, None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), 0 if wt is None else _DTYPE_CODE[wt], eps, q_out.data_ptr(), at_ko,
+            qo[0], qo[1], ko[0], ko[1], _stream(device)), "sbq_qk_norm_rope")
     return q_out, k_out
+
+
+def _refuse_rope(q, positions, inv_freq, q_weight, k_weight):
+    """The reason why qk_norm_rope does not take these."""
+    if not q.is_cuda:
+        raise ValueError("qk_norm_rope: q must be a GPU tensor")
+    if q.dtype not in _DTYPE_CODE:
+        raise ValueError(f"qk_norm_rope: unsupported dtype {q.dtype}; expected float32, float16 or bfloat16")
+    if q.dim() != 3:
+        raise ValueError("qk_norm_rope: expected q [tokens, heads, dim] and k [tokens, kv_heads, dim] of one dtype on one GPU")
+    tokens, _, dim = q.shape
+    n = positions.numel()
+    if positions.dtype != torch.int64 or positions.device != q.device or not positions.is_contiguous() \
+            or (tokens % n if n else tokens):
+        raise ValueError(f"qk_norm_rope: positions must be a contiguous int64 tensor on {q.device} whose size divides {tokens} "
+                         "tokens")
+    if (inv_freq.dtype != torch.float32 or inv_freq.device != q.device or not inv_freq.is_contiguous()
+            or 2 * inv_freq.numel() > dim or dim > 256):
+        raise ValueError(f"qk_norm_rope: inv_freq must be a contiguous float32 tensor on {q.device} of at most dim / 2 entries, "
+                         "dim at most 256")
+    raise ValueError(f"qk_norm_rope: weights must be contiguous [{dim}] tensors of one float dtype on {q.device}")
 
 
 class DeviceKVBuffer:
@@ -571,7 +591,8 @@ class DevicePagedKVBuffer:
         """int64 [n] on the device; an int for every sequence."""
         if not isinstance(t, torch.Tensor):
             return torch.full((n,), int(t), dtype=torch.long, device=self.device)
-        if t.dtype != torch.int64 or t.numel() != n or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not torch.int64 or t.numel() != n or t.get_device() != self._tensors["length"].get_device() \
+                or not t.is_contiguous():
             raise ValueError(f"DevicePagedKVBuffer.{fn}: {name} must be a contiguous int64 tensor of {n} on {self.device}")
         return t
 
@@ -603,10 +624,11 @@ class DevicePagedKVBuffer:
             k, v = k.contiguous(), v.contiguous()
             st = k.stride()
         at_k, at_v = k.data_ptr(), v.data_ptr()
-        if any(0 <= x - pool < self._bytes for x in (at_k, at_v) for pool in cache[:2]):  # (would be overwritten as they are read)
+        pool_k, pool_v, room, length = cache[0], cache[1], self._bytes, cache[12]
+        if 0 <= at_k - pool_k < room or 0 <= at_k - pool_v < room or 0 <= at_v - pool_k < room or 0 <= at_v - pool_v < room:
+            # (rows of the pool itself: they would be overwritten as they are read)
             k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
             at_k, at_v, st = k.data_ptr(), v.data_ptr(), k.stride()
-        length = cache[12]
         at = length
         if start is not None:
             start = self._places("append", "start", start, n)
@@ -641,7 +663,8 @@ class DevicePagedKVBuffer:
         start = self._places("read", "start", start, n)
         heads, dim, dev = self.heads, self.dim, self._dev
         shape = (n, count, heads, dim) if sequence is None else (count, heads, dim)
-        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
         with _on_device(dev):
             _lib.check(_lib.load().sbq_paged_read(*cache, start.data_ptr(), count, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[dtype],
                                                   count * heads * dim, heads * dim, dim, _stream(dev)), "sbq_paged_read")
