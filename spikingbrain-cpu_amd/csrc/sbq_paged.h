@@ -335,40 +335,52 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         for (int st = 0; st < SUB; ++st)
           ids[st] = uniform_load(table + min(((p.from + n) * SB + st * 16) >> pc.page_log, pc.max_pages - 1));
       };
+      // (sixteen rows of a page through a buffer each: the lane's offset in one
+      // register, what the wave shares in scalar ones; past the sixteen rows zeros)
+      auto rows_at = [&](const void* pool, int st, int n) {
+        const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
+        const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
+        return raw_rsrc((const char*)pool + block * head_bytes + in_page * row_bytes, 16 * row_bytes);
+      };
+      auto scales_at = [&](const float* scale, int st, int n) {
+        const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
+        const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                             raw_rsrc(scale + (block << pc.page_log) + in_page, 64), 16 * g, 0, 0));
+      };
       auto load_k = [&](int n) {
         held_k = 0;
 #pragma unroll
         for (int st = 0; st < SUB; ++st) {
           if (valid_page(pc, ids[st])) held_k |= 1u << st;
           ids_v[st] = valid_page(pc, ids[st]) ? ids[st] : 0;
-          const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
-          const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
-          const char* const kp = (const char*)pc.k + block * head_bytes + in_page * row_bytes;
+          const __amdgpu_buffer_rsrc_t rs = rows_at(pc.k, st, n);
 #pragma unroll
-          for (int ch = 0; ch < NCH; ++ch) {
-            if (EXACT || ch * 4 * E + g * E < pc.row)
-              kf[st][ch] = *(const KV*)(kp + (k_lane + ch * 64));
-            else
-              kf[st][ch] = (KV)(0u);
-          }
-          if constexpr (B8) ks[st] = *(const f32x4*)(pc.k_scale + (block << pc.page_log) + in_page + 4 * g);
+          for (int ch = 0; ch < NCH; ++ch)
+            kf[st][ch] = __builtin_amdgcn_raw_buffer_load_b128(
+                rs, EXACT || ch * 4 * E + g * E < pc.row ? k_lane + ch * 64 : ~0u, 0, 0);
+          if constexpr (B8) ks[st] = scales_at(pc.k_scale, st, n);
         }
       };
       auto load_v = [&](int n) {
 #pragma unroll
         for (int st = 0; st < SUB; ++st) {
-          const int64_t block = (int64_t)ids_v[st] * pc.Hk + kvh;
-          const uint32_t in_page = ((p.from + n) * SB + st * 16) & page_mask;
-          const char* const vp = (const char*)pc.v + block * head_bytes + in_page * row_bytes;
-          if constexpr (B8) vs[st] = *(const f32x4*)(pc.v_scale + (block << pc.page_log) + in_page + 4 * g);
+          const __amdgpu_buffer_rsrc_t rs = rows_at(pc.v, st, n);
+          if constexpr (B8) vs[st] = scales_at(pc.v_scale, st, n);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-              if (EXACT || db * 16 * EV + c * EV < pc.row)
-                vf[st * 4 + j][db] = *(const VW*)(vp + (v_lane + j * row_bytes + db * 16 * EV * ES));
+              const uint32_t at = EXACT                            ? v_lane + db * 16 * EV * ES
+                                  : db * 16 * EV + c * EV < pc.row ? v_lane + j * row_bytes + db * 16 * EV * ES
+                                                                   : ~0u;
+              VW& to = vf[st * 4 + j][db];
+              if constexpr (EV * ES == 16)
+                to = __builtin_amdgcn_raw_buffer_load_b128(rs, at, EXACT ? j * row_bytes : 0, 0);
+              else if constexpr (EV * ES == 8)
+                to = __builtin_amdgcn_raw_buffer_load_b64(rs, at, EXACT ? j * row_bytes : 0, 0);
               else
-                vf[st * 4 + j][db] = (VW)(0u);
+                to[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, EXACT ? j * row_bytes : 0, 0);
             }
         }
       };
@@ -454,7 +466,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 #pragma unroll
       for (int f = 0; f < NF; ++f) o[f] = (f32x4)(0.0f);
       float m = kNone, l = 0.0f;
-      float vref = 1.17549435e-38f;  // 8-bit: O's unit, the largest value scale that the row saw so far
+      float vref = 1.17549435e-38f, vinv = 1.0f / vref;  // 8-bit: O's unit, the largest value scale that the row saw so far
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {
         const int s0 = (p.from + n) * SB;
@@ -546,15 +558,14 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
             top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
             top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
             const float up = __builtin_fmaxf(vref, top), alpha = vref / up;
-            vref = up;
+            vref = up, vinv = 1.0f / up;
 #pragma unroll
             for (int f = 0; f < NF; ++f) o[f] *= alpha;
           }
-          const float inv = 1.0f / vref;
 #pragma unroll
           for (int st = 0; st < SUB; ++st)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) e[st][v] *= vs[st][v] * inv;
+            for (int v = 0; v < 4; ++v) e[st][v] *= vs[st][v] * vinv;
         }
 
         // infinities and NaN in values that not every row sees (codes have none)
