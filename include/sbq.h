@@ -568,7 +568,8 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
  * fp32, rounded once to the output's type.
  * q: device [tokens, heads, D], k: device [tokens, kv_heads, D] (kv_heads 0:
  * none) of one type, strides in elements, unit stride in D <= 256.
- * positions: device int64; token t stands at positions[t / per] + t % per.
+ * positions: device int64, below 2^53; token t stands at positions[t / per] +
+ * t % per.
  * inv_freq: device fp32 [pairs].  q_weight, k_weight: device [D] of
  * weight_dtype, or NULL.  q_out, k_out: device, of q's type, the input itself
  * (with its strides) or apart from both inputs. */
@@ -597,8 +598,8 @@ int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, in
  * in page table[b][p / page], row p % page; an entry outside 0 .. pages - 1
  * is no page: what stands there is neither written nor seen.  Pages that two
  * sequences write to must differ.  length: device int64 [sequences]: positions
- * held.  max_pages * page <= 2^30, sequences <= 65536.  k, v and the scales
- * are 16-byte aligned.
+ * held.  max_pages * page <= 2^30, sequences <= 65536, T (count) * kv_heads <=
+ * 2^30.  k, v and the scales are 16-byte aligned, E4M3 codes finite.
  *
  * sbq_paged_append: T new tokens of each sequence (k_new, v_new: device
  * [sequences, T, kv_heads, D], both with strides n_sb, n_st, n_sh, F32, F16 or
@@ -636,11 +637,11 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * cache's type (8-bit caches: any); out: the same shape and type, apart from
  * every input.  Scores, maxima and sums are fp32; fp32 queries are multiplied
  * to 22 significant bits or more, and so are their weights; with 2-byte
- * queries the weights keep 11 bits (bf16 caches: 16).  scale * q . k is to
- * stay below 2^27 in magnitude.
+ * queries the weights keep 16 bits or more (8-bit caches with bf16: 11).
+ * scale * q . k is to be finite, below 2^27 in magnitude.
  * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
- * content; one call at a time.  The result does not depend on timing, nor on other sequences'
- * lengths. */
+ * content; one call at a time.  The result does not depend on timing; how a
+ * long sequence is split, and so its last bits, goes by all sequences' lengths. */
 int64_t sbq_paged_attn_workspace_bytes(int64_t sequences, int64_t T, int64_t heads, int64_t kv_heads,
                                        int64_t D, int64_t page, int64_t max_pages, int64_t window,
                                        int cache_dtype);

@@ -840,7 +840,7 @@ int sbq_paged_append(void* k, void* v, float* k_scale, float* v_scale, int cache
   const int rc = check_paged(k, v, k_scale, v_scale, cache_dtype, pages, page, kv_heads, D, table, sequences, max_pages,
                              length, &s.c);
   if (rc) return rc;
-  if (T < 0 || T > (1 << 30) || n_sb < 0 || n_st < 0 || n_sh < 0) return SBQ_ERR_ARG;
+  if (T < 0 || T > (1 << 30) / kv_heads || n_sb < 0 || n_st < 0 || n_sh < 0) return SBQ_ERR_ARG;
   if (sequences == 0) return SBQ_OK;
   if (!start || (T > 0 && (!k_new || !v_new)) || shifted(start, length, sequences)) return SBQ_ERR_ARG;
   if (counts && (counts == length || shifted(counts, length, sequences))) return SBQ_ERR_ARG;
@@ -860,7 +860,7 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
   const int rc = check_paged(k, v, k_scale, v_scale, cache_dtype, pages, page, kv_heads, D, table, sequences, max_pages,
                              length, &s.c);
   if (rc) return rc;
-  if (count < 0 || count > (1 << 30)) return SBQ_ERR_ARG;
+  if (count < 0 || count > (1 << 30) / kv_heads) return SBQ_ERR_ARG;
   if (sequences == 0 || count == 0) return SBQ_OK;
   if (!start || !k_out || !v_out) return SBQ_ERR_ARG;
   // (a sequence's [count, kv_heads, D] lies apart from the next one's)

@@ -57,6 +57,7 @@ def test_c_abi_refuses_bad_arguments():
         for bad in (dict(k=p + 8), dict(v=p + 4), dict(ks=p + 4), dict(vs=p + 8), dict(table=p + 2), dict(length=p + 4)):
             assert call(**bad) == -3, (call.__name__, bad)
         assert call(B=0) == 0
+    assert append(T=(1 << 29) + 1) == -1 and read(count=(1 << 29) + 1) == -1
     assert append(nt=3) == -2 and append(T=-1) == -1 and append(nst=-1) == -1 and append(start=None) == -1
     assert append(kn=None) == -1 and append(vn=None) == -1
     assert append(start=2 * p + 8) == -1 and append(start=2 * p - 16) == -1  # other sequences' lengths
@@ -166,7 +167,7 @@ def test_largest_launches(grids):
             for rep in (1, 4) if Hk < 65536 else (1,):
                 calls.append(["sbq_paged_attention", "@0", 0, T, rep * Hk, rep * T * row, rep * row, D, *c, None, None, 0, 0.1,
                               "@8", rep * T * row, rep * row, D, "@9", 1 << 50, None])
-        calls.append(["sbq_paged_append", *cache(ct, 8, 128, 1, 64, 1 << 24), "@7", None, "@8", "@9", 2, 1 << 30, 0, 1024, 128,
+        calls.append(["sbq_paged_append", *cache(ct, 8, 128, 1, 64, 1 << 24), "@7", None, "@8", "@9", 2, 1 << 27, 0, 1024, 128,
                       None])
     for B, V in ((1, 1), (65535, 1), (65535, 1 << 23), (7, 151936)):
         calls.append(["sbq_verify_drafts", "@0", 2 * V, V, "@1", V, V, 0, B, 1, V, "@2", "@3", None, "@4", "@5", "@6", 1 << 50,
