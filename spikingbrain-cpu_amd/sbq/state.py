@@ -670,6 +670,19 @@ class DevicePagedKVBuffer:
                                                   count * heads * dim, heads * dim, dim, _stream(dev)), "sbq_paged_read")
         return k, v
 
+    def _query(self, fn: str, q: torch.Tensor) -> int:
+        """The C ABI's type of queries that attend takes."""
+        n, kv_heads, shape = self.sequences, self.heads, q.shape
+        if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != self.dim or shape[-2] % kv_heads or shape[-2] == 0:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: expected q [{n}, T, heads, {self.dim}], heads a multiple of {kv_heads}")
+        if len(shape) == 4 and shape[1] > _lib.SBQ_PAGED_MAX_T:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: at most {_lib.SBQ_PAGED_MAX_T} tokens per call")
+        code = _DTYPE_CODE.get(q.dtype)
+        if q.get_device() != self._gpu or code is None or not (self._b8 or code in (self._sizes[0], _lib.SBQ_F32)):
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: q must be on {self.device}, of the pool's dtype or float32 (8-bit pools: "
+                             "float32, float16 or bfloat16)")
+        return code
+
     def attend(self, q: torch.Tensor, start=None, counts: torch.Tensor | None = None, scale: float | None = None,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """The attention of q [sequences, T, q heads, dim] (or [sequences, q
@@ -683,12 +696,7 @@ class DevicePagedKVBuffer:
         the result has q's."""
         cache = self._cache("attend", None)
         n, gpu, dim, kv_heads, dev, shape = cache[10], self._gpu, self.dim, self.heads, self._dev, q.shape
-        if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != dim or shape[-2] % kv_heads or shape[-2] == 0:
-            raise ValueError(f"DevicePagedKVBuffer.attend: expected q [{n}, T, heads, {dim}], heads a multiple of {kv_heads}")
-        code = _DTYPE_CODE.get(q.dtype)
-        if q.get_device() != gpu or code is None or not (self._b8 or code in (cache[4], _lib.SBQ_F32)):
-            raise ValueError(f"DevicePagedKVBuffer.attend: q must be on {dev}, of the pool's dtype or float32 (8-bit pools: "
-                             "float32, float16 or bfloat16)")
+        code = self._query("attend", q)
         if out is None:
             out = torch.empty(shape, dtype=q.dtype, device=dev)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(-1) != 1):
@@ -696,8 +704,6 @@ class DevicePagedKVBuffer:
         elif out.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("DevicePagedKVBuffer.attend: out must not be q itself")
         T, heads = shape[1] if len(shape) == 4 else 1, shape[-2]
-        if T > _lib.SBQ_PAGED_MAX_T:
-            raise ValueError(f"DevicePagedKVBuffer.attend: at most {_lib.SBQ_PAGED_MAX_T} tokens per call")
         if T == 0:
             return out
         if dim > 1 and q.stride(-1) != 1:
@@ -734,6 +740,12 @@ class DevicePagedKVBuffer:
         if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[0] != self.sequences:
             raise ValueError(f"DevicePagedKVBuffer.step: expected q [{self.sequences}, T, q heads, dim] and k, v "
                              f"[{self.sequences}, T, heads, dim]")
+        if v.shape != k.shape or v.get_device() != k.get_device():
+            raise ValueError(f"DevicePagedKVBuffer.step: v must have k's shape, and be on {self.device}")
+        self._cache("step", None)
+        self._query("step", q)  # (refused before anything is stored)
+        if scale is not None and scale != scale:
+            raise ValueError("DevicePagedKVBuffer.step: scale must be a number")
         qr, kr = qk_norm_rope(q.flatten(0, 1), k.flatten(0, 1), self.length, inv_freq, q_weight, k_weight, eps, interleaved)
         self.append(kr.view(k.shape), v, None, counts)
         return self.attend(qr.view(q.shape), None, counts, scale)

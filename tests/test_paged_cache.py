@@ -731,6 +731,28 @@ def test_step_with_drafts(dev, dtype):
 
 
 @pytest.mark.gpu
+def test_a_refused_step_stores_nothing(dev):
+    B, T, H, heads, dim = 2, 3, 4, 2, 64
+    b = DevicePagedKVBuffer(B, heads, dim, 8, 16, 4, None, dev, F16)
+    for i in range(B):
+        b.reserve(i, 40)
+    f = (1e4 ** -(torch.arange(32) / 32)).to(dev)
+    q, k, v = [torch.randn(B, T, n, dim, device=dev) for n in (H, heads, heads)]
+    b.step(q, k, v, f)
+    before = [t.clone() for t in (b.k, b.v, b.length)]
+    long = [torch.zeros(B, _lib.SBQ_PAGED_MAX_T + 1, n, dim, device=dev) for n in (H, heads, heads)]
+    for bad in (lambda: b.step(q.bfloat16(), k.bfloat16(), v, f), lambda: b.step(q[:, :, :3], k, v, f),
+                lambda: b.step(q, k, v[:, :1], f), lambda: b.step(q, k, v, f, scale=float("nan")), lambda: b.step(*long, f),
+                lambda: b.step(q, k, v, f, counts=torch.ones(3, dtype=torch.long, device=dev))):
+        with pytest.raises(ValueError):
+            bad()
+    none = [t[:, :0] for t in (q, k, v)]
+    assert b.step(*none, f).shape == (B, 0, H, dim)  # no tokens
+    for x, y in zip((b.k, b.v, b.length), before):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, I8])
 def test_step_captured_and_replayed(dev, dtype):
     """A captured step, replayed with other inputs and eager calls between, on another stream too."""
