@@ -752,11 +752,11 @@ class DevicePagedKVBuffer:
 
     def truncate(self, length) -> None:
         """Forget positions >= length (an int or int64 [sequences]), for
-        instance the drafts that were refused."""
+        instance the drafts that were refused; below 0 as 0."""
         if isinstance(length, torch.Tensor):
-            self.length.copy_(torch.minimum(self.length, self._places("truncate", "length", length, self.sequences)))
+            self.length.copy_(torch.minimum(self.length, self._places("truncate", "length", length, self.sequences)).clamp_(min=0))
         else:
-            self.length.clamp_(max=int(length))
+            self.length.clamp_(max=max(0, int(length)))
 
 
 @dataclass

@@ -119,6 +119,8 @@ def test_pages_are_given_out_and_taken_back():
     b.length.copy_(torch.tensor([9, 4, 70]))
     b.truncate(40)
     assert b.length.tolist() == [9, 4, 40]
+    b.truncate(-3)
+    assert b.length.tolist() == [0, 0, 0]
 
 
 def test_buffer_refuses():
@@ -728,6 +730,17 @@ def test_step_with_drafts(dev, dtype):
         assert torch.equal(b.length, start + kept) and torch.equal(plain.length, b.length)
         for x, y in zip(b.read(0, 100), plain.read(0, 100)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_truncate_by_tensors(dev):
+    b = DevicePagedKVBuffer(4, 1, 16, 4, 16, device=dev)
+    b.length.copy_(torch.tensor([5, 9, 0, 7]))
+    b.truncate(torch.tensor([6, 3, 2, -4], device=dev))
+    assert b.length.tolist() == [5, 3, 0, 0]
+    for bad in (torch.tensor([1, 2], device=dev), torch.tensor([1, 2, 3, 4]), torch.ones(4, device=dev)):
+        with pytest.raises(ValueError, match="length"):
+            b.truncate(bad)
 
 
 @pytest.mark.gpu
