@@ -346,7 +346,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   p.SB = ct == XT_F32 ? 16 : 32;
   p.rtiles = (R + 15) / 16;
-  if (window > 0 && window + T < room) room = window + T;  // (what the tokens of a call can look at)
+  if (window > 0 && window < room - T) room = window + T;  // (what the tokens of a call can look at)
   const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB + (window > 0), fours = (blocks + kAttnWaves - 1) / kAttnWaves;
   p.n = std::min(B, kPagedGroup);
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 30) / (fours * kAttnWaves)));  // (all blocks fit an int)

@@ -472,8 +472,8 @@ class DevicePagedKVBuffer:
             raise ValueError("DevicePagedKVBuffer: 1 to 65536 sequences and heads, a dim of at most 256, and pages >= 1")
         if page not in (16, 32, 64, 128, 256, 512, 1024) or max_pages < 1 or max_pages * page > 1 << 30:
             raise ValueError("DevicePagedKVBuffer: page must be a power of two from 16 to 1024, and max_pages * page at most 2^30")
-        if window is not None and window < 1:
-            raise ValueError("DevicePagedKVBuffer: window must be >= 1")
+        if window is not None and not 1 <= window < 1 << 62:
+            raise ValueError("DevicePagedKVBuffer: window must be 1 to 2^62 - 1")
         self.sequences, self.heads, self.dim, self.page, self.window = sequences, heads, dim, page, window
         self._tensors: dict[str, torch.Tensor | None] = {}
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())

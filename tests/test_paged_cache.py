@@ -79,6 +79,8 @@ def test_c_abi_refuses_bad_arguments():
                 (3, 1, 4, 2, 257, 16, 100, 0, 3), (3, 1, 4, 2, 24, 17, 100, 0, 3), (3, 1, 4, 2, 24, 16, 0, 0, 3),
                 (3, 1, 4, 2, 24, 16, 100, -1, 3), (3, 1, 4, 2, 24, 16, 100, 0, 9), (3, 1, 4, 2, 24, 16, 4, 0, 3)):
         assert L.sbq_paged_attn_workspace_bytes(*bad) == 0
+    for window in (1 << 40, (1 << 63) - 1):  # every position
+        assert L.sbq_paged_attn_workspace_bytes(3, 1, 4, 2, 24, 16, 100, window, 3) >= need
 
 
 def test_pages_are_given_out_and_taken_back():
@@ -125,7 +127,8 @@ def test_pages_are_given_out_and_taken_back():
 
 def test_buffer_refuses():
     for bad in (dict(dtype=torch.float64), dict(sequences=0), dict(heads=0), dict(dim=0), dict(dim=257), dict(pages=0),
-                dict(page=8), dict(page=40), dict(page=2048), dict(max_pages=0), dict(max_pages=1 << 27), dict(window=0)):
+                dict(page=8), dict(page=40), dict(page=2048), dict(max_pages=0), dict(max_pages=1 << 27), dict(window=0),
+                dict(window=1 << 62)):
         a = dict(sequences=2, heads=2, dim=8, pages=4, page=16, device="cpu")
         with pytest.raises(ValueError):
             DevicePagedKVBuffer(**{**a, **bad})
