@@ -553,6 +553,61 @@ def test_attention_of_one_long_sequence(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,qt", [(F32, F32), (BF16, BF16), (I8, BF16)])
+@pytest.mark.parametrize("width", [1, 40])
+def test_attention_of_more_sequences_than_a_launch_takes(dev, dtype, qt, width):
+    """600 sequences, some over shared pages, in tables that are not split and that are."""
+    announce(f"attend 600 sequences width={width} {dtype} {qt}")
+    b = _buffer(dev, [16] * 20, 1, 32, 16, dtype, seed=4)
+    many = DevicePagedKVBuffer(600, 1, 32, 1, 16, width, None, dev, dtype)
+    many.k, many.v, many.k_scale, many.v_scale = b.k, b.v, b.k_scale, b.v_scale
+    g = torch.Generator().manual_seed(5)
+    many.table.copy_(b.table.flatten()[torch.randint(0, 20, (600, width), generator=g).to(dev)])
+    many.length.copy_(torch.randint(0, 16 * width + 1, (600,), generator=g))
+    q = torch.randn(600, 1, 3, 32, generator=g).to(qt).to(dev)
+    _compare(many, q, many.attend(q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,qt", [(F16, F32), (E4M3, F16)])
+def test_attention_of_many_tokens(dev, dtype, qt):
+    """Row tiles that begin and end inside a token's heads, over more positions than a workgroup takes whole, pages of 1024."""
+    b = _buffer(dev, [1100, 207, 40], 2, 72, 1024, dtype, seed=9, room=2048)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(3, 207, 6, 72, generator=g).to(qt).to(dev)
+    counts = torch.tensor([207, 207, 31], device=dev)
+    _compare(b, q, b.attend(q, counts=counts), counts=counts)
+    b.window = 77
+    _compare(b, q, b.attend(q, counts=counts), counts=counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,pages", [(I8, 17000), (F32, 4300)])
+def test_pools_and_inputs_past_32_bits(dev, dtype, pages):
+    """Pages more than 4 GiB into the pool, sequences' inputs as far apart, against a small pool and packed inputs."""
+    announce(f"pool of {pages} pages {dtype}")
+    heads, dim, page, T = 2, 128, 1024, 1500
+    small, large = [DevicePagedKVBuffer(2, heads, dim, n, page, 3, None, dev, dtype) for n in (6, pages)]
+    assert large.k.stride(0) * (pages - 1) * large.k.element_size() > 1 << 32
+    small.table.copy_(torch.arange(6).view(2, 3))
+    large.table.copy_(torch.tensor([[pages - 1, 0, pages - 3], [pages - 2, pages - 6, 5]]))
+    apart = torch.empty(2 * T * heads * dim + (1 << 30) + 4096, dtype=F32, device=dev)  # 2^32 bytes between the sequences
+    k, v, q = [apart[i:].as_strided((2, n, h, dim), (1 << 30, h * dim, dim, 1))
+               for i, n, h in ((0, T, heads), (T * heads * dim, T, heads), (2 * T * heads * dim, 2, 4))]
+    g = torch.Generator().manual_seed(7)
+    for x in (k, v, q):
+        x.copy_(torch.randn(x.shape, generator=g))
+    small.append(k.contiguous(), v.contiguous())
+    large.append(k, v)
+    for x, y in zip(large.read(3, T), small.read(3, T)):
+        assert torch.equal(x, y)
+    assert torch.equal(large.attend(q), small.attend(q.contiguous()))
+    kept = small.length.clone()
+    assert torch.equal(large.length, kept) and int(kept[0]) == T
+    _compare(small, q[:, 1:].contiguous(), small.attend(q[:, 1:].contiguous()))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,qt", [(F32, F32), (F16, F16), (I8, F32), (E4M3, BF16)])
 def test_attention_starts_counts_and_missing_pages(dev, dtype, qt):
     lengths, T = [100, 100, 100, 100, 100, 100, 100, 0], 5

@@ -239,3 +239,31 @@ def test_other_stream_and_graph(dev):
         torch.cuda.synchronize()
         eager = qk_norm_rope(q, k, pos, f, wq, wk)
         assert torch.equal(held[0], eager[0]) and torch.equal(held[1], eager[1])
+
+
+@pytest.mark.gpu
+def test_tokens_further_apart_than_32_bits(dev):
+    q, k, pos, f, wq, wk = _case(dev, 3, 2, 1, 64, 32, False, BF16, True)
+    apart = torch.empty(2 * (5 << 28) + 512, dtype=BF16, device=dev)  # 2.5 GiB between tokens
+    views = [apart[i:].as_strided((3, n, 64), (5 << 28, 64, 1)) for i, n in ((0, 2), (128, 1), (192, 2), (320, 1))]
+    views[0].copy_(q)
+    views[1].copy_(k)
+    want = qk_norm_rope(q, k, pos, f, wq, wk)
+    got = qk_norm_rope(views[0], views[1], pos, f, wq, wk, q_out=views[2], k_out=views[3])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_two_streams(dev):
+    """Two calls at once."""
+    cases = [_case(dev, 2000, 8, 2, 128, 64, inter, BF16, True) for inter in (False, True)]
+    want = [qk_norm_rope(q, k, pos, f, wq, wk, interleaved=bool(i)) for i, (q, k, pos, f, wq, wk) in enumerate(cases)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(10):
+        for i, (s, (q, k, pos, f, wq, wk)) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(qk_norm_rope(q, k, pos, f, wq, wk, interleaved=bool(i)))
+    torch.cuda.synchronize()
+    for w, results in zip(want, got):
+        assert all(torch.equal(r[0], w[0]) and torch.equal(r[1], w[1]) for r in results)

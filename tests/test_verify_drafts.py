@@ -254,3 +254,40 @@ def test_other_stream_and_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         _same(held, [w.cpu().numpy() for w in quant.verify_drafts(target, draft, tokens, u)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 20001])
+def test_rows_further_apart_than_32_bits(dev, V):
+    B, T = 2, 1
+    g = torch.Generator().manual_seed(V)
+    target, draft = _probs(g, B, T + 1, V, 1.5, F32), _probs(g, B, T, V, 1.5, F32)
+    tokens, u = torch.randint(0, V, (B, T), generator=g), torch.rand(B, T + 1, generator=g)
+    apart = torch.empty(4 * (3 << 28), device=dev)  # 3 GiB between rows, 6 between sequences
+    p = apart.as_strided((B, T + 1, V), (3 << 29, 3 << 28, 1))
+    q = apart[1 << 27:].as_strided((B, T, V), (3 << 29, 3 << 28, 1))
+    p.copy_(target)
+    q.copy_(draft)
+    _same(*_run(dev, target, draft, tokens, u))
+    got = quant.verify_drafts(p, q, tokens.to(dev), u.to(dev))
+    _same(got, _rule(target.numpy(), draft.numpy(), tokens.numpy(), u.numpy(), None))
+
+
+@pytest.mark.gpu
+def test_two_streams(dev):
+    """Two calls at once, each with a workspace of its own."""
+    g = torch.Generator().manual_seed(11)
+    cases = []
+    for B, T, V in ((9, 3, 40000), (4, 2, 9000)):
+        target, draft = _probs(g, B, T + 1, V, 2.0, BF16).to(dev), _probs(g, B, T, V, 2.0, BF16).to(dev)
+        cases.append((target, draft, torch.randint(0, V, (B, T), generator=g).to(dev), torch.rand(B, T + 1, generator=g).to(dev)))
+    want = [quant.verify_drafts(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(quant.verify_drafts(*c))
+    torch.cuda.synchronize()
+    for w, results in zip(want, got):
+        assert all(torch.equal(r[0], w[0]) and torch.equal(r[1], w[1]) for r in results)
