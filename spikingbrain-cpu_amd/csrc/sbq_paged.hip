@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kStoreThreads = 256;
 constexpr int kStoreAlone = 128;  // vectors of a sequence that one workgroup stores by itself
-constexpr int64_t kStoreGroups = 2048;  // workgroups of a launch at most
+constexpr int64_t kStoreGroups = 1536;  // workgroups of a launch about (8192 x 8 x 128 bf16 to e4m3, at 1024, 1536, 2048, 4096: 15.2, 14.0, 14.9, 15.9 us)
 
 // Largest code of an 8-bit type.
 template <int CT>
@@ -26,18 +26,48 @@ __device__ __forceinline__ float largest() {
   return CT == CT_I8 ? 127.0f : 448.0f;
 }
 
-template <int XT, bool VEC>
-__device__ __forceinline__ void load_cols(const typename XElem<XT>::T* p, int n, float (&x)[8]) {
-  if constexpr (VEC) {
-    if (n > 0) {
-      load8_f32_vec<XT>(p, x);
+// Eight columns as they lie in memory: they become floats where they are used,
+// so that nothing waits for them before the next ones are on their way.
+template <int XT>
+struct Cols {
+  typedef typename XElem<XT>::T T;
+  typedef T V __attribute__((ext_vector_type(8)));
+  V x;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p, int n) {  // (n of them there; VEC: all or none)
+    if constexpr (VEC) {
+      if (n > 0) x = *(const V*)p;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+      for (int j = 0; j < 8; ++j)
+        if (j < n) x[j] = p[j];
     }
-  } else {
+  }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+    for (int j = 0; j < 8; ++j) x[j] = (T)0.0f;
+  }
+  __device__ __forceinline__ void floats(float (&to)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to[j] = (float)x[j];
+  }
+};
+
+// Eight columns to y from element `at` on, n of them there (vec: eight or none).
+__device__ __forceinline__ void store_cols8(void* y, int type, int64_t at, const float (&x)[8], bool vec, int n) {
+  if (vec && type != XT_F32) {
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+      w[j] = type == XT_F16 ? __builtin_bit_cast(uint32_t, (H2){out_f16(x[2 * j]), out_f16(x[2 * j + 1])})
+                            : __builtin_bit_cast(uint32_t, (B2){out_bf16(x[2 * j]), out_bf16(x[2 * j + 1])});
+    }
+    *(u32x4*)((uint16_t*)y + at) = w;
+  } else {
+    store_y4(y, type, at, (f32x4){x[0], x[1], x[2], x[3]}, vec, n);
+    store_y4(y, type, at + 4, (f32x4){x[4], x[5], x[6], x[7]}, vec, n - 4);
   }
 }
 
@@ -102,8 +132,7 @@ __device__ __forceinline__ void store_cols(const PagedCache& c, bool value, int6
     if (d == 0) (value ? c.v_scale : c.k_scale)[at] = scale;
   } else {
     if (n <= 0) return;
-    store_y4(pool, CT, at * c.row + d, (f32x4){x[0], x[1], x[2], x[3]}, true, 4);
-    store_y4(pool, CT, at * c.row + d + 4, (f32x4){x[4], x[5], x[6], x[7]}, true, 4);
+    store_cols8(pool, CT, at * c.row + d, x, true, 8);
   }
 }
 
@@ -113,35 +142,25 @@ __device__ __forceinline__ int64_t paged_end(int64_t start, int64_t count, int64
   return start >= room ? room : start + count < room ? start + count : room;
 }
 
-// Walks a sequence's vectors, `lanes` lanes each, in tiles of a workgroup's lane
+// A sequence's vectors, `lanes` lanes each, in tiles of a workgroup's lane
 // groups: `tile` neighbouring tokens of a head, which stand side by side in a
 // page (as do their scales, that lines of either are written whole), and as
-// many heads as there are groups left.  U tiles at a time: `load` for all of
-// them, then `use`.
-template <int U, class L, class F>
-__device__ __forceinline__ void paged_walk(const PagedStore& a, int part, L load, F use) {
-  const int group = threadIdx.x / a.lanes, t_in = group & (a.tile - 1), h_in = group / a.tile;
-  const int heads = kStoreThreads / a.lanes / a.tile, across = (a.c.Hk + heads - 1) / heads;  // heads of a tile, tiles across them
-  const int tiles = (int)((a.T + a.tile - 1) / a.tile) * across;
-  for (int q0 = part; q0 < tiles; q0 += U * a.parts) {
-    int ts[U], hs[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int q = q0 + u * a.parts, row = q / across;
-      ts[u] = row * a.tile + t_in, hs[u] = (q - row * across) * heads + h_in;
-      if (q >= tiles || hs[u] >= a.c.Hk) ts[u] = INT32_MAX;
-      load(u, ts[u], hs[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (ts[u] < a.T) use(u, ts[u], hs[u]);
+// many heads as there are groups left.
+struct PagedTiles {
+  int t_in, h_in, heads, across, n;  // the group's token and head of a tile, a tile's heads, tiles across them, tiles in all
+  __device__ __forceinline__ explicit PagedTiles(const PagedStore& a) {
+    const int group = threadIdx.x / a.lanes;
+    t_in = group & (a.tile - 1), h_in = group / a.tile;
+    heads = kStoreThreads / a.lanes / a.tile, across = (a.c.Hk + heads - 1) / heads;
+    n = (int)((a.T + a.tile - 1) / a.tile) * across;
   }
-}
-
-// The row of position pos and head h in the pool; -1: it has none.
-__device__ __forceinline__ int64_t paged_row(const PagedCache& c, int64_t b, int64_t pos, int h) {
-  return paged_row_of(c.table[b * c.max_pages + (pos >> c.page_log)], c.pages, pos, h, c.Hk, c.page_log);
-}
+  // The group's token and head of tile q (token INT32_MAX: none).
+  __device__ __forceinline__ void at(const PagedStore& a, int q, int& t, int& h) const {
+    const int row = q / across;
+    t = row * a.tile + t_in, h = (q - row * across) * heads + h_in;
+    if (q >= n || h >= a.c.Hk) t = INT32_MAX;
+  }
+};
 
 template <int CT, int XT, bool VEC>
 __global__ __launch_bounds__(kStoreThreads) void paged_append_kernel(PagedStore a) {
@@ -149,27 +168,39 @@ __global__ __launch_bounds__(kStoreThreads) void paged_append_kernel(PagedStore 
   const PagedCache& c = a.c;
   const int64_t b = blockIdx.x / a.parts, room = (int64_t)c.max_pages << c.page_log;
   const int part = blockIdx.x % a.parts, d = (threadIdx.x & (a.lanes - 1)) * 8, n = c.D - d;
+  // A tile's loads go ahead of the one before it: of its rows, whether the
+  // sequence has as many or not, and of its page, which the length leads to.
+  const PagedTiles tiles(a);
+  Cols<XT> k, v;
+  int t, h;
+  auto fetch = [&](int q) {
+    tiles.at(a, q, t, h);
+    k.zero(), v.zero();
+    if (t >= a.T) return;
+    const int64_t from = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
+    k.template load<VEC>((const T*)a.kn + from, n);
+    v.template load<VEC>((const T*)a.vn + from, n);
+  };
+  fetch(part);
   const int64_t start = a.start[b], count = paged_count(a.counts, b, a.T);
-  constexpr int U = 2;
-  float k[U][8], v[U][8];
-  int64_t at[U];
-  paged_walk<U>(
-      a, part,
-      [&](int u, int t, int h) {
-        const int64_t pos = start + t;
-        at[u] = -1;
-        // (the lanes of a vector go together)
-        if (t >= count || start < 0 || start >= room || pos >= room) return;
-        const int64_t from = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
-        at[u] = paged_row(c, b, pos, h);
-        load_cols<XT, VEC>((const T*)a.kn + from, n, k[u]);
-        load_cols<XT, VEC>((const T*)a.vn + from, n, v[u]);
-      },
-      [&](int u, int, int) {
-        if (at[u] < 0) return;
-        store_cols<CT>(c, false, at[u], d, n, k[u], a.lanes);
-        store_cols<CT>(c, true, at[u], d, n, v[u], a.lanes);
-      });
+  int32_t id = -1;
+  auto look_up = [&]() {
+    const int64_t pos = start + t;
+    id = t >= count || start < 0 || start >= room || pos >= room ? -1 : c.table[b * c.max_pages + (pos >> c.page_log)];
+  };
+  look_up();
+  for (int q = part; q < tiles.n; q += a.parts) {
+    const Cols<XT> k0 = k, v0 = v;
+    const int64_t at = paged_row_of(id, c.pages, start + t, h, c.Hk, c.page_log);
+    fetch(q + a.parts);
+    look_up();
+    if (at < 0) continue;  // (the lanes of a vector go together)
+    float x[8];
+    k0.floats(x);
+    store_cols<CT>(c, false, at, d, n, x, a.lanes);
+    v0.floats(x);
+    store_cols<CT>(c, true, at, d, n, x, a.lanes);
+  }
   if (a.set_length && part == 0) {
     __syncthreads();  // (start may be the length itself, then with one workgroup a sequence)
     if (threadIdx.x == 0) c.length[b] = paged_end(start, count, room);
@@ -183,28 +214,41 @@ __global__ __launch_bounds__(kStoreThreads) void paged_length_kernel(PagedStore 
   a.c.length[b] = paged_end(start, paged_count(a.counts, b, a.T), room);
 }
 
+// Eight columns of a row of the pool, and its scale.
 template <int CT>
-__device__ __forceinline__ void read_cols(const PagedCache& c, bool value, int64_t at, int d, float (&x)[8]) {
-  const void* const pool = value ? c.v : c.k;
-  if constexpr (is_8bit(CT)) {
-    const u32x2 w = *(const u32x2*)((const uint8_t*)pool + at * c.row + d);
-    const float scale = (value ? c.v_scale : c.k_scale)[at];
+struct Held : Cols<CT> {
+  __device__ __forceinline__ void zero() { Cols<CT>::zero(); }
+  __device__ __forceinline__ void load(const PagedCache& c, bool value, int64_t at, int d) {
+    Cols<CT>::template load<true>((const typename XElem<CT>::T*)(value ? c.v : c.k) + at * c.row + d, 8);
+  }
+};
+template <>
+struct Held<CT_I8> {
+  u32x2 w;
+  float scale;
+  __device__ __forceinline__ void zero() { w = (u32x2){0, 0}, scale = 0.0f; }
+  __device__ __forceinline__ void load(const PagedCache& c, bool value, int64_t at, int d) {
+    w = *(const u32x2*)((const uint8_t*)(value ? c.v : c.k) + at * c.row + d);
+    scale = (value ? c.v_scale : c.k_scale)[at];
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale;
+  }
+};
+template <>
+struct Held<CT_E4M3> : Held<CT_I8> {
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if constexpr (CT == CT_I8) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * h + j] = (float)(int8_t)(w[h] >> (8 * j)) * scale;
-      } else {
-        x[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 0) * scale;
-        x[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 1) * scale;
-        x[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 2) * scale;
-        x[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[h], 3) * scale;
-      }
+      const int v = (int)w[h];
+      x[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(v, 0) * scale;
+      x[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(v, 1) * scale;
+      x[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(v, 2) * scale;
+      x[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(v, 3) * scale;
     }
-  } else {
-    load8_f32_vec<CT>((const typename XElem<CT>::T*)pool + at * c.row + d, x);
   }
-}
+};
 
 // Positions start .. start + T - 1 of each sequence, zeros for those it does not hold.
 template <int CT>
@@ -214,27 +258,42 @@ __global__ __launch_bounds__(kStoreThreads) void paged_read_kernel(PagedStore a)
   const int part = blockIdx.x % a.parts, d = (threadIdx.x & (a.lanes - 1)) * 8, n = c.D - d;
   const int64_t start = a.start[b], held = c.length[b] < room ? c.length[b] : room;
   if (n <= 0) return;
-  constexpr int U = 2;
-  float k[U][8], v[U][8];
-  paged_walk<U>(
-      a, part,
-      [&](int u, int t, int h) {
-        const int64_t pos = start + t;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) k[u][j] = v[u][j] = 0.0f;
-        if (t >= a.T || pos < 0 || pos >= held) return;
-        const int64_t at = paged_row(c, b, pos, h);
-        if (at < 0) return;
-        read_cols<CT>(c, false, at, d, k[u]);
-        read_cols<CT>(c, true, at, d, v[u]);
-      },
-      [&](int u, int t, int h) {
-        const int64_t to = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
-        store_y4(a.k_out, a.xt, to, (f32x4){k[u][0], k[u][1], k[u][2], k[u][3]}, a.vec && n >= 4, n);
-        store_y4(a.k_out, a.xt, to + 4, (f32x4){k[u][4], k[u][5], k[u][6], k[u][7]}, a.vec && n >= 8, n - 4);
-        store_y4(a.v_out, a.xt, to, (f32x4){v[u][0], v[u][1], v[u][2], v[u][3]}, a.vec && n >= 4, n);
-        store_y4(a.v_out, a.xt, to + 4, (f32x4){v[u][4], v[u][5], v[u][6], v[u][7]}, a.vec && n >= 8, n - 4);
-      });
+  // A tile's rows are on their way before the one ahead of it is written, its page before that.
+  const PagedTiles tiles(a);
+  int32_t id;
+  auto look_up = [&](int q) {
+    int t, h;
+    tiles.at(a, q, t, h);
+    const int64_t pos = start + t;
+    id = t >= a.T || pos < 0 || pos >= held ? -1 : c.table[b * c.max_pages + (pos >> c.page_log)];
+  };
+  Held<CT> k, v;
+  auto fetch = [&](int q) {
+    int t, h;
+    tiles.at(a, q, t, h);
+    k.zero(), v.zero();
+    const int64_t at = paged_row_of(id, c.pages, start + t, h, c.Hk, c.page_log);
+    if (at < 0) return;
+    k.load(c, false, at, d);
+    v.load(c, true, at, d);
+  };
+  look_up(part);
+  fetch(part);
+  look_up(part + a.parts);
+  for (int q = part; q < tiles.n; q += a.parts) {
+    const Held<CT> k0 = k, v0 = v;
+    fetch(q + a.parts);
+    look_up(q + 2 * a.parts);
+    int t, h;
+    tiles.at(a, q, t, h);
+    if (t >= a.T) continue;
+    const int64_t to = b * a.n_sb + (int64_t)t * a.n_st + (int64_t)h * a.n_sh + d;
+    float x[8];
+    k0.floats(x);
+    store_cols8(a.k_out, a.xt, to, x, a.vec && n >= 8, n);
+    v0.floats(x);
+    store_cols8(a.v_out, a.xt, to, x, a.vec && n >= 8, n);
+  }
 }
 
 template <int CT, int XT>
@@ -258,7 +317,7 @@ int launch_read_ct(const PagedStore& a, unsigned grid, hipStream_t st) {
 }
 
 // Lanes of a vector, and how many workgroups share a sequence's vectors: each
-// wave a few, up to about 8 workgroups a CU.
+// wave a few, up to about 6 workgroups a CU.
 void plan(PagedStore& a) {
   a.lanes = 1;
   while (a.lanes * 8 < a.c.D) a.lanes <<= 1;
@@ -442,9 +501,9 @@ int launch_paged_append(const PagedStore& c, hipStream_t st) {
 int launch_paged_read(const PagedStore& c, hipStream_t st) {
   PagedStore a = c;
   plan(a);
-  const int64_t n = a.xt == XT_F32 ? 16 : 8;
-  a.vec = (uintptr_t)a.k_out % n == 0 && (uintptr_t)a.v_out % n == 0 && a.n_sb % 4 == 0 && a.n_st % 4 == 0 && a.n_sh % 4 == 0;
-  const int64_t es = a.xt == XT_F32 ? 4 : 2, B = a.c.B, most = std::max<int64_t>(1, kLaunchThreads / kStoreThreads / a.parts);
+  const int64_t es = a.xt == XT_F32 ? 4 : 2, n = 16 / es;
+  a.vec = (uintptr_t)a.k_out % 16 == 0 && (uintptr_t)a.v_out % 16 == 0 && a.n_sb % n == 0 && a.n_st % n == 0 && a.n_sh % n == 0;
+  const int64_t B = a.c.B, most = std::max<int64_t>(1, kLaunchThreads / kStoreThreads / a.parts);
   for (int64_t b0 = 0; b0 < B; b0 += most) {
     PagedStore s = a;
     s.c.B = std::min(most, B - b0);
