@@ -105,6 +105,8 @@ SBQ_HD int paged_each(int total, int slots, float per_slot) {  // per_slot: 1 / 
   while ((int64_t)n * slots < total) ++n;
   return n < kPagedWaves ? kPagedWaves : n;
 }
+// A sequence's blocks in whole parts: then no part holds two sequences, if the slots suffice.
+SBQ_HD int paged_padded(int own, int each) { return (int)(((unsigned)own + (unsigned)each - 1u) / (unsigned)each) * each; }
 SBQ_HD void paged_piece(int slot, int each, int before, int blocks, int& n0, int& n1) {  // (none: n0 >= n1)
   const int64_t x0 = (int64_t)slot * each;
   const int own = blocks > 1 ? blocks : 1;

@@ -124,13 +124,16 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // How the slots, the workgroups of a key head and row tile, share a launch's
-// sequences (the arithmetic is in sbq_index.h).  All sequences' blocks, one sequence after another and
-// each in whole fours (one block for each wave), are cut into equal parts of
-// four blocks or more, one for each slot: a long sequence among short ones has
-// as much of the chip as its length asks for, whatever the host knows of
-// lengths, and while there are slots enough none holds two sequences.  A part
-// that meets several does them in turn.  Slot s's piece of sequence b leaves
-// its partial results at place s + b, of which a sequence's are neighbours.
+// sequences (the arithmetic is in sbq_index.h).  All sequences' blocks, one
+// sequence after another and each in whole fours (one block for each wave), are
+// cut into equal parts of four blocks or more, one for each slot: a long
+// sequence among short ones has as much of the chip as its length asks for,
+// whatever the host knows of lengths.  A part that meets several does them in
+// turn, which costs it the way to the first keys and the joining of its waves
+// again (about what kPagedLonger fours cost): where parts of up to so many more
+// are enough for the sequences to begin with a part each, they do.  Slot s's
+// piece of sequence b leaves its partial results at place s + b, of which a
+// sequence's are neighbours.
 // Every workgroup finds its part by a scan over the lengths.  Where no sequence
 // is long (kPagedWhole), each has a workgroup of its own, and nothing is joined.
 struct PagedPlace {
@@ -138,6 +141,8 @@ struct PagedPlace {
   int before, own;      // the parts' blocks before it, and its own
   int each, total;      // a part's, and all
 };
+constexpr int kPagedLonger = 3;
+
 template <bool UNIFORM>
 __device__ __forceinline__ void paged_look(const PagedArgs& a, int b, int t0, int t1, int SB, PagedPlace& p) {
   PagedSpan span;
@@ -180,6 +185,16 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
     p.total += __builtin_amdgcn_readlane(sum, 63);
   }
   p.each = paged_each(p.total, a.slots, a.per_slot);
+  if (a.n <= 64 && 2 * a.n <= a.slots && p.each > kPagedWaves) {  // (parts of one four hold one sequence anyway)
+    const int e0 = (p.each + kPagedWaves - 1) & ~(kPagedWaves - 1);
+    for (int e = e0; e < e0 + kPagedLonger * kPagedWaves; e += kPagedWaves) {
+      const int own = paged_padded(l.own, e), before = wave_scan(own), all = __builtin_amdgcn_readlane(before, 63);
+      if (all <= (int64_t)a.slots * e) {
+        l.own = own, sum = before, p.total = all, p.each = e;
+        break;
+      }
+    }
+  }
   p.b = a.n;
   if (BY_SLOT && (int64_t)key * p.each >= p.total) return p;
   const int at = key * p.each;

@@ -408,7 +408,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int
   if (window > 0 && window < room - T) room = window + T;  // (what the tokens of a call can look at)
   const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB + (window > 0), fours = (blocks + kAttnWaves - 1) / kAttnWaves;
   p.n = std::min(B, kPagedGroup);
-  p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 30) / (fours * kAttnWaves)));  // (all blocks fit an int)
+  p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 29) / (fours * kAttnWaves)));  // (all blocks fit an int, in whole parts too)
   const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
   if (fours <= kPagedWhole) p.slots = 0;

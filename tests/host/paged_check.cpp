@@ -42,24 +42,41 @@ int main() {
   for (int round = 0; round < 3000; ++round) {
     const int n = 1 + (int)below(round % 3 ? 20 : 512), slots = 1 + (int)below(round % 2 ? 1024 : 40);
     const float per_slot = 1.0f / (float)slots;
-    std::vector<int> blocks(n), before(n);
+    std::vector<int> blocks(n), before(n), own(n);
     int64_t total = 0;
     const int64_t top = (int64_t)1 << below(round % 5 ? 12 : 20);
     for (int b = 0; b < n; ++b) {
       blocks[b] = (int)below(below(4) ? top + 1 : 3);
       before[b] = (int)total;
-      total += paged_own(blocks[b]);
+      total += own[b] = paged_own(blocks[b]);
       if (paged_own(blocks[b]) < blocks[b] || paged_own(blocks[b]) % kPagedWaves) return fail("own", blocks[b]);
     }
-    const int each = paged_each((int)total, slots, per_slot);
+    int each = paged_each((int)total, slots, per_slot);
     if (each < kPagedWaves || (int64_t)each * slots < total) return fail("each", each, slots, total);
     if (each > kPagedWaves && (int64_t)(each - 1) * slots >= total) return fail("each too large", each, slots, total);
-    std::vector<char> used(slots + n);
+    bool padded = false;
+    if (n <= slots && round % 4) {  // each sequence from a part of its own on, where the slots suffice
+      const int e = (each + 3) / 4 * 4 + 4 * (int)below(3);
+      int64_t all = 0;
+      for (int b = 0; b < n; ++b) {
+        const int p = paged_padded(own[b], e);
+        if (p < own[b] || p >= own[b] + e || p % e) return fail("padded", own[b], e, p);
+        all += p;
+      }
+      if (all <= (int64_t)slots * e) {
+        padded = true, each = e, total = 0;
+        for (int b = 0; b < n; ++b) {
+          before[b] = (int)total;
+          total += own[b] = paged_padded(own[b], e);
+        }
+      }
+    }
+    std::vector<char> used(slots + n), taken(slots);
     for (int b = 0; b < n; ++b) {
       int first, covered = 0;
       const int count = paged_places(b, each, before[b], blocks[b], first);
       if (count < 1 || first < 0 || first + count > slots + n) return fail("places", b, first, count);
-      const int s_from = before[b] / each, s_to = (before[b] + paged_own(blocks[b]) - 1) / each;
+      const int s_from = before[b] / each, s_to = (before[b] + own[b] - 1) / each;
       if (s_to >= slots) return fail("slot", s_to, slots);
       for (int s = 0; s < slots; ++s) {
         if (s < s_from - 2 || s > s_to + 2) continue;
@@ -68,6 +85,7 @@ int main() {
         if (n0 >= n1) continue;
         if (n0 != covered || n1 > (blocks[b] > 1 ? blocks[b] : 1)) return fail("piece", b, n0, n1);
         covered = n1;
+        if (taken[s]++ && padded) return fail("two sequences in a part", b, s);
         const int place = s + b;
         if (place < first || place >= first + count || used[place]++) return fail("place", b, s, place);
       }
