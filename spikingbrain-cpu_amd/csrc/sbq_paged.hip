@@ -341,29 +341,34 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   const int r = blockIdx.x, kvh = blockIdx.y;
   int t = 0, t0 = 0, t1 = 0;
   if (a.T > 1) t = r / a.rep, t0 = (r & ~15) / a.rep, t1 = min(r | 15, R - 1) / a.rep;
+  const int64_t b = a.first + blockIdx.z;
+  PagedSpan span;
+  span.of<true>(a, b);
+  const bool any = span.last(t) >= span.first(t, a.window);
   const PagedPlace p = paged_place<false>(a, blockIdx.z, t0, t1, SB);
   int place;
   const int used = paged_places(p.b, p.each, p.before, p.blocks, place);
   if (used == 1) return;  // (written by the one workgroup)
-  const int64_t b = a.first + p.b, at = ((int64_t)kvh * a.places + place) * R + r;
-  PagedSpan span;
-  span.of<true>(a, b);
+  const int64_t at = ((int64_t)kvh * a.places + place) * R + r;
   const float2* const ml = a.part_ml + at;
-  float top = -__builtin_inff();
-  for (int s = lane; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
-  top = wave_max(top);
-  const float from = top == -__builtin_inff() ? 0.0f : top;
-  f32x4 sum = (f32x4)(0.0f);
-  float l = 0.0f;
-  for (int s0 = grp; s0 < used; s0 += U * NG) {
-    f32x4 x[U];
-    float2 y[U];
+  float top = -__builtin_inff(), l = 0.0f;
+  if (lane < used) top = ml[(int64_t)lane * R].x;
+  f32x4 x[U], sum = (f32x4)(0.0f);
+  float2 y[U];
+  auto fetch = [&](int s0) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int s = min(s0 + k * NG, used - 1);
       x[k] = *(const f32x4*)(a.part_o + (at + (int64_t)s * R) * DP + d);
       y[k] = ml[(int64_t)s * R];
     }
+  };
+  fetch(grp);  // (on their way while the maximum is found)
+  for (int s = lane + 64; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
+  top = wave_max(top);
+  const float from = top == -__builtin_inff() ? 0.0f : top;
+  for (int s0 = grp; s0 < used; s0 += U * NG) {
+    if (s0 != grp) fetch(s0);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const float f = __builtin_amdgcn_exp2f(y[k].x - from);
@@ -384,7 +389,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
     l += lds_l[k];
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  sum = span.last(t) >= span.first(t, a.window) ? sum * inv : (f32x4)(0.0f);
+  sum = any ? sum * inv : (f32x4)(0.0f);
   const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r - t * a.rep) * a.o_sh + d;
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
