@@ -17,7 +17,10 @@ namespace sbq {
 namespace {
 
 constexpr int kStoreThreads = 256;
-constexpr int kStoreAlone = 128;  // vectors of a sequence that one workgroup stores by itself
+// Vectors of a sequence that one workgroup stores by itself, and moves the length; more
+// need a second launch for that (32 vectors of 128 int8 columns 6.3 us the one way, 6.1
+// the other, eager 3 us less; 128 vectors 14.8 against 6.0).
+constexpr int kStoreAlone = 32;
 constexpr int64_t kStoreGroups = 1536;  // workgroups of a launch about (8192 x 8 x 128 bf16 to e4m3, at 1024, 1536, 2048, 4096: 15.2, 14.0, 14.9, 15.9 us)
 
 // Largest code of an 8-bit type.
@@ -394,8 +397,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
 
-constexpr int64_t kPagedWhole = 4;    // blocks of a wave up to which a workgroup takes a whole sequence
-constexpr int64_t kPagedGroup = 512;  // sequences of a launch at most (each workgroup scans their lengths)
+// Rounds of a wave's blocks up to which a workgroup takes a whole sequence, which
+// saves the joining and, where a workgroup would do several sequences' parts in
+// turn, the way to each one's first keys; what it costs is the wait for the longest.
+// So: kPagedWhole rounds, and kPagedWholeFull more (kPagedWholeMost in all) for each
+// time that the sequences' workgroups fill the chip.  8 key heads of 128 columns,
+// e4m3 or int8, all sequences full / of lengths spread evenly / one full among
+// short ones, whole against split in us: 16 x 512 positions 9.8 against 13.4, 16 x
+// 1024 15.8 against 16.1, 1 x 1024 15.0 against 10.4; 64 x 2048 47, 33, 21 against
+// 52, 39, 17; 128 x 4096 193, 130, 35 against 212, 127, 30; 256 x 4096 377, 231, 40
+// against 408, 255, 60.
+constexpr int64_t kPagedWhole = 4, kPagedWholeFull = 12, kPagedWholeMost = 32;
+constexpr int64_t kPagedGroup = 512;   // sequences of a launch that are split at most (each workgroup scans their lengths)
+constexpr int64_t kPagedRows = 65535;  // ... of one that are not: the grid's limit
 
 struct PagedPlan {
   int DP, SB;
@@ -416,7 +430,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 29) / (fours * kAttnWaves)));  // (all blocks fit an int, in whole parts too)
   const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
-  if (fours <= kPagedWhole) p.slots = 0;
+  if (fours <= std::min(kPagedWhole + kPagedWholeFull * B * one / groups, kPagedWholeMost)) p.slots = 0, p.n = std::min(B, kPagedRows);
   p.places = p.slots + p.n;
   p.joins = p.slots > 1;
   return p;

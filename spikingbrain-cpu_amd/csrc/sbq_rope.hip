@@ -234,8 +234,10 @@ int launch_rope(const RopeArgs& c, bool inter, int xt, hipStream_t st) {
   while (a.lanes < items) a.lanes <<= 1;
   const int groups = kRopeThreads / a.lanes;
   a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kRopeTokens, a.T / 1024));
-  // few tokens: a vector a lane group, on as many workgroups as that takes
-  a.parts = a.T < 512 ? (a.rows + groups - 1) / groups : 1;
+  // few tokens: a vector a lane group, on as many workgroups as that takes; else a
+  // workgroup a token's vectors (40 x 128 bf16: 1, 200, 256, 300, 400 tokens 6.1, 7.1,
+  // 7.2, 9.3, 11.0 us the one way, 7.0, 7.4, 7.5, 7.9, 8.2 the other)
+  a.parts = a.T <= 256 ? (a.rows + groups - 1) / groups : 1;
   const size_t lds = (size_t)a.tokens * ((a.pairs + N - 1) / N) * N * sizeof(float2);
   const int64_t most = kLaunchThreads / kRopeThreads / a.parts * a.tokens;  // tokens of a launch
   for (int64_t t0 = 0; t0 < c.T; t0 += most) {
