@@ -74,6 +74,7 @@ struct PagedArgs {
   void* out;
   float* part_o;    // [Hk][places][R][DP]
   float2* part_ml;  // [Hk][places][R]
+  int2* joins;      // [row tiles][n]: a sequence's first place, and how many
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
   int T, rep, qt;
   int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile (0: one each), and both
@@ -134,8 +135,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 // are enough for the sequences to begin with a part each, they do.  Slot s's
 // piece of sequence b leaves its partial results at place s + b, of which a
 // sequence's are neighbours.
-// Every workgroup finds its part by a scan over the lengths.  Where no sequence
-// is long (kPagedWhole), each has a workgroup of its own, and nothing is joined.
+// Every workgroup finds its part by a scan over the lengths; which places a
+// sequence's are the workgroup of its first block notes for the joining.  Where no
+// sequence is long (kPagedWhole), each has a workgroup of its own, and nothing is
+// joined.
 struct PagedPlace {
   int b, from, blocks;  // the sequence (n: none), its first block and how many (0: sees nothing)
   int before, own;      // the parts' blocks before it, and its own
@@ -152,15 +155,13 @@ __device__ __forceinline__ void paged_look(const PagedArgs& a, int b, int t0, in
   p.blocks = hi >= lo ? hi / SB + 1 - p.from : 0;
   p.own = paged_own(p.blocks);
 }
-// BY_SLOT: the sequence that slot `key`'s part begins in, else sequence `key`.
-// t0, t1: the row tile's first and last token.
-template <bool BY_SLOT>
-__device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, int t0, int t1, int SB) {
+// The sequence that a slot's part begins in.  t0, t1: the row tile's first and last token.
+__device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int slot, int t0, int t1, int SB) {
   PagedPlace p;
   p.before = 0;
   if (a.slots == 0) {  // a slot for every sequence
-    p.b = key;
-    paged_look<true>(a, key, t0, t1, SB, p);
+    p.b = slot;
+    paged_look<true>(a, slot, t0, t1, SB, p);
     p.total = p.each = p.own;
     return p;
   }
@@ -168,7 +169,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
     paged_look<true>(a, 0, t0, t1, SB, p);
     p.total = p.own;
     p.each = paged_each(p.total, a.slots, a.per_slot);
-    p.b = BY_SLOT && (int64_t)key * p.each >= p.total ? 1 : 0;
+    p.b = (int64_t)slot * p.each >= p.total ? 1 : 0;
     return p;
   }
   const int lane = threadIdx.x & 63;
@@ -196,11 +197,11 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs& a, int key, i
     }
   }
   p.b = a.n;
-  if (BY_SLOT && (int64_t)key * p.each >= p.total) return p;
-  const int at = key * p.each;
+  if ((int64_t)slot * p.each >= p.total) return p;
+  const int at = slot * p.each;
   for (int b0 = 0; b0 < a.n; b0 += 64) {
     if (a.n > 64) look(b0);
-    const int i = BY_SLOT ? __builtin_popcountll(__ballot(p.before + sum <= at)) : key - b0;
+    const int i = __builtin_popcountll(__ballot(p.before + sum <= at));
     if (i < 64) {
       p.b = b0 + i;
       p.own = __builtin_amdgcn_readlane(l.own, i), p.from = __builtin_amdgcn_readlane(l.from, i);
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   if (R > 16) row0 = kvh / pc.Hk * 16, kvh %= pc.Hk;
   int t0 = 0, t1 = 0;
   if (a.T > 1) t0 = row0 / a.rep, t1 = min(row0 + 15, R - 1) / a.rep;
-  PagedPlace p = paged_place<true>(a, slot, t0, t1, SB);
+  PagedPlace p = paged_place(a, slot, t0, t1, SB);
   if (p.b >= a.n) return;
 
   for (;;) {
@@ -699,9 +700,11 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       }
 
       // the workgroup's waves joined
-      int place;
-      const bool alone = paged_places(p.b, p.each, p.before, p.blocks, place) == 1;
-      place = slot + p.b;
+      int first = 0, places = 1;
+      if (a.slots) places = paged_places(p.b, p.each, p.before, p.blocks, first);
+      const int place = slot + p.b;
+      const bool alone = places == 1;
+      if (a.joins && n0 == 0 && kvh == 0 && tid == 0) a.joins[row0 / 16 * a.n + p.b] = make_int2(first, places);
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
       __syncthreads();  // (every wave has read its Q)

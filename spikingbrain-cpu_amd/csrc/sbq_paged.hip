@@ -333,26 +333,21 @@ void plan(PagedStore& a) {
 }
 
 // One row's splits joined: the maximum over their maxima, then the partial sums
-// scaled to it, independent loads eight at a time.  How many splits have
-// written theirs follows from the length, as in paged_attn_kernel.
+// scaled to it, independent loads eight at a time.
 template <int DP>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   constexpr int ND = DP / 4, NG = 256 / ND, U = 8;
   __shared__ __align__(16) f32x4 lds[NG][ND];
   __shared__ float lds_l[NG];
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
-  const int r = blockIdx.x, kvh = blockIdx.y;
-  int t = 0, t0 = 0, t1 = 0;
-  if (a.T > 1) t = r / a.rep, t0 = (r & ~15) / a.rep, t1 = min(r | 15, R - 1) / a.rep;
+  const int r = blockIdx.x, kvh = blockIdx.y, t = a.T > 1 ? r / a.rep : 0;
   const int64_t b = a.first + blockIdx.z;
+  const int2 places = a.joins[r / 16 * a.n + (int)blockIdx.z];
   PagedSpan span;
   span.of<true>(a, b);
-  const bool any = span.last(t) >= span.first(t, a.window);
-  const PagedPlace p = paged_place<false>(a, blockIdx.z, t0, t1, SB);
-  int place;
-  const int used = paged_places(p.b, p.each, p.before, p.blocks, place);
+  const int used = places.y;
   if (used == 1) return;  // (written by the one workgroup)
-  const int64_t at = ((int64_t)kvh * a.places + place) * R + r;
+  const int64_t at = ((int64_t)kvh * a.places + places.x) * R + r;
   const float2* const ml = a.part_ml + at;
   float top = -__builtin_inff(), l = 0.0f;
   if (lane < used) top = ml[(int64_t)lane * R].x;
@@ -392,7 +387,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
     l += lds_l[k];
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  sum = any ? sum * inv : (f32x4)(0.0f);
+  sum = span.last(t) >= span.first(t, a.window) ? sum * inv : (f32x4)(0.0f);
   const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r - t * a.rep) * a.o_sh + d;
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }
@@ -402,12 +397,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int SB) {
 // turn, the way to each one's first keys; what it costs is the wait for the longest.
 // So: kPagedWhole rounds, and kPagedWholeFull more (kPagedWholeMost in all) for each
 // time that the sequences' workgroups fill the chip.  8 key heads of 128 columns,
-// e4m3 or int8, all sequences full / of lengths spread evenly / one full among
-// short ones, whole against split in us: 16 x 512 positions 9.8 against 13.4, 16 x
-// 1024 15.8 against 16.1, 1 x 1024 15.0 against 10.4; 64 x 2048 47, 33, 21 against
-// 52, 39, 17; 128 x 4096 193, 130, 35 against 212, 127, 30; 256 x 4096 377, 231, 40
-// against 408, 255, 60.
-constexpr int64_t kPagedWhole = 4, kPagedWholeFull = 12, kPagedWholeMost = 32;
+// e4m3, all sequences full / of lengths spread evenly / one full among short ones,
+// whole against split in us: 16 x 512 positions 9.8 against 13.4 (all full), 16 x 1024
+// 16.0, 13.6, 13.4 against 15.4, 14.4, 10.5; 64 x 2048 46, 34, 21 against 48, 41, 16;
+// 256 x 2048 191, 119, 24 against 199, 126, 34; 256 x 4096 374, 233, 40 against 379,
+// 233, 34.
+constexpr int64_t kPagedWhole = 4, kPagedWholeFull = 12, kPagedWholeMost = 16;
 constexpr int64_t kPagedGroup = 512;   // sequences of a launch that are split at most (each workgroup scans their lengths)
 constexpr int64_t kPagedRows = 65535;  // ... of one that are not: the grid's limit
 
@@ -446,7 +441,7 @@ int64_t paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t heads, int64_t 
   for (bool wide : {false, true}) {  // (the queries' type is not known here)
     const PagedPlan p = paged_plan(B, T, R, Hk, D, room, window, ct, wide);
     const int64_t parts = Hk * R * p.places;
-    if (p.joins) n = std::max(n, round256(parts * p.DP * 4) + round256(parts * 8));
+    if (p.joins) n = std::max(n, round256(parts * p.DP * 4) + round256(parts * 8) + p.rtiles * p.n * 8);
   }
   return n;
 }
@@ -465,6 +460,7 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   if (p.joins) {
     a.part_o = (float*)c.ws;
     a.part_ml = (float2*)((uint8_t*)c.ws + round256(Hk * R * p.places * p.DP * 4));
+    a.joins = (int2*)((uint8_t*)a.part_ml + round256(Hk * R * p.places * 8));
   }
   for (a.first = 0; a.first < B; a.first += p.n) {
     a.n = (int)std::min(p.n, B - a.first);
@@ -478,11 +474,11 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
     if (!p.joins) continue;
     const dim3 joins((unsigned)R, (unsigned)Hk, (unsigned)a.n);
     if (p.DP == 64)
-      paged_join_kernel<64><<<joins, 256, 0, st>>>(a, p.SB);
+      paged_join_kernel<64><<<joins, 256, 0, st>>>(a);
     else if (p.DP == 128)
-      paged_join_kernel<128><<<joins, 256, 0, st>>>(a, p.SB);
+      paged_join_kernel<128><<<joins, 256, 0, st>>>(a);
     else
-      paged_join_kernel<256><<<joins, 256, 0, st>>>(a, p.SB);
+      paged_join_kernel<256><<<joins, 256, 0, st>>>(a);
     if ((rc = check_launch())) return rc;
   }
   return 0;
