@@ -603,7 +603,7 @@ int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, in
  *
  * sbq_paged_append: T new tokens of each sequence (k_new, v_new: device
  * [sequences, T, kv_heads, D], both with strides n_sb, n_st, n_sh, F32, F16 or
- * BF16), of which the first counts[b] (NULL: all; device int64, limited to 0 ..
+ * BF16, apart from the pool), of which the first counts[b] (NULL: all; device int64, limited to 0 ..
  * T) are there, go to the positions start[b] on (device int64; may be `length`
  * itself, not a part of it elsewhere); length[b] = start[b] + counts[b], at
  * most max_pages * page (a token past that is dropped).  8-bit caches:
@@ -669,8 +669,9 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
  *     draft's rows (p's own where nothing is left), or p's row counts[b].
  * Products and sums are 64-bit.  A draft outside 0 .. V - 1 is refused.  token
  * is -1 where the whole mass is 0, infinite or NaN.  B, T <= 65535.
- * kept, token: device int64 [B].  workspace: >= sbq_verify_workspace_bytes
- * bytes (0: NULL will do), any content; one call at a time. */
+ * kept, token: device int64 [B], apart from every input.  workspace: >=
+ * sbq_verify_workspace_bytes bytes (0: NULL will do), any content; one call at
+ * a time. */
 int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V);
 int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st,
                       int dtype, int64_t B, int64_t T, int64_t V, const int64_t* tokens, const float* u,

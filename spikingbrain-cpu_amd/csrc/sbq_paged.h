@@ -51,8 +51,10 @@ __device__ __forceinline__ int64_t paged_count(const int64_t* counts, int64_t b,
 // four positions of row c, the operand that O^T = V^T P^T needs.  A wave walks
 // blocks of SB positions, loads their keys and values straight to registers
 // and keeps a running maximum and sum; LDS only joins a workgroup's waves.
-// The cache's bytes, read once, bound long sequences; short ones are bound by
-// the instructions around the loop, which every wave of a CU issues in turn.
+// The cache's bytes, read once, bound long sequences (32 query heads over 8 x 128:
+// 65536 bf16 positions 53 us, 5.1 TB/s with the joining; 64 sequences of up to 16384
+// e4m3 ones 116 us, 4.9 TB/s); short ones the way to the first keys (launch, lengths,
+// page: 3 us) and from the last ones (3 us, and 4 for the joining).
 //
 // Types of the products:
 //   fp32 cache: fp32 (16x16x4).
@@ -273,7 +275,10 @@ struct Pair {
   }
 };
 
-// Workgroups of a CU that the registers are bounded for.
+// Workgroups of a CU that the registers are bounded for, as many as a launch has: the
+// next block's keys and values lie in them (128 columns: 160 to 235 registers; three
+// workgroups a CU, in fewer registers or waiting for their turn, 33.6 us for 16 x 8192
+// int8 positions, two 27.6).
 constexpr int paged_occupancy(int ct, int qt, int DP) {
   return DP == 256 ? is_8bit(ct) && qt != XT_F32 ? 2 : 1 : DP == 128 ? 2 : 3;
 }

@@ -11,9 +11,12 @@
 // that a sequence needs, so a first launch finds the row and sums it in
 // segments of kVerSeg tokens, each workgroup deciding by itself which drafts
 // are kept; a second launch looks the segment up and goes through it once
-// more.  A row of up to kVerWhole tokens is one workgroup's, in one launch.
-// Few sequences are bound by the two launches and three dependent loads
-// (token, probability, row), many by the rows' bytes.
+// more.  A row of up to kVerWhole tokens is one workgroup's, in one launch (1 and 64
+// sequences of 1000 tokens 4.4 and 4.7 us, of 16384 7.0 and 8.0, 300 of 16384 16.5; in
+// two launches 9.1, 10.1, 9.7, 10.5, 16.7; up to 4096 tokens 256 threads, 1024 are 1 us
+// slower there).  Few sequences are bound by the two launches and three dependent
+// loads (token, probability, row; 10 us), many by the rows' bytes (64 x 151936 fp32 20
+// us, 3.9 TB/s).
 #include <algorithm>
 
 #include "sbq_common.h"

@@ -459,8 +459,9 @@ class DevicePagedKVBuffer:
     reaches so far, release(sequence) when it is done.  append, attend, read
     and truncate find everything else on the device and keep every address, so
     a step can be captured in a HIP graph, and replayed for as long as its
-    tokens fit what is reserved.  What an append finds no page for is dropped.
-    GPU only."""
+    tokens fit what is reserved.  What an append finds no page for is dropped,
+    counted in the length all the same up to max_pages * page positions: reserve
+    first.  GPU only."""
 
     def __init__(self, sequences: int, heads: int, dim: int, pages: int, page: int = 64, max_pages: int | None = None,
                  window: int | None = None, device: torch.device | str | None = None, dtype: torch.dtype = torch.float32):
