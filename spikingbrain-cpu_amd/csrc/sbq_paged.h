@@ -76,9 +76,9 @@ struct PagedArgs {
   void* out;
   float* part_o;    // [Hk][places][R][DP]
   float2* part_ml;  // [Hk][places][R]
-  int2* joins;      // [row tiles][n]: a sequence's first place, and how many
+  int2* joins;      // [tiles of tile_rows rows][n]: a sequence's first place, and how many
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
-  int T, rep, qt;
+  int T, rep, qt, tile_rows;
   int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile (0: one each), and both
   float per_slot;        // 1 / slots
   float scale;               // times log2(e)
@@ -283,9 +283,15 @@ constexpr int paged_occupancy(int ct, int qt, int DP) {
   return DP == 256 ? is_8bit(ct) && qt != XT_F32 ? 2 : 1 : DP == 128 ? 2 : 3;
 }
 
+// Sixteens of rows that a workgroup can take: two where the registers hold them (fp32
+// queries and 256 columns spill: 16 x 8192 int8 positions, 8 tokens 122 us against 95).
+constexpr int paged_tiles(int qt, int DP) { return qt == XT_F32 || DP > 128 ? 1 : 2; }
+
 // CT: the cache's type, QT: the queries', DP: columns the registers hold (64,
-// 128, 256), EXACT: row == DP.  Grid: key heads of every row tile x slots.
-template <int CT, int QT, int DP, bool EXACT>
+// 128, 256), EXACT: row == DP, RT: sixteens of rows that a block serves (its keys and
+// values are loaded and converted once for them).  Grid: key heads of every RT
+// sixteens x slots.
+template <int CT, int QT, int DP, bool EXACT, int RT>
 __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void paged_attn_kernel(PagedArgs a) {
   constexpr bool B8 = is_8bit(CT), F32 = CT == XT_F32, WIDE = QT == XT_F32 && !F32;
   // pieces of a query and of a weight
@@ -302,14 +308,15 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   typedef uint32_t KV __attribute__((ext_vector_type(4)));
   typedef uint32_t VW __attribute__((ext_vector_type(EV * ES / 4)));
   __shared__ __align__(16) float lds_o[kAttnWaves * 16 * OLD];
-  __shared__ float lds_m[kAttnWaves][16], lds_l[kAttnWaves][16];
+  __shared__ float lds_m[RT][kAttnWaves][16], lds_l[RT][kAttnWaves][16];
+  static_assert(16 * RT * (DP + 4) <= kAttnWaves * 16 * OLD, "the rows of Q fit");
 
   const PagedCache& pc = a.c;
   const int slot = blockIdx.y, R = a.rep * a.T;
   int kvh = blockIdx.x, row0 = 0;
-  if (R > 16) row0 = kvh / pc.Hk * 16, kvh %= pc.Hk;
+  if (R > 16 * RT) row0 = kvh / pc.Hk * (16 * RT), kvh %= pc.Hk;
   int t0 = 0, t1 = 0;
-  if (a.T > 1) t0 = row0 / a.rep, t1 = min(row0 + 15, R - 1) / a.rep;
+  if (a.T > 1) t0 = row0 / a.rep, t1 = min(row0 + 16 * RT - 1, R - 1) / a.rep;
   PagedPlace p = paged_place(a, slot, t0, t1, SB);
   if (p.b >= a.n) return;
 
@@ -320,9 +327,6 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       int tid = threadIdx.x;
       asm volatile("" : "+v"(tid));  // (or what depends on it is kept in registers across the sequences)
       const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-      const int row = min(row0 + c, R - 1);
-      int tok = 0, head = row;
-      if (a.T > 1) tok = row / a.rep, head = row - tok * a.rep;
       const int page_mask = (1 << pc.page_log) - 1;
       // lane offsets in bytes inside a page of a head: its key row (c) and value rows (4g + j)
       const uint32_t row_bytes = pc.row * ES, k_lane = c * row_bytes + g * 16, v_lane = 4 * g * row_bytes + c * EV * ES;
@@ -330,9 +334,14 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       const int64_t b = a.first + p.b;
       PagedSpan span;
       span.of<true>(a, b);
-      const int lo = span.first(tok, a.window), hi = span.last(tok);
-      // what every row that sees anything sees
-      int lo_max = hi < lo ? 0 : lo, hi_min = hi < lo ? INT32_MAX : hi;
+      // the lane's rows' positions, and what every row that sees anything sees
+      int lo[RT], hi[RT], lo_max = 0, hi_min = INT32_MAX;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row0 + rt * 16 + c, R - 1), tok = a.T > 1 ? row / a.rep : 0;
+        lo[rt] = span.first(tok, a.window), hi[rt] = span.last(tok);
+        if (hi[rt] >= lo[rt]) lo_max = max(lo_max, lo[rt]), hi_min = min(hi_min, hi[rt]);
+      }
       if (a.T > 1) {
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) {
@@ -413,13 +422,14 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       }
 
       // the rows of Q by all threads to LDS, and the lane's share of its own
-      MV qm[F32 ? 1 : NFR][NQ];
-      f32x4 qf[F32 ? NCH : 1];
-      float factor = a.scale;
+      MV qm[RT][F32 ? 1 : NFR][NQ];
+      f32x4 qf[RT][F32 ? NCH : 1];
+      float factor[RT];
+      const int rows = min(R - row0, 16 * RT);
       {
         typedef typename XElem<QT>::T T;
         constexpr int LD = DP + 4, STEP = kAttnWaves * 64 / DP;
-        const int d = tid & (DP - 1), rows = min(R - row0, 16);
+        const int d = tid & (DP - 1);
         const T* const q = (const T*)a.q + b * a.q_sb + (int64_t)kvh * a.rep * a.q_sh + min(d, pc.D - 1);
         __syncthreads();  // (LDS is free of the last sequence)
 #pragma unroll 1
@@ -439,55 +449,64 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
             if (r + i * STEP < rows) lds_o[(r + i * STEP) * LD + d] = d < pc.D ? (float)x[i] : 0.0f;
         }
         __syncthreads();
-        const float* const mine = lds_o + (row - row0) * LD;
-        if constexpr (F32) {
 #pragma unroll
-          for (int ch = 0; ch < NCH; ++ch) qf[ch] = *(const f32x4*)(mine + ch * 16 + g * 4);
-        } else {
-          constexpr bool SCALED = B8 || (CT == XT_F16 && WIDE);
-          f32x4 x[NFR][2];
-          float most = 0.0f;
+        for (int rt = 0; rt < RT; ++rt) {
+          const float* const mine = lds_o + min(rt * 16 + c, rows - 1) * LD;
+          factor[rt] = a.scale;
+          if constexpr (F32) {
 #pragma unroll
-          for (int f = 0; f < NFR; ++f)
+            for (int ch = 0; ch < NCH; ++ch) qf[rt][ch] = *(const f32x4*)(mine + ch * 16 + g * 4);
+          } else {
+            constexpr bool SCALED = B8 || (CT == XT_F16 && WIDE);
+            f32x4 x[NFR][2];
+            float most = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              x[f][k] = *(const f32x4*)(mine + (B8 ? f / 2 * 64 + g * 16 + f % 2 * 8 : f * 32 + g * 8) + k * 4);
-              if constexpr (SCALED) {
+            for (int f = 0; f < NFR; ++f)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) most = __builtin_fmaxf(most, __builtin_fabsf(x[f][k][j]));
+              for (int k = 0; k < 2; ++k) {
+                x[f][k] = *(const f32x4*)(mine + (B8 ? f / 2 * 64 + g * 16 + f % 2 * 8 : f * 32 + g * 8) + k * 4);
+                if constexpr (SCALED) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) most = __builtin_fmaxf(most, __builtin_fabsf(x[f][k][j]));
+                }
               }
-            }
-          float unit = 1.0f;
-          if constexpr (SCALED) {
-            most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
-            most = __builtin_fmaxf(most, __shfl_xor(most, 32, 64));
-            const int e = row_scale_exp(most);
-            unit = __builtin_ldexpf(1.0f, e);
-            factor = __builtin_ldexpf(factor, -e);
-          }
-#pragma unroll
-          for (int f = 0; f < NFR; ++f) {
-            u32x4 words[NQ];
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              uint32_t to[NQ];
-              const float y = x[f][column_of<CT>(j) / 4][column_of<CT>(j) % 4];
-              const float z = x[f][column_of<CT>(j + 1) / 4][column_of<CT>(j + 1) % 4];
-              Pair<M>::pieces(SCALED ? y * unit : y, SCALED ? z * unit : z, to);
-#pragma unroll
-              for (int i = 0; i < NQ; ++i) words[i][j / 2] = to[i];
+            float unit = 1.0f;
+            if constexpr (SCALED) {
+              most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
+              most = __builtin_fmaxf(most, __shfl_xor(most, 32, 64));
+              const int e = row_scale_exp(most);
+              unit = __builtin_ldexpf(1.0f, e);
+              factor[rt] = __builtin_ldexpf(a.scale, -e);
             }
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) qm[f][i] = __builtin_bit_cast(MV, words[i]);
+            for (int f = 0; f < NFR; ++f) {
+              u32x4 words[NQ];
+#pragma unroll
+              for (int j = 0; j < 8; j += 2) {
+                uint32_t to[NQ];
+                const float y = x[f][column_of<CT>(j) / 4][column_of<CT>(j) % 4];
+                const float z = x[f][column_of<CT>(j + 1) / 4][column_of<CT>(j + 1) % 4];
+                Pair<M>::pieces(SCALED ? y * unit : y, SCALED ? z * unit : z, to);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) words[i][j / 2] = to[i];
+              }
+#pragma unroll
+              for (int i = 0; i < NQ; ++i) qm[rt][f][i] = __builtin_bit_cast(MV, words[i]);
+            }
           }
         }
       }
 
-      f32x4 o[NF];
+      f32x4 o[RT][NF];
+      float m[RT], l[RT];
+      float vref[RT], vinv[RT];  // 8-bit: O's unit, the largest value scale that the row saw so far
 #pragma unroll
-      for (int f = 0; f < NF; ++f) o[f] = (f32x4)(0.0f);
-      float m = kNone, l = 0.0f;
-      float vref = 1.17549435e-38f, vinv = 1.0f / vref;  // 8-bit: O's unit, the largest value scale that the row saw so far
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[rt][f] = (f32x4)(0.0f);
+        m[rt] = kNone, l[rt] = 0.0f;
+        vref[rt] = 1.17549435e-38f, vinv[rt] = 1.0f / vref[rt];
+      }
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {
         const int s0 = (p.from + n) * SB;
@@ -495,23 +514,33 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         const bool full = held == (1u << SUB) - 1 && s0 >= lo_max && s0 + SB - 1 <= hi_min;
 
         // scores, in powers of two
-        float e[SUB][4];
+        float e[RT][SUB][4];
 #pragma unroll
         for (int st = 0; st < SUB; ++st) {
-          f32x4 s = (f32x4)(0.0f);
+          f32x4 s[RT];
           if constexpr (F32) {
-            f32x4 t[4] = {(f32x4)(0.0f), (f32x4)(0.0f), (f32x4)(0.0f), (f32x4)(0.0f)};
+            f32x4 t[RT][4];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) t[rt][j] = (f32x4)(0.0f);
 #pragma unroll
             for (int ch = 0; ch < NCH; ++ch) {
               const f32x4 kk = __builtin_bit_cast(f32x4, kf[st][ch]);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) t[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[j], qf[ch][j], t[j], 0, 0, 0);
-            }
-            s = (t[0] + t[1]) + (t[2] + t[3]);
-          } else {
-            f32x4 t[NQ];
+              for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) t[i] = (f32x4)(0.0f);
+                for (int j = 0; j < 4; ++j)
+                  t[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[j], qf[rt][ch][j], t[rt][j], 0, 0, 0);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt] = (t[rt][0] + t[rt][1]) + (t[rt][2] + t[rt][3]);
+          } else {
+            f32x4 t[RT][NQ];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int i = 0; i < NQ; ++i) t[rt][i] = (f32x4)(0.0f);
 #pragma unroll
             for (int f = 0; f < NFR; ++f) {
               MV kk;
@@ -520,73 +549,89 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
               else
                 kk = __builtin_bit_cast(MV, kf[st][f]);
 #pragma unroll
-              for (int i = 0; i < NQ; ++i) t[i] = PagedMath<CT>::mfma(kk, qm[f][i], t[i]);
+              for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) t[rt][i] = PagedMath<CT>::mfma(kk, qm[rt][f][i], t[rt][i]);
             }
 #pragma unroll
-            for (int i = NQ - 1; i > 0; --i) t[i - 1] += t[i];
-            s = t[0];
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+              for (int i = NQ - 1; i > 0; --i) t[rt][i - 1] += t[rt][i];
+              s[rt] = t[rt][0];
+            }
           }
 #pragma unroll
-          for (int v = 0; v < 4; ++v) e[st][v] = s[v] * (B8 ? factor * ks[st][v] : factor);
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) e[rt][st][v] = s[rt][v] * (B8 ? factor[rt] * ks[st][v] : factor[rt]);
         }
         const bool more = n + kAttnWaves < n1;
         if (more) load_k(n + kAttnWaves);
 
-        uint32_t seen = ~0u;  // bit st * 4 + v: the lane's row sees that position
-        if (!full) {
-          seen = 0;
+        uint32_t seen[RT];  // bit st * 4 + v: the lane's row sees that position
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          seen[rt] = ~0u;
+          f32x4 vr[B8 ? SUB : 1];  // the values' scales, as far as the row sees them
+          if constexpr (B8) {
+#pragma unroll
+            for (int st = 0; st < SUB; ++st) vr[st] = vs[st];
+          }
+          if (!full) {
+            seen[rt] = 0;
+#pragma unroll
+            for (int st = 0; st < SUB; ++st)
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const int at = s0 + st * 16 + 4 * g + v;
+                if (at >= lo[rt] && at <= hi[rt] && (held >> st & 1)) seen[rt] |= 1u << (st * 4 + v);
+                e[rt][st][v] = seen[rt] >> (st * 4 + v) & 1 ? e[rt][st][v] : kNone;
+                if constexpr (B8) vr[st][v] = seen[rt] >> (st * 4 + v) & 1 ? vr[st][v] : 0.0f;
+              }
+          }
+          float mx = kNone;
 #pragma unroll
           for (int st = 0; st < SUB; ++st)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const int s = s0 + st * 16 + 4 * g + v;
-              if (s >= lo && s <= hi && (held >> st & 1)) seen |= 1u << (st * 4 + v);
-              e[st][v] = seen >> (st * 4 + v) & 1 ? e[st][v] : kNone;
-              if constexpr (B8) vs[st][v] = seen >> (st * 4 + v) & 1 ? vs[st][v] : 0.0f;
+            for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, e[rt][st][v]);
+          mx = reference<XT_F16, !F32 && CT != XT_BF16>(mx);
+          if (__any(mx > m[rt])) {
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float up = __builtin_fmaxf(m[rt], mx), alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
+            m[rt] = up;
+            l[rt] *= alpha;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) o[rt][f] *= alpha;
+          }
+          const float from = m[rt] == kNone ? 0.0f : m[rt];
+#pragma unroll
+          for (int st = 0; st < SUB; ++st)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {  // (exp2 of -infinity: what is not seen has weight 0)
+              e[rt][st][v] = __builtin_amdgcn_exp2f(e[rt][st][v] - from);
+              l[rt] += e[rt][st][v];
             }
-        }
-        float mx = kNone;
-#pragma unroll
-        for (int st = 0; st < SUB; ++st)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, e[st][v]);
-        mx = reference<XT_F16, !F32 && CT != XT_BF16>(mx);
-        if (__any(mx > m)) {
-          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float up = __builtin_fmaxf(m, mx), alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m - up);
-          m = up;
-          l *= alpha;
-#pragma unroll
-          for (int f = 0; f < NF; ++f) o[f] *= alpha;
-        }
-        const float from = m == kNone ? 0.0f : m;
-#pragma unroll
-        for (int st = 0; st < SUB; ++st)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {  // (exp2 of -infinity: what is not seen has weight 0)
-            e[st][v] = __builtin_amdgcn_exp2f(e[st][v] - from);
-            l += e[st][v];
-          }
 
-        if constexpr (B8) {  // the weights times the values' scales, in units of vref
-          float top = 0.0f;
+          if constexpr (B8) {  // the weights times the values' scales, in units of vref
+            float top = 0.0f;
 #pragma unroll
-          for (int st = 0; st < SUB; ++st)
+            for (int st = 0; st < SUB; ++st)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, vs[st][v]);  // (NaN: the other one)
-          if (__any(top > vref)) {
-            top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
-            top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
-            const float up = __builtin_fmaxf(vref, top), alpha = vref / up;
-            vref = up, vinv = 1.0f / up;
+              for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, vr[st][v]);  // (NaN: the other one)
+            if (__any(top > vref[rt])) {
+              top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
+              top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
+              const float up = __builtin_fmaxf(vref[rt], top), alpha = vref[rt] / up;
+              vref[rt] = up, vinv[rt] = 1.0f / up;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) o[f] *= alpha;
+              for (int f = 0; f < NF; ++f) o[rt][f] *= alpha;
+            }
+#pragma unroll
+            for (int st = 0; st < SUB; ++st)
+#pragma unroll
+              for (int v = 0; v < 4; ++v) e[rt][st][v] *= vr[st][v] * vinv[rt];
           }
-#pragma unroll
-          for (int st = 0; st < SUB; ++st)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) e[st][v] *= vs[st][v] * vinv;
         }
 
         // infinities and NaN in values that not every row sees (codes have none)
@@ -618,30 +663,38 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
               for (int k = 0; k < EV; ++k) {
                 float x = __uint_as_float(vf[j][db][k]);
                 if (odd) {
-#pragma unroll 1
-                  for (int kind = 0; kind < 3; ++kind) {
-                    const f32x4 cnt = __builtin_amdgcn_mfma_f32_16x16x4f32(odd_one(x, kind), seen >> j & 1 ? 1.0f : 0.0f,
-                                                                           (f32x4)(0.0f), 0, 0, 0);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                      if (cnt[v] > 0.0f) o[db * EV + k][v] += odd_value(kind);
+                  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; ++kind) {
+                      const f32x4 cnt = __builtin_amdgcn_mfma_f32_16x16x4f32(odd_one(x, kind), seen[rt] >> j & 1 ? 1.0f : 0.0f,
+                                                                             (f32x4)(0.0f), 0, 0, 0);
+#pragma unroll
+                      for (int v = 0; v < 4; ++v)
+                        if (cnt[v] > 0.0f) o[rt][db * EV + k][v] += odd_value(kind);
+                    }
                   }
                   x = finite(x) ? x : 0.0f;
                 }
-                o[db * EV + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, e[0][j], o[db * EV + k], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                  o[rt][db * EV + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, e[rt][0][j], o[rt][db * EV + k], 0, 0, 0);
               }
         } else {
-          u32x4 words[NP];
+          MV pf[RT][NP];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            uint32_t to[NP];
-            Pair<M>::pieces(e[j >> 2][j & 3], e[j >> 2][(j & 3) + 1], to);
+          for (int rt = 0; rt < RT; ++rt) {
+            u32x4 words[NP];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) words[i][j / 2] = to[i];
+            for (int j = 0; j < 8; j += 2) {
+              uint32_t to[NP];
+              Pair<M>::pieces(e[rt][j >> 2][j & 3], e[rt][j >> 2][(j & 3) + 1], to);
+#pragma unroll
+              for (int i = 0; i < NP; ++i) words[i][j / 2] = to[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) pf[rt][i] = __builtin_bit_cast(MV, words[i]);
           }
-          MV pf[NP];
-#pragma unroll
-          for (int i = 0; i < NP; ++i) pf[i] = __builtin_bit_cast(MV, words[i]);
 #pragma unroll
           for (int db = 0; db < DB; ++db) {
             VW vw[8];
@@ -674,18 +727,21 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
                 const int f = db * EV + e0 + k;
                 if constexpr (!B8) {
                   if (odd) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll 1
-                    for (int kind = 0; kind < 3; ++kind) {
-                      u32x4 ones;
-                      MV sees;
+                      for (int kind = 0; kind < 3; ++kind) {
+                        u32x4 ones;
+                        MV sees;
 #pragma unroll
-                      for (int j = 0; j < 4; ++j) ones[j] = Odd2<CT>::ones(t[k][j], kind);
+                        for (int j = 0; j < 4; ++j) ones[j] = Odd2<CT>::ones(t[k][j], kind);
 #pragma unroll
-                      for (int j = 0; j < 8; ++j) sees[j] = (M)(seen >> j & 1 ? 1.0f : 0.0f);
-                      const f32x4 cnt = PagedMath<CT>::mfma(__builtin_bit_cast(MV, ones), sees, (f32x4)(0.0f));
+                        for (int j = 0; j < 8; ++j) sees[j] = (M)(seen[rt] >> j & 1 ? 1.0f : 0.0f);
+                        const f32x4 cnt = PagedMath<CT>::mfma(__builtin_bit_cast(MV, ones), sees, (f32x4)(0.0f));
 #pragma unroll
-                      for (int v = 0; v < 4; ++v)
-                        if (cnt[v] > 0.0f) o[f][v] += odd_value(kind);
+                        for (int v = 0; v < 4; ++v)
+                          if (cnt[v] > 0.0f) o[rt][f][v] += odd_value(kind);
+                      }
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) t[k][j] = Odd2<CT>::finite(t[k][j]);
@@ -693,7 +749,9 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
                 }
                 const MV vt = __builtin_bit_cast(MV, t[k]);
 #pragma unroll
-                for (int i = 0; i < NP; ++i) o[f] = PagedMath<CT>::mfma(vt, pf[i], o[f]);
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                  for (int i = 0; i < NP; ++i) o[rt][f] = PagedMath<CT>::mfma(vt, pf[rt][i], o[rt][f]);
               }
             }
           }
@@ -709,55 +767,58 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       if (a.slots) places = paged_places(p.b, p.each, p.before, p.blocks, first);
       const int place = slot + p.b;
       const bool alone = places == 1;
-      if (a.joins && n0 == 0 && kvh == 0 && tid == 0) a.joins[row0 / 16 * a.n + p.b] = make_int2(first, places);
-      l += __shfl_xor(l, 16, 64);
-      l += __shfl_xor(l, 32, 64);
+      if (a.joins && n0 == 0 && kvh == 0 && tid == 0) a.joins[row0 / (16 * RT) * a.n + p.b] = make_int2(first, places);
       __syncthreads();  // (every wave has read its Q)
-      if (g == 0) lds_m[w][c] = m, lds_l[w][c] = l;
-      const float unit = B8 ? vref : 1.0f;
-      const int rows = min(R - row0, 16);
 #pragma unroll
-      for (int h0 = 0; h0 < DP; h0 += HP) {
-        if (h0) __syncthreads();
-        float* const to = lds_o + (w * 16 + c) * OLD;
-        if (c < rows) {
+      for (int rt = 0; rt < RT; ++rt) {
+        l[rt] += __shfl_xor(l[rt], 16, 64);
+        l[rt] += __shfl_xor(l[rt], 32, 64);
+        if (g == 0) lds_m[rt][w][c] = m[rt], lds_l[rt][w][c] = l[rt];
+        const float unit = B8 ? vref[rt] : 1.0f;
+        const int here = min(rows - rt * 16, 16);  // (none: nothing is copied or joined)
 #pragma unroll
-          for (int db = h0 / (16 * EV); db < (h0 + HP) / (16 * EV); ++db)
+        for (int h0 = 0; h0 < DP; h0 += HP) {
+          if (h0 || rt) __syncthreads();
+          float* const to = lds_o + (w * 16 + c) * OLD;
+          if (c < here) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
+            for (int db = h0 / (16 * EV); db < (h0 + HP) / (16 * EV); ++db)
 #pragma unroll
-              for (int k = 0; k < EV; ++k) to[db * 16 * EV - h0 + (4 * g + v) * EV + k] = o[db * EV + k][v] * unit;
-        }
-        __syncthreads();
-        for (int u = tid; u < rows * (HP / 4); u += kAttnWaves * 64) {
-          const int rr = u / (HP / 4), d = h0 + u % (HP / 4) * 4;
-          float top = kNone;
+              for (int v = 0; v < 4; ++v)
 #pragma unroll
-          for (int k = 0; k < kAttnWaves; ++k) top = __builtin_fmaxf(top, lds_m[k][rr]);
-          const float ref = top == kNone ? 0.0f : top;
-          f32x4 sum = (f32x4)(0.0f);
-          float ls = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kAttnWaves; ++k) {
-            const float f = __builtin_amdgcn_exp2f(lds_m[k][rr] - ref), lk = lds_l[k][rr];
-            const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
-            if (lk != 0.0f) {  // (a wave that saw nothing adds nothing)
-              sum += x * f;
-              ls += lk * f;
-            }
+                for (int k = 0; k < EV; ++k) to[db * 16 * EV - h0 + (4 * g + v) * EV + k] = o[rt][db * EV + k][v] * unit;
           }
-          const int r = row0 + rr;
-          if (!alone) {
-            const int64_t at = ((int64_t)kvh * a.places + place) * R + r;
-            *(f32x4*)(a.part_o + at * DP + d) = sum;
-            if (d == 0) a.part_ml[at] = make_float2(top, ls);
-          } else {
-            int t = 0, h = r;
-            if (a.T > 1) t = r / a.rep, h = r - t * a.rep;
-            const bool any = span.last(t) >= span.first(t, a.window);
-            const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
-            const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + h) * a.o_sh + d;
-            if (d < pc.D) store_y4(a.out, QT, out, any ? sum * inv : (f32x4)(0.0f), a.ovec && d + 4 <= pc.D, pc.D - d);
+          __syncthreads();
+          for (int u = tid; u < here * (HP / 4); u += kAttnWaves * 64) {
+            const int rr = u / (HP / 4), d = h0 + u % (HP / 4) * 4;
+            float top = kNone;
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k) top = __builtin_fmaxf(top, lds_m[rt][k][rr]);
+            const float ref = top == kNone ? 0.0f : top;
+            f32x4 sum = (f32x4)(0.0f);
+            float ls = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k) {
+              const float f = __builtin_amdgcn_exp2f(lds_m[rt][k][rr] - ref), lk = lds_l[rt][k][rr];
+              const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
+              if (lk != 0.0f) {  // (a wave that saw nothing adds nothing)
+                sum += x * f;
+                ls += lk * f;
+              }
+            }
+            const int r = row0 + rt * 16 + rr;
+            if (!alone) {
+              const int64_t at = ((int64_t)kvh * a.places + place) * R + r;
+              *(f32x4*)(a.part_o + at * DP + d) = sum;
+              if (d == 0) a.part_ml[at] = make_float2(top, ls);
+            } else {
+              int t = 0, h = r;
+              if (a.T > 1) t = r / a.rep, h = r - t * a.rep;
+              const bool any = span.last(t) >= span.first(t, a.window);
+              const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
+              const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + h) * a.o_sh + d;
+              if (d < pc.D) store_y4(a.out, QT, out, any ? sum * inv : (f32x4)(0.0f), a.ovec && d + 4 <= pc.D, pc.D - d);
+            }
           }
         }
       }
@@ -769,20 +830,26 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   }
 }
 
+template <int CT, int QT, int DP>
+int launch_paged_dp(const PagedArgs& a, dim3 grid, hipStream_t st) {
+  constexpr int threads = kAttnWaves * 64, RT = paged_tiles(QT, DP);
+  const bool exact = a.c.row == DP;
+  if constexpr (RT > 1) {
+    if (a.tile_rows > 16) {
+      exact ? paged_attn_kernel<CT, QT, DP, true, RT><<<grid, threads, 0, st>>>(a)
+            : paged_attn_kernel<CT, QT, DP, false, RT><<<grid, threads, 0, st>>>(a);
+      return check_launch();
+    }
+  }
+  exact ? paged_attn_kernel<CT, QT, DP, true, 1><<<grid, threads, 0, st>>>(a)
+        : paged_attn_kernel<CT, QT, DP, false, 1><<<grid, threads, 0, st>>>(a);
+  return check_launch();
+}
 template <int CT, int QT>
 int launch_paged_types(const PagedArgs& a, int DP, dim3 grid, hipStream_t st) {
-  constexpr int threads = kAttnWaves * 64;
-  const bool exact = a.c.row == DP;
-  if (DP == 64)
-    exact ? paged_attn_kernel<CT, QT, 64, true><<<grid, threads, 0, st>>>(a)
-          : paged_attn_kernel<CT, QT, 64, false><<<grid, threads, 0, st>>>(a);
-  else if (DP == 128)
-    exact ? paged_attn_kernel<CT, QT, 128, true><<<grid, threads, 0, st>>>(a)
-          : paged_attn_kernel<CT, QT, 128, false><<<grid, threads, 0, st>>>(a);
-  else
-    exact ? paged_attn_kernel<CT, QT, 256, true><<<grid, threads, 0, st>>>(a)
-          : paged_attn_kernel<CT, QT, 256, false><<<grid, threads, 0, st>>>(a);
-  return check_launch();
+  return DP == 64    ? launch_paged_dp<CT, QT, 64>(a, grid, st)
+         : DP == 128 ? launch_paged_dp<CT, QT, 128>(a, grid, st)
+                     : launch_paged_dp<CT, QT, 256>(a, grid, st);
 }
 
 int launch_paged_attn_f32(const PagedArgs& a, int DP, dim3 grid, hipStream_t st);

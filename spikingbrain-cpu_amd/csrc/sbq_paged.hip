@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
   const int r = blockIdx.x, kvh = blockIdx.y, t = a.T > 1 ? r / a.rep : 0;
   const int64_t b = a.first + blockIdx.z;
-  const int2 places = a.joins[r / 16 * a.n + (int)blockIdx.z];
+  const int2 places = a.joins[r / a.tile_rows * a.n + (int)blockIdx.z];
   PagedSpan span;
   span.of<true>(a, b);
   const int used = places.y;
@@ -404,11 +404,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 // 256 x 2048 191, 119, 24 against 199, 126, 34; 256 x 4096 374, 233, 40 against 379,
 // 233, 34.
 constexpr int64_t kPagedWhole = 4, kPagedWholeFull = 12, kPagedWholeMost = 16;
+// Rounds of all workgroups' blocks, in times the chip, from which a workgroup takes two
+// sixteens of rows (half of that where workgroups of whole sequences fill the chip): the
+// way to and from a part's blocks is 3 to 5 us longer with them, the blocks are read
+// and converted half as often.  32 query heads over 8 x 128, two sixteens against one
+// in us: 16 x 1024 e4m3 positions, 8 tokens 31 against 19; 16 x 2048 36.4 against 35.5;
+// 16 x 4096 44.9 against 47.1, bf16 61.7 against 60.6; 16 x 8192 66 against 77, bf16 115
+// against 119; 64 x 512 e4m3 25.6 against 29.4; a chunk of 512 tokens over 2048 bf16
+// positions 46 against 77, over 8192 153 against 286.
+constexpr int64_t kPagedTiles = 8;
 constexpr int64_t kPagedGroup = 512;   // sequences of a launch that are split at most (each workgroup scans their lengths)
 constexpr int64_t kPagedRows = 65535;  // ... of one that are not: the grid's limit
 
 struct PagedPlan {
-  int DP, SB;
+  int DP, SB, tile_rows;
   int64_t rtiles, n, slots, places;
   bool joins;  // can a sequence have several parts?
 };
@@ -419,12 +428,15 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int
   PagedPlan p;
   p.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   p.SB = ct == XT_F32 ? 16 : 32;
-  p.rtiles = (R + 15) / 16;
   if (window > 0 && window < room - T) room = window + T;  // (what the tokens of a call can look at)
-  const int64_t one = Hk * p.rtiles, blocks = (room + p.SB - 1) / p.SB + (window > 0), fours = (blocks + kAttnWaves - 1) / kAttnWaves;
+  const int64_t blocks = (room + p.SB - 1) / p.SB + (window > 0), fours = (blocks + kAttnWaves - 1) / kAttnWaves;
+  const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
+  const int64_t most = 16 * paged_tiles(wide ? XT_F32 : XT_F16, p.DP), tiles = B * Hk * ((R + most - 1) / most);
+  p.tile_rows = R > 16 && tiles * fours >= (tiles >= groups ? kPagedTiles / 2 : kPagedTiles) * groups ? (int)most : 16;
+  p.rtiles = (R + p.tile_rows - 1) / p.tile_rows;
+  const int64_t one = Hk * p.rtiles;
   p.n = std::min(B, kPagedGroup);
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 29) / (fours * kAttnWaves)));  // (all blocks fit an int, in whole parts too)
-  const int64_t groups = 256 * paged_occupancy(ct, wide ? XT_F32 : XT_F16, p.DP);
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
   if (fours <= std::min(kPagedWhole + kPagedWholeFull * B * one / groups, kPagedWholeMost)) p.slots = 0, p.n = std::min(B, kPagedRows);
   p.places = p.slots + p.n;
@@ -453,7 +465,7 @@ int launch_paged_attention(const PagedCall& c, hipStream_t st) {
   PagedArgs a{};
   a.c = c.c, a.q = c.q, a.start = c.start, a.counts = c.counts, a.out = c.out;
   a.q_sb = c.q_sb, a.q_st = c.q_st, a.q_sh = c.q_sh, a.o_sb = c.o_sb, a.o_st = c.o_st, a.o_sh = c.o_sh;
-  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.slots = (int)p.slots, a.per_slot = p.slots ? 1.0f / (float)p.slots : 0.0f;
+  a.window = c.window, a.T = (int)c.T, a.rep = (int)rep, a.qt = c.qt, a.tile_rows = p.tile_rows, a.slots = (int)p.slots, a.per_slot = p.slots ? 1.0f / (float)p.slots : 0.0f;
   a.places = (int)p.places;
   a.scale = c.scale * 1.44269504f;
   const int64_t eq = c.qt == XT_F32 ? 4 : 2;

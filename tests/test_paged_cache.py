@@ -448,7 +448,13 @@ def test_append_strides(dev, dtype):
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-def _attention(b, q, start, counts, scale=None):
+def _attention_of(b, q, counts, tokens, sequences):
+    """_attention of some tokens of the first few sequences."""
+    out, tol = _attention(b, q, None, counts, None, tokens, sequences)
+    return out[:sequences][:, tokens], tol[:sequences][:, tokens]
+
+
+def _attention(b, q, start, counts, scale=None, tokens=None, sequences=None):
     """The documented attention and its tolerance, in 64 bits.
 
     With u = 2^-24: a score carries (D + 16) u of scale sum |q||k| (products and sums of D
@@ -462,12 +468,14 @@ def _attention(b, q, start, counts, scale=None):
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
     rep, eps = H // b.heads, torch.finfo(q.dtype).eps / 2
     piece = 2.0 ** -11 if q.dtype == BF16 and b.k_scale is not None else 2.0 ** -20
-    for i in range(B):
+    for i in range(B if sequences is None else min(B, sequences)):
         n = max(0, min(int(b.length[i]), b.table.shape[1] * b.page))
         count = T if counts is None else int(np.clip(int(counts[i]), 0, T))
         first = int(b.length[i]) - count if start is None else int(start[i])
         k, v, there = _held(b, i, n)
         for t in range(count):
+            if tokens is not None and t not in tokens:
+                continue
             pos = first + t
             see = there & (np.arange(n) <= pos)
             if b.window:
@@ -579,6 +587,43 @@ def test_attention_of_many_tokens(dev, dtype, qt):
     _compare(b, q, b.attend(q, counts=counts), counts=counts)
     b.window = 77
     _compare(b, q, b.attend(q, counts=counts), counts=counts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,qt", [(F16, F16), (BF16, BF16), (I8, F16), (E4M3, BF16), (E4M3, F16), (I8, F32)])
+@pytest.mark.parametrize("lengths,T,heads,kv,dim,room", [
+    ([1500, 330], 300, 8, 2, 128, 9000),                  # two row tiles at a time, sequences in parts
+    ([700, 100], 301, 7, 1, 72, 20000),                   # ... that end inside a tile
+    ([600, 290, 10], 290, 8, 2, 64, 16000),
+    ([40, 33, 129, 512] * 16, 6, 32, 8, 112, 512),        # ... whole sequences
+])
+def test_attention_of_rows_in_twos(dev, lengths, T, heads, kv, dim, room, dtype, qt):
+    announce(f"attend lengths={lengths[:4]} T={T} heads={heads} kv={kv} dim={dim} room={room} {dtype} {qt}")
+    b = _buffer(dev, lengths, kv, dim, 16, dtype, seed=dim, room=room)
+    g = torch.Generator().manual_seed(T)
+    q = torch.randn(len(lengths), T, heads, dim, generator=g).to(qt).to(dev)
+    counts = torch.tensor([min(n, T) - (i % 3) for i, n in enumerate(lengths)], device=dev)
+    got = b.attend(q, counts=counts)
+    few = list(range(0, T, 23)) + [T - 1]  # (the oracle for some of the tokens, of four sequences)
+    want, tol = _attention_of(b, q, counts, few, 4)
+    bad = np.abs(got.float().cpu().double().numpy()[:4][:, few] - want) > tol
+    assert not bad.any()
+    for i in range(len(lengths)):
+        assert float(got[i, int(counts[i]):].float().abs().sum()) == 0
+    assert torch.isfinite(got).all()
+    # an infinity (a NaN scale) in the last position: the last token alone sees it
+    last = lengths[0] - 1
+    page, row = int(b.table[0, last // 16]), last % 16
+    if b.v_scale is None:
+        b.v[page, :, row, 0] = float("inf")
+    else:
+        b.v_scale[page, :, row] = float("nan")
+    now, end = b.attend(q, counts=counts), int(counts[0]) - 1
+    assert torch.equal(now[0, :end], got[0, :end]) and torch.equal(now[1:], got[1:])
+    if b.v_scale is None:
+        assert torch.isinf(now[0, end, :, 0]).all() and torch.equal(now[0, end, :, 1:], got[0, end, :, 1:])
+    else:
+        assert torch.isnan(now[0, end]).all()
 
 
 @pytest.mark.gpu
