@@ -15,8 +15,8 @@
 // sequences of 1000 tokens 4.4 and 4.7 us, of 16384 7.0 and 8.0, 300 of 16384 16.5; in
 // two launches 9.1, 10.1, 9.7, 10.5, 16.7; up to 4096 tokens 256 threads, 1024 are 1 us
 // slower there).  Few sequences are bound by the two launches and three dependent
-// loads (token, probability, row; 10 us), many by the rows' bytes (64 x 151936 fp32 20
-// us, 3.9 TB/s).
+// loads (token, probability, row; 9.3 us), many by the rows' bytes (64 x 151936 fp32 18.4
+// us, 4.2 TB/s).
 #include <algorithm>
 
 #include "sbq_common.h"
@@ -31,38 +31,54 @@ constexpr int kVerWholeThreads = 1024, kVerWhole = 16 * kVerWholeThreads;  // a 
 
 __device__ __forceinline__ double shfl_xor_f64(double v, int o) { return __shfl_xor(v, o, 64); }
 
-__device__ __forceinline__ double block_sum(double v, double* lds) {
+// Two sums over the workgroup at once.
+__device__ __forceinline__ double2 block_sum(double2 v, double2* lds) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += shfl_xor_f64(v, o);
+  for (int o = 32; o > 0; o >>= 1) v.x += shfl_xor_f64(v.x, o), v.y += shfl_xor_f64(v.y, o);
   __syncthreads();  // (lds is free)
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  double sum = 0.0;
-  for (int k = 0; k < (int)blockDim.x >> 6; ++k) sum += lds[k];
+  double2 sum = make_double2(0.0, 0.0);
+  for (int k = 0; k < (int)blockDim.x >> 6; ++k) sum.x += lds[k].x, sum.y += lds[k].y;
   return sum;
 }
 
-// Sums of the threads before this one, in thread order; `total` of all.
-__device__ __forceinline__ double block_before(double v, double* lds, double* total) {
+// N sums of the threads before this one, in thread order; `total` of all.
+template <int N>
+struct Sums {
+  double v[N];
+};
+template <int N>
+__device__ __forceinline__ Sums<N> block_before(Sums<N> x, Sums<N>* lds, Sums<N>* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double sum = v;
+  Sums<N> sum = x, before, base;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(sum, o, 64);
-    if (lane >= o) sum += t;
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double t = __shfl_up(sum.v[i], o, 64);
+      if (lane >= o) sum.v[i] += t;
+    }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    before.v[i] = __shfl_up(sum.v[i], 1, 64);
+    if (lane == 0) before.v[i] = 0.0;
+    base.v[i] = total->v[i] = 0.0;
   }
-  double before = __shfl_up(sum, 1, 64);
-  if (lane == 0) before = 0.0;
-  __syncthreads();
+  __syncthreads();  // (lds is free)
   if (lane == 63) lds[w] = sum;
   __syncthreads();
-  double base = 0.0, all = 0.0;
   for (int k = 0; k < (int)blockDim.x >> 6; ++k) {
-    base = k == w ? all : base;
-    all += lds[k];
+    const Sums<N> s = lds[k];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      base.v[i] = k == w ? total->v[i] : base.v[i];
+      total->v[i] += s.v[i];
+    }
   }
-  *total = all;
-  return base + before;
+#pragma unroll
+  for (int i = 0; i < N; ++i) before.v[i] += base.v[i];
+  return before;
 }
 
 template <int XT>
@@ -184,7 +200,7 @@ __device__ __forceinline__ void choose(const double (&m)[N], double sum, double 
 
 template <int XT, bool VEC>
 __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerifyArgs a) {
-  __shared__ double lds[4];
+  __shared__ double2 lds[4];
   const int64_t b = a.first + blockIdx.x / a.segs;
   const int seg = blockIdx.x % a.segs, n = count_of(a, b), kept = kept_of<XT>(a, b, n);
   const VerRow r = row_of<XT>(a, b, n, kept);
@@ -196,30 +212,32 @@ __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerifyArgs a) {
     left += (l[0] + l[1]) + (l[2] + l[3]);
     all += (w[0] + w[1]) + (w[2] + w[3]);
   }
-  left = block_sum(left, lds);
-  all = block_sum(all, lds);
+  const double2 sums = block_sum(make_double2(left, all), lds);
   if (threadIdx.x == 0) {
-    a.part[b * a.segs + seg] = make_double2(left, all);
+    a.part[b * a.segs + seg] = sums;
     if (seg == 0) a.kept[b] = kept;
   }
 }
 
 template <int XT, bool VEC>
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double lds[4], seg_before;
+  __shared__ Sums<2> lds[4];
+  __shared__ Sums<1> lds_seg[4];
+  __shared__ double seg_before;
   __shared__ int hit;
   const int64_t b = a.first + blockIdx.x;
   const int n = count_of(a, b), kept = (int)a.kept[b], each = (a.segs + kVerThreads - 1) / kVerThreads;
   const double2* const part = a.part + b * a.segs;
+  const double u = (double)a.u[b * (a.T + 1) + a.T];
   const int s0 = threadIdx.x * each;
-  double left = 0.0, all = 0.0, total_left, total_all;
-  for (int s = s0; s < min(s0 + each, a.segs); ++s) left += part[s].x, all += part[s].y;
-  const double before_left = block_before(left, lds, &total_left), before_all = block_before(all, lds, &total_all);
+  Sums<2> mine = {{0.0, 0.0}}, totals;
+  for (int s = s0; s < min(s0 + each, a.segs); ++s) mine.v[0] += part[s].x, mine.v[1] += part[s].y;
+  if (threadIdx.x == 0) hit = -1;
+  const Sums<2> before = block_before(mine, lds, &totals);
+  const double total_left = totals.v[0], total_all = totals.v[1], before_left = before.v[0], before_all = before.v[1];
   // (without a refusal the two are equal; nothing left after one: p itself)
   const bool use = total_left > 0.0 || total_left != total_left;
-  const double total = use ? total_left : total_all, want = (double)a.u[b * (a.T + 1) + a.T] * total;
-  if (threadIdx.x == 0) hit = -1;
-  __syncthreads();
+  const double total = use ? total_left : total_all, want = u * total;
   if (!(total > 0.0 && total < __builtin_inf())) {  // (NaN too)
     if (threadIdx.x == 0) a.token[b] = -1;
     return;
@@ -227,11 +245,14 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
   // the segment: the last with mass whose prefix is not beyond `want` (threads'
   // prefixes are sums in different orders, so no segment's end is compared)
   double at = use ? before_left : before_all;
+  int last = -1;
   for (int s = s0; s < min(s0 + each, a.segs); ++s) {
     const double mass = use ? part[s].x : part[s].y;
-    if (at <= want && mass > 0.0) atomicMax(&hit, s);
+    if (at <= want && mass > 0.0) last = s;
     at += mass;
   }
+  const uint64_t any = __ballot(last >= 0);
+  if (any && (threadIdx.x & 63) == 63 - __builtin_clzll(any)) atomicMax(&hit, last);
   __syncthreads();
   const int seg = hit;
   if (seg < 0) {  // (a uniform that is not a number)
@@ -248,7 +269,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
   const VerRow r = row_of<XT>(a, b, n, kept);
   constexpr int kEach = kVerSeg / kVerThreads;
   const int64_t i0 = (int64_t)seg * kVerSeg + threadIdx.x * kEach;
-  double m[kEach], sum = 0.0, total_seg;
+  double m[kEach], sum = 0.0;
+  Sums<1> total_seg;
 #pragma unroll
   for (int k = 0; k < kEach; k += 4) {
     double l[4], w[4];
@@ -259,7 +281,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
       sum += m[k + j];
     }
   }
-  at = seg_before + block_before(sum, lds, &total_seg);
+  at = seg_before + block_before(Sums<1>{{sum}}, lds_seg, &total_seg).v[0];
   choose<kEach>(m, sum, at, want, i0, a.token + b);
 }
 
@@ -267,14 +289,16 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs a) 
 // share in registers from the sums to the choice.
 template <int XT, bool VEC>
 __global__ __launch_bounds__(kVerWholeThreads) void verify_whole_kernel(VerifyArgs a) {
-  __shared__ double lds[kVerWholeThreads / 64];
+  __shared__ Sums<1> lds[kVerWholeThreads / 64];
   constexpr int kEach = kVerWhole / kVerWholeThreads;
   const int64_t b = a.first + blockIdx.x;
+  const double u = (double)a.u[b * (a.T + 1) + a.T];
   const int n = count_of(a, b), kept = kept_of<XT>(a, b, n);
   const VerRow r = row_of<XT>(a, b, n, kept);
   const int each = ((int)(a.V + blockDim.x - 1) / (int)blockDim.x + 3) & ~3;
   const int64_t i0 = (int64_t)threadIdx.x * each;
-  double left[kEach], all[kEach], sum_left = 0.0, sum_all = 0.0, total;
+  double left[kEach], all[kEach], sum_left = 0.0, sum_all = 0.0;
+  Sums<1> sums;
 #pragma unroll
   for (int k = 0; k < kEach; k += 4) {
     double l[4] = {}, w[4] = {};
@@ -286,11 +310,11 @@ __global__ __launch_bounds__(kVerWholeThreads) void verify_whole_kernel(VerifyAr
     }
   }
   if (threadIdx.x == 0) a.kept[b] = kept;
-  double at = block_before(sum_left, lds, &total);
+  double at = block_before(Sums<1>{{sum_left}}, lds, &sums).v[0], total = sums.v[0];
   // (without a refusal the two are equal; nothing left after one: p itself)
   const bool use = total > 0.0 || total != total;
   if (!use) {
-    at = block_before(sum_all, lds, &total);
+    at = block_before(Sums<1>{{sum_all}}, lds, &sums).v[0], total = sums.v[0];
 #pragma unroll
     for (int k = 0; k < kEach; ++k) left[k] = all[k];
     sum_left = sum_all;
@@ -299,7 +323,7 @@ __global__ __launch_bounds__(kVerWholeThreads) void verify_whole_kernel(VerifyAr
     if (threadIdx.x == 0) a.token[b] = -1;
     return;
   }
-  choose<kEach>(left, sum_left, at, (double)a.u[b * (a.T + 1) + a.T] * total, i0, a.token + b);
+  choose<kEach>(left, sum_left, at, u * total, i0, a.token + b);
 }
 
 template <int XT, bool VEC>
