@@ -189,7 +189,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         q = q.contiguous()
         qs = q.stride()
     if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif q_out.shape != shape or q_out.dtype != dtype or q_out.get_device() != gpu or (dim > 1 and q_out.stride(2) != 1) \
             or (q_out.data_ptr() == q.data_ptr() and q_out.stride() != qs):
         raise ValueError("qk_norm_rope: q_out must have q's shape, dtype and device, with unit stride in dim")
@@ -206,7 +206,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             k = k.contiguous()
             ks = k.stride()
         if k_out is None:
-            k_out = torch.empty(kshape, dtype=dtype, device=device)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         elif k_out.shape != kshape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1) \
                 or (k_out.data_ptr() == k.data_ptr() and k_out.stride() != ks):
             raise ValueError("qk_norm_rope: k_out must have k's shape, dtype and device, with unit stride in dim")
@@ -699,7 +699,7 @@ class DevicePagedKVBuffer:
         n, gpu, dim, kv_heads, dev, shape = cache[10], self._gpu, self.dim, self.heads, self._dev, q.shape
         code = self._query("attend", q)
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(-1) != 1):
             raise ValueError("DevicePagedKVBuffer.attend: out must have q's shape, dtype and device, with unit stride in dim")
         elif out.data_ptr() == q.data_ptr() and q.numel():
