@@ -31,6 +31,7 @@ ROCm GPU every entry point raises: there is no CPU implementation here.
 from __future__ import annotations
 
 import ctypes
+import functools
 import weakref
 
 import torch
@@ -617,9 +618,14 @@ def sample(logits: torch.Tensor, params, generator: torch.Generator | None = Non
     return int(tok[0])
 
 
+@functools.lru_cache(maxsize=256)
+def _verify_workspace_bytes(B: int, V: int) -> int:
+    return _lib.load().sbq_verify_workspace_bytes(B, V)
+
+
 def verify_workspace(B: int, V: int, device: torch.device) -> torch.Tensor:
     """Scratch of verify_drafts for B sequences and V tokens (any content; one call at a time)."""
-    return torch.empty((_lib.load().sbq_verify_workspace_bytes(B, V),), dtype=torch.uint8, device=device)
+    return torch.empty(_verify_workspace_bytes(B, V), dtype=torch.uint8, device=device)
 
 
 def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, u: torch.Tensor,
@@ -661,19 +667,19 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
         draft = draft.contiguous()
     tokens, u = tokens.contiguous(), u.contiguous()
     counts = None if counts is None else counts.contiguous()
-    both = torch.empty((2, B), dtype=torch.int64, device=dev)
+    kept, token = tokens.new_empty(B), tokens.new_empty(B)
     if workspace is None:
-        room = _lib.load().sbq_verify_workspace_bytes(B, V)
-        workspace = torch.empty((room,), dtype=torch.uint8, device=dev) if room else None
+        room = _verify_workspace_bytes(B, V)
+        workspace = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
     elif workspace.device != dev or not workspace.is_contiguous():
         raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device")
     ps, qs = target.stride(), (0, 0) if draft is None else draft.stride()
     with _on_device(dev):
         _lib.check(_lib.load().sbq_verify_drafts(
             _ptr(target), ps[0], ps[1], _ptr(draft), qs[0], qs[1], _DTYPE_CODE[target.dtype], B, T, V, _ptr(tokens), _ptr(u),
-            _ptr(counts), both.data_ptr(), both.data_ptr() + 8 * B, _ptr(workspace), _nbytes(workspace), _stream(dev)),
+            _ptr(counts), kept.data_ptr(), token.data_ptr(), _ptr(workspace), _nbytes(workspace), _stream(dev)),
             "sbq_verify_drafts")
-    return both[0], both[1]
+    return kept, token
 
 
 def argmax_state(device: torch.device) -> torch.Tensor:
