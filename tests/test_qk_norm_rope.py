@@ -194,6 +194,27 @@ def test_views_of_one_projection_in_place_and_strides(dev, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("D,pairs", [(90, 45), (128, 63), (31, 9), (33, 16), (14, 7), (250, 117)])
+def test_in_place_at_no_alignment(dev, D, pairs, inter, dtype):
+    """Pieces that begin early over the columns of the one before, in rows that begin anywhere."""
+    T, H, kv = 530, 5, 2
+    announce(f"rope in place D={D} pairs={pairs} inter={inter} {dtype}")
+    g = torch.Generator().manual_seed(D)
+    qkv = torch.randn(T, (H + kv) * D + 3, generator=g).to(dtype).to(dev)
+    f, pos = torch.from_numpy(_freq(pairs)).to(dev), torch.arange(T, device=dev) + 7
+    w = (torch.rand(D + 1, generator=g) + 0.5).to(dev)[1:]
+    q, k = qkv[:, 1:1 + H * D].unflatten(1, (H, D)), qkv[:, 1 + H * D:1 + (H + kv) * D].unflatten(1, (kv, D))
+    ends = qkv[:, 0].clone(), qkv[:, 1 + (H + kv) * D:].clone()
+    want = qk_norm_rope(q, k, pos, f, w, w, interleaved=inter)
+    _check(want, q, k, pos, f, w, w, inter)
+    qk_norm_rope(q, k, pos, f, w, w, interleaved=inter, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    assert torch.equal(qkv[:, 0], ends[0]) and torch.equal(qkv[:, 1 + (H + kv) * D:], ends[1])
+
+
+@pytest.mark.gpu
 def test_starts_of_sequences(dev):
     q, k, _, f, wq, wk = _case(dev, 12, 4, 2, 32, 16, False, F32, True)
     starts = torch.tensor([5, 0, 1000], device=dev)
