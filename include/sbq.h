@@ -637,7 +637,7 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * cache's type (8-bit caches: any); out: the same shape and type, apart from
  * every input.  Scores, maxima and sums are fp32; fp32 queries are multiplied
  * to 22 significant bits or more, and so are their weights; with 2-byte
- * queries the weights keep 16 bits or more (8-bit caches with bf16: 11).
+ * queries the weights keep 16 bits or more.
  * scale * q . k is to be finite, below 2^27 in magnitude.
  * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
  * content; one call at a time.  The result does not depend on timing; how a

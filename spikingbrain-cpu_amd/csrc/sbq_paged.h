@@ -66,8 +66,7 @@ __device__ __forceinline__ int64_t paged_count(const int64_t* counts, int64_t b,
 //     position's scales multiply its score and its weight.
 // The weights are rounded for the product with V: as many pieces as the queries
 // with fp32 ones; else two, whose error stays far below the output's rounding
-// (one of the output's own type would add as much again), or one of fp16 where
-// the output is bf16.  fp16 weights are taken against 2^14 at the maximum, so
+// (one would add to it: the sum of weights is not rounded with them).  fp16 weights are taken against 2^14 at the maximum, so
 // that one 2^-28 of it keeps its bits.
 struct PagedArgs {
   PagedCache c;
@@ -295,7 +294,7 @@ template <int CT, int QT, int DP, bool EXACT, int RT>
 __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void paged_attn_kernel(PagedArgs a) {
   constexpr bool B8 = is_8bit(CT), F32 = CT == XT_F32, WIDE = QT == XT_F32 && !F32;
   // pieces of a query and of a weight
-  constexpr int NQ = !WIDE ? 1 : CT == XT_BF16 ? 3 : 2, NP = WIDE ? NQ : CT == XT_BF16 || QT == XT_F16 ? 2 : 1;
+  constexpr int NQ = !WIDE ? 1 : CT == XT_BF16 ? 3 : 2, NP = WIDE ? NQ : 2;
   constexpr int ES = ct_bytes(CT), E = 16 / ES, NCH = DP / (4 * E);  // columns in 16 bytes, key loads of a lane's row
   constexpr int SUB = F32 ? 1 : 2, SB = 16 * SUB;
   constexpr int EV = E < DP / 16 ? E : DP / 16, DB = DP / (16 * EV), NF = DP / 16;  // columns of a value load, loads

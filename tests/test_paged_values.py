@@ -1,0 +1,69 @@
+"""The attention over an 8-bit paged cache (DevicePagedKVBuffer.attend) where the
+values' scales differ: inputs whose scores are exact, so that the bound is that
+of the weights times the values alone.
+
+With u = 2^-24 and scores that the kernel has exactly (0, or below all weight):
+a weight times its value's scale is off by two roundings and by 2^-22 of itself
+(two fp16 pieces), the sum of n products by (n + 16) u of its size, the sum of
+weights and the division by (n + 8) u; the output by half a step of its type."""
+import pytest
+import torch
+
+from conftest import announce
+from sbq.state import DevicePagedKVBuffer
+
+F32, F16, BF16, I8, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
+U = 2.0 ** -24
+
+
+def _codes(shape, dtype, g):
+    """Random codes: whole numbers, exact in either type."""
+    return torch.randint(-120 if dtype == I8 else -15, 121 if dtype == I8 else 16, shape, generator=g)
+
+
+def _cache(dev, dtype, k_codes, v_codes, v_scale, page=16, window=None):
+    """A buffer that holds codes [B, n, heads, dim] and the values' scales [B, n, heads]; the keys' are 1."""
+    B, n, heads, dim = v_codes.shape
+    width = -(-n // page)
+    b = DevicePagedKVBuffer(B, heads, dim, B * width, page, width, window, dev, dtype)
+    g = torch.Generator().manual_seed(n)
+    b.table.copy_(torch.randperm(B * width, generator=g).view(B, width))
+    b.length.fill_(n)
+    pos = torch.arange(n)
+    at = b.table.cpu().long()[:, pos // page]  # [B, n]
+    for pool, scale, codes, scales in ((b.k, b.k_scale, k_codes, torch.ones(B, n, heads)), (b.v, b.v_scale, v_codes, v_scale)):
+        host, s = torch.zeros(pool.shape), torch.zeros(scale.shape)
+        host[at, :, pos % page] = codes.float()
+        s[at, :, pos % page] = scales.float()
+        pool.copy_(host.to(dtype))
+        scale.copy_(s)
+    return b
+
+
+def _step(t, out):
+    """Half a step of type t at `out`, and of its smallest numbers."""
+    return out.abs() * (torch.finfo(t).eps / 2) * 1.001 + (2.0 ** -25 if t == F16 else 1e-38)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+def test_weights_keep_more_bits_than_the_output(dev, dtype, qt):
+    """Equal scores and different scales of values: no rounding of the weights shows in the output."""
+    g = torch.Generator().manual_seed(1)
+    for n in (2, 40):
+        announce(f"{n} values of equal weight, {dtype} {qt}")
+        B, heads, dim = 16, 2, 64
+        v = _codes((B, n, heads, dim), dtype, g)
+        if n == 2:
+            v[:, 1] = 0  # the larger scale has no values
+        scale = torch.rand(B, n, heads, generator=g) / 2 + 0.5
+        scale[:, 1] = 1.0
+        b = _cache(dev, dtype, torch.zeros(B, n, heads, dim), v, scale)
+        q = torch.randn(B, 1, 4, dim, generator=g).to(qt).to(dev)
+        got = b.attend(q)[:, 0].double().cpu()
+        x = v.double() * scale.double()[..., None]
+        want, size = [t.mean(1).repeat_interleave(2, 1) for t in (x, x.abs())]
+        tol = size * (2.0 ** -22 + (2 * n + 28) * U)
+        tol += _step(qt, want.abs() + tol)
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
