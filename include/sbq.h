@@ -635,10 +635,15 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * What a row does not see does not reach it, infinities and NaN included.
  * q: device [sequences, T, heads, D], T <= SBQ_PAGED_MAX_T, F32, or the
  * cache's type (8-bit caches: any); out: the same shape and type, apart from
- * every input.  Scores, maxima and sums are fp32; fp32 queries are multiplied
- * to 22 significant bits or more, and so are their weights; with 2-byte
- * queries the weights keep 16 bits or more.
+ * every input.  Scores, maxima and sums are fp32.  The other factors are multiplied
+ * as they are, or where the cache's type has fewer bits in pieces of it (8 bits: of
+ * fp16): BF16 caches 24 bits of fp32 queries and their weights, 16 of the weights of
+ * BF16 queries; F16 and 8-bit caches each element of an fp32 query, and each weight
+ * (8 bits: times its value's scale), to 2^-22 of itself or 2^-39 of the row's
+ * largest, whichever is more (F16, scores from 2^23 on: weights 2^-25 of the largest).
  * scale * q . k is to be finite, below 2^27 in magnitude.
+ * F32 and BF16 caches: |v| times the positions that a row sees is to stay below
+ * 2^127, what the fp32 sums hold.
  * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
  * content; one call at a time.  The result does not depend on timing; how a
  * long sequence is split, and so its last bits, goes by all sequences' lengths. */

@@ -278,6 +278,11 @@ __device__ __forceinline__ float wave_minmax(float v) {
 }
 __device__ __forceinline__ float wave_max(float v) { return wave_minmax<true>(v); }
 __device__ __forceinline__ float wave_min(float v) { return wave_minmax<false>(v); }
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
 __device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

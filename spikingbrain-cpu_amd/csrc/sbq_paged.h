@@ -66,15 +66,18 @@ __device__ __forceinline__ int64_t paged_count(const int64_t* counts, int64_t b,
 //     position's scales multiply its score and its weight.
 // The weights are rounded for the product with V: as many pieces as the queries
 // with fp32 ones; else two, whose error stays far below the output's rounding
-// (one would add to it: the sum of weights is not rounded with them).  fp16 weights are taken against 2^14 at the maximum, so
-// that one 2^-28 of it keeps its bits.
+// (one would add to it: the sum of weights is not rounded with them).  fp16 pieces
+// are of what is multiplied, against 2^14 at the row's largest so far: of the
+// weight, or with 8 bits of the weight times the value's scale (against the largest
+// scale, one far above the others would take their bits with no weight of its own).
+// So 2^-28 of the largest keeps 11 bits, and what is lost is 2^-39 of it.
 struct PagedArgs {
   PagedCache c;
   const void* q;
   const int64_t *start, *counts;
   void* out;
-  float* part_o;    // [Hk][places][R][DP]
-  float2* part_ml;  // [Hk][places][R]
+  float* part_o;    // [Hk][places][R][DP]: a part's mean of the values
+  float2* part_ml;  // [Hk][places][R]: its largest score, and its sum of weights against that
   int2* joins;      // [tiles of tile_rows rows][n]: a sequence's first place, and how many
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
   int T, rep, qt, tile_rows;
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
   constexpr int NFR = DP / 32;                                                       // 16x16x32 steps of a score
   constexpr int HP = 16 * EV > 128 || DP < 128 ? DP : 128, OLD = HP + 4;  // columns joined at a time: whole value loads
   static_assert(HP % (16 * EV) == 0 && DP % HP == 0, "the joining takes whole value loads");
-  constexpr float kNone = -__builtin_inff();
+  constexpr float kNone = -__builtin_inff(), kUnitMin = 0x1p-112f;
   typedef typename PagedMath<CT>::T M;
   typedef typename PagedMath<CT>::V MV;
   typedef uint32_t KV __attribute__((ext_vector_type(4)));
@@ -498,13 +501,13 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 
       f32x4 o[RT][NF];
       float m[RT], l[RT];
-      float vref[RT], vinv[RT];  // 8-bit: O's unit, the largest value scale that the row saw so far
+      float vref[RT], vinv[RT];  // 8-bit: O's unit, the row's largest weight times value scale so far, and 2^14 of its inverse
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) o[rt][f] = (f32x4)(0.0f);
         m[rt] = kNone, l[rt] = 0.0f;
-        vref[rt] = 1.17549435e-38f, vinv[rt] = 1.0f / vref[rt];
+        vref[rt] = kUnitMin, vinv[rt] = 0x1p14f / kUnitMin;
       }
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {
@@ -593,15 +596,20 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
           for (int st = 0; st < SUB; ++st)
 #pragma unroll
             for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, e[rt][st][v]);
-          mx = reference<XT_F16, !F32 && CT != XT_BF16>(mx);
+          mx = reference<XT_F16, CT == XT_F16>(mx);
+          float kept = 1.0f;  // 8-bit: what of the unit is left
           if (__any(mx > m[rt])) {
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float up = __builtin_fmaxf(m[rt], mx), alpha = up == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
             m[rt] = up;
             l[rt] *= alpha;
+            if constexpr (B8) {
+              kept = alpha;
+            } else {
 #pragma unroll
-            for (int f = 0; f < NF; ++f) o[rt][f] *= alpha;
+              for (int f = 0; f < NF; ++f) o[rt][f] *= alpha;
+            }
           }
           const float from = m[rt] == kNone ? 0.0f : m[rt];
 #pragma unroll
@@ -612,24 +620,28 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
               l[rt] += e[rt][st][v];
             }
 
-          if constexpr (B8) {  // the weights times the values' scales, in units of vref
+          if constexpr (B8) {  // the weights times the values' scales, against 2^14 at the largest of them
             float top = 0.0f;
 #pragma unroll
             for (int st = 0; st < SUB; ++st)
 #pragma unroll
-              for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, vr[st][v]);  // (NaN: the other one)
-            if (__any(top > vref[rt])) {
+              for (int v = 0; v < 4; ++v) {
+                e[rt][st][v] *= vr[st][v];
+                top = __builtin_fmaxf(top, e[rt][st][v]);  // (NaN: the other one)
+              }
+            const float unit = vref[rt] * kept;
+            if (__any(kept != 1.0f || top > unit)) {
               top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
               top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
-              const float up = __builtin_fmaxf(vref[rt], top), alpha = vref[rt] / up;
-              vref[rt] = up, vinv[rt] = 1.0f / up;
+              const float up = __builtin_fmaxf(__builtin_fmaxf(unit, top), kUnitMin), alpha = unit / up;
+              vref[rt] = up, vinv[rt] = 0x1p14f / up;
 #pragma unroll
               for (int f = 0; f < NF; ++f) o[rt][f] *= alpha;
             }
 #pragma unroll
             for (int st = 0; st < SUB; ++st)
 #pragma unroll
-              for (int v = 0; v < 4; ++v) e[rt][st][v] *= vr[st][v] * vinv[rt];
+              for (int v = 0; v < 4; ++v) e[rt][st][v] *= vinv[rt];
           }
         }
 
@@ -761,7 +773,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         }
       }
 
-      // the workgroup's waves joined
+      // the workgroup's waves joined: each one's mean of the values, which is never
+      // larger than they are, and its sum of weights
       int first = 0, places = 1;
       if (a.slots) places = paged_places(p.b, p.each, p.before, p.blocks, first);
       const int place = slot + p.b;
@@ -773,7 +786,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         l[rt] += __shfl_xor(l[rt], 16, 64);
         l[rt] += __shfl_xor(l[rt], 32, 64);
         if (g == 0) lds_m[rt][w][c] = m[rt], lds_l[rt][w][c] = l[rt];
-        const float unit = B8 ? vref[rt] : 1.0f;
+        const float less = (B8 ? 0x1p-14f : 1.0f) * (l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f);
+        const float unit = B8 ? vref[rt] : 1.0f;  // (after `less`: the product of both can underflow)
         const int here = min(rows - rt * 16, 16);  // (none: nothing is copied or joined)
 #pragma unroll
         for (int h0 = 0; h0 < DP; h0 += HP) {
@@ -785,7 +799,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 #pragma unroll
               for (int v = 0; v < 4; ++v)
 #pragma unroll
-                for (int k = 0; k < EV; ++k) to[db * 16 * EV - h0 + (4 * g + v) * EV + k] = o[rt][db * EV + k][v] * unit;
+                for (int k = 0; k < EV; ++k) to[db * 16 * EV - h0 + (4 * g + v) * EV + k] = o[rt][db * EV + k][v] * less * unit;
           }
           __syncthreads();
           for (int u = tid; u < here * (HP / 4); u += kAttnWaves * 64) {
@@ -795,15 +809,18 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
             for (int k = 0; k < kAttnWaves; ++k) top = __builtin_fmaxf(top, lds_m[rt][k][rr]);
             const float ref = top == kNone ? 0.0f : top;
             f32x4 sum = (f32x4)(0.0f);
-            float ls = 0.0f;
+            float part[kAttnWaves], ls = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k) {  // (a wave that saw nothing adds nothing)
+              const float lk = lds_l[rt][k][rr];
+              part[k] = lk != 0.0f ? __builtin_amdgcn_exp2f(lds_m[rt][k][rr] - ref) * lk : 0.0f;
+              ls += part[k];
+            }
+            const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
 #pragma unroll
             for (int k = 0; k < kAttnWaves; ++k) {
-              const float f = __builtin_amdgcn_exp2f(lds_m[rt][k][rr] - ref), lk = lds_l[rt][k][rr];
               const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
-              if (lk != 0.0f) {  // (a wave that saw nothing adds nothing)
-                sum += x * f;
-                ls += lk * f;
-              }
+              if (part[k] != 0.0f) sum += x * (part[k] * inv);
             }
             const int r = row0 + rt * 16 + rr;
             if (!alone) {
@@ -814,9 +831,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
               int t = 0, h = r;
               if (a.T > 1) t = r / a.rep, h = r - t * a.rep;
               const bool any = span.last(t) >= span.first(t, a.window);
-              const float inv = ls != 0.0f ? 1.0f / ls : 0.0f;
               const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + h) * a.o_sh + d;
-              if (d < pc.D) store_y4(a.out, QT, out, any ? sum * inv : (f32x4)(0.0f), a.ovec && d + 4 <= pc.D, pc.D - d);
+              if (d < pc.D) store_y4(a.out, QT, out, any ? sum : (f32x4)(0.0f), a.ovec && d + 4 <= pc.D, pc.D - d);
             }
           }
         }

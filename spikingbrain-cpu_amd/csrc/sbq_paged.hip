@@ -333,13 +333,14 @@ void plan(PagedStore& a) {
   a.parts = (int)std::max<int64_t>(1, std::min(want, room));
 }
 
-// One row's splits joined: the maximum over their maxima, then the partial sums
-// scaled to it, independent loads eight at a time.
+// One row's splits joined: the maximum over their maxima and the sum of weights
+// against it by every wave, then the means by their shares of that sum (no more
+// than the values themselves, whatever their number), independent loads eight at
+// a time.
 template <int DP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   constexpr int ND = DP / 4, NG = 256 / ND, U = 8;
   __shared__ __align__(16) f32x4 lds[NG][ND];
-  __shared__ float lds_l[NG];
   const int R = a.rep * a.T, lane = threadIdx.x & 63, d = threadIdx.x % ND * 4, grp = threadIdx.x / ND;
   const int r = blockIdx.x, kvh = blockIdx.y, t = a.T > 1 ? r / a.rep : 0;
   const int64_t b = a.first + blockIdx.z;
@@ -350,8 +351,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   if (used == 1) return;  // (written by the one workgroup)
   const int64_t at = ((int64_t)kvh * a.places + places.x) * R + r;
   const float2* const ml = a.part_ml + at;
-  float top = -__builtin_inff(), l = 0.0f;
-  if (lane < used) top = ml[(int64_t)lane * R].x;
+  float2 mine = make_float2(-__builtin_inff(), 0.0f);
+  if (lane < used) mine = ml[(int64_t)lane * R];
   f32x4 x[U], sum = (f32x4)(0.0f);
   float2 y[U];
   auto fetch = [&](int s0) {
@@ -363,32 +364,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     }
   };
   fetch(grp);  // (on their way while the maximum is found)
+  float top = mine.x;
   for (int s = lane + 64; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
   top = wave_max(top);
   const float from = top == -__builtin_inff() ? 0.0f : top;
+  // (a split that saw nothing adds nothing)
+  auto weight = [&](float2 v) { return v.y != 0.0f ? __builtin_amdgcn_exp2f(v.x - from) * v.y : 0.0f; };
+  float l = weight(mine);
+  for (int s = lane + 64; s < used; s += 64) l += weight(ml[(int64_t)s * R]);
+  l = wave_sum(l);
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   for (int s0 = grp; s0 < used; s0 += U * NG) {
     if (s0 != grp) fetch(s0);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const float f = __builtin_amdgcn_exp2f(y[k].x - from);
-      if (s0 + k * NG < used && y[k].y != 0.0f) {  // (a split that saw nothing adds nothing)
-        sum += x[k] * f;
-        l += y[k].y * f;
-      }
+      const float f = weight(y[k]);
+      if (s0 + k * NG < used && f != 0.0f) sum += x[k] * (f * inv);
     }
   }
   lds[grp][threadIdx.x % ND] = sum;
-  if (d == 0) lds_l[grp] = l;
   __syncthreads();
   if (grp) return;
-  l = lds_l[0];
 #pragma unroll
-  for (int k = 1; k < NG; ++k) {
-    sum += lds[k][threadIdx.x];
-    l += lds_l[k];
-  }
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  sum = span.last(t) >= span.first(t, a.window) ? sum * inv : (f32x4)(0.0f);
+  for (int k = 1; k < NG; ++k) sum += lds[k][threadIdx.x];
+  if (span.last(t) < span.first(t, a.window)) sum = (f32x4)(0.0f);
   const int64_t out = b * a.o_sb + (int64_t)t * a.o_st + (int64_t)(kvh * a.rep + r - t * a.rep) * a.o_sh + d;
   if (d < a.c.D) store_y4(a.out, a.qt, out, sum, a.ovec && d + 4 <= a.c.D, a.c.D - d);
 }

@@ -67,3 +67,65 @@ def test_weights_keep_more_bits_than_the_output(dev, dtype, qt):
         tol = size * (2.0 ** -22 + (2 * n + 28) * U)
         tol += _step(qt, want.abs() + tol)
         assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt", [F32, F16, BF16])
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+@pytest.mark.parametrize("n,heavy", [(2, 0), (2, 1), (30, 7), (200, 0), (200, 133), (200, 199), (3000, 17), (3000, 2900)])
+def test_scales_of_values_without_weight(dev, n, heavy, dtype, qt):
+    """One position takes the weight, the others have values up to 2^90 times as
+    large and weights 2^-60: each sequence its own ratio, from one where the others
+    are nothing to one where they are all.  The scores are 0 and -42 (a whole number
+    in every type; its weight is off by 2^-18 of itself: 61 powers of two in fp32
+    steps of 2^-19, and exp2).  A weight times a scale far below the row's largest is
+    off by 2^-39 of that instead of 2^-22 of itself."""
+    announce(f"{n} values, the weight at {heavy}, {dtype} {qt}")
+    ratios = [0, 3, 14, 20, 24, 27, 30, 34, 38, 45, 55, 58, 60, 62, 66, 80, 90]
+    B, heads, dim = len(ratios), 2, 64
+    g = torch.Generator().manual_seed(n + heavy)
+    v = _codes((B, n, heads, dim), dtype, g)
+    k = torch.zeros(B, n, heads, dim)
+    k[..., 5] = -1
+    k[:, heavy, :, 5] = 0
+    q = torch.zeros(B, 1, 4, dim)
+    q[..., 5] = 42
+    light = torch.exp2(torch.tensor(ratios).double())[:, None, None]
+    is_heavy = (torch.arange(n) == heavy)[None, :, None]
+    for unit in (1.0, 2.0 ** -100, 2.0 ** 28):
+        scale = (torch.where(is_heavy, 1.0, light) * unit).expand(B, n, heads) * (1 + torch.randint(0, 128, (B, n, heads), generator=g) / 128)
+        b = _cache(dev, dtype, k, v, scale)
+        got = b.attend(q.to(qt).to(dev), scale=1.0)[:, 0].double().cpu()
+        p = torch.where(is_heavy, 1.0, torch.tensor(-42.0).double().exp())[..., None].expand(B, n, heads, 1)
+        x, total = v.double() * scale[..., None], p.sum(1)
+        want, size, small = [((p * t).sum(1) / total).repeat_interleave(2, 1)
+                             for t in (x, x.abs(), torch.where(is_heavy[..., None], 0.0, x.abs()))]
+        top = (p * scale[..., None]).amax(1, keepdim=True) * v.abs().double()  # the unit times each code
+        tol = size * (2.0 ** -22 + (2 * n + 28) * U) + small * 2.0 ** -18 + top.sum(1).repeat_interleave(2, 1) * 2.0 ** -39
+        tol += _step(qt, want.abs() + tol)
+        if qt == F16:  # (an output past its largest number)
+            over = (want.abs() + tol) > 65504
+            want, got, tol = [torch.where(over, 0.0, t) for t in (want, got, tol)]
+        assert torch.isfinite(got).all()
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).amax((1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qt", [F32, BF16])
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+def test_largest_and_smallest_values(dev, dtype, qt):
+    """Values up to 2^126 (their sums still below fp32's largest), down to 2^-120, of equal weight."""
+    B, n, heads, dim = 2, 3, 1, 64
+    g = torch.Generator().manual_seed(3)
+    for e in (118, 100, -100, -113):
+        announce(f"values of 2^{e} {dtype} {qt}")
+        v = _codes((B, n, heads, dim), dtype, g).clamp(-80, 80)
+        scale = torch.full((B, n, heads), 2.0 ** e) * (1 + torch.rand(B, n, heads, generator=g) / 8)
+        b = _cache(dev, dtype, torch.zeros(B, n, heads, dim), v, scale)
+        got = b.attend(torch.zeros(B, 1, 2, dim, dtype=qt, device=dev))[:, 0].double().cpu()
+        x = v.double() * scale.double()[..., None]
+        want, size = [t.mean(1).expand(B, 2, dim) for t in (x, x.abs())]
+        tol = size * (2.0 ** -22 + (2 * n + 28) * U) + 2.0 ** -140
+        tol += _step(qt, want.abs() + tol)
+        assert torch.isfinite(got).all()
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
