@@ -512,12 +512,16 @@ class DevicePagedKVBuffer:
 
     def reserve(self, sequence: int, length: int) -> None:
         """Give `sequence` the pages that positions below `length` need and it
-        does not have.  All or none of them: ValueError if the table's row is
-        too short, RuntimeError if the pool has too few free pages."""
+        does not have, from those released behind a position on.  All or none of
+        them: ValueError if the table's row is too short or all those positions
+        were released, RuntimeError if the pool has too few free pages."""
         held = self._held[self._row("reserve", sequence)]
         last = -(-length // self.page)
         if last > self.table.shape[1]:
             raise ValueError(f"DevicePagedKVBuffer.reserve: {length} positions are more than the table's row holds")
+        if 0 < last <= self._first[sequence]:
+            raise ValueError(f"DevicePagedKVBuffer.reserve: the pages of the first {self._first[sequence] * self.page} positions "
+                             "were released")
         want = [i for i in range(self._first[sequence], last) if i not in held]
         if len(want) > len(self._free):
             raise RuntimeError(f"DevicePagedKVBuffer.reserve: {len(want)} pages wanted, {len(self._free)} free")
@@ -532,7 +536,8 @@ class DevicePagedKVBuffer:
     def release(self, sequence: int, before: int | None = None) -> None:
         """Take the sequence's pages back and forget its positions; with
         `before` only the pages that end at or below that position (which a
-        window has left behind)."""
+        window has left behind): nothing is stored there again before the whole
+        sequence is released or truncated to 0."""
         held = self._held[self._row("release", sequence)]
         first = self.table.shape[1] if before is None else max(0, before // self.page)
         for i in [i for i in held if i < first]:
@@ -588,6 +593,12 @@ class DevicePagedKVBuffer:
                 t["table"].data_ptr() + 4 * width * at, self.sequences if sequence is None else 1, width,
                 t["length"].data_ptr() + 8 * at)
 
+    def _not_released(self, fn: str, position: int, sequence: int | None) -> None:
+        """No page from `position` on was released."""
+        first = max(self._first) if sequence is None else self._first[sequence]
+        if first and position < first * self.page:
+            raise ValueError(f"DevicePagedKVBuffer.{fn}: the pages of the first {first * self.page} positions were released")
+
     def _places(self, fn: str, name: str, t, n: int) -> torch.Tensor:
         """int64 [n] on the device; an int for every sequence."""
         if not isinstance(t, torch.Tensor):
@@ -632,6 +643,8 @@ class DevicePagedKVBuffer:
             at_k, at_v, st = k.data_ptr(), v.data_ptr(), k.stride()
         at = length
         if start is not None:
+            if not isinstance(start, torch.Tensor):
+                self._not_released("append", start, sequence)
             start = self._places("append", "start", start, n)
             at = start.data_ptr()
             if at != length and abs(at - length) < 8 * n:  # (other sequences' lengths, which this call moves)
@@ -753,11 +766,18 @@ class DevicePagedKVBuffer:
 
     def truncate(self, length) -> None:
         """Forget positions >= length (an int or int64 [sequences]), for
-        instance the drafts that were refused; below 0 as 0."""
+        instance the drafts that were refused; below 0 as 0.  No further back
+        than pages that were released, but for an int of 0, which forgets all
+        positions: then those pages can be reserved again."""
         if isinstance(length, torch.Tensor):
             self.length.copy_(torch.minimum(self.length, self._places("truncate", "length", length, self.sequences)).clamp_(min=0))
         else:
-            self.length.clamp_(max=max(0, int(length)))
+            length = max(0, int(length))
+            if length:
+                self._not_released("truncate", length, None)
+            self.length.clamp_(max=length)
+            if not length:
+                self._first = [0] * self.sequences
 
 
 @dataclass
