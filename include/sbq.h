@@ -613,7 +613,8 @@ int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, in
  *
  * sbq_paged_read: positions start[b] .. start[b] + count - 1 of each sequence,
  * to k_out, v_out (device [sequences, count, kv_heads, D], strides o_sb, o_st,
- * o_sh, rounded to out_dtype); positions that it does not hold are 0. */
+ * o_sh in any order of the axes, no two elements in one place, rounded to out_dtype);
+ * positions that it does not hold are 0. */
 int sbq_paged_append(void* k, void* v, float* k_scale, float* v_scale, int cache_dtype, int64_t pages,
                      int64_t page, int64_t kv_heads, int64_t D, const int32_t* table, int64_t sequences,
                      int64_t max_pages, int64_t* length, const int64_t* start, const int64_t* counts,
@@ -634,8 +635,8 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * see nothing.  A row that sees nothing (or only scores of -infinity) is 0.
  * What a row does not see does not reach it, infinities and NaN included.
  * q: device [sequences, T, heads, D], T <= SBQ_PAGED_MAX_T, F32, or the
- * cache's type (8-bit caches: any); out: the same shape and type, apart from
- * every input.  Scores, maxima and sums are fp32.  The other factors are multiplied
+ * cache's type (8-bit caches: any); out: the same shape and type, its axes in any
+ * order, no two elements in one place, apart from every input.  Scores, maxima and sums are fp32.  The other factors are multiplied
  * as they are, or where the cache's type has fewer bits in pieces of it (8 bits: of
  * fp16): BF16 caches 24 bits of fp32 queries and their weights, 16 of the weights of
  * BF16 queries; F16 and 8-bit caches each element of an fp32 query, and each weight

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <utility>
 
 #include "sbq.h"
 #include "sbq_common.h"
@@ -678,11 +679,21 @@ static int check_attn(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int
   return SBQ_OK;
 }
 
-// Do the elements of a written [n, heads, D] array lie apart?
-static bool apart(int64_t n, int64_t heads, int64_t D, int64_t st, int64_t sh) {
-  const __int128 D1 = D, n1 = n - 1, h1 = heads - 1;
-  return (heads == 1 || sh >= D) && (n == 1 || st >= D) &&
-         (n == 1 || heads == 1 || st >= h1 * sh + D1 || sh >= n1 * st + D1);
+// Do the elements of a written [n, heads, D] array (of `B` such, sb apart) lie
+// apart?  In any order of the axes, each one's stride past all that the smaller
+// ones span.
+static bool apart(int64_t n, int64_t heads, int64_t D, int64_t st, int64_t sh, int64_t B = 1, int64_t sb = 0) {
+  int64_t axis[3][2] = {{st, n}, {sh, heads}, {sb, B}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (axis[j][0] > axis[j + 1][0]) std::swap(axis[j], axis[j + 1]);
+  __int128 span = D;
+  for (const auto& x : axis) {
+    if (x[1] == 1) continue;
+    if (x[0] < span) return false;
+    span += (__int128)(x[1] - 1) * x[0];
+  }
+  return true;
 }
 
 int64_t sbq_attn_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int64_t slots, int weight) {
@@ -863,10 +874,7 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
   if (count < 0 || count > (1 << 30) / kv_heads) return SBQ_ERR_ARG;
   if (sequences == 0 || count == 0) return SBQ_OK;
   if (!start || !k_out || !v_out) return SBQ_ERR_ARG;
-  // (a sequence's [count, kv_heads, D] lies apart from the next one's)
-  if (!apart(count, kv_heads, D, o_st, o_sh) ||
-      (sequences > 1 && (__int128)o_sb < (__int128)(count - 1) * o_st + (__int128)(kv_heads - 1) * o_sh + D))
-    return SBQ_ERR_ARG;
+  if (!apart(count, kv_heads, D, o_st, o_sh, sequences, o_sb)) return SBQ_ERR_ARG;
   const int64_t es = esize(out_dtype);
   if (!aligned(start, 8) || !aligned(k_out, es) || !aligned(v_out, es)) return SBQ_ERR_ALIGN;
   s.start = start, s.k_out = k_out, s.v_out = v_out, s.T = count, s.n_sb = o_sb, s.n_st = o_st, s.n_sh = o_sh;
@@ -902,9 +910,7 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
   if (!paged_rows_ok(T, heads, kv_heads) || window < 0 || scale != scale) return SBQ_ERR_ARG;
   if (sequences == 0 || T == 0) return SBQ_OK;
   if (!q || !out || q_sb < 0 || q_st < 0 || q_sh < 0) return SBQ_ERR_ARG;
-  if (!apart(T, heads, D, o_st, o_sh) ||
-      (sequences > 1 && (__int128)o_sb < (__int128)(T - 1) * o_st + (__int128)(heads - 1) * o_sh + D))
-    return SBQ_ERR_ARG;
+  if (!apart(T, heads, D, o_st, o_sh, sequences, o_sb)) return SBQ_ERR_ARG;
   const int64_t es = esize(q_dtype);
   if (!aligned(q, es) || !aligned(out, es) || !aligned(start, 8) || !aligned(counts, 8)) return SBQ_ERR_ALIGN;
   const int64_t need = sbq_paged_attn_workspace_bytes(sequences, T, heads, kv_heads, D, page, max_pages, window, cache_dtype);
