@@ -143,6 +143,34 @@ def _nbytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from t's first byte to past its last."""
+    at, n = t.data_ptr(), 1
+    for size, stride in zip(t.shape, t.stride()):
+        if size == 0:
+            return 0, 0
+        n += (size - 1) * stride
+    return at, at + n * t.element_size()
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do a and b share memory?  Between each other's rows they do not: where for
+    some stride, of which the others are parts or multiples, the parts lie apart in
+    every one of its steps (views of one projection's output)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    axes = []
+    for t in (a, b):
+        size = t.element_size()
+        axes.append([(s * size, n) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, size)])
+    for step in {s for s, _ in axes[0] if s > 1}:
+        ea, eb = (1 + sum((n - 1) * s for s, n in x if s % step) for x in axes)
+        if ea <= (b0 - a0) % step <= step - eb:
+            return False
+    return True
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, features]."""
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -671,8 +699,9 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     if workspace is None:
         room = _verify_workspace_bytes(B, V)
         workspace = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device")
+    elif workspace.device != dev or not workspace.is_contiguous() or any(
+            t is not None and _meet(workspace, t) for t in (target, draft, tokens, u, counts)):
+        raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device, apart from the inputs")
     ps, qs = target.stride(), (0, 0) if draft is None else draft.stride()
     with _on_device(dev):
         _lib.check(_lib.load().sbq_verify_drafts(

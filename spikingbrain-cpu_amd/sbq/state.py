@@ -36,7 +36,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from .quant import _DTYPE_CODE, _on_device, _stream
+from .quant import _DTYPE_CODE, _meet, _on_device, _span, _stream
 
 
 def _as_pos(p, device: torch.device) -> torch.Tensor:
@@ -169,7 +169,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     positions: int64 [n], tokens a multiple of n: token t stands at positions[t
     // (tokens / n)] + t % (tokens / n), so [tokens] gives each its own and the
     starts of n sequences are enough for their next tokens.  q_out, k_out: q and
-    k themselves, or tensors apart from both (default: new ones)."""
+    k themselves, or tensors apart from each other and every input (default: new
+    ones)."""
     gpu, dtype, shape, device = q.get_device(), q.dtype, q.shape, q.device
     code, n, pairs = _DTYPE_CODE.get(dtype), positions.numel(), inv_freq.numel()
     wt = None if q_weight is None else q_weight.dtype
@@ -188,10 +189,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if qs[2] != 1 and dim > 1:
         q = q.contiguous()
         qs = q.stride()
+    given = q_out is not None or k_out is not None
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif q_out.shape != shape or q_out.dtype != dtype or q_out.get_device() != gpu or (dim > 1 and q_out.stride(2) != 1) \
-            or (q_out.data_ptr() == q.data_ptr() and q_out.stride() != qs):
+    elif q_out.shape != shape or q_out.dtype != dtype or q_out.get_device() != gpu or (dim > 1 and q_out.stride(2) != 1):
         raise ValueError("qk_norm_rope: q_out must have q's shape, dtype and device, with unit stride in dim")
     kv_heads = at_k = at_ko = 0
     ks = ko = (0, 0)
@@ -207,12 +208,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             ks = k.stride()
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-        elif k_out.shape != kshape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1) \
-                or (k_out.data_ptr() == k.data_ptr() and k_out.stride() != ks):
+        elif k_out.shape != kshape or k_out.dtype != dtype or k_out.get_device() != gpu or (dim > 1 and k_out.stride(2) != 1):
             raise ValueError("qk_norm_rope: k_out must have k's shape, dtype and device, with unit stride in dim")
         kv_heads, ko, at_k, at_ko = kshape[1], k_out.stride(), k.data_ptr(), k_out.data_ptr()
     if tokens == 0:
         return q_out, k_out
+    if given and not (q_out is q and k_out is k and _plainly_apart(q, k, (positions, inv_freq, q_weight, k_weight))):
+        _apart_rope(q, k, q_out, k_out, (positions, inv_freq, q_weight, k_weight))
     qo = q_out.stride()
     with _on_device(device):
         _lib.check(_lib.load().sbq_qk_norm_rope(
@@ -221,6 +223,41 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             None if k_weight is None else k_weight.data_ptr(), 0 if wt is None else _DTYPE_CODE[wt], eps, q_out.data_ptr(), at_ko,
             qo[0], qo[1], ko[0], ko[1], _stream(device)), "sbq_qk_norm_rope")
     return q_out, k_out
+
+
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Are a and b, of one shape and dtype, the same elements?"""
+    return a.data_ptr() == b.data_ptr() and all(s == t for n, s, t in zip(a.shape, a.stride(), b.stride()) if n > 1)
+
+
+def _plainly_apart(q: torch.Tensor, k: torch.Tensor | None, others) -> bool:
+    """Are q and k, written in place, heads of one projection's rows, and the
+    others elsewhere?  (The quick answer for what a step does every time.)"""
+    lo, (tokens, heads, dim), (st, sh, _), size = q.data_ptr(), q.shape, q.stride(), q.element_size()
+    step, of_q = st * size, ((heads - 1) * sh + dim) * size
+    hi = lo + (tokens - 1) * step + of_q
+    if k is not None:
+        at, (kt, kh, _) = k.data_ptr() - lo, k.stride()
+        of_k = ((k.shape[1] - 1) * kh + dim) * size
+        if kt != st or not of_q <= at <= step - of_k:
+            return False
+        hi += at + of_k - of_q
+    for t in others:
+        if t is not None and lo - 8 * t.numel() < t.data_ptr() < hi:
+            return False
+    return True
+
+
+def _apart_rope(q, k, q_out, k_out, others) -> None:
+    """Refuses outputs that are neither an input nor apart from everything."""
+    in_q, in_k = _same_place(q, q_out), k is not None and _same_place(k, k_out)
+    pairs = [] if in_q else [(q_out, q)]
+    if k is not None:
+        pairs += [(q_out, k_out)] + ([] if in_k else [(k_out, k), (q_out, k)]) + ([] if in_q else [(k_out, q)])
+    outs = [_span(t) for t in (q_out, k_out) if t is not None]
+    spans = [_span(t) for t in others if t is not None]
+    if any(_meet(a, b) for a, b in pairs) or any(a[0] < b[1] and b[0] < a[1] for a in outs for b in spans):
+        raise ValueError("qk_norm_rope: q_out and k_out must be q and k themselves, or apart from each other and every input")
 
 
 def _refuse_rope(q, positions, inv_freq, q_weight, k_weight):
@@ -582,6 +619,7 @@ class DevicePagedKVBuffer:
         self._sizes = (code, k.shape[0], self.page, self.heads, self.dim, table.shape[1])
         self._dev, self._gpu, self._b8 = dev, k.get_device(), code >= _lib.SBQ_I8
         self._bytes = k.shape[0] * strides[0] * k.element_size()
+        self._spans = [_span(t) for t in self._tensors.values() if t is not None]
         return self._sizes
 
     def _cache(self, fn: str, sequence: int | None) -> tuple:
@@ -707,16 +745,15 @@ class DevicePagedKVBuffer:
         default T) being how many of the T are there; the others' rows are 0,
         as is a row that sees nothing.  Query head h reads key head h // (q
         heads / heads).  q has the pool's dtype or float32 (8-bit pools: any);
-        the result has q's."""
+        the result has q's.  out and workspace lie apart from everything else."""
         cache = self._cache("attend", None)
         n, gpu, dim, kv_heads, dev, shape = cache[10], self._gpu, self.dim, self.heads, self._dev, q.shape
         code = self._query("attend", q)
+        given = [t for t in (out, workspace) if t is not None]
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(-1) != 1):
             raise ValueError("DevicePagedKVBuffer.attend: out must have q's shape, dtype and device, with unit stride in dim")
-        elif out.data_ptr() == q.data_ptr() and q.numel():
-            raise ValueError("DevicePagedKVBuffer.attend: out must not be q itself")
         T, heads = shape[1] if len(shape) == 4 else 1, shape[-2]
         if T == 0:
             return out
@@ -735,6 +772,8 @@ class DevicePagedKVBuffer:
             start = self._places("attend", "start", start, n)
         if counts is not None:
             counts = self._places("attend", "counts", counts, n)
+        if given:
+            self._apart(given, [t for t in (q, start, counts) if t is not None])
         qs, os_ = q.stride(), out.stride()
         with _on_device(dev):
             _lib.check(_lib.load().sbq_paged_attention(
@@ -743,6 +782,14 @@ class DevicePagedKVBuffer:
                 out.data_ptr(), os_[0], os_[-3], os_[-2], workspace.data_ptr() if room else None, room, _stream(dev)),
                 "sbq_paged_attention")
         return out
+
+    def _apart(self, written: list, read: list) -> None:
+        """Refuses an output or a workspace of attend that meets the other, an input or the buffer."""
+        for i, t in enumerate(written):
+            lo, hi = _span(t)
+            if any(lo < b and a < hi for a, b in self._spans) or any(_meet(t, r) for r in read + written[:i]):
+                raise ValueError("DevicePagedKVBuffer.attend: out and workspace must lie apart from each other, the inputs and "
+                                 "the buffer")
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
