@@ -92,8 +92,7 @@ SBQ_HD int64_t paged_row_of(int32_t id, int64_t pages, int64_t pos, int h, int H
 // How its attention cuts a launch's sequences into parts, one for each of `slots`
 // workgroups of kPagedWaves waves: a sequence counts its blocks in whole rounds of the
 // waves, one round at least (a sequence that sees nothing writes its zeros); a
-// part is `each` of all those; slot s's piece of sequence b, blocks n0..n1-1 of
-// it, leaves its partial results at place s + b.
+// part is `each` of all those; slot s's piece of sequence b are blocks n0..n1-1 of it.
 constexpr int kPagedWaves = 4;
 SBQ_HD int paged_own(int blocks) {
   const int n = (blocks + kPagedWaves - 1) / kPagedWaves * kPagedWaves;
@@ -113,11 +112,16 @@ SBQ_HD void paged_piece(int slot, int each, int before, int blocks, int& n0, int
   n0 = x0 > before ? (int)(x0 - before) : 0;
   n1 = x0 + each - before < own ? (int)(x0 + each - before) : own;
 }
-SBQ_HD int paged_places(int b, int each, int before, int blocks, int& first) {  // how many, from `first` on
+SBQ_HD int paged_places(int b, int each, int before, int blocks, int& first) {  // slots with a piece of it, from first - b on
   const unsigned s0 = (unsigned)before / (unsigned)each, s1 = (unsigned)(before + (blocks > 1 ? blocks : 1) - 1) / (unsigned)each;
   first = (int)s0 + b;
   return (int)(s1 - s0) + 1;
 }
+
+// Where a slot leaves the partial result of a sequence in several parts, whose first one
+// is slot `first`'s: two places a slot, for the sequence that its part goes on with and
+// the one that its part ends with and the next goes on with.
+SBQ_HD int paged_part_place(int slot, int first) { return 2 * slot + (slot == first); }
 
 // Column index of a key from argmax_key.
 SBQ_HD int argmax_key_index(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }

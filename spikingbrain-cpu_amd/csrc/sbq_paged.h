@@ -78,10 +78,10 @@ struct PagedArgs {
   void* out;
   float* part_o;    // [Hk][places][R][DP]: a part's mean of the values
   float2* part_ml;  // [Hk][places][R]: its largest score, and its sum of weights against that
-  int2* joins;      // [tiles of tile_rows rows][n]: a sequence's first place, and how many
+  int2* joins;      // [tiles of tile_rows rows][n]: a sequence's first slot, and how many
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, window, first;
   int T, rep, qt, tile_rows;
-  int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile (0: one each), and both
+  int n, slots, places;  // sequences of the launch, workgroups of a key head and row tile (0: one each), their places
   float per_slot;        // 1 / slots
   float scale;               // times log2(e)
   bool ovec;
@@ -136,11 +136,11 @@ __device__ __forceinline__ int wave_scan(int v) {
 // whatever the host knows of lengths.  A part that meets several does them in
 // turn, which costs it the way to the first keys and the joining of its waves
 // again (about what kPagedLonger fours cost): where parts of up to so many more
-// are enough for the sequences to begin with a part each, they do.  Slot s's
-// piece of sequence b leaves its partial results at place s + b, of which a
-// sequence's are neighbours.
-// Every workgroup finds its part by a scan over the lengths; which places a
-// sequence's are the workgroup of its first block notes for the joining.  Where no
+// are enough for the sequences to begin with a part each, they do.  A slot has
+// at most two pieces of sequences that others share, its first and its last, and
+// two places for their partial results (paged_part_place).
+// Every workgroup finds its part by a scan over the lengths; which slots a
+// sequence has the workgroup of its first block notes for the joining.  Where no
 // sequence is long (kPagedWhole), each has a workgroup of its own, and nothing is
 // joined.
 struct PagedPlace {
@@ -776,8 +776,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
       // the workgroup's waves joined: each one's mean of the values, which is never
       // larger than they are, and its sum of weights
       int first = 0, places = 1;
-      if (a.slots) places = paged_places(p.b, p.each, p.before, p.blocks, first);
-      const int place = slot + p.b;
+      if (a.slots) places = paged_places(p.b, p.each, p.before, p.blocks, first), first -= p.b;
+      const int place = paged_part_place(slot, first);
       const bool alone = places == 1;
       if (a.joins && n0 == 0 && kvh == 0 && tid == 0) a.joins[row0 / (16 * RT) * a.n + p.b] = make_int2(first, places);
       __syncthreads();  // (every wave has read its Q)

@@ -349,29 +349,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   span.of<true>(a, b);
   const int used = places.y;
   if (used == 1) return;  // (written by the one workgroup)
-  const int64_t at = ((int64_t)kvh * a.places + places.x) * R + r;
-  const float2* const ml = a.part_ml + at;
+  // the s-th of its partial results
+  auto at = [&](int s) { return ((int64_t)kvh * a.places + paged_part_place(places.x + s, places.x)) * R + r; };
   float2 mine = make_float2(-__builtin_inff(), 0.0f);
-  if (lane < used) mine = ml[(int64_t)lane * R];
+  if (lane < used) mine = a.part_ml[at(lane)];
   f32x4 x[U], sum = (f32x4)(0.0f);
   float2 y[U];
   auto fetch = [&](int s0) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int s = min(s0 + k * NG, used - 1);
-      x[k] = *(const f32x4*)(a.part_o + (at + (int64_t)s * R) * DP + d);
-      y[k] = ml[(int64_t)s * R];
+      x[k] = *(const f32x4*)(a.part_o + at(s) * DP + d);
+      y[k] = a.part_ml[at(s)];
     }
   };
   fetch(grp);  // (on their way while the maximum is found)
   float top = mine.x;
-  for (int s = lane + 64; s < used; s += 64) top = __builtin_fmaxf(top, ml[(int64_t)s * R].x);
+  for (int s = lane + 64; s < used; s += 64) top = __builtin_fmaxf(top, a.part_ml[at(s)].x);
   top = wave_max(top);
   const float from = top == -__builtin_inff() ? 0.0f : top;
   // (a split that saw nothing adds nothing)
   auto weight = [&](float2 v) { return v.y != 0.0f ? __builtin_amdgcn_exp2f(v.x - from) * v.y : 0.0f; };
   float l = weight(mine);
-  for (int s = lane + 64; s < used; s += 64) l += weight(ml[(int64_t)s * R]);
+  for (int s = lane + 64; s < used; s += 64) l += weight(a.part_ml[at(s)]);
   l = wave_sum(l);
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   for (int s0 = grp; s0 < used; s0 += U * NG) {
@@ -438,7 +438,7 @@ PagedPlan paged_plan(int64_t B, int64_t T, int64_t R, int64_t Hk, int64_t D, int
   p.n = std::max<int64_t>(1, std::min(p.n, ((int64_t)1 << 29) / (fours * kAttnWaves)));  // (all blocks fit an int, in whole parts too)
   p.slots = std::max<int64_t>(1, std::min(groups / one, p.n * fours));
   if (fours <= std::min(kPagedWhole + kPagedWholeFull * B * one / groups, kPagedWholeMost)) p.slots = 0, p.n = std::min(B, kPagedRows);
-  p.places = p.slots + p.n;
+  p.places = 2 * p.slots;
   p.joins = p.slots > 1;
   return p;
 }

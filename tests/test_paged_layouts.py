@@ -9,7 +9,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from sbq import quant
+from sbq import _lib, quant
 from sbq.quant import _meet
 from sbq.state import DevicePagedKVBuffer, _apart_rope, _plainly_apart, qk_norm_rope
 
@@ -193,3 +193,32 @@ def test_outputs_that_meet_an_input_are_refused(dev):
     tokens, u = torch.zeros(1, 1, dtype=torch.long, device=dev), torch.rand(1, 2, device=dev)
     with pytest.raises(ValueError, match="apart"):
         quant.verify_drafts(target, None, tokens, u, workspace=target)
+
+
+# ---------------------------------------------------------------------------
+# the attention's workspace
+# ---------------------------------------------------------------------------
+def test_places_of_partial_results(tmp_path):
+    exe = tmp_path / "paged_parts_check"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", str(PKG / "csrc"),
+                    str(HOST / "paged_parts_check.cpp"), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+def test_workspace_goes_by_the_chip_not_by_the_sequences():
+    """Two partial results for each of at most 768 workgroups, 32 rows of 256 columns
+    each, and a note for each of 512 sequences and 384 row tiles: 54 MB."""
+    L = _lib.load()
+    rng, most = random.Random(2), 0
+    calls = [(512, 16, 32, 8, 128, 64, 128, 0, 3), (256, 64, 32, 8, 128, 64, 128, 0, 3), (512, 64, 32, 8, 256, 64, 128, 0, 2),
+             (65536, 1, 1, 1, 256, 64, 4096, 0, 4)]
+    for _ in range(4000):
+        kv = rng.choice((1, 2, 8, 40))
+        page = 1 << rng.randrange(4, 11)
+        calls.append((rng.choice((1, 7, 64, 600, 5000)), rng.choice((1, 4, 64, 1024)), kv * rng.choice((1, 4, 7, 64)), kv,
+                      rng.choice((16, 64, 128, 256)), page, rng.randrange(1, (1 << rng.randrange(8, 21)) // page + 2),
+                      rng.choice((0, 0, 1000)), rng.randrange(5)))
+    for call in calls:
+        most = max(most, L.sbq_paged_attn_workspace_bytes(*call))
+    assert 10 << 20 < most < 54 * 10 ** 6
