@@ -278,10 +278,19 @@ __device__ __forceinline__ float wave_minmax(float v) {
 }
 __device__ __forceinline__ float wave_max(float v) { return wave_minmax<true>(v); }
 __device__ __forceinline__ float wave_min(float v) { return wave_minmax<false>(v); }
+// Their sum by the same moves (rows that a broadcast leaves out add 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  v = dpp_add<0xb1, 0xf>(v);
+  v = dpp_add<0x4e, 0xf>(v);
+  v = dpp_add<0x141, 0xf>(v);
+  v = dpp_add<0x140, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);
+  v = dpp_add<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
