@@ -568,7 +568,7 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
  * fp32, rounded once to the output's type.
  * q: device [tokens, heads, D], k: device [tokens, kv_heads, D] (kv_heads 0:
  * none) of one type, strides in elements, unit stride in D <= 256.
- * positions: device int64, below 2^53; token t stands at positions[t / per] +
+ * positions: device int64, below 2^53 (and so their angles); token t stands at positions[t / per] +
  * t % per.
  * inv_freq: device fp32 [pairs].  q_weight, k_weight: device [D] of
  * weight_dtype, or NULL.  q_out, k_out: device, of q's type, the input itself
