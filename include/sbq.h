@@ -606,7 +606,8 @@ int sbq_qk_norm_rope(const void* q, const void* k, int dtype, int64_t tokens, in
  * BF16, apart from the pool), of which the first counts[b] (NULL: all; device int64, limited to 0 ..
  * T) are there, go to the positions start[b] on (device int64; may be `length`
  * itself, not a part of it elsewhere); length[b] = start[b] + counts[b], at
- * most max_pages * page (a token past that is dropped).  8-bit caches:
+ * most max_pages * page (a token past that is dropped; a start below 0 stores
+ * nothing and leaves length 0).  8-bit caches:
  *   scale = max |x| / 127 (I8) or / 448 (E4M3), code = the nearest to x / scale
  * (fp32 IEEE divisions, half to even; a scale of 0: codes 0).  A vector with
  * an infinity or NaN reads back as NaN (scale NaN, codes 0).
@@ -632,7 +633,7 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * over the positions p < length[b] that token t sees: p <= start[b] + t, and
  * with a window (> 0) p > start[b] + t - window.  start NULL: length[b] -
  * counts[b], the tokens appended last.  Tokens from counts[b] (NULL: T) on
- * see nothing.  A row that sees nothing (or only scores of -infinity) is 0.
+ * see nothing.  A row that sees nothing is 0.
  * What a row does not see does not reach it, infinities and NaN included.
  * q: device [sequences, T, heads, D], T <= SBQ_PAGED_MAX_T, F32, or the
  * cache's type (8-bit caches: any); out: the same shape and type, its axes in any
