@@ -676,9 +676,9 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
  *     draft's rows (p's own where nothing is left), or p's row counts[b].
  * Products and sums are 64-bit.  A draft outside 0 .. V - 1 is refused.  token
  * is -1 where the whole mass is 0, infinite or NaN.  B, T <= 65535.
- * kept, token: device int64 [B], apart from every input.  workspace: >=
- * sbq_verify_workspace_bytes bytes (0: NULL will do), any content; one call at
- * a time. */
+ * kept, token: device int64 [B].  workspace: >= sbq_verify_workspace_bytes bytes
+ * (0: NULL will do), any content; one call at a time.  All three lie apart from
+ * each other and from the inputs, first byte to last (SBQ_ERR_ARG). */
 int64_t sbq_verify_workspace_bytes(int64_t B, int64_t V);
 int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, int64_t q_sb, int64_t q_st,
                       int dtype, int64_t B, int64_t T, int64_t V, const int64_t* tokens, const float* u,

@@ -924,6 +924,16 @@ int sbq_paged_attention(const void* q, int q_dtype, int64_t T, int64_t heads, in
 
 // ---- drafted tokens against the target's probabilities ----
 
+// Bytes from p on (none: null), and whether two such ranges meet.
+struct Bytes {
+  const void* p;
+  __int128 n;
+};
+static bool meet(const Bytes& a, const Bytes& b) {
+  const __int128 x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return a.p && b.p && x < y + b.n && y < x + a.n;
+}
+
 static bool verify_sizes_ok(int64_t B, int64_t T, int64_t V) {
   return B >= 0 && B <= 65535 && T >= 0 && T <= 65535 && V >= 1 && V <= ((int64_t)1 << 23);
 }
@@ -947,6 +957,16 @@ int sbq_verify_drafts(const void* p, int64_t p_sb, int64_t p_st, const void* q, 
     return SBQ_ERR_ALIGN;
   const int64_t need = sbq_verify_workspace_bytes(B, V);
   if (need && (!workspace || (int64_t)workspace_bytes < need)) return SBQ_ERR_WORKSPACE;
+  const __int128 rows = (__int128)(B - 1) * p_sb + (__int128)T * p_st + V;
+  const Bytes written[] = {{kept, B * 8}, {token, B * 8}, {need ? workspace : nullptr, need}};
+  const Bytes read[] = {{p, rows * es}, {T ? q : nullptr, ((__int128)(B - 1) * q_sb + (__int128)(T - 1) * q_st + V) * es},
+                        {T ? tokens : nullptr, B * T * 8}, {u, B * (T + 1) * 4}, {counts, B * 8}};
+  for (int i = 0; i < 3; ++i) {
+    for (const Bytes& r : read)
+      if (meet(written[i], r)) return SBQ_ERR_ARG;
+    for (int j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return SBQ_ERR_ARG;
+  }
   sbq::VerifyArgs a{};
   a.p = p, a.q = q, a.tokens = tokens, a.counts = counts, a.u = u, a.kept = kept, a.token = token;
   a.part = (double2*)(((uintptr_t)workspace + 15) & ~(uintptr_t)15), a.B = B, a.T = T, a.V = V, a.p_sb = p_sb, a.p_st = p_st;

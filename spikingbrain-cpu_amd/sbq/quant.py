@@ -153,6 +153,15 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return at, at + n * t.element_size()
 
 
+def _reached(workspace: torch.Tensor, others) -> bool:
+    """Does the contiguous workspace lie between the first and the last byte of one of them?"""
+    lo, hi = _span(workspace)
+    for t in others:
+        if t is not None and t.data_ptr() < hi and _span(t)[1] > lo:
+            return True
+    return False
+
+
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do a and b share memory?  Between each other's rows they do not: where for
     some stride, of which the others are parts or multiples, the parts lie apart in
@@ -699,9 +708,8 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     if workspace is None:
         room = _verify_workspace_bytes(B, V)
         workspace = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
-    elif workspace.device != dev or not workspace.is_contiguous() or any(
-            t is not None and _meet(workspace, t) for t in (target, draft, tokens, u, counts)):
-        raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device, apart from the inputs")
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("verify_drafts: workspace must be a contiguous tensor on target's device")
     ps, qs = target.stride(), (0, 0) if draft is None else draft.stride()
     with _on_device(dev):
         _lib.check(_lib.load().sbq_verify_drafts(

@@ -36,7 +36,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib
-from .quant import _DTYPE_CODE, _meet, _on_device, _span, _stream
+from .quant import _DTYPE_CODE, _meet, _on_device, _reached, _span, _stream
 
 
 def _as_pos(p, device: torch.device) -> torch.Tensor:
@@ -526,7 +526,8 @@ class DevicePagedKVBuffer:
         self._held: list[dict[int, int]] = [{} for _ in range(sequences)]  # page of the sequence -> page of the pool
         self._first = [0] * sequences  # pages of the sequence before this one were given back
 
-    # The pool's tensors may be replaced (a caller's own memory); they are checked when that happens.
+    # The pool's tensors may be replaced (a caller's own memory, its columns from dim on 0 and e4m3 codes
+    # finite throughout); they are checked when that happens.
     k = property(lambda self: self._tensors["k"], lambda self, t: self._replace("k", t))
     v = property(lambda self: self._tensors["v"], lambda self, t: self._replace("v", t))
     k_scale = property(lambda self: self._tensors["k_scale"], lambda self, t: self._replace("k_scale", t))
@@ -750,7 +751,7 @@ class DevicePagedKVBuffer:
         cache = self._cache("attend", None)
         n, gpu, dim, kv_heads, dev, shape = cache[10], self._gpu, self.dim, self.heads, self._dev, q.shape
         code = self._query("attend", q)
-        given = [t for t in (out, workspace) if t is not None]
+        given, room_given = out is not None, workspace is not None
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != gpu or (dim > 1 and out.stride(-1) != 1):
@@ -773,8 +774,8 @@ class DevicePagedKVBuffer:
             start = self._places("attend", "start", start, n)
         if counts is not None:
             counts = self._places("attend", "counts", counts, n)
-        if given:
-            self._apart(given, [t for t in (q, start, counts) if t is not None])
+        if given or room_given:
+            self._apart(out if given else None, workspace if room_given else None, q, start, counts)
         qs, os_ = q.stride(), out.stride()
         with _on_device(dev):
             _lib.check(_lib.load().sbq_paged_attention(
@@ -784,13 +785,18 @@ class DevicePagedKVBuffer:
                 "sbq_paged_attention")
         return out
 
-    def _apart(self, written: list, read: list) -> None:
+    def _apart(self, out, workspace, q, start, counts) -> None:
         """Refuses an output or a workspace of attend that meets the other, an input or the buffer."""
-        for i, t in enumerate(written):
-            lo, hi = _span(t)
-            if any(lo < b and a < hi for a, b in self._spans) or any(_meet(t, r) for r in read + written[:i]):
-                raise ValueError("DevicePagedKVBuffer.attend: out and workspace must lie apart from each other, the inputs and "
-                                 "the buffer")
+        for t in (out, workspace):
+            if t is not None:
+                lo, hi = _span(t)
+                if any(lo < b and a < hi for a, b in self._spans):
+                    break
+        else:
+            if (out is None or not (_meet(out, q) or any(t is not None and _meet(out, t) for t in (start, counts)))) \
+                    and (workspace is None or not _reached(workspace, (q, out, start, counts))):
+                return
+        raise ValueError("DevicePagedKVBuffer.attend: out and workspace must lie apart from each other, the inputs and the buffer")
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,

@@ -150,6 +150,16 @@ def test_norms_outputs_apart():
             _apart_rope(q, k, room[:T * H * D].view(T, H, D), k, tuple(o))
 
 
+def test_verification_written_over_an_input(tmp_path):
+    def call(V=20000, kept="@5", token="@6", ws="@7", q="@1", T=2, counts="@4"):
+        return ["sbq_verify_drafts", "@0", (T + 1) * V, V, q, T * V, V, 0, 3, T, V, "@2", "@3", counts, kept, token, ws, 1 << 20, None]
+
+    bad = [call(kept=at) for at in ("@0", "@1", "@2", "@3", "@4", "@6")] + [call(token=at) for at in ("@0", "@2", "@3", "@4")] \
+        + [call(ws=at) for at in ("@0", "@1", "@2", "@3", "@4", "@5", "@6")]
+    good = [call(), call(V=100, ws="@0"), call(T=0, q="@5"), call(q=None), call(counts=None)]  # (a short row takes no workspace)
+    assert _grids(tmp_path, bad) == [-1] * len(bad) and _grids(tmp_path, good) == [0] * len(good)
+
+
 @pytest.mark.gpu
 def test_outputs_that_meet_an_input_are_refused(dev):
     B, T, H, heads, dim = 2, 3, 4, 2, 32
@@ -191,7 +201,7 @@ def test_outputs_that_meet_an_input_are_refused(dev):
     # the verification's workspace
     target = torch.softmax(torch.randn(1, 2, 20000, device=dev), -1)
     tokens, u = torch.zeros(1, 1, dtype=torch.long, device=dev), torch.rand(1, 2, device=dev)
-    with pytest.raises(ValueError, match="apart"):
+    with pytest.raises(ValueError, match="invalid argument"):
         quant.verify_drafts(target, None, tokens, u, workspace=target)
 
 
