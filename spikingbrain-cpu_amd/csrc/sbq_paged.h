@@ -70,7 +70,9 @@ __device__ __forceinline__ int64_t paged_count(const int64_t* counts, int64_t b,
 // are of what is multiplied, against 2^14 at the row's largest so far: of the
 // weight, or with 8 bits of the weight times the value's scale (against the largest
 // scale, one far above the others would take their bits with no weight of its own).
-// So 2^-28 of the largest keeps 11 bits, and what is lost is 2^-39 of it.
+// So 2^-28 of the largest keeps 11 bits, and what is lost is 2^-39 of it.  bf16 and
+// fp32 ones are against a power of two below it that their number makes up for, or
+// large values' sums overflowed on the way to a mean that does not.
 struct PagedArgs {
   PagedCache c;
   const void* q;
@@ -509,6 +511,8 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         m[rt] = kNone, l[rt] = 0.0f;
         vref[rt] = kUnitMin, vinv[rt] = 0x1p14f / kUnitMin;
       }
+      // fp32's exponents: weights against 2^-k of the largest, for up to 2^k positions, so that their sums with V stay within V's range
+      const float less_than_all = F32 || CT == XT_BF16 ? (float)(32 - __builtin_clz((unsigned)((n1 - n0) * SB))) : 0.0f;
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {
         const int s0 = (p.from + n) * SB;
@@ -596,7 +600,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
           for (int st = 0; st < SUB; ++st)
 #pragma unroll
             for (int v = 0; v < 4; ++v) mx = __builtin_fmaxf(mx, e[rt][st][v]);
-          mx = reference<XT_F16, CT == XT_F16>(mx);
+          mx = reference<XT_F16, CT == XT_F16>(mx) + less_than_all;
           float kept = 1.0f;  // 8-bit: what of the unit is left
           if (__any(mx > m[rt])) {
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16, 64));

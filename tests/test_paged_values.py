@@ -129,3 +129,33 @@ def test_largest_and_smallest_values(dev, dtype, qt):
         tol += _step(qt, want.abs() + tol)
         assert torch.isfinite(got).all()
         assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,qt", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16), (F16, F32), (I8, F32), (E4M3, BF16)])
+@pytest.mark.parametrize("n", [1, 37, 500, 3000])
+def test_means_of_large_and_small_values(dev, n, dtype, qt):
+    """Values up to just below 2^127 (fp16: 65504) in every position, which add up to far more than fp32 holds, and of
+    2^-100 (2^-10): equal weights, so the mean.  Tolerance as above; one product below fp32's smallest steps each."""
+    B, heads, dim = 2, 2, 64
+    g = torch.Generator().manual_seed(n)
+    for e in ((15, -10) if dtype == F16 else (119, 0, -100) if dtype in (I8, E4M3) else (126, 0, -100)):
+        announce(f"{n} values of 2^{e} {dtype} {qt}")
+        if dtype in (I8, E4M3):
+            codes = _codes((B, n, heads, dim), dtype, g).abs()
+            b = _cache(dev, dtype, torch.zeros(B, n, heads, dim), codes, torch.full((B, n, heads), 2.0 ** e))
+            x = codes.double() * 2.0 ** e
+        else:
+            x = ((torch.rand(B, n, heads, dim, generator=g) + 0.99) * 2.0 ** e).to(dtype)
+            b = DevicePagedKVBuffer(B, heads, dim, 2 * (n // 16 + 1), 16, n // 16 + 1, device=dev, dtype=dtype)
+            for i in range(B):
+                b.reserve(i, n)
+            b.append(torch.zeros_like(x).to(dev), x.to(dev))
+            x = x.double()
+        assert e != 126 or n < 3 or float(x.sum(1).max()) > 2.0 ** 128
+        got = b.attend(torch.zeros(B, 1, 4, dim, dtype=qt, device=dev))[:, 0].double().cpu()
+        want = x.mean(1).repeat_interleave(2, 1)
+        tol = want.abs() * (2.0 ** -22 + (2 * n + 28) * U) + 2.0 ** -149
+        tol += _step(qt, want.abs() + tol)
+        assert torch.isfinite(got).all()
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
