@@ -17,6 +17,8 @@ from perf import more_operators as ops  # noqa: E402
 HEADS = {"heads": 32, "kv": 8, "D": 128}
 MORE = [
     {"name": "norms, 126 of 128 columns rotated", "op": "rope", "T": 8192, **HEADS, "pairs": 63, "inter": False, "norm": True, "x": "bf16"},
+    {"name": "norms, 126 columns, all rotated", "op": "rope", "T": 8192, "heads": 32, "kv": 8, "D": 126, "pairs": 63, "inter": False,
+     "norm": True, "x": "bf16"},
     {"name": "append and read 32768 tokens, fp32 and int8", "op": "store", "B": 1, "T": 32768, "kv": 8, "D": 128, "page": 64, "max": 32784,
      "one": True, "new": "f32", "cache": "i8", "ragged": False},
     {"name": "512 tokens over 8192, bf16", "op": "attend", "B": 1, "T": 512, **HEADS, "page": 64, "max": 8192, "window": 0, "q": "bf16",

@@ -52,8 +52,8 @@ __device__ __forceinline__ int64_t paged_count(const int64_t* counts, int64_t b,
 // blocks of SB positions, loads their keys and values straight to registers
 // and keeps a running maximum and sum; LDS only joins a workgroup's waves.
 // The cache's bytes, read once, bound long sequences (32 query heads over 8 x 128:
-// 65536 bf16 positions 53 us, 5.1 TB/s with the joining; 64 sequences of up to 16384
-// e4m3 ones 116 us, 4.9 TB/s); short ones the way to the first keys (launch, lengths,
+// 65536 bf16 positions 54 us, 5.0 TB/s with the joining; 64 sequences of up to 16384
+// e4m3 ones 119 us, 4.8 TB/s); short ones the way to the first keys (launch, lengths,
 // page: 3 us) and from the last ones (3 us, and 4 for the joining).
 //
 // Types of the products:
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
         m[rt] = kNone, l[rt] = 0.0f;
         vref[rt] = kUnitMin, vinv[rt] = 0x1p14f / kUnitMin;
       }
-      // fp32's exponents: weights against 2^-k of the largest, for up to 2^k positions, so that their sums with V stay within V's range
+      // fp32's exponents: weights against 2^-k of the largest, for fewer than 2^k positions
       const float less_than_all = F32 || CT == XT_BF16 ? (float)(32 - __builtin_clz((unsigned)((n1 - n0) * SB))) : 0.0f;
 #pragma unroll 1
       for (int n = n0 + w; n < n1; n += kAttnWaves) {

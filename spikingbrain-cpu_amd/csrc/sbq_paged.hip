@@ -7,7 +7,7 @@
 // value, or 2^-4 of each.  Each vector is read once and written once; a lane
 // takes 8 columns, so that a vector of 128 lies in 16 lanes and its maximum
 // crosses those alone.  A prompt is bound by its bytes (8192 tokens of 8 x 128 bf16
-// to e4m3 14 us, 3.6 TB/s, back 12.2; 32768 fp32 tokens to int8 75 us, 4.5 TB/s), a
+// to e4m3 14 us, 3.6 TB/s, back 12; 32768 fp32 tokens to int8 87 us, 3.9 TB/s), a
 // step's few rows by the loads one after another: start, table, row (4.4 us).
 #include "sbq_paged.h"
 
@@ -398,19 +398,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 // So: kPagedWhole rounds, and kPagedWholeFull more (kPagedWholeMost in all) for each
 // time that the sequences' workgroups fill the chip.  8 key heads of 128 columns,
 // e4m3, all sequences full / of lengths spread evenly / one full among short ones,
-// whole against split in us: 16 x 512 positions 9.8 against 13.4 (all full), 16 x 1024
-// 16.0, 13.6, 13.4 against 15.4, 14.4, 10.5; 64 x 2048 46, 34, 21 against 48, 41, 16;
-// 256 x 2048 191, 119, 24 against 199, 126, 34; 256 x 4096 374, 233, 40 against 379,
-// 233, 34.
+// whole against split in us: 16 x 512 positions 10.8 against 14.2 (all full), 16 x 1024
+// 17.4, 14.9, 14.7 against 16.9, 14.1, 11.2; 64 x 2048 47, 35, 23 against 50, 45, 17;
+// 256 x 2048 191, 121, 25 against 202, 127, 37; 256 x 4096 371, 219, 44 against 382,
+// 217, 37.
 constexpr int64_t kPagedWhole = 4, kPagedWholeFull = 12, kPagedWholeMost = 16;
 // Rounds of all workgroups' blocks, in times the chip, from which a workgroup takes two
 // sixteens of rows (half of that where workgroups of whole sequences fill the chip): the
 // way to and from a part's blocks is 3 to 5 us longer with them, the blocks are read
 // and converted half as often.  32 query heads over 8 x 128, two sixteens against one
-// in us: 16 x 1024 e4m3 positions, 8 tokens 31 against 19; 16 x 2048 36.4 against 35.5;
-// 16 x 4096 44.9 against 47.1, bf16 61.7 against 60.6; 16 x 8192 66 against 77, bf16 115
-// against 119; 64 x 512 e4m3 25.6 against 29.4; a chunk of 512 tokens over 2048 bf16
-// positions 46 against 77, over 8192 153 against 286.
+// in us (bf16 queries, a pool of zeros): 16 x 1024 e4m3 positions, 8 tokens 33 against
+// 20; 16 x 2048 38 against 37; 16 x 4096 47 against 49, bf16 63 against 62; 16 x 8192 69
+// against 81, bf16 118 against 119; 64 x 512 e4m3 27 against 30; a chunk of 512 tokens
+// over 2048 bf16 positions 47 against 77, over 8192 153 against 286, e4m3 145 against 212.
 constexpr int64_t kPagedTiles = 8;
 constexpr int64_t kPagedGroup = 512;   // sequences of a launch that are split at most (each workgroup scans their lengths)
 constexpr int64_t kPagedRows = 65535;  // ... of one that are not: the grid's limit

@@ -6,9 +6,9 @@
 //
 // a pair i being the columns (i, i + F) or (2i, 2i + 1).  Every vector is read
 // and written once, which is what bounds a long prompt (8192 tokens of 40 x 128 bf16
-// 31 us, 5.4 TB/s, also where the halves of 126 columns begin at no vector's alignment);
+// 33 us, 5.1 TB/s; of 126 columns, whose halves begin at no vector's alignment, 37);
 // a step's few rows are bound by the latency of one load after the launch (4.1 us).
-// Other widths of what is not rotated (128 columns, 126 of them rotated: 72 us) leave
+// Other widths of what is not rotated (128 columns, 126 of them rotated: 77 us) leave
 // half of the lanes without a piece.  A lane holds four pairs
 // (or eight columns that are not rotated), so that a vector of 128 columns lies
 // in 16 lanes, four vectors in a wave, and the rotation crosses no lanes.
