@@ -644,7 +644,8 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * (8 bits: times its value's scale), to 2^-22 of itself or 2^-39 of the row's
  * largest, whichever is more (F16, scores from 2^23 on: weights 2^-25 of the largest).
  * scale * q . k is to be finite, below 2^27 in magnitude.
- * |v| is to stay below 2^127.
+ * |v| is to stay below 2^127; over F32 and BF16 caches results keep their bits down
+ * to 2^-126 times the positions that a row sees.
  * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
  * content; one call at a time.  The result does not depend on timing; how a
  * long sequence is split, and so its last bits, goes by all sequences' lengths. */

@@ -824,7 +824,7 @@ __global__ __launch_bounds__(kAttnWaves * 64, paged_occupancy(CT, QT, DP)) void 
 #pragma unroll
             for (int k = 0; k < kAttnWaves; ++k) {
               const f32x4 x = *(const f32x4*)(lds_o + (k * 16 + rr) * OLD + d - h0);
-              if (part[k] != 0.0f) sum += x * (part[k] * inv);
+              if (lds_l[rt][k][rr] != 0.0f) sum += x * (part[k] * inv);  // (an infinity also where its weight is below fp32's)
             }
             const int r = row0 + rt * 16 + rr;
             if (!alone) {

@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const float f = weight(y[k]);
-      if (s0 + k * NG < used && f != 0.0f) sum += x[k] * (f * inv);
+      if (s0 + k * NG < used && y[k].y != 0.0f) sum += x[k] * (f * inv);
     }
   }
   lds[grp][threadIdx.x % ND] = sum;

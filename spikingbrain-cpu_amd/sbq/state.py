@@ -550,9 +550,9 @@ class DevicePagedKVBuffer:
 
     def reserve(self, sequence: int, length: int) -> None:
         """Give `sequence` the pages that positions below `length` need and it
-        does not have, from those released behind a position on.  All or none of
-        them: ValueError if the table's row is too short or all those positions
-        were released, RuntimeError if the pool has too few free pages."""
+        does not have, but for those that release(before) took back.  All or none
+        of them: ValueError if the table's row is too short or all of them were
+        taken back, RuntimeError if the pool has too few free pages."""
         held = self._held[self._row("reserve", sequence)]
         last = -(-length // self.page)
         if last > self.table.shape[1]:

@@ -159,3 +159,36 @@ def test_means_of_large_and_small_values(dev, n, dtype, qt):
         tol += _step(qt, want.abs() + tol)
         assert torch.isfinite(got).all()
         assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,qt", [(F32, F32), (BF16, BF16), (F16, F16), (F16, F32), (I8, F32), (E4M3, BF16)])
+def test_what_is_no_number_shows_at_any_weight(dev, dtype, qt):
+    """An infinity or NaN among the values that a row sees is in its result, also where its weight is far below fp32's
+    smallest (scores 0 and -420), in whichever wave or part of the sequence it lies; no other column changes."""
+    n, heads, dim = 3000, 1, 64
+    g = torch.Generator().manual_seed(4)
+    b = DevicePagedKVBuffer(1, heads, dim, 200, 16, 200, device=dev, dtype=dtype)
+    b.reserve(0, n)
+    k = torch.zeros(1, n, heads, dim)
+    k[..., 5] = -10
+    k[:, 1700, :, 5] = 0
+    b.append(k.to(dev), torch.randn(1, n, heads, dim, generator=g).to(dev))
+    q = torch.zeros(1, 1, 2, dim, dtype=qt, device=dev)
+    q[..., 5] = 42
+    want = b.attend(q, scale=1.0)
+    assert torch.isfinite(want).all()
+    for at in (0, 33, 700, 1699, 1701, 1801, 2999):
+        for what in (float("inf"), float("nan")):
+            announce(f"{what} at {at} {dtype} {qt}")
+            page, row = int(b.table[0, at // 16]), at % 16
+            cell = b.v[page, 0, row, 9:10] if b.v_scale is None else b.v_scale[page, 0, row:row + 1]
+            keep = cell.clone()
+            cell.fill_(what)
+            got = b.attend(q, scale=1.0)
+            cell.copy_(keep)
+            if b.v_scale is None:
+                assert not torch.isfinite(got[..., 9]).any()
+                assert torch.equal(got[..., :9], want[..., :9]) and torch.equal(got[..., 10:], want[..., 10:])
+            else:
+                assert not torch.isfinite(got).any()
