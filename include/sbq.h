@@ -568,8 +568,8 @@ int sbq_kv_take(const int64_t* slot_pos, const float* weight, int64_t slots, con
  * fp32, rounded once to the output's type.
  * q: device [tokens, heads, D], k: device [tokens, kv_heads, D] (kv_heads 0:
  * none) of one type, strides in elements, unit stride in D <= 256.
- * positions: device int64, below 2^53 (and so their angles); token t stands at positions[t / per] +
- * t % per.
+ * positions: device int64, below 2^53 (and so their angles); token t stands at
+ * positions[t / per] + t % per.
  * inv_freq: device fp32 [pairs].  q_weight, k_weight: device [D] of
  * weight_dtype, or NULL.  q_out, k_out: device, of q's type, the input itself
  * (with its strides) or apart from both inputs. */
@@ -637,15 +637,16 @@ int sbq_paged_read(const void* k, const void* v, const float* k_scale, const flo
  * What a row does not see does not reach it, infinities and NaN included.
  * q: device [sequences, T, heads, D], T <= SBQ_PAGED_MAX_T, F32, or the
  * cache's type (8-bit caches: any); out: the same shape and type, its axes in any
- * order, no two elements in one place, apart from every input.  Scores, maxima and sums are fp32.  The other factors are multiplied
- * as they are, or where the cache's type has fewer bits in pieces of it (8 bits: of
- * fp16): BF16 caches 24 bits of fp32 queries and their weights, 16 of the weights of
- * BF16 queries; F16 and 8-bit caches each element of an fp32 query, and each weight
- * (8 bits: times its value's scale), to 2^-22 of itself or 2^-39 of the row's
- * largest, whichever is more (F16, scores from 2^23 on: weights 2^-25 of the largest).
- * scale * q . k is to be finite, below 2^27 in magnitude.
- * |v| is to stay below 2^127; over F32 and BF16 caches results keep their bits down
- * to 2^-126 times the positions that a row sees.
+ * order, no two elements in one place, apart from every input.
+ * Scores, maxima and sums are fp32.  The other factors are multiplied as they are,
+ * or where the cache's type has fewer bits in pieces of it (8 bits: of fp16): BF16
+ * caches 24 bits of fp32 queries and their weights, 16 of the weights of BF16
+ * queries; F16 and 8-bit caches each element of an fp32 query, and each weight (8
+ * bits: times its value's scale), to 2^-22 of itself or 2^-39 of the row's largest,
+ * whichever is more (F16, scores from 2^23 on: weights 2^-25 of the largest).
+ * scale * q . k is to be finite, below 2^27 in magnitude, |v| below 2^127; over F32
+ * and BF16 caches results keep their bits down to 2^-126 times the positions that a
+ * row sees.
  * workspace: >= sbq_paged_attn_workspace_bytes bytes (0: NULL will do), any
  * content; one call at a time.  The result does not depend on timing; how a
  * long sequence is split, and so its last bits, goes by all sequences' lengths. */

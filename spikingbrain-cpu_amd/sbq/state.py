@@ -653,9 +653,8 @@ class DevicePagedKVBuffer:
         start .. start + T - 1 (default: after those it holds; an int or int64
         [sequences]), the first counts[b] of them where counts (int64
         [sequences]) is given; length becomes start + counts (0, and nothing is
-        stored, for a start below 0).  With `sequence`
-        k, v [T, heads, dim] go to that one alone, and start and counts are of
-        one entry."""
+        stored, for a start below 0).  With `sequence` k, v [T, heads, dim] go
+        to that one alone, and start and counts are of one entry."""
         cache = self._cache("append", sequence)
         n, heads, dim, shape = cache[10], self.heads, self.dim, k.shape
         if sequence is None:
